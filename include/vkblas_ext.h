@@ -59,8 +59,13 @@ typedef enum {
                                            tiles, the slice's K over the waves  */
     VKBLAS_KERNEL_DIRECT = 8,           /* small tiles, K over the waves, MFMA
                                            fragments straight from memory       */
-    VKBLAS_KERNEL_FLOW = 9              /* 16-bit 128 x 128 / 128 x 64 tiles, any
+    VKBLAS_KERNEL_FLOW = 9,             /* 16-bit 128 x 128 / 128 x 64 tiles, any
                                            M, N and C, K in 16-byte chunks      */
+    /* the operators of vkblas_nn.h */
+    VKBLAS_KERNEL_NORM = 10,            /* layer norm, rows in registers        */
+    VKBLAS_KERNEL_NORM_LONG = 11,       /* layer norm, rows read again          */
+    VKBLAS_KERNEL_JOINED = 12           /* GEMMs by their plans, then a kernel
+                                           over their results                   */
 } vkblas_kernel_t;
 
 typedef struct {

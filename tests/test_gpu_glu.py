@@ -1,0 +1,174 @@
+"""vkblas_glu_async and its backward pass against the definition in float64: activations, types, one row to
+several tiles, ragged sizes, strides, alignments, accumulation, and values at the ends of the activations."""
+import pytest
+import torch
+
+import nn_ref as R
+import vkblas_amd as vk
+
+pytestmark = pytest.mark.gpu
+
+
+def stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+def forward(x, w, dt, act, keep=True, pad=0, off=0):
+    M, K = x.shape
+    N = w.shape[0] // 2
+    bx, bw = R.Buf(M, K, dt, pad, off, x), R.Buf(2 * N, K, dt, pad, off, w)
+    h, gu = R.Buf(M, N, dt, pad, off), R.Buf(M, 2 * N, dt, pad, off)
+    vk.glu_async(R.ENGINE[dt], R.ACTS[act], M, N, K, bx.ptr, bx.ld, bw.ptr, bw.ld, h.ptr, h.ld,
+                 gu.ptr if keep else None, gu.ld, stream=stream())
+    h.check_around()
+    gu.check_around()
+    return h.get(), gu.get() if keep else None
+
+
+def check_forward(got, x, w, dt, act):
+    N = w.shape[0] // 2
+    gu, e = x @ w.t(), R.dot_bound(x, w.t())
+    g, u = gu[:, :N], gu[:, N:]
+    a = R.act(act, g)
+    # the activations' slopes are below 1.13; their own error is STEP of the argument and of the value
+    ea = 1.13 * e[:, :N] + R.STEP * (g.abs() + a.abs())
+    h = a * u
+    R.close(got[0], h, R.rounded(h, dt, ea * (u.abs() + e[:, N:]) + a.abs() * e[:, N:] + R.STEP * h.abs()), "h")
+    if got[1] is not None:
+        R.close(got[1], gu, R.rounded(gu, dt, e), "gu")
+
+
+# one row, decode batches, rows of one and of several tiles, whole and ragged
+SIZES = [(1, 1, 1), (1, 64, 64), (1, 500, 784), (2, 129, 72), (7, 256, 512), (16, 320, 128), (33, 100, 100),
+         (64, 128, 256), (65, 192, 192), (100, 33, 57), (128, 128, 128), (200, 500, 784), (255, 320, 64),
+         (256, 128, 128), (257, 129, 128), (300, 200, 320), (511, 264, 192), (130, 72, 1000)]
+
+
+@pytest.mark.parametrize("M,N,K", SIZES)
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+def test_forward(M, N, K, dt):
+    x, w = R.values(M, K, dt, 1), R.values(2 * N, K, dt, 2, K ** -0.5)
+    check_forward(forward(x, w, dt, "silu"), x, w, dt, "silu")
+    check_forward(forward(x, w, dt, "silu", keep=False), x, w, dt, "silu")
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 300, 256), (40, 96, 128), (300, 160, 128), (90, 41, 77)])
+@pytest.mark.parametrize("act", list(R.ACTS))
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+def test_activations(M, N, K, act, dt):
+    x, w = R.values(M, K, dt, 3), R.values(2 * N, K, dt, 4, 2 * K ** -0.5)
+    check_forward(forward(x, w, dt, act), x, w, dt, act)
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 128, 128), (30, 128, 128), (300, 136, 192)])
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("pad,off", [(8, 0), (4, 4), (1, 0), (3, 1)])
+def test_strides_and_alignment(M, N, K, dt, pad, off):
+    x, w = R.values(M, K, dt, 5), R.values(2 * N, K, dt, 6, K ** -0.5)
+    check_forward(forward(x, w, dt, "gelu", pad=pad, off=off), x, w, dt, "gelu")
+
+
+@pytest.mark.parametrize("act", list(R.ACTS))
+@pytest.mark.parametrize("M", [1, 300])
+def test_ends_of_the_activations(act, M):
+    """Gates of -200 .. 200 (exponentials that overflow and vanish), zeros, and NaN kept to its own outputs."""
+    N, K = 128, 128
+    x, w = torch.zeros(M, K, dtype=torch.float64), torch.zeros(2 * N, K, dtype=torch.float64)
+    x[:, 0], x[:, 1] = 1.0, 2.0
+    w[:N, 0] = torch.linspace(-200, 200, N, dtype=torch.float64).float().double()
+    w[N:, 1] = 1.5
+    check_forward(forward(x, w, "f32", act), x, w, "f32", act)
+    w[5, 3] = float("nan")
+    h, gu = forward(x, w, "f32", act)
+    assert bool(torch.isnan(h[:, 5]).all()) and bool(torch.isnan(gu[:, 5]).all())
+    rest = [i for i in range(N) if i != 5]
+    assert bool(torch.isfinite(h[:, rest]).all())
+
+
+def backward(dh, gu, x, w, dt, act, wt=None, pad=0, off=0, beta=0.0, dw0=None, want="xwg", inplace=False):
+    M, K = x.shape
+    N = w.shape[0] // 2
+    wt = wt or dt
+    bh, bg = R.Buf(M, N, dt, pad, off, dh), R.Buf(M, 2 * N, dt, pad, off, gu)
+    bx, bw = R.Buf(M, K, dt, pad, off, x), R.Buf(2 * N, K, dt, pad, off, w)
+    dx, dw = R.Buf(M, K, dt, pad, off), R.Buf(2 * N, K, wt, pad, off, dw0)
+    dgu = bg if inplace else R.Buf(M, 2 * N, dt, pad, off)
+    vk.glu_backward_async(R.ENGINE[dt], R.ACTS[act], M, N, K, bh.ptr, bh.ld, bg.ptr, bg.ld, bx.ptr, bx.ld, bw.ptr,
+                          bw.ld, dgu.ptr if "g" in want else None, dgu.ld, dx.ptr if "x" in want else None, dx.ld,
+                          dw.ptr if "w" in want else None, dw.ld, R.ENGINE[wt], beta, stream=stream())
+    for o in (dx, dw, dgu):
+        o.check_around()
+    return dx.get(), dw.get(), dgu.get()
+
+
+def check_backward(got, dh, gu, x, w, dt, act, wt=None, beta=0.0, dw0=None, want="xwg"):
+    N = w.shape[0] // 2
+    wt = wt or dt
+    g, u = gu[:, :N], gu[:, N:]
+    a, da = R.act(act, g), R.act_slope(act, g)
+    d = torch.cat((dh * u * da, dh * a), 1)
+    # act' has terms of size 1 + |g| exp(-g^2 / 2) <= 2 whose sum may cancel
+    ed = torch.cat(((dh * u).abs() * R.STEP * (2 + g.abs().clamp(max=16)), dh.abs() * R.STEP * (g.abs() + a.abs())), 1)
+    ed = R.rounded(d, dt, ed)
+    if "g" in want:
+        R.close(got[2], d, ed, "dgu")
+    if "x" in want:
+        dx = d @ w
+        R.close(got[0], dx, R.rounded(dx, dt, ed @ w.abs() + R.dot_bound(d.abs() + ed, w)), "dx")
+    if "w" in want:
+        old = torch.zeros_like(w) if dw0 is None else dw0
+        dw = d.t() @ x + beta * old
+        err = ed.t() @ x.abs() + R.dot_bound((d.abs() + ed).t(), x) + 4 * R.E * (beta * old).abs()
+        R.close(got[1], dw, R.rounded(dw, wt, err), "dw")
+
+
+def grad_inputs(M, N, K, dt, seed=20):
+    x, w = R.values(M, K, dt, seed), R.values(2 * N, K, dt, seed + 1, K ** -0.5)
+    return R.values(M, N, dt, seed + 2, 0.1), (x @ w.t()).to(R.TORCH[dt]).double(), x, w
+
+
+@pytest.mark.parametrize("M,N,K", SIZES)
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+def test_backward(M, N, K, dt):
+    args = grad_inputs(M, N, K, dt)
+    check_backward(backward(*args, dt, "silu"), *args, dt, "silu")
+
+
+@pytest.mark.parametrize("act", list(R.ACTS))
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+def test_backward_forms(act, dt):
+    """Each activation; single outputs, dgu in gu's place or in the workspace, fp32 accumulation, strides."""
+    args = grad_inputs(70, 40, 64, dt)
+    dw0 = R.values(80, 64, "f32", 30, 2.0)
+    for kw in (dict(), dict(want="x"), dict(want="w"), dict(want="g"), dict(want="xw"), dict(inplace=True),
+               dict(wt="f32", beta=0.5, dw0=dw0), dict(pad=8), dict(pad=3, off=1)):
+        check_backward(backward(*args, dt, act, **kw), *args, dt, act,
+                       **{k: v for k, v in kw.items() if k in ("wt", "beta", "dw0", "want")})
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
+def test_gradients_against_differences(act):
+    """<gradient, v> against central differences of the definition, h = 1e-4 (the kept projections in fp32)."""
+    M, N, K, h = 5, 24, 40, 1e-4
+    x, w, c = R.values(M, K, "f32", 41), R.values(2 * N, K, "f32", 42, 0.3), R.values(M, N, "f32", 43)
+
+    def f(x, w):
+        gu = x @ w.t()
+        return float((R.act(act, gu[:, :N]) * gu[:, N:] * c).sum())
+    dx, dw, _ = backward(c, (x @ w.t()), x, w, "f32", act)
+    for i, (grad, at) in enumerate(((dx, x), (dw, w))):
+        v = R.values(*at.shape, "f32", 50 + i)
+        lo, hi = [x, w], [x, w]
+        hi[i], lo[i] = at + h * v, at - h * v
+        diff = (f(*hi) - f(*lo)) / (2 * h)
+        assert abs(float((grad * v).sum()) - diff) <= 1e-5 * float((grad * v).abs().sum()) + 1e-6
+
+
+def test_empty_batch():
+    dw = R.Buf(20, 30, "f32", 2, values=torch.full((20, 30), 3.0))
+    assert vk.glu_async(0, 0, 0, 10, 30, None, 30, None, 30, None, 10) == vk.OK
+    for beta, want in ((0.5, 1.5), (0.0, 0.0)):
+        vk.glu_backward_async(0, 0, 0, 10, 30, None, 10, None, 20, None, 30, None, 30, None, 0, None, 30, dw.ptr, dw.ld,
+                              0, beta, stream=stream())
+        assert bool((dw.get() == want).all())
+    dw.check_around()

@@ -37,6 +37,8 @@ OP_N, OP_T = 0, 1
 DT_F32, DT_F16, DT_BF16 = 0, 1, 2
 # vkblas_scalar_mode_t
 SCALAR_HOST, SCALAR_DEV_F32, SCALAR_DEV_F16 = 0, 1, 2
+# vkblas_act_t (include/vkblas_nn.h)
+ACT_SILU, ACT_GELU, ACT_GELU_TANH, ACT_RELU = range(4)
 # vkblas_path_t
 PATH_NONE, PATH_TILE64, PATH_TILE128, PATH_TILE256, PATH_SPLITK, PATH_SKINNY, PATH_TAIL = range(7)
 PATH_NAMES = {0: "none", 1: "tile64", 2: "tile128", 3: "tile256", 4: "splitk", 5: "skinny", 6: "tail"}
@@ -69,6 +71,20 @@ _ex_addr = 0        # address of vkblas_gemm_ex_async
 
 _u32, _i64, _f, _vp, _int = ctypes.c_uint32, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p, ctypes.c_int
 _ENGINE_ARGS = [_int, _int, _u32, _u32, _u32, _f, _vp, _u32, _vp, _u32, _f, _vp, _u32, _u32, _i64, _i64, _i64]
+
+
+# include/vkblas_nn.h
+_NN_ARGS = {
+    "vkblas_layer_norm_async": [_int, _int, _u32, _u32, _vp, _u32, _vp, _vp, _f, _vp, _u32, _vp, _vp, _vp],
+    "vkblas_layer_norm_backward_async": [_int, _int, _u32, _u32, _vp, _u32, _vp, _u32, _vp, _vp, _vp, _vp, _u32, _vp,
+                                         _vp, _int, _f, _vp],
+    "vkblas_glu_async": [_int, _int, _u32, _u32, _u32, _vp, _u32, _vp, _u32, _vp, _u32, _vp, _u32, _vp],
+    "vkblas_glu_backward_async": [_int, _int, _u32, _u32, _u32, _vp, _u32, _vp, _u32, _vp, _u32, _vp, _u32, _vp, _u32,
+                                  _vp, _u32, _vp, _u32, _int, _f, _vp],
+    "vkblas_linear_xent_async": [_int, _u32, _u32, _u32, _vp, _u32, _vp, _u32, _vp, _i64, _vp, _vp, _vp],
+    "vkblas_linear_xent_backward_async": [_int, _u32, _u32, _u32, _vp, _u32, _vp, _u32, _vp, _i64, _vp, _vp, _vp, _u32,
+                                          _vp, _u32, _int, _f, _vp],
+}
 
 
 def build(jobs: int = 8) -> None:
@@ -111,6 +127,10 @@ def load():
     L.vkblas_gemm_noalloc_async.argtypes = L.vkblas_gemm_async.argtypes
     L.vkblas_gemm_noalloc_async.restype = _int
     L.vkblas_noalloc_scratch_bytes.restype = ctypes.c_size_t
+    for name, args in _NN_ARGS.items():
+        fn = getattr(L, name)
+        fn.argtypes = args
+        fn.restype = _int
     try:
         from ._call import gemm_ex
     except ImportError:     # not built, or for another interpreter
@@ -147,7 +167,8 @@ def last_path() -> int:
 
 # vkblas_kernel_t (include/vkblas_ext.h)
 KERNEL_NONE, KERNEL_GENERIC, KERNEL_GENERIC_CHECKED, KERNEL_PIPE256, KERNEL_PIPE128, KERNEL_PIPE128_4, \
-    KERNEL_SKINNY, KERNEL_WAVEK, KERNEL_DIRECT, KERNEL_FLOW = range(10)
+    KERNEL_SKINNY, KERNEL_WAVEK, KERNEL_DIRECT, KERNEL_FLOW, KERNEL_NORM, KERNEL_NORM_LONG, \
+    KERNEL_JOINED = range(13)
 
 
 def workspace_release() -> None:
@@ -228,6 +249,59 @@ def gemm_batched_async(ab_type, c_type, op_a, op_b, M, N, K, alpha, A, lda, B, l
     if check and st != OK:
         raise VkblasError(st, "vkblas_gemm_batched_async")
     return st
+
+
+def _nn(name, check, *args) -> int:
+    """A call of vkblas_nn.h; its status (raises if check)."""
+    st = getattr(_lib or load(), name)(*args)
+    if check and st != OK:
+        raise VkblasError(st, name)
+    return st
+
+
+def layer_norm_async(dtype, w_dtype, M, N, x, ldx, w, b, eps, y, ldy, mean=None, rstd=None, stream=None,
+                     check=True) -> int:
+    """vkblas_layer_norm_async: y = (x - mean) * rstd * w + b over M rows of N;
+    mean and rstd (M floats each) kept where given."""
+    return _nn("vkblas_layer_norm_async", check, dtype, w_dtype, M, N, x, ldx, w, b, eps, y, ldy, mean, rstd, stream)
+
+
+def layer_norm_backward_async(dtype, w_dtype, M, N, dy, lddy, x, ldx, w, mean, rstd, dx, lddx, dw, db, g_dtype,
+                              beta=0.0, stream=None, check=True) -> int:
+    """vkblas_layer_norm_backward_async: dx, and dw and db (beta times what
+    they held, plus the sums over the rows); each may be None."""
+    return _nn("vkblas_layer_norm_backward_async", check, dtype, w_dtype, M, N, dy, lddy, x, ldx, w, mean, rstd, dx,
+               lddx, dw, db, g_dtype, beta, stream)
+
+
+def glu_async(dtype, act, M, N, K, x, ldx, w, ldw, h, ldh, gu=None, ldgu=0, stream=None, check=True) -> int:
+    """vkblas_glu_async: h = act(G) * U with [G | U] = x w^T (w is 2N x K, the
+    gate's rows first); gu (M x 2N) receives [G | U] where given."""
+    return _nn("vkblas_glu_async", check, dtype, act, M, N, K, x, ldx, w, ldw, h, ldh, gu, ldgu, stream)
+
+
+def glu_backward_async(dtype, act, M, N, K, dh, lddh, gu, ldgu, x, ldx, w, ldw, dgu, lddgu, dx, lddx, dw, lddw,
+                       dw_dtype, beta=0.0, stream=None, check=True) -> int:
+    """vkblas_glu_backward_async: dgu = [dG | dU], dx = dgu w and dw = beta dw
+    + dgu^T x; each may be None."""
+    return _nn("vkblas_glu_backward_async", check, dtype, act, M, N, K, dh, lddh, gu, ldgu, x, ldx, w, ldw, dgu, lddgu,
+               dx, lddx, dw, lddw, dw_dtype, beta, stream)
+
+
+def linear_xent_async(dtype, M, V, K, x, ldx, w, ldw, target, ignore_index, loss, lse, stream=None,
+                      check=True) -> int:
+    """vkblas_linear_xent_async: each row's cross entropy (loss) and
+    log-sum-exp (lse) of the logits x w^T, which are not kept."""
+    return _nn("vkblas_linear_xent_async", check, dtype, M, V, K, x, ldx, w, ldw, target, ignore_index, loss, lse,
+               stream)
+
+
+def linear_xent_backward_async(dtype, M, V, K, x, ldx, w, ldw, target, ignore_index, lse, dloss, dx, lddx, dw, lddw,
+                               dw_dtype, beta=0.0, stream=None, check=True) -> int:
+    """vkblas_linear_xent_backward_async: dx and dw = beta dw + D^T x from the
+    rows' loss gradients; each may be None."""
+    return _nn("vkblas_linear_xent_backward_async", check, dtype, M, V, K, x, ldx, w, ldw, target, ignore_index, lse,
+               dloss, dx, lddx, dw, lddw, dw_dtype, beta, stream)
 
 
 def gemm_f32(op_a, op_b, M, N, K, alpha, A, lda, B, ldb, beta, C, ldc, batch=1, sa=0, sb=0, sc=0) -> int:

@@ -161,12 +161,7 @@ static ws_slot_t g_ws[VKB_WS_SLOTS] = {[0 ... VKB_WS_SLOTS - 1] = {.lock = PTHRE
 static int g_nws = 0;            /* slots claimed (never unclaimed) */
 static size_t g_ws_total = 0;    /* bytes cached in the slots */
 
-typedef struct {
-    void* ptr;
-    int slot;                    /* locked slot, or -1 */
-    int owned;                   /* free ptr on the stream after the kernels */
-    hipStream_t stream;
-} ws_lease_t;
+typedef vkb_ws_lease ws_lease_t;
 
 /* A workspace starts with VKB_WS_HEADER bytes of arrival counters, zero
  * when the buffer is new (the partials follow; see vkb_launch.h).  Never
@@ -278,6 +273,14 @@ static void ws_release(ws_lease_t* L) {
     L->slot = -1;
     L->owned = 0;
 }
+
+int vkb_ws_acquire(void* stream, size_t bytes, vkb_ws_lease* L) {
+    const int rc = ws_acquire((hipStream_t)stream, bytes, L);
+    if (rc != 0) ws_release(L);
+    return rc;
+}
+
+void vkb_ws_release(vkb_ws_lease* L) { ws_release(L); }
 
 vkblas_status_t vkblas_workspace_release(void) {
     pthread_once(&g_once, init_once);
@@ -656,11 +659,7 @@ static const char* path_name(int p) {
  * time of the call's kernels (events on the stream; the call then waits for
  * its kernels, as every call of the reference's engine did,
  * src/vkblas.c:954-968).  Not under stream capture. */
-typedef struct {
-    int on;
-    double t0, t1;
-    hipEvent_t e0, e1;
-} prof_t;
+typedef vkb_prof prof_t;
 
 static double now_us(void) {
     struct timespec ts;
@@ -673,8 +672,8 @@ static void prof_begin(prof_t* pf, hipStream_t stream) {
     if (!g_profile) return;
     hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
     if (hipStreamIsCapturing(stream, &cs) != hipSuccess || cs != hipStreamCaptureStatusNone) return;
-    if (hipEventCreate(&pf->e0) != hipSuccess) return;
-    if (hipEventCreate(&pf->e1) != hipSuccess) {
+    if (hipEventCreate((hipEvent_t*)&pf->e0) != hipSuccess) return;
+    if (hipEventCreate((hipEvent_t*)&pf->e1) != hipSuccess) {
         hipEventDestroy(pf->e0);
         return;
     }
@@ -693,6 +692,9 @@ static void prof_end(prof_t* pf, hipStream_t stream, const char* what, int ok) {
     hipEventDestroy(pf->e0);
     hipEventDestroy(pf->e1);
 }
+
+void vkb_prof_begin(vkb_prof* pf, void* stream) { prof_begin(pf, (hipStream_t)stream); }
+void vkb_prof_end(vkb_prof* pf, void* stream, const char* what, int ok) { prof_end(pf, (hipStream_t)stream, what, ok); }
 
 /* A decode-planned call small enough for gemm_direct_kernel, one launch of
  * small tiles: the decode kernels then run a handful of workgroups, or split
@@ -726,6 +728,26 @@ static int small_decode(vkblas_dtype_t ab_type, vkblas_op_t op_b, uint32_t M, ui
            N <= (kn && !f32 ? 16384u : 8192u) && K <= (f32 ? 1280u : 2048u) && !(f32 && kn && M <= 2 && K <= 32) &&
            (f32 || kn || K <= 512 || ((M + 31) / 32) * ((N + 31) / 32) <= 256) &&
            (uint64_t)N * K <= (f32 ? 1ull << 20 : 1ull << 22);
+}
+
+/* Workspace bytes of a plan with a K split: the arrival counters, the
+ * partials (*part_bytes) and, for divided slices, the parts' sums. */
+static size_t plan_ws_bytes(const vkblas_plan_t* plan, uint32_t M, uint32_t N, size_t* part_bytes) {
+    const int divided = plan->path == VKBLAS_PATH_SPLITK && plan->tile == VKB_TILE_64Q;
+    const uint32_t rows = plan->path == VKBLAS_PATH_TAIL ? plan->tail_rows : M;
+    *part_bytes = ((size_t)plan->split * rows * N * sizeof(float) + 255) & ~(size_t)255;
+    return VKB_WS_HEADER + *part_bytes * (divided ? 1 + VKB_WAVEK_NQ : 1);
+}
+
+size_t vkb_gemm_scratch_bytes(vkblas_dtype_t ab_type, vkblas_dtype_t c_type, vkblas_op_t op_a, vkblas_op_t op_b,
+                              uint32_t M, uint32_t N, uint32_t K, uint32_t lda, uint32_t ldb, uint32_t ldc,
+                              int aligned) {
+    vkblas_plan_t plan;
+    size_t part_bytes;
+    if (vkblas_plan_gemm(ab_type, c_type, op_a, op_b, M, N, K, lda, ldb, ldc, 1, 0, aligned, &plan) != VKBLAS_OK ||
+        plan.split <= 1)
+        return 0;
+    return plan_ws_bytes(&plan, M, N, &part_bytes);
 }
 
 /* The body of vkblas_gemm_async.  ws_ext != NULL: the split-K / decode
@@ -792,12 +814,9 @@ static vkblas_status_t gemm_impl(vkblas_dtype_t ab_type, vkblas_dtype_t c_type, 
     }
     int partials = !direct && plan.split > 1 && (plan.path == VKBLAS_PATH_SKINNY || plan.path == VKBLAS_PATH_SPLITK ||
                                       plan.path == VKBLAS_PATH_TAIL);
-    const size_t part_bytes =
-        partials ? (((size_t)plan.split * (plan.path == VKBLAS_PATH_TAIL ? plan.tail_rows : M) * N * sizeof(float) +
-                     255) & ~(size_t)255)
-                 : 0;
+    size_t part_bytes = 0;
     const int divided = partials && plan.path == VKBLAS_PATH_SPLITK && plan.tile == VKB_TILE_64Q;
-    size_t ws_bytes = partials ? VKB_WS_HEADER + part_bytes * (divided ? 1 + VKB_WAVEK_NQ : 1) : 0;
+    size_t ws_bytes = partials ? plan_ws_bytes(&plan, M, N, &part_bytes) : 0;
     /* The planner's own K splits (split-K for few output tiles, the split
      * tail) only speed a call up: where their partials have no room (the
      * caller's scratch is smaller; a capturing stream declines the
@@ -1043,6 +1062,13 @@ vkblas_status_t vkblas_gemm_batched_async(vkblas_dtype_t ab_type, vkblas_dtype_t
     g_last_path = plan.path;
     g_last_kernel = kernel;
     return VKBLAS_OK;
+}
+
+int vkb_engine_ready(void) { return ensure_init(); }
+int vkb_engine_trace(void) { return g_trace; }
+void vkb_engine_ran(int path, int kernel) {
+    g_last_path = path;
+    g_last_kernel = kernel;
 }
 
 int vkblas_last_path(void) { return g_last_path; }

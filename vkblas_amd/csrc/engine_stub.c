@@ -1,6 +1,6 @@
 /*
  * engine_stub.c — the public C API of libvkblas_hipblas.so (include/vkblas.h,
- * include/vkblas_ext.h), forwarded to libvkblas_engine.so, the host
+ * include/vkblas_ext.h, include/vkblas_nn.h), forwarded to libvkblas_engine.so, the host
  * dispatcher and gfx950 kernels, which is loaded from this library's own
  * directory at the first call.
  *
@@ -30,7 +30,7 @@
 #include <stdio.h>
 #include <string.h>
 
-#include "vkblas_ext.h"
+#include "vkblas_nn.h"
 
 #define ENGINE_NAME "libvkblas_engine.so"
 
@@ -137,3 +137,35 @@ VKB_ENGINE_FN(int, VKBLAS_KERNEL_NONE, vkblas_last_kernel, (void), ())
 VKB_ENGINE_FN(size_t, 0, vkblas_noalloc_scratch_bytes, (void), ())
 VKB_ENGINE_FN(vkblas_status_t, VKBLAS_ERR_INIT, vkblas_workspace_release, (void), ())
 VKB_ENGINE_FN(const char*, "vkblas-mi355x (engine not loaded)", vkblas_version, (void), ())
+
+/* include/vkblas_nn.h */
+VKB_ENGINE_FN(vkblas_status_t, VKBLAS_ERR_INIT, vkblas_layer_norm_async,
+              (vkblas_dtype_t type, vkblas_dtype_t w_type, uint32_t M, uint32_t N, const void* x, uint32_t ldx,
+               const void* w, const void* b, float eps, void* y, uint32_t ldy, float* mean, float* rstd, void* stream),
+              (type, w_type, M, N, x, ldx, w, b, eps, y, ldy, mean, rstd, stream))
+VKB_ENGINE_FN(vkblas_status_t, VKBLAS_ERR_INIT, vkblas_layer_norm_backward_async,
+              (vkblas_dtype_t type, vkblas_dtype_t w_type, uint32_t M, uint32_t N, const void* dy, uint32_t lddy,
+               const void* x, uint32_t ldx, const void* w, const float* mean, const float* rstd, void* dx,
+               uint32_t lddx, void* dw, void* db, vkblas_dtype_t g_type, float beta, void* stream),
+              (type, w_type, M, N, dy, lddy, x, ldx, w, mean, rstd, dx, lddx, dw, db, g_type, beta, stream))
+VKB_ENGINE_FN(vkblas_status_t, VKBLAS_ERR_INIT, vkblas_glu_async,
+              (vkblas_dtype_t type, vkblas_act_t act, uint32_t M, uint32_t N, uint32_t K, const void* x, uint32_t ldx,
+               const void* w, uint32_t ldw, void* h, uint32_t ldh, void* gu, uint32_t ldgu, void* stream),
+              (type, act, M, N, K, x, ldx, w, ldw, h, ldh, gu, ldgu, stream))
+VKB_ENGINE_FN(vkblas_status_t, VKBLAS_ERR_INIT, vkblas_glu_backward_async,
+              (vkblas_dtype_t type, vkblas_act_t act, uint32_t M, uint32_t N, uint32_t K, const void* dh,
+               uint32_t lddh, const void* gu, uint32_t ldgu, const void* x, uint32_t ldx, const void* w, uint32_t ldw,
+               void* dgu, uint32_t lddgu, void* dx, uint32_t lddx, void* dw, uint32_t lddw, vkblas_dtype_t dw_type,
+               float beta, void* stream),
+              (type, act, M, N, K, dh, lddh, gu, ldgu, x, ldx, w, ldw, dgu, lddgu, dx, lddx, dw, lddw, dw_type, beta,
+               stream))
+VKB_ENGINE_FN(vkblas_status_t, VKBLAS_ERR_INIT, vkblas_linear_xent_async,
+              (vkblas_dtype_t type, uint32_t M, uint32_t V, uint32_t K, const void* x, uint32_t ldx, const void* w,
+               uint32_t ldw, const int64_t* target, int64_t ignore_index, float* loss, float* lse, void* stream),
+              (type, M, V, K, x, ldx, w, ldw, target, ignore_index, loss, lse, stream))
+VKB_ENGINE_FN(vkblas_status_t, VKBLAS_ERR_INIT, vkblas_linear_xent_backward_async,
+              (vkblas_dtype_t type, uint32_t M, uint32_t V, uint32_t K, const void* x, uint32_t ldx, const void* w,
+               uint32_t ldw, const int64_t* target, int64_t ignore_index, const float* lse, const float* dloss,
+               void* dx, uint32_t lddx, void* dw, uint32_t lddw, vkblas_dtype_t dw_type, float beta, void* stream),
+              (type, M, V, K, x, ldx, w, ldw, target, ignore_index, lse, dloss, dx, lddx, dw, lddw, dw_type, beta,
+               stream))

@@ -1,0 +1,139 @@
+// glu.hip — the gated projection's activation and product, and their
+// gradients, on projections that a GEMM computed:
+//   h = act(G) * U,  dG = dh * U * act'(G),  dU = dh * act(G)
+// Elementwise, one pass, bound by memory: a thread takes 16 bytes of the
+// 16-bit (or fp32) rows at a time.
+#include <type_traits>
+#include "nn_common.hpp"
+#include "vkb_nn_launch.h"
+
+namespace vkb {
+namespace {
+
+constexpr uint32_t THREADS = 256;
+
+// column blocks in x, rows in y (strided: y holds at most 65535)
+template <typename T>
+static dim3 rows_grid(uint32_t M, uint32_t N) {
+    const uint32_t per = THREADS * Elem<T>::VEC;
+    return dim3((N + per - 1) / per, M < 65535u ? M : 65535u);
+}
+
+template <typename T, int ACT>
+__global__ __launch_bounds__(THREADS) void glu_join_kernel(uint32_t M, uint32_t N, const float* z, int64_t ldz, T* h,
+                                                           int64_t ldh, T* gu, int64_t ldgu) {
+    constexpr int VEC = Elem<T>::VEC;
+    const int64_t n = ((int64_t)blockIdx.x * THREADS + threadIdx.x) * VEC;
+    if (n >= N) return;
+    for (uint32_t m = blockIdx.y; m < M; m += gridDim.y) {
+        float g[VEC], u[VEC], r[VEC];
+#pragma unroll
+        for (int q = 0; q < VEC; q += 4) {
+            unpack<float>(ld_chunk(z + (int64_t)m * ldz, n + q, N), g + q);
+            unpack<float>(ld_chunk(z + (int64_t)m * ldz + N, n + q, N), u + q);
+        }
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) r[i] = act<ACT>(g[i]) * u[i];
+        st_chunk(h + (int64_t)m * ldh, n, N, pack<T>(r));
+        if (gu) {
+            st_chunk(gu + (int64_t)m * ldgu, n, N, pack<T>(g));
+            st_chunk(gu + (int64_t)m * ldgu + N, n, N, pack<T>(u));
+        }
+    }
+}
+
+// dgu may be gu: a thread reads its elements before it writes them
+template <typename T, int ACT>
+__global__ __launch_bounds__(THREADS) void glu_join_backward_kernel(uint32_t M, uint32_t N, const T* dh, int64_t lddh,
+                                                                    const T* gu, int64_t ldgu, T* dgu, int64_t lddgu) {
+    constexpr int VEC = Elem<T>::VEC;
+    const int64_t n = ((int64_t)blockIdx.x * THREADS + threadIdx.x) * VEC;
+    if (n >= N) return;
+    for (uint32_t m = blockIdx.y; m < M; m += gridDim.y) {
+        float g[VEC], u[VEC], d[VEC];
+        unpack<T>(ld_chunk(gu + (int64_t)m * ldgu, n, N), g);
+        unpack<T>(ld_chunk(gu + (int64_t)m * ldgu + N, n, N), u);
+        unpack<T>(ld_chunk(dh + (int64_t)m * lddh, n, N), d);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            float a, da;
+            act_and_slope<ACT>(g[i], a, da);
+            g[i] = d[i] * u[i] * da;
+            u[i] = d[i] * a;
+        }
+        st_chunk(dgu + (int64_t)m * lddgu, n, N, pack<T>(g));
+        st_chunk(dgu + (int64_t)m * lddgu + N, n, N, pack<T>(u));
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(THREADS) void scale_kernel(uint32_t M, uint32_t N, T* C, int64_t ldc, float beta) {
+    for (uint32_t m = blockIdx.y; m < M; m += gridDim.y)
+        for (int64_t n = (int64_t)blockIdx.x * THREADS + threadIdx.x; n < N; n += (int64_t)gridDim.x * THREADS) {
+            T* c = C + (int64_t)m * ldc + n;
+            *c = beta == 0.0f ? (T)0.0f : (T)(beta * (float)*c);
+        }
+}
+
+template <typename T>
+__global__ __launch_bounds__(THREADS) void convert_kernel(uint32_t M, uint32_t N, const float* A, int64_t lda, T* C,
+                                                          int64_t ldc) {
+    constexpr int VEC = Elem<T>::VEC;
+    const int64_t n = ((int64_t)blockIdx.x * THREADS + threadIdx.x) * VEC;
+    if (n >= N) return;
+    for (uint32_t m = blockIdx.y; m < M; m += gridDim.y) {
+        float x[VEC];
+#pragma unroll
+        for (int q = 0; q < VEC; q += 4) unpack<float>(ld_chunk(A + (int64_t)m * lda, n + q, N), x + q);
+        st_chunk(C + (int64_t)m * ldc, n, N, pack<T>(x));
+    }
+}
+
+}  // namespace
+}  // namespace vkb
+
+using namespace vkb;
+
+extern "C" int vkb_launch_glu_join(int type, int act_code, uint32_t M, uint32_t N, const float* z, int64_t ldz,
+                                   void* h, int64_t ldh, void* gu, int64_t ldgu, void* stream) {
+    const bool ok = with_type(type, [&](auto t) {
+        using T = decltype(t);
+        with_act(act_code, [&](auto a) {
+            hipLaunchKernelGGL((glu_join_kernel<T, decltype(a)::value>), rows_grid<T>(M, N), dim3(THREADS), 0,
+                               (hipStream_t)stream, M, N, z, ldz, (T*)h, ldh, (T*)gu, ldgu);
+        });
+    });
+    return ok ? (int)hipGetLastError() : (int)hipErrorInvalidValue;
+}
+
+extern "C" int vkb_launch_glu_join_backward(int type, int act_code, uint32_t M, uint32_t N, const void* dh,
+                                            int64_t lddh, const void* gu, int64_t ldgu, void* dgu, int64_t lddgu,
+                                            void* stream) {
+    const bool ok = with_type(type, [&](auto t) {
+        using T = decltype(t);
+        with_act(act_code, [&](auto a) {
+            hipLaunchKernelGGL((glu_join_backward_kernel<T, decltype(a)::value>), rows_grid<T>(M, N), dim3(THREADS),
+                               0, (hipStream_t)stream, M, N, (const T*)dh, lddh, (const T*)gu, ldgu, (T*)dgu, lddgu);
+        });
+    });
+    return ok ? (int)hipGetLastError() : (int)hipErrorInvalidValue;
+}
+
+extern "C" int vkb_launch_scale(int type, uint32_t M, uint32_t N, void* C, int64_t ldc, float beta, void* stream) {
+    const bool ok = with_type(type, [&](auto t) {
+        using T = decltype(t);
+        hipLaunchKernelGGL((scale_kernel<T>), rows_grid<T>(M, N), dim3(THREADS), 0, (hipStream_t)stream, M, N, (T*)C,
+                           ldc, beta);
+    });
+    return ok ? (int)hipGetLastError() : (int)hipErrorInvalidValue;
+}
+
+extern "C" int vkb_launch_convert(int type, uint32_t M, uint32_t N, const float* A, int64_t lda, void* C, int64_t ldc,
+                                  void* stream) {
+    const bool ok = with_type(type, [&](auto t) {
+        using T = decltype(t);
+        hipLaunchKernelGGL((convert_kernel<T>), rows_grid<T>(M, N), dim3(THREADS), 0, (hipStream_t)stream, M, N, A,
+                           lda, (T*)C, ldc);
+    });
+    return ok ? (int)hipGetLastError() : (int)hipErrorInvalidValue;
+}

@@ -1,0 +1,138 @@
+// nn_common.hpp — what the kernels of vkblas_nn.h share: 16-byte accesses of
+// any element alignment, reductions over a wave, the activations.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+#include "gemm_mfma.hpp"
+#include "vkb_launch.h"
+#include "vkblas_nn.h"
+
+namespace vkb {
+
+// VEC = 16 / sizeof(T) values of a row from n on, of which only those below N
+// exist; the others read as zero.  The address has its element's alignment.
+template <typename T>
+__device__ __forceinline__ u32x4 ld_chunk(const T* row, int64_t n, int64_t N) {
+    constexpr int VEC = Elem<T>::VEC;
+    if (n + VEC <= N) return ld16_any(row + n);
+    u32x4 v = {0u, 0u, 0u, 0u};
+    if (n < N) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            if (n + i >= N) break;
+            if constexpr (sizeof(T) == 4) v[i] = *(const uint32_t*)(row + n + i);
+            else v[i / 2] |= (uint32_t)*(const uint16_t*)(row + n + i) << (16 * (i & 1));
+        }
+    }
+    return v;
+}
+
+template <typename T>
+__device__ __forceinline__ void unpack(u32x4 v, float* x) {
+    constexpr int VEC = Elem<T>::VEC;
+    typedef T tvec __attribute__((ext_vector_type(VEC)));
+    const tvec t = __builtin_bit_cast(tvec, v);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) x[i] = (float)t[i];
+}
+
+template <typename T>
+__device__ __forceinline__ u32x4 pack(const float* x) {
+    constexpr int VEC = Elem<T>::VEC;
+    typedef T tvec __attribute__((ext_vector_type(VEC)));
+    tvec t;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) t[i] = (T)x[i];
+    return __builtin_bit_cast(u32x4, t);
+}
+
+template <typename T>
+__device__ __forceinline__ void st_chunk(T* row, int64_t n, int64_t N, u32x4 v) {
+    constexpr int VEC = Elem<T>::VEC;
+    if (n + VEC <= N) {
+        *(u32x4_any*)(row + n) = v;
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+        if (n + i >= N) break;
+        if constexpr (sizeof(T) == 4) *(uint32_t*)(row + n + i) = v[i];
+        else *(uint16_t*)(row + n + i) = (uint16_t)(v[i / 2] >> (16 * (i & 1)));
+    }
+}
+
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
+    return v;
+}
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+    for (int d = 32; d; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
+    return v;
+}
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+// exp(x) by the hardware's 2^x: relative error about |x| 2^-24 from rounding
+// x log2(e), plus one unit of the result
+__device__ __forceinline__ float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * LOG2E); }
+__device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + fast_exp(-x)); }
+
+constexpr float GELU_C = 0.7978845608028654f;   // sqrt(2 / pi)
+constexpr float GELU_A = 0.044715f;
+
+template <int ACT>
+__device__ __forceinline__ float act(float g) {
+    if constexpr (ACT == VKBLAS_ACT_SILU) return g * sigmoid(g);
+    // (1 + tanh y) / 2 = 1 / (1 + exp(-2 y))
+    if constexpr (ACT == VKBLAS_ACT_GELU_TANH) return g * sigmoid(2.0f * GELU_C * (g + GELU_A * g * g * g));
+    if constexpr (ACT == VKBLAS_ACT_GELU) return 0.5f * g * (1.0f + erff(g * 0.7071067811865476f));
+    return g > 0.0f ? g : (g != g ? g : 0.0f);   // max(g, 0), a NaN stays
+}
+
+// act(g) and its derivative
+template <int ACT>
+__device__ __forceinline__ void act_and_slope(float g, float& a, float& da) {
+    if constexpr (ACT == VKBLAS_ACT_SILU) {
+        const float s = sigmoid(g);
+        a = g * s;
+        da = s + a * (1.0f - s);
+    } else if constexpr (ACT == VKBLAS_ACT_GELU_TANH) {
+        const float s = sigmoid(2.0f * GELU_C * (g + GELU_A * g * g * g));
+        a = g * s;
+        da = s + a * (1.0f - s) * (2.0f * GELU_C * (1.0f + 3.0f * GELU_A * g * g));
+    } else if constexpr (ACT == VKBLAS_ACT_GELU) {
+        const float p = 0.5f * (1.0f + erff(g * 0.7071067811865476f));
+        a = g * p;
+        da = p + g * (0.3989422804014327f * fast_exp(-0.5f * g * g));
+    } else {
+        a = act<ACT>(g);
+        da = g > 0.0f ? 1.0f : (g != g ? g : 0.0f);
+    }
+}
+
+// f(integral_constant<int, ACT>) for the activation's code; false: unknown
+template <typename F>
+static inline bool with_act(int code, F f) {
+    switch (code) {
+        case VKBLAS_ACT_SILU: f(std::integral_constant<int, VKBLAS_ACT_SILU>{}); return true;
+        case VKBLAS_ACT_GELU: f(std::integral_constant<int, VKBLAS_ACT_GELU>{}); return true;
+        case VKBLAS_ACT_GELU_TANH: f(std::integral_constant<int, VKBLAS_ACT_GELU_TANH>{}); return true;
+        case VKBLAS_ACT_RELU: f(std::integral_constant<int, VKBLAS_ACT_RELU>{}); return true;
+        default: return false;
+    }
+}
+
+// f(T{}) for the element type's code; false: unknown
+template <typename F>
+static inline bool with_type(int code, F f) {
+    switch (code) {
+        case VKB_T_F32: f(float{}); return true;
+        case VKB_T_F16: f((_Float16)0); return true;
+        case VKB_T_BF16: f((__bf16)0.0f); return true;
+        default: return false;
+    }
+}
+
+}  // namespace vkb

@@ -1,0 +1,62 @@
+/*
+ * vkb_nn_launch.h — internal C ABI between the host side of the operators in
+ * vkblas_nn.h (nn.c) and their gfx950 kernels.  As vkb_launch.h: plain
+ * pointers and sizes, element types VKB_T_*, every launcher enqueues on the
+ * stream and returns 0 or a hipError_t value.
+ */
+#pragma once
+#include <stdint.h>
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+/* Layer norm (layer_norm.hip).  The backward pass writes its partial sums of
+ * dw and db to part, vkb_layer_norm_parts rows of 2 N floats (dw's N, then
+ * db's), and vkb_launch_layer_norm_reduce adds them up. */
+int vkb_launch_layer_norm(int type, int w_type, uint32_t M, uint32_t N, const void* x, int64_t ldx, const void* w,
+                          const void* b, float eps, void* y, int64_t ldy, float* mean, float* rstd, void* stream);
+uint32_t vkb_layer_norm_parts(int type, uint32_t M, uint32_t N);
+int vkb_layer_norm_long(uint32_t N);   /* rows past a workgroup's registers */
+int vkb_launch_layer_norm_backward(int type, int w_type, uint32_t M, uint32_t N, const void* dy, int64_t lddy,
+                                   const void* x, int64_t ldx, const void* w, const float* mean, const float* rstd,
+                                   void* dx, int64_t lddx, float* part, void* stream);
+int vkb_launch_layer_norm_reduce(const float* part, uint32_t parts, uint32_t N, void* dw, void* db, int g_type,
+                                 float beta, void* stream);
+
+/* C = beta * C on M x N (a gradient over an empty batch). */
+int vkb_launch_scale(int type, uint32_t M, uint32_t N, void* C, int64_t ldc, float beta, void* stream);
+
+/* C = A rounded to type, A in fp32. */
+int vkb_launch_convert(int type, uint32_t M, uint32_t N, const float* A, int64_t lda, void* C, int64_t ldc,
+                       void* stream);
+
+/* Gated projection (glu.hip), from projections computed before:
+ * h = act(G) * U from z = [G | U] in fp32, and gu = z rounded (NULL: not
+ * stored); and [dG | dU] from dh and gu. */
+int vkb_launch_glu_join(int type, int act, uint32_t M, uint32_t N, const float* z, int64_t ldz, void* h, int64_t ldh,
+                        void* gu, int64_t ldgu, void* stream);
+int vkb_launch_glu_join_backward(int type, int act, uint32_t M, uint32_t N, const void* dh, int64_t lddh,
+                                 const void* gu, int64_t ldgu, void* dgu, int64_t lddgu, void* stream);
+
+/* Linear cross entropy (xent.hip).  stats: over z, columns v0 .. v0 + n - 1
+ * of the logits, the pair (max, sum of exp(z - max)) of each row and each
+ * VKB_XENT_SLICE columns, to parts[slice * M + m], and the target's logit to
+ * zt[m].  finish: lse and loss of S such slices. */
+#define VKB_XENT_SLICE 4096u
+int vkb_launch_xent_stats(uint32_t M, uint32_t n, uint32_t v0, const float* z, int64_t ldz, const int64_t* target,
+                          float* parts, float* zt, void* stream);
+int vkb_launch_xent_finish(uint32_t M, uint32_t V, uint32_t S, const float* parts, const float* zt,
+                           const int64_t* target, int64_t ignore, float* loss, float* lse, void* stream);
+/* scal[0] = the power of two s that brings max |dloss| into [2^13, 2^14),
+ * scal[1] = 1 / s, scal[2] = beta, scal[3] = 1, scal[4] = 0 (device scalars
+ * of products). */
+int vkb_launch_xent_scale(uint32_t M, const float* dloss, float beta, float* scal, void* stream);
+/* D = scal[0] * dloss * (exp(z - lse) - [v == target]), scal NULL = 1. */
+int vkb_launch_xent_grad(int type, uint32_t M, uint32_t n, uint32_t v0, uint32_t V, const float* z, int64_t ldz,
+                         const int64_t* target, int64_t ignore, const float* lse, const float* dloss,
+                         const float* scal, void* D, int64_t ldd, void* stream);
+
+#ifdef __cplusplus
+}
+#endif

@@ -1,0 +1,192 @@
+// xent.hip — softmax cross entropy on logits that a GEMM computed in pieces
+// of the vocabulary: each piece's row statistics, their join into log-sum-exp
+// and loss, and the logits' gradient.
+//
+// A row's statistics over some columns are the pair (top, s): top = max z and
+// s = sum exp(z - top), and pairs join by
+//   T = max top_i,  S = sum s_i exp(top_i - T),  lse = T + log S.
+// Infinities follow the formula: where top is not finite the exponentials
+// take 0 in its place, so an all -inf part has s = 0 and drops out of the
+// join, a +inf gives s = inf and lse = inf, and a NaN reaches s and lse.
+#include "nn_common.hpp"
+#include "vkb_nn_launch.h"
+
+namespace vkb {
+namespace {
+
+constexpr uint32_t THREADS = 256, WAVES = THREADS / 64;
+
+__device__ __forceinline__ float finite_or_0(float x) { return __builtin_isinf(x) ? 0.0f : x; }
+
+__device__ __forceinline__ float block_max(float v, float* sh) {
+    v = wave_max(v);
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+    __syncthreads();
+    float r = sh[0];
+    for (uint32_t i = 1; i < WAVES; ++i) r = fmaxf(r, sh[i]);
+    __syncthreads();
+    return r;
+}
+__device__ __forceinline__ float block_sum(float v, float* sh) {
+    v = wave_sum(v);
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+    __syncthreads();
+    float r = sh[0];
+    for (uint32_t i = 1; i < WAVES; ++i) r += sh[i];
+    __syncthreads();
+    return r;
+}
+
+// One workgroup per row and slice of VKB_XENT_SLICE columns, the slice in
+// registers between the two reductions; rows strided over y.
+__global__ __launch_bounds__(THREADS) void xent_stats_kernel(uint32_t M, uint32_t n, uint32_t v0, const float* z,
+                                                             int64_t ldz, const int64_t* target, float2* parts,
+                                                             float* zt) {
+    constexpr int NV = VKB_XENT_SLICE / THREADS / 4;
+    __shared__ float sh[WAVES];
+    const int64_t c0 = (int64_t)blockIdx.x * VKB_XENT_SLICE + threadIdx.x * 4;
+    for (uint32_t m = blockIdx.y; m < M; m += gridDim.y) {
+        const float* row = z + (int64_t)m * ldz;
+        float x[NV][4], top = -INFINITY, s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int64_t c = c0 + (int64_t)i * THREADS * 4;
+            unpack<float>(ld_chunk(row, c, n), x[i]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (c + e >= n) x[i][e] = -INFINITY;
+                top = fmaxf(top, x[i][e]);
+            }
+        }
+        top = block_max(top, sh);
+        const float off = finite_or_0(top);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s += fast_exp(x[i][e] - off);
+        s = block_sum(s, sh);
+        if (threadIdx.x == 0) {
+            parts[(int64_t)blockIdx.x * M + m] = float2{top, s};
+            if (target) {
+                const int64_t t = target[m] - v0 - (int64_t)blockIdx.x * VKB_XENT_SLICE;
+                if (t >= 0 && t < VKB_XENT_SLICE && target[m] - v0 < n) zt[m] = row[target[m] - v0];
+            }
+        }
+    }
+}
+
+// 16 rows x 16 lanes per workgroup: lane j of a row joins slices j, j + 16, ..
+__global__ __launch_bounds__(THREADS) void xent_finish_kernel(uint32_t M, uint32_t V, uint32_t S, const float2* parts,
+                                                              const float* zt, const int64_t* target, int64_t ignore,
+                                                              float* loss, float* lse) {
+    __shared__ float2 sh[16][17];
+    const uint32_t r = threadIdx.x & 15, j = threadIdx.x >> 4;
+    const uint32_t m = blockIdx.x * 16 + r;
+    float top = -INFINITY, s = 0.0f;
+    if (m < M)
+        for (uint32_t i = j; i < S; i += 16) {
+            const float2 p = parts[(int64_t)i * M + m];
+            const float t = fmaxf(top, p.x), off = finite_or_0(t);
+            s = s * fast_exp(top - off) + p.y * fast_exp(p.x - off);
+            top = t;
+        }
+    sh[j][r] = float2{top, s};
+    __syncthreads();
+    if (j || m >= M) return;
+    for (uint32_t i = 1; i < 16; ++i) top = fmaxf(top, sh[i][r].x);
+    const float off = finite_or_0(top);
+    s = 0.0f;
+    for (uint32_t i = 0; i < 16; ++i) s += sh[i][r].y * fast_exp(sh[i][r].x - off);
+    const float l = off + logf(s);
+    lse[m] = l;
+    if (loss) {
+        const int64_t t = target[m];
+        loss[m] = t == ignore ? 0.0f : (t >= 0 && t < V ? l - zt[m] : __builtin_nanf(""));
+    }
+}
+
+__global__ __launch_bounds__(1024) void xent_scale_kernel(uint32_t M, const float* dloss, float beta, float* scal) {
+    __shared__ float sh[16];
+    float top = 0.0f;
+    for (uint32_t m = threadIdx.x; m < M; m += 1024) top = fmaxf(top, fabsf(dloss[m]));
+    top = wave_max(top);
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = top;
+    __syncthreads();
+    if (threadIdx.x) return;
+    for (int i = 1; i < 16; ++i) top = fmaxf(top, sh[i]);
+    int e = 0;
+    if (top > 0.0f && !__builtin_isinf(top)) {
+        e = 13 - ilogbf(top);
+        e = e > 100 ? 100 : e < -100 ? -100 : e;
+    }
+    scal[0] = ldexpf(1.0f, e);
+    scal[1] = ldexpf(1.0f, -e);
+    scal[2] = beta;
+    scal[3] = 1.0f;
+    scal[4] = 0.0f;
+}
+
+template <typename T>
+__global__ __launch_bounds__(THREADS) void xent_grad_kernel(uint32_t M, uint32_t n, uint32_t v0, uint32_t V,
+                                                            const float* z, int64_t ldz, const int64_t* target,
+                                                            int64_t ignore, const float* lse, const float* dloss,
+                                                            const float* scal, T* D, int64_t ldd) {
+    constexpr int VEC = Elem<T>::VEC;
+    const int64_t c = ((int64_t)blockIdx.x * THREADS + threadIdx.x) * VEC;
+    if (c >= n) return;
+    const float sc = scal ? scal[0] : 1.0f;
+    for (uint32_t m = blockIdx.y; m < M; m += gridDim.y) {
+        const int64_t t = target[m];
+        const float l = lse[m];
+        // the three kinds of rows: counted, ignored (all zero), target out of range (all NaN)
+        const float k = t == ignore ? 0.0f : (t >= 0 && t < V ? dloss[m] * sc : __builtin_nanf(""));
+        float x[VEC];
+#pragma unroll
+        for (int q = 0; q < VEC; q += 4) unpack<float>(ld_chunk(z + (int64_t)m * ldz, c + q, n), x + q);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            const float p = fast_exp(x[i] - l) - (c + i == t - v0 ? 1.0f : 0.0f);
+            x[i] = t == ignore ? 0.0f : k * p;
+        }
+        st_chunk(D + (int64_t)m * ldd, c, n, pack<T>(x));
+    }
+}
+
+}  // namespace
+}  // namespace vkb
+
+using namespace vkb;
+
+static uint32_t rows_y(uint32_t M) { return M < 65535u ? M : 65535u; }
+
+extern "C" int vkb_launch_xent_stats(uint32_t M, uint32_t n, uint32_t v0, const float* z, int64_t ldz,
+                                     const int64_t* target, float* parts, float* zt, void* stream) {
+    hipLaunchKernelGGL(xent_stats_kernel, dim3((n + VKB_XENT_SLICE - 1) / VKB_XENT_SLICE, rows_y(M)), dim3(THREADS), 0,
+                       (hipStream_t)stream, M, n, v0, z, ldz, target, (float2*)parts, zt);
+    return (int)hipGetLastError();
+}
+
+extern "C" int vkb_launch_xent_finish(uint32_t M, uint32_t V, uint32_t S, const float* parts, const float* zt,
+                                      const int64_t* target, int64_t ignore, float* loss, float* lse, void* stream) {
+    // 2^31 rows / 16 per workgroup: below 2^32 threads
+    hipLaunchKernelGGL(xent_finish_kernel, dim3((uint32_t)(((uint64_t)M + 15) / 16)), dim3(THREADS), 0,
+                       (hipStream_t)stream, M, V, S, (const float2*)parts, zt, target, ignore, loss, lse);
+    return (int)hipGetLastError();
+}
+
+extern "C" int vkb_launch_xent_scale(uint32_t M, const float* dloss, float beta, float* scal, void* stream) {
+    hipLaunchKernelGGL(xent_scale_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, M, dloss, beta, scal);
+    return (int)hipGetLastError();
+}
+
+extern "C" int vkb_launch_xent_grad(int type, uint32_t M, uint32_t n, uint32_t v0, uint32_t V, const float* z,
+                                    int64_t ldz, const int64_t* target, int64_t ignore, const float* lse,
+                                    const float* dloss, const float* scal, void* D, int64_t ldd, void* stream) {
+    const bool ok = with_type(type, [&](auto t) {
+        using T = decltype(t);
+        const uint32_t per = THREADS * Elem<T>::VEC;
+        hipLaunchKernelGGL((xent_grad_kernel<T>), dim3((n + per - 1) / per, rows_y(M)), dim3(THREADS), 0,
+                           (hipStream_t)stream, M, n, v0, V, z, ldz, target, ignore, lse, dloss, scal, (T*)D, ldd);
+    });
+    return ok ? (int)hipGetLastError() : (int)hipErrorInvalidValue;
+}
