@@ -64,8 +64,9 @@ typedef enum {
     /* the operators of vkblas_nn.h */
     VKBLAS_KERNEL_NORM = 10,            /* layer norm, rows in registers        */
     VKBLAS_KERNEL_NORM_LONG = 11,       /* layer norm, rows read again          */
-    VKBLAS_KERNEL_JOINED = 12           /* GEMMs by their plans, then a kernel
+    VKBLAS_KERNEL_JOINED = 12,          /* GEMMs by their plans, then a kernel
                                            over their results                   */
+    VKBLAS_KERNEL_FUSED = 13            /* inside the pipelined GEMM kernel     */
 } vkblas_kernel_t;
 
 typedef struct {

@@ -119,6 +119,20 @@ constexpr RdSeq make_rdseq() {
     return r;
 }
 
+// What a kernel does with its tile of A B^T.  PlainOp: the GEMM's epilogue
+// below.  Other operators (gemm_ops.hpp) take the accumulators from here, on
+// K-major operands:
+//  * OP::Params: KParams with the operator's own arguments;
+//  * GATED: B has 2 N rows and a tile holds BN / 2 columns of both halves: of
+//    each wave's WT columns the first WT / 2 are rows n of B, the others rows
+//    N + n, so a lane holds both products of one output;
+//  * any M and N: rows past the last are read as the last (an offset register
+//    per DMA instruction), and the operator drops their results.
+struct PlainOp {
+    using Params = KParams;
+    static constexpr bool PLAIN = true, GATED = false;
+};
+
 // WT: wave tile edge.  128: 256x256 workgroup tile, one workgroup per CU;
 // 64: 128x128 workgroup tile for shapes with too few 256x256 tiles to fill
 // the chip (fp32 always with two stages).
@@ -126,9 +140,11 @@ constexpr RdSeq make_rdseq() {
 // (WT 64 only, 144 KB: one workgroup per CU, for grids of at most one
 // workgroup per CU): three steps ahead, since a 128x128 step (512 MFMA
 // cycles) is shorter than the load latency.
-template <typename T, typename TC, bool AK, bool BKM, int WT = 128, int NST = 2>
-__global__ __launch_bounds__(256, (WT == 128 || NST == 4) ? 1 : 2) void gemm_pipe_kernel(KParams p) {
+template <typename T, typename TC, bool AK, bool BKM, int WT = 128, int NST = 2, typename OP = PlainOp>
+__global__ __launch_bounds__(256, (WT == 128 || NST == 4) ? 1 : 2) void gemm_pipe_kernel(typename OP::Params p) {
     constexpr bool F16 = sizeof(T) == 2;
+    constexpr bool CLIP = !OP::PLAIN;
+    static_assert(!CLIP || (AK && BKM), "operators: K-major operands");
     static_assert(WT == 128 || WT == 64, "256x256 or 128x128 tiles");
     static_assert(NST == 2 || (NST == 4 && WT == 64 && F16), "four stages: 16-bit 128x128 tiles only");
     constexpr int ES = sizeof(T);                   // element bytes
@@ -172,9 +188,9 @@ __global__ __launch_bounds__(256, (WT == 128 || NST == 4) ? 1 : 2) void gemm_pip
     // starts at row 0, A rows past M - 1 are read as row M - 1 and C rows
     // from M on are not stored.
     const int m_lo = (int)(first_m + tin % gm) * BM;
-    const int n_lo = (int)(tin / gm) * BN;
-    const int m0 = max(0, min(m_lo, (int)p.M - BM));
-    const int n0 = min(n_lo, (int)p.N - BN);
+    const int n_lo = (int)(tin / gm) * (OP::GATED ? BN / 2 : BN);
+    const int m0 = CLIP ? m_lo : max(0, min(m_lo, (int)p.M - BM));
+    const int n0 = CLIP ? n_lo : min(n_lo, (int)p.N - BN);
 
     const int lda = (int)p.lda, ldb = (int)p.ldb;
     // Split-K pass 1 (split > 1, batch 1): slice b covers k in
@@ -187,7 +203,9 @@ __global__ __launch_bounds__(256, (WT == 128 || NST == 4) ? 1 : 2) void gemm_pip
     // Buffer resources on the tile's first element; all per-lane parts are
     // 32-bit byte offsets (the launcher guarantees they fit).
     const T* At = (const T*)p.A + bat * p.sa + (AK ? (int64_t)m0 * p.lda + kbeg : kbeg * p.lda + m0);
-    const T* Bt = (const T*)p.B + bat * p.sb + (BKM ? (int64_t)n0 * p.ldb + kbeg : kbeg * p.ldb + n0);
+    // GATED: even waves load the first half's rows, odd ones the second's
+    const int64_t brow = OP::GATED ? (int64_t)(wave & 1) * p.N + n0 : n0;
+    const T* Bt = (const T*)p.B + bat * p.sb + (BKM ? brow * p.ldb + kbeg : kbeg * p.ldb + n0);
     const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc((void*)At, (short)0, -1, 0x00020000);
     const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc((void*)Bt, (short)0, -1, 0x00020000);
     TC* Cb = (TC*)p.C + (sk ? (int64_t)b * p.s_split : (int64_t)b * p.sc);
@@ -202,12 +220,20 @@ __global__ __launch_bounds__(256, (WT == 128 || NST == 4) ? 1 : 2) void gemm_pip
     const int a_voff = ((BM / 4) * wave + (lane >> 3)) * lda * ES + koff;
     // 128x128 tiles: one VGPR offset per instruction, its row clamped to the
     // last row of A (a no-op unless M < BM)
-    constexpr int NAV = (WT == 64 && AK) ? NDMA : 1;
+    constexpr int NAV = ((WT == 64 || CLIP) && AK) ? NDMA : 1;
     int a_vn[NAV];
 #pragma unroll
     for (int n = 0; n < NAV; ++n)
         a_vn[n] = min((BM / 4) * wave + (lane >> 3) + 8 * n, (int)p.M - 1 - m0) * lda * ES + koff;
     const int b_voff = ((BN / 4) * wave + (lane >> 3)) * ldb * ES + koff;
+    constexpr int NBV = CLIP ? NDMA : 1;
+    int b_vn[NBV];
+    if constexpr (CLIP) {
+#pragma unroll
+        for (int n = 0; n < NBV; ++n)
+            b_vn[n] = min((OP::GATED ? (BN / 4) * (wave >> 1) : (BN / 4) * wave) + (lane >> 3) + 8 * n,
+                          (int)p.N - 1 - n0) * ldb * ES + koff;
+    }
     // 16-bit MN-major direct loads: instruction n of this wave fills the
     // 1-KiB block NDMA wave + n (k rows RPB (NDMA wave + n) + [0, RPB); lane ->
     // row + lane / CPR, slot lane % CPR, which holds chunk
@@ -291,7 +317,9 @@ __global__ __launch_bounds__(256, (WT == 128 || NST == 4) ? 1 : 2) void gemm_pip
                     (k0 + MNR * (NDMA * wave + n)) * lda * ES);
         } else {
             const int m = n - NDMA;
-            if constexpr (BKM)
+            if constexpr (CLIP)
+                dma(false, (lds_ptr_t)&lds[B0 + S * STG + (NDMA * wave + m) * GRP], b_vn[m], k0 * ES);
+            else if constexpr (BKM)
                 dma(false, (lds_ptr_t)&lds[B0 + S * STG + (NDMA * wave + m) * GRP], b_voff, (k0 + m * 8 * ldb) * ES);
             else if constexpr (BTR)
                 dma(false, (lds_ptr_t)&lds[B0 + S * STG + (NDMA * wave + m) * 64], b_tr[trv(m)],
@@ -576,6 +604,10 @@ __global__ __launch_bounds__(256, (WT == 128 || NST == 4) ? 1 : 2) void gemm_pip
     // instead, two of them were spilled to scratch on every call.
     {
     const int lane = fresh_lane_id();
+    if constexpr (CLIP) {
+        OP::template run<WT, SH, sizeof(lds)>(p, acc, (char*)lds, m0, n0, wave, lane);
+        return;
+    } else {
     const int h = lane >> 5;
     const int fl = SH == 0 ? (lane & 15) : (lane & 31);
     float alpha, beta;
@@ -802,6 +834,7 @@ __global__ __launch_bounds__(256, (WT == 128 || NST == 4) ? 1 : 2) void gemm_pip
                 }
             }
         }
+    }
     }
     }
 }

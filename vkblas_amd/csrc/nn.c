@@ -18,6 +18,8 @@
 #define DIM_MAX 0x7fffffffu
 /* fp32 logits or projections that a joined call holds at a time */
 #define JOIN_BYTES ((uint64_t)256 << 20)
+/* the logits' gradient of a piece of the vocabulary */
+#define PIECE_BYTES ((uint64_t)512 << 20)
 
 static int known_type(vkblas_dtype_t t) {
     return t == VKBLAS_DT_F32 || t == VKBLAS_DT_F16 || t == VKBLAS_DT_BF16;
@@ -115,8 +117,71 @@ static int product(op_call* c, vkblas_dtype_t ab, vkblas_dtype_t ct, vkblas_op_t
 static vkblas_status_t op_end(op_call* c, int kernel) {
     if (c->held) vkb_ws_release(&c->ws);
     vkb_prof_end(&c->prof, c->stream, c->what, c->st == VKBLAS_OK);
-    if (c->st == VKBLAS_OK) vkb_engine_ran(kernel == VKBLAS_KERNEL_JOINED ? vkblas_last_path() : VKBLAS_PATH_NONE, kernel);
+    if (c->st == VKBLAS_OK) vkb_engine_ran(kernel >= VKBLAS_KERNEL_JOINED ? vkblas_last_path() : VKBLAS_PATH_NONE, kernel);
     return c->st;
+}
+
+/* ------------------------------------------- inside the pipelined kernel */
+
+extern int vkb_launch_glu_f32(const vkb_op_args*, int, void*, int64_t, void*, int64_t, void*);
+extern int vkb_launch_glu_f16(const vkb_op_args*, int, void*, int64_t, void*, int64_t, void*);
+extern int vkb_launch_glu_bf16(const vkb_op_args*, int, void*, int64_t, void*, int64_t, void*);
+extern int vkb_launch_xent_stats_f32(const vkb_op_args*, const int64_t*, float*, float*, void*);
+extern int vkb_launch_xent_stats_f16(const vkb_op_args*, const int64_t*, float*, float*, void*);
+extern int vkb_launch_xent_stats_bf16(const vkb_op_args*, const int64_t*, float*, float*, void*);
+typedef int xent_grad_fn(const vkb_op_args*, uint32_t, uint32_t, const int64_t*, int64_t, const float*, const float*,
+                         const float*, void*, int64_t, void*);
+extern xent_grad_fn vkb_launch_xent_grad_f32, vkb_launch_xent_grad_f16, vkb_launch_xent_grad_bf16;
+
+int vkb_launch_glu(const vkb_op_args* a, int act, void* h, int64_t ldh, void* gu, int64_t ldgu, void* stream) {
+    return (a->type == VKB_T_F16 ? vkb_launch_glu_f16 : a->type == VKB_T_BF16 ? vkb_launch_glu_bf16
+                                                                             : vkb_launch_glu_f32)(
+        a, act, h, ldh, gu, ldgu, stream);
+}
+int vkb_launch_xent_stats_op(const vkb_op_args* a, const int64_t* target, float* parts, float* zt, void* stream) {
+    return (a->type == VKB_T_F16 ? vkb_launch_xent_stats_f16 : a->type == VKB_T_BF16 ? vkb_launch_xent_stats_bf16
+                                                                                    : vkb_launch_xent_stats_f32)(
+        a, target, parts, zt, stream);
+}
+int vkb_launch_xent_grad_op(const vkb_op_args* a, uint32_t v0, uint32_t V, const int64_t* target, int64_t ignore,
+                            const float* lse, const float* dloss, const float* scal, void* D, int64_t ldd,
+                            void* stream) {
+    return (a->type == VKB_T_F16 ? vkb_launch_xent_grad_f16 : a->type == VKB_T_BF16 ? vkb_launch_xent_grad_bf16
+                                                                                   : vkb_launch_xent_grad_f32)(
+        a, v0, V, target, ignore, lse, dloss, scal, D, ldd, stream);
+}
+uint32_t vkb_xent_slices(const vkb_op_args* a) {
+    const uint64_t tile = vkb_tile_bn(a->tile);
+    return (uint32_t)(((uint64_t)a->N + tile - 1) / tile * 2);
+}
+
+/* Whether the pipelined kernel takes x w^T with an operator at its end, and
+ * on which tiles; cols: the columns that one tile of 256 holds (128 gated).
+ *  - 16-byte aligned operands and leading dimensions, K in whole steps: 64 for
+ *    16-bit types, from two steps on, and pairs of 32 for fp32; the bytes
+ *    that a tile's rows span below 2^31 (offsets are 32-bit);
+ *  - more than 64 rows: below that the decode kernels stream the weight;
+ *  - 256 x 256 tiles where the planner of the plain products takes them:
+ *    16-bit from more than 128 of them on, fp32 for about whole waves. */
+static int op_plan(vkblas_dtype_t type, uint32_t M, uint32_t N, uint32_t K, const void* x, uint32_t ldx,
+                   const void* w, uint32_t ldw, uint32_t cols, vkb_op_args* a) {
+    const uint32_t vec = type == VKBLAS_DT_F32 ? 4 : 8;
+    const uint64_t es = type_size(type);
+    const uint64_t ld = ldx > ldw ? ldx : ldw;
+    if (!aligned16(x) || !aligned16(w) || ldx % vec || ldw % vec || K % 64 || K < 128 || M <= 64 ||
+        (256 * ld + K) * es >= 1ull << 31)
+        return 0;
+    const uint64_t t = (uint64_t)((M + 255) / 256) * ((N + cols - 1) / cols);
+    a->x = x;
+    a->w = w;
+    a->ldx = ldx;
+    a->ldw = ldw;
+    a->M = M;
+    a->N = N;
+    a->K = K;
+    a->type = type;
+    a->tile = (type == VKBLAS_DT_F32 ? 8 * t >= 7 * 256 * ((t + 255) / 256) : t > 128) ? VKB_TILE_256 : VKB_TILE_128;
+    return 1;
 }
 
 /* A gradient over no rows: C = beta * C. */
@@ -187,6 +252,12 @@ vkblas_status_t vkblas_glu_async(vkblas_dtype_t type, vkblas_act_t act, uint32_t
     op_call c;
     op_begin(&c, "glu", stream);
     if (vkb_engine_trace()) fprintf(stderr, "[vkblas] glu type=%d act=%d M=%u N=%u K=%u\n", (int)type, (int)act, M, N, K);
+    vkb_op_args a;
+    if (op_plan(type, M, N, K, x, ldx, w, ldw, 128, &a)) {
+        if (room(&c) != VKBLAS_OK) return c.st;
+        step(&c, vkb_launch_glu(&a, act, h, ldh, gu, ldgu, stream), 1);
+        return op_end(&c, VKBLAS_KERNEL_FUSED);
+    }
     /* both projections in fp32, some rows at a time, then the join; an fp32
      * gu takes them itself */
     const int direct = type == VKBLAS_DT_F32 && gu;
@@ -248,6 +319,8 @@ vkblas_status_t vkblas_glu_backward_async(vkblas_dtype_t type, vkblas_act_t act,
 
 /* --------------------------------------------------- linear cross entropy */
 
+typedef struct { uint32_t v, cols; } piece_t;
+
 /* Columns of the vocabulary at a time, so that M of them take about `bytes`
  * at `each` bytes a logit: whole slices of 256. */
 static uint32_t piece_columns(uint32_t M, uint32_t V, uint64_t bytes, uint64_t each) {
@@ -267,6 +340,16 @@ vkblas_status_t vkblas_linear_xent_async(vkblas_dtype_t type, uint32_t M, uint32
     op_call c;
     op_begin(&c, "linear_xent", stream);
     if (vkb_engine_trace()) fprintf(stderr, "[vkblas] linear_xent type=%d M=%u V=%u K=%u\n", (int)type, M, V, K);
+    vkb_op_args a;
+    if (op_plan(type, M, V, K, x, ldx, w, ldw, 256, &a)) {
+        const uint32_t S = vkb_xent_slices(&a);
+        const size_t o_p = buf(&c, (uint64_t)S * M * 2 * sizeof(float)), o_t = buf(&c, (uint64_t)M * sizeof(float));
+        if (room(&c) != VKBLAS_OK) return c.st;
+        float *parts = at(&c, o_p), *zt = at(&c, o_t);
+        if (step(&c, vkb_launch_xent_stats_op(&a, target, parts, zt, stream), 0))
+            step(&c, vkb_launch_xent_finish(M, V, S, parts, zt, target, ignore_index, loss, lse, stream), 1);
+        return op_end(&c, VKBLAS_KERNEL_FUSED);
+    }
     const uint32_t n = piece_columns(M, V, JOIN_BYTES, sizeof(float)), ldz = (uint32_t)round_up(n, 4);
     const uint32_t last = V % n;
     const uint32_t per = (n + VKB_XENT_SLICE - 1) / VKB_XENT_SLICE;   /* slices of a piece; the last may have fewer */
@@ -307,46 +390,66 @@ vkblas_status_t vkblas_linear_xent_backward_async(vkblas_dtype_t type, uint32_t 
     if (!dx && !dw) return VKBLAS_OK;
     if (vkb_engine_trace())
         fprintf(stderr, "[vkblas] linear_xent_backward type=%d M=%u V=%u K=%u\n", (int)type, M, V, K);
+    /* D of a piece of the vocabulary at a time, in type: from the pipelined
+     * kernel, or over the piece's logits in fp32 (fp32: in their place).
+     * Pieces are whole tiles, then the rest of the vocabulary: odd classes
+     * would cost both products of a whole piece their fast kernels. */
     const int f32 = type == VKBLAS_DT_F32;
     const size_t es = type_size(type);
-    /* a piece's logits in fp32 and its D in type (fp32: in the logits' place) */
-    const uint32_t n = piece_columns(M, V, JOIN_BYTES, sizeof(float)), ldz = (uint32_t)round_up(n, 8);
-    const uint32_t last = V % n;
+    vkb_op_args a;
+    const int fused = op_plan(type, M, V, K, x, ldx, w, ldw, 256, &a);
+    uint32_t n = piece_columns(M, V, fused ? PIECE_BYTES : JOIN_BYTES, fused ? es : sizeof(float));
+    if (n == V && V > 256 && V % 128) n = V / 128 * 128;
+    const uint32_t ldd = (uint32_t)round_up(n, 8);
+    piece_t pieces[3];           /* the kinds of pieces: n columns, then whole tiles, then the rest */
+    int kinds = 0;
+    const uint32_t tail = V % n;
+    pieces[kinds++] = (piece_t){0, n};
+    if (tail >= 128) pieces[kinds++] = (piece_t){V - tail, tail / 128 * 128};
+    if (tail % 128) pieces[kinds++] = (piece_t){V - tail % 128, tail % 128};
     /* dx adds up over the pieces in fp32: in dx itself or in the workspace */
-    const int several = n < V, acc = dx && several && !f32;
+    const int acc = dx && n < V && !f32;
     const vkblas_dtype_t xt = acc ? VKBLAS_DT_F32 : type;
     const uint32_t lda = acc ? (uint32_t)round_up(K, 4) : lddx;
-    for (int i = 0; i < 2; ++i) {
-        const uint32_t cols = i ? last : n;
-        if (!cols) continue;
-        need_gemm(&c, type, VKBLAS_DT_F32, VKBLAS_OP_N, VKBLAS_OP_T, M, cols, K, x, ldx, w, ldw, ldz);
-        if (dx) need_gemm(&c, type, xt, VKBLAS_OP_N, VKBLAS_OP_N, M, K, cols, NULL, ldz, w, ldw, lda);
-        if (dw) need_gemm(&c, type, dw_type, VKBLAS_OP_T, VKBLAS_OP_N, cols, K, M, NULL, ldz, x, ldx, lddw);
+    for (int i = 0; i < kinds; ++i) {
+        const uint32_t cols = pieces[i].cols;
+        if (!fused)
+            need_gemm(&c, type, VKBLAS_DT_F32, VKBLAS_OP_N, VKBLAS_OP_T, M, cols, K, x, ldx, w, ldw, ldd);
+        if (dx) need_gemm(&c, type, xt, VKBLAS_OP_N, VKBLAS_OP_N, M, K, cols, NULL, ldd, w, ldw, lda);
+        if (dw) need_gemm(&c, type, dw_type, VKBLAS_OP_T, VKBLAS_OP_N, cols, K, M, NULL, ldd, x, ldx, lddw);
     }
-    const size_t o_z = buf(&c, (uint64_t)M * ldz * sizeof(float));
-    const size_t o_d = f32 ? o_z : buf(&c, (uint64_t)M * ldz * es);
+    const size_t o_z = fused ? 0 : buf(&c, (uint64_t)M * ldd * sizeof(float));
+    const size_t o_d = f32 && !fused ? o_z : buf(&c, (uint64_t)M * ldd * es);
     const size_t o_a = acc ? buf(&c, (uint64_t)M * lda * sizeof(float)) : 0;
     const size_t o_s = buf(&c, 8 * sizeof(float));
     if (room(&c) != VKBLAS_OK) return c.st;
     float *z = at(&c, o_z), *scal = type == VKBLAS_DT_F16 ? (float*)at(&c, o_s) : NULL;
     void *d = at(&c, o_d), *xo = acc ? at(&c, o_a) : dx;
     int ok = !scal || step(&c, vkb_launch_xent_scale(M, dloss, beta, scal, stream), 0);
-    for (uint64_t v = 0; ok && v < V; v += n) {
-        const uint32_t cols = (uint32_t)(V - v < n ? V - v : n);
+    for (uint64_t v = 0; ok && v < V;) {
+        const uint32_t left = (uint32_t)(V - v), cols = left >= n ? n : left >= 128 ? left / 128 * 128 : left;
         const char* wv = (const char*)w + v * ldw * es;
-        ok = product(&c, type, VKBLAS_DT_F32, VKBLAS_OP_N, VKBLAS_OP_T, M, cols, K, host_scalars(1.0f, 0.0f), x, ldx, wv,
-                     ldw, z, ldz, 0) &&
-             step(&c, vkb_launch_xent_grad(type, M, cols, (uint32_t)v, V, z, ldz, target, ignore_index, lse, dloss,
-                                           scal, d, ldz, stream), 0);
-        scalars sw = {1.0f, beta, scal ? scal + 1 : NULL, scal ? scal + 2 : NULL};
-        scalars sx = {1.0f, v ? 1.0f : 0.0f, scal ? scal + 1 : NULL, scal ? scal + (v ? 3 : 4) : NULL};
+        if (fused) {
+            a.w = wv;
+            a.N = cols;
+            ok = step(&c, vkb_launch_xent_grad_op(&a, (uint32_t)v, V, target, ignore_index, lse, dloss, scal, d, ldd,
+                                                  stream), 0);
+        } else {
+            ok = product(&c, type, VKBLAS_DT_F32, VKBLAS_OP_N, VKBLAS_OP_T, M, cols, K, host_scalars(1.0f, 0.0f), x,
+                         ldx, wv, ldw, z, ldd, 0) &&
+                 step(&c, vkb_launch_xent_grad(type, M, cols, (uint32_t)v, V, z, ldd, target, ignore_index, lse, dloss,
+                                               scal, d, ldd, stream), 0);
+        }
+        const scalars sw = {1.0f, beta, scal ? scal + 1 : NULL, scal ? scal + 2 : NULL};
+        const scalars sx = {1.0f, v ? 1.0f : 0.0f, scal ? scal + 1 : NULL, scal ? scal + (v ? 3 : 4) : NULL};
         if (ok && dw)
-            ok = product(&c, type, dw_type, VKBLAS_OP_T, VKBLAS_OP_N, cols, K, M, sw, d, ldz, x, ldx,
+            ok = product(&c, type, dw_type, VKBLAS_OP_T, VKBLAS_OP_N, cols, K, M, sw, d, ldd, x, ldx,
                          (char*)dw + v * lddw * type_size(dw_type), lddw, 1);
         if (ok && dx)
-            ok = product(&c, type, xt, VKBLAS_OP_N, VKBLAS_OP_N, M, K, cols, sx, d, ldz, wv, ldw, xo, lda, !acc);
+            ok = product(&c, type, xt, VKBLAS_OP_N, VKBLAS_OP_N, M, K, cols, sx, d, ldd, wv, ldw, xo, lda, !acc);
+        v += cols;
     }
     if (ok && acc)
         step(&c, vkb_launch_convert(type, M, K, xo, lda, dx, lddx, stream), 1);
-    return op_end(&c, VKBLAS_KERNEL_JOINED);
+    return op_end(&c, fused ? VKBLAS_KERNEL_FUSED : VKBLAS_KERNEL_JOINED);
 }

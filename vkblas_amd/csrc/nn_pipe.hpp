@@ -1,0 +1,94 @@
+// nn_pipe.hpp — launchers of the operators that run inside the pipelined GEMM
+// kernel; nn_f32.hip, nn_f16.hip and nn_bf16.hip instantiate them by type.
+#pragma once
+#include "gemm_ops.hpp"
+#include "vkb_nn_launch.h"
+
+namespace vkb {
+
+template <typename T, typename OP, int WT>
+static int launch_op(typename OP::Params p, hipStream_t st) {
+    constexpr int BM = 2 * WT, BN = OP::GATED ? WT : 2 * WT;
+    p.tiles_m = (p.M + BM - 1) / BM;
+    p.tiles_n = (p.N + BN - 1) / BN;
+    const uint64_t grid = (uint64_t)p.tiles_m * p.tiles_n;
+    if (grid > 0xffffffffull / 256) return (int)hipErrorInvalidValue;
+    hipLaunchKernelGGL((gemm_pipe_kernel<T, T, true, true, WT, 2, OP>), dim3((uint32_t)grid), dim3(256), 0, st, p);
+    return (int)hipGetLastError();
+}
+
+template <typename T, typename P>
+static P op_params(const vkb_op_args* a) {
+    P p{};
+    p.A = a->x;
+    p.B = a->w;
+    p.lda = a->ldx;
+    p.ldb = a->ldw;
+    p.M = a->M;
+    p.N = a->N;
+    p.K = a->K;
+    p.batch = p.split = 1;
+    p.kps = a->K;
+    return p;
+}
+
+template <typename T>
+static int launch_glu(const vkb_op_args* a, int act_code, void* h, int64_t ldh, void* gu, int64_t ldgu,
+                      hipStream_t st) {
+    GluParams p = op_params<T, GluParams>(a);
+    p.h = h;
+    p.ldh = ldh;
+    p.gu = gu;
+    p.ldgu = ldgu;
+    int rc = (int)hipErrorInvalidValue;
+    with_act(act_code, [&](auto act) {
+        using OP = GluOp<T, decltype(act)::value>;
+        rc = a->tile == VKB_TILE_256 ? launch_op<T, OP, 128>(p, st) : launch_op<T, OP, 64>(p, st);
+    });
+    return rc;
+}
+
+template <typename T>
+static int launch_xent_stats(const vkb_op_args* a, const int64_t* target, float* parts, float* zt, hipStream_t st) {
+    XentParams p = op_params<T, XentParams>(a);
+    p.target = target;
+    p.parts = (float2*)parts;
+    p.zt = zt;
+    using OP = XentStatsOp<T>;
+    return a->tile == VKB_TILE_256 ? launch_op<T, OP, 128>(p, st) : launch_op<T, OP, 64>(p, st);
+}
+
+template <typename T>
+static int launch_xent_grad(const vkb_op_args* a, uint32_t v0, uint32_t V, const int64_t* target, int64_t ignore,
+                            const float* lse, const float* dloss, const float* scal, void* D, int64_t ldd,
+                            hipStream_t st) {
+    XentParams p = op_params<T, XentParams>(a);
+    p.target = target;
+    p.v0 = v0;
+    p.V = V;
+    p.ignore = ignore;
+    p.lse = lse;
+    p.dloss = dloss;
+    p.scal = scal;
+    p.C = D;
+    p.ldc = ldd;
+    using OP = XentGradOp<T>;
+    return a->tile == VKB_TILE_256 ? launch_op<T, OP, 128>(p, st) : launch_op<T, OP, 64>(p, st);
+}
+
+}  // namespace vkb
+
+#define VKB_NN_TYPE(NAME, T)                                                                                         \
+    extern "C" int vkb_launch_glu_##NAME(const vkb_op_args* a, int act, void* h, int64_t ldh, void* gu,              \
+                                         int64_t ldgu, void* st) {                                                   \
+        return vkb::launch_glu<T>(a, act, h, ldh, gu, ldgu, (hipStream_t)st);                                        \
+    }                                                                                                                \
+    extern "C" int vkb_launch_xent_stats_##NAME(const vkb_op_args* a, const int64_t* target, float* parts,           \
+                                                float* zt, void* st) {                                               \
+        return vkb::launch_xent_stats<T>(a, target, parts, zt, (hipStream_t)st);                                     \
+    }                                                                                                                \
+    extern "C" int vkb_launch_xent_grad_##NAME(const vkb_op_args* a, uint32_t v0, uint32_t V, const int64_t* target, \
+                                               int64_t ignore, const float* lse, const float* dloss,                 \
+                                               const float* scal, void* D, int64_t ldd, void* st) {                  \
+        return vkb::launch_xent_grad<T>(a, v0, V, target, ignore, lse, dloss, scal, D, ldd, (hipStream_t)st);        \
+    }

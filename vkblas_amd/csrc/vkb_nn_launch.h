@@ -57,6 +57,26 @@ int vkb_launch_xent_grad(int type, uint32_t M, uint32_t n, uint32_t v0, uint32_t
                          const int64_t* target, int64_t ignore, const float* lse, const float* dloss,
                          const float* scal, void* D, int64_t ldd, void* stream);
 
+/* Operators inside the pipelined GEMM kernel (nn_pipe.hpp): x M x K, w the
+ * weight (2 N x K gated projection, N x K of the logits' classes), both as
+ * vkb_op_plan accepts them.  tile: VKB_TILE_256 or VKB_TILE_128. */
+typedef struct vkb_op_args {
+    const void *x, *w;
+    int64_t ldx, ldw;
+    uint32_t M, N, K;
+    int type, tile;
+} vkb_op_args;
+int vkb_launch_glu(const vkb_op_args* a, int act, void* h, int64_t ldh, void* gu, int64_t ldgu, void* stream);
+/* parts: a pair for each row and each half of a tile's columns (128 or 64),
+ * vkb_xent_slices of them */
+uint32_t vkb_xent_slices(const vkb_op_args* a);
+int vkb_launch_xent_stats_op(const vkb_op_args* a, const int64_t* target, float* parts, float* zt, void* stream);
+/* D as vkb_launch_xent_grad; ldd a multiple of 8 and at least N rounded up to
+ * one (the columns between are written too) */
+int vkb_launch_xent_grad_op(const vkb_op_args* a, uint32_t v0, uint32_t V, const int64_t* target, int64_t ignore,
+                            const float* lse, const float* dloss, const float* scal, void* D, int64_t ldd,
+                            void* stream);
+
 #ifdef __cplusplus
 }
 #endif
