@@ -48,22 +48,26 @@ __device__ __forceinline__ void load_params(const W* w, int t, uint32_t N, float
 }
 
 // Mean and sum of squares about it over a row.  Each wave forms its own mean
-// and squares about that (no barrier), and the waves' join as
-//   mean = sum c_i mean_i / N,  M2 = sum M2_i + c_i (mean_i - mean)^2:
-// one barrier per row and no cancellation.  sh is the row parity's buffer.
+// and squares about that (no barrier), and the waves' join, over c_i columns
+// each, as
+//   mean = sum S_i / N,  M2 = sum M2_i + c_i (S_i / c_i - mean)^2:
+// one barrier per row and no cancellation (the mean comes from the sums: from
+// the rounded wave means it was 16 times less exact where it is near zero).
+// sh is the row parity's buffer.
 template <int WAVES>
-__device__ __forceinline__ void join_stats(float cnt, float sum, float& mean, float& m2, float (*sh)[3], float N) {
+__device__ __forceinline__ void join_stats(float cnt, float sum, float& mean, float& m2, float (*sh)[4], float N) {
     if constexpr (WAVES == 1) return;
     const int wave = threadIdx.x >> 6;
     if ((threadIdx.x & 63) == 0) {
         sh[wave][0] = cnt;
         sh[wave][1] = mean;
         sh[wave][2] = m2;
+        sh[wave][3] = sum;
     }
     __syncthreads();
     float tot = 0.0f;
 #pragma unroll
-    for (int i = 0; i < WAVES; ++i) tot += sh[i][0] * sh[i][1];
+    for (int i = 0; i < WAVES; ++i) tot += sh[i][3];
     mean = tot / N;
     m2 = 0.0f;
 #pragma unroll
@@ -79,7 +83,7 @@ __global__ __launch_bounds__((RowMap<T, WAVES, EPT>::THREADS)) void layer_norm_k
     float* mean_out, float* rstd_out) {
     using R = RowMap<T, WAVES, EPT>;
     constexpr int VEC = R::VEC, NV = R::NV;
-    __shared__ float sh[2][WAVES][3];
+    __shared__ float sh[2][WAVES][4];
     const int t = WAVES == 1 ? (threadIdx.x & 63) : threadIdx.x;
     const uint32_t sub = WAVES == 1 ? threadIdx.x >> 6 : 0;
     const uint32_t step = gridDim.x * R::RPB;
@@ -111,7 +115,8 @@ __global__ __launch_bounds__((RowMap<T, WAVES, EPT>::THREADS)) void layer_norm_k
             if (m + step < M && m + step > m) load_row(m + step);
 #pragma unroll
         for (int i = 0; i < EPT; ++i) sum += v[i];
-        float mean = cnt > 0.0f ? wave_sum(sum) / cnt : 0.0f;
+        sum = wave_sum(sum);
+        float mean = cnt > 0.0f ? sum / cnt : 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll

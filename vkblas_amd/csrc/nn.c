@@ -423,9 +423,9 @@ vkblas_status_t vkblas_linear_xent_backward_async(vkblas_dtype_t type, uint32_t 
     const size_t o_a = acc ? buf(&c, (uint64_t)M * lda * sizeof(float)) : 0;
     const size_t o_s = buf(&c, 8 * sizeof(float));
     if (room(&c) != VKBLAS_OK) return c.st;
-    float *z = at(&c, o_z), *scal = type == VKBLAS_DT_F16 ? (float*)at(&c, o_s) : NULL;
+    float *z = at(&c, o_z), *scal = f32 ? NULL : (float*)at(&c, o_s);
     void *d = at(&c, o_d), *xo = acc ? at(&c, o_a) : dx;
-    int ok = !scal || step(&c, vkb_launch_xent_scale(M, dloss, beta, scal, stream), 0);
+    int ok = !scal || step(&c, vkb_launch_xent_scale(type, M, dloss, beta, scal, stream), 0);
     for (uint64_t v = 0; ok && v < V;) {
         const uint32_t left = (uint32_t)(V - v), cols = left >= n ? n : left >= 128 ? left / 128 * 128 : left;
         const char* wv = (const char*)w + v * ldw * es;

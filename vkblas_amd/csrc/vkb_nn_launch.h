@@ -48,10 +48,10 @@ int vkb_launch_xent_stats(uint32_t M, uint32_t n, uint32_t v0, const float* z, i
                           float* parts, float* zt, void* stream);
 int vkb_launch_xent_finish(uint32_t M, uint32_t V, uint32_t S, const float* parts, const float* zt,
                            const int64_t* target, int64_t ignore, float* loss, float* lse, void* stream);
-/* scal[0] = the power of two s that brings max |dloss| into [2^13, 2^14),
- * scal[1] = 1 / s, scal[2] = beta, scal[3] = 1, scal[4] = 0 (device scalars
- * of products). */
-int vkb_launch_xent_scale(uint32_t M, const float* dloss, float beta, float* scal, void* stream);
+/* scal[0] = s = 1 / max |dloss| (fp16: 2^13 times that; 1 where the largest is
+ * 0, infinite or outside 1e-30 .. 1e30), scal[1] = 1 / s, scal[2] = beta,
+ * scal[3] = 1, scal[4] = 0 (device scalars of products). */
+int vkb_launch_xent_scale(int type, uint32_t M, const float* dloss, float beta, float* scal, void* stream);
 /* D = scal[0] * dloss * (exp(z - lse) - [v == target]), scal NULL = 1. */
 int vkb_launch_xent_grad(int type, uint32_t M, uint32_t n, uint32_t v0, uint32_t V, const float* z, int64_t ldz,
                          const int64_t* target, int64_t ignore, const float* lse, const float* dloss,

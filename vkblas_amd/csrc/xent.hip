@@ -105,7 +105,8 @@ __global__ __launch_bounds__(THREADS) void xent_finish_kernel(uint32_t M, uint32
     }
 }
 
-__global__ __launch_bounds__(1024) void xent_scale_kernel(uint32_t M, const float* dloss, float beta, float* scal) {
+__global__ __launch_bounds__(1024) void xent_scale_kernel(uint32_t M, const float* dloss, bool fp16, float beta,
+                                                            float* scal) {
     __shared__ float sh[16];
     float top = 0.0f;
     for (uint32_t m = threadIdx.x; m < M; m += 1024) top = fmaxf(top, fabsf(dloss[m]));
@@ -114,13 +115,13 @@ __global__ __launch_bounds__(1024) void xent_scale_kernel(uint32_t M, const floa
     __syncthreads();
     if (threadIdx.x) return;
     for (int i = 1; i < 16; ++i) top = fmaxf(top, sh[i]);
-    int e = 0;
-    if (top > 0.0f && !__builtin_isinf(top)) {
-        e = 13 - ilogbf(top);
-        e = e > 100 ? 100 : e < -100 ? -100 : e;
-    }
-    scal[0] = ldexpf(1.0f, e);
-    scal[1] = ldexpf(1.0f, -e);
+    // by the largest itself, not a power of two near it: equal loss gradients
+    // (a mean's) then round the target's p - 1 near -1 almost exactly, where
+    // any other factor puts one and the same error on every row
+    const bool fine = top > 1e-30f && top < 1e30f;
+    const float to = fp16 ? 8192.0f : 1.0f;
+    scal[0] = fine ? to / top : 1.0f;
+    scal[1] = fine ? top / to : 1.0f;
     scal[2] = beta;
     scal[3] = 1.0f;
     scal[4] = 0.0f;
@@ -174,8 +175,10 @@ extern "C" int vkb_launch_xent_finish(uint32_t M, uint32_t V, uint32_t S, const 
     return (int)hipGetLastError();
 }
 
-extern "C" int vkb_launch_xent_scale(uint32_t M, const float* dloss, float beta, float* scal, void* stream) {
-    hipLaunchKernelGGL(xent_scale_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, M, dloss, beta, scal);
+extern "C" int vkb_launch_xent_scale(int type, uint32_t M, const float* dloss, float beta, float* scal,
+                                     void* stream) {
+    hipLaunchKernelGGL(xent_scale_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, M, dloss, type == VKB_T_F16,
+                       beta, scal);
     return (int)hipGetLastError();
 }
 
