@@ -10,7 +10,9 @@ and ``__graft_entry__``: it loads the built library with ctypes and mirrors the
 engine entry points (``vkblas_gemm_f32`` / ``vkblas_gemm_f16`` of the
 reference's ``src/vkblas.h:27-77``) with the same argument meaning and status
 codes.  There is no fallback: if the library is missing, loading raises.
-The asynchronous GEMMs go through ``_call`` (csrc/pycall.c), which converts
+The asynchronous GEMMs and the operators of ``include/vkblas_nn.h`` (layer norm,
+gated projection, linear cross entropy, with their gradients; ``torch_nn`` wraps
+them for autograd) go through ``_call`` (csrc/pycall.c), which converts
 their arguments natively; arguments it does not know, and every call of an
 interpreter it is not built for, go through ctypes.
 """
@@ -73,18 +75,21 @@ _u32, _i64, _f, _vp, _int = ctypes.c_uint32, ctypes.c_int64, ctypes.c_float, cty
 _ENGINE_ARGS = [_int, _int, _u32, _u32, _u32, _f, _vp, _u32, _vp, _u32, _f, _vp, _u32, _u32, _i64, _i64, _i64]
 
 
-# include/vkblas_nn.h
+# include/vkblas_nn.h: the arguments of vkblas_<name>_async
 _NN_ARGS = {
-    "vkblas_layer_norm_async": [_int, _int, _u32, _u32, _vp, _u32, _vp, _vp, _f, _vp, _u32, _vp, _vp, _vp],
-    "vkblas_layer_norm_backward_async": [_int, _int, _u32, _u32, _vp, _u32, _vp, _u32, _vp, _vp, _vp, _vp, _u32, _vp,
+    "layer_norm": [_int, _int, _u32, _u32, _vp, _u32, _vp, _vp, _f, _vp, _u32, _vp, _vp, _vp],
+    "layer_norm_backward": [_int, _int, _u32, _u32, _vp, _u32, _vp, _u32, _vp, _vp, _vp, _vp, _u32, _vp,
                                          _vp, _int, _f, _vp],
-    "vkblas_glu_async": [_int, _int, _u32, _u32, _u32, _vp, _u32, _vp, _u32, _vp, _u32, _vp, _u32, _vp],
-    "vkblas_glu_backward_async": [_int, _int, _u32, _u32, _u32, _vp, _u32, _vp, _u32, _vp, _u32, _vp, _u32, _vp, _u32,
+    "glu": [_int, _int, _u32, _u32, _u32, _vp, _u32, _vp, _u32, _vp, _u32, _vp, _u32, _vp],
+    "glu_backward": [_int, _int, _u32, _u32, _u32, _vp, _u32, _vp, _u32, _vp, _u32, _vp, _u32, _vp, _u32,
                                   _vp, _u32, _vp, _u32, _int, _f, _vp],
-    "vkblas_linear_xent_async": [_int, _u32, _u32, _u32, _vp, _u32, _vp, _u32, _vp, _i64, _vp, _vp, _vp],
-    "vkblas_linear_xent_backward_async": [_int, _u32, _u32, _u32, _vp, _u32, _vp, _u32, _vp, _i64, _vp, _vp, _vp, _u32,
+    "linear_xent": [_int, _u32, _u32, _u32, _vp, _u32, _vp, _u32, _vp, _i64, _vp, _vp, _vp],
+    "linear_xent_backward": [_int, _u32, _u32, _u32, _vp, _u32, _vp, _u32, _vp, _i64, _vp, _vp, _vp, _u32,
                                           _vp, _u32, _int, _f, _vp],
 }
+
+
+_nn_calls = {}      # by name: the native call, the function's address, the function
 
 
 def build(jobs: int = 8) -> None:
@@ -127,16 +132,17 @@ def load():
     L.vkblas_gemm_noalloc_async.argtypes = L.vkblas_gemm_async.argtypes
     L.vkblas_gemm_noalloc_async.restype = _int
     L.vkblas_noalloc_scratch_bytes.restype = ctypes.c_size_t
+    try:
+        from . import _call
+    except ImportError:     # not built, or for another interpreter
+        _call = None
+    else:
+        _native, _ex_addr = _call.gemm_ex, ctypes.cast(L.vkblas_gemm_ex_async, ctypes.c_void_p).value
     for name, args in _NN_ARGS.items():
-        fn = getattr(L, name)
+        fn = getattr(L, f"vkblas_{name}_async")
         fn.argtypes = args
         fn.restype = _int
-    try:
-        from ._call import gemm_ex
-    except ImportError:     # not built, or for another interpreter
-        pass
-    else:
-        _native, _ex_addr = gemm_ex, ctypes.cast(L.vkblas_gemm_ex_async, ctypes.c_void_p).value
+        _nn_calls[name] = (getattr(_call, name, _ctypes_call), ctypes.cast(fn, ctypes.c_void_p).value, fn)
     _lib = L
     return L
 
@@ -253,9 +259,14 @@ def gemm_batched_async(ab_type, c_type, op_a, op_b, M, N, K, alpha, A, lda, B, l
 
 def _nn(name, check, *args) -> int:
     """A call of vkblas_nn.h; its status (raises if check)."""
-    st = getattr(_lib or load(), name)(*args)
+    if not _nn_calls:
+        load()
+    native, addr, fn = _nn_calls[name]
+    st = native(addr, *args)
+    if st is None:
+        st = fn(*args)
     if check and st != OK:
-        raise VkblasError(st, name)
+        raise VkblasError(st, f"vkblas_{name}_async")
     return st
 
 
@@ -263,28 +274,28 @@ def layer_norm_async(dtype, w_dtype, M, N, x, ldx, w, b, eps, y, ldy, mean=None,
                      check=True) -> int:
     """vkblas_layer_norm_async: y = (x - mean) * rstd * w + b over M rows of N;
     mean and rstd (M floats each) kept where given."""
-    return _nn("vkblas_layer_norm_async", check, dtype, w_dtype, M, N, x, ldx, w, b, eps, y, ldy, mean, rstd, stream)
+    return _nn("layer_norm", check, dtype, w_dtype, M, N, x, ldx, w, b, eps, y, ldy, mean, rstd, stream)
 
 
 def layer_norm_backward_async(dtype, w_dtype, M, N, dy, lddy, x, ldx, w, mean, rstd, dx, lddx, dw, db, g_dtype,
                               beta=0.0, stream=None, check=True) -> int:
     """vkblas_layer_norm_backward_async: dx, and dw and db (beta times what
     they held, plus the sums over the rows); each may be None."""
-    return _nn("vkblas_layer_norm_backward_async", check, dtype, w_dtype, M, N, dy, lddy, x, ldx, w, mean, rstd, dx,
+    return _nn("layer_norm_backward", check, dtype, w_dtype, M, N, dy, lddy, x, ldx, w, mean, rstd, dx,
                lddx, dw, db, g_dtype, beta, stream)
 
 
 def glu_async(dtype, act, M, N, K, x, ldx, w, ldw, h, ldh, gu=None, ldgu=0, stream=None, check=True) -> int:
     """vkblas_glu_async: h = act(G) * U with [G | U] = x w^T (w is 2N x K, the
     gate's rows first); gu (M x 2N) receives [G | U] where given."""
-    return _nn("vkblas_glu_async", check, dtype, act, M, N, K, x, ldx, w, ldw, h, ldh, gu, ldgu, stream)
+    return _nn("glu", check, dtype, act, M, N, K, x, ldx, w, ldw, h, ldh, gu, ldgu, stream)
 
 
 def glu_backward_async(dtype, act, M, N, K, dh, lddh, gu, ldgu, x, ldx, w, ldw, dgu, lddgu, dx, lddx, dw, lddw,
                        dw_dtype, beta=0.0, stream=None, check=True) -> int:
     """vkblas_glu_backward_async: dgu = [dG | dU], dx = dgu w and dw = beta dw
     + dgu^T x; each may be None."""
-    return _nn("vkblas_glu_backward_async", check, dtype, act, M, N, K, dh, lddh, gu, ldgu, x, ldx, w, ldw, dgu, lddgu,
+    return _nn("glu_backward", check, dtype, act, M, N, K, dh, lddh, gu, ldgu, x, ldx, w, ldw, dgu, lddgu,
                dx, lddx, dw, lddw, dw_dtype, beta, stream)
 
 
@@ -292,7 +303,7 @@ def linear_xent_async(dtype, M, V, K, x, ldx, w, ldw, target, ignore_index, loss
                       check=True) -> int:
     """vkblas_linear_xent_async: each row's cross entropy (loss) and
     log-sum-exp (lse) of the logits x w^T, which are not kept."""
-    return _nn("vkblas_linear_xent_async", check, dtype, M, V, K, x, ldx, w, ldw, target, ignore_index, loss, lse,
+    return _nn("linear_xent", check, dtype, M, V, K, x, ldx, w, ldw, target, ignore_index, loss, lse,
                stream)
 
 
@@ -300,7 +311,7 @@ def linear_xent_backward_async(dtype, M, V, K, x, ldx, w, ldw, target, ignore_in
                                dw_dtype, beta=0.0, stream=None, check=True) -> int:
     """vkblas_linear_xent_backward_async: dx and dw = beta dw + D^T x from the
     rows' loss gradients; each may be None."""
-    return _nn("vkblas_linear_xent_backward_async", check, dtype, M, V, K, x, ldx, w, ldw, target, ignore_index, lse,
+    return _nn("linear_xent_backward", check, dtype, M, V, K, x, ldx, w, ldw, target, ignore_index, lse,
                dloss, dx, lddx, dw, lddw, dw_dtype, beta, stream)
 
 

@@ -1,8 +1,8 @@
 /*
- * pycall.c — the Python binding's GEMM call without ctypes (module
- * vkblas_amd._call).
+ * pycall.c — the Python binding's calls without ctypes (module
+ * vkblas_amd._call): vkblas_gemm_ex_async and the functions of vkblas_nn.h.
  *
- * A small GEMM is bound by its launch on the host, and ctypes' conversion of
+ * A small call is bound by its launch on the host, and ctypes' conversion of
  * 25 arguments was the largest part of that: 3.1 us for vkblas_gemm_async and
  * 3.7 for vkblas_gemm_ex_async with its structure, of about 8 a call.  Here
  * the arguments are read from the interpreter's vector directly.
@@ -15,7 +15,7 @@
  */
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
-#include "vkblas_ext.h"
+#include "vkblas_nn.h"
 
 typedef vkblas_status_t (*gemm_ex_fn)(vkblas_dtype_t, vkblas_dtype_t, vkblas_op_t, vkblas_op_t, uint32_t, uint32_t,
                                       uint32_t, float, const void*, uint32_t, const void*, uint32_t, float, void*,
@@ -78,9 +78,76 @@ static PyObject* gemm_ex(PyObject* self, PyObject* const* a, Py_ssize_t n) {
     return PyLong_FromLong(st);
 }
 
-static PyMethodDef methods[] = {{"gemm_ex", (PyCFunction)(void (*)(void))gemm_ex, METH_FASTCALL,
+/* v[k] and f[] (the floats in order) from n arguments of these kinds; 1, or
+ * 0 with *result set: an exception (NULL) or None */
+static int get_args(const char* name, const char* kind, PyObject* const* a, Py_ssize_t n, unsigned long long* v,
+                    float* f, PyObject** result) {
+    *result = NULL;
+    const Py_ssize_t want = (Py_ssize_t)strlen(kind);
+    if (n != want) {
+        PyErr_Format(PyExc_TypeError, "%s takes %zd arguments (%zd given)", name, want, n);
+        return 0;
+    }
+    for (Py_ssize_t k = 0; k < n; ++k) {
+        const int ok = kind[k] == 'i' ? get_int(a[k], &v[k]) : kind[k] == 'p' ? get_ptr(a[k], &v[k]) : get_float(a[k], f);
+        if (!ok) {
+            PyErr_Clear();
+            Py_INCREF(Py_None);
+            *result = Py_None;
+            return 0;
+        }
+        if (kind[k] == 'f') ++f;
+    }
+    if (!v[0]) {
+        PyErr_Format(PyExc_ValueError, "no function address");
+        return 0;
+    }
+    return 1;
+}
+
+/* name(address of vkblas_<name>_async, its arguments): KIND starts with the
+ * address; CALL is the call's argument list in terms of v[] and f[] */
+#define P(k) ((void*)(uintptr_t)v[k])
+#define U(k) ((uint32_t)v[k])
+#define I(k) ((int)v[k])
+#define NN_CALL(NAME, KIND, CALL)                                                                  \
+    static PyObject* NAME(PyObject* self, PyObject* const* a, Py_ssize_t n) {                      \
+        (void)self;                                                                                \
+        unsigned long long v[sizeof(KIND)];                                                        \
+        float f[2];                                                                                \
+        PyObject* result;                                                                          \
+        if (!get_args(#NAME, KIND, a, n, v, f, &result)) return result;                            \
+        int st;                                                                                    \
+        Py_BEGIN_ALLOW_THREADS                                                                     \
+        st = (int)((__typeof__(&vkblas_##NAME##_async))(uintptr_t)v[0]) CALL;                      \
+        Py_END_ALLOW_THREADS                                                                       \
+        return PyLong_FromLong(st);                                                                \
+    }
+
+NN_CALL(layer_norm, "piiiipippfpippp",
+        (I(1), I(2), U(3), U(4), P(5), U(6), P(7), P(8), f[0], P(10), U(11), P(12), P(13), P(14)))
+NN_CALL(layer_norm_backward, "piiiipipippppippifp",
+        (I(1), I(2), U(3), U(4), P(5), U(6), P(7), U(8), P(9), P(10), P(11), P(12), U(13), P(14), P(15), I(16), f[0],
+         P(18)))
+NN_CALL(glu, "piiiiipipipipip",
+        (I(1), I(2), U(3), U(4), U(5), P(6), U(7), P(8), U(9), P(10), U(11), P(12), U(13), P(14)))
+NN_CALL(glu_backward, "piiiiipipipipipipipiifp",
+        (I(1), I(2), U(3), U(4), U(5), P(6), U(7), P(8), U(9), P(10), U(11), P(12), U(13), P(14), U(15), P(16), U(17),
+         P(18), U(19), I(20), f[0], P(22)))
+NN_CALL(linear_xent, "piiiipipipippp",
+        (I(1), U(2), U(3), U(4), P(5), U(6), P(7), U(8), P(9), (int64_t)v[10], P(11), P(12), P(13)))
+NN_CALL(linear_xent_backward, "piiiipipipipppipiifp",
+        (I(1), U(2), U(3), U(4), P(5), U(6), P(7), U(8), P(9), (int64_t)v[10], P(11), P(12), P(13), U(14), P(15),
+         U(16), I(17), f[0], P(19)))
+
+static PyMethodDef methods[] = {
+#define NN_METHOD(NAME) {#NAME, (PyCFunction)(void (*)(void))NAME, METH_FASTCALL, \
+                         "vkblas_" #NAME "_async by address; None if an argument is not a plain int, float or None"}
+                                NN_METHOD(layer_norm), NN_METHOD(layer_norm_backward), NN_METHOD(glu),
+                                NN_METHOD(glu_backward), NN_METHOD(linear_xent), NN_METHOD(linear_xent_backward),
+                                {"gemm_ex", (PyCFunction)(void (*)(void))gemm_ex, METH_FASTCALL,
                                  "vkblas_gemm_ex_async by address; None if an argument is not a plain int, float or None"},
                                 {NULL, NULL, 0, NULL}};
-static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_call", "GEMM calls of the binding", -1, methods,
+static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_call", "calls of the binding", -1, methods,
                                     NULL, NULL, NULL, NULL};
 PyMODINIT_FUNC PyInit__call(void) { return PyModule_Create(&module); }
