@@ -108,7 +108,8 @@ struct XentParams : KParams {
     // the targets' logits
     float2* parts;
     float* zt;
-    // gradient
+    // gradient: rows and columns of D stored, zero past M and N
+    uint32_t Ms, Ns;
     int64_t V, ignore;
     const float *lse, *dloss, *scal;
 };
@@ -220,10 +221,21 @@ struct XentGradOp {
                             if (in && tc == G::col(lane, j, q) + e) acc[i][j][4 * q + e] -= k;
             }
         }
+        const int left = (int)min((int64_t)WT, p.N - col0);
+        if (left < WT) {
+#pragma unroll
+            for (int j = 0; j < G::NF; ++j)
+#pragma unroll
+                for (int r = 0; r < 4 * G::NQ; ++r)
+                    if (G::col(lane, j, r / 4) + r % 4 >= left) {
+#pragma unroll
+                        for (int i = 0; i < G::NF; ++i) acc[i][j][r] = 0.0f;
+                    }
+        }
         store_block<T, WT, WT, SH, LDS>([&](int i, int j, int q, float* x) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[e] = acc[i][j][4 * q + e];
-        }, (T*)p.C, p.ldc, row0, col0, p.M, (p.N + 7) / 8 * 8, lds, wave, lane);
+        }, (T*)p.C, p.ldc, row0, col0, p.Ms, p.Ns, lds, wave, lane);
     }
 };
 

@@ -42,14 +42,21 @@ __global__ __launch_bounds__(THREADS) void glu_join_kernel(uint32_t M, uint32_t 
     }
 }
 
-// dgu may be gu: a thread reads its elements before it writes them
+// dgu may be gu: a thread reads its elements before it writes them.  dG and dU
+// are Np columns each (Np >= N) on Mp rows (Mp >= M), zero past N and M.
 template <typename T, int ACT>
 __global__ __launch_bounds__(THREADS) void glu_join_backward_kernel(uint32_t M, uint32_t N, const T* dh, int64_t lddh,
-                                                                    const T* gu, int64_t ldgu, T* dgu, int64_t lddgu) {
+                                                                    const T* gu, int64_t ldgu, T* dgu, int64_t lddgu,
+                                                                    uint32_t Mp, uint32_t Np) {
     constexpr int VEC = Elem<T>::VEC;
     const int64_t n = ((int64_t)blockIdx.x * THREADS + threadIdx.x) * VEC;
-    if (n >= N) return;
-    for (uint32_t m = blockIdx.y; m < M; m += gridDim.y) {
+    if (n >= Np) return;
+    for (uint32_t m = blockIdx.y; m < Mp; m += gridDim.y) {
+        if (m >= M || n >= N) {
+            st_chunk(dgu + (int64_t)m * lddgu, n, Np, u32x4{0u, 0u, 0u, 0u});
+            st_chunk(dgu + (int64_t)m * lddgu + Np, n, Np, u32x4{0u, 0u, 0u, 0u});
+            continue;
+        }
         float g[VEC], u[VEC], d[VEC];
         unpack<T>(ld_chunk(gu + (int64_t)m * ldgu, n, N), g);
         unpack<T>(ld_chunk(gu + (int64_t)m * ldgu + N, n, N), u);
@@ -61,31 +68,9 @@ __global__ __launch_bounds__(THREADS) void glu_join_backward_kernel(uint32_t M, 
             g[i] = d[i] * u[i] * da;
             u[i] = d[i] * a;
         }
-        st_chunk(dgu + (int64_t)m * lddgu, n, N, pack<T>(g));
-        st_chunk(dgu + (int64_t)m * lddgu + N, n, N, pack<T>(u));
-    }
-}
-
-template <typename T>
-__global__ __launch_bounds__(THREADS) void scale_kernel(uint32_t M, uint32_t N, T* C, int64_t ldc, float beta) {
-    for (uint32_t m = blockIdx.y; m < M; m += gridDim.y)
-        for (int64_t n = (int64_t)blockIdx.x * THREADS + threadIdx.x; n < N; n += (int64_t)gridDim.x * THREADS) {
-            T* c = C + (int64_t)m * ldc + n;
-            *c = beta == 0.0f ? (T)0.0f : (T)(beta * (float)*c);
-        }
-}
-
-template <typename T>
-__global__ __launch_bounds__(THREADS) void convert_kernel(uint32_t M, uint32_t N, const float* A, int64_t lda, T* C,
-                                                          int64_t ldc) {
-    constexpr int VEC = Elem<T>::VEC;
-    const int64_t n = ((int64_t)blockIdx.x * THREADS + threadIdx.x) * VEC;
-    if (n >= N) return;
-    for (uint32_t m = blockIdx.y; m < M; m += gridDim.y) {
-        float x[VEC];
-#pragma unroll
-        for (int q = 0; q < VEC; q += 4) unpack<float>(ld_chunk(A + (int64_t)m * lda, n + q, N), x + q);
-        st_chunk(C + (int64_t)m * ldc, n, N, pack<T>(x));
+        // (columns past N read as zeros, and d = 0 gives zeros)
+        st_chunk(dgu + (int64_t)m * lddgu, n, Np, pack<T>(g));
+        st_chunk(dgu + (int64_t)m * lddgu + Np, n, Np, pack<T>(u));
     }
 }
 
@@ -108,32 +93,14 @@ extern "C" int vkb_launch_glu_join(int type, int act_code, uint32_t M, uint32_t 
 
 extern "C" int vkb_launch_glu_join_backward(int type, int act_code, uint32_t M, uint32_t N, const void* dh,
                                             int64_t lddh, const void* gu, int64_t ldgu, void* dgu, int64_t lddgu,
-                                            void* stream) {
+                                            uint32_t Mp, uint32_t Np, void* stream) {
     const bool ok = with_type(type, [&](auto t) {
         using T = decltype(t);
         with_act(act_code, [&](auto a) {
-            hipLaunchKernelGGL((glu_join_backward_kernel<T, decltype(a)::value>), rows_grid<T>(M, N), dim3(THREADS),
-                               0, (hipStream_t)stream, M, N, (const T*)dh, lddh, (const T*)gu, ldgu, (T*)dgu, lddgu);
+            hipLaunchKernelGGL((glu_join_backward_kernel<T, decltype(a)::value>), rows_grid<T>(Mp, Np), dim3(THREADS),
+                               0, (hipStream_t)stream, M, N, (const T*)dh, lddh, (const T*)gu, ldgu, (T*)dgu, lddgu,
+                               Mp, Np);
         });
-    });
-    return ok ? (int)hipGetLastError() : (int)hipErrorInvalidValue;
-}
-
-extern "C" int vkb_launch_scale(int type, uint32_t M, uint32_t N, void* C, int64_t ldc, float beta, void* stream) {
-    const bool ok = with_type(type, [&](auto t) {
-        using T = decltype(t);
-        hipLaunchKernelGGL((scale_kernel<T>), rows_grid<T>(M, N), dim3(THREADS), 0, (hipStream_t)stream, M, N, (T*)C,
-                           ldc, beta);
-    });
-    return ok ? (int)hipGetLastError() : (int)hipErrorInvalidValue;
-}
-
-extern "C" int vkb_launch_convert(int type, uint32_t M, uint32_t N, const float* A, int64_t lda, void* C, int64_t ldc,
-                                  void* stream) {
-    const bool ok = with_type(type, [&](auto t) {
-        using T = decltype(t);
-        hipLaunchKernelGGL((convert_kernel<T>), rows_grid<T>(M, N), dim3(THREADS), 0, (hipStream_t)stream, M, N, A,
-                           lda, (T*)C, ldc);
     });
     return ok ? (int)hipGetLastError() : (int)hipErrorInvalidValue;
 }

@@ -129,8 +129,8 @@ extern int vkb_launch_glu_bf16(const vkb_op_args*, int, void*, int64_t, void*, i
 extern int vkb_launch_xent_stats_f32(const vkb_op_args*, const int64_t*, float*, float*, void*);
 extern int vkb_launch_xent_stats_f16(const vkb_op_args*, const int64_t*, float*, float*, void*);
 extern int vkb_launch_xent_stats_bf16(const vkb_op_args*, const int64_t*, float*, float*, void*);
-typedef int xent_grad_fn(const vkb_op_args*, uint32_t, uint32_t, const int64_t*, int64_t, const float*, const float*,
-                         const float*, void*, int64_t, void*);
+typedef int xent_grad_fn(const vkb_op_args*, uint32_t, uint32_t, uint32_t, uint32_t, const int64_t*, int64_t,
+                         const float*, const float*, const float*, void*, int64_t, void*);
 extern xent_grad_fn vkb_launch_xent_grad_f32, vkb_launch_xent_grad_f16, vkb_launch_xent_grad_bf16;
 
 int vkb_launch_glu(const vkb_op_args* a, int act, void* h, int64_t ldh, void* gu, int64_t ldgu, void* stream) {
@@ -143,12 +143,12 @@ int vkb_launch_xent_stats_op(const vkb_op_args* a, const int64_t* target, float*
                                                                                     : vkb_launch_xent_stats_f32)(
         a, target, parts, zt, stream);
 }
-int vkb_launch_xent_grad_op(const vkb_op_args* a, uint32_t v0, uint32_t V, const int64_t* target, int64_t ignore,
-                            const float* lse, const float* dloss, const float* scal, void* D, int64_t ldd,
-                            void* stream) {
+int vkb_launch_xent_grad_op(const vkb_op_args* a, uint32_t Ms, uint32_t Ns, uint32_t v0, uint32_t V,
+                            const int64_t* target, int64_t ignore, const float* lse, const float* dloss,
+                            const float* scal, void* D, int64_t ldd, void* stream) {
     return (a->type == VKB_T_F16 ? vkb_launch_xent_grad_f16 : a->type == VKB_T_BF16 ? vkb_launch_xent_grad_bf16
                                                                                    : vkb_launch_xent_grad_f32)(
-        a, v0, V, target, ignore, lse, dloss, scal, D, ldd, stream);
+        a, Ms, Ns, v0, V, target, ignore, lse, dloss, scal, D, ldd, stream);
 }
 uint32_t vkb_xent_slices(const vkb_op_args* a) {
     const uint64_t tile = vkb_tile_bn(a->tile);
@@ -182,6 +182,73 @@ static int op_plan(vkblas_dtype_t type, uint32_t M, uint32_t N, uint32_t K, cons
     a->type = type;
     a->tile = (type == VKBLAS_DT_F32 ? 8 * t >= 7 * 256 * ((t + 255) / 256) : t > 128) ? VKB_TILE_256 : VKB_TILE_128;
     return 1;
+}
+
+/* ----------------------------------------------- operands and their copies */
+
+/* A program's matrix (S of M x N below each other), or a copy of it in the
+ * workspace, padded with zeros to Mp x Np each: what the fast kernels do not
+ * take (rows off 16-byte units, sizes off whole steps) costs them 3 to 8 times
+ * their time, and a copy one pass over it. */
+typedef struct {
+    const void* p;
+    uint32_t ld, S, M, N, Mp, Np;
+    int copy;
+    size_t off;
+} operand;
+
+static uint32_t vec_of(vkblas_dtype_t t) { return t == VKBLAS_DT_F32 ? 4 : 8; }
+static int off_units(vkblas_dtype_t t, const void* p, uint32_t ld) { return !aligned16(p) || ld % vec_of(t); }
+
+static operand as_is(const void* p, uint32_t ld, uint32_t S, uint32_t M, uint32_t N) {
+    operand o = {p, ld, S, M, N, M, N, 0, 0};
+    return o;
+}
+/* ... copied, to Mp x Np; Np in whole 16-byte units */
+static void pad_to(operand* o, uint32_t Mp, uint32_t Np) {
+    o->copy = 1;
+    o->Mp = Mp;
+    o->Np = Np;
+    o->ld = Np;
+    o->p = NULL;                 /* in the workspace: aligned */
+}
+static void place(op_call* c, operand* o, vkblas_dtype_t t) {
+    if (o->copy) o->off = buf(c, (uint64_t)o->S * o->Mp * o->Np * type_size(t));
+}
+/* after room(): the copy, and from where */
+static int bring(op_call* c, operand* o, vkblas_dtype_t t, const void* src, uint32_t lds) {
+    if (!o->copy) return 1;
+    void* d = at(c, o->off);
+    o->p = d;
+    return step(c, vkb_launch_pad(t, o->S, o->M, o->N, src, lds, d, o->Mp, o->Np, c->stream), 0);
+}
+
+/* K as the pipelined kernel takes it */
+static uint32_t whole_k(uint32_t K) { return K <= 128 ? 128 : (uint32_t)round_up(K, 64); }
+/* x (M x K) and w (S of N x K) for x w^T inside the pipelined kernel: copied
+ * where they have to be and the product is worth it.  Below 1 GFLOP the
+ * copies' launches cost more than they save. */
+static int fusable(vkblas_dtype_t type, uint32_t M, uint32_t N, uint32_t K, operand* x, operand* w, uint32_t cols,
+                   vkb_op_args* a) {
+    const uint32_t Kp = whole_k(K);
+    const int rx = Kp != K || off_units(type, x->p, x->ld), rw = Kp != K || off_units(type, w->p, w->ld);
+    operand px = *x, pw = *w;
+    if (rx || rw) {
+        if (2.0 * M * w->S * w->M * K < 1e9) return 0;
+        if (rx) pad_to(&px, x->Mp, Kp);
+        if (rw) pad_to(&pw, w->Mp, Kp);
+    }
+    if (!op_plan(type, M, N, Kp, px.p, px.ld, pw.p, pw.ld, cols, a)) return 0;
+    *x = px;
+    *w = pw;
+    return 1;
+}
+/* the arguments with the operands where they are now */
+static void bound(vkb_op_args* a, const operand* x, const operand* w) {
+    a->x = x->p;
+    a->w = w->p;
+    a->ldx = x->ld;
+    a->ldw = w->ld;
 }
 
 /* A gradient over no rows: C = beta * C. */
@@ -253,9 +320,15 @@ vkblas_status_t vkblas_glu_async(vkblas_dtype_t type, vkblas_act_t act, uint32_t
     op_begin(&c, "glu", stream);
     if (vkb_engine_trace()) fprintf(stderr, "[vkblas] glu type=%d act=%d M=%u N=%u K=%u\n", (int)type, (int)act, M, N, K);
     vkb_op_args a;
-    if (op_plan(type, M, N, K, x, ldx, w, ldw, 128, &a)) {
+    operand ox = as_is(x, ldx, 1, M, K), ow = as_is(w, ldw, 2, N, K);
+    if (fusable(type, M, N, K, &ox, &ow, 128, &a)) {
+        place(&c, &ox, type);
+        place(&c, &ow, type);
         if (room(&c) != VKBLAS_OK) return c.st;
-        step(&c, vkb_launch_glu(&a, act, h, ldh, gu, ldgu, stream), 1);
+        if (bring(&c, &ox, type, x, ldx) && bring(&c, &ow, type, w, ldw)) {
+            bound(&a, &ox, &ow);
+            step(&c, vkb_launch_glu(&a, act, h, ldh, gu, ldgu, stream), 1);
+        }
         return op_end(&c, VKBLAS_KERNEL_FUSED);
     }
     /* both projections in fp32, some rows at a time, then the join; an fp32
@@ -302,24 +375,51 @@ vkblas_status_t vkblas_glu_backward_async(vkblas_dtype_t type, vkblas_act_t act,
     if (!dgu && !dx && !dw) return VKBLAS_OK;
     if (vkb_engine_trace())
         fprintf(stderr, "[vkblas] glu_backward type=%d act=%d M=%u N=%u K=%u\n", (int)type, (int)act, M, N, K);
-    const uint32_t ldd = dgu ? lddgu : (uint32_t)round_up(2 * N, 8);
-    if (dx) need_gemm(&c, type, type, VKBLAS_OP_N, VKBLAS_OP_N, M, K, 2 * N, dgu, ldd, w, ldw, lddx);
-    if (dw) need_gemm(&c, type, dw_type, VKBLAS_OP_T, VKBLAS_OP_N, 2 * N, K, M, dgu, ldd, x, ldx, lddw);
-    const size_t o_d = dgu ? 0 : buf(&c, (uint64_t)M * ldd * type_size(type));
+    /* The two products as the fast kernels take them, where their work is
+     * worth the copies (from 4 GFLOP each on) and the layout of [dG | dU] is
+     * this call's own: K in whole 16-byte units (columns of both results), M
+     * (which dw sums over) in whole pairs of K steps, and N (dx sums over both
+     * halves) so that 2 N is, for an odd N from 128 rows on, else from 1024. */
+    const size_t es = type_size(type);
+    const uint32_t vec = vec_of(type), steps = type == VKBLAS_DT_F32 ? 64 : 128;
+    const int big = 4.0 * M * N * K >= 4e9;
+    uint32_t Mp = M, Np = N, Kp = K;
+    if (big && K % vec) Kp = (uint32_t)round_up(K, vec);
+    if (big && !dgu && dw && M % steps) Mp = (uint32_t)round_up(M, steps);
+    if (big && !dgu && N % (steps / 2) && M >= (2 * N % vec ? 128 : 1024)) Np = (uint32_t)round_up(N, steps / 2);
+    operand ox = as_is(x, ldx, 1, M, K), ow = as_is(w, ldw, 2, N, K);
+    if (dw && big && (Mp != M || Kp != K || off_units(type, x, ldx))) pad_to(&ox, Mp, (uint32_t)round_up(K, vec));
+    if (dx && big && (Np != N || Kp != K || off_units(type, w, ldw))) pad_to(&ow, Np, (uint32_t)round_up(K, vec));
+    const uint32_t ldd = dgu ? lddgu : (uint32_t)round_up(2 * Np, 8);
+    /* results of other sizes than the program's go by the workspace; a dw that
+     * adds to what is there is rounded once, after that */
+    const int px = dx && Kp != K, pw = dw && (Kp != K || Np != N);
+    const vkblas_dtype_t wt = pw && beta != 0.0f ? VKBLAS_DT_F32 : dw_type;
+    const uint32_t ldxo = px ? Kp : lddx, ldwo = pw ? Kp : lddw;
+    if (dx) need_gemm(&c, type, type, VKBLAS_OP_N, VKBLAS_OP_N, M, Kp, 2 * Np, dgu, ldd, ow.p, ow.ld, ldxo);
+    if (dw) need_gemm(&c, type, wt, VKBLAS_OP_T, VKBLAS_OP_N, 2 * Np, Kp, Mp, dgu, ldd, ox.p, ox.ld, ldwo);
+    const size_t o_d = dgu ? 0 : buf(&c, (uint64_t)Mp * ldd * es);
+    place(&c, &ox, type);
+    place(&c, &ow, type);
+    const size_t o_x = px ? buf(&c, (uint64_t)M * Kp * es) : 0;
+    const size_t o_w = pw ? buf(&c, (uint64_t)2 * Np * Kp * type_size(wt)) : 0;
     if (room(&c) != VKBLAS_OK) return c.st;
-    void* d = dgu ? dgu : at(&c, o_d);
-    if (step(&c, vkb_launch_glu_join_backward(type, act, M, N, dh, lddh, gu, ldgu, d, ldd, stream), dgu != NULL) &&
-        (!dx || product(&c, type, type, VKBLAS_OP_N, VKBLAS_OP_N, M, K, 2 * N, host_scalars(1.0f, 0.0f), d, ldd, w,
-                        ldw, dx, lddx, 1)) &&
-        dw)
-        product(&c, type, dw_type, VKBLAS_OP_T, VKBLAS_OP_N, 2 * N, K, M, host_scalars(1.0f, beta), d, ldd, x, ldx, dw,
-                lddw, 1);
+    void *d = dgu ? dgu : at(&c, o_d), *xo = px ? at(&c, o_x) : dx, *wo = pw ? at(&c, o_w) : dw;
+    int ok = step(&c, vkb_launch_glu_join_backward(type, act, M, N, dh, lddh, gu, ldgu, d, ldd, Mp, Np, stream),
+                  dgu != NULL) &&
+             bring(&c, &ox, type, x, ldx) && bring(&c, &ow, type, w, ldw);
+    if (ok && dx)
+        ok = product(&c, type, type, VKBLAS_OP_N, VKBLAS_OP_N, M, Kp, 2 * Np, host_scalars(1.0f, 0.0f), d, ldd, ow.p,
+                     ow.ld, xo, ldxo, !px) &&
+             (!px || step(&c, vkb_launch_unpad(type, type, 1, M, K, xo, Kp, M, dx, lddx, 0.0f, stream), 1));
+    if (ok && dw)
+        ok = product(&c, type, wt, VKBLAS_OP_T, VKBLAS_OP_N, 2 * Np, Kp, Mp, host_scalars(1.0f, pw ? 0.0f : beta), d,
+                     ldd, ox.p, ox.ld, wo, ldwo, !pw) &&
+             (!pw || step(&c, vkb_launch_unpad(wt, dw_type, 2, N, K, wo, Kp, Np, dw, lddw, beta, stream), 1));
     return op_end(&c, VKBLAS_KERNEL_JOINED);
 }
 
 /* --------------------------------------------------- linear cross entropy */
-
-typedef struct { uint32_t v, cols; } piece_t;
 
 /* Columns of the vocabulary at a time, so that M of them take about `bytes`
  * at `each` bytes a logit: whole slices of 256. */
@@ -341,13 +441,19 @@ vkblas_status_t vkblas_linear_xent_async(vkblas_dtype_t type, uint32_t M, uint32
     op_begin(&c, "linear_xent", stream);
     if (vkb_engine_trace()) fprintf(stderr, "[vkblas] linear_xent type=%d M=%u V=%u K=%u\n", (int)type, M, V, K);
     vkb_op_args a;
-    if (op_plan(type, M, V, K, x, ldx, w, ldw, 256, &a)) {
+    operand ox = as_is(x, ldx, 1, M, K), ow = as_is(w, ldw, 1, V, K);
+    if (fusable(type, M, V, K, &ox, &ow, 256, &a)) {
         const uint32_t S = vkb_xent_slices(&a);
+        place(&c, &ox, type);
+        place(&c, &ow, type);
         const size_t o_p = buf(&c, (uint64_t)S * M * 2 * sizeof(float)), o_t = buf(&c, (uint64_t)M * sizeof(float));
         if (room(&c) != VKBLAS_OK) return c.st;
         float *parts = at(&c, o_p), *zt = at(&c, o_t);
-        if (step(&c, vkb_launch_xent_stats_op(&a, target, parts, zt, stream), 0))
-            step(&c, vkb_launch_xent_finish(M, V, S, parts, zt, target, ignore_index, loss, lse, stream), 1);
+        if (bring(&c, &ox, type, x, ldx) && bring(&c, &ow, type, w, ldw)) {
+            bound(&a, &ox, &ow);
+            if (step(&c, vkb_launch_xent_stats_op(&a, target, parts, zt, stream), 0))
+                step(&c, vkb_launch_xent_finish(M, V, S, parts, zt, target, ignore_index, loss, lse, stream), 1);
+        }
         return op_end(&c, VKBLAS_KERNEL_FUSED);
     }
     const uint32_t n = piece_columns(M, V, JOIN_BYTES, sizeof(float)), ldz = (uint32_t)round_up(n, 4);
@@ -392,64 +498,111 @@ vkblas_status_t vkblas_linear_xent_backward_async(vkblas_dtype_t type, uint32_t 
         fprintf(stderr, "[vkblas] linear_xent_backward type=%d M=%u V=%u K=%u\n", (int)type, M, V, K);
     /* D of a piece of the vocabulary at a time, in type: from the pipelined
      * kernel, or over the piece's logits in fp32 (fp32: in their place).
-     * Pieces are whole tiles, then the rest of the vocabulary: odd classes
-     * would cost both products of a whole piece their fast kernels. */
+     * Where the products' work is worth it, their sums run over whole steps:
+     *  - dw's over M rows padded with zeros (D's, and a copy of x);
+     *  - dx's over whole tiles of classes, and the rest of the vocabulary by a
+     *    padded copy of its rows of w, whose part of dw comes by the workspace;
+     *    a w that is copied in any case is padded there. */
     const int f32 = type == VKBLAS_DT_F32;
     const size_t es = type_size(type);
+    const double work = 2.0 * M * V * K;
     vkb_op_args a;
-    const int fused = op_plan(type, M, V, K, x, ldx, w, ldw, 256, &a);
+    operand ox = as_is(x, ldx, 1, M, K), ow = as_is(w, ldw, 1, V, K);
+    const int fused = fusable(type, M, V, K, &ox, &ow, 256, &a);
+    const uint32_t Kp = fused ? a.K : K, steps = f32 ? 64 : 128;
+    const int whole = fused && (work >= (f32 ? 2e9 : V % 8 ? 1e10 : 4e10) || ow.copy);
+    uint32_t Mp = M;
+    if (fused && dw && M % steps && work >= (f32 ? 2e9 : 1e10)) Mp = (uint32_t)round_up(M, steps);
+    if (ox.copy || Mp != M) pad_to(&ox, Mp, Kp);
+    if (ow.copy) pad_to(&ow, (uint32_t)round_up(V, 128), Kp);
+    const uint32_t rest = whole && !ow.copy ? V % 128 : 0;   /* classes that the tail takes */
     uint32_t n = piece_columns(M, V, fused ? PIECE_BYTES : JOIN_BYTES, fused ? es : sizeof(float));
-    if (n == V && V > 256 && V % 128) n = V / 128 * 128;
-    const uint32_t ldd = (uint32_t)round_up(n, 8);
-    piece_t pieces[3];           /* the kinds of pieces: n columns, then whole tiles, then the rest */
-    int kinds = 0;
-    const uint32_t tail = V % n;
-    pieces[kinds++] = (piece_t){0, n};
-    if (tail >= 128) pieces[kinds++] = (piece_t){V - tail, tail / 128 * 128};
-    if (tail % 128) pieces[kinds++] = (piece_t){V - tail % 128, tail % 128};
-    /* dx adds up over the pieces in fp32: in dx itself or in the workspace */
-    const int acc = dx && n < V && !f32;
+    const uint32_t ldd = (uint32_t)round_up(n, whole ? 128 : 8);
+    /* dx adds up over several products in fp32: in dx itself or in the workspace */
+    const int several = n < V || rest, acc = dx && (Kp != K || (several && !f32));
     const vkblas_dtype_t xt = acc ? VKBLAS_DT_F32 : type;
-    const uint32_t lda = acc ? (uint32_t)round_up(K, 4) : lddx;
-    for (int i = 0; i < kinds; ++i) {
-        const uint32_t cols = pieces[i].cols;
+    const uint32_t ldxo = acc ? (uint32_t)round_up(Kp, 4) : lddx;
+    /* dw's rows of other sizes than the program's go by the workspace */
+    const int pw = dw && (Kp != K || (ow.copy && V % 128));
+    const vkblas_dtype_t wt = (pw || rest) && beta != 0.0f ? VKBLAS_DT_F32 : dw_type;
+    for (int i = 0; i < 2; ++i) {   /* a piece of n columns, and the last one */
+        const uint32_t cols = i ? V % n : n;
+        if (!cols) continue;
+        const uint32_t main = whole ? (ow.copy ? (uint32_t)round_up(cols, 128) : cols / 128 * 128) : cols;
         if (!fused)
             need_gemm(&c, type, VKBLAS_DT_F32, VKBLAS_OP_N, VKBLAS_OP_T, M, cols, K, x, ldx, w, ldw, ldd);
-        if (dx) need_gemm(&c, type, xt, VKBLAS_OP_N, VKBLAS_OP_N, M, K, cols, NULL, ldd, w, ldw, lda);
-        if (dw) need_gemm(&c, type, dw_type, VKBLAS_OP_T, VKBLAS_OP_N, cols, K, M, NULL, ldd, x, ldx, lddw);
+        if (dx && main) need_gemm(&c, type, xt, VKBLAS_OP_N, VKBLAS_OP_N, M, Kp, main, NULL, ldd, ow.p, ow.ld, ldxo);
+        if (dw && main)
+            need_gemm(&c, type, pw ? wt : dw_type, VKBLAS_OP_T, VKBLAS_OP_N, main, Kp, Mp, NULL, ldd, ox.p, ox.ld,
+                      pw ? Kp : lddw);
+    }
+    if (rest) {
+        if (dx) need_gemm(&c, type, xt, VKBLAS_OP_N, VKBLAS_OP_N, M, Kp, 128, NULL, ldd, NULL, Kp, ldxo);
+        if (dw) need_gemm(&c, type, wt, VKBLAS_OP_T, VKBLAS_OP_N, 128, Kp, Mp, NULL, ldd, ox.p, ox.ld, Kp);
     }
     const size_t o_z = fused ? 0 : buf(&c, (uint64_t)M * ldd * sizeof(float));
-    const size_t o_d = f32 && !fused ? o_z : buf(&c, (uint64_t)M * ldd * es);
-    const size_t o_a = acc ? buf(&c, (uint64_t)M * lda * sizeof(float)) : 0;
+    const size_t o_d = f32 && !fused ? o_z : buf(&c, (uint64_t)Mp * ldd * es);
+    place(&c, &ox, type);
+    place(&c, &ow, type);
+    operand tail = as_is(NULL, Kp, 1, rest, K);
+    if (rest) {
+        pad_to(&tail, 128, Kp);
+        place(&c, &tail, type);
+    }
+    const size_t o_x = acc ? buf(&c, (uint64_t)M * ldxo * sizeof(float)) : 0;
+    const size_t o_w = pw || rest ? buf(&c, (pw ? round_up(n, 128) : 128) * Kp * type_size(wt)) : 0;
     const size_t o_s = buf(&c, 8 * sizeof(float));
     if (room(&c) != VKBLAS_OK) return c.st;
     float *z = at(&c, o_z), *scal = f32 ? NULL : (float*)at(&c, o_s);
-    void *d = at(&c, o_d), *xo = acc ? at(&c, o_a) : dx;
-    int ok = !scal || step(&c, vkb_launch_xent_scale(type, M, dloss, beta, scal, stream), 0);
+    void *d = at(&c, o_d), *xo = acc ? at(&c, o_x) : dx, *wo = at(&c, o_w);
+    int ok = (!scal || step(&c, vkb_launch_xent_scale(type, M, dloss, beta, scal, stream), 0)) &&
+             bring(&c, &ox, type, x, ldx) && bring(&c, &ow, type, w, ldw) &&
+             (!rest || !dx || bring(&c, &tail, type, (const char*)w + (uint64_t)(V - rest) * ldw * es, ldw));
+    int summed = 0;              /* dx holds a product already */
     for (uint64_t v = 0; ok && v < V;) {
-        const uint32_t left = (uint32_t)(V - v), cols = left >= n ? n : left >= 128 ? left / 128 * 128 : left;
-        const char* wv = (const char*)w + v * ldw * es;
+        const uint32_t cols = (uint32_t)(V - v < n ? V - v : n);
+        const uint32_t main = whole ? (ow.copy ? (uint32_t)round_up(cols, 128) : cols / 128 * 128) : cols;
+        const char* wv = (const char*)ow.p + v * ow.ld * es;
+        char* dwv = (char*)dw + v * lddw * (dw ? type_size(dw_type) : 0);
         if (fused) {
+            bound(&a, &ox, &ow);
             a.w = wv;
             a.N = cols;
-            ok = step(&c, vkb_launch_xent_grad_op(&a, (uint32_t)v, V, target, ignore_index, lse, dloss, scal, d, ldd,
-                                                  stream), 0);
+            ok = step(&c, vkb_launch_xent_grad_op(&a, Mp, (uint32_t)round_up(cols, whole ? 128 : 8), (uint32_t)v, V,
+                                                  target, ignore_index, lse, dloss, scal, d, ldd, stream), 0);
         } else {
             ok = product(&c, type, VKBLAS_DT_F32, VKBLAS_OP_N, VKBLAS_OP_T, M, cols, K, host_scalars(1.0f, 0.0f), x,
                          ldx, wv, ldw, z, ldd, 0) &&
                  step(&c, vkb_launch_xent_grad(type, M, cols, (uint32_t)v, V, z, ldd, target, ignore_index, lse, dloss,
                                                scal, d, ldd, stream), 0);
         }
-        const scalars sw = {1.0f, beta, scal ? scal + 1 : NULL, scal ? scal + 2 : NULL};
-        const scalars sx = {1.0f, v ? 1.0f : 0.0f, scal ? scal + 1 : NULL, scal ? scal + (v ? 3 : 4) : NULL};
-        if (ok && dw)
-            ok = product(&c, type, dw_type, VKBLAS_OP_T, VKBLAS_OP_N, cols, K, M, sw, d, ldd, x, ldx,
-                         (char*)dw + v * lddw * type_size(dw_type), lddw, 1);
-        if (ok && dx)
-            ok = product(&c, type, xt, VKBLAS_OP_N, VKBLAS_OP_N, M, K, cols, sx, d, ldd, wv, ldw, xo, lda, !acc);
+        /* the whole tiles, then the tail */
+        for (int t = 0; ok && t < 2; ++t) {
+            const uint32_t rows = t ? cols - (main < cols ? main : cols) : main < cols ? main : cols;   /* of dw */
+            const uint32_t sum = t ? 128 : main;
+            if (!rows) continue;
+            const char* dt = (const char*)d + (t ? (uint64_t)main * es : 0);
+            const int by_ws = pw || t;
+            if (dw) {
+                const scalars sw = {1.0f, by_ws ? 0.0f : beta, scal ? scal + 1 : NULL,
+                                    scal ? scal + (by_ws ? 4 : 2) : NULL};
+                char* to = dwv + (t ? (uint64_t)main * lddw * type_size(dw_type) : 0);
+                ok = product(&c, type, by_ws ? wt : dw_type, VKBLAS_OP_T, VKBLAS_OP_N, by_ws ? sum : rows, Kp, Mp, sw,
+                             dt, ldd, ox.p, ox.ld, by_ws ? wo : to, by_ws ? Kp : lddw, !by_ws) &&
+                     (!by_ws || step(&c, vkb_launch_unpad(wt, dw_type, 1, rows, K, wo, Kp, rows, to, lddw, beta,
+                                                          stream), 1));
+            }
+            if (ok && dx) {
+                const scalars sx = {1.0f, summed ? 1.0f : 0.0f, scal ? scal + 1 : NULL,
+                                    scal ? scal + (summed ? 3 : 4) : NULL};
+                ok = product(&c, type, xt, VKBLAS_OP_N, VKBLAS_OP_N, M, Kp, sum, sx, dt, ldd, t ? tail.p : wv,
+                             t ? Kp : ow.ld, xo, ldxo, !acc);
+                summed = 1;
+            }
+        }
         v += cols;
     }
     if (ok && acc)
-        step(&c, vkb_launch_convert(type, M, K, xo, lda, dx, lddx, stream), 1);
+        step(&c, vkb_launch_unpad(VKBLAS_DT_F32, type, 1, M, K, xo, ldxo, M, dx, lddx, 0.0f, stream), 1);
     return op_end(&c, fused ? VKBLAS_KERNEL_FUSED : VKBLAS_KERNEL_JOINED);
 }

@@ -59,11 +59,13 @@ static int launch_xent_stats(const vkb_op_args* a, const int64_t* target, float*
 }
 
 template <typename T>
-static int launch_xent_grad(const vkb_op_args* a, uint32_t v0, uint32_t V, const int64_t* target, int64_t ignore,
-                            const float* lse, const float* dloss, const float* scal, void* D, int64_t ldd,
+static int launch_xent_grad(const vkb_op_args* a, uint32_t Ms, uint32_t Ns, uint32_t v0, uint32_t V,
+                            const int64_t* target, int64_t ignore, const float* lse, const float* dloss, const float* scal, void* D, int64_t ldd,
                             hipStream_t st) {
     XentParams p = op_params<T, XentParams>(a);
     p.target = target;
+    p.Ms = Ms;
+    p.Ns = Ns;
     p.v0 = v0;
     p.V = V;
     p.ignore = ignore;
@@ -87,8 +89,10 @@ static int launch_xent_grad(const vkb_op_args* a, uint32_t v0, uint32_t V, const
                                                 float* zt, void* st) {                                               \
         return vkb::launch_xent_stats<T>(a, target, parts, zt, (hipStream_t)st);                                     \
     }                                                                                                                \
-    extern "C" int vkb_launch_xent_grad_##NAME(const vkb_op_args* a, uint32_t v0, uint32_t V, const int64_t* target, \
-                                               int64_t ignore, const float* lse, const float* dloss,                 \
-                                               const float* scal, void* D, int64_t ldd, void* st) {                  \
-        return vkb::launch_xent_grad<T>(a, v0, V, target, ignore, lse, dloss, scal, D, ldd, (hipStream_t)st);        \
+    extern "C" int vkb_launch_xent_grad_##NAME(const vkb_op_args* a, uint32_t Ms, uint32_t Ns, uint32_t v0,          \
+                                               uint32_t V, const int64_t* target, int64_t ignore, const float* lse,  \
+                                               const float* dloss, const float* scal, void* D, int64_t ldd,          \
+                                               void* st) {                                                           \
+        return vkb::launch_xent_grad<T>(a, Ms, Ns, v0, V, target, ignore, lse, dloss, scal, D, ldd,                  \
+                                        (hipStream_t)st);                                                            \
     }

@@ -27,17 +27,23 @@ int vkb_launch_layer_norm_reduce(const float* part, uint32_t parts, uint32_t N, 
 /* C = beta * C on M x N (a gradient over an empty batch). */
 int vkb_launch_scale(int type, uint32_t M, uint32_t N, void* C, int64_t ldc, float beta, void* stream);
 
-/* C = A rounded to type, A in fp32. */
-int vkb_launch_convert(int type, uint32_t M, uint32_t N, const float* A, int64_t lda, void* C, int64_t ldc,
-                       void* stream);
+/* Copies (pad.hip) of S matrices of M x N below each other, from or to rows
+ * of Mp >= M in the workspace.  pad: P, of Np >= N columns, zero past M and N;
+ * unpad: out = beta * out + P, P of out_type or fp32. */
+int vkb_launch_pad(int type, uint32_t S, uint32_t M, uint32_t N, const void* A, int64_t lda, void* P, uint32_t Mp,
+                   uint32_t Np, void* stream);
+int vkb_launch_unpad(int type, int out_type, uint32_t S, uint32_t M, uint32_t N, const void* P, int64_t ldp,
+                     uint32_t Mp, void* out, int64_t ldc, float beta, void* stream);
 
 /* Gated projection (glu.hip), from projections computed before:
  * h = act(G) * U from z = [G | U] in fp32, and gu = z rounded (NULL: not
- * stored); and [dG | dU] from dh and gu. */
+ * stored); and [dG | dU] from dh and gu, Np >= N columns each on Mp >= M
+ * rows, zero past N and M. */
 int vkb_launch_glu_join(int type, int act, uint32_t M, uint32_t N, const float* z, int64_t ldz, void* h, int64_t ldh,
                         void* gu, int64_t ldgu, void* stream);
 int vkb_launch_glu_join_backward(int type, int act, uint32_t M, uint32_t N, const void* dh, int64_t lddh,
-                                 const void* gu, int64_t ldgu, void* dgu, int64_t lddgu, void* stream);
+                                 const void* gu, int64_t ldgu, void* dgu, int64_t lddgu, uint32_t Mp, uint32_t Np,
+                                 void* stream);
 
 /* Linear cross entropy (xent.hip).  stats: over z, columns v0 .. v0 + n - 1
  * of the logits, the pair (max, sum of exp(z - max)) of each row and each
@@ -71,11 +77,11 @@ int vkb_launch_glu(const vkb_op_args* a, int act, void* h, int64_t ldh, void* gu
  * vkb_xent_slices of them */
 uint32_t vkb_xent_slices(const vkb_op_args* a);
 int vkb_launch_xent_stats_op(const vkb_op_args* a, const int64_t* target, float* parts, float* zt, void* stream);
-/* D as vkb_launch_xent_grad; ldd a multiple of 8 and at least N rounded up to
- * one (the columns between are written too) */
-int vkb_launch_xent_grad_op(const vkb_op_args* a, uint32_t v0, uint32_t V, const int64_t* target, int64_t ignore,
-                            const float* lse, const float* dloss, const float* scal, void* D, int64_t ldd,
-                            void* stream);
+/* D as vkb_launch_xent_grad, stored on Ms rows and Ns columns, zero past M and
+ * N: at least those, at most them rounded up to 128, Ns a multiple of 8 */
+int vkb_launch_xent_grad_op(const vkb_op_args* a, uint32_t Ms, uint32_t Ns, uint32_t v0, uint32_t V,
+                            const int64_t* target, int64_t ignore, const float* lse, const float* dloss,
+                            const float* scal, void* D, int64_t ldd, void* stream);
 
 #ifdef __cplusplus
 }
