@@ -44,7 +44,7 @@ def check_forward(got, x, w, b, dt, eps=EPS):
     R.close(got[0], y, R.rounded(y, dt, err), "y")
 
 
-SIZES = [(1, 1), (3, 7), (5, 64), (2, 511), (9, 512), (4, 513), (6, 1000), (3, 1024), (2, 1025), (5, 2047), (2, 2048),
+SIZES = [(1, 1), (3, 7), (3, 8), (5, 9), (2, 15), (5, 64), (2, 511), (9, 512), (4, 513), (6, 1000), (3, 1024), (2, 1025), (5, 2047), (2, 2048),
          (3, 4096), (2, 4097), (3, 5003), (2, 8192), (2, 9001), (1, 16384), (2, 16385), (2, 40000), (1500, 96),
          (4500, 40), (1100, 1100), (300, 5000)]
 
@@ -57,7 +57,7 @@ def test_forward(M, N, dt, wt):
     w, b = 1 + 0.2 * R.values(1, N, wt, 2)[0], R.values(1, N, wt, 3)[0]
     w = w.to(R.TORCH[wt]).double()
     check_forward(forward(x, w, b, dt, wt), x, w, b, dt)
-    assert vk.last_kernel() == (vk.KERNEL_NORM_LONG if N > 16384 else vk.KERNEL_NORM)
+    assert vk.last_kernel() == (vk.KERNEL_NORM_LONG if N > 16384 or N < 8 else vk.KERNEL_NORM)
 
 
 @pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])

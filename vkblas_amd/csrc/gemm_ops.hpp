@@ -25,8 +25,9 @@ struct Frag {
 // Stores a wave's WT x WC block to rows row0 .. of C (leading dimension ldc),
 // columns col0 .., those below M and N: f(i, j, q, x) gives four consecutive
 // columns.  Through LDS, so that rows leave in 16-byte chunks of whole
-// segments; non-temporal, which leaves L2 to the operands other tiles still
-// read.
+// segments; non-temporal where rows lie on 16-byte units, which leaves L2 to
+// the operands other tiles still read (else lines are written in parts, which
+// L2 has to join).
 template <typename T, int WT, int WC, int SH, int LDS, typename F>
 __device__ __forceinline__ void store_block(F f, T* C, int64_t ldc, int64_t row0, int64_t col0, int64_t M, int64_t N,
                                             char* lds, int wave, int lane) {
@@ -38,6 +39,7 @@ __device__ __forceinline__ void store_block(F f, T* C, int64_t ldc, int64_t row0
     constexpr int VEC = Elem<T>::VEC;
     static_assert(4 * PROWS * STR <= LDS, "staging exceeds LDS");
     char* wl = lds + wave * (PROWS * STR);
+    const bool units = (((uint64_t)C | (uint64_t)(ldc * (int64_t)sizeof(T))) & 15) == 0;
 #pragma unroll
     for (int pass = 0; pass < PASSES; ++pass) {
 #pragma unroll
@@ -62,7 +64,7 @@ __device__ __forceinline__ void store_block(F f, T* C, int64_t ldc, int64_t row0
             const u32x4 v = *(const u32x4*)(wl + r * STR + c * 16);
             const int64_t m = row0 + pass * PROWS + r, n = col0 + c * VEC;
             if (m >= M) continue;
-            if (n + VEC <= N) __builtin_nontemporal_store(v, (u32x4_any*)(C + m * ldc + n));
+            if (units && n + VEC <= N) __builtin_nontemporal_store(v, (u32x4*)(C + m * ldc + n));
             else st_chunk(C + m * ldc, n, N, v);
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");

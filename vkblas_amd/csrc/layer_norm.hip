@@ -16,36 +16,134 @@
 namespace vkb {
 namespace {
 
-// A row's columns over WAVES waves: thread t holds the 16-byte chunks
-// t + i TPR, i < EPT / VEC.  WAVES == 1: four rows per workgroup, one per
-// wave, no barrier.
-template <typename T, int WAVES, int EPT>
+// How a row's columns lie in a workgroup: its threads hold the 16-byte chunks
+// t + i * (threads per row), i < EPT / VEC.
+//  ONE:  a wave per row, four rows per workgroup, no barrier;
+//  FEW:  a workgroup of up to eight waves per row, w and b in registers;
+//  MANY: up to sixteen, which leaves 128 registers a thread: w and b in LDS
+//        (read from L2 for every row they were the bound: 14080 columns of
+//        bf16 with fp32 parameters 196 us against 143).
+// As many waves as the columns need, past four in whole rounds of the CU's
+// four SIMDs: a row is about half bound by its instructions, and a fifth wave
+// doubles one SIMD's (8192 x 4352 bf16 58 us with five waves).
+enum { ONE, FEW, MANY };
+constexpr uint32_t LAST = 16384;
+template <typename T, int MAP, int EPT>
 struct RowMap {
     static constexpr int VEC = Elem<T>::VEC, NV = EPT / VEC;
-    static constexpr int TPR = WAVES * 64;                   // threads per row
-    static constexpr int RPB = WAVES == 1 ? 4 : 1;           // rows at a time
-    static constexpr int THREADS = TPR * RPB;
-    // sixteen waves leave 128 registers a thread: with 16 values, w and b are
-    // read again for every row and no row is loaded ahead
-    static constexpr bool LEAN = WAVES == 16 && EPT == 16;
+    static constexpr int RPB = MAP == ONE ? 4 : 1;           // rows at a time
+    static constexpr int MAXW = MAP == ONE ? 1 : MAP == FEW ? 8 : 16;
+    static constexpr int THREADS = MAXW * RPB * 64;          // at most
     static_assert(EPT % VEC == 0, "whole chunks");
+    // waves per row of N columns
+    static uint32_t waves(uint32_t N) {
+        const uint32_t w = (N + 64 * EPT - 1) / (64 * EPT);
+        return MAP == ONE ? 1 : w <= 4 ? w : (w + 3) / 4 * 4;
+    }
 };
 
-template <typename W, typename T, int WAVES, int EPT>
-__device__ __forceinline__ void load_params(const W* w, int t, uint32_t N, float none, float* out) {
-    using R = RowMap<T, WAVES, EPT>;
+// A thread's chunks of a row of N >= VEC columns, the same for every row, so
+// that a row is loaded without a branch (one between lanes made every load wait
+// for the one before it, one around a wave's load for the last row's stores:
+// rows of 4832 against 4096 81 us against 37).  Chunk i is read from column
+// off(i): the one at the row's end from N - VEC on, and threads past the end
+// read that too; its elements before from(i) are another thread's.  whole: every
+// chunk of this wave is a lane's own throughout (the same in all its lanes).
+template <typename T, int NV>
+struct Chunks {
+    static constexpr int VEC = Elem<T>::VEC;
+    int t, tpr;
+    uint32_t N;
+    bool whole;
+    __device__ __forceinline__ Chunks(int t_, int tpr_, uint32_t N_) : t(t_), tpr(tpr_), N(N_) {
+        bool all = true;
 #pragma unroll
-    for (int i = 0; i < R::NV; ++i) {
-        const int64_t c = (int64_t)(t + i * R::TPR) * R::VEC;
-        if (!w) {
-#pragma unroll
-            for (int e = 0; e < R::VEC; ++e) out[i * R::VEC + e] = none;
-            continue;
-        }
-#pragma unroll
-        for (int q = 0; q < R::VEC; q += Elem<W>::VEC) unpack<W>(ld_chunk(w, c + q, N), out + i * R::VEC + q);
+        for (int i = 0; i < NV; ++i) all = all && from(i) == 0;
+        whole = __all(all);
     }
+    __device__ __forceinline__ uint32_t off(int i) const { return min((uint32_t)(t + i * tpr) * VEC, N - VEC); }
+    __device__ __forceinline__ int from(int i) const {
+        return (int)min((uint32_t)(t + i * tpr) * VEC - off(i), (uint32_t)VEC);
+    }
+    // a value of t that the compiler takes for a new one: nothing derived from
+    // it is kept in registers over the rows before this
+    __device__ __forceinline__ void fresh() { asm volatile("" : "+v"(t)); }
+    __device__ __forceinline__ float count() const {
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) c += VEC - from(i);
+        return (float)c;
+    }
+    // x[e] becomes 0 unless it is this thread's
+    __device__ __forceinline__ void own(int i, float* x) const {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) x[e] = e >= from(i) ? x[e] : 0.0f;
+    }
+    __device__ __forceinline__ void store(int i, T* row, u32x4 v) const {
+        if (whole || from(i) == 0) {
+            *(u32x4_any*)(row + off(i)) = v;
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                if (e < from(i)) continue;
+                if constexpr (sizeof(T) == 4) *(uint32_t*)(row + off(i) + e) = v[e];
+                else *(uint16_t*)(row + off(i) + e) = (uint16_t)(v[e / 2] >> (16 * (e & 1)));
+            }
+        }
+    }
+};
+
+template <typename W, int VEC>
+__device__ __forceinline__ void load_params(const W* w, uint32_t c, float none, float* out) {
+    if (!w) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) out[e] = none;
+        return;
+    }
+#pragma unroll
+    for (int q = 0; q < VEC; q += Elem<W>::VEC) unpack<W>(ld16_any(w + c + q), out + q);
 }
+
+// w or b of a thread's columns: registers, or this thread's own words of LDS
+template <typename T, int MAP, int EPT>
+struct Params {
+    using R = RowMap<T, MAP, EPT>;
+    float reg[MAP == MANY ? 1 : EPT];
+    float4* lds;             // MANY: chunk i, quarter q of thread t at (i VEC / 4 + q) * threads + t
+    int t, tpr;
+    template <typename W>
+    __device__ __forceinline__ void load(const W* w, float none, uint32_t N, float4* mem, int t_, int tpr_) {
+        lds = mem;
+        t = t_;
+        tpr = tpr_;
+#pragma unroll
+        for (int i = 0; i < R::NV; ++i) {
+            float x[R::VEC];
+            load_params<W, R::VEC>(w, min((uint32_t)(t + i * tpr) * R::VEC, N - R::VEC), none, x);   // as Chunks
+#pragma unroll
+            for (int e = 0; e < R::VEC; ++e) {
+                if constexpr (MAP != MANY) reg[i * R::VEC + e] = x[e];
+            }
+            if constexpr (MAP == MANY)
+#pragma unroll
+                for (int q = 0; q < R::VEC / 4; ++q)
+                    lds[(i * (R::VEC / 4) + q) * tpr + t] = float4{x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
+        }
+    }
+    // the VEC values of chunk i
+    __device__ __forceinline__ void get(int i, float* x) const {
+        if constexpr (MAP == MANY) {
+#pragma unroll
+            for (int q = 0; q < R::VEC / 4; ++q) {
+                const float4 v = lds[(i * (R::VEC / 4) + q) * tpr + t];
+                x[4 * q] = v.x, x[4 * q + 1] = v.y, x[4 * q + 2] = v.z, x[4 * q + 3] = v.w;
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < R::VEC; ++e) x[e] = reg[i * R::VEC + e];
+        }
+    }
+};
 
 // Mean and sum of squares about it over a row.  Each wave forms its own mean
 // and squares about that (no barrier), and the waves' join, over c_i columns
@@ -54,168 +152,176 @@ __device__ __forceinline__ void load_params(const W* w, int t, uint32_t N, float
 // one barrier per row and no cancellation (the mean comes from the sums: from
 // the rounded wave means it was 16 times less exact where it is near zero).
 // sh is the row parity's buffer.
-template <int WAVES>
-__device__ __forceinline__ void join_stats(float cnt, float sum, float& mean, float& m2, float (*sh)[4], float N) {
-    if constexpr (WAVES == 1) return;
-    const int wave = threadIdx.x >> 6;
-    if ((threadIdx.x & 63) == 0) {
-        sh[wave][0] = cnt;
-        sh[wave][1] = mean;
-        sh[wave][2] = m2;
-        sh[wave][3] = sum;
-    }
+__device__ __forceinline__ void join_stats(float cnt, float sum, float& mean, float& m2, float4* sh, int waves,
+                                           float N) {
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = float4{cnt, mean, m2, sum};
     __syncthreads();
     float tot = 0.0f;
-#pragma unroll
-    for (int i = 0; i < WAVES; ++i) tot += sh[i][3];
+    for (int i = 0; i < waves; ++i) tot += sh[i].w;
     mean = tot / N;
     m2 = 0.0f;
-#pragma unroll
-    for (int i = 0; i < WAVES; ++i) {
-        const float d = sh[i][1] - mean;
-        m2 += sh[i][2] + sh[i][0] * d * d;
+    for (int i = 0; i < waves; ++i) {
+        const float4 v = sh[i];
+        const float d = v.y - mean;
+        m2 += v.z + v.x * d * d;
     }
 }
 
-template <typename T, typename W, int WAVES, int EPT>
-__global__ __launch_bounds__((RowMap<T, WAVES, EPT>::THREADS)) void layer_norm_kernel(
+template <typename T, typename W, int MAP, int EPT>
+__global__ __launch_bounds__((RowMap<T, MAP, EPT>::THREADS)) void layer_norm_kernel(
     uint32_t M, uint32_t N, const T* x, int64_t ldx, const W* w, const W* b, float eps, T* y, int64_t ldy,
     float* mean_out, float* rstd_out) {
-    using R = RowMap<T, WAVES, EPT>;
+    using R = RowMap<T, MAP, EPT>;
     constexpr int VEC = R::VEC, NV = R::NV;
-    __shared__ float sh[2][WAVES][4];
-    const int t = WAVES == 1 ? (threadIdx.x & 63) : threadIdx.x;
-    const uint32_t sub = WAVES == 1 ? threadIdx.x >> 6 : 0;
+    __shared__ float4 sh[2][R::MAXW];
+    __shared__ float4 prm[MAP == MANY ? 2 : 1][MAP == MANY ? LAST / 4 : 1];
+    const int t = MAP == ONE ? (threadIdx.x & 63) : threadIdx.x, tpr = MAP == ONE ? 64 : blockDim.x;
+    const uint32_t sub = MAP == ONE ? threadIdx.x >> 6 : 0;
     const uint32_t step = gridDim.x * R::RPB;
     uint32_t m = blockIdx.x * R::RPB + sub;
+    const Chunks<T, NV> ch(t, tpr, N);
+    const float cnt = wave_sum(ch.count());   // columns of this wave
     u32x4 raw[NV];
     auto load_row = [&](uint32_t r) {
+        const T* row = x + (int64_t)r * ldx;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) raw[i] = ld_chunk(x + (int64_t)r * ldx, (int64_t)(t + i * R::TPR) * VEC, N);
+        for (int i = 0; i < NV; ++i) raw[i] = ld16_any(row + ch.off(i));
     };
-    float wv[EPT], bv[EPT];
-    if constexpr (!R::LEAN) {
-        if (m < M) load_row(m);
-        load_params<W, T, WAVES, EPT>(w, t, N, 1.0f, wv);
-        load_params<W, T, WAVES, EPT>(b, t, N, 0.0f, bv);
-    }
-    float cnt = 0.0f;   // columns of this thread, then of its wave
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int64_t left = (int64_t)N - (int64_t)(t + i * R::TPR) * VEC;
-        cnt += (float)(left < 0 ? 0 : left < VEC ? left : VEC);
-    }
-    cnt = wave_sum(cnt);
-    for (int par = 0; m < M; m += step, par ^= 1) {
-        float v[EPT], sum = 0.0f, m2 = 0.0f;
-        if constexpr (R::LEAN) load_row(m);
+    if (m < M) load_row(m);
+    Params<T, MAP, EPT> wv, bv;
+    wv.load(w, 1.0f, N, prm[0], t, tpr);
+    bv.load(b, 0.0f, N, prm[MAP == MANY], t, tpr);
+    float v[EPT];
+    auto unpack_row = [&]() {
 #pragma unroll
         for (int i = 0; i < NV; ++i) unpack<T>(raw[i], v + i * VEC);
-        if constexpr (!R::LEAN)
-            if (m + step < M && m + step > m) load_row(m + step);
+    };
+    if (m < M) unpack_row();
+    for (int par = 0; m < M; m += step, par ^= 1) {
+        const bool next = m + step < M && m + step > m;   // (past 2^32 rows: none)
+        if (next) load_row(m + step);
+        float sum = 0.0f, m2 = 0.0f;
 #pragma unroll
-        for (int i = 0; i < EPT; ++i) sum += v[i];
+        for (int i = 0; i < NV; ++i) {
+            float own[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) own[e] = v[i * VEC + e];
+            if (!ch.whole) ch.own(i, own);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) sum += own[e];
+        }
         sum = wave_sum(sum);
         float mean = cnt > 0.0f ? sum / cnt : 0.0f;
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+        for (int i = 0; i < NV; ++i) {
+            float d[VEC];
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                const bool in = (int64_t)(t + i * R::TPR) * VEC + e < N;
-                const float d = v[i * VEC + e] - mean;
-                m2 += in ? d * d : 0.0f;
-            }
+            for (int e = 0; e < VEC; ++e) d[e] = v[i * VEC + e] - mean;
+            if (!ch.whole) ch.own(i, d);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) m2 += d[e] * d[e];
+        }
         m2 = wave_sum(m2);
-        join_stats<WAVES>(cnt, sum, mean, m2, sh[par], (float)N);
+        if constexpr (MAP != ONE) join_stats(cnt, sum, mean, m2, sh[par], tpr >> 6, (float)N);
         const float rstd = 1.0f / sqrtf(m2 / (float)N + eps);
+        u32x4 out[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            float r[VEC], wi[VEC], bi[VEC];
+            wv.get(i, wi);
+            bv.get(i, bi);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) r[e] = (v[i * VEC + e] - mean) * rstd * wi[e] + bi[e];
+            out[i] = pack<T>(r);
+        }
+        // the next row is waited for before this one's stores leave: after
+        // them, its loads would be waited for together with the stores
+        if (next) unpack_row();
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) ch.store(i, y + (int64_t)m * ldy, out[i]);
         if (t == 0) {
             if (mean_out) mean_out[m] = mean;
             if (rstd_out) rstd_out[m] = rstd;
         }
-        if constexpr (R::LEAN) {
-            load_params<W, T, WAVES, EPT>(w, t, N, 1.0f, wv);
-            load_params<W, T, WAVES, EPT>(b, t, N, 0.0f, bv);
-        }
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            float r[VEC];
-#pragma unroll
-            for (int e = 0; e < VEC; ++e)
-                r[e] = (v[i * VEC + e] - mean) * rstd * wv[i * VEC + e] + bv[i * VEC + e];
-            st_chunk(y + (int64_t)m * ldy, (int64_t)(t + i * R::TPR) * VEC, N, pack<T>(r));
-        }
-        if (m + step < m) break;   // past 2^32 rows
+        if (!next) break;
     }
 }
 
-template <typename T, typename W, int WAVES, int EPT>
-__global__ __launch_bounds__((RowMap<T, WAVES, EPT>::THREADS)) void layer_norm_backward_kernel(
+template <typename T, typename W, int MAP, int EPT>
+__global__ __launch_bounds__((RowMap<T, MAP, EPT>::THREADS)) void layer_norm_backward_kernel(
     uint32_t M, uint32_t N, const T* dy, int64_t lddy, const T* x, int64_t ldx, const W* w, const float* mean,
     const float* rstd, T* dx, int64_t lddx, float* part) {
-    using R = RowMap<T, WAVES, EPT>;
+    using R = RowMap<T, MAP, EPT>;
     constexpr int VEC = R::VEC, NV = R::NV;
-    __shared__ float sh[2][WAVES][2];
-    const int t = WAVES == 1 ? (threadIdx.x & 63) : threadIdx.x;
-    const uint32_t sub = WAVES == 1 ? threadIdx.x >> 6 : 0;
+    __shared__ float2 sh[2][R::MAXW];
+    __shared__ float4 prm[MAP == MANY ? LAST / 4 : 1];
+    const int t = MAP == ONE ? (threadIdx.x & 63) : threadIdx.x, tpr = MAP == ONE ? 64 : blockDim.x;
+    const uint32_t sub = MAP == ONE ? threadIdx.x >> 6 : 0;
     const uint32_t step = gridDim.x * R::RPB;
     uint32_t m = blockIdx.x * R::RPB + sub;
+    Chunks<T, NV> ch(t, tpr, N);
     u32x4 rx[NV], rd[NV];
     float mu = 0.0f, rs = 0.0f;
     auto load_row = [&](uint32_t r) {
+        const T *xr = x + (int64_t)r * ldx, *dr = dy + (int64_t)r * lddy;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int64_t c = (int64_t)(t + i * R::TPR) * VEC;
-            rx[i] = ld_chunk(x + (int64_t)r * ldx, c, N);
-            rd[i] = ld_chunk(dy + (int64_t)r * lddy, c, N);
+            rx[i] = ld16_any(xr + ch.off(i));
+            rd[i] = ld16_any(dr + ch.off(i));
         }
         mu = mean[r];
         rs = rstd[r];
     };
-    float wv[EPT], dw[EPT], db[EPT];
-    if constexpr (!R::LEAN) {
-        if (m < M) load_row(m);
-        load_params<W, T, WAVES, EPT>(w, t, N, 1.0f, wv);
-    }
+    // MANY: no registers for a row loaded ahead
+    constexpr bool AHEAD = MAP != MANY;
+    if (AHEAD && m < M) load_row(m);
+    Params<T, MAP, EPT> wv;
+    wv.load(w, 1.0f, N, prm, t, tpr);
+    float dw[EPT], db[EPT];
 #pragma unroll
     for (int i = 0; i < EPT; ++i) dw[i] = db[i] = 0.0f;
     for (int par = 0; m < M; m += step, par ^= 1) {
-        float xh[EPT], d[EPT], s1 = 0.0f, s2 = 0.0f;
-        if constexpr (R::LEAN) {
+        const bool next = m + step < M && m + step > m;   // (past 2^32 rows: none)
+        float xh[EPT], g[EPT], s1 = 0.0f, s2 = 0.0f;
+        if (!AHEAD) {
+            ch.fresh();
             load_row(m);
-            load_params<W, T, WAVES, EPT>(w, t, N, 1.0f, wv);
         }
-        const float r = rs;
+        const float r = rs, mr = mu;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             unpack<T>(rx[i], xh + i * VEC);
-            unpack<T>(rd[i], d + i * VEC);
+            unpack<T>(rd[i], g + i * VEC);
+            if (!ch.whole) ch.own(i, g + i * VEC);   // 0: adds to no sum
         }
+        if (AHEAD && next) load_row(m + step);
 #pragma unroll
-        for (int i = 0; i < EPT; ++i) xh[i] = (xh[i] - mu) * r;
-        if constexpr (!R::LEAN)
-            if (m + step < M && m + step > m) load_row(m + step);
+        for (int i = 0; i < NV; ++i) {
+            float wi[VEC];
+            wv.get(i, wi);
 #pragma unroll
-        for (int i = 0; i < EPT; ++i) {
-            const float g = d[i] * wv[i];
-            s1 += g;
-            s2 += g * xh[i];
-            dw[i] += d[i] * xh[i];
-            db[i] += d[i];
+            for (int e = 0; e < VEC; ++e) {
+                const int k = i * VEC + e;
+                xh[k] = (xh[k] - mr) * r;
+                dw[k] += g[k] * xh[k];
+                db[k] += g[k];
+                g[k] *= wi[e];
+                s1 += g[k];
+                s2 += g[k] * xh[k];
+            }
+            if (MAP == MANY) __builtin_amdgcn_sched_barrier(0);   // one chunk's temporaries at a time
         }
         if (dx) {
             s1 = wave_sum(s1);
             s2 = wave_sum(s2);
-            if constexpr (WAVES > 1) {
-                if ((threadIdx.x & 63) == 0) {
-                    sh[par][threadIdx.x >> 6][0] = s1;
-                    sh[par][threadIdx.x >> 6][1] = s2;
-                }
+            if constexpr (MAP != ONE) {
+                if ((threadIdx.x & 63) == 0) sh[par][threadIdx.x >> 6] = float2{s1, s2};
                 __syncthreads();
                 s1 = s2 = 0.0f;
-#pragma unroll
-                for (int i = 0; i < WAVES; ++i) {
-                    s1 += sh[par][i][0];
-                    s2 += sh[par][i][1];
+                for (int i = 0; i < tpr >> 6; ++i) {
+                    s1 += sh[par][i].x;
+                    s2 += sh[par][i].y;
                 }
             }
             s1 /= (float)N;
@@ -224,30 +330,60 @@ __global__ __launch_bounds__((RowMap<T, WAVES, EPT>::THREADS)) void layer_norm_b
             for (int i = 0; i < NV; ++i) {
                 float o[VEC];
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const int k = i * VEC + e;
-                    o[e] = r * (d[k] * wv[k] - s1 - xh[k] * s2);
-                }
-                st_chunk(dx + (int64_t)m * lddx, (int64_t)(t + i * R::TPR) * VEC, N, pack<T>(o));
+                for (int e = 0; e < VEC; ++e) o[e] = r * (g[i * VEC + e] - s1 - xh[i * VEC + e] * s2);
+                ch.store(i, dx + (int64_t)m * lddx, pack<T>(o));
+                if (MAP == MANY) __builtin_amdgcn_sched_barrier(0);
             }
         }
-        if (m + step < m) break;   // past 2^32 rows
+        if (!next) break;
+    }
+    if constexpr (MAP == ONE) {
+        // the four waves' sums, in their order
+        __shared__ float sums[2][EPT][64];
+        for (uint32_t k = 1; k < R::RPB; ++k) {
+            __syncthreads();
+            if (sub == k)
+#pragma unroll
+                for (int i = 0; i < EPT; ++i) {
+                    sums[0][i][t] = dw[i];
+                    sums[1][i][t] = db[i];
+                }
+            __syncthreads();
+            if (sub == 0)
+#pragma unroll
+                for (int i = 0; i < EPT; ++i) {
+                    dw[i] += sums[0][i][t];
+                    db[i] += sums[1][i][t];
+                }
+        }
+        if (sub) return;
     }
     if (part) {
-        float* pw = part + (int64_t)(blockIdx.x * R::RPB + sub) * 2 * N;
+        float* pw = part + (int64_t)blockIdx.x * 2 * N;
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+        for (int i = 0; i < NV; ++i) {
+            float* pi = pw + ch.off(i);
 #pragma unroll
             for (int q = 0; q < VEC; q += 4) {
-                const int64_t c = (int64_t)(t + i * R::TPR) * VEC + q;
-                st_chunk(pw, c, N, pack<float>(dw + i * VEC + q));
-                st_chunk(pw + N, c, N, pack<float>(db + i * VEC + q));
+                if (ch.from(i) <= q) {
+                    *(u32x4_any*)(pi + q) = pack<float>(dw + i * VEC + q);
+                    *(u32x4_any*)(pi + N + q) = pack<float>(db + i * VEC + q);
+                } else {
+#pragma unroll
+                    for (int e = q; e < q + 4; ++e)
+                        if (e >= ch.from(i)) {
+                            pi[e] = dw[i * VEC + e];
+                            pi[N + e] = db[i * VEC + e];
+                        }
+                }
+                if (MAP == MANY) __builtin_amdgcn_sched_barrier(0);
             }
+        }
     }
 }
 
-// Rows too long for a workgroup's registers (N > 16384): read once more for
-// each step.
+// Rows too long for a workgroup's registers (N > 16384), or shorter than a
+// chunk: read once more for each step.
 constexpr int LONG = 1024;
 
 __device__ __forceinline__ float long_sum(float v, float* sh) {
@@ -326,58 +462,62 @@ __global__ __launch_bounds__(256) void layer_norm_long_dw_kernel(uint32_t M, uin
     part[(int64_t)blockIdx.y * 2 * N + N + n] = db;
 }
 
-// dw and db from the partial rows, in their order: 16 waves take 1/16 of the
-// rows each for 64 columns, then the first adds the waves' sums in order
+// dw and db from the partial rows: of a workgroup's 64 threads per column
+// each adds the rows of 1/64 of them in order, 16 loads in flight, and the
+// sums join in a fixed tree
 template <typename G>
 __global__ __launch_bounds__(1024) void layer_norm_reduce_kernel(const float* part, uint32_t parts, uint32_t N, G* dw,
                                                                  G* db, float beta) {
-    __shared__ float sh[16][64];
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __shared__ float sh[16][16];
+    const uint32_t col = threadIdx.x & 15, slice = threadIdx.x >> 4;
     G* out = blockIdx.y ? db : dw;
     if (!out) return;
-    const uint32_t n = blockIdx.x * 64 + lane;
+    const uint32_t n = blockIdx.x * 16 + col;
     const float* src = part + (blockIdx.y ? N : 0) + n;
-    const uint32_t p0 = (uint32_t)((uint64_t)parts * wave / 16), p1 = (uint32_t)((uint64_t)parts * (wave + 1) / 16);
+    const uint32_t p0 = (uint32_t)((uint64_t)parts * slice / 64), p1 = (uint32_t)((uint64_t)parts * (slice + 1) / 64);
     float s = 0.0f;
-    if (n < N) {
-        uint32_t p = p0;
-        for (; p + 8 <= p1; p += 8) {
-            float v[8];
+    if (n < N)
+        for (uint32_t p = p0; p < p1; p += 16) {
+            float v[16];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = src[(int64_t)(p + i) * 2 * N];
+            for (int i = 0; i < 16; ++i) v[i] = p + i < p1 ? src[(int64_t)(p + i) * 2 * N] : 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s += v[i];
+            for (int i = 0; i < 16; ++i) s += v[i];
         }
-        for (; p < p1; ++p) s += src[(int64_t)p * 2 * N];
-    }
-    sh[wave][lane] = s;
+    s += __shfl_xor(s, 16);
+    s += __shfl_xor(s, 32);
+    if ((threadIdx.x & 63) < 16) sh[threadIdx.x >> 6][col] = s;
     __syncthreads();
-    if (wave || n >= N) return;
-    for (int i = 1; i < 16; ++i) s += sh[i][lane];
+    if (threadIdx.x >= 16 || n >= N) return;
+    s = sh[0][col];
+    for (int i = 1; i < 16; ++i) s += sh[i][col];
     out[n] = (G)(beta == 0.0f ? s : s + beta * (float)out[n]);
 }
 
-// Rows are held by one wave up to 1024 columns, by four up to 4096, by
-// sixteen up to LAST: 8 or 16 values a thread.
-constexpr uint32_t LAST = 16384;
+// f(map, values a thread) for rows of N columns; false: rows shorter than a
+// chunk or past a workgroup's registers
 template <typename F>
 static bool with_map(uint32_t N, F f) {
     using std::integral_constant;
-    if (N <= 512) f(integral_constant<int, 1>{}, integral_constant<int, 8>{});
-    else if (N <= 1024) f(integral_constant<int, 1>{}, integral_constant<int, 16>{});
-    else if (N <= 2048) f(integral_constant<int, 4>{}, integral_constant<int, 8>{});
-    else if (N <= 4096) f(integral_constant<int, 4>{}, integral_constant<int, 16>{});
-    else if (N <= 8192) f(integral_constant<int, 16>{}, integral_constant<int, 8>{});
-    else if (N <= LAST) f(integral_constant<int, 16>{}, integral_constant<int, 16>{});
+    if (N < 8) return false;
+    if (N <= 512) f(integral_constant<int, ONE>{}, integral_constant<int, 8>{});
+    else if (N <= 1024) f(integral_constant<int, ONE>{}, integral_constant<int, 16>{});
+    else if (N <= 2048) f(integral_constant<int, FEW>{}, integral_constant<int, 8>{});
+    else if (N <= 8192) f(integral_constant<int, FEW>{}, integral_constant<int, 16>{});
+    else if (N <= LAST) f(integral_constant<int, MANY>{}, integral_constant<int, 16>{});
     else return false;
     return true;
 }
 
-// Workgroups for M rows of N: 16 waves per CU of 256
-static uint32_t norm_blocks(uint32_t M, uint32_t waves) {
-    const uint32_t rpb = waves == 1 ? 4 : 1;
+// Workgroups for M rows: 16 waves per CU of 256, or 8 in the backward pass,
+// whose workgroups leave 8 N bytes of partial sums each.  us, bf16 with fp32
+// parameters, 4 / 8 / 12 / 16 / 24 waves: 8192 x 4096 forward 50 / 31 / 28 / 27 / 28,
+// backward 49 / 46 / 52 / 56 / 63.
+static uint32_t norm_blocks(uint32_t M, int map, uint32_t waves, bool backward) {
+    const uint32_t rpb = map == ONE ? 4 : 1;
     const uint64_t need = ((uint64_t)M + rpb - 1) / rpb;
-    const uint64_t most = 256ull * (waves == 1 ? 4 : 16 / waves);
+    const uint32_t per = (backward ? 8 : 16) / (waves * rpb);
+    const uint64_t most = 256ull * (per ? per : 1);
     return (uint32_t)(need < most ? need : most);
 }
 
@@ -404,11 +544,12 @@ extern "C" int vkb_launch_layer_norm(int type, int w_type, uint32_t M, uint32_t 
     const bool ok = with_types(type, w_type, [&](auto tt, auto tw) {
         using T = decltype(tt);
         using W = decltype(tw);
-        const bool fits = with_map(N, [&](auto waves, auto ept) {
-            using R = RowMap<T, waves.value, ept.value>;
-            hipLaunchKernelGGL((layer_norm_kernel<T, W, waves.value, ept.value>),
-                               dim3(norm_blocks(M, waves.value)), dim3(R::THREADS), 0, st, M, N, (const T*)x, ldx,
-                               (const W*)w, (const W*)b, eps, (T*)y, ldy, mean, rstd);
+        const bool fits = with_map(N, [&](auto map, auto ept) {
+            using R = RowMap<T, map.value, ept.value>;
+            const uint32_t waves = R::waves(N);
+            hipLaunchKernelGGL((layer_norm_kernel<T, W, map.value, ept.value>),
+                               dim3(norm_blocks(M, map.value, waves, false)), dim3(64 * waves * R::RPB), 0, st, M, N,
+                               (const T*)x, ldx, (const W*)w, (const W*)b, eps, (T*)y, ldy, mean, rstd);
         });
         if (!fits)
             hipLaunchKernelGGL((layer_norm_long_kernel<T, W>), dim3(M < 4096u ? M : 4096u), dim3(LONG), 0, st, M, N,
@@ -417,13 +558,13 @@ extern "C" int vkb_launch_layer_norm(int type, int w_type, uint32_t M, uint32_t 
     return ok ? (int)hipGetLastError() : (int)hipErrorInvalidValue;
 }
 
-extern "C" int vkb_layer_norm_long(uint32_t N) { return N > LAST; }
+extern "C" int vkb_layer_norm_long(uint32_t N) { return !with_map(N, [](auto, auto) {}); }
 
 extern "C" uint32_t vkb_layer_norm_parts(int type, uint32_t M, uint32_t N) {
     (void)type;
     uint32_t parts = long_slices(M);
-    with_map(N, [&](auto waves, auto ept) {
-        parts = norm_blocks(M, waves.value) * (waves.value == 1 ? 4 : 1);
+    with_map(N, [&](auto map, auto ept) {
+        parts = norm_blocks(M, map.value, RowMap<float, map.value, ept.value>::waves(N), true);
     });
     return parts;
 }
@@ -436,10 +577,12 @@ extern "C" int vkb_launch_layer_norm_backward(int type, int w_type, uint32_t M, 
     const bool ok = with_types(type, w_type, [&](auto tt, auto tw) {
         using T = decltype(tt);
         using W = decltype(tw);
-        const bool fits = with_map(N, [&](auto waves, auto ept) {
-            using R = RowMap<T, waves.value, ept.value>;
-            hipLaunchKernelGGL((layer_norm_backward_kernel<T, W, waves.value, ept.value>),
-                               dim3(norm_blocks(M, waves.value)), dim3(R::THREADS), 0, st, M, N, (const T*)dy, lddy,
+        const bool fits = with_map(N, [&](auto map, auto ept) {
+            using R = RowMap<T, map.value, ept.value>;
+            const uint32_t waves = R::waves(N);
+            hipLaunchKernelGGL((layer_norm_backward_kernel<T, W, map.value, ept.value>),
+                               dim3(norm_blocks(M, map.value, waves, true)), dim3(64 * waves * R::RPB), 0, st, M, N,
+                               (const T*)dy, lddy,
                                (const T*)x, ldx, (const W*)w, mean, rstd, (T*)dx, lddx, part);
         });
         if (fits) return;
@@ -458,7 +601,7 @@ extern "C" int vkb_launch_layer_norm_reduce(const float* part, uint32_t parts, u
                                             int g_type, float beta, void* stream) {
     const bool ok = with_type(g_type, [&](auto t) {
         using G = decltype(t);
-        hipLaunchKernelGGL((layer_norm_reduce_kernel<G>), dim3((N + 63) / 64, 2), dim3(1024), 0, (hipStream_t)stream,
+        hipLaunchKernelGGL((layer_norm_reduce_kernel<G>), dim3((N + 15) / 16, 2), dim3(1024), 0, (hipStream_t)stream,
                            part, parts, N, (G*)dw, (G*)db, beta);
     });
     return ok ? (int)hipGetLastError() : (int)hipErrorInvalidValue;

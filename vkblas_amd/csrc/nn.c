@@ -161,8 +161,16 @@ uint32_t vkb_xent_slices(const vkb_op_args* a) {
  *    16-bit types, from two steps on, and pairs of 32 for fp32; the bytes
  *    that a tile's rows span below 2^31 (offsets are 32-bit);
  *  - more than 64 rows: below that the decode kernels stream the weight;
- *  - 256 x 256 tiles where the planner of the plain products takes them:
- *    16-bit from more than 128 of them on, fp32 for about whole waves. */
+ *  - enough tiles of 128 for their K: few tiles with a long K are faster as a
+ *    product with K split and a pass over its result.  us, joined / here, gated
+ *    projection bf16: 16 tiles K = 1024 10.8 / 9.7, 4096 21.4 / 26.8; 64 tiles 512
+ *    12.0 / 7.3, 4096 25.2 / 27.2; 128 tiles 4096 33.3 / 30.1; fp32: 32 tiles K = 1024
+ *    25 / 59, 128 tiles 63.8 / 62.1, K = 4096 149 / 233, 256 tiles 269 / 244;
+ *  - 16-bit: the tile whose waves of workgroups (one 256 x 256 or two 128 x 128
+ *    per CU) take less at the rates measured, a K step of 64 1.45 and 0.83 us and
+ *    an epilogue 6 and 4 (us on 128 / 256: 2048 x 4096 x 4096 gated, one wave of 256,
+ *    107 / 94; 2048 x 5120 x 4096, 1.25 waves, 146 / 160; 1000 x 16000 x 384 29 / 34);
+ *    fp32: 256 x 256 only for about whole waves, as the plain products. */
 static int op_plan(vkblas_dtype_t type, uint32_t M, uint32_t N, uint32_t K, const void* x, uint32_t ldx,
                    const void* w, uint32_t ldw, uint32_t cols, vkb_op_args* a) {
     const uint32_t vec = type == VKBLAS_DT_F32 ? 4 : 8;
@@ -172,6 +180,17 @@ static int op_plan(vkblas_dtype_t type, uint32_t M, uint32_t N, uint32_t K, cons
         (256 * ld + K) * es >= 1ull << 31)
         return 0;
     const uint64_t t = (uint64_t)((M + 255) / 256) * ((N + cols - 1) / cols);
+    const uint64_t t128 = (uint64_t)((M + 127) / 128) * ((N + cols / 2 - 1) / (cols / 2));
+    int large;
+    if (type == VKBLAS_DT_F32) {
+        if (t128 < (K <= 2048 ? 128 : 200)) return 0;
+        large = 8 * t >= 7 * 256 * ((t + 255) / 256);
+    } else {
+        if (t128 < 96 && K > 1024 && K > 32 * t128) return 0;
+        const double w256 = t < 1024 ? (double)((t + 255) / 256) : (double)t / 256;
+        const double w128 = t128 < 2048 ? (double)((t128 + 511) / 512) : (double)t128 / 512;
+        large = t > 128 && w256 * (1.45 * K / 64 + 6) <= w128 * (0.83 * K / 64 + 4);
+    }
     a->x = x;
     a->w = w;
     a->ldx = ldx;
@@ -180,7 +199,7 @@ static int op_plan(vkblas_dtype_t type, uint32_t M, uint32_t N, uint32_t K, cons
     a->N = N;
     a->K = K;
     a->type = type;
-    a->tile = (type == VKBLAS_DT_F32 ? 8 * t >= 7 * 256 * ((t + 255) / 256) : t > 128) ? VKB_TILE_256 : VKB_TILE_128;
+    a->tile = large ? VKB_TILE_256 : VKB_TILE_128;
     return 1;
 }
 

@@ -61,15 +61,31 @@ __device__ __forceinline__ void st_chunk(T* row, int64_t n, int64_t N, u32x4 v) 
     }
 }
 
+// Reductions over a wave in a fixed order, the result in every lane: four
+// shifts within each row of 16 lanes, the last lanes of rows 0 and 2 to rows 1
+// and 3, then that of row 1 to rows 2 and 3.  As DPP operands of the additions
+// (about 8 instructions; through LDS permutes they were a third of a layer
+// norm row's instructions).
+template <int CTRL, int ROWS, typename F>
+__device__ __forceinline__ float dpp_step(float v, float none, F f) {
+    const int o = __builtin_amdgcn_update_dpp(__float_as_int(none), __float_as_int(v), CTRL, ROWS, 0xf, false);
+    return f(v, __int_as_float(o));
+}
+template <typename F>
+__device__ __forceinline__ float wave_reduce(float v, float none, F f) {
+    v = dpp_step<0x111, 0xf>(v, none, f);
+    v = dpp_step<0x112, 0xf>(v, none, f);
+    v = dpp_step<0x114, 0xf>(v, none, f);
+    v = dpp_step<0x118, 0xf>(v, none, f);
+    v = dpp_step<0x142, 0xa>(v, none, f);
+    v = dpp_step<0x143, 0xc>(v, none, f);
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
 __device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
-    return v;
+    return wave_reduce(v, 0.0f, [](float a, float b) { return a + b; });
 }
 __device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
-    return v;
+    return wave_reduce(v, -INFINITY, [](float a, float b) { return fmaxf(a, b); });
 }
 
 constexpr float LOG2E = 1.4426950408889634f;

@@ -6,15 +6,29 @@
 
 namespace vkb {
 
-template <typename T, typename OP, int WT>
+template <typename T, typename OP, int WT, int NST = 2>
 static int launch_op(typename OP::Params p, hipStream_t st) {
     constexpr int BM = 2 * WT, BN = OP::GATED ? WT : 2 * WT;
     p.tiles_m = (p.M + BM - 1) / BM;
     p.tiles_n = (p.N + BN - 1) / BN;
     const uint64_t grid = (uint64_t)p.tiles_m * p.tiles_n;
     if (grid > 0xffffffffull / 256) return (int)hipErrorInvalidValue;
-    hipLaunchKernelGGL((gemm_pipe_kernel<T, T, true, true, WT, 2, OP>), dim3((uint32_t)grid), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((gemm_pipe_kernel<T, T, true, true, WT, NST, OP>), dim3((uint32_t)grid), dim3(256), 0, st, p);
     return (int)hipGetLastError();
+}
+
+// The tile of a->tile; 128 x 128 ones of 16-bit operands with four LDS stages
+// where the grid is at most one workgroup per CU (their 144 KB allow no
+// second; the loads of three K steps in flight instead of one).
+template <typename T, typename OP>
+static int launch_tiles(const vkb_op_args* a, const typename OP::Params& p, hipStream_t st) {
+    if (a->tile == VKB_TILE_256) return launch_op<T, OP, 128>(p, st);
+    if constexpr (sizeof(T) == 2) {
+        const uint64_t cols = OP::GATED ? 64 : 128;
+        const uint64_t grid = (uint64_t)((p.M + 127) / 128) * ((p.N + cols - 1) / cols);
+        if (grid <= 256 && (p.K == 128 || p.K >= 256)) return launch_op<T, OP, 64, 4>(p, st);
+    }
+    return launch_op<T, OP, 64>(p, st);
 }
 
 template <typename T, typename P>
@@ -43,7 +57,7 @@ static int launch_glu(const vkb_op_args* a, int act_code, void* h, int64_t ldh, 
     int rc = (int)hipErrorInvalidValue;
     with_act(act_code, [&](auto act) {
         using OP = GluOp<T, decltype(act)::value>;
-        rc = a->tile == VKB_TILE_256 ? launch_op<T, OP, 128>(p, st) : launch_op<T, OP, 64>(p, st);
+        rc = launch_tiles<T, OP>(a, p, st);
     });
     return rc;
 }
@@ -54,8 +68,7 @@ static int launch_xent_stats(const vkb_op_args* a, const int64_t* target, float*
     p.target = target;
     p.parts = (float2*)parts;
     p.zt = zt;
-    using OP = XentStatsOp<T>;
-    return a->tile == VKB_TILE_256 ? launch_op<T, OP, 128>(p, st) : launch_op<T, OP, 64>(p, st);
+    return launch_tiles<T, XentStatsOp<T>>(a, p, st);
 }
 
 template <typename T>
@@ -74,8 +87,7 @@ static int launch_xent_grad(const vkb_op_args* a, uint32_t Ms, uint32_t Ns, uint
     p.scal = scal;
     p.C = D;
     p.ldc = ldd;
-    using OP = XentGradOp<T>;
-    return a->tile == VKB_TILE_256 ? launch_op<T, OP, 128>(p, st) : launch_op<T, OP, 64>(p, st);
+    return launch_tiles<T, XentGradOp<T>>(a, p, st);
 }
 
 }  // namespace vkb

@@ -75,28 +75,41 @@ __global__ __launch_bounds__(THREADS) void xent_stats_kernel(uint32_t M, uint32_
     }
 }
 
-// 16 rows x 16 lanes per workgroup: lane j of a row joins slices j, j + 16, ..
+// FROWS rows per workgroup of 256, 256 / FROWS threads each: thread j of a row
+// joins slices j, j + 256 / FROWS, .., eight loads in flight; then the threads'
+// pairs join in LDS.
+constexpr int FROWS = 8, FSLICES = THREADS / FROWS;
 __global__ __launch_bounds__(THREADS) void xent_finish_kernel(uint32_t M, uint32_t V, uint32_t S, const float2* parts,
                                                               const float* zt, const int64_t* target, int64_t ignore,
                                                               float* loss, float* lse) {
-    __shared__ float2 sh[16][17];
-    const uint32_t r = threadIdx.x & 15, j = threadIdx.x >> 4;
-    const uint32_t m = blockIdx.x * 16 + r;
+    __shared__ float2 sh[FSLICES][FROWS + 1];
+    const uint32_t r = threadIdx.x % FROWS, j = threadIdx.x / FROWS;
+    const uint32_t m = blockIdx.x * FROWS + r;
     float top = -INFINITY, s = 0.0f;
     if (m < M)
-        for (uint32_t i = j; i < S; i += 16) {
-            const float2 p = parts[(int64_t)i * M + m];
-            const float t = fmaxf(top, p.x), off = finite_or_0(t);
-            s = s * fast_exp(top - off) + p.y * fast_exp(p.x - off);
+        for (uint32_t i = j; i < S; i += 8 * FSLICES) {
+            float2 p[8];
+            float t = top;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const uint32_t c = i + k * FSLICES;
+                p[k] = c < S ? parts[(int64_t)c * M + m] : float2{-INFINITY, 0.0f};
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) t = fmaxf(t, p[k].x);
+            const float off = finite_or_0(t);
+            s *= fast_exp(top - off);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) s += p[k].y * fast_exp(p[k].x - off);
             top = t;
         }
     sh[j][r] = float2{top, s};
     __syncthreads();
     if (j || m >= M) return;
-    for (uint32_t i = 1; i < 16; ++i) top = fmaxf(top, sh[i][r].x);
+    for (uint32_t i = 1; i < FSLICES; ++i) top = fmaxf(top, sh[i][r].x);
     const float off = finite_or_0(top);
     s = 0.0f;
-    for (uint32_t i = 0; i < 16; ++i) s += sh[i][r].y * fast_exp(sh[i][r].x - off);
+    for (uint32_t i = 0; i < FSLICES; ++i) s += sh[i][r].y * fast_exp(sh[i][r].x - off);
     const float l = off + logf(s);
     lse[m] = l;
     if (loss) {
@@ -169,8 +182,9 @@ extern "C" int vkb_launch_xent_stats(uint32_t M, uint32_t n, uint32_t v0, const 
 
 extern "C" int vkb_launch_xent_finish(uint32_t M, uint32_t V, uint32_t S, const float* parts, const float* zt,
                                       const int64_t* target, int64_t ignore, float* loss, float* lse, void* stream) {
-    // 2^31 rows / 16 per workgroup: below 2^32 threads
-    hipLaunchKernelGGL(xent_finish_kernel, dim3((uint32_t)(((uint64_t)M + 15) / 16)), dim3(THREADS), 0,
+    const uint64_t groups = ((uint64_t)M + FROWS - 1) / FROWS;
+    if (groups > 0xffffffffull / THREADS) return (int)hipErrorInvalidValue;
+    hipLaunchKernelGGL(xent_finish_kernel, dim3((uint32_t)groups), dim3(THREADS), 0,
                        (hipStream_t)stream, M, V, S, (const float2*)parts, zt, target, ignore, loss, lse);
     return (int)hipGetLastError();
 }
