@@ -60,8 +60,8 @@ vkblas_status_t vkblas_layer_norm_async(
  *   w: NULL = ones; mean, rstd: as the forward pass wrote them
  *   dx, dw, db: each NULL or computed; dw, db of g_type (w_type or F32)
  * dx may be dy or x.  Sums over rows run in an order that depends on M and N
- * alone: equal calls give equal bits.  Needs a workspace when dw or db is
- * wanted.
+ * alone: equal calls give equal bits.  Needs a workspace when dw or db of more
+ * than 256 rows is wanted.
  */
 vkblas_status_t vkblas_layer_norm_backward_async(
     vkblas_dtype_t type, vkblas_dtype_t w_type,

@@ -46,9 +46,9 @@ class Buf:
     def ptr(self):
         return self.all.data_ptr() + self.off * self.all.element_size()
 
-    def get(self):
+    def get(self, device="cpu"):
         torch.cuda.synchronize()
-        return self.t.double().cpu()
+        return self.t.double().to(device)
 
     def check_around(self):
         """Nothing was written outside the matrix."""
@@ -65,6 +65,7 @@ def values(rows, cols, dt, seed, scale=1.0):
 
 
 def close(got, ref, bound, what):
+    got = got.to(ref.device)
     bad = ~((got - ref).abs() <= bound)
     if bool(bad.any()):
         i = int(torch.argmax(((got - ref).abs() / (bound + 1e-300)).nan_to_num(nan=float("inf")).flatten()))

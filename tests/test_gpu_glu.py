@@ -172,3 +172,73 @@ def test_empty_batch():
                               0, beta, stream=stream())
         assert bool((dw.get() == want).all())
     dw.check_around()
+
+
+# sizes whose work is worth copies of the operands: K in no 16-byte units, M and N in no whole steps, together
+# and alone; a misaligned x or w alone; the references in float64 on the GPU
+LARGE = [(300, 600, 1501), (1100, 1001, 1003), (1030, 2051, 512), (1100, 1024, 1000), (129, 4099, 2048)]
+
+
+@pytest.mark.parametrize("M,N,K", LARGE)
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+def test_padded_operands(M, N, K, dt):
+    x, w = R.values(M, K, dt, 60).cuda(), R.values(2 * N, K, dt, 61, K ** -0.5).cuda()
+    check_forward(forward(x, w, dt, "silu"), x, w, dt, "silu")
+    assert (vk.last_kernel() == vk.KERNEL_FUSED) == (N != 600)   # few tiles with a long K are joined
+    dh = R.values(M, N, dt, 62, 0.1).cuda()
+    args = (dh, (x @ w.t()).to(R.TORCH[dt]).double(), x, w)
+    dw0 = R.values(2 * N, K, "f32", 63).cuda()
+    for kw in (dict(want="xw"), dict(), dict(want="xw", wt="f32", beta=0.5, dw0=dw0), dict(want="xw", pad=3, off=1)):
+        check_backward(backward(*args, dt, "silu", **kw), *args, dt, "silu",
+                       **{k: v for k, v in kw.items() if k in ("wt", "beta", "dw0", "want")})
+
+
+def test_offsets_past_32_bits():
+    """gu of 2.2e9 elements: the last rows and columns are right."""
+    M, N, K = 70000, 16000, 128
+    x, w = torch.randn(M, K, device="cuda").bfloat16(), (torch.randn(2 * N, K, device="cuda") * K ** -0.5).bfloat16()
+    h, gu = (torch.empty(M, c, device="cuda", dtype=torch.bfloat16) for c in (N, 2 * N))
+    vk.glu_async(vk.DT_BF16, vk.ACT_SILU, M, N, K, x.data_ptr(), K, w.data_ptr(), K, h.data_ptr(), N, gu.data_ptr(),
+                 2 * N, stream=stream())
+    for rows in (slice(0, 3), slice(M - 3, M)):
+        check_forward((h[rows].double(), gu[rows].double()), x[rows].double(), w.double(), "bf16", "silu")
+    dh = torch.randn(M, N, device="cuda").bfloat16()
+    dx = torch.empty(M, K, device="cuda", dtype=torch.bfloat16)
+    vk.glu_backward_async(vk.DT_BF16, vk.ACT_SILU, M, N, K, dh.data_ptr(), N, gu.data_ptr(), 2 * N, None, 0,
+                          w.data_ptr(), K, gu.data_ptr(), 2 * N, dx.data_ptr(), K, None, 0, vk.DT_BF16, 0.0,
+                          stream=stream())
+    # dgu took gu's place: what it was, from x again
+    for rows in (slice(0, 3), slice(M - 3, M)):
+        pre = (x[rows].double() @ w.double().t()).bfloat16().double()
+        check_backward((dx[rows].double(), None, gu[rows].double()), dh[rows].double(), pre, x[rows].double(),
+                       w.double(), "bf16", "silu", want="x")
+
+
+def test_graph_capture_and_workspace():
+    """A fused forward pass needs no workspace: captured and replayed, equal to the eager result each time.  A
+    backward pass without dgu needs one: refused under capture, nothing launched."""
+    M, N, K = 300, 200, 256
+    x, w = (torch.randn(r, K, device="cuda").half() for r in (M, 2 * N))
+    h, gu, dx = (torch.zeros(M, c, device="cuda", dtype=torch.half) for c in (N, 2 * N, K))
+
+    def call(s):
+        return vk.glu_async(vk.DT_F16, vk.ACT_GELU, M, N, K, x.data_ptr(), K, w.data_ptr(), K, h.data_ptr(), N,
+                            gu.data_ptr(), 2 * N, stream=s)
+    call(stream())
+    torch.cuda.synchronize()
+    eager = h.clone()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        call(stream())
+        st = vk.glu_backward_async(vk.DT_F16, vk.ACT_GELU, M, N, K, h.data_ptr(), N, gu.data_ptr(), 2 * N, x.data_ptr(),
+                                   K, w.data_ptr(), K, None, 0, dx.data_ptr(), K, None, 0, vk.DT_F16, 0.0,
+                                   stream=stream(), check=False)
+    assert st == vk.ERR_INIT
+    for _ in range(3):
+        h.zero_()
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(h, eager)
+        call(stream())
+    assert not dx.any()

@@ -45,7 +45,7 @@ def check_forward(got, x, w, b, dt, eps=EPS):
 
 
 SIZES = [(1, 1), (3, 7), (3, 8), (5, 9), (2, 15), (5, 64), (2, 511), (9, 512), (4, 513), (6, 1000), (3, 1024), (2, 1025), (5, 2047), (2, 2048),
-         (3, 4096), (2, 4097), (3, 5003), (2, 8192), (2, 9001), (1, 16384), (2, 16385), (2, 40000), (1500, 96),
+         (3, 4096), (2, 4097), (3, 5003), (2, 8192), (2, 9001), (1, 16384), (2, 16385), (2, 40000), (1500, 96), (256, 200), (257, 200),
          (4500, 40), (1100, 1100), (300, 5000)]
 
 
@@ -199,3 +199,56 @@ def test_side_stream():
         z = y * 2
     s.synchronize()
     check_forward((z.cpu().double() / 2, mean.cpu().double(), rstd.cpu().double()), x, None, None, "f32")
+
+
+def test_offsets_past_32_bits():
+    """2.2e9 elements: the last rows and the sums over all of them."""
+    M, N = 140000, 16000
+    x = torch.randn(M, N, device="cuda", dtype=torch.bfloat16)
+    y = torch.empty_like(x)
+    mean, rstd = torch.empty(M, device="cuda"), torch.empty(M, device="cuda")
+    vk.layer_norm_async(vk.DT_BF16, 0, M, N, x.data_ptr(), N, None, None, EPS, y.data_ptr(), N, mean.data_ptr(),
+                        rstd.data_ptr(), stream=stream())
+    end = slice(M - 3, M)
+    check_forward([v[end].double().cpu() for v in (y, mean, rstd)], x[end].double().cpu(), None, None, "bf16")
+    dw, db = torch.empty(N, device="cuda"), torch.empty(N, device="cuda")
+    dx = torch.empty_like(x)
+    vk.layer_norm_backward_async(vk.DT_BF16, 0, M, N, y.data_ptr(), N, x.data_ptr(), N, None, mean.data_ptr(),
+                                 rstd.data_ptr(), dx.data_ptr(), N, dw.data_ptr(), db.data_ptr(), 0, 0.0,
+                                 stream=stream())
+    args = [v[end].double().cpu() for v in (y, x)] + [None] + [v[end].double().cpu() for v in (mean, rstd)]
+    check_backward((dx[end].double().cpu(), None, None), *args, "bf16", "f32", want="x")
+    cols = slice(N - 64, N)
+    d = y[:, cols].double()
+    ref = (d * (x[:, cols].double() - mean[:, None]) * rstd[:, None]).sum(0)
+    assert torch.allclose(dw[cols].double(), ref, rtol=1e-4) and torch.allclose(db[cols].double(), d.sum(0), atol=0.5)
+
+
+def test_graph_capture():
+    """The forward pass needs no workspace: captured, replayed with eager work between, equal each time; the
+    backward pass's sums need one: refused, nothing launched."""
+    x = torch.randn(300, 3000, device="cuda")
+    y, dx = torch.zeros_like(x), torch.zeros_like(x)
+    mean, rstd, dw = torch.zeros(300, device="cuda"), torch.zeros(300, device="cuda"), torch.zeros(3000, device="cuda")
+
+    def call():
+        vk.layer_norm_async(0, 0, 300, 3000, x.data_ptr(), 3000, None, None, EPS, y.data_ptr(), 3000, mean.data_ptr(),
+                            rstd.data_ptr(), stream=stream())
+    call()
+    torch.cuda.synchronize()
+    eager = y.clone()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        call()
+        st = vk.layer_norm_backward_async(0, 0, 300, 3000, x.data_ptr(), 3000, x.data_ptr(), 3000, None,
+                                          mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), 3000, dw.data_ptr(), None, 0,
+                                          stream=stream(), check=False)
+    assert st == vk.ERR_INIT
+    for _ in range(3):
+        y.zero_()
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, eager)
+        call()
+    assert not dx.any() and not dw.any()

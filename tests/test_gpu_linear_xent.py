@@ -15,13 +15,13 @@ def stream():
     return torch.cuda.current_stream().cuda_stream
 
 
-def inputs(M, V, K, dt, seed=1, scale=2.0):
+def inputs(M, V, K, dt, seed=1, scale=2.0, device="cpu"):
     x, w = R.values(M, K, dt, seed), R.values(V, K, dt, seed + 1, scale * K ** -0.5)
     g = torch.Generator().manual_seed(seed + 2)
     t = torch.randint(0, V, (M,), generator=g)
     t[::5] = IGNORE
     t[0], t[-1] = 0, V - 1
-    return x, w, t
+    return x.to(device), w.to(device), t.to(device)
 
 
 def forward(x, w, t, dt, pad=0, off=0, ignore=IGNORE, want_loss=True):
@@ -44,6 +44,7 @@ def check_forward(got, x, w, t, ignore=IGNORE):
     e = ez + 600 * R.E + R.STEP * (lse.abs() + 1)
     R.close(got[1], lse, e, "lse")
     fine = ~torch.isnan(loss)
+    got = [v.to(loss.device) for v in got]
     assert torch.equal(torch.isnan(got[0]), ~fine)
     R.close(got[0][fine], loss[fine], (e + ez + 4 * R.E * z.abs().max(1).values)[fine], "loss")
     assert bool((got[0][t == ignore] == 0).all())
@@ -51,7 +52,7 @@ def check_forward(got, x, w, t, ignore=IGNORE):
 
 SIZES = [(1, 1, 1), (1, 5, 8), (1, 1000, 256), (3, 333, 72), (17, 4097, 64), (64, 515, 128), (65, 1000, 100),
          (128, 256, 128), (200, 300, 64), (256, 256, 192), (257, 1001, 128), (300, 700, 320), (511, 130, 128),
-         (100, 10007, 77), (40, 20001, 64)]
+         (100, 10007, 77), (40, 20001, 64), (3, 16384, 72), (3, 16385, 72)]
 
 
 @pytest.mark.parametrize("M,V,K", SIZES)
@@ -133,7 +134,7 @@ def check_backward(got, x, w, t, lse, dloss, dt, wt=None, beta=0.0, dw0=None, wa
     d = (p - hot) * k
     # p moves with its logit's error and with the rounding of z - lse
     ed = k.abs() * (p * (R.dot_bound(x, w.t()) + R.STEP * (1 + (z - lse[:, None]).abs())) + 4 * R.E)
-    # rounded to the type; fp16 times a power of two that puts max |dloss| in [2^13, 2^14)
+    # rounded to the type; over max |dloss|, fp16 times 2^13
     ed = ed + R.U[dt] * (d.abs() + ed) + (2.0 ** -25 * 2.0 ** -13 * float(dloss.abs().max()) if dt == "f16" else 0.0)
     if "x" in want:
         dx = d @ w
@@ -145,11 +146,11 @@ def check_backward(got, x, w, t, lse, dloss, dt, wt=None, beta=0.0, dw0=None, wa
         R.close(got[1], dw, R.rounded(dw, wt, err), "dw")
 
 
-def grad_inputs(M, V, K, dt, loss_scale=1.0):
-    x, w, t = inputs(M, V, K, dt)
+def grad_inputs(M, V, K, dt, loss_scale=1.0, device="cpu"):
+    x, w, t = inputs(M, V, K, dt, device=device)
     lse = torch.logsumexp(x @ w.t(), 1).float().double()
     dloss = (R.values(1, M, "f32", 9)[0].abs() + 0.5) * loss_scale / M
-    return x, w, t, lse, dloss.float().double()
+    return x, w, t, lse, dloss.float().double().to(device)
 
 
 @pytest.mark.parametrize("M,V,K", SIZES)
@@ -222,12 +223,73 @@ def test_empty_batch():
     dw.check_around()
 
 
+@pytest.mark.parametrize("K", [16, 128])
 @pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
-def test_pieces(dt):
-    """More rows than one piece of the vocabulary's logits holds: several pieces, a ragged last one."""
-    M, V, K = 70000, 1000, 16
-    x, w, t = inputs(M, V, K, dt)
+def test_pieces(dt, K):
+    """More rows than one piece of the vocabulary's logits (K = 16) or of their gradient holds: several pieces, a
+    ragged last one.  References in float64 on the GPU."""
+    M, V = 70000, 1000 if K == 16 else 4101
+    x, w, t = inputs(M, V, K, dt, device="cuda")
     check_forward(forward(x, w, t, dt), x, w, t)
     lse = torch.logsumexp(x @ w.t(), 1).float().double()
-    args = (x, w, t, lse, torch.full((M,), 1.0 / 64, dtype=torch.float64))
+    args = (x, w, t, lse, torch.full((M,), 1.0 / 64, dtype=torch.float64, device="cuda"))
     check_backward(backward(*args, dt), *args, dt)
+
+
+# work that is worth copies: K in no 16-byte units, classes and rows in no whole steps, together and alone
+LARGE = [(300, 2003, 1001), (1000, 10003, 512), (1025, 40000, 520), (640, 8205, 1024)]
+
+
+@pytest.mark.parametrize("M,V,K", LARGE)
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+def test_padded_operands(M, V, K, dt):
+    args = grad_inputs(M, V, K, dt, 64.0, device="cuda")
+    x, w, t = args[:3]
+    check_forward(forward(x, w, t, dt), x, w, t)
+    assert (vk.last_kernel() == vk.KERNEL_FUSED) == (M > 300 or dt != "f32")   # few tiles: joined
+    dw0 = R.values(V, K, "f32", 30, 2.0).cuda()
+    for kw in (dict(), dict(want="x"), dict(want="w"), dict(wt="f32", beta=0.5, dw0=dw0), dict(pad=3, off=1)):
+        check_backward(backward(*args, dt, **kw), *args, dt,
+                       **{k: v for k, v in kw.items() if k in ("wt", "beta", "dw0", "want")})
+
+
+def test_offsets_past_32_bits():
+    """A weight of 2.5e9 elements: statistics and gradients reach its last classes."""
+    M, V, K = 65, 600000, 4096
+    x = torch.randn(M, K, device="cuda").bfloat16()
+    w = torch.randn(V, K, device="cuda", dtype=torch.bfloat16) * 0.03
+    t = V - 1 - torch.arange(M, device="cuda")
+    loss, lse = torch.empty(M, device="cuda"), torch.empty(M, device="cuda")
+    vk.linear_xent_async(vk.DT_BF16, M, V, K, x.data_ptr(), K, w.data_ptr(), K, t.data_ptr(), IGNORE, loss.data_ptr(),
+                         lse.data_ptr(), stream=stream())
+    z = x.float() @ w.float().t()
+    want = torch.logsumexp(z.double(), 1)
+    R.close(lse.double(), want, 1e-4 * want.abs(), "lse")
+    R.close(loss.double(), want - z.gather(1, t[:, None])[:, 0], 1e-3 * want.abs(), "loss")
+    dloss = torch.ones(M, device="cuda")
+    dx, dw = torch.empty_like(x), torch.empty_like(w)
+    vk.linear_xent_backward_async(vk.DT_BF16, M, V, K, x.data_ptr(), K, w.data_ptr(), K, t.data_ptr(), IGNORE,
+                                  lse.data_ptr(), dloss.data_ptr(), dx.data_ptr(), K, dw.data_ptr(), K, vk.DT_BF16, 0.0,
+                                  stream=stream())
+    d = torch.exp(z - lse[:, None])
+    d[torch.arange(M, device="cuda"), t] -= 1
+    tail = (d[:, V - 200:].double().t() @ x.double())
+    R.close(dw[V - 200:].double(), tail, 2.0 ** -7 * (d[:, V - 200:].abs().double().t() @ x.abs().double()), "dw")
+    ref = (d @ w.float()).double()
+    R.close(dx.double(), ref, 2.0 ** -7 * ref.abs() + 1e-3 * ref.abs().max(), "dx")
+
+
+def test_workspace_under_capture():
+    """Needs a workspace: refused while the stream captures, nothing written."""
+    x, w = (torch.randn(r, 128, device="cuda").half() for r in (300, 400))
+    t, loss, lse = torch.zeros(300, dtype=torch.int64, device="cuda"), *torch.zeros(2, 300, device="cuda")
+    y = torch.zeros(4, device="cuda")
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y += 1
+        st = vk.linear_xent_async(vk.DT_F16, 300, 400, 128, x.data_ptr(), 128, w.data_ptr(), 128, t.data_ptr(), IGNORE,
+                                  loss.data_ptr(), lse.data_ptr(), stream=stream(), check=False)
+    assert st == vk.ERR_INIT
+    g.replay()
+    torch.cuda.synchronize()
+    assert not lse.any()

@@ -10,22 +10,12 @@
 namespace vkb {
 namespace {
 
-constexpr uint32_t THREADS = 256;
-
-// column blocks in x, rows in y (strided: y holds at most 65535)
-template <typename T>
-static dim3 rows_grid(uint32_t M, uint32_t N) {
-    const uint32_t per = THREADS * Elem<T>::VEC;
-    return dim3((N + per - 1) / per, M < 65535u ? M : 65535u);
-}
-
 template <typename T, int ACT>
-__global__ __launch_bounds__(THREADS) void glu_join_kernel(uint32_t M, uint32_t N, const float* z, int64_t ldz, T* h,
-                                                           int64_t ldh, T* gu, int64_t ldgu) {
+__global__ __launch_bounds__(WORK) void glu_join_kernel(uint32_t M, uint32_t N, const float* z, int64_t ldz, T* h,
+                                                        int64_t ldh, T* gu, int64_t ldgu, uint32_t chunks) {
     constexpr int VEC = Elem<T>::VEC;
-    const int64_t n = ((int64_t)blockIdx.x * THREADS + threadIdx.x) * VEC;
-    if (n >= N) return;
-    for (uint32_t m = blockIdx.y; m < M; m += gridDim.y) {
+    for_chunks(M, chunks, 0, gridDim.x, [&](uint64_t m, uint32_t c) {
+        const int64_t n = (int64_t)c * VEC;
         float g[VEC], u[VEC], r[VEC];
 #pragma unroll
         for (int q = 0; q < VEC; q += 4) {
@@ -39,39 +29,37 @@ __global__ __launch_bounds__(THREADS) void glu_join_kernel(uint32_t M, uint32_t 
             st_chunk(gu + (int64_t)m * ldgu, n, N, pack<T>(g));
             st_chunk(gu + (int64_t)m * ldgu + N, n, N, pack<T>(u));
         }
-    }
+    });
 }
 
 // dgu may be gu: a thread reads its elements before it writes them.  dG and dU
 // are Np columns each (Np >= N) on Mp rows (Mp >= M), zero past N and M.
 template <typename T, int ACT>
-__global__ __launch_bounds__(THREADS) void glu_join_backward_kernel(uint32_t M, uint32_t N, const T* dh, int64_t lddh,
-                                                                    const T* gu, int64_t ldgu, T* dgu, int64_t lddgu,
-                                                                    uint32_t Mp, uint32_t Np) {
+__global__ __launch_bounds__(WORK) void glu_join_backward_kernel(uint32_t M, uint32_t N, const T* dh, int64_t lddh,
+                                                                 const T* gu, int64_t ldgu, T* dgu, int64_t lddgu,
+                                                                 uint32_t Mp, uint32_t Np, uint32_t chunks) {
     constexpr int VEC = Elem<T>::VEC;
-    const int64_t n = ((int64_t)blockIdx.x * THREADS + threadIdx.x) * VEC;
-    if (n >= Np) return;
-    for (uint32_t m = blockIdx.y; m < Mp; m += gridDim.y) {
-        if (m >= M || n >= N) {
-            st_chunk(dgu + (int64_t)m * lddgu, n, Np, u32x4{0u, 0u, 0u, 0u});
-            st_chunk(dgu + (int64_t)m * lddgu + Np, n, Np, u32x4{0u, 0u, 0u, 0u});
-            continue;
-        }
+    for_chunks(Mp, chunks, 0, gridDim.x, [&](uint64_t m, uint32_t c) {
+        const int64_t n = (int64_t)c * VEC;
         float g[VEC], u[VEC], d[VEC];
-        unpack<T>(ld_chunk(gu + (int64_t)m * ldgu, n, N), g);
-        unpack<T>(ld_chunk(gu + (int64_t)m * ldgu + N, n, N), u);
-        unpack<T>(ld_chunk(dh + (int64_t)m * lddh, n, N), d);
+        if (m >= M || n >= N) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            float a, da;
-            act_and_slope<ACT>(g[i], a, da);
-            g[i] = d[i] * u[i] * da;
-            u[i] = d[i] * a;
+            for (int i = 0; i < VEC; ++i) g[i] = u[i] = 0.0f;
+        } else {
+            unpack<T>(ld_chunk(gu + (int64_t)m * ldgu, n, N), g);
+            unpack<T>(ld_chunk(gu + (int64_t)m * ldgu + N, n, N), u);
+            unpack<T>(ld_chunk(dh + (int64_t)m * lddh, n, N), d);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                float a, da;
+                act_and_slope<ACT>(g[i], a, da);
+                g[i] = d[i] * u[i] * da;
+                u[i] = d[i] * a;   // (columns past N read as zeros, and d = 0 gives zeros)
+            }
         }
-        // (columns past N read as zeros, and d = 0 gives zeros)
         st_chunk(dgu + (int64_t)m * lddgu, n, Np, pack<T>(g));
         st_chunk(dgu + (int64_t)m * lddgu + Np, n, Np, pack<T>(u));
-    }
+    });
 }
 
 }  // namespace
@@ -84,8 +72,9 @@ extern "C" int vkb_launch_glu_join(int type, int act_code, uint32_t M, uint32_t 
     const bool ok = with_type(type, [&](auto t) {
         using T = decltype(t);
         with_act(act_code, [&](auto a) {
-            hipLaunchKernelGGL((glu_join_kernel<T, decltype(a)::value>), rows_grid<T>(M, N), dim3(THREADS), 0,
-                               (hipStream_t)stream, M, N, z, ldz, (T*)h, ldh, (T*)gu, ldgu);
+            hipLaunchKernelGGL((glu_join_kernel<T, decltype(a)::value>), dim3(chunk_blocks(M, chunks_of<T>(N))),
+                               dim3(WORK), 0, (hipStream_t)stream, M, N, z, ldz, (T*)h, ldh, (T*)gu, ldgu,
+                               chunks_of<T>(N));
         });
     });
     return ok ? (int)hipGetLastError() : (int)hipErrorInvalidValue;
@@ -97,9 +86,9 @@ extern "C" int vkb_launch_glu_join_backward(int type, int act_code, uint32_t M, 
     const bool ok = with_type(type, [&](auto t) {
         using T = decltype(t);
         with_act(act_code, [&](auto a) {
-            hipLaunchKernelGGL((glu_join_backward_kernel<T, decltype(a)::value>), rows_grid<T>(Mp, Np), dim3(THREADS),
-                               0, (hipStream_t)stream, M, N, (const T*)dh, lddh, (const T*)gu, ldgu, (T*)dgu, lddgu,
-                               Mp, Np);
+            hipLaunchKernelGGL((glu_join_backward_kernel<T, decltype(a)::value>),
+                               dim3(chunk_blocks(Mp, chunks_of<T>(Np))), dim3(WORK), 0, (hipStream_t)stream, M, N,
+                               (const T*)dh, lddh, (const T*)gu, ldgu, (T*)dgu, lddgu, Mp, Np, chunks_of<T>(Np));
         });
     });
     return ok ? (int)hipGetLastError() : (int)hipErrorInvalidValue;

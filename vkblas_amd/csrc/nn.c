@@ -160,7 +160,9 @@ uint32_t vkb_xent_slices(const vkb_op_args* a) {
  *  - 16-byte aligned operands and leading dimensions, K in whole steps: 64 for
  *    16-bit types, from two steps on, and pairs of 32 for fp32; the bytes
  *    that a tile's rows span below 2^31 (offsets are 32-bit);
- *  - more than 64 rows: below that the decode kernels stream the weight;
+ *  - more than 64 rows, below which the decode kernels stream the weight, or
+ *    16-bit operands with K of at most 512: then one launch instead of two or
+ *    three is ahead;
  *  - enough tiles of 128 for their K: few tiles with a long K are faster as a
  *    product with K split and a pass over its result.  us, joined / here, gated
  *    projection bf16: 16 tiles K = 1024 10.8 / 9.7, 4096 21.4 / 26.8; 64 tiles 512
@@ -176,7 +178,7 @@ static int op_plan(vkblas_dtype_t type, uint32_t M, uint32_t N, uint32_t K, cons
     const uint32_t vec = type == VKBLAS_DT_F32 ? 4 : 8;
     const uint64_t es = type_size(type);
     const uint64_t ld = ldx > ldw ? ldx : ldw;
-    if (!aligned16(x) || !aligned16(w) || ldx % vec || ldw % vec || K % 64 || K < 128 || M <= 64 ||
+    if (!aligned16(x) || !aligned16(w) || ldx % vec || ldw % vec || K % 64 || K < 128 || (M <= 64 && (K > 512 || type == VKBLAS_DT_F32)) ||
         (256 * ld + K) * es >= 1ull << 31)
         return 0;
     const uint64_t t = (uint64_t)((M + 255) / 256) * ((N + cols - 1) / cols);
@@ -234,26 +236,35 @@ static void pad_to(operand* o, uint32_t Mp, uint32_t Np) {
 static void place(op_call* c, operand* o, vkblas_dtype_t t) {
     if (o->copy) o->off = buf(c, (uint64_t)o->S * o->Mp * o->Np * type_size(t));
 }
-/* after room(): the copy, and from where */
-static int bring(op_call* c, operand* o, vkblas_dtype_t t, const void* src, uint32_t lds) {
-    if (!o->copy) return 1;
+/* After room(): a call's copies, gathered by bring() and launched by brought()
+ * together with the scalars of a cross entropy's gradient (scal, or NULL). */
+typedef struct {
+    vkb_pad_job job[VKB_PAD_JOBS];
+    int n;
+} copies;
+static void bring(op_call* c, copies* j, operand* o, const void* src, uint32_t lds) {
+    if (!o->copy) return;
     void* d = at(c, o->off);
     o->p = d;
-    return step(c, vkb_launch_pad(t, o->S, o->M, o->N, src, lds, d, o->Mp, o->Np, c->stream), 0);
+    j->job[j->n++] = (vkb_pad_job){src, d, lds, o->S, o->M, o->N, o->Mp, o->Np};
+}
+static int brought(op_call* c, const copies* j, vkblas_dtype_t t, uint32_t M, const float* dloss, float beta,
+                   float* scal) {
+    return (j->n == 0 && !scal) || step(c, vkb_launch_pad(t, j->job, j->n, M, dloss, beta, scal, c->stream), 0);
 }
 
 /* K as the pipelined kernel takes it */
 static uint32_t whole_k(uint32_t K) { return K <= 128 ? 128 : (uint32_t)round_up(K, 64); }
 /* x (M x K) and w (S of N x K) for x w^T inside the pipelined kernel: copied
- * where they have to be and the product is worth it.  Below 1 GFLOP the
- * copies' launches cost more than they save. */
+ * where they have to be and the product is worth it.  Below 0.5 GFLOP the
+ * copies' launch costs more than it saves. */
 static int fusable(vkblas_dtype_t type, uint32_t M, uint32_t N, uint32_t K, operand* x, operand* w, uint32_t cols,
                    vkb_op_args* a) {
     const uint32_t Kp = whole_k(K);
     const int rx = Kp != K || off_units(type, x->p, x->ld), rw = Kp != K || off_units(type, w->p, w->ld);
     operand px = *x, pw = *w;
     if (rx || rw) {
-        if (2.0 * M * w->S * w->M * K < 1e9) return 0;
+        if (2.0 * M * w->S * w->M * K < 5e8) return 0;
         if (rx) pad_to(&px, x->Mp, Kp);
         if (rw) pad_to(&pw, w->Mp, Kp);
     }
@@ -261,6 +272,16 @@ static int fusable(vkblas_dtype_t type, uint32_t M, uint32_t N, uint32_t K, oper
     *x = px;
     *w = pw;
     return 1;
+}
+/* x and w for a joined product: copied where their rows lie off 16-byte units
+ * and the product is worth it.  Returns the product's K. */
+static uint32_t joinable(vkblas_dtype_t type, uint32_t M, uint32_t K, operand* x, operand* w) {
+    const int off = K % vec_of(type) != 0;
+    if (2.0 * M * w->S * w->M * K < 5e8) return K;
+    const uint32_t Kp = off ? whole_k(K) : K;
+    if (off || off_units(type, x->p, x->ld)) pad_to(x, x->Mp, Kp);
+    if (off || off_units(type, w->p, w->ld)) pad_to(w, w->Mp, Kp);
+    return Kp;
 }
 /* the arguments with the operands where they are now */
 static void bound(vkb_op_args* a, const operand* x, const operand* w) {
@@ -313,8 +334,19 @@ vkblas_status_t vkblas_layer_norm_backward_async(vkblas_dtype_t type, vkblas_dty
     if (!dy || !x || !mean || !rstd) return VKBLAS_ERR_PARAM;
     if (!dx && !dw && !db) return VKBLAS_OK;
     if (vkb_engine_trace()) fprintf(stderr, "[vkblas] layer_norm_backward type=%d M=%u N=%u\n", (int)type, M, N);
+    /* Up to 256 rows (a workgroup's partial sums would be one row's), dw and db
+     * come from the rows themselves, before dx, which may take their place:
+     * us, partial sums / this: 139 x 15104 bf16 21.7 / 10.3. */
+    const int few = M <= 256 && (dw || db);
+    if (few && vkb_engine_ready() &&
+        !step(&c, vkb_launch_layer_norm_few(type, M, N, dy, lddy, x, ldx, mean, rstd, dw, db, g_type, beta, stream), 1))
+        return c.st;
+    if (few && !dx) {
+        vkb_engine_ran(VKBLAS_PATH_NONE, VKBLAS_KERNEL_NORM);
+        return vkb_engine_ready() ? VKBLAS_OK : VKBLAS_ERR_INIT;
+    }
     const uint32_t parts = vkb_layer_norm_parts(type, M, N);
-    const int sums = dw || db;
+    const int sums = !few && (dw || db);
     const size_t o_part = sums ? buf(&c, (uint64_t)parts * 2 * N * sizeof(float)) : 0;
     if (room(&c) != VKBLAS_OK) return c.st;
     float* part = sums ? (float*)at(&c, o_part) : NULL;
@@ -344,7 +376,10 @@ vkblas_status_t vkblas_glu_async(vkblas_dtype_t type, vkblas_act_t act, uint32_t
         place(&c, &ox, type);
         place(&c, &ow, type);
         if (room(&c) != VKBLAS_OK) return c.st;
-        if (bring(&c, &ox, type, x, ldx) && bring(&c, &ow, type, w, ldw)) {
+        copies jobs = {.n = 0};
+        bring(&c, &jobs, &ox, x, ldx);
+        bring(&c, &jobs, &ow, w, ldw);
+        if (brought(&c, &jobs, type, 0, NULL, 0.0f, NULL)) {
             bound(&a, &ox, &ow);
             step(&c, vkb_launch_glu(&a, act, h, ldh, gu, ldgu, stream), 1);
         }
@@ -353,26 +388,32 @@ vkblas_status_t vkblas_glu_async(vkblas_dtype_t type, vkblas_act_t act, uint32_t
     /* both projections in fp32, some rows at a time, then the join; an fp32
      * gu takes them itself */
     const int direct = type == VKBLAS_DT_F32 && gu;
+    const size_t es = type_size(type);
     uint64_t rows = direct ? M : JOIN_BYTES / ((uint64_t)8 * N);
     if (rows < 64) rows = 64;
     if (rows > M) rows = M;
     const uint32_t ldz = direct ? ldgu : (uint32_t)round_up(2 * N, 4);
-    need_gemm(&c, type, VKBLAS_DT_F32, VKBLAS_OP_N, VKBLAS_OP_T, (uint32_t)rows, 2 * N, K, x, ldx, w, ldw, ldz);
-    const size_t es = type_size(type);
-    if (M % rows)
-        need_gemm(&c, type, VKBLAS_DT_F32, VKBLAS_OP_N, VKBLAS_OP_T, (uint32_t)(M % rows), 2 * N, K,
-                  (const char*)x + (M - M % rows) * ldx * es, ldx, w, ldw, ldz);
+    const uint32_t Kp = joinable(type, M, K, &ox, &ow);
+    need_gemm(&c, type, VKBLAS_DT_F32, VKBLAS_OP_N, VKBLAS_OP_T, (uint32_t)rows, 2 * N, Kp, ox.p, ox.ld, ow.p, ow.ld,
+              ldz);
+    if (M % rows)   /* (from an address that the program's x has; a copy is aligned) */
+        need_gemm(&c, type, VKBLAS_DT_F32, VKBLAS_OP_N, VKBLAS_OP_T, (uint32_t)(M % rows), 2 * N, Kp,
+                  ox.copy ? NULL : (const char*)x + (M - M % rows) * ldx * es, ox.ld, ow.p, ow.ld, ldz);
+    place(&c, &ox, type);
+    place(&c, &ow, type);
     const size_t o_z = direct ? 0 : buf(&c, rows * ldz * sizeof(float));
     if (room(&c) != VKBLAS_OK) return c.st;
-    for (uint64_t m = 0; m < M; m += rows) {
+    copies jobs = {.n = 0};
+    bring(&c, &jobs, &ox, x, ldx);
+    bring(&c, &jobs, &ow, w, ldw);
+    int ok = brought(&c, &jobs, type, 0, NULL, 0.0f, NULL);
+    for (uint64_t m = 0; ok && m < M; m += rows) {
         const uint32_t n = (uint32_t)(M - m < rows ? M - m : rows);
         float* z = direct ? (float*)gu : (float*)at(&c, o_z);
-        if (!product(&c, type, VKBLAS_DT_F32, VKBLAS_OP_N, VKBLAS_OP_T, n, 2 * N, K, host_scalars(1.0f, 0.0f),
-                     (const char*)x + m * ldx * es, ldx, w, ldw, z, ldz, direct))
-            break;
-        if (!step(&c, vkb_launch_glu_join(type, act, n, N, z, ldz, (char*)h + m * ldh * es, ldh,
-                                          direct || !gu ? NULL : (char*)gu + m * ldgu * es, ldgu, stream), 1))
-            break;
+        ok = product(&c, type, VKBLAS_DT_F32, VKBLAS_OP_N, VKBLAS_OP_T, n, 2 * N, Kp, host_scalars(1.0f, 0.0f),
+                     (const char*)ox.p + m * ox.ld * es, ox.ld, ow.p, ow.ld, z, ldz, direct) &&
+             step(&c, vkb_launch_glu_join(type, act, n, N, z, ldz, (char*)h + m * ldh * es, ldh,
+                                          direct || !gu ? NULL : (char*)gu + m * ldgu * es, ldgu, stream), 1);
     }
     return op_end(&c, VKBLAS_KERNEL_JOINED);
 }
@@ -395,13 +436,13 @@ vkblas_status_t vkblas_glu_backward_async(vkblas_dtype_t type, vkblas_act_t act,
     if (vkb_engine_trace())
         fprintf(stderr, "[vkblas] glu_backward type=%d act=%d M=%u N=%u K=%u\n", (int)type, (int)act, M, N, K);
     /* The two products as the fast kernels take them, where their work is
-     * worth the copies (from 4 GFLOP each on) and the layout of [dG | dU] is
+     * worth the copies (from 4 GFLOP each on, 2 in fp32) and the layout of [dG | dU] is
      * this call's own: K in whole 16-byte units (columns of both results), M
      * (which dw sums over) in whole pairs of K steps, and N (dx sums over both
      * halves) so that 2 N is, for an odd N from 128 rows on, else from 1024. */
     const size_t es = type_size(type);
     const uint32_t vec = vec_of(type), steps = type == VKBLAS_DT_F32 ? 64 : 128;
-    const int big = 4.0 * M * N * K >= 4e9;
+    const int big = 4.0 * M * N * K >= (type == VKBLAS_DT_F32 ? 2e9 : 4e9);
     uint32_t Mp = M, Np = N, Kp = K;
     if (big && K % vec) Kp = (uint32_t)round_up(K, vec);
     if (big && !dgu && dw && M % steps) Mp = (uint32_t)round_up(M, steps);
@@ -424,17 +465,23 @@ vkblas_status_t vkblas_glu_backward_async(vkblas_dtype_t type, vkblas_act_t act,
     const size_t o_w = pw ? buf(&c, (uint64_t)2 * Np * Kp * type_size(wt)) : 0;
     if (room(&c) != VKBLAS_OK) return c.st;
     void *d = dgu ? dgu : at(&c, o_d), *xo = px ? at(&c, o_x) : dx, *wo = pw ? at(&c, o_w) : dw;
+    copies jobs = {.n = 0};
+    bring(&c, &jobs, &ox, x, ldx);
+    bring(&c, &jobs, &ow, w, ldw);
     int ok = step(&c, vkb_launch_glu_join_backward(type, act, M, N, dh, lddh, gu, ldgu, d, ldd, Mp, Np, stream),
                   dgu != NULL) &&
-             bring(&c, &ox, type, x, ldx) && bring(&c, &ow, type, w, ldw);
+             brought(&c, &jobs, type, 0, NULL, 0.0f, NULL);
     if (ok && dx)
         ok = product(&c, type, type, VKBLAS_OP_N, VKBLAS_OP_N, M, Kp, 2 * Np, host_scalars(1.0f, 0.0f), d, ldd, ow.p,
-                     ow.ld, xo, ldxo, !px) &&
-             (!px || step(&c, vkb_launch_unpad(type, type, 1, M, K, xo, Kp, M, dx, lddx, 0.0f, stream), 1));
+                     ow.ld, xo, ldxo, !px);
     if (ok && dw)
         ok = product(&c, type, wt, VKBLAS_OP_T, VKBLAS_OP_N, 2 * Np, Kp, Mp, host_scalars(1.0f, pw ? 0.0f : beta), d,
-                     ldd, ox.p, ox.ld, wo, ldwo, !pw) &&
-             (!pw || step(&c, vkb_launch_unpad(wt, dw_type, 2, N, K, wo, Kp, Np, dw, lddw, beta, stream), 1));
+                     ldd, ox.p, ox.ld, wo, ldwo, !pw);
+    vkb_unpad_job out[2];
+    int n = 0;
+    if (px) out[n++] = (vkb_unpad_job){xo, dx, Kp, lddx, 1, M, K, M, (int)type, (int)type, 0.0f};
+    if (pw) out[n++] = (vkb_unpad_job){wo, dw, Kp, lddw, 2, N, K, Np, (int)wt, (int)dw_type, beta};
+    if (ok && n) step(&c, vkb_launch_unpad(out, n, stream), 1);
     return op_end(&c, VKBLAS_KERNEL_JOINED);
 }
 
@@ -468,7 +515,10 @@ vkblas_status_t vkblas_linear_xent_async(vkblas_dtype_t type, uint32_t M, uint32
         const size_t o_p = buf(&c, (uint64_t)S * M * 2 * sizeof(float)), o_t = buf(&c, (uint64_t)M * sizeof(float));
         if (room(&c) != VKBLAS_OK) return c.st;
         float *parts = at(&c, o_p), *zt = at(&c, o_t);
-        if (bring(&c, &ox, type, x, ldx) && bring(&c, &ow, type, w, ldw)) {
+        copies jobs = {.n = 0};
+        bring(&c, &jobs, &ox, x, ldx);
+        bring(&c, &jobs, &ow, w, ldw);
+        if (brought(&c, &jobs, type, 0, NULL, 0.0f, NULL)) {
             bound(&a, &ox, &ow);
             if (step(&c, vkb_launch_xent_stats_op(&a, target, parts, zt, stream), 0))
                 step(&c, vkb_launch_xent_finish(M, V, S, parts, zt, target, ignore_index, loss, lse, stream), 1);
@@ -479,23 +529,31 @@ vkblas_status_t vkblas_linear_xent_async(vkblas_dtype_t type, uint32_t M, uint32
     const uint32_t last = V % n;
     const uint32_t per = (n + VKB_XENT_SLICE - 1) / VKB_XENT_SLICE;   /* slices of a piece; the last may have fewer */
     const uint32_t S = V / n * per + (last + VKB_XENT_SLICE - 1) / VKB_XENT_SLICE;
-    need_gemm(&c, type, VKBLAS_DT_F32, VKBLAS_OP_N, VKBLAS_OP_T, M, n, K, x, ldx, w, ldw, ldz);
-    if (last) need_gemm(&c, type, VKBLAS_DT_F32, VKBLAS_OP_N, VKBLAS_OP_T, M, last, K, x, ldx, w, ldw, ldz);
+    const int rows = n == V && V <= VKB_XENT_ROW;                     /* one kernel for a row's statistics and loss */
+    const uint32_t Kp = joinable(type, M, K, &ox, &ow);
+    need_gemm(&c, type, VKBLAS_DT_F32, VKBLAS_OP_N, VKBLAS_OP_T, M, n, Kp, ox.p, ox.ld, ow.p, ow.ld, ldz);
+    if (last) need_gemm(&c, type, VKBLAS_DT_F32, VKBLAS_OP_N, VKBLAS_OP_T, M, last, Kp, ox.p, ox.ld, ow.p, ow.ld, ldz);
+    place(&c, &ox, type);
+    place(&c, &ow, type);
     const size_t o_z = buf(&c, (uint64_t)M * ldz * sizeof(float));
     const size_t o_p = buf(&c, (uint64_t)S * M * 2 * sizeof(float));
     const size_t o_t = buf(&c, (uint64_t)M * sizeof(float));
     if (room(&c) != VKBLAS_OK) return c.st;
     float *z = at(&c, o_z), *parts = at(&c, o_p), *zt = at(&c, o_t);
-    int ok = 1;
+    copies jobs = {.n = 0};
+    bring(&c, &jobs, &ox, x, ldx);
+    bring(&c, &jobs, &ow, w, ldw);
+    int ok = brought(&c, &jobs, type, 0, NULL, 0.0f, NULL);
     uint32_t slice = 0;
     for (uint64_t v = 0; ok && v < V; v += n, slice += per) {
         const uint32_t cols = (uint32_t)(V - v < n ? V - v : n);
-        ok = product(&c, type, VKBLAS_DT_F32, VKBLAS_OP_N, VKBLAS_OP_T, M, cols, K, host_scalars(1.0f, 0.0f), x, ldx,
-                     (const char*)w + v * ldw * type_size(type), ldw, z, ldz, 0) &&
-             step(&c, vkb_launch_xent_stats(M, cols, (uint32_t)v, z, ldz, target, parts + (uint64_t)slice * M * 2, zt,
-                                            stream), 0);
+        ok = product(&c, type, VKBLAS_DT_F32, VKBLAS_OP_N, VKBLAS_OP_T, M, cols, Kp, host_scalars(1.0f, 0.0f), ox.p,
+                     ox.ld, (const char*)ow.p + v * ow.ld * type_size(type), ow.ld, z, ldz, 0) &&
+             (rows ? step(&c, vkb_launch_xent_rows(M, V, z, ldz, target, ignore_index, loss, lse, stream), 1)
+                   : step(&c, vkb_launch_xent_stats(M, cols, (uint32_t)v, z, ldz, target,
+                                                    parts + (uint64_t)slice * M * 2, zt, stream), 0));
     }
-    if (ok) step(&c, vkb_launch_xent_finish(M, V, S, parts, zt, target, ignore_index, loss, lse, stream), 1);
+    if (ok && !rows) step(&c, vkb_launch_xent_finish(M, V, S, parts, zt, target, ignore_index, loss, lse, stream), 1);
     return op_end(&c, VKBLAS_KERNEL_JOINED);
 }
 
@@ -574,9 +632,13 @@ vkblas_status_t vkblas_linear_xent_backward_async(vkblas_dtype_t type, uint32_t 
     if (room(&c) != VKBLAS_OK) return c.st;
     float *z = at(&c, o_z), *scal = f32 ? NULL : (float*)at(&c, o_s);
     void *d = at(&c, o_d), *xo = acc ? at(&c, o_x) : dx, *wo = at(&c, o_w);
-    int ok = (!scal || step(&c, vkb_launch_xent_scale(type, M, dloss, beta, scal, stream), 0)) &&
-             bring(&c, &ox, type, x, ldx) && bring(&c, &ow, type, w, ldw) &&
-             (!rest || !dx || bring(&c, &tail, type, (const char*)w + (uint64_t)(V - rest) * ldw * es, ldw));
+    copies jobs = {.n = 0};
+    bring(&c, &jobs, &ox, x, ldx);
+    bring(&c, &jobs, &ow, w, ldw);
+    if (rest && dx) bring(&c, &jobs, &tail, (const char*)w + (uint64_t)(V - rest) * ldw * es, ldw);
+    int ok = brought(&c, &jobs, type, M, dloss, beta, scal);
+    vkb_unpad_job out[2];        /* dw's rows still in the workspace, and dx */
+    int outs = 0;
     int summed = 0;              /* dx holds a product already */
     for (uint64_t v = 0; ok && v < V;) {
         const uint32_t cols = (uint32_t)(V - v < n ? V - v : n);
@@ -606,10 +668,14 @@ vkblas_status_t vkblas_linear_xent_backward_async(vkblas_dtype_t type, uint32_t 
                 const scalars sw = {1.0f, by_ws ? 0.0f : beta, scal ? scal + 1 : NULL,
                                     scal ? scal + (by_ws ? 4 : 2) : NULL};
                 char* to = dwv + (t ? (uint64_t)main * lddw * type_size(dw_type) : 0);
-                ok = product(&c, type, by_ws ? wt : dw_type, VKBLAS_OP_T, VKBLAS_OP_N, by_ws ? sum : rows, Kp, Mp, sw,
-                             dt, ldd, ox.p, ox.ld, by_ws ? wo : to, by_ws ? Kp : lddw, !by_ws) &&
-                     (!by_ws || step(&c, vkb_launch_unpad(wt, dw_type, 1, rows, K, wo, Kp, rows, to, lddw, beta,
-                                                          stream), 1));
+                if (by_ws && outs) {   /* the workspace's rows make room */
+                    ok = step(&c, vkb_launch_unpad(out, outs, stream), 1);
+                    outs = 0;
+                }
+                ok = ok && product(&c, type, by_ws ? wt : dw_type, VKBLAS_OP_T, VKBLAS_OP_N, by_ws ? sum : rows, Kp, Mp, sw,
+                             dt, ldd, ox.p, ox.ld, by_ws ? wo : to, by_ws ? Kp : lddw, !by_ws);
+                if (by_ws)
+                    out[outs++] = (vkb_unpad_job){wo, to, Kp, lddw, 1, rows, K, rows, (int)wt, (int)dw_type, beta};
             }
             if (ok && dx) {
                 const scalars sx = {1.0f, summed ? 1.0f : 0.0f, scal ? scal + 1 : NULL,
@@ -621,7 +687,7 @@ vkblas_status_t vkblas_linear_xent_backward_async(vkblas_dtype_t type, uint32_t 
         }
         v += cols;
     }
-    if (ok && acc)
-        step(&c, vkb_launch_unpad(VKBLAS_DT_F32, type, 1, M, K, xo, ldxo, M, dx, lddx, 0.0f, stream), 1);
+    if (acc) out[outs++] = (vkb_unpad_job){xo, dx, ldxo, lddx, 1, M, K, M, VKB_T_F32, (int)type, 0.0f};
+    if (ok && outs) step(&c, vkb_launch_unpad(out, outs, stream), 1);
     return op_end(&c, fused ? VKBLAS_KERNEL_FUSED : VKBLAS_KERNEL_JOINED);
 }

@@ -128,6 +128,33 @@ __device__ __forceinline__ void act_and_slope(float g, float& a, float& da) {
     }
 }
 
+// f(row, 16-byte chunk of the row) for rows of `chunks` chunks each, over the
+// workgroups first .. first + blocks - 1 of WORK threads
+constexpr uint32_t WORK = 256;
+template <typename F>
+__device__ __forceinline__ void for_chunks(uint64_t rows, uint32_t chunks, uint32_t first, uint32_t blocks, F f) {
+    const uint64_t total = rows * chunks;
+    const uint32_t step = blocks * WORK, start = (blockIdx.x - first) * WORK + threadIdx.x;
+    if (total + step <= 0xffffffffull) {
+        for (uint32_t i = start; i < (uint32_t)total; i += step) {
+            const uint32_t r = i / chunks;
+            f((uint64_t)r, i - r * chunks);
+        }
+    } else {
+        for (uint64_t i = start; i < total; i += step) {
+            const uint64_t r = i / chunks;
+            f(r, (uint32_t)(i - r * chunks));
+        }
+    }
+}
+// ... its workgroups: one chunk a thread, up to 32 per CU of 256
+static inline uint32_t chunk_blocks(uint64_t rows, uint32_t chunks) {
+    const uint64_t b = (rows * chunks + WORK - 1) / WORK;
+    return (uint32_t)(b < 8192 ? b : 8192);
+}
+template <typename T>
+static inline uint32_t chunks_of(uint32_t N) { return (N + Elem<T>::VEC - 1) / Elem<T>::VEC; }
+
 // f(integral_constant<int, ACT>) for the activation's code; false: unknown
 template <typename F>
 static inline bool with_act(int code, F f) {

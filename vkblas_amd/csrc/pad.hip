@@ -1,67 +1,138 @@
 // pad.hip — copies between a program's matrices and the workspace: operands
 // padded with zeros to sizes and alignments the fast GEMM kernels take, and
-// results taken out again.  Bound by memory: 16 bytes a thread.
+// results taken out again.  Bound by memory, 16 bytes a thread; a call's copies
+// are one launch (a launch of its own costs each about 4 us).
 #include "nn_common.hpp"
 #include "vkb_nn_launch.h"
 
 namespace vkb {
 namespace {
 
-constexpr uint32_t THREADS = 256;
+struct PadJobs {
+    vkb_pad_job job[VKB_PAD_JOBS];
+    uint32_t first[VKB_PAD_JOBS + 1];   // a job's first workgroup
+    int n;
+    // workgroup 0, where scal is set: the loss gradients' scale
+    uint32_t M;
+    const float* dloss;
+    float beta, to;
+    float* scal;
+};
 
-// column blocks in x, rows in y (strided: y holds at most 65535)
-template <typename T>
-static dim3 rows_grid(uint32_t M, uint32_t N) {
-    const uint32_t per = THREADS * Elem<T>::VEC;
-    return dim3((N + per - 1) / per, M < 65535u ? M : 65535u);
+__device__ __forceinline__ void find_scale(const PadJobs& p) {
+    __shared__ float sh[WORK / 64];
+    float top = 0.0f;
+    for (uint32_t m = threadIdx.x; m < p.M; m += 4 * WORK) {
+        float v[4];
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) v[i] = m + i * WORK < p.M ? fabsf(p.dloss[m + i * WORK]) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, v[i]);
+    }
+    top = wave_max(top);
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = top;
+    __syncthreads();
+    if (threadIdx.x) return;
+    for (uint32_t i = 1; i < WORK / 64; ++i) top = fmaxf(top, sh[i]);
+    // by the largest itself, not a power of two near it: equal loss gradients
+    // (a mean's) then round the target's p - 1 near -1 almost exactly, where
+    // any other factor puts one and the same error on every row
+    const bool fine = top > 1e-30f && top < 1e30f;
+    p.scal[0] = fine ? p.to / top : 1.0f;
+    p.scal[1] = fine ? top / p.to : 1.0f;
+    p.scal[2] = p.beta;
+    p.scal[3] = 1.0f;
+    p.scal[4] = 0.0f;
 }
 
 template <typename T>
-__global__ __launch_bounds__(THREADS) void pad_kernel(uint32_t S, uint32_t M, uint32_t N, const T* A, int64_t lda,
-                                                      T* P, uint32_t Mp, uint32_t Np) {
+__global__ __launch_bounds__(WORK) void pad_kernel(PadJobs p) {
     constexpr int VEC = Elem<T>::VEC;
-    const int64_t n = ((int64_t)blockIdx.x * THREADS + threadIdx.x) * VEC;
-    if (n >= Np) return;
-    for (uint64_t r = blockIdx.y; r < (uint64_t)S * Mp; r += gridDim.y) {
-        const uint32_t s = (uint32_t)(r / Mp), m = (uint32_t)(r % Mp);
-        u32x4 v = {0u, 0u, 0u, 0u};
-        if (m < M) v = ld_chunk(A + ((int64_t)s * M + m) * lda, n, N);
-        st_chunk(P + (int64_t)r * Np, n, Np, v);
+    if (p.scal && blockIdx.x == 0) {
+        find_scale(p);
+        return;
     }
+    int k = 0;
+    while (k + 1 < p.n && blockIdx.x >= p.first[k + 1]) ++k;
+    const vkb_pad_job& j = p.job[k];
+    const T* A = (const T*)j.src;
+    T* P = (T*)j.dst;
+    for_chunks((uint64_t)j.S * j.Mp, j.Np / VEC, p.first[k], p.first[k + 1] - p.first[k], [&](uint64_t r, uint32_t c) {
+        const uint32_t s = (uint32_t)(r / j.Mp), m = (uint32_t)(r - (uint64_t)s * j.Mp);
+        const int64_t n = (int64_t)c * VEC;
+        u32x4 v = {0u, 0u, 0u, 0u};
+        if (m < j.M) v = ld_chunk(A + ((int64_t)s * j.M + m) * j.ld, n, j.N);
+        *(u32x4*)(P + (int64_t)r * j.Np + n) = v;   // the workspace's rows lie on 16-byte units
+    });
 }
 
-template <typename T, typename C>
-__global__ __launch_bounds__(THREADS) void unpad_kernel(uint32_t S, uint32_t M, uint32_t N, const T* P, int64_t ldp,
-                                                        uint32_t Mp, C* out, int64_t ldc, float beta) {
-    constexpr int VEC = Elem<C>::VEC;
-    const int64_t n = ((int64_t)blockIdx.x * THREADS + threadIdx.x) * VEC;
-    if (n >= N) return;
-    for (uint64_t r = blockIdx.y; r < (uint64_t)S * M; r += gridDim.y) {
-        const T* src = P + ((int64_t)(r / M) * Mp + r % M) * ldp;
-        C* dst = out + (int64_t)r * ldc;
-        float x[VEC], o[VEC];
-        if constexpr (sizeof(T) == sizeof(C)) {
-            unpack<T>(ld_chunk(src, n, N), x);
-        } else {
+struct UnpadJobs {
+    vkb_unpad_job job[2];
+    uint32_t first[3];
+    int n;
+};
+
+// four values a thread: of fp32 or of T, either side
+template <typename T>
+__global__ __launch_bounds__(WORK) void unpad_kernel(UnpadJobs p) {
+    const int k = p.n > 1 && blockIdx.x >= p.first[1];
+    const vkb_unpad_job& j = p.job[k];
+    const bool sf = j.type == VKB_T_F32, df = j.out_type == VKB_T_F32;
+    constexpr int VEC = 4;
+    for_chunks((uint64_t)j.S * j.M, (j.N + VEC - 1) / VEC, p.first[k], p.first[k + 1] - p.first[k],
+               [&](uint64_t r, uint32_t c) {
+        const int64_t n = (int64_t)c * VEC;
+        const int64_t from = ((int64_t)(r / j.M) * j.Mp + (int64_t)(r % j.M)) * j.ldp + n, to = (int64_t)r * j.ldc + n;
+        float x[VEC] = {0.f, 0.f, 0.f, 0.f};
+        const bool all = n + VEC <= j.N;
+        const int have = all ? VEC : (int)(j.N - n);
+        auto load = [&](const auto* q, float* out) {
+            using E = std::remove_cv_t<std::remove_reference_t<decltype(*q)>>;
+            typedef E ev __attribute__((ext_vector_type(VEC), aligned(sizeof(E))));
+            if (all) {
+                const ev v = *(const ev*)q;
 #pragma unroll
-            for (int q = 0; q < VEC; q += Elem<T>::VEC) unpack<T>(ld_chunk(src, n + q, N), x + q);
-        }
-        if (beta != 0.0f) {
-            unpack<C>(ld_chunk(dst, n, N), o);
+                for (int e = 0; e < VEC; ++e) out[e] = (float)v[e];
+            } else {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) x[i] += beta * o[i];
+                for (int e = 0; e < VEC; ++e)
+                    if (e < have) out[e] = (float)q[e];
+            }
+        };
+        auto store = [&](auto* q) {
+            using E = std::remove_reference_t<decltype(*q)>;
+            typedef E ev __attribute__((ext_vector_type(VEC), aligned(sizeof(E))));
+            if (all) {
+                ev v;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) v[e] = (E)x[e];
+                *(ev*)q = v;
+            } else {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e)
+                    if (e < have) q[e] = (E)x[e];
+            }
+        };
+        if (sf) load((const float*)j.src + from, x);
+        else load((const T*)j.src + from, x);
+        if (j.beta != 0.0f) {
+            float o[VEC] = {0.f, 0.f, 0.f, 0.f};
+            if (df) load((const float*)j.dst + to, o);
+            else load((const T*)j.dst + to, o);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) x[e] += j.beta * o[e];
         }
-        st_chunk(dst, n, N, pack<C>(x));
-    }
+        if (df) store((float*)j.dst + to);
+        else store((T*)j.dst + to);
+    });
 }
 
 template <typename T>
-__global__ __launch_bounds__(THREADS) void scale_kernel(uint32_t M, uint32_t N, T* C, int64_t ldc, float beta) {
-    for (uint32_t m = blockIdx.y; m < M; m += gridDim.y)
-        for (int64_t n = (int64_t)blockIdx.x * THREADS + threadIdx.x; n < N; n += (int64_t)gridDim.x * THREADS) {
-            T* c = C + (int64_t)m * ldc + n;
-            *c = beta == 0.0f ? (T)0.0f : (T)(beta * (float)*c);
-        }
+__global__ __launch_bounds__(WORK) void scale_kernel(uint32_t M, uint32_t N, T* C, int64_t ldc, float beta) {
+    for_chunks(M, N, 0, gridDim.x, [&](uint64_t m, uint32_t n) {
+        T* c = C + (int64_t)m * ldc + n;
+        *c = beta == 0.0f ? (T)0.0f : (T)(beta * (float)*c);
+    });
 }
 
 }  // namespace
@@ -69,30 +140,47 @@ __global__ __launch_bounds__(THREADS) void scale_kernel(uint32_t M, uint32_t N, 
 
 using namespace vkb;
 
-extern "C" int vkb_launch_pad(int type, uint32_t S, uint32_t M, uint32_t N, const void* A, int64_t lda, void* P,
-                              uint32_t Mp, uint32_t Np, void* stream) {
+extern "C" int vkb_launch_pad(int type, const vkb_pad_job* jobs, int n, uint32_t M, const float* dloss, float beta,
+                              float* scal, void* stream) {
+    if (n < 0 || n > VKB_PAD_JOBS || (n == 0 && !scal)) return (int)hipErrorInvalidValue;
+    PadJobs p{};
+    p.n = n;
+    p.M = M;
+    p.dloss = dloss;
+    p.beta = beta;
+    p.to = type == VKB_T_F16 ? 8192.0f : 1.0f;
+    p.scal = scal;
     const bool ok = with_type(type, [&](auto t) {
         using T = decltype(t);
-        const uint64_t rows = (uint64_t)S * Mp;
-        hipLaunchKernelGGL((pad_kernel<T>), rows_grid<T>((uint32_t)(rows < 65535 ? rows : 65535), Np), dim3(THREADS),
-                           0, (hipStream_t)stream, S, M, N, (const T*)A, lda, (T*)P, Mp, Np);
+        uint32_t at = scal ? 1 : 0;
+        for (int i = 0; i < n; ++i) {
+            p.job[i] = jobs[i];
+            p.first[i] = at;
+            at += chunk_blocks((uint64_t)jobs[i].S * jobs[i].Mp, jobs[i].Np / Elem<T>::VEC);
+        }
+        p.first[n] = at;
+        hipLaunchKernelGGL((pad_kernel<T>), dim3(at), dim3(WORK), 0, (hipStream_t)stream, p);
     });
     return ok ? (int)hipGetLastError() : (int)hipErrorInvalidValue;
 }
 
-extern "C" int vkb_launch_unpad(int type, int out_type, uint32_t S, uint32_t M, uint32_t N, const void* P, int64_t ldp,
-                                uint32_t Mp, void* out, int64_t ldc, float beta, void* stream) {
-    bool ok = type == out_type || type == VKB_T_F32;
-    ok = ok && with_type(out_type, [&](auto t) {
-        using C = decltype(t);
-        const uint64_t rows = (uint64_t)S * M;
-        const dim3 grid = rows_grid<C>((uint32_t)(rows < 65535 ? rows : 65535), N);
-        if (type == VKB_T_F32)
-            hipLaunchKernelGGL((unpad_kernel<float, C>), grid, dim3(THREADS), 0, (hipStream_t)stream, S, M, N,
-                               (const float*)P, ldp, Mp, (C*)out, ldc, beta);
-        else
-            hipLaunchKernelGGL((unpad_kernel<C, C>), grid, dim3(THREADS), 0, (hipStream_t)stream, S, M, N,
-                               (const C*)P, ldp, Mp, (C*)out, ldc, beta);
+extern "C" int vkb_launch_unpad(const vkb_unpad_job* jobs, int n, void* stream) {
+    if (n < 1 || n > 2) return (int)hipErrorInvalidValue;
+    UnpadJobs p{};
+    p.n = n;
+    int type = VKB_T_F32;   // the 16-bit type among them
+    uint32_t at = 0;
+    for (int i = 0; i < n; ++i) {
+        p.job[i] = jobs[i];
+        p.first[i] = at;
+        at += chunk_blocks((uint64_t)jobs[i].S * jobs[i].M, (jobs[i].N + 3) / 4);
+        if (jobs[i].type != VKB_T_F32) type = jobs[i].type;
+        if (jobs[i].out_type != VKB_T_F32) type = jobs[i].out_type;
+    }
+    p.first[n] = at;
+    const bool ok = with_type(type, [&](auto t) {
+        using T = decltype(t);
+        hipLaunchKernelGGL((unpad_kernel<T>), dim3(at), dim3(WORK), 0, (hipStream_t)stream, p);
     });
     return ok ? (int)hipGetLastError() : (int)hipErrorInvalidValue;
 }
@@ -100,7 +188,7 @@ extern "C" int vkb_launch_unpad(int type, int out_type, uint32_t S, uint32_t M, 
 extern "C" int vkb_launch_scale(int type, uint32_t M, uint32_t N, void* C, int64_t ldc, float beta, void* stream) {
     const bool ok = with_type(type, [&](auto t) {
         using T = decltype(t);
-        hipLaunchKernelGGL((scale_kernel<T>), rows_grid<T>(M, N), dim3(THREADS), 0, (hipStream_t)stream, M, N, (T*)C,
+        hipLaunchKernelGGL((scale_kernel<T>), dim3(chunk_blocks(M, N)), dim3(WORK), 0, (hipStream_t)stream, M, N, (T*)C,
                            ldc, beta);
     });
     return ok ? (int)hipGetLastError() : (int)hipErrorInvalidValue;

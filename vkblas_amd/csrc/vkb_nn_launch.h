@@ -17,6 +17,10 @@ extern "C" {
 int vkb_launch_layer_norm(int type, int w_type, uint32_t M, uint32_t N, const void* x, int64_t ldx, const void* w,
                           const void* b, float eps, void* y, int64_t ldy, float* mean, float* rstd, void* stream);
 uint32_t vkb_layer_norm_parts(int type, uint32_t M, uint32_t N);
+/* dw and db (NULL: not) without partial sums, for few rows */
+int vkb_launch_layer_norm_few(int type, uint32_t M, uint32_t N, const void* dy, int64_t lddy, const void* x,
+                              int64_t ldx, const float* mean, const float* rstd, void* dw, void* db, int g_type,
+                              float beta, void* stream);
 int vkb_layer_norm_long(uint32_t N);   /* rows past a workgroup's registers */
 int vkb_launch_layer_norm_backward(int type, int w_type, uint32_t M, uint32_t N, const void* dy, int64_t lddy,
                                    const void* x, int64_t ldx, const void* w, const float* mean, const float* rstd,
@@ -27,13 +31,33 @@ int vkb_launch_layer_norm_reduce(const float* part, uint32_t parts, uint32_t N, 
 /* C = beta * C on M x N (a gradient over an empty batch). */
 int vkb_launch_scale(int type, uint32_t M, uint32_t N, void* C, int64_t ldc, float beta, void* stream);
 
-/* Copies (pad.hip) of S matrices of M x N below each other, from or to rows
- * of Mp >= M in the workspace.  pad: P, of Np >= N columns, zero past M and N;
- * unpad: out = beta * out + P, P of out_type or fp32. */
-int vkb_launch_pad(int type, uint32_t S, uint32_t M, uint32_t N, const void* A, int64_t lda, void* P, uint32_t Mp,
-                   uint32_t Np, void* stream);
-int vkb_launch_unpad(int type, int out_type, uint32_t S, uint32_t M, uint32_t N, const void* P, int64_t ldp,
-                     uint32_t Mp, void* out, int64_t ldc, float beta, void* stream);
+/* Copies (pad.hip) between a program's S matrices of M x N below each other
+ * (leading dimension ld) and the workspace, one launch for all of a call's.
+ * pad: to S of Mp x Np, Np a multiple of 16 bytes, zero past M and N; all of
+ * type.  With scal set, also the device scalars of products of a gradient
+ * that is divided by the largest |dloss| of M: scal[0] = s = 1 / max |dloss|
+ * (fp16: 2^13 times that; 1 where the largest is 0, infinite or outside 1e-30
+ * .. 1e30), scal[1] = 1 / s, scal[2] = beta, scal[3] = 1, scal[4] = 0. */
+#define VKB_PAD_JOBS 3
+typedef struct vkb_pad_job {
+    const void* src;
+    void* dst;
+    int64_t ld;
+    uint32_t S, M, N, Mp, Np;
+} vkb_pad_job;
+int vkb_launch_pad(int type, const vkb_pad_job* jobs, int n, uint32_t M, const float* dloss, float beta, float* scal,
+                   void* stream);
+/* unpad (up to 2): dst = beta * dst + src, src in rows of ldp and matrices of
+ * Mp rows; type and out_type fp32 or one and the same 16-bit type */
+typedef struct vkb_unpad_job {
+    const void* src;
+    void* dst;
+    int64_t ldp, ldc;
+    uint32_t S, M, N, Mp;
+    int type, out_type;
+    float beta;
+} vkb_unpad_job;
+int vkb_launch_unpad(const vkb_unpad_job* jobs, int n, void* stream);
 
 /* Gated projection (glu.hip), from projections computed before:
  * h = act(G) * U from z = [G | U] in fp32, and gu = z rounded (NULL: not
@@ -48,16 +72,16 @@ int vkb_launch_glu_join_backward(int type, int act, uint32_t M, uint32_t N, cons
 /* Linear cross entropy (xent.hip).  stats: over z, columns v0 .. v0 + n - 1
  * of the logits, the pair (max, sum of exp(z - max)) of each row and each
  * VKB_XENT_SLICE columns, to parts[slice * M + m], and the target's logit to
- * zt[m].  finish: lse and loss of S such slices. */
+ * zt[m].  finish: lse and loss of S such slices.  rows: both at once, for
+ * logits of at most VKB_XENT_ROW columns in all. */
 #define VKB_XENT_SLICE 4096u
 int vkb_launch_xent_stats(uint32_t M, uint32_t n, uint32_t v0, const float* z, int64_t ldz, const int64_t* target,
                           float* parts, float* zt, void* stream);
+#define VKB_XENT_ROW 16384u
+int vkb_launch_xent_rows(uint32_t M, uint32_t V, const float* z, int64_t ldz, const int64_t* target, int64_t ignore,
+                         float* loss, float* lse, void* stream);
 int vkb_launch_xent_finish(uint32_t M, uint32_t V, uint32_t S, const float* parts, const float* zt,
                            const int64_t* target, int64_t ignore, float* loss, float* lse, void* stream);
-/* scal[0] = s = 1 / max |dloss| (fp16: 2^13 times that; 1 where the largest is
- * 0, infinite or outside 1e-30 .. 1e30), scal[1] = 1 / s, scal[2] = beta,
- * scal[3] = 1, scal[4] = 0 (device scalars of products). */
-int vkb_launch_xent_scale(int type, uint32_t M, const float* dloss, float beta, float* scal, void* stream);
 /* D = scal[0] * dloss * (exp(z - lse) - [v == target]), scal NULL = 1. */
 int vkb_launch_xent_grad(int type, uint32_t M, uint32_t n, uint32_t v0, uint32_t V, const float* z, int64_t ldz,
                          const int64_t* target, int64_t ignore, const float* lse, const float* dloss,

@@ -118,52 +118,78 @@ __global__ __launch_bounds__(THREADS) void xent_finish_kernel(uint32_t M, uint32
     }
 }
 
-__global__ __launch_bounds__(1024) void xent_scale_kernel(uint32_t M, const float* dloss, bool fp16, float beta,
-                                                            float* scal) {
-    __shared__ float sh[16];
-    float top = 0.0f;
-    for (uint32_t m = threadIdx.x; m < M; m += 1024) top = fmaxf(top, fabsf(dloss[m]));
-    top = wave_max(top);
-    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = top;
-    __syncthreads();
-    if (threadIdx.x) return;
-    for (int i = 1; i < 16; ++i) top = fmaxf(top, sh[i]);
-    // by the largest itself, not a power of two near it: equal loss gradients
-    // (a mean's) then round the target's p - 1 near -1 almost exactly, where
-    // any other factor puts one and the same error on every row
-    const bool fine = top > 1e-30f && top < 1e30f;
-    const float to = fp16 ? 8192.0f : 1.0f;
-    scal[0] = fine ? to / top : 1.0f;
-    scal[1] = fine ? top / to : 1.0f;
-    scal[2] = beta;
-    scal[3] = 1.0f;
-    scal[4] = 0.0f;
+// A row of at most VKB_XENT_ROW logits, in the registers of one workgroup.
+constexpr uint32_t ROW_THREADS = 1024;
+__global__ __launch_bounds__(ROW_THREADS) void xent_rows_kernel(uint32_t M, uint32_t V, const float* z, int64_t ldz,
+                                                                const int64_t* target, int64_t ignore, float* loss,
+                                                                float* lse) {
+    constexpr int NV = VKB_XENT_ROW / ROW_THREADS / 4;
+    __shared__ float sh[2][ROW_THREADS / 64];
+    const uint32_t waves = blockDim.x / 64;
+    for (uint64_t m = blockIdx.x; m < M; m += gridDim.x) {
+        const float* row = z + (int64_t)m * ldz;
+        float x[NV][4], top = -INFINITY, s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int64_t c = ((int64_t)i * blockDim.x + threadIdx.x) * 4;
+            if (c + 3 < V) {
+                unpack<float>(ld16_any(row + c), x[i]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[i][e] = c + e < V ? row[c + e] : -INFINITY;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) top = fmaxf(top, x[i][e]);
+        top = wave_max(top);
+        if ((threadIdx.x & 63) == 0) sh[0][threadIdx.x >> 6] = top;
+        __syncthreads();
+        for (uint32_t i = 0; i < waves; ++i) top = fmaxf(top, sh[0][i]);
+        const float off = finite_or_0(top);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s += fast_exp(x[i][e] - off);
+        s = wave_sum(s);
+        if ((threadIdx.x & 63) == 0) sh[1][threadIdx.x >> 6] = s;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            for (uint32_t i = 1; i < waves; ++i) s += sh[1][i];
+            const float l = off + logf(s);
+            lse[m] = l;
+            if (loss) {
+                const int64_t t = target[m];
+                loss[m] = t == ignore ? 0.0f : (t >= 0 && t < V ? l - row[t] : __builtin_nanf(""));
+            }
+        }
+        __syncthreads();   // the next row writes sh again
+    }
 }
 
 template <typename T>
-__global__ __launch_bounds__(THREADS) void xent_grad_kernel(uint32_t M, uint32_t n, uint32_t v0, uint32_t V,
+__global__ __launch_bounds__(WORK) void xent_grad_kernel(uint32_t M, uint32_t n, uint32_t v0, uint32_t V,
                                                             const float* z, int64_t ldz, const int64_t* target,
                                                             int64_t ignore, const float* lse, const float* dloss,
                                                             const float* scal, T* D, int64_t ldd) {
     constexpr int VEC = Elem<T>::VEC;
-    const int64_t c = ((int64_t)blockIdx.x * THREADS + threadIdx.x) * VEC;
-    if (c >= n) return;
     const float sc = scal ? scal[0] : 1.0f;
-    for (uint32_t m = blockIdx.y; m < M; m += gridDim.y) {
-        const int64_t t = target[m];
+    for_chunks(M, (n + VEC - 1) / VEC, 0, gridDim.x, [&](uint64_t m, uint32_t k) {
+        const int64_t c = (int64_t)k * VEC, t = target[m];
         const float l = lse[m];
         // the three kinds of rows: counted, ignored (all zero), target out of range (all NaN)
-        const float k = t == ignore ? 0.0f : (t >= 0 && t < V ? dloss[m] * sc : __builtin_nanf(""));
+        const float w = t == ignore ? 0.0f : (t >= 0 && t < V ? dloss[m] * sc : __builtin_nanf(""));
         float x[VEC];
 #pragma unroll
         for (int q = 0; q < VEC; q += 4) unpack<float>(ld_chunk(z + (int64_t)m * ldz, c + q, n), x + q);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
             const float p = fast_exp(x[i] - l) - (c + i == t - v0 ? 1.0f : 0.0f);
-            x[i] = t == ignore ? 0.0f : k * p;
+            x[i] = t == ignore ? 0.0f : w * p;
         }
         st_chunk(D + (int64_t)m * ldd, c, n, pack<T>(x));
-    }
+    });
 }
 
 }  // namespace
@@ -189,10 +215,13 @@ extern "C" int vkb_launch_xent_finish(uint32_t M, uint32_t V, uint32_t S, const 
     return (int)hipGetLastError();
 }
 
-extern "C" int vkb_launch_xent_scale(int type, uint32_t M, const float* dloss, float beta, float* scal,
-                                     void* stream) {
-    hipLaunchKernelGGL(xent_scale_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, M, dloss, type == VKB_T_F16,
-                       beta, scal);
+extern "C" int vkb_launch_xent_rows(uint32_t M, uint32_t V, const float* z, int64_t ldz, const int64_t* target,
+                                    int64_t ignore, float* loss, float* lse, void* stream) {
+    if (V > VKB_XENT_ROW) return (int)hipErrorInvalidValue;
+    // whole waves for 16 values a thread
+    const uint32_t threads = (V + 1023) / 1024 * 64;
+    hipLaunchKernelGGL(xent_rows_kernel, dim3(M < 65536u ? M : 65536u), dim3(threads), 0, (hipStream_t)stream, M, V, z,
+                       ldz, target, ignore, loss, lse);
     return (int)hipGetLastError();
 }
 
@@ -201,8 +230,7 @@ extern "C" int vkb_launch_xent_grad(int type, uint32_t M, uint32_t n, uint32_t v
                                     const float* dloss, const float* scal, void* D, int64_t ldd, void* stream) {
     const bool ok = with_type(type, [&](auto t) {
         using T = decltype(t);
-        const uint32_t per = THREADS * Elem<T>::VEC;
-        hipLaunchKernelGGL((xent_grad_kernel<T>), dim3((n + per - 1) / per, rows_y(M)), dim3(THREADS), 0,
+        hipLaunchKernelGGL((xent_grad_kernel<T>), dim3(chunk_blocks(M, chunks_of<T>(n))), dim3(WORK), 0,
                            (hipStream_t)stream, M, n, v0, V, z, ldz, target, ignore, lse, dloss, scal, (T*)D, ldd);
     });
     return ok ? (int)hipGetLastError() : (int)hipErrorInvalidValue;
