@@ -174,7 +174,7 @@ def last_path() -> int:
 # vkblas_kernel_t (include/vkblas_ext.h)
 KERNEL_NONE, KERNEL_GENERIC, KERNEL_GENERIC_CHECKED, KERNEL_PIPE256, KERNEL_PIPE128, KERNEL_PIPE128_4, \
     KERNEL_SKINNY, KERNEL_WAVEK, KERNEL_DIRECT, KERNEL_FLOW, KERNEL_NORM, KERNEL_NORM_LONG, \
-    KERNEL_JOINED, KERNEL_FUSED = range(14)
+    KERNEL_JOINED, KERNEL_FUSED, KERNEL_FEW = range(15)
 
 
 def workspace_release() -> None:

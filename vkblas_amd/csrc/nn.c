@@ -291,6 +291,34 @@ static void bound(vkb_op_args* a, const operand* x, const operand* w) {
     a->ldw = w->ld;
 }
 
+/* ------------------------------------------------------------- few rows */
+
+/* Whether the one-pass kernels take a call; off: some operand's rows lie off
+ * 16-byte units, which the kernels that take more rows at a time have no fast
+ * form for.
+ * Forward: up to `rows` rows, and VKB_FEW where off (us, other kernels / these:
+ * gated fp16 1 x 14336 x 4096 36.9 / 34.4, 2 x 1344 x 310 9.4 / 6.3; logits bf16
+ * 5 x 107712 x 6965 883 / 410).
+ * Backward: up to 8 rows, where off or the weight is so small that launches
+ * count (R K elements, us: bf16 3 x 3584 x 128 15.5 / 11.2, fp16 2 x 75421 x 3456,
+ * odd, 576 / 308; but 3 x 13144 x 5312 86 / 121: two passes on MFMAs, each at the
+ * full rate of reads or of writes). */
+static int few_forward(vkblas_dtype_t t, uint32_t M, uint32_t K, uint32_t rows, int off) {
+    return K >= vec_of(t) && (M <= rows || (M <= VKB_FEW && off));
+}
+static int few_backward_rows(vkblas_dtype_t t, uint32_t M, uint32_t R, uint32_t K, int off) {
+    return K >= vec_of(t) && M <= 8 && (off || (uint64_t)R * K <= 2u << 20);
+}
+
+/* D's two products in one pass; p: everything but the division and part. */
+static vkblas_status_t few_backward(op_call* c, vkblas_dtype_t type, vkblas_dtype_t dw_type, vkb_few_backward* p,
+                                    int glu, size_t o_part, uint32_t slices, void* dx, uint32_t lddx) {
+    p->part = dx ? (float*)at(c, o_part) : NULL;
+    if (step(c, vkb_launch_few_backward(type, p->dw ? dw_type : type, p, glu, c->stream), p->dw != NULL) && dx)
+        step(c, vkb_launch_few_reduce(type, p->part, slices, p->M, p->K, dx, lddx, c->stream), 1);
+    return op_end(c, VKBLAS_KERNEL_FEW);
+}
+
 /* A gradient over no rows: C = beta * C. */
 static vkblas_status_t empty_gradient(op_call* c, vkblas_dtype_t type, uint32_t M, uint32_t N, void* C, uint32_t ldc,
                                       float beta) {
@@ -372,6 +400,12 @@ vkblas_status_t vkblas_glu_async(vkblas_dtype_t type, vkblas_act_t act, uint32_t
     if (vkb_engine_trace()) fprintf(stderr, "[vkblas] glu type=%d act=%d M=%u N=%u K=%u\n", (int)type, (int)act, M, N, K);
     vkb_op_args a;
     operand ox = as_is(x, ldx, 1, M, K), ow = as_is(w, ldw, 2, N, K);
+    if (few_forward(type, M, K, 4, K % vec_of(type) || off_units(type, x, ldx) || off_units(type, w, ldw))) {
+        if (room(&c) != VKBLAS_OK) return c.st;
+        const vkb_few_forward p = {x, w, h, gu, ldx, ldw, ldh, ldgu, M, N, K, (int)act};
+        step(&c, vkb_launch_few_forward(type, &p, 1, stream), 1);
+        return op_end(&c, VKBLAS_KERNEL_FEW);
+    }
     if (fusable(type, M, N, K, &ox, &ow, 128, &a)) {
         place(&c, &ox, type);
         place(&c, &ow, type);
@@ -435,6 +469,15 @@ vkblas_status_t vkblas_glu_backward_async(vkblas_dtype_t type, vkblas_act_t act,
     if (!dgu && !dx && !dw) return VKBLAS_OK;
     if (vkb_engine_trace())
         fprintf(stderr, "[vkblas] glu_backward type=%d act=%d M=%u N=%u K=%u\n", (int)type, (int)act, M, N, K);
+    if (!dgu && few_backward_rows(type, M, 2 * N, K,
+                                  K % vec_of(type) || N % 4 || off_units(type, x, ldx) || off_units(type, w, ldw))) {
+        vkb_few_backward p = {.x = x, .w = w, .dw = dw, .ldx = ldx, .ldw = ldw, .lddw = lddw, .M = M, .R = 2 * N, .K = K,
+                              .beta = beta, .dh = dh, .gu = gu, .lddh = lddh, .ldgu = ldgu, .act = (int)act};
+        const uint32_t slices = vkb_few_slices(type, &p);
+        const size_t o_part = dx ? buf(&c, (uint64_t)slices * M * K * sizeof(float)) : 0;
+        if (room(&c) != VKBLAS_OK) return c.st;
+        return few_backward(&c, type, dw_type, &p, 1, o_part, slices, dx, lddx);
+    }
     /* The two products as the fast kernels take them, where their work is
      * worth the copies (from 4 GFLOP each on, 2 in fp32) and the layout of [dG | dU] is
      * this call's own: K in whole 16-byte units (columns of both results), M
@@ -530,7 +573,8 @@ vkblas_status_t vkblas_linear_xent_async(vkblas_dtype_t type, uint32_t M, uint32
     const uint32_t per = (n + VKB_XENT_SLICE - 1) / VKB_XENT_SLICE;   /* slices of a piece; the last may have fewer */
     const uint32_t S = V / n * per + (last + VKB_XENT_SLICE - 1) / VKB_XENT_SLICE;
     const int rows = n == V && V <= VKB_XENT_ROW;                     /* one kernel for a row's statistics and loss */
-    const uint32_t Kp = joinable(type, M, K, &ox, &ow);
+    const int few = n == V && few_forward(type, M, K, 0, K % vec_of(type) || off_units(type, x, ldx) || off_units(type, w, ldw));
+    const uint32_t Kp = few ? K : joinable(type, M, K, &ox, &ow);
     need_gemm(&c, type, VKBLAS_DT_F32, VKBLAS_OP_N, VKBLAS_OP_T, M, n, Kp, ox.p, ox.ld, ow.p, ow.ld, ldz);
     if (last) need_gemm(&c, type, VKBLAS_DT_F32, VKBLAS_OP_N, VKBLAS_OP_T, M, last, Kp, ox.p, ox.ld, ow.p, ow.ld, ldz);
     place(&c, &ox, type);
@@ -547,8 +591,10 @@ vkblas_status_t vkblas_linear_xent_async(vkblas_dtype_t type, uint32_t M, uint32
     uint32_t slice = 0;
     for (uint64_t v = 0; ok && v < V; v += n, slice += per) {
         const uint32_t cols = (uint32_t)(V - v < n ? V - v : n);
-        ok = product(&c, type, VKBLAS_DT_F32, VKBLAS_OP_N, VKBLAS_OP_T, M, cols, Kp, host_scalars(1.0f, 0.0f), ox.p,
-                     ox.ld, (const char*)ow.p + v * ow.ld * type_size(type), ow.ld, z, ldz, 0) &&
+        const vkb_few_forward fw = {x, w, z, NULL, ldx, ldw, ldz, 0, M, V, K, 0};
+        ok = (few ? step(&c, vkb_launch_few_forward(type, &fw, 0, stream), 0)
+                  : product(&c, type, VKBLAS_DT_F32, VKBLAS_OP_N, VKBLAS_OP_T, M, cols, Kp, host_scalars(1.0f, 0.0f),
+                            ox.p, ox.ld, (const char*)ow.p + v * ow.ld * type_size(type), ow.ld, z, ldz, 0)) &&
              (rows ? step(&c, vkb_launch_xent_rows(M, V, z, ldz, target, ignore_index, loss, lse, stream), 1)
                    : step(&c, vkb_launch_xent_stats(M, cols, (uint32_t)v, z, ldz, target,
                                                     parts + (uint64_t)slice * M * 2, zt, stream), 0));
@@ -573,6 +619,26 @@ vkblas_status_t vkblas_linear_xent_backward_async(vkblas_dtype_t type, uint32_t 
     if (!dx && !dw) return VKBLAS_OK;
     if (vkb_engine_trace())
         fprintf(stderr, "[vkblas] linear_xent_backward type=%d M=%u V=%u K=%u\n", (int)type, M, V, K);
+    const int off = K % vec_of(type) || off_units(type, x, ldx) || off_units(type, w, ldw);
+    if (few_backward_rows(type, M, V, K, off || V % 8)) {
+        const uint32_t ldz = (uint32_t)round_up(V, 4);
+        vkb_few_backward p = {.x = x, .w = w, .dw = dw, .ldx = ldx, .ldw = ldw, .lddw = lddw, .M = M, .R = V, .K = K,
+                              .beta = beta, .lse = lse, .dloss = dloss, .ldz = ldz, .ignore = ignore_index,
+                              .target = target};
+        if (!off) need_gemm(&c, type, VKBLAS_DT_F32, VKBLAS_OP_N, VKBLAS_OP_T, M, V, K, x, ldx, w, ldw, ldz);
+        const uint32_t slices = vkb_few_slices(type, &p);
+        const size_t o_z = buf(&c, (uint64_t)M * ldz * sizeof(float));
+        const size_t o_part = dx ? buf(&c, (uint64_t)slices * M * K * sizeof(float)) : 0;
+        if (room(&c) != VKBLAS_OK) return c.st;
+        float* z = at(&c, o_z);
+        p.z = z;
+        const vkb_few_forward fw = {x, w, z, NULL, ldx, ldw, ldz, 0, M, V, K, 0};
+        const int ok = off ? step(&c, vkb_launch_few_forward(type, &fw, 0, stream), 0)
+                           : product(&c, type, VKBLAS_DT_F32, VKBLAS_OP_N, VKBLAS_OP_T, M, V, K,
+                                     host_scalars(1.0f, 0.0f), x, ldx, w, ldw, z, ldz, 0);
+        if (!ok) return op_end(&c, VKBLAS_KERNEL_FEW);
+        return few_backward(&c, type, dw_type, &p, 0, o_part, slices, dx, lddx);
+    }
     /* D of a piece of the vocabulary at a time, in type: from the pipelined
      * kernel, or over the piece's logits in fp32 (fp32: in their place).
      * Where the products' work is worth it, their sums run over whole steps:

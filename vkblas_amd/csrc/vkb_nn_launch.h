@@ -87,6 +87,45 @@ int vkb_launch_xent_grad(int type, uint32_t M, uint32_t n, uint32_t v0, uint32_t
                          const int64_t* target, int64_t ignore, const float* lse, const float* dloss,
                          const float* scal, void* D, int64_t ldd, void* stream);
 
+/* The operators for up to VKB_FEW rows (few.hip), operands at any alignment.
+ * forward: y = x w^T, R rows of w, fp32; or (glu) y = h = act(G) * U of R
+ * columns, w of 2 R rows, and gu = [G | U] unless NULL.  K of at least 16
+ * bytes.
+ * backward: dw = beta * dw + D^T x (dw NULL: not) and, per slice of w's rows and
+ * group of threads, the part of dx = D w (part NULL: not), vkb_few_slices
+ * matrices of M x K that reduce adds up.  D (M x R) is the gated
+ * projection's [dG | dU] from dh and gu, or the cross entropy's from z, fp32.
+ * vkb_few_slices fills in kthreads and slice.  K of at least 16 bytes. */
+#define VKB_FEW 16
+#define VKB_FEW_BACK 8           /* rows of the backward pass */
+typedef struct vkb_few_forward {
+    const void *x, *w;
+    void *y, *gu;
+    int64_t ldx, ldw, ldy, ldgu;
+    uint32_t M, R, K;
+    int act;
+} vkb_few_forward;
+int vkb_launch_few_forward(int type, const vkb_few_forward* p, int glu, void* stream);
+typedef struct vkb_few_backward {
+    const void *x, *w;
+    void* dw;
+    int64_t ldx, ldw, lddw;
+    float* part;
+    uint32_t M, R, K;
+    uint32_t kthreads, slice;
+    float beta;
+    const void *dh, *gu;
+    int64_t lddh, ldgu;
+    int act;
+    const float *z, *lse, *dloss;
+    int64_t ldz, ignore;
+    const int64_t* target;
+} vkb_few_backward;
+uint32_t vkb_few_slices(int type, vkb_few_backward* p);
+int vkb_launch_few_reduce(int type, const float* part, uint32_t parts, uint32_t M, uint32_t K, void* dx, int64_t lddx,
+                          void* stream);
+int vkb_launch_few_backward(int type, int g_type, const vkb_few_backward* p, int glu, void* stream);
+
 /* Operators inside the pipelined GEMM kernel (nn_pipe.hpp): x M x K, w the
  * weight (2 N x K gated projection, N x K of the logits' classes), both as
  * vkb_op_plan accepts them.  tile: VKB_TILE_256 or VKB_TILE_128. */
