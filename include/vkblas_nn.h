@@ -19,8 +19,8 @@
  * weight's type or F32 (a program's fp32 accumulators).  dw is read only
  * when beta != 0.  A gradient whose pointer is NULL is not computed.
  *
- * Workspace: calls that need one take their stream's workspace, as split-K
- * GEMMs do (vkblas_workspace_release frees it), and return VKBLAS_ERR_INIT
+ * Workspace: calls that need one take their stream's workspace, as GEMMs that
+ * split K do (vkblas_workspace_release frees it), and return VKBLAS_ERR_INIT
  * under stream capture; each function says when it needs one.
  *
  * Status: VKBLAS_OK; VKBLAS_ERR_PARAM (null pointer, zero size, leading
@@ -60,8 +60,8 @@ vkblas_status_t vkblas_layer_norm_async(
  *   w: NULL = ones; mean, rstd: as the forward pass wrote them
  *   dx, dw, db: each NULL or computed; dw, db of g_type (w_type or F32)
  * dx may be dy or x.  Sums over rows run in an order that depends on M and N
- * alone: equal calls give equal bits.  Needs a workspace when dw or db of more
- * than 256 rows is wanted.
+ * alone: equal calls give equal bits.  Needs a workspace when dw or db is wanted
+ * of more than 512 rows (1024 for N up to 4096), or for N below 8 or above 16384.
  */
 vkblas_status_t vkblas_layer_norm_backward_async(
     vkblas_dtype_t type, vkblas_dtype_t w_type,
@@ -87,8 +87,10 @@ typedef enum {
  *   projection's; h: M x N; all of one type
  *   gu: NULL, or M x 2N of the same type: G and U, kept for the backward
  *   pass (h is computed from their fp32 values)
- * Needs a workspace where no fused kernel takes the shape (M <= 64, or
- * operands off 16-byte units).
+ * Needs no workspace for M <= 4 (16 where rows lie off 16-byte units, K at
+ * least one of them), nor for more than 64 rows whose h has at least 96 tiles of
+ * 128 x 64 (200 in fp32), all rows on 16-byte units and K a multiple of 64 from 128
+ * on.  Other calls may take one.
  */
 vkblas_status_t vkblas_glu_async(
     vkblas_dtype_t type, vkblas_act_t act,
@@ -106,7 +108,8 @@ vkblas_status_t vkblas_glu_async(
  *   dgu: NULL, or M x 2N of type: receives [dG | dU], rounded to type (the
  *   two products read it); may be gu itself.  NULL: kept in the workspace.
  *   dx: M x K or NULL; dw: 2N x K of dw_type or NULL
- * Needs a workspace unless dgu is given and no product splits K.
+ * Takes a workspace for [dG | dU] (without dgu), for the sums of products that
+ * split K, and for copies of operands that lie off 16-byte units or whole steps.
  */
 vkblas_status_t vkblas_glu_backward_async(
     vkblas_dtype_t type, vkblas_act_t act,

@@ -510,35 +510,115 @@ __global__ __launch_bounds__(1024) void layer_norm_reduce_kernel(const float* pa
     if (threadIdx.x < COLS && n < N) put_grad(out + n, s, beta);
 }
 
-// dw and db of few rows, from the rows themselves
+// The gradients of few rows in one launch, without partial sums: the first
+// workgroups take dx's rows (a wave or a workgroup each, as the maps above),
+// the others 32 columns of dw and db each, from the rows themselves.  dx must
+// not be dy or x where both are wanted (the others still read them): then two
+// launches, the columns' first.
+constexpr int FEW_THREADS = 1024;
+
+template <typename T, typename W, int MAP, int EPT>
+__device__ __forceinline__ void few_dx(uint32_t M, uint32_t N, uint32_t waves, const T* dy, int64_t lddy, const T* x,
+                                       int64_t ldx, const W* w, const float* mean, const float* rstd, T* dx,
+                                       int64_t lddx) {
+    using R = RowMap<T, MAP, EPT>;
+    constexpr int VEC = R::VEC, NV = R::NV;
+    __shared__ float2 sh[FEW_THREADS / 64];
+    const int wave = threadIdx.x >> 6;
+    const int t = MAP == ONE ? (threadIdx.x & 63) : threadIdx.x, tpr = MAP == ONE ? 64 : (int)waves * 64;
+    const uint32_t m = MAP == ONE ? blockIdx.x * (FEW_THREADS / 64) + wave : blockIdx.x;
+    if (MAP == ONE && m >= M) return;   // (no barrier there)
+    // waves past the row's hold no chunk of their own: they add and store nothing
+    const Chunks<T, NV> ch(t, tpr, N);
+    const T *xr = x + (int64_t)m * ldx, *dr = dy + (int64_t)m * lddy;
+    const float mu = mean[m], r = rstd[m];
+    u32x4 rx[NV], rd[NV];
+    float g[EPT], xh[EPT], s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        rx[i] = ld16_any(xr + ch.off(i));
+        rd[i] = ld16_any(dr + ch.off(i));
+        load_params<W, VEC>(w, ch.off(i), 1.0f, g + i * VEC);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        float d[VEC];
+        unpack<T>(rx[i], xh + i * VEC);
+        unpack<T>(rd[i], d);
+        if (!ch.whole) ch.own(i, d);   // 0: adds to no sum
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const int k = i * VEC + e;
+            xh[k] = (xh[k] - mu) * r;
+            g[k] *= d[e];
+            s1 += g[k];
+            s2 += g[k] * xh[k];
+        }
+    }
+    s1 = wave_sum(s1);
+    s2 = wave_sum(s2);
+    if constexpr (MAP != ONE) {
+        if ((threadIdx.x & 63) == 0) sh[wave] = float2{s1, s2};
+        __syncthreads();
+        s1 = s2 = 0.0f;
+        for (uint32_t i = 0; i < waves; ++i) {
+            s1 += sh[i].x;
+            s2 += sh[i].y;
+        }
+    }
+    s1 /= (float)N;
+    s2 /= (float)N;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        float o[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) o[e] = r * (g[i * VEC + e] - s1 - xh[i * VEC + e] * s2);
+        ch.store(i, dx + (int64_t)m * lddx, pack<T>(o));
+    }
+}
+
 template <typename T, typename G>
-__global__ __launch_bounds__(1024) void layer_norm_few_kernel(uint32_t M, uint32_t N, const T* dy, int64_t lddy,
-                                                              const T* x, int64_t ldx, const float* mean,
-                                                              const float* rstd, G* dw, G* db, float beta) {
+__device__ __forceinline__ void few_dw(uint32_t block, uint32_t M, uint32_t N, const T* dy, int64_t lddy, const T* x,
+                                       int64_t ldx, const float* mean, const float* rstd, G* dw, G* db, float beta) {
     __shared__ float sh[16][32];
+    constexpr int U = 8;         // rows in flight
     const uint32_t slice = threadIdx.x >> 5;
-    const uint32_t n = blockIdx.x * 32 + (threadIdx.x & 31);
+    const uint32_t n = block * 32 + (threadIdx.x & 31);
     float sw = 0.0f, sb = 0.0f;
     if (n < N)
-        for (uint32_t m = slice; m < M; m += 32 * 4) {
-            float d[4], h[4];
+        for (uint32_t m = slice; m < M; m += 32 * U) {
+            float d[U], h[U];
 #pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) {
+            for (uint32_t i = 0; i < U; ++i) {
                 const uint32_t r = min(m + 32 * i, M - 1);
-                d[i] = m + 32 * i < M ? (float)dy[(int64_t)r * lddy + n] : 0.0f;
+                d[i] = (float)dy[(int64_t)r * lddy + n];
                 h[i] = ((float)x[(int64_t)r * ldx + n] - mean[r]) * rstd[r];
             }
 #pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) {
-                if (m + 32 * i < M) sw += d[i] * h[i];
-                sb += d[i];
-            }
+            for (uint32_t i = 0; i < U; ++i)
+                if (m + 32 * i < M) {
+                    sw += d[i] * h[i];
+                    sb += d[i];
+                }
         }
     sw = join_slices<32>(sw, sh);
     sb = join_slices<32>(sb, sh);
     if (threadIdx.x >= 32 || n >= N) return;
     if (dw) put_grad(dw + n, sw, beta);
     if (db) put_grad(db + n, sb, beta);
+}
+
+template <typename T, typename W, int MAP, int EPT>
+__global__ __launch_bounds__(FEW_THREADS) void layer_norm_few_kernel(
+    uint32_t M, uint32_t N, uint32_t waves, uint32_t dx_blocks, const T* dy, int64_t lddy, const T* x, int64_t ldx,
+    const W* w, const float* mean, const float* rstd, T* dx, int64_t lddx, void* dw, void* db, bool g_f32, float beta) {
+    if (blockIdx.x < dx_blocks) {
+        few_dx<T, W, MAP, EPT>(M, N, waves, dy, lddy, x, ldx, w, mean, rstd, dx, lddx);
+    } else if (g_f32) {
+        few_dw<T, float>(blockIdx.x - dx_blocks, M, N, dy, lddy, x, ldx, mean, rstd, (float*)dw, (float*)db, beta);
+    } else {
+        few_dw<T, T>(blockIdx.x - dx_blocks, M, N, dy, lddy, x, ldx, mean, rstd, (T*)dw, (T*)db, beta);
+    }
 }
 
 // f(map, values a thread) for rows of N columns; false: rows shorter than a
@@ -658,14 +738,23 @@ extern "C" int vkb_launch_layer_norm_reduce(const float* part, uint32_t parts, u
     return ok ? (int)hipGetLastError() : (int)hipErrorInvalidValue;
 }
 
-extern "C" int vkb_launch_layer_norm_few(int type, uint32_t M, uint32_t N, const void* dy, int64_t lddy, const void* x,
-                                         int64_t ldx, const float* mean, const float* rstd, void* dw, void* db,
-                                         int g_type, float beta, void* stream) {
-    const bool ok = with_types(type, g_type, [&](auto tt, auto tg) {
+extern "C" int vkb_launch_layer_norm_few(int type, int w_type, uint32_t M, uint32_t N, const void* dy, int64_t lddy,
+                                         const void* x, int64_t ldx, const void* w, const float* mean,
+                                         const float* rstd, void* dx, int64_t lddx, void* dw, void* db, int g_type,
+                                         float beta, void* stream) {
+    if (g_type != type && g_type != VKB_T_F32) return (int)hipErrorInvalidValue;
+    bool fits = false;
+    const bool ok = with_types(type, w_type, [&](auto tt, auto tw) {
         using T = decltype(tt);
-        using G = decltype(tg);
-        hipLaunchKernelGGL((layer_norm_few_kernel<T, G>), dim3((N + 31) / 32), dim3(1024), 0, (hipStream_t)stream, M, N,
-                           (const T*)dy, lddy, (const T*)x, ldx, mean, rstd, (G*)dw, (G*)db, beta);
+        using W = decltype(tw);
+        fits = with_map(N, [&](auto map, auto ept) {
+            const uint32_t waves = RowMap<T, map.value, ept.value>::waves(N);
+            const uint32_t rows = map.value == ONE ? FEW_THREADS / 64 : 1;
+            const uint32_t rb = dx ? (M + rows - 1) / rows : 0, cb = dw || db ? (N + 31) / 32 : 0;
+            hipLaunchKernelGGL((layer_norm_few_kernel<T, W, map.value, ept.value>), dim3(rb + cb), dim3(FEW_THREADS), 0,
+                               (hipStream_t)stream, M, N, waves, rb, (const T*)dy, lddy, (const T*)x, ldx, (const W*)w,
+                               mean, rstd, (T*)dx, lddx, dw, db, g_type == VKB_T_F32, beta);
+        });
     });
-    return ok ? (int)hipGetLastError() : (int)hipErrorInvalidValue;
+    return ok && fits ? (int)hipGetLastError() : (int)hipErrorInvalidValue;
 }

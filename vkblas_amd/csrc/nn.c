@@ -362,19 +362,21 @@ vkblas_status_t vkblas_layer_norm_backward_async(vkblas_dtype_t type, vkblas_dty
     if (!dy || !x || !mean || !rstd) return VKBLAS_ERR_PARAM;
     if (!dx && !dw && !db) return VKBLAS_OK;
     if (vkb_engine_trace()) fprintf(stderr, "[vkblas] layer_norm_backward type=%d M=%u N=%u\n", (int)type, M, N);
-    /* Up to 256 rows (a workgroup's partial sums would be one row's), dw and db
-     * come from the rows themselves, before dx, which may take their place:
-     * us, partial sums / this: 139 x 15104 bf16 21.7 / 10.3. */
-    const int few = M <= 256 && (dw || db);
-    if (few && vkb_engine_ready() &&
-        !step(&c, vkb_launch_layer_norm_few(type, M, N, dy, lddy, x, ldx, mean, rstd, dw, db, g_type, beta, stream), 1))
-        return c.st;
-    if (few && !dx) {
-        vkb_engine_ran(VKBLAS_PATH_NONE, VKBLAS_KERNEL_NORM);
-        return vkb_engine_ready() ? VKBLAS_OK : VKBLAS_ERR_INIT;
+    /* Few rows all in one launch, without partial sums (us, with / this, bf16: 139 x
+     * 15104 21.7 / 9.2, 500 x 4096 16.7 / 10.6, 1000 x 4096 18.6 / 18.5, 1000 x 12000
+     * 28 / 29.6, 2000 x 2000 16.1 / 22.3); dw and db first where dx takes the place of
+     * their operands. */
+    if (M <= (N <= 4096 ? 1024u : 512u) && !vkb_layer_norm_long(N)) {
+        const int apart = dx && (dw || db) && (dx == dy || dx == x);
+        if (room(&c) != VKBLAS_OK) return c.st;
+        if (!apart || step(&c, vkb_launch_layer_norm_few(type, w_type, M, N, dy, lddy, x, ldx, w, mean, rstd, NULL, 0, dw,
+                                                         db, g_type, beta, stream), 1))
+            step(&c, vkb_launch_layer_norm_few(type, w_type, M, N, dy, lddy, x, ldx, w, mean, rstd, dx, lddx,
+                                               apart ? NULL : dw, apart ? NULL : db, g_type, beta, stream), 1);
+        return op_end(&c, VKBLAS_KERNEL_NORM);
     }
     const uint32_t parts = vkb_layer_norm_parts(type, M, N);
-    const int sums = !few && (dw || db);
+    const int sums = dw || db;
     const size_t o_part = sums ? buf(&c, (uint64_t)parts * 2 * N * sizeof(float)) : 0;
     if (room(&c) != VKBLAS_OK) return c.st;
     float* part = sums ? (float*)at(&c, o_part) : NULL;

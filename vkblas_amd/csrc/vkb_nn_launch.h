@@ -17,10 +17,12 @@ extern "C" {
 int vkb_launch_layer_norm(int type, int w_type, uint32_t M, uint32_t N, const void* x, int64_t ldx, const void* w,
                           const void* b, float eps, void* y, int64_t ldy, float* mean, float* rstd, void* stream);
 uint32_t vkb_layer_norm_parts(int type, uint32_t M, uint32_t N);
-/* dw and db (NULL: not) without partial sums, for few rows */
-int vkb_launch_layer_norm_few(int type, uint32_t M, uint32_t N, const void* dy, int64_t lddy, const void* x,
-                              int64_t ldx, const float* mean, const float* rstd, void* dw, void* db, int g_type,
-                              float beta, void* stream);
+/* dx, dw and db (NULL: not) of few rows in one launch, without partial sums;
+ * not for vkb_layer_norm_long rows, nor dx in dy's or x's place along with dw or
+ * db */
+int vkb_launch_layer_norm_few(int type, int w_type, uint32_t M, uint32_t N, const void* dy, int64_t lddy, const void* x,
+                              int64_t ldx, const void* w, const float* mean, const float* rstd, void* dx, int64_t lddx,
+                              void* dw, void* db, int g_type, float beta, void* stream);
 int vkb_layer_norm_long(uint32_t N);   /* rows past a workgroup's registers */
 int vkb_launch_layer_norm_backward(int type, int w_type, uint32_t M, uint32_t N, const void* dy, int64_t lddy,
                                    const void* x, int64_t ldx, const void* w, const float* mean, const float* rstd,
