@@ -89,8 +89,8 @@ typedef enum {
  *   pass (h is computed from their fp32 values)
  * Needs no workspace for M <= 4 (16 where rows lie off 16-byte units, K at
  * least one of them), nor for more than 64 rows whose h has at least 96 tiles of
- * 128 x 64 (200 in fp32), all rows on 16-byte units and K a multiple of 64 from 128
- * on.  Other calls may take one.
+ * 128 x 64 (200 in fp32), K in whole 16-byte units and all rows on whole lines of
+ * 128 bytes (fp32: on 16-byte units).  Other calls may take one.
  */
 vkblas_status_t vkblas_glu_async(
     vkblas_dtype_t type, vkblas_act_t act,

@@ -69,6 +69,15 @@ def test_strides_and_alignment(M, N, K, dt, pad, off):
     check_forward(forward(x, w, dt, "gelu", pad=pad, off=off), x, w, dt, "gelu")
 
 
+# K that ends inside a step, in its first one, on it, and NaN behind each row; few tiles and many, of both sizes
+@pytest.mark.parametrize("M,N", [(300, 136), (1100, 3300), (2100, 4400)])
+@pytest.mark.parametrize("K", [8, 32, 64, 72, 136, 200, 232, 328])
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+def test_ends_of_k(M, N, K, dt):
+    x, w = R.values(M, K, dt, 7).cuda(), R.values(2 * N, K, dt, 8, K ** -0.5).cuda()
+    check_forward(forward(x, w, dt, "silu", keep=False, pad=8), x, w, dt, "silu")
+
+
 @pytest.mark.parametrize("act", list(R.ACTS))
 @pytest.mark.parametrize("M", [1, 300])
 def test_ends_of_the_activations(act, M):

@@ -71,6 +71,17 @@ def test_strides_and_alignment(M, V, K, dt, pad, off):
     check_forward(forward(x, w, t, dt, pad, off), x, w, t)
 
 
+# K that ends inside a step, in its first one, on it, and NaN behind each row; few tiles and many, of both sizes
+@pytest.mark.parametrize("M,V", [(300, 513), (1100, 6500), (2100, 9000)])
+@pytest.mark.parametrize("K", [8, 32, 64, 72, 136, 200, 232, 328])
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+def test_ends_of_k(M, V, K, dt):
+    args = grad_inputs(M, V, K, dt, 64.0, device="cuda")
+    x, w, t = args[:3]
+    check_forward(forward(x, w, t, dt, pad=8), x, w, t)
+    check_backward(backward(*args, dt, pad=8), *args, dt)
+
+
 @pytest.mark.parametrize("M", [4, 300])
 def test_targets(M):
     """An ignore_index inside the vocabulary, all rows ignored, invalid targets (NaN), lse alone."""

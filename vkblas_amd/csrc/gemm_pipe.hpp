@@ -127,7 +127,11 @@ constexpr RdSeq make_rdseq() {
 //    each wave's WT columns the first WT / 2 are rows n of B, the others rows
 //    N + n, so a lane holds both products of one output;
 //  * any M and N: rows past the last are read as the last (an offset register
-//    per DMA instruction), and the operator drops their results.
+//    per DMA instruction), and the operator drops their results;
+//  * any K of whole 16-byte chunks: lanes whose chunk lies past K get the
+//    offset OP_BYTES, the resources' size, where a buffer load returns zeros
+//    and reads nothing.
+constexpr uint32_t OP_BYTES = 0x80000000u;
 struct PlainOp {
     using Params = KParams;
     static constexpr bool PLAIN = true, GATED = false;
@@ -206,10 +210,13 @@ __global__ __launch_bounds__(256, (WT == 128 || NST == 4) ? 1 : 2) void gemm_pip
     // GATED: even waves load the first half's rows, odd ones the second's
     const int64_t brow = OP::GATED ? (int64_t)(wave & 1) * p.N + n0 : n0;
     const T* Bt = (const T*)p.B + bat * p.sb + (BKM ? brow * p.ldb + kbeg : kbeg * p.ldb + n0);
-    const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc((void*)At, (short)0, -1, 0x00020000);
-    const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc((void*)Bt, (short)0, -1, 0x00020000);
+    constexpr int RANGE = CLIP ? (int)OP_BYTES : -1;
+    const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc((void*)At, (short)0, RANGE, 0x00020000);
+    const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc((void*)Bt, (short)0, RANGE, 0x00020000);
     TC* Cb = (TC*)p.C + (sk ? (int64_t)b * p.s_split : (int64_t)b * p.sc);
-    const int nkt = (int)(klen / BK);
+    // operators: whole steps past K, at least two, of fp32 an even number
+    constexpr int EVEN = F16 ? 1 : 2;
+    const int nkt = CLIP ? max(2, (int)((klen + EVEN * BK - 1) / (EVEN * BK)) * EVEN) : (int)(klen / BK);
 
     // K-major direct loads: instruction i of this wave fills the 8-row group
     // NDMA wave + i (rows (BM / 4) wave + 8 i + [0, 8); lane -> row + lane / 8,
@@ -234,6 +241,20 @@ __global__ __launch_bounds__(256, (WT == 128 || NST == 4) ? 1 : 2) void gemm_pip
             b_vn[n] = min((OP::GATED ? (BN / 4) * (wave >> 1) : (BN / 4) * wave) + (lane >> 3) + 8 * n,
                           (int)p.N - 1 - n0) * ldb * ES + koff;
     }
+    // before the DMA of K step kt: this lane's offsets where its chunk lies
+    // past K (from then on for good: later steps do too)
+    auto past_k = [&](int kt) {
+        if constexpr (CLIP) {
+            if ((uint32_t)(kt + 1) * BK > klen) {
+                const bool past = (uint32_t)(kt * BK + koff / ES) >= klen;
+#pragma unroll
+                for (int n = 0; n < NDMA; ++n) {
+                    a_vn[n] = past ? (int)OP_BYTES : a_vn[n];
+                    b_vn[n] = past ? (int)OP_BYTES : b_vn[n];
+                }
+            }
+        }
+    };
     // 16-bit MN-major direct loads: instruction n of this wave fills the
     // 1-KiB block NDMA wave + n (k rows RPB (NDMA wave + n) + [0, RPB); lane ->
     // row + lane / CPR, slot lane % CPR, which holds chunk
@@ -287,7 +308,7 @@ __global__ __launch_bounds__(256, (WT == 128 || NST == 4) ? 1 : 2) void gemm_pip
     auto rsrc_words = [](const void* base) {
         const uint64_t a = (uint64_t)base;
         return i32x4{__builtin_amdgcn_readfirstlane((int)(uint32_t)a),
-                     __builtin_amdgcn_readfirstlane((int)(uint32_t)(a >> 32) & 0xffff), -1, 0x00020000};
+                     __builtin_amdgcn_readfirstlane((int)(uint32_t)(a >> 32) & 0xffff), RANGE, 0x00020000};
     };
     const i32x4 ra_w = rsrc_words(At), rb_w = rsrc_words(Bt);
     auto dma = [&](bool isA, lds_ptr_t dst, int voff, int soff) {
@@ -508,6 +529,8 @@ __global__ __launch_bounds__(256, (WT == 128 || NST == 4) ? 1 : 2) void gemm_pip
     // next: this region issues the DMA of step kt + NST - 1 (into the stage
     // step kt - 1 used); wc: the vmcnt that leaves step kt + 1 landed.
     auto region = [&](int kt, int S, bool prev, bool next, auto wc) {
+        if constexpr (NST == 4)
+            if (next) past_k(kt + 3);
 #pragma unroll
         for (int u = prev ? 0 : UPS; u < 32; ++u) {
             const int sub = u / UPS - 1;          // sub-step of kt run here (-1: kt-1's last)
@@ -525,13 +548,16 @@ __global__ __launch_bounds__(256, (WT == 128 || NST == 4) ? 1 : 2) void gemm_pip
     using W0 = std::integral_constant<int, 0>;
 
     // ---- prologue: K step 0 into stage 0 (NST 4: steps 1 and 2 too) ----
+    past_k(0);
 #pragma unroll
     for (int n = 0; n < ND; ++n) dma_load(0, 0, n);
     if constexpr (NST == 4) {
         // steps 1 and 2 as well (nkt >= 4), or step 1 only (nkt == 2)
+        past_k(1);
 #pragma unroll
         for (int n = 0; n < ND; ++n) dma_load(1, 1, n);
         if (nkt > 2) {
+            past_k(2);
 #pragma unroll
             for (int n = 0; n < ND; ++n) dma_load(2, 2, n);
             sync_vm(std::integral_constant<int, 2 * ND>{});
@@ -562,6 +588,7 @@ __global__ __launch_bounds__(256, (WT == 128 || NST == 4) ? 1 : 2) void gemm_pip
             region(kt + 2, (kt + 2) & 3, true, false, W0{});
         }
     } else if (nkt == 2) {
+        past_k(1);
         region(0, 0, false, true, W0{});
         region(1, 1, true, false, W0{});
     } else {
@@ -581,14 +608,25 @@ __global__ __launch_bounds__(256, (WT == 128 || NST == 4) ? 1 : 2) void gemm_pip
             // The last region's copy re-reads step nkt - 1 (from L2) into the
             // stage no later read uses; its end-of-region wait retires that
             // copy before the epilogue reuses the LDS.
+            // An operator's last step may end past K: its offsets change
+            // between two passes over the same loop (a test in every region
+            // costs 1.3% of a 4096-long K).
+            int end = CLIP ? nkt - 2 : nkt;
 #pragma clang loop unroll(disable)
-            for (; kt < nkt; ++kt) region(kt, kt & 1, true, true, W0{});
+            do {
+#pragma clang loop unroll(disable)
+                for (; kt < end; ++kt) region(kt, kt & 1, true, true, W0{});
+                if constexpr (CLIP) past_k(nkt - 1);
+                end += 2;
+            } while (CLIP && end <= nkt);
         } else {
             for (; kt + 3 < nkt; kt += 2) {
                 region(kt, 1, true, true, W0{});
                 region(kt + 1, 0, true, true, W0{});
             }
+            past_k(nkt - 2);
             region(kt, 1, true, true, W0{});       // kt == nkt - 3
+            past_k(nkt - 1);
             region(kt + 1, 0, true, true, W0{});   // loads step nkt-1
             region(kt + 2, 1, true, false, W0{});
         }

@@ -157,9 +157,8 @@ uint32_t vkb_xent_slices(const vkb_op_args* a) {
 
 /* Whether the pipelined kernel takes x w^T with an operator at its end, and
  * on which tiles; cols: the columns that one tile of 256 holds (128 gated).
- *  - 16-byte aligned operands and leading dimensions, K in whole steps: 64 for
- *    16-bit types, from two steps on, and pairs of 32 for fp32; the bytes
- *    that a tile's rows span below 2^31 (offsets are 32-bit);
+ *  - 16-byte aligned operands and leading dimensions, K in whole 16-byte units;
+ *    the bytes that a tile's rows span below 2^31 (offsets are 32-bit);
  *  - more than 64 rows, below which the decode kernels stream the weight, or
  *    16-bit operands with K of at most 512: then one launch instead of two or
  *    three is ahead;
@@ -178,7 +177,7 @@ static int op_plan(vkblas_dtype_t type, uint32_t M, uint32_t N, uint32_t K, cons
     const uint32_t vec = type == VKBLAS_DT_F32 ? 4 : 8;
     const uint64_t es = type_size(type);
     const uint64_t ld = ldx > ldw ? ldx : ldw;
-    if (!aligned16(x) || !aligned16(w) || ldx % vec || ldw % vec || K % 64 || K < 128 || (M <= 64 && (K > 512 || type == VKBLAS_DT_F32)) ||
+    if (!aligned16(x) || !aligned16(w) || ldx % vec || ldw % vec || K % vec || (M <= 64 && (K > 512 || type == VKBLAS_DT_F32)) ||
         (256 * ld + K) * es >= 1ull << 31)
         return 0;
     const uint64_t t = (uint64_t)((M + 255) / 256) * ((N + cols - 1) / cols);
@@ -220,6 +219,12 @@ typedef struct {
 
 static uint32_t vec_of(vkblas_dtype_t t) { return t == VKBLAS_DT_F32 ? 4 : 8; }
 static int off_units(vkblas_dtype_t t, const void* p, uint32_t ld) { return !aligned16(p) || ld % vec_of(t); }
+/* Whether a 16-bit operand's K steps lie across two lines each, which loads
+ * both, and K is long enough for the loads to count: the kernel takes 20 to 50%
+ * longer (bf16 xent 4323 x 1209 x 4984 90 us, 66 on a copy; 5886 x 79834 x 712 756, 638). */
+static int off_lines(vkblas_dtype_t t, uint32_t K, const void* p, uint32_t ld) {
+    return t != VKBLAS_DT_F32 && K >= 512 && (((uintptr_t)p | (uint64_t)ld * 2) & 127) != 0;
+}
 
 static operand as_is(const void* p, uint32_t ld, uint32_t S, uint32_t M, uint32_t N) {
     operand o = {p, ld, S, M, N, M, N, 0, 0};
@@ -253,20 +258,22 @@ static int brought(op_call* c, const copies* j, vkblas_dtype_t t, uint32_t M, co
     return (j->n == 0 && !scal) || step(c, vkb_launch_pad(t, j->job, j->n, M, dloss, beta, scal, c->stream), 0);
 }
 
-/* K as the pipelined kernel takes it */
-static uint32_t whole_k(uint32_t K) { return K <= 128 ? 128 : (uint32_t)round_up(K, 64); }
+/* A copied row's columns: rows start on whole lines (bf16 gradient of a cross
+ * entropy 174 x 41152 x 2084 as 2112 columns 372 us, as 2088 417) */
+static uint32_t line_k(vkblas_dtype_t t, uint32_t K) { return (uint32_t)round_up(K, K > 64 ? 64 : vec_of(t)); }
 /* x (M x K) and w (S of N x K) for x w^T inside the pipelined kernel: copied
  * where they have to be and the product is worth it.  Below 0.5 GFLOP the
  * copies' launch costs more than it saves. */
 static int fusable(vkblas_dtype_t type, uint32_t M, uint32_t N, uint32_t K, operand* x, operand* w, uint32_t cols,
                    vkb_op_args* a) {
-    const uint32_t Kp = whole_k(K);
-    const int rx = Kp != K || off_units(type, x->p, x->ld), rw = Kp != K || off_units(type, w->p, w->ld);
+    const uint32_t Kp = K % vec_of(type) ? line_k(type, K) : K;
+    const int rx = Kp != K || off_units(type, x->p, x->ld) || (N >= 1000 && off_lines(type, K, x->p, x->ld));
+    const int rw = Kp != K || off_units(type, w->p, w->ld) || (M >= 1000 && off_lines(type, K, w->p, w->ld));
     operand px = *x, pw = *w;
     if (rx || rw) {
         if (2.0 * M * w->S * w->M * K < 5e8) return 0;
-        if (rx) pad_to(&px, x->Mp, Kp);
-        if (rw) pad_to(&pw, w->Mp, Kp);
+        if (rx) pad_to(&px, x->Mp, line_k(type, K));
+        if (rw) pad_to(&pw, w->Mp, line_k(type, K));
     }
     if (!op_plan(type, M, N, Kp, px.p, px.ld, pw.p, pw.ld, cols, a)) return 0;
     *x = px;
@@ -278,7 +285,7 @@ static int fusable(vkblas_dtype_t type, uint32_t M, uint32_t N, uint32_t K, oper
 static uint32_t joinable(vkblas_dtype_t type, uint32_t M, uint32_t K, operand* x, operand* w) {
     const int off = K % vec_of(type) != 0;
     if (2.0 * M * w->S * w->M * K < 5e8) return K;
-    const uint32_t Kp = off ? whole_k(K) : K;
+    const uint32_t Kp = off ? K <= 128 ? 128 : (uint32_t)round_up(K, 64) : K;   /* its K steps, two at least */
     if (off || off_units(type, x->p, x->ld)) pad_to(x, x->Mp, Kp);
     if (off || off_units(type, w->p, w->ld)) pad_to(w, w->Mp, Kp);
     return Kp;
@@ -647,7 +654,7 @@ vkblas_status_t vkblas_linear_xent_backward_async(vkblas_dtype_t type, uint32_t 
      *  - dw's over M rows padded with zeros (D's, and a copy of x);
      *  - dx's over whole tiles of classes, and the rest of the vocabulary by a
      *    padded copy of its rows of w, whose part of dw comes by the workspace;
-     *    a w that is copied in any case is padded there. */
+     *    a w copied to another K is padded there. */
     const int f32 = type == VKBLAS_DT_F32;
     const size_t es = type_size(type);
     const double work = 2.0 * M * V * K;
@@ -655,25 +662,25 @@ vkblas_status_t vkblas_linear_xent_backward_async(vkblas_dtype_t type, uint32_t 
     operand ox = as_is(x, ldx, 1, M, K), ow = as_is(w, ldw, 1, V, K);
     const int fused = fusable(type, M, V, K, &ox, &ow, 256, &a);
     const uint32_t Kp = fused ? a.K : K, steps = f32 ? 64 : 128;
-    const int whole = fused && (work >= (f32 ? 2e9 : V % 8 ? 1e10 : 4e10) || ow.copy);
+    const int vpad = Kp != K;    /* w is copied and dw goes by the workspace: both in whole tiles of classes */
+    const int whole = fused && (work >= (f32 ? 2e9 : V % 8 ? 1e10 : 4e10) || vpad);
     uint32_t Mp = M;
     if (fused && dw && M % steps && work >= (f32 ? 2e9 : 1e10)) Mp = (uint32_t)round_up(M, steps);
-    if (ox.copy || Mp != M) pad_to(&ox, Mp, Kp);
-    if (ow.copy) pad_to(&ow, (uint32_t)round_up(V, 128), Kp);
-    const uint32_t rest = whole && !ow.copy ? V % 128 : 0;   /* classes that the tail takes */
+    if (ox.copy || Mp != M) pad_to(&ox, Mp, line_k(type, K));
+    if (vpad) pad_to(&ow, (uint32_t)round_up(V, 128), Kp);
+    const uint32_t rest = whole && !vpad ? V % 128 : 0;   /* classes that the tail takes */
     uint32_t n = piece_columns(M, V, fused ? PIECE_BYTES : JOIN_BYTES, fused ? es : sizeof(float));
     const uint32_t ldd = (uint32_t)round_up(n, whole ? 128 : 8);
     /* dx adds up over several products in fp32: in dx itself or in the workspace */
     const int several = n < V || rest, acc = dx && (Kp != K || (several && !f32));
     const vkblas_dtype_t xt = acc ? VKBLAS_DT_F32 : type;
     const uint32_t ldxo = acc ? (uint32_t)round_up(Kp, 4) : lddx;
-    /* dw's rows of other sizes than the program's go by the workspace */
-    const int pw = dw && (Kp != K || (ow.copy && V % 128));
+    const int pw = dw && vpad;
     const vkblas_dtype_t wt = (pw || rest) && beta != 0.0f ? VKBLAS_DT_F32 : dw_type;
     for (int i = 0; i < 2; ++i) {   /* a piece of n columns, and the last one */
         const uint32_t cols = i ? V % n : n;
         if (!cols) continue;
-        const uint32_t main = whole ? (ow.copy ? (uint32_t)round_up(cols, 128) : cols / 128 * 128) : cols;
+        const uint32_t main = whole ? (vpad ? (uint32_t)round_up(cols, 128) : cols / 128 * 128) : cols;
         if (!fused)
             need_gemm(&c, type, VKBLAS_DT_F32, VKBLAS_OP_N, VKBLAS_OP_T, M, cols, K, x, ldx, w, ldw, ldd);
         if (dx && main) need_gemm(&c, type, xt, VKBLAS_OP_N, VKBLAS_OP_N, M, Kp, main, NULL, ldd, ow.p, ow.ld, ldxo);
@@ -710,7 +717,7 @@ vkblas_status_t vkblas_linear_xent_backward_async(vkblas_dtype_t type, uint32_t 
     int summed = 0;              /* dx holds a product already */
     for (uint64_t v = 0; ok && v < V;) {
         const uint32_t cols = (uint32_t)(V - v < n ? V - v : n);
-        const uint32_t main = whole ? (ow.copy ? (uint32_t)round_up(cols, 128) : cols / 128 * 128) : cols;
+        const uint32_t main = whole ? (vpad ? (uint32_t)round_up(cols, 128) : cols / 128 * 128) : cols;
         const char* wv = (const char*)ow.p + v * ow.ld * es;
         char* dwv = (char*)dw + v * lddw * (dw ? type_size(dw_type) : 0);
         if (fused) {

@@ -19,14 +19,15 @@ static int launch_op(typename OP::Params p, hipStream_t st) {
 
 // The tile of a->tile; 128 x 128 ones of 16-bit operands with four LDS stages
 // where the grid is at most one workgroup per CU (their 144 KB allow no
-// second; the loads of three K steps in flight instead of one).
+// second; the loads of three K steps in flight instead of one); the kernel
+// takes two steps so, or from four on.
 template <typename T, typename OP>
 static int launch_tiles(const vkb_op_args* a, const typename OP::Params& p, hipStream_t st) {
     if (a->tile == VKB_TILE_256) return launch_op<T, OP, 128>(p, st);
     if constexpr (sizeof(T) == 2) {
         const uint64_t cols = OP::GATED ? 64 : 128;
         const uint64_t grid = (uint64_t)((p.M + 127) / 128) * ((p.N + cols - 1) / cols);
-        if (grid <= 256 && (p.K == 128 || p.K >= 256)) return launch_op<T, OP, 64, 4>(p, st);
+        if (grid <= 256 && (p.K <= 128 || p.K > 192)) return launch_op<T, OP, 64, 4>(p, st);
     }
     return launch_op<T, OP, 64>(p, st);
 }
