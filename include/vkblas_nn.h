@@ -88,7 +88,7 @@ typedef enum {
  *   gu: NULL, or M x 2N of the same type: G and U, kept for the backward
  *   pass (h is computed from their fp32 values)
  * Needs no workspace for M <= 4 (16 where rows lie off 16-byte units, K at
- * least one of them), nor for more than 64 rows whose h has at least 96 tiles of
+ * least one of them, and 32 for N of at least 2048 there), nor for more than 64 rows whose h has at least 96 tiles of
  * 128 x 64 (200 in fp32), K in whole 16-byte units and all rows on whole lines of
  * 128 bytes (fp32: on 16-byte units).  Other calls may take one.
  */

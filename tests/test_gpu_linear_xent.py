@@ -53,7 +53,7 @@ def check_forward(got, x, w, t, ignore=IGNORE):
 SIZES = [(1, 1, 1), (1, 5, 8), (2, 77, 9), (4, 3000, 515), (5, 1031, 2056), (8, 20000, 520), (9, 513, 1031), (16, 999, 700),
          (15, 1024, 1024), (1, 1000, 256), (3, 333, 72), (17, 4097, 64), (64, 515, 128), (65, 1000, 100),
          (128, 256, 128), (200, 300, 64), (256, 256, 192), (257, 1001, 128), (300, 700, 320), (511, 130, 128),
-         (100, 10007, 77), (40, 20001, 64), (3, 16384, 72), (3, 16385, 72)]
+         (100, 10007, 77), (40, 20001, 64), (9, 5001, 9), (16, 17003, 515), (17, 4097, 1031), (32, 16500, 131), (3, 16384, 72), (3, 16385, 72)]
 
 
 @pytest.mark.parametrize("M,V,K", SIZES)

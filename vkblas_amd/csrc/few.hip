@@ -2,7 +2,7 @@
 // bound by one pass over the weight, with what the operator does to them in
 // the same pass.
 //
-// Forward, y = x W^T for up to 16 rows of x: a workgroup takes four rows of W,
+// Forward, y = x W^T for up to 32 rows of x; the first kernel: a workgroup takes four rows of W,
 // its four waves a quarter of K's chunks each; a lane multiplies its 16 bytes
 // of every W row (non-temporal: they stream through once) with the same k of
 // every x row (v_dot2 of 16-bit types, fp32 sums), the next chunk's loads in
@@ -136,6 +136,128 @@ __global__ __launch_bounds__(THREADS) void few_forward_kernel(vkb_few_forward p)
         }
     } else {
         ((float*)p.y)[(int64_t)m * p.ldy + n] = sum(r);
+    }
+}
+
+// ... for more rows of x and many of W (vkb_few_mfma): 16 rows of W times MF fragments of 16 x rows on
+// the matrix units, RF fragments of W's rows a wave (gated: one of the gate's,
+// one of the up projection's).  A lane's 16 bytes of a row, at any alignment, are
+// its part of a 64-byte step of k, four steps at a time and the next four in
+// flight; the workgroup's waves take every fourth four steps.  us, the kernel
+// above / this, cross entropy bf16: 10 x 126144 x 4502 536 / 316, 16 x 32003 x 1027 118 /
+// 35, 12 x 2003 x 4101 19.6 / 24.2, 5 x 107712 x 6965 408 / 552 (rows at 2-byte
+// alignment: 2.7 TB/s; at 4 bytes 3.6).
+template <typename T, int MF, int RF, bool GLU>
+__global__ __launch_bounds__(THREADS) void few_mfma_kernel(vkb_few_forward p) {
+    constexpr int VEC = Elem<T>::VEC, U = 4, STEP = 4 * VEC * U;
+    static_assert(!GLU || RF == 2, "gate and up projection");
+    __shared__ floatx4 red[4][RF][MF][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 15, g = lane >> 4;
+    const uint32_t first = blockIdx.x * (GLU ? 16 : 16 * RF);
+    const T *wr[RF], *xr[MF];
+    // rows past the last are read as the last
+#pragma unroll
+    for (int f = 0; f < RF; ++f) {
+        const uint32_t n = min(first + (GLU ? 0 : 16 * f) + r, p.R - 1);
+        wr[f] = (const T*)p.w + ((GLU && f ? (int64_t)p.R : 0) + n) * p.ldw;
+    }
+#pragma unroll
+    for (int f = 0; f < MF; ++f) xr[f] = (const T*)p.x + (int64_t)min((uint32_t)(16 * f + r), p.M - 1) * p.ldx;
+    const uint32_t K = p.K, steps = (K + STEP - 1) / STEP;
+    floatx4 acc[RF][MF];
+#pragma unroll
+    for (int i = 0; i < RF; ++i)
+#pragma unroll
+        for (int j = 0; j < MF; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+    u32x4 wn[U][RF], xn[U][MF];
+    // a chunk past K is read as K's last, and one that straddles it too
+    auto load = [&](uint32_t s) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint32_t k = min(s * STEP + (4 * u + g) * VEC, K - VEC);
+#pragma unroll
+            for (int f = 0; f < RF; ++f) wn[u][f] = ld16_any(wr[f] + k);
+#pragma unroll
+            for (int f = 0; f < MF; ++f) xn[u][f] = ld16_any(xr[f] + k);
+        }
+    };
+    auto drop = [&](u32x4 v, int from) {   // zeros for elements before `from`
+        float f[VEC];
+        unpack<T>(v, f);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) f[e] = e < from ? 0.0f : f[e];
+        return pack<T>(f);
+    };
+    if ((uint32_t)wave < steps) load(wave);
+    for (uint32_t s = wave; s < steps; s += 4) {
+        u32x4 w[U][RF], x[U][MF];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+            for (int f = 0; f < RF; ++f) w[u][f] = wn[u][f];
+#pragma unroll
+            for (int f = 0; f < MF; ++f) x[u][f] = xn[u][f];
+        }
+        if (s + 4 < steps) load(s + 4);
+        if (s * STEP + STEP > K) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const uint32_t k = s * STEP + (4 * u + g) * VEC;
+                const int from = (int)min(k - min(k, K - VEC), (uint32_t)VEC);
+#pragma unroll
+                for (int f = 0; f < RF; ++f) w[u][f] = drop(w[u][f], from);
+#pragma unroll
+                for (int f = 0; f < MF; ++f) x[u][f] = drop(x[u][f], from);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < RF; ++i)
+#pragma unroll
+                for (int j = 0; j < MF; ++j) {
+                    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                                __uint_as_float(w[u][i][e]), __uint_as_float(x[u][j][e]), acc[i][j], 0, 0, 0);
+                    } else {
+                        acc[i][j] = mfma_16x16x32<T>(w[u][i], x[u][j], acc[i][j]);
+                    }
+                }
+    }
+#pragma unroll
+    for (int i = 0; i < RF; ++i)
+#pragma unroll
+        for (int j = 0; j < MF; ++j) red[wave][i][j][lane] = acc[i][j];
+    __syncthreads();
+    // a wave's lanes: rows n .. n + 3 of W, row m of x
+    constexpr int OUTS = GLU ? MF : RF * MF;
+    for (int o = wave; o < OUTS; o += 4) {
+        const int i = o / MF, j = o % MF;
+        const uint32_t n = first + 16 * i + 4 * g, m = 16 * j + r;
+        floatx4 a = red[0][i][j][lane], b = red[0][RF - 1][j][lane];
+#pragma unroll
+        for (int v = 1; v < 4; ++v) {
+            a += red[v][i][j][lane];
+            if (GLU) b += red[v][RF - 1][j][lane];
+        }
+        if (m >= p.M) continue;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (n + e >= p.R) break;
+            if constexpr (GLU) {
+                ((T*)p.y)[(int64_t)m * p.ldy + n + e] = (T)(act_of(p.act, a[e]) * b[e]);
+                if (p.gu) {
+                    T* gu = (T*)p.gu + (int64_t)m * p.ldgu + n + e;
+                    gu[0] = (T)a[e];
+                    gu[p.R] = (T)b[e];
+                }
+            } else {
+                ((float*)p.y)[(int64_t)m * p.ldy + n + e] = a[e];
+            }
+        }
     }
 }
 
@@ -308,13 +430,38 @@ static uint32_t backward_columns(int type) { return type == VKB_T_F32 ? 4 : 8; }
 
 using namespace vkb;
 
+// One fragment of W's rows a wave where two would leave CUs without work (us,
+// one / two: 16 x 32003 x 1027 bf16 41 / 34, 12 x 2003 x 4101 24 / 34).
+static int few_mfma(int type, const vkb_few_forward* p, int glu, hipStream_t st) {
+    const int rf = glu || p->R >= 16384 ? 2 : 1;
+    const uint64_t rows = glu ? 16 : 16 * rf, grid = (p->R + rows - 1) / rows;
+    if (grid > 0xffffffffull / THREADS) return (int)hipErrorInvalidValue;
+    const bool ok = with_type(type, [&](auto t) {
+        using T = decltype(t);
+        auto go = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3((uint32_t)grid), dim3(THREADS), 0, st, *p);
+        };
+        if (p->M <= 16) {
+            if (glu) go(few_mfma_kernel<T, 1, 2, true>);
+            else if (rf == 2) go(few_mfma_kernel<T, 1, 2, false>);
+            else go(few_mfma_kernel<T, 1, 1, false>);
+        } else {
+            if (glu) go(few_mfma_kernel<T, 2, 2, true>);
+            else if (rf == 2) go(few_mfma_kernel<T, 2, 2, false>);
+            else go(few_mfma_kernel<T, 2, 1, false>);
+        }
+    });
+    return ok ? (int)hipGetLastError() : (int)hipErrorInvalidValue;
+}
+
 extern "C" int vkb_launch_few_forward(int type, const vkb_few_forward* p, int glu, void* stream) {
-    if (p->M == 0 || p->M > VKB_FEW || p->R == 0 || p->K < (type == VKB_T_F32 ? 4u : 8u)) return (int)hipErrorInvalidValue;
+    if (p->M == 0 || (p->M > 16 && !vkb_few_mfma(p->M, glu ? 2 * (uint64_t)p->R : p->R)) || p->R == 0 || p->K < (type == VKB_T_F32 ? 4u : 8u)) return (int)hipErrorInvalidValue;
+    if (vkb_few_mfma(p->M, glu ? 2 * (uint64_t)p->R : p->R)) return few_mfma(type, p, glu, (hipStream_t)stream);
     const uint64_t grid = ((uint64_t)p->R + (glu ? 1 : 3)) / (glu ? 2 : 4);
     if (grid > 0xffffffffull / THREADS) return (int)hipErrorInvalidValue;
     const bool ok = with_type(type, [&](auto t) {
         using T = decltype(t);
-        with_rows<VKB_FEW>(p->M, [&](auto mb) {
+        with_rows<16>(p->M, [&](auto mb) {
             if (glu)
                 hipLaunchKernelGGL((few_forward_kernel<T, mb.value, true>), dim3((uint32_t)grid), dim3(THREADS), 0,
                                    (hipStream_t)stream, *p);

@@ -113,7 +113,8 @@ struct XentParams : KParams {
     // gradient: rows and columns of D stored, zero past M and N
     uint32_t Ms, Ns;
     int64_t V, ignore;
-    const float *lse, *dloss, *scal;
+    const float *lse, *dloss;
+    Scale scale;
 };
 
 // Fragments of rows whose target lies in this wave's columns are rare: f(i, t)
@@ -196,7 +197,7 @@ struct XentGradOp {
                                                int lane) {
         using G = Frag<WT, SH>;
         const int64_t row0 = m0 + (wave >> 1) * WT, col0 = n0 + (wave & 1) * WT;
-        const float sc = p.scal ? p.scal[0] : 1.0f;
+        const float sc = scale_of(p.scale, p.dloss, p.M, blockIdx.x == 0 && wave == 0, lane);
 #pragma unroll
         for (int i = 0; i < G::NF; ++i) {
             const int64_t m = row0 + G::row(lane, i);

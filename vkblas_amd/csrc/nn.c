@@ -130,7 +130,7 @@ extern int vkb_launch_xent_stats_f32(const vkb_op_args*, const int64_t*, float*,
 extern int vkb_launch_xent_stats_f16(const vkb_op_args*, const int64_t*, float*, float*, void*);
 extern int vkb_launch_xent_stats_bf16(const vkb_op_args*, const int64_t*, float*, float*, void*);
 typedef int xent_grad_fn(const vkb_op_args*, uint32_t, uint32_t, uint32_t, uint32_t, const int64_t*, int64_t,
-                         const float*, const float*, const float*, void*, int64_t, void*);
+                         const float*, const float*, vkb_scale, void*, int64_t, void*);
 extern xent_grad_fn vkb_launch_xent_grad_f32, vkb_launch_xent_grad_f16, vkb_launch_xent_grad_bf16;
 
 int vkb_launch_glu(const vkb_op_args* a, int act, void* h, int64_t ldh, void* gu, int64_t ldgu, void* stream) {
@@ -145,10 +145,10 @@ int vkb_launch_xent_stats_op(const vkb_op_args* a, const int64_t* target, float*
 }
 int vkb_launch_xent_grad_op(const vkb_op_args* a, uint32_t Ms, uint32_t Ns, uint32_t v0, uint32_t V,
                             const int64_t* target, int64_t ignore, const float* lse, const float* dloss,
-                            const float* scal, void* D, int64_t ldd, void* stream) {
+                            vkb_scale scale, void* D, int64_t ldd, void* stream) {
     return (a->type == VKB_T_F16 ? vkb_launch_xent_grad_f16 : a->type == VKB_T_BF16 ? vkb_launch_xent_grad_bf16
                                                                                    : vkb_launch_xent_grad_f32)(
-        a, Ms, Ns, v0, V, target, ignore, lse, dloss, scal, D, ldd, stream);
+        a, Ms, Ns, v0, V, target, ignore, lse, dloss, scale, D, ldd, stream);
 }
 uint32_t vkb_xent_slices(const vkb_op_args* a) {
     const uint64_t tile = vkb_tile_bn(a->tile);
@@ -164,9 +164,10 @@ uint32_t vkb_xent_slices(const vkb_op_args* a) {
  *    three is ahead;
  *  - enough tiles of 128 for their K: few tiles with a long K are faster as a
  *    product with K split and a pass over its result.  us, joined / here, gated
- *    projection bf16: 16 tiles K = 1024 10.8 / 9.7, 4096 21.4 / 26.8; 64 tiles 512
- *    12.0 / 7.3, 4096 25.2 / 27.2; 128 tiles 4096 33.3 / 30.1; fp32: 32 tiles K = 1024
- *    25 / 59, 128 tiles 63.8 / 62.1, K = 4096 149 / 233, 256 tiles 269 / 244;
+ *    projection bf16: 16 tiles K = 1024 10.8 / 9.7, 4096 21.4 / 26.8; 44 tiles 2048
+ *    20.5 / 16.9; 64 tiles 512 12.0 / 7.3, 4096 25.2 / 27.2; 74 tiles 2432 22.4 / 19.9;
+ *    128 tiles 4096 33.3 / 30.1; fp32: 32 tiles K = 1024 25 / 59, 128 tiles 63.8 / 62.1,
+ *    K = 4096 149 / 233, 256 tiles 269 / 244;
  *  - 16-bit: the tile whose waves of workgroups (one 256 x 256 or two 128 x 128
  *    per CU) take less at the rates measured, a K step of 64 1.45 and 0.83 us and
  *    an epilogue 6 and 4 (us on 128 / 256: 2048 x 4096 x 4096 gated, one wave of 256,
@@ -187,7 +188,7 @@ static int op_plan(vkblas_dtype_t type, uint32_t M, uint32_t N, uint32_t K, cons
         if (t128 < (K <= 2048 ? 128 : 200)) return 0;
         large = 8 * t >= 7 * 256 * ((t + 255) / 256);
     } else {
-        if (t128 < 96 && K > 1024 && K > 32 * t128) return 0;
+        if (t128 < 96 && K > 1024 && (K > 64 * t128 || K > 2560)) return 0;
         const double w256 = t < 1024 ? (double)((t + 255) / 256) : (double)t / 256;
         const double w128 = t128 < 2048 ? (double)((t128 + 511) / 512) : (double)t128 / 512;
         large = t > 128 && w256 * (1.45 * K / 64 + 6) <= w128 * (0.83 * K / 64 + 4);
@@ -303,15 +304,15 @@ static void bound(vkb_op_args* a, const operand* x, const operand* w) {
 /* Whether the one-pass kernels take a call; off: some operand's rows lie off
  * 16-byte units, which the kernels that take more rows at a time have no fast
  * form for.
- * Forward: up to `rows` rows, and VKB_FEW where off (us, other kernels / these:
- * gated fp16 1 x 14336 x 4096 36.9 / 34.4, 2 x 1344 x 310 9.4 / 6.3; logits bf16
- * 5 x 107712 x 6965 883 / 410).
+ * Forward: up to `rows` rows, and 16 (VKB_FEW of many weight rows) where off (us,
+ * other kernels / these: gated fp16 1 x 14336 x 4096 36.9 / 34.4, 2 x 1344 x 310 9.4 /
+ * 6.3, bf16 27 x 11264 x 1658 44.7 / 23; logits bf16 5 x 107712 x 6965 883 / 410).
  * Backward: up to 8 rows, where off or the weight is so small that launches
  * count (R K elements, us: bf16 3 x 3584 x 128 15.5 / 11.2, fp16 2 x 75421 x 3456,
  * odd, 576 / 308; but 3 x 13144 x 5312 86 / 121: two passes on MFMAs, each at the
  * full rate of reads or of writes). */
-static int few_forward(vkblas_dtype_t t, uint32_t M, uint32_t K, uint32_t rows, int off) {
-    return K >= vec_of(t) && (M <= rows || (M <= VKB_FEW && off));
+static int few_forward(vkblas_dtype_t t, uint32_t M, uint64_t R, uint32_t K, uint32_t rows, int off) {
+    return K >= vec_of(t) && (M <= rows || (off && (M <= 16 || (M <= VKB_FEW && vkb_few_mfma(M, R)))));
 }
 static int few_backward_rows(vkblas_dtype_t t, uint32_t M, uint32_t R, uint32_t K, int off) {
     return K >= vec_of(t) && M <= 8 && (off || (uint64_t)R * K <= 2u << 20);
@@ -409,7 +410,8 @@ vkblas_status_t vkblas_glu_async(vkblas_dtype_t type, vkblas_act_t act, uint32_t
     if (vkb_engine_trace()) fprintf(stderr, "[vkblas] glu type=%d act=%d M=%u N=%u K=%u\n", (int)type, (int)act, M, N, K);
     vkb_op_args a;
     operand ox = as_is(x, ldx, 1, M, K), ow = as_is(w, ldw, 2, N, K);
-    if (few_forward(type, M, K, 4, K % vec_of(type) || off_units(type, x, ldx) || off_units(type, w, ldw))) {
+    if (few_forward(type, M, 2 * (uint64_t)N, K, 4,
+                    K % vec_of(type) || off_units(type, x, ldx) || off_units(type, w, ldw))) {
         if (room(&c) != VKBLAS_OK) return c.st;
         const vkb_few_forward p = {x, w, h, gu, ldx, ldw, ldh, ldgu, M, N, K, (int)act};
         step(&c, vkb_launch_few_forward(type, &p, 1, stream), 1);
@@ -582,7 +584,8 @@ vkblas_status_t vkblas_linear_xent_async(vkblas_dtype_t type, uint32_t M, uint32
     const uint32_t per = (n + VKB_XENT_SLICE - 1) / VKB_XENT_SLICE;   /* slices of a piece; the last may have fewer */
     const uint32_t S = V / n * per + (last + VKB_XENT_SLICE - 1) / VKB_XENT_SLICE;
     const int rows = n == V && V <= VKB_XENT_ROW;                     /* one kernel for a row's statistics and loss */
-    const int few = n == V && few_forward(type, M, K, 0, K % vec_of(type) || off_units(type, x, ldx) || off_units(type, w, ldw));
+    const int few = n == V && few_forward(type, M, V, K, 0,
+                                          K % vec_of(type) || off_units(type, x, ldx) || off_units(type, w, ldw));
     const uint32_t Kp = few ? K : joinable(type, M, K, &ox, &ow);
     need_gemm(&c, type, VKBLAS_DT_F32, VKBLAS_OP_N, VKBLAS_OP_T, M, n, Kp, ox.p, ox.ld, ow.p, ow.ld, ldz);
     if (last) need_gemm(&c, type, VKBLAS_DT_F32, VKBLAS_OP_N, VKBLAS_OP_T, M, last, Kp, ox.p, ox.ld, ow.p, ow.ld, ldz);
@@ -654,20 +657,24 @@ vkblas_status_t vkblas_linear_xent_backward_async(vkblas_dtype_t type, uint32_t 
      *  - dw's over M rows padded with zeros (D's, and a copy of x);
      *  - dx's over whole tiles of classes, and the rest of the vocabulary by a
      *    padded copy of its rows of w, whose part of dw comes by the workspace;
-     *    a w copied to another K is padded there. */
+     *    or a copied w is padded there. */
     const int f32 = type == VKBLAS_DT_F32;
     const size_t es = type_size(type);
-    const double work = 2.0 * M * V * K;
+    const double work = 2.0 * M * V * K, worth = f32 ? 2e9 : V % 8 ? 1e9 : 4e10;
     vkb_op_args a;
     operand ox = as_is(x, ldx, 1, M, K), ow = as_is(w, ldw, 1, V, K);
     const int fused = fusable(type, M, V, K, &ox, &ow, 256, &a);
     const uint32_t Kp = fused ? a.K : K, steps = f32 ? 64 : 128;
-    const int vpad = Kp != K;    /* w is copied and dw goes by the workspace: both in whole tiles of classes */
-    const int whole = fused && (work >= (f32 ? 2e9 : V % 8 ? 1e10 : 4e10) || vpad);
+    /* Whether a copy of w, and dw by the workspace, are in whole tiles of classes: where
+     * they are of another K, or small enough that the two passes cost less than a tail
+     * (us, with a tail / so: bf16 4258 x 817 x 656 83 / 56, 3812 x 17898 x 96 197 / 164,
+     * fp32 4994 x 522 x 564 163 / 136) */
+    const int vpad = fused && (Kp != K || (V % 128 && (ow.copy || work >= worth) && (uint64_t)V * K * es <= 16u << 20));
+    const int whole = fused && (work >= worth || vpad);
     uint32_t Mp = M;
     if (fused && dw && M % steps && work >= (f32 ? 2e9 : 1e10)) Mp = (uint32_t)round_up(M, steps);
     if (ox.copy || Mp != M) pad_to(&ox, Mp, line_k(type, K));
-    if (vpad) pad_to(&ow, (uint32_t)round_up(V, 128), Kp);
+    if (vpad) pad_to(&ow, (uint32_t)round_up(V, 128), line_k(type, K));
     const uint32_t rest = whole && !vpad ? V % 128 : 0;   /* classes that the tail takes */
     uint32_t n = piece_columns(M, V, fused ? PIECE_BYTES : JOIN_BYTES, fused ? es : sizeof(float));
     const uint32_t ldd = (uint32_t)round_up(n, whole ? 128 : 8);
@@ -711,7 +718,8 @@ vkblas_status_t vkblas_linear_xent_backward_async(vkblas_dtype_t type, uint32_t 
     bring(&c, &jobs, &ox, x, ldx);
     bring(&c, &jobs, &ow, w, ldw);
     if (rest && dx) bring(&c, &jobs, &tail, (const char*)w + (uint64_t)(V - rest) * ldw * es, ldw);
-    int ok = brought(&c, &jobs, type, M, dloss, beta, scal);
+    const vkb_scale scale = {scal, beta, !jobs.n && M <= VKB_SCALE_ROWS};
+    int ok = brought(&c, &jobs, type, M, dloss, beta, scale.find ? NULL : scal);
     vkb_unpad_job out[2];        /* dw's rows still in the workspace, and dx */
     int outs = 0;
     int summed = 0;              /* dx holds a product already */
@@ -725,12 +733,12 @@ vkblas_status_t vkblas_linear_xent_backward_async(vkblas_dtype_t type, uint32_t 
             a.w = wv;
             a.N = cols;
             ok = step(&c, vkb_launch_xent_grad_op(&a, Mp, (uint32_t)round_up(cols, whole ? 128 : 8), (uint32_t)v, V,
-                                                  target, ignore_index, lse, dloss, scal, d, ldd, stream), 0);
+                                                  target, ignore_index, lse, dloss, scale, d, ldd, stream), 0);
         } else {
             ok = product(&c, type, VKBLAS_DT_F32, VKBLAS_OP_N, VKBLAS_OP_T, M, cols, K, host_scalars(1.0f, 0.0f), x,
                          ldx, wv, ldw, z, ldd, 0) &&
                  step(&c, vkb_launch_xent_grad(type, M, cols, (uint32_t)v, V, z, ldd, target, ignore_index, lse, dloss,
-                                               scal, d, ldd, stream), 0);
+                                               scale, d, ldd, stream), 0);
         }
         /* the whole tiles, then the tail */
         for (int t = 0; ok && t < 2; ++t) {

@@ -5,6 +5,7 @@
 #include <stdint.h>
 #include "gemm_mfma.hpp"
 #include "vkb_launch.h"
+#include "vkb_nn_launch.h"
 #include "vkblas_nn.h"
 
 namespace vkb {
@@ -86,6 +87,48 @@ __device__ __forceinline__ float wave_sum(float v) {
 }
 __device__ __forceinline__ float wave_max(float v) {
     return wave_reduce(v, -INFINITY, [](float a, float b) { return fmaxf(a, b); });
+}
+
+// The factor of a cross entropy's D, and where it and its inverse go
+// (vkb_launch_pad in vkb_nn_launch.h; to: fp16's 2^13).
+struct Scale {
+    float* scal;
+    float beta, to;
+    int find;
+};
+template <typename T>
+static inline Scale with_to(vkb_scale s) {
+    return Scale{s.scal, s.beta, sizeof(T) == 2 && !is_bf16<T> ? 8192.0f : 1.0f, s.find};
+}
+// By the largest itself, not a power of two near it: equal loss gradients (a
+// mean's) then round the target's p - 1 near -1 almost exactly, where any other
+// factor puts one and the same error on every row.
+__device__ __forceinline__ float scale_by(const Scale& s, float top) {
+    return top > 1e-30f && top < 1e30f ? s.to / top : 1.0f;
+}
+__device__ __forceinline__ void set_scale(const Scale& s, float top) {
+    s.scal[0] = scale_by(s, top);
+    s.scal[1] = top > 1e-30f && top < 1e30f ? top / s.to : 1.0f;
+    s.scal[2] = s.beta;
+    s.scal[3] = 1.0f;
+    s.scal[4] = 0.0f;
+}
+// The factor in every lane: read, or found by this wave over all M rows (the
+// wave with `write` leaves it for the products that follow).
+__device__ __forceinline__ float scale_of(const Scale& s, const float* dloss, uint32_t M, bool write, int lane) {
+    if (!s.scal) return 1.0f;
+    if (!s.find) return s.scal[0];
+    float top = 0.0f;
+    for (uint32_t m = 0; m < M; m += 256) {
+        float v[4];
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) v[i] = fabsf(dloss[min(m + 64 * i + lane, M - 1)]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, v[i]);
+    }
+    top = wave_max(top);
+    if (write && lane == 0) set_scale(s, top);
+    return scale_by(s, top);
 }
 
 constexpr float LOG2E = 1.4426950408889634f;

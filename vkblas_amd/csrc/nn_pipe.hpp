@@ -74,8 +74,8 @@ static int launch_xent_stats(const vkb_op_args* a, const int64_t* target, float*
 
 template <typename T>
 static int launch_xent_grad(const vkb_op_args* a, uint32_t Ms, uint32_t Ns, uint32_t v0, uint32_t V,
-                            const int64_t* target, int64_t ignore, const float* lse, const float* dloss, const float* scal, void* D, int64_t ldd,
-                            hipStream_t st) {
+                            const int64_t* target, int64_t ignore, const float* lse, const float* dloss,
+                            vkb_scale scale, void* D, int64_t ldd, hipStream_t st) {
     XentParams p = op_params<T, XentParams>(a);
     p.target = target;
     p.Ms = Ms;
@@ -85,7 +85,7 @@ static int launch_xent_grad(const vkb_op_args* a, uint32_t Ms, uint32_t Ns, uint
     p.ignore = ignore;
     p.lse = lse;
     p.dloss = dloss;
-    p.scal = scal;
+    p.scale = with_to<T>(scale);
     p.C = D;
     p.ldc = ldd;
     return launch_tiles<T, XentGradOp<T>>(a, p, st);
@@ -104,8 +104,8 @@ static int launch_xent_grad(const vkb_op_args* a, uint32_t Ms, uint32_t Ns, uint
     }                                                                                                                \
     extern "C" int vkb_launch_xent_grad_##NAME(const vkb_op_args* a, uint32_t Ms, uint32_t Ns, uint32_t v0,          \
                                                uint32_t V, const int64_t* target, int64_t ignore, const float* lse,  \
-                                               const float* dloss, const float* scal, void* D, int64_t ldd,          \
+                                               const float* dloss, vkb_scale scale, void* D, int64_t ldd,            \
                                                void* st) {                                                           \
-        return vkb::launch_xent_grad<T>(a, Ms, Ns, v0, V, target, ignore, lse, dloss, scal, D, ldd,                  \
+        return vkb::launch_xent_grad<T>(a, Ms, Ns, v0, V, target, ignore, lse, dloss, scale, D, ldd,                 \
                                         (hipStream_t)st);                                                            \
     }

@@ -15,9 +15,14 @@ struct PadJobs {
     // workgroup 0, where scal is set: the loss gradients' scale
     uint32_t M;
     const float* dloss;
-    float beta, to;
-    float* scal;
+    Scale scale;
 };
+
+// Row r of matrices of M rows below each other (two at most)
+__device__ __forceinline__ void split_row(uint64_t r, uint32_t M, uint32_t& s, uint32_t& m) {
+    s = r >= M;
+    m = (uint32_t)(r - (s ? M : 0u));
+}
 
 __device__ __forceinline__ void find_scale(const PadJobs& p) {
     __shared__ float sh[WORK / 64];
@@ -34,21 +39,13 @@ __device__ __forceinline__ void find_scale(const PadJobs& p) {
     __syncthreads();
     if (threadIdx.x) return;
     for (uint32_t i = 1; i < WORK / 64; ++i) top = fmaxf(top, sh[i]);
-    // by the largest itself, not a power of two near it: equal loss gradients
-    // (a mean's) then round the target's p - 1 near -1 almost exactly, where
-    // any other factor puts one and the same error on every row
-    const bool fine = top > 1e-30f && top < 1e30f;
-    p.scal[0] = fine ? p.to / top : 1.0f;
-    p.scal[1] = fine ? top / p.to : 1.0f;
-    p.scal[2] = p.beta;
-    p.scal[3] = 1.0f;
-    p.scal[4] = 0.0f;
+    set_scale(p.scale, top);
 }
 
 template <typename T>
 __global__ __launch_bounds__(WORK) void pad_kernel(PadJobs p) {
     constexpr int VEC = Elem<T>::VEC;
-    if (p.scal && blockIdx.x == 0) {
+    if (p.scale.scal && blockIdx.x == 0) {
         find_scale(p);
         return;
     }
@@ -58,7 +55,8 @@ __global__ __launch_bounds__(WORK) void pad_kernel(PadJobs p) {
     const T* A = (const T*)j.src;
     T* P = (T*)j.dst;
     for_chunks((uint64_t)j.S * j.Mp, j.Np / VEC, p.first[k], p.first[k + 1] - p.first[k], [&](uint64_t r, uint32_t c) {
-        const uint32_t s = (uint32_t)(r / j.Mp), m = (uint32_t)(r - (uint64_t)s * j.Mp);
+        uint32_t s, m;
+        split_row(r, j.Mp, s, m);
         const int64_t n = (int64_t)c * VEC;
         u32x4 v = {0u, 0u, 0u, 0u};
         if (m < j.M) v = ld_chunk(A + ((int64_t)s * j.M + m) * j.ld, n, j.N);
@@ -66,23 +64,28 @@ __global__ __launch_bounds__(WORK) void pad_kernel(PadJobs p) {
     });
 }
 
+// values of a thread (bf16 174 x 41152 x 2084, its weight's gradient: 4 76 us, 8 68)
+constexpr int UNPAD_VEC = 8;
+
 struct UnpadJobs {
     vkb_unpad_job job[2];
     uint32_t first[3];
     int n;
 };
 
-// four values a thread: of fp32 or of T, either side
+// of fp32 or of T, either side
 template <typename T>
 __global__ __launch_bounds__(WORK) void unpad_kernel(UnpadJobs p) {
     const int k = p.n > 1 && blockIdx.x >= p.first[1];
     const vkb_unpad_job& j = p.job[k];
     const bool sf = j.type == VKB_T_F32, df = j.out_type == VKB_T_F32;
-    constexpr int VEC = 4;
+    constexpr int VEC = UNPAD_VEC;
     for_chunks((uint64_t)j.S * j.M, (j.N + VEC - 1) / VEC, p.first[k], p.first[k + 1] - p.first[k],
                [&](uint64_t r, uint32_t c) {
         const int64_t n = (int64_t)c * VEC;
-        const int64_t from = ((int64_t)(r / j.M) * j.Mp + (int64_t)(r % j.M)) * j.ldp + n, to = (int64_t)r * j.ldc + n;
+        uint32_t s, m;
+        split_row(r, j.M, s, m);
+        const int64_t from = ((int64_t)s * j.Mp + m) * j.ldp + n, to = (int64_t)r * j.ldc + n;
         float x[VEC] = {0.f, 0.f, 0.f, 0.f};
         const bool all = n + VEC <= j.N;
         const int have = all ? VEC : (int)(j.N - n);
@@ -147,11 +150,9 @@ extern "C" int vkb_launch_pad(int type, const vkb_pad_job* jobs, int n, uint32_t
     p.n = n;
     p.M = M;
     p.dloss = dloss;
-    p.beta = beta;
-    p.to = type == VKB_T_F16 ? 8192.0f : 1.0f;
-    p.scal = scal;
     const bool ok = with_type(type, [&](auto t) {
         using T = decltype(t);
+        p.scale = with_to<T>(vkb_scale{scal, beta, 0});
         uint32_t at = scal ? 1 : 0;
         for (int i = 0; i < n; ++i) {
             p.job[i] = jobs[i];
@@ -173,7 +174,7 @@ extern "C" int vkb_launch_unpad(const vkb_unpad_job* jobs, int n, void* stream) 
     for (int i = 0; i < n; ++i) {
         p.job[i] = jobs[i];
         p.first[i] = at;
-        at += chunk_blocks((uint64_t)jobs[i].S * jobs[i].M, (jobs[i].N + 3) / 4);
+        at += chunk_blocks((uint64_t)jobs[i].S * jobs[i].M, (jobs[i].N + UNPAD_VEC - 1) / UNPAD_VEC);
         if (jobs[i].type != VKB_T_F32) type = jobs[i].type;
         if (jobs[i].out_type != VKB_T_F32) type = jobs[i].out_type;
     }

@@ -40,6 +40,14 @@ int vkb_launch_scale(int type, uint32_t M, uint32_t N, void* C, int64_t ldc, flo
  * that is divided by the largest |dloss| of M: scal[0] = s = 1 / max |dloss|
  * (fp16: 2^13 times that; 1 where the largest is 0, infinite or outside 1e-30
  * .. 1e30), scal[1] = 1 / s, scal[2] = beta, scal[3] = 1, scal[4] = 0. */
+/* ... or found by the kernels that compute D themselves (find; M of at most
+ * VKB_SCALE_ROWS), which saves the launch where there are no copies. */
+#define VKB_SCALE_ROWS 1024u
+typedef struct vkb_scale {
+    float* scal;                     /* NULL: no scale */
+    float beta;
+    int find;
+} vkb_scale;
 #define VKB_PAD_JOBS 3
 typedef struct vkb_pad_job {
     const void* src;
@@ -84,10 +92,10 @@ int vkb_launch_xent_rows(uint32_t M, uint32_t V, const float* z, int64_t ldz, co
                          float* loss, float* lse, void* stream);
 int vkb_launch_xent_finish(uint32_t M, uint32_t V, uint32_t S, const float* parts, const float* zt,
                            const int64_t* target, int64_t ignore, float* loss, float* lse, void* stream);
-/* D = scal[0] * dloss * (exp(z - lse) - [v == target]), scal NULL = 1. */
+/* D = scal[0] * dloss * (exp(z - lse) - [v == target]), without scal by 1. */
 int vkb_launch_xent_grad(int type, uint32_t M, uint32_t n, uint32_t v0, uint32_t V, const float* z, int64_t ldz,
                          const int64_t* target, int64_t ignore, const float* lse, const float* dloss,
-                         const float* scal, void* D, int64_t ldd, void* stream);
+                         vkb_scale scale, void* D, int64_t ldd, void* stream);
 
 /* The operators for up to VKB_FEW rows (few.hip), operands at any alignment.
  * forward: y = x w^T, R rows of w, fp32; or (glu) y = h = act(G) * U of R
@@ -98,7 +106,10 @@ int vkb_launch_xent_grad(int type, uint32_t M, uint32_t n, uint32_t v0, uint32_t
  * matrices of M x K that reduce adds up.  D (M x R) is the gated
  * projection's [dG | dU] from dh and gu, or the cross entropy's from z, fp32.
  * vkb_few_slices fills in kthreads and slice.  K of at least 16 bytes. */
-#define VKB_FEW 16
+#define VKB_FEW 32
+/* whether rows of a forward pass go on the matrix units; R: the weight's rows (then
+ * up to VKB_FEW, else up to 16) */
+static inline int vkb_few_mfma(uint32_t M, uint64_t R) { return M > 8 && R >= 4096; }
 #define VKB_FEW_BACK 8           /* rows of the backward pass */
 typedef struct vkb_few_forward {
     const void *x, *w;
@@ -146,7 +157,7 @@ int vkb_launch_xent_stats_op(const vkb_op_args* a, const int64_t* target, float*
  * N: at least those, at most them rounded up to 128, Ns a multiple of 8 */
 int vkb_launch_xent_grad_op(const vkb_op_args* a, uint32_t Ms, uint32_t Ns, uint32_t v0, uint32_t V,
                             const int64_t* target, int64_t ignore, const float* lse, const float* dloss,
-                            const float* scal, void* D, int64_t ldd, void* stream);
+                            vkb_scale scale, void* D, int64_t ldd, void* stream);
 
 #ifdef __cplusplus
 }

@@ -172,9 +172,9 @@ template <typename T>
 __global__ __launch_bounds__(WORK) void xent_grad_kernel(uint32_t M, uint32_t n, uint32_t v0, uint32_t V,
                                                             const float* z, int64_t ldz, const int64_t* target,
                                                             int64_t ignore, const float* lse, const float* dloss,
-                                                            const float* scal, T* D, int64_t ldd) {
+                                                            Scale scale, T* D, int64_t ldd) {
     constexpr int VEC = Elem<T>::VEC;
-    const float sc = scal ? scal[0] : 1.0f;
+    const float sc = scale_of(scale, dloss, M, blockIdx.x == 0 && threadIdx.x < 64, threadIdx.x & 63);
     for_chunks(M, (n + VEC - 1) / VEC, 0, gridDim.x, [&](uint64_t m, uint32_t k) {
         const int64_t c = (int64_t)k * VEC, t = target[m];
         const float l = lse[m];
@@ -227,11 +227,11 @@ extern "C" int vkb_launch_xent_rows(uint32_t M, uint32_t V, const float* z, int6
 
 extern "C" int vkb_launch_xent_grad(int type, uint32_t M, uint32_t n, uint32_t v0, uint32_t V, const float* z,
                                     int64_t ldz, const int64_t* target, int64_t ignore, const float* lse,
-                                    const float* dloss, const float* scal, void* D, int64_t ldd, void* stream) {
+                                    const float* dloss, vkb_scale scale, void* D, int64_t ldd, void* stream) {
     const bool ok = with_type(type, [&](auto t) {
         using T = decltype(t);
         hipLaunchKernelGGL((xent_grad_kernel<T>), dim3(chunk_blocks(M, chunks_of<T>(n))), dim3(WORK), 0,
-                           (hipStream_t)stream, M, n, v0, V, z, ldz, target, ignore, lse, dloss, scal, (T*)D, ldd);
+                           (hipStream_t)stream, M, n, v0, V, z, ldz, target, ignore, lse, dloss, with_to<T>(scale), (T*)D, ldd);
     });
     return ok ? (int)hipGetLastError() : (int)hipErrorInvalidValue;
 }
