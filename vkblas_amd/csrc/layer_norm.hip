@@ -8,7 +8,9 @@
 // (and in the backward pass the running sums of dw and db) stay in registers
 // too, and the next row's loads leave before the present row's reductions.
 // 16-byte accesses of any alignment; columns past N are zeros that no
-// statistic counts.
+// statistic counts.  us (TB/s read and written; a 1 GiB copy reaches 5.2): 8192 x
+// 4096 bf16 with fp32 parameters forward 24.5 (5.4), backward 33.1 (6.1) and the
+// sums' join 4.8; 1003 x 997 fp32 gradients in one launch 9.5; one row 3.5.
 #include <type_traits>
 #include "nn_common.hpp"
 #include "vkb_nn_launch.h"
