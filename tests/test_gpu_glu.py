@@ -43,7 +43,8 @@ SIZES = [(1, 1, 1), (1, 64, 64), (1, 3, 8), (2, 40, 9), (3, 17, 515), (4, 70, 41
          (9, 51, 1031), (16, 250, 700), (15, 64, 1024), (17, 65, 96), (1, 500, 784), (2, 129, 72), (7, 256, 512), (16, 320, 128), (33, 100, 100),
          (64, 128, 256), (65, 192, 192), (100, 33, 57), (128, 128, 128), (200, 500, 784), (255, 320, 64),
          (256, 128, 128), (257, 129, 128), (300, 200, 320), (511, 264, 192), (130, 72, 1000),
-         (9, 2100, 77), (16, 2048, 1031), (17, 2050, 515), (31, 2500, 9), (32, 9001, 130)]
+         (9, 2100, 77), (16, 2048, 1031), (17, 2050, 515), (31, 2500, 9), (32, 9001, 130), (1500, 700, 200),
+         (1000, 500, 1000), (70, 15, 40), (70, 16, 32)]
 
 
 @pytest.mark.parametrize("M,N,K", SIZES)

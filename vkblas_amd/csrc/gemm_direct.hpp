@@ -137,22 +137,28 @@ struct DirectOperand {
     }
 };
 
+// The workgroup's sums in LDS, rows padded.
+template <int MF, int NF>
+struct DirectSums {
+    static constexpr int LDR = 16 * NF + 4;
+    float wave[4][16 * MF * LDR];
+};
+
 // T, TC, AK, BKM as gemm_kernel; MF x NF fragments of 16 rows / columns per
-// workgroup, U K steps of loads in flight per wave.
+// workgroup, U K steps of loads in flight per wave; workgroup bid of nwg.
 template <typename T, typename TC, bool AK, bool BKM, int MF, int NF, int U>
-__global__ __launch_bounds__(256) void gemm_direct_kernel(KParams p) {
+__device__ __forceinline__ void direct_tile_run(const KParams& p, uint32_t bid, uint32_t nwg,
+                                                DirectSums<MF, NF>& sums) {
     constexpr int TM = 16 * MF, TN = 16 * NF;
     constexpr int KS = 4 * Elem<T>::VEC;            // k per step
-    constexpr int LDR = TN + 4;                     // padded row of the sums in LDS
-    __shared__ float red[4][TM * LDR];
+    constexpr int LDR = DirectSums<MF, NF>::LDR;
+    auto& red = sums.wave;
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 15, g = lane >> 4;
 
     // tile / batch / split decode with XCD-aware remap, as gemm_kernel
-    uint32_t bid = blockIdx.x;
-    const uint32_t nwg = gridDim.x;
     if ((nwg & 7u) == 0) bid = (bid & 7u) * (nwg >> 3) + (bid >> 3);
     const uint32_t per = p.tiles_m * p.tiles_n;
     const uint32_t z = bid / per;
@@ -300,6 +306,12 @@ __global__ __launch_bounds__(256) void gemm_direct_kernel(KParams p) {
             }
         }
     }
+}
+
+template <typename T, typename TC, bool AK, bool BKM, int MF, int NF, int U>
+__global__ __launch_bounds__(256) void gemm_direct_kernel(KParams p) {
+    __shared__ DirectSums<MF, NF> sums;
+    direct_tile_run<T, TC, AK, BKM, MF, NF, U>(p, blockIdx.x, gridDim.x, sums);
 }
 
 }  // namespace vkb

@@ -39,6 +39,7 @@ typedef struct {
     size_t used;                 /* bytes planned */
     int held;
     int written;                 /* an output's kernel is enqueued */
+    int path;                    /* of the last product */
     vkblas_status_t st;
 } op_call;
 
@@ -47,6 +48,7 @@ static void op_begin(op_call* c, const char* what, void* stream) {
     c->stream = stream;
     c->what = what;
     c->gemm_bytes = VKB_WS_HEADER;
+    c->path = VKBLAS_PATH_NONE;
 }
 
 /* Plan: a product of the call (its scratch), then its buffers, whose offset
@@ -110,6 +112,7 @@ static int product(op_call* c, vkblas_dtype_t ab, vkblas_dtype_t ct, vkblas_op_t
         c->st = c->written || (out && st == VKBLAS_ERR_PARTIAL) ? VKBLAS_ERR_PARTIAL : VKBLAS_ERR_INIT;
         return 0;
     }
+    c->path = vkblas_last_path();
     if (out) c->written = 1;
     return 1;
 }
@@ -117,7 +120,7 @@ static int product(op_call* c, vkblas_dtype_t ab, vkblas_dtype_t ct, vkblas_op_t
 static vkblas_status_t op_end(op_call* c, int kernel) {
     if (c->held) vkb_ws_release(&c->ws);
     vkb_prof_end(&c->prof, c->stream, c->what, c->st == VKBLAS_OK);
-    if (c->st == VKBLAS_OK) vkb_engine_ran(kernel >= VKBLAS_KERNEL_JOINED ? vkblas_last_path() : VKBLAS_PATH_NONE, kernel);
+    if (c->st == VKBLAS_OK) vkb_engine_ran(c->path, kernel);
     return c->st;
 }
 
@@ -327,6 +330,26 @@ static vkblas_status_t few_backward(op_call* c, vkblas_dtype_t type, vkblas_dtyp
     return op_end(c, VKBLAS_KERNEL_FEW);
 }
 
+/* Whether the two products of a gradient run side by side (pair.hip): where
+ * both sums are short enough for four waves and no kernel for more columns is
+ * ahead (us, one after the other / side by side, M R K: bf16 97 384 256 12.9 / 10.1,
+ * 512 1024 1024 21.4 / 20.5, 64 1024 4096 16.5 / 34, 166 3328 944 25.2 / 31.5; 1547 512
+ * 64 27.3 / 20.4; fp32 103 560 2240 29.2 / 20.7, 29 640 4456 22.8 / 29.1). */
+static int pairs(vkblas_dtype_t t, uint32_t M, uint32_t R, uint32_t K, uint32_t ldd, uint32_t ldw, uint32_t ldx) {
+    const int fits = t == VKBLAS_DT_F32 ? M <= 2560 && R <= 2560 && (M > 64 || K <= 512)
+                   : (M <= 1024 && R <= 1024 && (K % 8 || K <= 1280) && (uint64_t)R * K <= 2u << 20) ||
+                         (M <= 4096 && R <= 2560 && K <= 256);
+    return fits && 2.0 * M * R * K <= 2e9 && vkb_pair_fits(t, M, R, K, ldd, ldw, ldx);
+}
+static int pair(op_call* c, vkblas_dtype_t t, vkblas_dtype_t wt, uint32_t M, uint32_t R, uint32_t K, const void* d,
+                uint32_t ldd, const void* w, uint32_t ldw, void* dx, uint32_t lddx, scalars sx, const void* x,
+                uint32_t ldx, void* dw, uint32_t lddw, scalars sw) {
+    c->path = VKBLAS_PATH_TILE64;
+    const vkb_pair_scalars px = {sx.alpha, sx.beta, sx.alpha_dev, sx.beta_dev};
+    const vkb_pair_scalars pw = {sw.alpha, sw.beta, sw.alpha_dev, sw.beta_dev};
+    return step(c, vkb_launch_pair(t, wt, M, R, K, d, ldd, w, ldw, dx, lddx, &px, x, ldx, dw, lddw, &pw, c->stream), 1);
+}
+
 /* A gradient over no rows: C = beta * C. */
 static vkblas_status_t empty_gradient(op_call* c, vkblas_dtype_t type, uint32_t M, uint32_t N, void* C, uint32_t ldc,
                                       float beta) {
@@ -510,8 +533,9 @@ vkblas_status_t vkblas_glu_backward_async(vkblas_dtype_t type, vkblas_act_t act,
     const int px = dx && Kp != K, pw = dw && (Kp != K || Np != N);
     const vkblas_dtype_t wt = pw && beta != 0.0f ? VKBLAS_DT_F32 : dw_type;
     const uint32_t ldxo = px ? Kp : lddx, ldwo = pw ? Kp : lddw;
-    if (dx) need_gemm(&c, type, type, VKBLAS_OP_N, VKBLAS_OP_N, M, Kp, 2 * Np, dgu, ldd, ow.p, ow.ld, ldxo);
-    if (dw) need_gemm(&c, type, wt, VKBLAS_OP_T, VKBLAS_OP_N, 2 * Np, Kp, Mp, dgu, ldd, ox.p, ox.ld, ldwo);
+    const int both = dx && dw && !px && !pw && Mp == M && pairs(type, M, 2 * N, K, ldd, ow.ld, ox.ld);
+    if (dx && !both) need_gemm(&c, type, type, VKBLAS_OP_N, VKBLAS_OP_N, M, Kp, 2 * Np, dgu, ldd, ow.p, ow.ld, ldxo);
+    if (dw && !both) need_gemm(&c, type, wt, VKBLAS_OP_T, VKBLAS_OP_N, 2 * Np, Kp, Mp, dgu, ldd, ox.p, ox.ld, ldwo);
     const size_t o_d = dgu ? 0 : buf(&c, (uint64_t)Mp * ldd * es);
     place(&c, &ox, type);
     place(&c, &ow, type);
@@ -525,6 +549,11 @@ vkblas_status_t vkblas_glu_backward_async(vkblas_dtype_t type, vkblas_act_t act,
     int ok = step(&c, vkb_launch_glu_join_backward(type, act, M, N, dh, lddh, gu, ldgu, d, ldd, Mp, Np, stream),
                   dgu != NULL) &&
              brought(&c, &jobs, type, 0, NULL, 0.0f, NULL);
+    if (ok && both) {
+        pair(&c, type, dw_type, M, 2 * N, K, d, ldd, ow.p, ow.ld, dx, lddx, host_scalars(1.0f, 0.0f), ox.p, ox.ld, dw, lddw,
+             host_scalars(1.0f, beta));
+        return op_end(&c, VKBLAS_KERNEL_JOINED);
+    }
     if (ok && dx)
         ok = product(&c, type, type, VKBLAS_OP_N, VKBLAS_OP_N, M, Kp, 2 * Np, host_scalars(1.0f, 0.0f), d, ldd, ow.p,
                      ow.ld, xo, ldxo, !px);
@@ -684,12 +713,14 @@ vkblas_status_t vkblas_linear_xent_backward_async(vkblas_dtype_t type, uint32_t 
     const uint32_t ldxo = acc ? (uint32_t)round_up(Kp, 4) : lddx;
     const int pw = dw && vpad;
     const vkblas_dtype_t wt = (pw || rest) && beta != 0.0f ? VKBLAS_DT_F32 : dw_type;
+    const int both = dx && dw && n == V && !rest && !acc && !pw && Mp == M && pairs(type, M, V, K, ldd, ow.ld, ox.ld);
     for (int i = 0; i < 2; ++i) {   /* a piece of n columns, and the last one */
         const uint32_t cols = i ? V % n : n;
         if (!cols) continue;
         const uint32_t main = whole ? (vpad ? (uint32_t)round_up(cols, 128) : cols / 128 * 128) : cols;
         if (!fused)
             need_gemm(&c, type, VKBLAS_DT_F32, VKBLAS_OP_N, VKBLAS_OP_T, M, cols, K, x, ldx, w, ldw, ldd);
+        if (both) continue;
         if (dx && main) need_gemm(&c, type, xt, VKBLAS_OP_N, VKBLAS_OP_N, M, Kp, main, NULL, ldd, ow.p, ow.ld, ldxo);
         if (dw && main)
             need_gemm(&c, type, pw ? wt : dw_type, VKBLAS_OP_T, VKBLAS_OP_N, main, Kp, Mp, NULL, ldd, ox.p, ox.ld,
@@ -739,6 +770,12 @@ vkblas_status_t vkblas_linear_xent_backward_async(vkblas_dtype_t type, uint32_t 
                          ldx, wv, ldw, z, ldd, 0) &&
                  step(&c, vkb_launch_xent_grad(type, M, cols, (uint32_t)v, V, z, ldd, target, ignore_index, lse, dloss,
                                                scale, d, ldd, stream), 0);
+        }
+        if (ok && both) {
+            const scalars sx = {1.0f, 0.0f, scal ? scal + 1 : NULL, scal ? scal + 4 : NULL};
+            const scalars sw = {1.0f, beta, scal ? scal + 1 : NULL, scal ? scal + 2 : NULL};
+            pair(&c, type, dw_type, M, V, K, d, ldd, wv, ow.ld, dx, lddx, sx, ox.p, ox.ld, dw, lddw, sw);
+            break;
         }
         /* the whole tiles, then the tail */
         for (int t = 0; ok && t < 2; ++t) {

@@ -97,6 +97,17 @@ int vkb_launch_xent_grad(int type, uint32_t M, uint32_t n, uint32_t v0, uint32_t
                          const int64_t* target, int64_t ignore, const float* lse, const float* dloss,
                          vkb_scale scale, void* D, int64_t ldd, void* stream);
 
+/* dx = D W and dw = beta dw + D^T x of a small gradient in one launch (pair.hip):
+ * D M x R, W R x K, x M x K; dx of type, dw of w_type. */
+typedef struct vkb_pair_scalars {
+    float alpha, beta;
+    const void *alpha_dev, *beta_dev;   /* fp32, in alpha's and beta's place where set */
+} vkb_pair_scalars;
+int vkb_pair_fits(int type, uint32_t M, uint32_t R, uint32_t K, uint32_t ldd, uint32_t ldw, uint32_t ldx);
+int vkb_launch_pair(int type, int w_type, uint32_t M, uint32_t R, uint32_t K, const void* d, uint32_t ldd,
+                    const void* w, uint32_t ldw, void* dx, uint32_t lddx, const vkb_pair_scalars* sx, const void* x,
+                    uint32_t ldx, void* dw, uint32_t lddw, const vkb_pair_scalars* sw, void* stream);
+
 /* The operators for up to VKB_FEW rows (few.hip), operands at any alignment.
  * forward: y = x w^T, R rows of w, fp32; or (glu) y = h = act(G) * U of R
  * columns, w of 2 R rows, and gu = [G | U] unless NULL.  K of at least 16
