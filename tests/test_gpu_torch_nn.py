@@ -88,6 +88,33 @@ def test_strided_inputs_and_no_gradients():
 
 
 @pytest.mark.gpu
+def test_projections_are_kept_for_a_backward_pass_only(monkeypatch):
+    import vkblas_amd as vk
+    from vkblas_amd import torch_nn as vnn
+    x, w = values(50, 128, dt="bf16", seed=1).cuda(), values(64, 128, dt="bf16", seed=2).cuda()
+    kept, call = [], vk.glu_async
+    monkeypatch.setattr(vk, "glu_async", lambda *a, **k: (kept.append(a[11]), call(*a, **k))[1])
+    vnn.gated_linear(x, w)
+    w.requires_grad_()
+    with torch.no_grad():
+        vnn.gated_linear(x, w)
+    with torch.inference_mode():
+        vnn.gated_linear(x, w)
+    assert kept == [None] * 3
+    assert vnn.gated_linear(x, w).requires_grad and kept[-1]
+
+
+@pytest.mark.gpu
+def test_empty_rows_are_refused():
+    from vkblas_amd import torch_nn as vnn
+    x, w = torch.zeros(4, 0, device="cuda"), torch.zeros(6, 0, device="cuda")
+    for call in (lambda: vnn.layer_norm(x), lambda: vnn.gated_linear(x, w),
+                 lambda: vnn.linear_cross_entropy(x, w, torch.zeros(4, dtype=torch.int64, device="cuda"))):
+        with pytest.raises(ValueError, match="empty"):
+            call()
+
+
+@pytest.mark.gpu
 def test_example_learns():
     sys.path.insert(0, os.path.join(REPO, "examples"))
     import train_step

@@ -43,6 +43,8 @@ def _ptr(t):
 def _check(name, x, weight, dims, same_type):
     if x.dim() < 1 or x.dtype not in _TYPES or not x.is_cuda:
         raise ValueError(f"{name}: x must be an fp32, fp16 or bf16 tensor on a GPU")
+    if not x.shape[-1]:
+        raise ValueError(f"{name}: x's rows are empty: {tuple(x.shape)}")
     if weight is not None:
         if weight.dim() != dims or weight.shape[-1] != x.shape[-1] or weight.device != x.device:
             raise ValueError(f"{name}: a weight of {dims} dimension(s), the last {x.shape[-1]}, on x's device; "
@@ -92,11 +94,10 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
 
 class _GatedLinear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, act):
+    def forward(ctx, x, weight, act, keep):
         m, w = _rows(x), _rows(weight)
         N = w.shape[0] // 2
         h = torch.empty(m.shape[0], N, dtype=m.dtype, device=m.device)
-        keep = any(ctx.needs_input_grad[:2])
         gu = torch.empty(m.shape[0], 2 * N, dtype=m.dtype, device=m.device) if keep else None
         with torch.cuda.device(m.device):
             vk.glu_async(_TYPES[m.dtype], act, m.shape[0], N, m.shape[1], _ptr(m), _ld(m), _ptr(w), _ld(w), _ptr(h), N,
@@ -116,7 +117,7 @@ class _GatedLinear(torch.autograd.Function):
             vk.glu_backward_async(_TYPES[m.dtype], ctx.act, m.shape[0], N, m.shape[1], _ptr(d), _ld(d), _ptr(gu), 2 * N,
                                   _ptr(m), _ld(m), _ptr(w), _ld(w), None, 0, _ptr(dx), m.shape[1], _ptr(dw), m.shape[1],
                                   _TYPES[w.dtype], 0.0, stream=_stream(m))
-        return dx.view(*dh.shape[:-1], m.shape[1]) if dx is not None else None, dw, None
+        return dx.view(*dh.shape[:-1], m.shape[1]) if dx is not None else None, dw, None, None
 
 
 def gated_linear(x, weight, activation="silu"):
@@ -126,7 +127,10 @@ def gated_linear(x, weight, activation="silu"):
         raise ValueError("gated_linear: the weight's rows are the gate's and as many of the up projection")
     if activation not in ACTIVATIONS:
         raise ValueError(f"gated_linear: activation {activation!r}, not one of {sorted(ACTIVATIONS)}")
-    return _GatedLinear.apply(x, weight, ACTIVATIONS[activation])
+    # both projections are kept only for a backward pass; inside a Function grad mode is off and a parameter
+    # asks for its gradient under no_grad too
+    keep = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad)
+    return _GatedLinear.apply(x, weight, ACTIVATIONS[activation], keep)
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
