@@ -66,7 +66,7 @@ typedef enum {
     VKBLAS_KERNEL_NORM_LONG = 11,       /* layer norm, rows read again          */
     VKBLAS_KERNEL_JOINED = 12,          /* GEMMs by their plans, then a kernel
                                            over their results                   */
-    VKBLAS_KERNEL_FUSED = 13,           /* inside the pipelined GEMM kernel     */
+    VKBLAS_KERNEL_FUSED = 13,           /* at the end of a GEMM kernel's tiles  */
     VKBLAS_KERNEL_FEW = 14              /* one pass over the weight, few rows   */
 } vkblas_kernel_t;
 

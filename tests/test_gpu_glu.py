@@ -71,6 +71,43 @@ def test_strides_and_alignment(M, N, K, dt, pad, off):
     check_forward(forward(x, w, dt, "gelu", pad=pad, off=off), x, w, dt, "gelu")
 
 
+# small calls on tiles with both projections: of 32 rows and of 64, ragged in M and N, K shorter than a step, on
+# one, past some, and past every step that is loaded ahead; rows at any alignment, NaN behind them
+@pytest.mark.parametrize("M,N", [(6, 500), (33, 17), (64, 250), (97, 31), (400, 123), (1000, 300)])
+@pytest.mark.parametrize("K", [3, 16, 40, 129, 500])
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+def test_small_tiles(M, N, K, dt):
+    x, w = R.values(M, K, dt, 70), R.values(2 * N, K, dt, 71, K ** -0.5)
+    for kw in (dict(), dict(keep=False), dict(pad=8), dict(pad=3, off=1)):
+        check_forward(forward(x, w, dt, "gelu_tanh", **kw), x, w, dt, "gelu_tanh")
+        if M > 32:
+            assert vk.last_kernel() == vk.KERNEL_FUSED
+
+
+def test_small_call_under_capture():
+    """A small fp32 call needs no workspace: captured, and each replay equal to the eager result."""
+    M, N, K = 200, 77, 130
+    x, w = torch.randn(M, K, device="cuda"), torch.randn(2 * N, K, device="cuda")
+    h = torch.zeros(M, N, device="cuda")
+
+    def call():
+        vk.glu_async(vk.DT_F32, vk.ACT_SILU, M, N, K, x.data_ptr(), K, w.data_ptr(), K, h.data_ptr(), N,
+                     stream=stream())
+    call()
+    torch.cuda.synchronize()
+    eager = h.clone()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        call()
+    for _ in range(3):
+        h.zero_()
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(h, eager)
+        call()
+
+
 # K that ends inside a step, in its first one, on it, and NaN behind each row; few tiles and many, of both sizes
 @pytest.mark.parametrize("M,N", [(300, 136), (1100, 3300), (2100, 4400)])
 @pytest.mark.parametrize("K", [8, 32, 64, 72, 136, 200, 232, 328])

@@ -144,37 +144,15 @@ struct DirectSums {
     float wave[4][16 * MF * LDR];
 };
 
-// T, TC, AK, BKM as gemm_kernel; MF x NF fragments of 16 rows / columns per
-// workgroup, U K steps of loads in flight per wave; workgroup bid of nwg.
-template <typename T, typename TC, bool AK, bool BKM, int MF, int NF, int U>
-__device__ __forceinline__ void direct_tile_run(const KParams& p, uint32_t bid, uint32_t nwg,
-                                                DirectSums<MF, NF>& sums) {
-    constexpr int TM = 16 * MF, TN = 16 * NF;
+// The tile's sums over klen k from its operands, left in LDS: wave w's part in
+// sums.wave[w], to be added in wave order.  All 256 threads of the workgroup.
+template <typename T, bool AK, bool BKM, int MF, int NF, int U, typename OA, typename OB>
+__device__ __forceinline__ void direct_sums(const OA& oa, const OB& ob, int klen, DirectSums<MF, NF>& sums) {
     constexpr int KS = 4 * Elem<T>::VEC;            // k per step
     constexpr int LDR = DirectSums<MF, NF>::LDR;
-    auto& red = sums.wave;
-
-    const int tid = threadIdx.x, lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, g = lane >> 4;
-
-    // tile / batch / split decode with XCD-aware remap, as gemm_kernel
-    if ((nwg & 7u) == 0) bid = (bid & 7u) * (nwg >> 3) + (bid >> 3);
-    const uint32_t per = p.tiles_m * p.tiles_n;
-    const uint32_t z = bid / per;
-    const uint32_t t = bid - z * per;
-    const uint32_t b = z / p.split;
-    const uint32_t s = z - b * p.split;
-    const int m_lo = (int)(t % p.tiles_m) * TM, n_lo = (int)(t / p.tiles_m) * TN;
-    const int m0 = AK ? m_lo : min(m_lo, (int)p.M - TM);
-    const int n0 = BKM ? n_lo : min(n_lo, (int)p.N - TN);
-
-    const int kbeg = (int)(s * p.kps);
-    const int klen = (int)min(p.K - (uint32_t)kbeg, p.kps);
-    DirectOperand<T, AK, MF> oa;
-    DirectOperand<T, BKM, NF> ob;
-    oa.init((const T*)p.A + (int64_t)b * p.sa, p.lda, m0, (int)p.M, kbeg, r, g);
-    ob.init((const T*)p.B + (int64_t)b * p.sb, p.ldb, n0, (int)p.N, kbeg, r, g);
 
     floatx4 acc[MF][NF];
 #pragma unroll
@@ -245,7 +223,7 @@ __device__ __forceinline__ void direct_tile_run(const KParams& p, uint32_t bid, 
     // ---- the four waves' sums, added in wave order ----
     // acc[i][j][e] is row (AK ? 16 i + r : MF r + i), column (BKM ? 16 j +
     // 4 g + e : NF (4 g + e) + j) of the tile
-    float* mine = red[wave];
+    float* mine = sums.wave[wave];
 #pragma unroll
     for (int i = 0; i < MF; ++i) {
         float* row = mine + (AK ? 16 * i + r : MF * r + i) * LDR;
@@ -260,6 +238,39 @@ __device__ __forceinline__ void direct_tile_run(const KParams& p, uint32_t bid, 
         }
     }
     __syncthreads();
+}
+
+// T, TC, AK, BKM as gemm_kernel; MF x NF fragments of 16 rows / columns per
+// workgroup, U K steps of loads in flight per wave; workgroup bid of nwg.
+template <typename T, typename TC, bool AK, bool BKM, int MF, int NF, int U>
+__device__ __forceinline__ void direct_tile_run(const KParams& p, uint32_t bid, uint32_t nwg,
+                                                DirectSums<MF, NF>& sums) {
+    constexpr int TM = 16 * MF, TN = 16 * NF;
+    constexpr int LDR = DirectSums<MF, NF>::LDR;
+    auto& red = sums.wave;
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int r = lane & 15, g = lane >> 4;
+
+    // tile / batch / split decode with XCD-aware remap, as gemm_kernel
+    if ((nwg & 7u) == 0) bid = (bid & 7u) * (nwg >> 3) + (bid >> 3);
+    const uint32_t per = p.tiles_m * p.tiles_n;
+    const uint32_t z = bid / per;
+    const uint32_t t = bid - z * per;
+    const uint32_t b = z / p.split;
+    const uint32_t s = z - b * p.split;
+    const int m_lo = (int)(t % p.tiles_m) * TM, n_lo = (int)(t / p.tiles_m) * TN;
+    const int m0 = AK ? m_lo : min(m_lo, (int)p.M - TM);
+    const int n0 = BKM ? n_lo : min(n_lo, (int)p.N - TN);
+
+    const int kbeg = (int)(s * p.kps);
+    const int klen = (int)min(p.K - (uint32_t)kbeg, p.kps);
+    DirectOperand<T, AK, MF> oa;
+    DirectOperand<T, BKM, NF> ob;
+    oa.init((const T*)p.A + (int64_t)b * p.sa, p.lda, m0, (int)p.M, kbeg, r, g);
+    ob.init((const T*)p.B + (int64_t)b * p.sb, p.ldb, n0, (int)p.N, kbeg, r, g);
+
+    direct_sums<T, AK, BKM, MF, NF, U>(oa, ob, klen, sums);
 
     float alpha, beta;
     load_scalars(p, alpha, beta);

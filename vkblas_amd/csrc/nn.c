@@ -419,6 +419,29 @@ vkblas_status_t vkblas_layer_norm_backward_async(vkblas_dtype_t type, vkblas_dty
 
 /* ------------------------------------------------------- gated projection */
 
+/* Whether the gated projection runs on small tiles that take both halves of w
+ * (glu_direct.hip); off: some operand's rows lie off 16-byte units.  Those tiles win
+ * where the launches and the fill of a pipeline are most of the time (us, other
+ * kernels / these, tiles of 32 x 16 in brackets):
+ *  - fp32 as a product and a pass over it: 200 x 500 x 784 11.2 / 9.0, 1000 x 60 x 96
+ *    7.9 / 3.9, 1000 x 500 x 301 20.6 / 12.2; past K = 512 from K / 8 tiles on: 64 x 500
+ *    x 1536 (64) 14.7 / 17.6, 400 x 250 x 2048 (208) 27.1 / 22.5; up to 16 rows the
+ *    decode kernels win past K = 512: 12 x 500 x 784 7.0 / 7.8; K = 4096 32.2 / 38.0;
+ *  - 16-bit against the pipelined kernel: 200 x 500 x 256 8.4 / 3.8, 100 x 250 x 1024
+ *    10.1 / 6.4, 400 x 500 x 784 (416) 9.7 / 7.9, x 1024 10.7 / 10.2; 400 x 1024 x 512
+ *    (832) 7.4 / 10.8; against a product and a pass: 200 x 250 x 2048 13.0 / 9.9, x 4096
+ *    17.0 / 16.8; 12 x 500 x 784 6.0 / 4.8, x 2048 6.2 / 8.1;
+ *  - 16-bit off 16-byte units until copies pay: 200 x 500 x 1001 14.2 / 10.9, 400 x 500
+ *    x 1001 (copied) 14.9 / 19.5. */
+static int glu_direct(vkblas_dtype_t t, uint32_t M, uint32_t N, uint32_t K, uint32_t ldx, uint32_t ldw, int off) {
+    const uint64_t t32 = (uint64_t)((M + 31) / 32) * ((N + 15) / 16), t64 = (uint64_t)((M + 63) / 64) * ((N + 31) / 32);
+    const double flops = 4.0 * M * N * K;
+    if (t64 > 256 || K > 2048 || !vkb_glu_direct_fits(t, M, N, K, ldx, ldw)) return 0;
+    if (t == VKBLAS_DT_F32) return flops <= 1e9 && (K <= 512 || (M > 16 && t32 >= K / 8));
+    if (M <= 16) return K <= 1024 && t32 <= 256;
+    return off ? flops < 5e8 : t32 <= (K < 1024 ? 512 : 256);
+}
+
 vkblas_status_t vkblas_glu_async(vkblas_dtype_t type, vkblas_act_t act, uint32_t M, uint32_t N, uint32_t K,
                                  const void* x, uint32_t ldx, const void* w, uint32_t ldw, void* h, uint32_t ldh,
                                  void* gu, uint32_t ldgu, void* stream) {
@@ -433,12 +456,18 @@ vkblas_status_t vkblas_glu_async(vkblas_dtype_t type, vkblas_act_t act, uint32_t
     if (vkb_engine_trace()) fprintf(stderr, "[vkblas] glu type=%d act=%d M=%u N=%u K=%u\n", (int)type, (int)act, M, N, K);
     vkb_op_args a;
     operand ox = as_is(x, ldx, 1, M, K), ow = as_is(w, ldw, 2, N, K);
-    if (few_forward(type, M, 2 * (uint64_t)N, K, 4,
-                    K % vec_of(type) || off_units(type, x, ldx) || off_units(type, w, ldw))) {
+    const int off = K % vec_of(type) || off_units(type, x, ldx) || off_units(type, w, ldw);
+    if (few_forward(type, M, 2 * (uint64_t)N, K, 4, off)) {
         if (room(&c) != VKBLAS_OK) return c.st;
         const vkb_few_forward p = {x, w, h, gu, ldx, ldw, ldh, ldgu, M, N, K, (int)act};
         step(&c, vkb_launch_few_forward(type, &p, 1, stream), 1);
         return op_end(&c, VKBLAS_KERNEL_FEW);
+    }
+    if (glu_direct(type, M, N, K, ldx, ldw, off)) {
+        if (room(&c) != VKBLAS_OK) return c.st;
+        c.path = VKBLAS_PATH_TILE64;
+        step(&c, vkb_launch_glu_direct(type, act, M, N, K, x, ldx, w, ldw, h, ldh, gu, ldgu, stream), 1);
+        return op_end(&c, VKBLAS_KERNEL_FUSED);
     }
     if (fusable(type, M, N, K, &ox, &ow, 128, &a)) {
         place(&c, &ox, type);

@@ -78,6 +78,10 @@ int vkb_launch_glu_join(int type, int act, uint32_t M, uint32_t N, const float* 
 int vkb_launch_glu_join_backward(int type, int act, uint32_t M, uint32_t N, const void* dh, int64_t lddh,
                                  const void* gu, int64_t ldgu, void* dgu, int64_t lddgu, uint32_t Mp, uint32_t Np,
                                  void* stream);
+/* ... of a small call in one launch, product and all (glu_direct.hip) */
+int vkb_glu_direct_fits(int type, uint32_t M, uint32_t N, uint32_t K, uint32_t ldx, uint32_t ldw);
+int vkb_launch_glu_direct(int type, int act, uint32_t M, uint32_t N, uint32_t K, const void* x, uint32_t ldx,
+                          const void* w, uint32_t ldw, void* h, uint32_t ldh, void* gu, uint32_t ldgu, void* stream);
 
 /* Linear cross entropy (xent.hip).  stats: over z, columns v0 .. v0 + n - 1
  * of the logits, the pair (max, sum of exp(z - max)) of each row and each
