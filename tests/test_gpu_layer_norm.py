@@ -144,6 +144,21 @@ def test_backward(M, N, dt, wt, gt):
     assert all(torch.equal(a, b) for a, b in zip(got, again)), "equal calls differ"
 
 
+# rows and columns on both sides of where a workgroup takes 16 columns and where 32, last columns ragged
+@pytest.mark.parametrize("M,N", [(256, 33), (257, 9), (300, 17), (511, 2047), (512, 2049), (700, 1000), (1003, 997),
+                                 (1024, 1024), (1024, 1040)])
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_backward_of_columns(dt, M, N):
+    x, dy, w = R.values(M, N, dt, 24), R.values(M, N, dt, 25), R.values(1, N, dt, 26)[0]
+    _, mean, rstd = R.norm(x, w, w, EPS)
+    mean, rstd = mean.float().double(), rstd.float().double()
+    dw0 = R.values(1, N, "f32", 27, 3.0)
+    for kw in (dict(), dict(pad=1, off=1, want="wb"), dict(beta=0.5, dw0=dw0)):
+        got = backward(dy, x, w, mean, rstd, dt, dt, "f32", **kw)
+        check_backward(got, dy, x, w, mean, rstd, dt, "f32",
+                       **{k: v for k, v in kw.items() if k in ("beta", "dw0", "want")})
+
+
 @pytest.mark.parametrize("M,N", [(3, 100), (70, 777), (4, 3000), (3, 6000), (2, 20000)])
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
 def test_backward_forms(dt, M, N):

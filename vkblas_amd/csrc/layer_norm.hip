@@ -514,8 +514,9 @@ __global__ __launch_bounds__(1024) void layer_norm_reduce_kernel(const float* pa
 
 // The gradients of few rows in one launch, without partial sums: the first
 // workgroups take dx's rows (a wave or a workgroup each, as the maps above),
-// the others 32 columns of dw and db each, from the rows themselves.  dx must
-// not be dy or x where both are wanted (the others still read them): then two
+// the others 32 columns of dw and db each, from the rows themselves; or 16 where
+// the walk down the rows is the longest chain of loads and twice the workgroups
+// still find idle CUs.  dx must not be dy or x where both are wanted (the others still read them): then two
 // launches, the columns' first.
 constexpr int FEW_THREADS = 1024;
 
@@ -579,33 +580,34 @@ __device__ __forceinline__ void few_dx(uint32_t M, uint32_t N, uint32_t waves, c
     }
 }
 
-template <typename T, typename G>
+template <int COLS, typename T, typename G>
 __device__ __forceinline__ void few_dw(uint32_t block, uint32_t M, uint32_t N, const T* dy, int64_t lddy, const T* x,
                                        int64_t ldx, const float* mean, const float* rstd, G* dw, G* db, float beta) {
-    __shared__ float sh[16][32];
+    constexpr uint32_t SLICES = FEW_THREADS / COLS;
+    __shared__ float sh[16][COLS];
     constexpr int U = 8;         // rows in flight
-    const uint32_t slice = threadIdx.x >> 5;
-    const uint32_t n = block * 32 + (threadIdx.x & 31);
+    const uint32_t slice = threadIdx.x / COLS;
+    const uint32_t n = block * COLS + threadIdx.x % COLS;
     float sw = 0.0f, sb = 0.0f;
     if (n < N)
-        for (uint32_t m = slice; m < M; m += 32 * U) {
+        for (uint32_t m = slice; m < M; m += SLICES * U) {
             float d[U], h[U];
 #pragma unroll
             for (uint32_t i = 0; i < U; ++i) {
-                const uint32_t r = min(m + 32 * i, M - 1);
+                const uint32_t r = min(m + SLICES * i, M - 1);
                 d[i] = (float)dy[(int64_t)r * lddy + n];
                 h[i] = ((float)x[(int64_t)r * ldx + n] - mean[r]) * rstd[r];
             }
 #pragma unroll
             for (uint32_t i = 0; i < U; ++i)
-                if (m + 32 * i < M) {
+                if (m + SLICES * i < M) {
                     sw += d[i] * h[i];
                     sb += d[i];
                 }
         }
-    sw = join_slices<32>(sw, sh);
-    sb = join_slices<32>(sb, sh);
-    if (threadIdx.x >= 32 || n >= N) return;
+    sw = join_slices<COLS>(sw, sh);
+    sb = join_slices<COLS>(sb, sh);
+    if (threadIdx.x >= COLS || n >= N) return;
     if (dw) put_grad(dw + n, sw, beta);
     if (db) put_grad(db + n, sb, beta);
 }
@@ -613,13 +615,17 @@ __device__ __forceinline__ void few_dw(uint32_t block, uint32_t M, uint32_t N, c
 template <typename T, typename W, int MAP, int EPT>
 __global__ __launch_bounds__(FEW_THREADS) void layer_norm_few_kernel(
     uint32_t M, uint32_t N, uint32_t waves, uint32_t dx_blocks, const T* dy, int64_t lddy, const T* x, int64_t ldx,
-    const W* w, const float* mean, const float* rstd, T* dx, int64_t lddx, void* dw, void* db, bool g_f32, float beta) {
+    const W* w, const float* mean, const float* rstd, T* dx, int64_t lddx, void* dw, void* db, bool g_f32, float beta,
+    bool narrow) {
+    const uint32_t block = blockIdx.x - dx_blocks;
     if (blockIdx.x < dx_blocks) {
         few_dx<T, W, MAP, EPT>(M, N, waves, dy, lddy, x, ldx, w, mean, rstd, dx, lddx);
     } else if (g_f32) {
-        few_dw<T, float>(blockIdx.x - dx_blocks, M, N, dy, lddy, x, ldx, mean, rstd, (float*)dw, (float*)db, beta);
+        if (narrow) few_dw<16, T, float>(block, M, N, dy, lddy, x, ldx, mean, rstd, (float*)dw, (float*)db, beta);
+        else few_dw<32, T, float>(block, M, N, dy, lddy, x, ldx, mean, rstd, (float*)dw, (float*)db, beta);
     } else {
-        few_dw<T, T>(blockIdx.x - dx_blocks, M, N, dy, lddy, x, ldx, mean, rstd, (T*)dw, (T*)db, beta);
+        if (narrow) few_dw<16, T, T>(block, M, N, dy, lddy, x, ldx, mean, rstd, (T*)dw, (T*)db, beta);
+        else few_dw<32, T, T>(block, M, N, dy, lddy, x, ldx, mean, rstd, (T*)dw, (T*)db, beta);
     }
 }
 
@@ -746,16 +752,20 @@ extern "C" int vkb_launch_layer_norm_few(int type, int w_type, uint32_t M, uint3
                                          float beta, void* stream) {
     if (g_type != type && g_type != VKB_T_F32) return (int)hipErrorInvalidValue;
     bool fits = false;
+    // us, 32 / 16 columns a workgroup: fp32 500 x 512 4.9 / 3.8, 1000 x 997 8.7 / 7.1, 500 x
+    // 2048 7.6 / 6.2, bf16 1000 x 1024 7.7 / 5.3; 256 x 1024 level, 139 x 2048 3.7 / 4.5, 1000
+    // x 2048 11.1 / 13.5, 500 x 4096 8.7 / 10.2
+    const bool narrow = M > 256 && N <= 2048 && (uint64_t)M * N <= 1u << 20;
     const bool ok = with_types(type, w_type, [&](auto tt, auto tw) {
         using T = decltype(tt);
         using W = decltype(tw);
         fits = with_map(N, [&](auto map, auto ept) {
             const uint32_t waves = RowMap<T, map.value, ept.value>::waves(N);
             const uint32_t rows = map.value == ONE ? FEW_THREADS / 64 : 1;
-            const uint32_t rb = dx ? (M + rows - 1) / rows : 0, cb = dw || db ? (N + 31) / 32 : 0;
+            const uint32_t rb = dx ? (M + rows - 1) / rows : 0, cols = narrow ? 16 : 32, cb = dw || db ? (N + cols - 1) / cols : 0;
             hipLaunchKernelGGL((layer_norm_few_kernel<T, W, map.value, ept.value>), dim3(rb + cb), dim3(FEW_THREADS), 0,
                                (hipStream_t)stream, M, N, waves, rb, (const T*)dy, lddy, (const T*)x, ldx, (const W*)w,
-                               mean, rstd, (T*)dx, lddx, dw, db, g_type == VKB_T_F32, beta);
+                               mean, rstd, (T*)dx, lddx, dw, db, g_type == VKB_T_F32, beta, narrow);
         });
     });
     return ok && fits ? (int)hipGetLastError() : (int)hipErrorInvalidValue;
