@@ -159,6 +159,22 @@ def test_backward_of_columns(dt, M, N):
                        **{k: v for k, v in kw.items() if k in ("beta", "dw0", "want")})
 
 
+@pytest.mark.parametrize("N", [1100, 2100, 3000, 5000, 8000, 9000])
+def test_equal_calls_of_rows_of_several_waves(N):
+    """Each element of dx is one thread's: no two write it, so equal calls give equal bits, time after time."""
+    M = 300
+    x, dy, w = (torch.randn(r, N, device="cuda").half() for r in (M, M, 1))
+    mean, rstd = x.float().mean(1), 1 / x.float().std(1)
+    outs = []
+    for _ in range(20):
+        dx, dw, db = torch.empty_like(x), *torch.empty(2, N, device="cuda", dtype=torch.half)
+        vk.layer_norm_backward_async(vk.DT_F16, vk.DT_F16, M, N, dy.data_ptr(), N, x.data_ptr(), N, w.data_ptr(),
+                                     mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), N, dw.data_ptr(), db.data_ptr(),
+                                     vk.DT_F16, 0.0, stream=stream())
+        outs.append((dx, dw, db))
+    assert all(torch.equal(a, b) for o in outs[1:] for a, b in zip(o, outs[0]))
+
+
 @pytest.mark.parametrize("M,N", [(3, 100), (70, 777), (4, 3000), (3, 6000), (2, 20000)])
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
 def test_backward_forms(dt, M, N):

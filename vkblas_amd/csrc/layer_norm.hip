@@ -528,10 +528,12 @@ __device__ __forceinline__ void few_dx(uint32_t M, uint32_t N, uint32_t waves, c
     constexpr int VEC = R::VEC, NV = R::NV;
     __shared__ float2 sh[FEW_THREADS / 64];
     const int wave = threadIdx.x >> 6;
-    const int t = MAP == ONE ? (threadIdx.x & 63) : threadIdx.x, tpr = MAP == ONE ? 64 : (int)waves * 64;
+    const int tpr = MAP == ONE ? 64 : (int)waves * 64;
+    // waves past the row's start past its last chunk (t of tpr on would be another
+    // thread's next one): none is theirs, they add and store nothing
+    const int t = MAP == ONE ? (int)(threadIdx.x & 63) : (int)threadIdx.x + ((int)threadIdx.x < tpr ? 0 : NV * tpr);
     const uint32_t m = MAP == ONE ? blockIdx.x * (FEW_THREADS / 64) + wave : blockIdx.x;
     if (MAP == ONE && m >= M) return;   // (no barrier there)
-    // waves past the row's hold no chunk of their own: they add and store nothing
     const Chunks<T, NV> ch(t, tpr, N);
     const T *xr = x + (int64_t)m * ldx, *dr = dy + (int64_t)m * lddy;
     const float mu = mean[m], r = rstd[m];
