@@ -516,8 +516,8 @@ __global__ __launch_bounds__(1024) void layer_norm_reduce_kernel(const float* pa
 // workgroups take dx's rows (a wave or a workgroup each, as the maps above),
 // the others 32 columns of dw and db each, from the rows themselves; or 16 where
 // the walk down the rows is the longest chain of loads and twice the workgroups
-// still find idle CUs.  dx must not be dy or x where both are wanted (the others still read them): then two
-// launches, the columns' first.
+// still find idle CUs.  dx must not be dy or x where both are wanted (the others
+// still read them): then two launches, the columns' first.
 constexpr int FEW_THREADS = 1024;
 
 template <typename T, typename W, int MAP, int EPT>
