@@ -147,8 +147,9 @@ vkblas_status_t vkblas_linear_xent_async(
  *   ignored rows, NaN for rows whose target is outside [0, V)
  *   dx = D w,  dw = beta * dw + D^T x
  * The logits are computed again in pieces of the vocabulary.  D is rounded
- * to type for the two products, divided by the largest |dloss| (fp16: times
- * 2^13 more, which keeps it in range), a factor they take out again in fp32.
+ * to type for the two products, divided by the largest finite |dloss| of the
+ * rows that count (fp16: times 2^13 more, which keeps it in range), a factor
+ * they take out again in fp32.  dloss of an ignored row may hold anything.
  *   dx: M x K or NULL; dw: V x K of dw_type or NULL
  * Needs a workspace.
  */

@@ -246,7 +246,7 @@ static void place(op_call* c, operand* o, vkblas_dtype_t t) {
     if (o->copy) o->off = buf(c, (uint64_t)o->S * o->Mp * o->Np * type_size(t));
 }
 /* After room(): a call's copies, gathered by bring() and launched by brought()
- * together with the scalars of a cross entropy's gradient (scal, or NULL). */
+ * together with the scalars of a cross entropy's gradient (scale, or NULL). */
 typedef struct {
     vkb_pad_job job[VKB_PAD_JOBS];
     int n;
@@ -257,9 +257,8 @@ static void bring(op_call* c, copies* j, operand* o, const void* src, uint32_t l
     o->p = d;
     j->job[j->n++] = (vkb_pad_job){src, d, lds, o->S, o->M, o->N, o->Mp, o->Np};
 }
-static int brought(op_call* c, const copies* j, vkblas_dtype_t t, uint32_t M, const float* dloss, float beta,
-                   float* scal) {
-    return (j->n == 0 && !scal) || step(c, vkb_launch_pad(t, j->job, j->n, M, dloss, beta, scal, c->stream), 0);
+static int brought(op_call* c, const copies* j, vkblas_dtype_t t, const vkb_scale* scale) {
+    return (j->n == 0 && !scale) || step(c, vkb_launch_pad(t, j->job, j->n, scale, c->stream), 0);
 }
 
 /* A copied row's columns: rows start on whole lines (bf16 gradient of a cross
@@ -476,7 +475,7 @@ vkblas_status_t vkblas_glu_async(vkblas_dtype_t type, vkblas_act_t act, uint32_t
         copies jobs = {.n = 0};
         bring(&c, &jobs, &ox, x, ldx);
         bring(&c, &jobs, &ow, w, ldw);
-        if (brought(&c, &jobs, type, 0, NULL, 0.0f, NULL)) {
+        if (brought(&c, &jobs, type, NULL)) {
             bound(&a, &ox, &ow);
             step(&c, vkb_launch_glu(&a, act, h, ldh, gu, ldgu, stream), 1);
         }
@@ -503,7 +502,7 @@ vkblas_status_t vkblas_glu_async(vkblas_dtype_t type, vkblas_act_t act, uint32_t
     copies jobs = {.n = 0};
     bring(&c, &jobs, &ox, x, ldx);
     bring(&c, &jobs, &ow, w, ldw);
-    int ok = brought(&c, &jobs, type, 0, NULL, 0.0f, NULL);
+    int ok = brought(&c, &jobs, type, NULL);
     for (uint64_t m = 0; ok && m < M; m += rows) {
         const uint32_t n = (uint32_t)(M - m < rows ? M - m : rows);
         float* z = direct ? (float*)gu : (float*)at(&c, o_z);
@@ -577,7 +576,7 @@ vkblas_status_t vkblas_glu_backward_async(vkblas_dtype_t type, vkblas_act_t act,
     bring(&c, &jobs, &ow, w, ldw);
     int ok = step(&c, vkb_launch_glu_join_backward(type, act, M, N, dh, lddh, gu, ldgu, d, ldd, Mp, Np, stream),
                   dgu != NULL) &&
-             brought(&c, &jobs, type, 0, NULL, 0.0f, NULL);
+             brought(&c, &jobs, type, NULL);
     if (ok && both) {
         pair(&c, type, dw_type, M, 2 * N, K, d, ldd, ow.p, ow.ld, dx, lddx, host_scalars(1.0f, 0.0f), ox.p, ox.ld, dw, lddw,
              host_scalars(1.0f, beta));
@@ -630,7 +629,7 @@ vkblas_status_t vkblas_linear_xent_async(vkblas_dtype_t type, uint32_t M, uint32
         copies jobs = {.n = 0};
         bring(&c, &jobs, &ox, x, ldx);
         bring(&c, &jobs, &ow, w, ldw);
-        if (brought(&c, &jobs, type, 0, NULL, 0.0f, NULL)) {
+        if (brought(&c, &jobs, type, NULL)) {
             bound(&a, &ox, &ow);
             if (step(&c, vkb_launch_xent_stats_op(&a, target, parts, zt, stream), 0))
                 step(&c, vkb_launch_xent_finish(M, V, S, parts, zt, target, ignore_index, loss, lse, stream), 1);
@@ -657,7 +656,7 @@ vkblas_status_t vkblas_linear_xent_async(vkblas_dtype_t type, uint32_t M, uint32
     copies jobs = {.n = 0};
     bring(&c, &jobs, &ox, x, ldx);
     bring(&c, &jobs, &ow, w, ldw);
-    int ok = brought(&c, &jobs, type, 0, NULL, 0.0f, NULL);
+    int ok = brought(&c, &jobs, type, NULL);
     uint32_t slice = 0;
     for (uint64_t v = 0; ok && v < V; v += n, slice += per) {
         const uint32_t cols = (uint32_t)(V - v < n ? V - v : n);
@@ -778,8 +777,8 @@ vkblas_status_t vkblas_linear_xent_backward_async(vkblas_dtype_t type, uint32_t 
     bring(&c, &jobs, &ox, x, ldx);
     bring(&c, &jobs, &ow, w, ldw);
     if (rest && dx) bring(&c, &jobs, &tail, (const char*)w + (uint64_t)(V - rest) * ldw * es, ldw);
-    const vkb_scale scale = {scal, beta, !jobs.n && M <= VKB_SCALE_ROWS};
-    int ok = brought(&c, &jobs, type, M, dloss, beta, scale.find ? NULL : scal);
+    const vkb_scale scale = {scal, beta, !jobs.n && M <= VKB_SCALE_ROWS, M, V, dloss, target, ignore_index};
+    int ok = brought(&c, &jobs, type, scal && !scale.find ? &scale : NULL);
     vkb_unpad_job out[2];        /* dw's rows still in the workspace, and dx */
     int outs = 0;
     int summed = 0;              /* dx holds a product already */

@@ -113,16 +113,25 @@ __device__ __forceinline__ void set_scale(const Scale& s, float top) {
     s.scal[3] = 1.0f;
     s.scal[4] = 0.0f;
 }
+// What a row adds to the search for the largest: |dloss| where it counts and is
+// finite, else 0.
+__device__ __forceinline__ float scale_row(const float* dloss, const int64_t* target, uint32_t m, int64_t V,
+                                           int64_t ignore) {
+    const float d = fabsf(dloss[m]);
+    const int64_t t = target[m];
+    return t != ignore && t >= 0 && t < V && d < INFINITY ? d : 0.0f;
+}
 // The factor in every lane: read, or found by this wave over all M rows (the
 // wave with `write` leaves it for the products that follow).
-__device__ __forceinline__ float scale_of(const Scale& s, const float* dloss, uint32_t M, bool write, int lane) {
+__device__ __forceinline__ float scale_of(const Scale& s, const float* dloss, const int64_t* target, uint32_t M,
+                                          int64_t V, int64_t ignore, bool write, int lane) {
     if (!s.scal) return 1.0f;
     if (!s.find) return s.scal[0];
     float top = 0.0f;
     for (uint32_t m = 0; m < M; m += 256) {
         float v[4];
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) v[i] = fabsf(dloss[min(m + 64 * i + lane, M - 1)]);
+        for (uint32_t i = 0; i < 4; ++i) v[i] = scale_row(dloss, target, min(m + 64 * i + lane, M - 1), V, ignore);
 #pragma unroll
         for (int i = 0; i < 4; ++i) top = fmaxf(top, v[i]);
     }

@@ -12,10 +12,9 @@ struct PadJobs {
     vkb_pad_job job[VKB_PAD_JOBS];
     uint32_t first[VKB_PAD_JOBS + 1];   // a job's first workgroup
     int n;
-    // workgroup 0, where scal is set: the loss gradients' scale
-    uint32_t M;
-    const float* dloss;
+    // workgroup 0, where its scal is set: the loss gradients' scale, over these rows
     Scale scale;
+    vkb_scale rows;
 };
 
 // Row r of matrices of M rows below each other (two at most)
@@ -27,10 +26,11 @@ __device__ __forceinline__ void split_row(uint64_t r, uint32_t M, uint32_t& s, u
 __device__ __forceinline__ void find_scale(const PadJobs& p) {
     __shared__ float sh[WORK / 64];
     float top = 0.0f;
-    for (uint32_t m = threadIdx.x; m < p.M; m += 4 * WORK) {
+    const vkb_scale& r = p.rows;
+    for (uint32_t m = threadIdx.x; m < r.M; m += 4 * WORK) {
         float v[4];
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) v[i] = m + i * WORK < p.M ? fabsf(p.dloss[m + i * WORK]) : 0.0f;
+        for (uint32_t i = 0; i < 4; ++i) v[i] = scale_row(r.dloss, r.target, min(m + i * WORK, r.M - 1), r.V, r.ignore);
 #pragma unroll
         for (int i = 0; i < 4; ++i) top = fmaxf(top, v[i]);
     }
@@ -143,17 +143,15 @@ __global__ __launch_bounds__(WORK) void scale_kernel(uint32_t M, uint32_t N, T* 
 
 using namespace vkb;
 
-extern "C" int vkb_launch_pad(int type, const vkb_pad_job* jobs, int n, uint32_t M, const float* dloss, float beta,
-                              float* scal, void* stream) {
-    if (n < 0 || n > VKB_PAD_JOBS || (n == 0 && !scal)) return (int)hipErrorInvalidValue;
+extern "C" int vkb_launch_pad(int type, const vkb_pad_job* jobs, int n, const vkb_scale* scale, void* stream) {
+    if (n < 0 || n > VKB_PAD_JOBS || (n == 0 && !scale)) return (int)hipErrorInvalidValue;
     PadJobs p{};
     p.n = n;
-    p.M = M;
-    p.dloss = dloss;
+    if (scale) p.rows = *scale;
     const bool ok = with_type(type, [&](auto t) {
         using T = decltype(t);
-        p.scale = with_to<T>(vkb_scale{scal, beta, 0});
-        uint32_t at = scal ? 1 : 0;
+        p.scale = with_to<T>(p.rows);
+        uint32_t at = scale ? 1 : 0;
         for (int i = 0; i < n; ++i) {
             p.job[i] = jobs[i];
             p.first[i] = at;

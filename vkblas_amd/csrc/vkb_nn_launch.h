@@ -36,10 +36,12 @@ int vkb_launch_scale(int type, uint32_t M, uint32_t N, void* C, int64_t ldc, flo
 /* Copies (pad.hip) between a program's S matrices of M x N below each other
  * (leading dimension ld) and the workspace, one launch for all of a call's.
  * pad: to S of Mp x Np, Np a multiple of 16 bytes, zero past M and N; all of
- * type.  With scal set, also the device scalars of products of a gradient
- * that is divided by the largest |dloss| of M: scal[0] = s = 1 / max |dloss|
- * (fp16: 2^13 times that; 1 where the largest is 0, infinite or outside 1e-30
- * .. 1e30), scal[1] = 1 / s, scal[2] = beta, scal[3] = 1, scal[4] = 0. */
+ * type.  With scale, also the device scalars of products of a gradient that
+ * is divided by the largest finite |dloss| of the M rows that count (target in
+ * [0, V) and not ignore: another row's loss gradient, whatever it holds, is no
+ * part of D): scal[0] = s = 1 / max |dloss| (fp16: 2^13 times that; 1 where
+ * the largest is outside 1e-30 .. 1e30), scal[1] = 1 / s, scal[2] = beta,
+ * scal[3] = 1, scal[4] = 0. */
 /* ... or found by the kernels that compute D themselves (find; M of at most
  * VKB_SCALE_ROWS), which saves the launch where there are no copies. */
 #define VKB_SCALE_ROWS 1024u
@@ -47,6 +49,10 @@ typedef struct vkb_scale {
     float* scal;                     /* NULL: no scale */
     float beta;
     int find;
+    uint32_t M, V;
+    const float* dloss;
+    const int64_t* target;
+    int64_t ignore;
 } vkb_scale;
 #define VKB_PAD_JOBS 3
 typedef struct vkb_pad_job {
@@ -55,8 +61,7 @@ typedef struct vkb_pad_job {
     int64_t ld;
     uint32_t S, M, N, Mp, Np;
 } vkb_pad_job;
-int vkb_launch_pad(int type, const vkb_pad_job* jobs, int n, uint32_t M, const float* dloss, float beta, float* scal,
-                   void* stream);
+int vkb_launch_pad(int type, const vkb_pad_job* jobs, int n, const vkb_scale* scale, void* stream);   /* scale NULL: none */
 /* unpad (up to 2): dst = beta * dst + src, src in rows of ldp and matrices of
  * Mp rows; type and out_type fp32 or one and the same 16-bit type */
 typedef struct vkb_unpad_job {
