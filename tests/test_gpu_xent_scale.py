@@ -53,3 +53,11 @@ def test_a_row_whose_loss_gradient_is_not_finite(M, V, K, value, dt):
     rows = torch.arange(M) != 3
     args = (x[rows], w, t[rows], lse[rows], dloss[rows])
     X.check_backward((dx[rows], None), *counted(args), dt, want="x")
+
+
+@pytest.mark.parametrize("M,V,K", SIZES)
+@pytest.mark.parametrize("loss_scale", [1e-30, 1e-28, 1e28, 1e33, 1e37])
+def test_loss_gradients_of_any_size(M, V, K, loss_scale):
+    """fp32 weight gradients of fp16 operands, far outside the type's own range."""
+    args = X.grad_inputs(M, V, K, "f16", loss_scale)
+    X.check_backward(X.backward(*args, "f16", wt="f32", want="w"), *args, "f16", wt="f32", want="w")

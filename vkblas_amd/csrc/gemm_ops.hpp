@@ -201,8 +201,8 @@ struct XentGradOp {
                                                int lane) {
         using G = Frag<WT, SH>;
         const int64_t row0 = m0 + (wave >> 1) * WT, col0 = n0 + (wave & 1) * WT;
-        const float sc = scale_of(p.scale, p.dloss, p.target, p.M, p.V, p.ignore,
-                                  blockIdx.x == 0 && wave == 0, lane);
+        const float sc = scale_of<T>(p.scale, p.dloss, p.target, p.M, p.V, p.ignore,
+                                     blockIdx.x == 0 && wave == 0, lane);
 #pragma unroll
         for (int i = 0; i < G::NF; ++i) {
             const int64_t m = row0 + G::row(lane, i);

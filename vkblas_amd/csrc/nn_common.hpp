@@ -103,12 +103,13 @@ static inline Scale with_to(vkb_scale s) {
 // By the largest itself, not a power of two near it: equal loss gradients (a
 // mean's) then round the target's p - 1 near -1 almost exactly, where any other
 // factor puts one and the same error on every row.
-__device__ __forceinline__ float scale_by(const Scale& s, float top) {
-    return top > 1e-30f && top < 1e30f ? s.to / top : 1.0f;
-}
+// Held where it and its inverse are normal fp32 numbers (of 2^-13 the smallest,
+// 1e-33, of 1 the largest, 8e37); what lies past that still fits the type.
+__device__ __forceinline__ float scale_top(float top) { return fminf(fmaxf(top, 1e-33f), 8e37f); }
+__device__ __forceinline__ float scale_by(const Scale& s, float top) { return s.to / scale_top(top); }
 __device__ __forceinline__ void set_scale(const Scale& s, float top) {
     s.scal[0] = scale_by(s, top);
-    s.scal[1] = top > 1e-30f && top < 1e30f ? top / s.to : 1.0f;
+    s.scal[1] = scale_top(top) / s.to;
     s.scal[2] = s.beta;
     s.scal[3] = 1.0f;
     s.scal[4] = 0.0f;
@@ -122,10 +123,11 @@ __device__ __forceinline__ float scale_row(const float* dloss, const int64_t* ta
     return t != ignore && t >= 0 && t < V && d < INFINITY ? d : 0.0f;
 }
 // The factor in every lane: read, or found by this wave over all M rows (the
-// wave with `write` leaves it for the products that follow).
+// wave with `write` leaves it for the products that follow).  fp32: none.
+template <typename T>
 __device__ __forceinline__ float scale_of(const Scale& s, const float* dloss, const int64_t* target, uint32_t M,
                                           int64_t V, int64_t ignore, bool write, int lane) {
-    if (!s.scal) return 1.0f;
+    if (sizeof(T) == 4 || !s.scal) return 1.0f;
     if (!s.find) return s.scal[0];
     float top = 0.0f;
     for (uint32_t m = 0; m < M; m += 256) {

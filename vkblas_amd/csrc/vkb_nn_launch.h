@@ -39,8 +39,8 @@ int vkb_launch_scale(int type, uint32_t M, uint32_t N, void* C, int64_t ldc, flo
  * type.  With scale, also the device scalars of products of a gradient that
  * is divided by the largest finite |dloss| of the M rows that count (target in
  * [0, V) and not ignore: another row's loss gradient, whatever it holds, is no
- * part of D): scal[0] = s = 1 / max |dloss| (fp16: 2^13 times that; 1 where
- * the largest is outside 1e-30 .. 1e30), scal[1] = 1 / s, scal[2] = beta,
+ * part of D): scal[0] = s = 1 / max |dloss| (fp16: 2^13 times that; a
+ * largest outside 1e-33 .. 8e37 counts as that end), scal[1] = 1 / s, scal[2] = beta,
  * scal[3] = 1, scal[4] = 0. */
 /* ... or found by the kernels that compute D themselves (find; M of at most
  * VKB_SCALE_ROWS), which saves the launch where there are no copies. */

@@ -174,7 +174,7 @@ __global__ __launch_bounds__(WORK) void xent_grad_kernel(uint32_t M, uint32_t n,
                                                             int64_t ignore, const float* lse, const float* dloss,
                                                             Scale scale, T* D, int64_t ldd) {
     constexpr int VEC = Elem<T>::VEC;
-    const float sc = scale_of(scale, dloss, target, M, V, ignore, blockIdx.x == 0 && threadIdx.x < 64, threadIdx.x & 63);
+    const float sc = scale_of<T>(scale, dloss, target, M, V, ignore, blockIdx.x == 0 && threadIdx.x < 64, threadIdx.x & 63);
     for_chunks(M, (n + VEC - 1) / VEC, 0, gridDim.x, [&](uint64_t m, uint32_t k) {
         const int64_t c = (int64_t)k * VEC, t = target[m];
         const float l = lse[m];
