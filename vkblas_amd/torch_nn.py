@@ -53,11 +53,14 @@ def _check(name, x, weight, dims, same_type):
             raise ValueError(f"{name}: weight of {weight.dtype} with x of {x.dtype}")
 
 
+# Results are allocated in the shape they are returned in: a view that a Function returns cannot be changed in place.
+
+
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
         m = _rows(x)
-        y = torch.empty(m.shape, dtype=m.dtype, device=m.device)
+        y = torch.empty(x.shape, dtype=m.dtype, device=m.device)
         mean, rstd = torch.empty(2, m.shape[0], dtype=torch.float32, device=m.device)
         ref = weight if weight is not None else bias
         ctx.w_type = _TYPES[ref.dtype] if ref is not None else _TYPES[m.dtype]
@@ -65,7 +68,7 @@ class _LayerNorm(torch.autograd.Function):
             vk.layer_norm_async(_TYPES[m.dtype], ctx.w_type, *m.shape, _ptr(m), _ld(m), _ptr(weight), _ptr(bias), eps,
                                 _ptr(y), m.shape[1], _ptr(mean), _ptr(rstd), stream=_stream(m))
         ctx.save_for_backward(m, weight, bias, mean, rstd)
-        return y.view(x.shape)
+        return y
 
     @staticmethod
     @once_differentiable
@@ -97,14 +100,14 @@ class _GatedLinear(torch.autograd.Function):
     def forward(ctx, x, weight, act, keep):
         m, w = _rows(x), _rows(weight)
         N = w.shape[0] // 2
-        h = torch.empty(m.shape[0], N, dtype=m.dtype, device=m.device)
+        h = torch.empty(*x.shape[:-1], N, dtype=m.dtype, device=m.device)
         gu = torch.empty(m.shape[0], 2 * N, dtype=m.dtype, device=m.device) if keep else None
         with torch.cuda.device(m.device):
             vk.glu_async(_TYPES[m.dtype], act, m.shape[0], N, m.shape[1], _ptr(m), _ld(m), _ptr(w), _ld(w), _ptr(h), N,
                          _ptr(gu), 2 * N, stream=_stream(m))
         ctx.act = act
         ctx.save_for_backward(m, w, gu)
-        return h.view(*x.shape[:-1], N)
+        return h
 
     @staticmethod
     @once_differentiable
@@ -138,7 +141,9 @@ class _LinearCrossEntropy(torch.autograd.Function):
     def forward(ctx, x, weight, target, ignore_index):
         m, w = _rows(x), _rows(weight)
         t = target.reshape(-1).contiguous()
-        loss, lse = torch.empty(2, m.shape[0], dtype=torch.float32, device=m.device)
+        # two tensors: loss is the program's to change, lse the backward pass's
+        loss = torch.empty(target.shape, dtype=torch.float32, device=m.device)
+        lse = torch.empty(m.shape[0], dtype=torch.float32, device=m.device)
         with torch.cuda.device(m.device):
             vk.linear_xent_async(_TYPES[m.dtype], m.shape[0], w.shape[0], m.shape[1], _ptr(m), _ld(m), _ptr(w), _ld(w),
                                  _ptr(t), ignore_index, _ptr(loss), _ptr(lse), stream=_stream(m))
@@ -170,6 +175,6 @@ def linear_cross_entropy(x, weight, target, ignore_index=-100, reduction="mean")
         raise ValueError(f"linear_cross_entropy: reduction {reduction!r}")
     loss = _LinearCrossEntropy.apply(x, weight, target, int(ignore_index))
     if reduction == "none":
-        return loss.view(target.shape)
+        return loss
     total = loss.sum()
     return total if reduction == "sum" else total / (target != ignore_index).sum()
