@@ -89,7 +89,19 @@ _NN_ARGS = {
 }
 
 
+# the kinds of those arguments, as _call.fits and _fits take them
+_NN_KINDS = {name: "".join({_u32: "u", _int: "i", _i64: "l"}.get(t, ".") for t in args)
+             for name, args in _NN_ARGS.items()}
+_RANGES = {"u": (0, 2 ** 32 - 1), "i": (-2 ** 31, 2 ** 31 - 1), "l": (-2 ** 63, 2 ** 63 - 1)}
 _nn_calls = {}      # by name: the native call, the function's address, the function
+
+
+def _fits(kinds, *args) -> bool:
+    """Whether the C types hold the whole numbers among args (_call.fits where that is not there)."""
+    return all(_RANGES[k][0] <= a <= _RANGES[k][1] for k, a in zip(kinds, args) if k in _RANGES and isinstance(a, int))
+
+
+_range_check = _fits
 
 
 def build(jobs: int = 8) -> None:
@@ -99,7 +111,7 @@ def build(jobs: int = 8) -> None:
 
 def load():
     """Load the built library (raises if it has not been built)."""
-    global _lib, _native, _ex_addr
+    global _lib, _native, _ex_addr, _range_check
     if _lib is not None:
         return _lib
     for path in (LIB_PATH, ENGINE_PATH):
@@ -136,7 +148,9 @@ def load():
         from . import _call
     except ImportError:     # not built, or for another interpreter
         _call = None
+        _range_check = _fits
     else:
+        _range_check = getattr(_call, "fits", _fits)
         _native, _ex_addr = _call.gemm_ex, ctypes.cast(L.vkblas_gemm_ex_async, ctypes.c_void_p).value
     for name, args in _NN_ARGS.items():
         fn = getattr(L, f"vkblas_{name}_async")
@@ -258,13 +272,17 @@ def gemm_batched_async(ab_type, c_type, op_a, op_b, M, N, K, alpha, A, lda, B, l
 
 
 def _nn(name, check, *args) -> int:
-    """A call of vkblas_nn.h; its status (raises if check)."""
+    """A call of vkblas_nn.h; its status (raises if check).  A number that its C type does not hold is refused like
+    the sizes that the library refuses, not passed as what is left of it."""
     if not _nn_calls:
         load()
     native, addr, fn = _nn_calls[name]
-    st = native(addr, *args)
-    if st is None:
-        st = fn(*args)
+    if not _range_check(_NN_KINDS[name], *args):
+        st = ERR_PARAM
+    else:
+        st = native(addr, *args)
+        if st is None:
+            st = fn(*args)
     if check and st != OK:
         raise VkblasError(st, f"vkblas_{name}_async")
     return st

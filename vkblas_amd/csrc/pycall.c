@@ -140,7 +140,31 @@ NN_CALL(linear_xent_backward, "piiiipipipipppipiifp",
         (I(1), U(2), U(3), U(4), P(5), U(6), P(7), U(8), P(9), (int64_t)v[10], P(11), P(12), P(13), U(14), P(15),
          U(16), I(17), f[0], P(19)))
 
+/* fits(kinds, arguments): whether the C types hold the whole numbers among
+ * them; u: uint32_t, i: int, l: int64_t, anything else is not looked at */
+static PyObject* fits(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+    (void)self;
+    Py_ssize_t kinds = 0;
+    const char* kind = n > 0 && PyUnicode_Check(a[0]) ? PyUnicode_AsUTF8AndSize(a[0], &kinds) : NULL;
+    if (!kind || kinds != n - 1) {
+        if (!PyErr_Occurred()) PyErr_Format(PyExc_TypeError, "fits takes the kinds of as many arguments as follow");
+        return NULL;
+    }
+    for (Py_ssize_t k = 0; k < kinds; ++k) {
+        PyObject* o = a[k + 1];
+        if ((kind[k] != 'u' && kind[k] != 'i' && kind[k] != 'l') || !PyLong_Check(o)) continue;
+        int past;
+        const long long v = PyLong_AsLongLongAndOverflow(o, &past);
+        if (past || (kind[k] == 'u' && (v < 0 || v > 0xffffffffll)) ||
+            (kind[k] == 'i' && (v < INT32_MIN || v > INT32_MAX)))
+            Py_RETURN_FALSE;
+    }
+    Py_RETURN_TRUE;
+}
+
 static PyMethodDef methods[] = {
+                                {"fits", (PyCFunction)(void (*)(void))fits, METH_FASTCALL,
+                                 "whether whole numbers lie in their C types' ranges"},
 #define NN_METHOD(NAME) {#NAME, (PyCFunction)(void (*)(void))NAME, METH_FASTCALL, \
                          "vkblas_" #NAME "_async by address; None if an argument is not a plain int, float or None"}
                                 NN_METHOD(layer_norm), NN_METHOD(layer_norm_backward), NN_METHOD(glu),

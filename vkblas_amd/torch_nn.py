@@ -23,9 +23,10 @@ ACTIVATIONS = {"silu": vk.ACT_SILU, "gelu": vk.ACT_GELU, "gelu_tanh": vk.ACT_GEL
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
-    """t as a matrix of its last dimension whose rows' elements are adjacent."""
+    """t as a matrix of its last dimension whose rows' elements are adjacent, and whose rows are no farther apart than
+    a leading dimension holds."""
     m = t.reshape(-1, t.shape[-1])
-    return m if m.stride(1) == 1 and m.stride(0) >= m.shape[1] else m.contiguous()
+    return m if m.stride(1) == 1 and m.shape[1] <= m.stride(0) < 2 ** 31 else m.contiguous()
 
 
 def _ld(m: torch.Tensor) -> int:
