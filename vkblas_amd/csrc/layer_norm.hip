@@ -752,7 +752,7 @@ extern "C" int vkb_launch_layer_norm_few(int type, int w_type, uint32_t M, uint3
                                          const void* x, int64_t ldx, const void* w, const float* mean,
                                          const float* rstd, void* dx, int64_t lddx, void* dw, void* db, int g_type,
                                          float beta, void* stream) {
-    if (g_type != type && g_type != VKB_T_F32) return (int)hipErrorInvalidValue;
+    if ((dw || db) && g_type != type && g_type != VKB_T_F32) return (int)hipErrorInvalidValue;
     bool fits = false;
     // us, 32 / 16 columns a workgroup: fp32 500 x 512 4.9 / 3.8, 1000 x 997 8.7 / 7.1, 500 x
     // 2048 7.6 / 6.2, bf16 1000 x 1024 7.7 / 5.3; 256 x 1024 level, 139 x 2048 3.7 / 4.5, 1000
