@@ -111,7 +111,7 @@ def build(jobs: int = 8) -> None:
 
 def load():
     """Load the built library (raises if it has not been built)."""
-    global _lib, _native, _ex_addr, _range_check
+    global _lib, _native, _ex_addr, _range_check, _nn_calls
     if _lib is not None:
         return _lib
     for path in (LIB_PATH, ENGINE_PATH):
@@ -152,11 +152,13 @@ def load():
     else:
         _range_check = getattr(_call, "fits", _fits)
         _native, _ex_addr = _call.gemm_ex, ctypes.cast(L.vkblas_gemm_ex_async, ctypes.c_void_p).value
+    calls = {}          # published whole: another thread may look while this one loads
     for name, args in _NN_ARGS.items():
         fn = getattr(L, f"vkblas_{name}_async")
         fn.argtypes = args
         fn.restype = _int
-        _nn_calls[name] = (getattr(_call, name, _ctypes_call), ctypes.cast(fn, ctypes.c_void_p).value, fn)
+        calls[name] = (getattr(_call, name, _ctypes_call), ctypes.cast(fn, ctypes.c_void_p).value, fn)
+    _nn_calls = calls
     _lib = L
     return L
 
