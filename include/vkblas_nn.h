@@ -21,7 +21,9 @@
  *
  * Workspace: calls that need one take their stream's workspace, as GEMMs that
  * split K do (vkblas_workspace_release frees it), and return VKBLAS_ERR_INIT
- * under stream capture; each function says when it needs one.
+ * under stream capture; each function says when it needs one.  A call that would
+ * use it for nothing but the partial sums of a K split then runs without the
+ * split, as a GEMM does (products of up to 64 rows, the decode kernels', aside).
  *
  * Status: VKBLAS_OK; VKBLAS_ERR_PARAM (null pointer, zero size, leading
  * dimension shorter than its row, dimension above 2^31 - 1, unknown type or

@@ -739,15 +739,37 @@ static size_t plan_ws_bytes(const vkblas_plan_t* plan, uint32_t M, uint32_t N, s
     return VKB_WS_HEADER + *part_bytes * (divided ? 1 + VKB_WAVEK_NQ : 1);
 }
 
+/* The planner's own K splits (split-K for few output tiles, the split tail)
+ * only speed a call up: where their partials have no room (the caller's
+ * scratch is smaller; a capturing stream declines the workspace) the call runs
+ * the plan without a split instead of failing: 1, and *plan is that plan.
+ * A caller's split (split_k > 1) and the decode kernels' splits keep their plan
+ * and fail: 0. */
+static int plan_unsplit(vkblas_dtype_t ab_type, vkblas_dtype_t c_type, vkblas_op_t op_a, vkblas_op_t op_b, uint32_t M,
+                        uint32_t N, uint32_t K, uint32_t lda, uint32_t ldb, uint32_t ldc, uint32_t batch,
+                        uint32_t split_k, int aligned, vkblas_plan_t* plan) {
+    if (split_k != 0 || (plan->path != VKBLAS_PATH_SPLITK && plan->path != VKBLAS_PATH_TAIL)) return 0;
+    if (plan->path == VKBLAS_PATH_SPLITK && plan->tile == VKB_TILE_64Q) return 0;
+    vkblas_plan_t one;
+    if (vkblas_plan_gemm(ab_type, c_type, op_a, op_b, M, N, K, lda, ldb, ldc, batch, 1, aligned, &one) != VKBLAS_OK ||
+        one.split != 1)
+        return 0;
+    *plan = one;
+    return 1;
+}
+
 size_t vkb_gemm_scratch_bytes(vkblas_dtype_t ab_type, vkblas_dtype_t c_type, vkblas_op_t op_a, vkblas_op_t op_b,
                               uint32_t M, uint32_t N, uint32_t K, uint32_t lda, uint32_t ldb, uint32_t ldc,
-                              int aligned) {
+                              int aligned, int* optional) {
     vkblas_plan_t plan;
     size_t part_bytes;
+    *optional = 1;
     if (vkblas_plan_gemm(ab_type, c_type, op_a, op_b, M, N, K, lda, ldb, ldc, 1, 0, aligned, &plan) != VKBLAS_OK ||
         plan.split <= 1)
         return 0;
-    return plan_ws_bytes(&plan, M, N, &part_bytes);
+    const size_t bytes = plan_ws_bytes(&plan, M, N, &part_bytes);
+    *optional = plan_unsplit(ab_type, c_type, op_a, op_b, M, N, K, lda, ldb, ldc, 1, 0, aligned, &plan);
+    return bytes;
 }
 
 /* The body of vkblas_gemm_async.  ws_ext != NULL: the split-K / decode
@@ -817,13 +839,6 @@ static vkblas_status_t gemm_impl(vkblas_dtype_t ab_type, vkblas_dtype_t c_type, 
     size_t part_bytes = 0;
     const int divided = partials && plan.path == VKBLAS_PATH_SPLITK && plan.tile == VKB_TILE_64Q;
     size_t ws_bytes = partials ? plan_ws_bytes(&plan, M, N, &part_bytes) : 0;
-    /* The planner's own K splits (split-K for few output tiles, the split
-     * tail) only speed a call up: where their partials have no room (the
-     * caller's scratch is smaller; a capturing stream declines the
-     * workspace) the call runs the plan without a split instead of failing.
-     * A caller's split (split_k > 1) and the decode kernels' splits keep
-     * their plan and fail. */
-    const int optional = split_k == 0 && (plan.path == VKBLAS_PATH_SPLITK || plan.path == VKBLAS_PATH_TAIL);
     prof_t pf;
     if (!ws_ext) prof_begin(&pf, hs);
     else memset(&pf, 0, sizeof(pf));
@@ -836,10 +851,7 @@ static vkblas_status_t gemm_impl(vkblas_dtype_t ab_type, vkblas_dtype_t c_type, 
         if (!room) ws_release(&lease);
         ws = lease.ptr;
     }
-    if (!room && optional && !divided &&
-        vkblas_plan_gemm(ab_type, c_type, op_a, op_b, M, N, K, lda, ldb, ldc, batch, 1, aligned, &plan) ==
-            VKBLAS_OK &&
-        plan.split == 1) {
+    if (!room && plan_unsplit(ab_type, c_type, op_a, op_b, M, N, K, lda, ldb, ldc, batch, split_k, aligned, &plan)) {
         if (g_trace) fprintf(stderr, "[vkblas] no room for the partials: plan without a split (%s)\n",
                              path_name(plan.path));
         partials = 0;

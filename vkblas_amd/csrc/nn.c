@@ -37,6 +37,7 @@ typedef struct {
     vkb_ws_lease ws;
     size_t gemm_bytes;           /* of the workspace, for the GEMMs' counters and partials */
     size_t used;                 /* bytes planned */
+    int must;                    /* a product has no plan without its partials */
     int held;
     int written;                 /* an output's kernel is enqueued */
     int path;                    /* of the last product */
@@ -55,8 +56,11 @@ static void op_begin(op_call* c, const char* what, void* stream) {
  * buf() returns; room() takes the workspace. */
 static void need_gemm(op_call* c, vkblas_dtype_t ab, vkblas_dtype_t ct, vkblas_op_t op_a, vkblas_op_t op_b, uint32_t M,
                       uint32_t N, uint32_t K, const void* A, uint32_t lda, const void* B, uint32_t ldb, uint32_t ldc) {
-    const size_t b = vkb_gemm_scratch_bytes(ab, ct, op_a, op_b, M, N, K, lda, ldb, ldc, aligned16(A) && aligned16(B));
+    int optional;
+    const size_t b = vkb_gemm_scratch_bytes(ab, ct, op_a, op_b, M, N, K, lda, ldb, ldc, aligned16(A) && aligned16(B),
+                                            &optional);
     if (b > c->gemm_bytes) c->gemm_bytes = b;
+    if (!optional) c->must = 1;
 }
 static size_t buf(op_call* c, uint64_t bytes) {
     if (!c->used) c->used = round_up(c->gemm_bytes, 256);
@@ -66,10 +70,12 @@ static size_t buf(op_call* c, uint64_t bytes) {
 }
 static vkblas_status_t room(op_call* c) {
     if (!vkb_engine_ready()) return c->st = VKBLAS_ERR_INIT;
+    /* wanted for nothing but K splits, the products run without it too */
+    const int optional = !c->used && !c->must;
     if (!c->used && c->gemm_bytes > VKB_WS_HEADER) c->used = c->gemm_bytes;
     if (c->used) {
-        if (vkb_ws_acquire(c->stream, c->used, &c->ws) != 0) return c->st = VKBLAS_ERR_INIT;
-        c->held = 1;
+        c->held = vkb_ws_acquire(c->stream, c->used, &c->ws) == 0;
+        if (!c->held && !optional) return c->st = VKBLAS_ERR_INIT;
     }
     vkb_prof_begin(&c->prof, c->stream);
     return VKBLAS_OK;
@@ -105,7 +111,7 @@ static int product(op_call* c, vkblas_dtype_t ab, vkblas_dtype_t ct, vkblas_op_t
     if (c->held)
         st = vkb_gemm_with_scratch(ab, ct, op_a, op_b, M, N, K, s.alpha, A, lda, B, ldb, s.beta, C, ldc, 1, 0, 0, 0,
                                    mode, s.alpha_dev, s.beta_dev, 0, c->stream, c->ws.ptr, c->gemm_bytes);
-    else   /* no workspace held: the plan has no split */
+    else   /* no workspace held: the plan has no split, or does without */
         st = vkblas_gemm_async(ab, ct, op_a, op_b, M, N, K, s.alpha, A, lda, B, ldb, s.beta, C, ldc, 1, 0, 0, 0, mode,
                                s.alpha_dev, s.beta_dev, 0, c->stream);
     if (st != VKBLAS_OK) {

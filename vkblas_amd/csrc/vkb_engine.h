@@ -25,11 +25,12 @@ vkblas_status_t vkb_gemm_with_scratch(vkblas_dtype_t ab_type, vkblas_dtype_t c_t
 
 /* Scratch bytes with which vkb_gemm_with_scratch (split_k = 0, batch 1) runs
  * the planner's own plan, its arrival counters included; 0 where that needs
- * none. */
+ * none.  *optional: without them vkblas_gemm_async runs a plan without a split
+ * (else it fails). */
 __attribute__((visibility("hidden")))
 size_t vkb_gemm_scratch_bytes(vkblas_dtype_t ab_type, vkblas_dtype_t c_type, vkblas_op_t op_a, vkblas_op_t op_b,
                               uint32_t M, uint32_t N, uint32_t K, uint32_t lda, uint32_t ldb, uint32_t ldc,
-                              int aligned);
+                              int aligned, int* optional);
 
 /* A workspace of the calling device and stream (engine.c, "Split-K and decode
  * partials"): held from vkb_ws_acquire (0, or -1: none, and nothing to
