@@ -89,10 +89,14 @@ typedef enum {
  *   projection's; h: M x N; all of one type
  *   gu: NULL, or M x 2N of the same type: G and U, kept for the backward
  *   pass (h is computed from their fp32 values)
- * Needs no workspace for M <= 4 (16 where rows lie off 16-byte units, K at
- * least one of them, and 32 for N of at least 2048 there), nor for more than 64 rows whose h has at least 96 tiles of
- * 128 x 64 (200 in fp32), K in whole 16-byte units and all rows on whole lines of
- * 128 bytes (fp32: on 16-byte units).  Other calls may take one.
+ * Needs no workspace for
+ *  - up to 4 rows, K of at least 16 bytes; where rows lie off 16-byte units up to
+ *    16 rows, or 32 for N of at least 2048;
+ *  - more than 64 rows whose h has at least 96 tiles of 128 x 64 (200 in fp32), K
+ *    in whole 16-byte units and all rows on whole lines of 128 bytes (fp32: on
+ *    16-byte units).
+ * Other calls may take one; most small ones (h of at most 256 tiles of 64 x 32, K up
+ * to 2048) are one launch of small tiles and take none.
  */
 vkblas_status_t vkblas_glu_async(
     vkblas_dtype_t type, vkblas_act_t act,

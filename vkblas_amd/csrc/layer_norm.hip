@@ -10,7 +10,9 @@
 // 16-byte accesses of any alignment; columns past N are zeros that no
 // statistic counts.  us (TB/s read and written; a 1 GiB copy reaches 5.2): 8192 x
 // 4096 bf16 with fp32 parameters forward 24.5 (5.4), backward 33.1 (6.1) and the
-// sums' join 4.8; 1003 x 997 fp32 gradients in one launch 9.5; one row 3.5.
+// sums' join 4.8; 1003 x 997 fp32 gradients in one launch 7.7 (27.5 MiB read for the operands'
+// 7.6: the rows' workgroups read them once, the columns' again, 64 bytes of a line
+// each, in two L2s); one row 3.4.
 #include <type_traits>
 #include "nn_common.hpp"
 #include "vkb_nn_launch.h"

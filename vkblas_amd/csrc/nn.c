@@ -230,8 +230,11 @@ typedef struct {
 static uint32_t vec_of(vkblas_dtype_t t) { return t == VKBLAS_DT_F32 ? 4 : 8; }
 static int off_units(vkblas_dtype_t t, const void* p, uint32_t ld) { return !aligned16(p) || ld % vec_of(t); }
 /* Whether a 16-bit operand's K steps lie across two lines each, which loads
- * both, and K is long enough for the loads to count: the kernel takes 20 to 50%
- * longer (bf16 xent 4323 x 1209 x 4984 90 us, 66 on a copy; 5886 x 79834 x 712 756, 638). */
+ * both, and K is long enough for the loads to count (us, as it is / on copies,
+ * other inputs each pass: bf16 xent 4323 x 1209 x 4984 98.7 / 82.0, 4000 x 32000 x 1000
+ * 285 / 262, 5886 x 79834 x 712 753 / 724, gated 4000 x 8000 x 4040 477 / 431).  The
+ * copies cost 3 to 8 us: level at 4000 x 4000 x 2000 (73.4 / 73.2), behind in shorter
+ * calls (1000 x 8000 x 1000 31.3 / 34.6, 4000 x 4000 x 520 32.5 / 39.0). */
 static int off_lines(vkblas_dtype_t t, uint32_t K, const void* p, uint32_t ld) {
     return t != VKBLAS_DT_F32 && K >= 512 && (((uintptr_t)p | (uint64_t)ld * 2) & 127) != 0;
 }
@@ -271,8 +274,11 @@ static int brought(op_call* c, const copies* j, vkblas_dtype_t t, const vkb_scal
  * entropy 174 x 41152 x 2084 as 2112 columns 372 us, as 2088 417) */
 static uint32_t line_k(vkblas_dtype_t t, uint32_t K) { return (uint32_t)round_up(K, K > 64 ? 64 : vec_of(t)); }
 /* x (M x K) and w (S of N x K) for x w^T inside the pipelined kernel: copied
- * where they have to be and the product is worth it.  Below 0.5 GFLOP the
- * copies' launch costs more than it saves. */
+ * where they have to be and the product is worth it (us, without / with copies,
+ * K = 1001: bf16 gated 300 x 500, 0.6 GFLOP, 22.7 / 15.0, 500 x 1000 25.3 / 17.0, xent
+ * 300 x 1000 23.3 / 19.5; below 0.5 GFLOP small tiles take such calls in 10.8.  fp32
+ * gains from about 6 GFLOP on: gated 1000 x 2000 91 / 75, xent 4000 x 4000 318 / 253; before
+ * that the copies cost more: 1000 x 2000 62 / 75, 300 x 1000 24.9 / 31.2). */
 static int fusable(vkblas_dtype_t type, uint32_t M, uint32_t N, uint32_t K, operand* x, operand* w, uint32_t cols,
                    vkb_op_args* a) {
     const uint32_t Kp = K % vec_of(type) ? line_k(type, K) : K;
@@ -337,9 +343,18 @@ static vkblas_status_t few_backward(op_call* c, vkblas_dtype_t type, vkblas_dtyp
 
 /* Whether the two products of a gradient run side by side (pair.hip): where
  * both sums are short enough for four waves and no kernel for more columns is
- * ahead (us, one after the other / side by side, M R K: bf16 97 384 256 12.9 / 10.1,
- * 512 1024 1024 21.4 / 20.5, 64 1024 4096 16.5 / 34, 166 3328 944 25.2 / 31.5; 1547 512
- * 64 27.3 / 20.4; fp32 103 560 2240 29.2 / 20.7, 29 640 4456 22.8 / 29.1). */
+ * ahead (us, one after the other / side by side, M R K:
+ *  16-bit, M and R up to 1024: 97 384 256 13.7 / 11.1, 512 512 512 13.3 / 10.6, 1000 1000
+ *   512 24.1 / 18.6; past them 1200 1000 512 26.3 / 27.6, 1000 1200 512 26.0 / 26.3; K up to
+ *   1280: 512 1024 1024 21.4 / 20.5, 1280 21.0 / 23.0, 1536 20.9 / 29.8, 64 1024 4096 16.5 /
+ *   34; R K up to 2 Mi: 166 3328 944 25.2 / 31.5;
+ *  short K, up to 256, and M to 4096: 1547 512 64 27.3 / 20.4; past them 3000 1000 320
+ *   41.3 / 42.9, 5000 1000 200 41.1 / 59.9;
+ *  fp32, M and R up to 2560: 100 1000 1024 22.4 / 16.2, 103 560 2240 29.2 / 20.7, 1000 2500
+ *   300 78.0 / 62.9; up to 64 rows K up to 512: 64 1000 512 14.8 / 13.9, 29 640 4456 22.8 /
+ *   29.1 (64 1000 1024, 19.1 / 14.4, is given away);
+ *  up to 2 GFLOP: 1000 2000 500 71.1 / 70.9, and 106.2 / 105.9 for K = 700 (long rows with a
+ *   short K would still gain: bf16 3000 2000 200 54.8 / 49.6, fp32 1000 3000 300 85.8 / 76.2)). */
 static int pairs(vkblas_dtype_t t, uint32_t M, uint32_t R, uint32_t K, uint32_t ldd, uint32_t ldw, uint32_t ldx) {
     const int fits = t == VKBLAS_DT_F32 ? M <= 2560 && R <= 2560 && (M > 64 || K <= 512)
                    : (M <= 1024 && R <= 1024 && (K % 8 || K <= 1280) && (uint64_t)R * K <= 2u << 20) ||
@@ -427,7 +442,9 @@ vkblas_status_t vkblas_layer_norm_backward_async(vkblas_dtype_t type, vkblas_dty
 /* Whether the gated projection runs on small tiles that take both halves of w
  * (glu_direct.hip); off: some operand's rows lie off 16-byte units.  Those tiles win
  * where the launches and the fill of a pipeline are most of the time (us, other
- * kernels / these, tiles of 32 x 16 in brackets):
+ * kernels / these, the same inputs each pass, tiles of 32 x 16 in brackets; other
+ * inputs each pass: fp32 200 x 500 x 784 12.1 / 10.0, bf16 100 x 250 x 1024 10.2 / 6.9,
+ * 400 x 500 x 784 11.4 / 8.6):
  *  - fp32 as a product and a pass over it: 200 x 500 x 784 11.2 / 9.0, 1000 x 60 x 96
  *    7.9 / 3.9, 1000 x 500 x 301 20.6 / 12.2; past K = 512 from K / 8 tiles on: 64 x 500
  *    x 1536 (64) 14.7 / 17.6, 400 x 250 x 2048 (208) 27.1 / 22.5; up to 16 rows the
@@ -550,7 +567,13 @@ vkblas_status_t vkblas_glu_backward_async(vkblas_dtype_t type, vkblas_act_t act,
      * worth the copies (from 4 GFLOP each on, 2 in fp32) and the layout of [dG | dU] is
      * this call's own: K in whole 16-byte units (columns of both results), M
      * (which dw sums over) in whole pairs of K steps, and N (dx sums over both
-     * halves) so that 2 N is, for an odd N from 128 rows on, else from 1024. */
+     * halves) so that 2 N is, for an odd N from 128 rows on, else from 1024.
+     * us, without / with copies, M N K: bf16 1000 1000 1001 53.6 / 45.3, 1000 2000 1001
+     * 88 / 62, 1000 2003 1024 84 / 51 (300 1000 1001, 1.2 GFLOP, 34.7 / 33.7); M alone
+     * off, 1001 2048 1024, 41.7 / 43.9; fp32 500 1003 1024 73 / 85, 1001 1003 1024 103 /
+     * 115, 1001 1024 1024 103 / 107.  N alone: bf16 128 4003 4096 111 / 100, 300 4003
+     * 2048 108 / 76, fp32 512 2003 1024 132 / 120; an even N 512 4040 2048 73 / 84,
+     * 2048 4040 2048 158 / 160. */
     const size_t es = type_size(type);
     const uint32_t vec = vec_of(type), steps = type == VKBLAS_DT_F32 ? 64 : 128;
     const int big = 4.0 * M * N * K >= (type == VKBLAS_DT_F32 ? 2e9 : 4e9);
@@ -716,7 +739,13 @@ vkblas_status_t vkblas_linear_xent_backward_async(vkblas_dtype_t type, uint32_t 
     }
     /* D of a piece of the vocabulary at a time, in type: from the pipelined
      * kernel, or over the piece's logits in fp32 (fp32: in their place).
-     * Where the products' work is worth it, their sums run over whole steps:
+     * Where the products' work is worth it, their sums run over whole steps (us,
+     * without / with, M V K: bf16, V odd, from 1 GFLOP: 500 4003 512 46.7 / 41.5, 1000
+     * 8003 512 105 / 59, below it 300 2003 512 27.8 / 32.3; V in units of 8 from 40
+     * GFLOP: 1000 40040 512 214 / 215, 2000 40040 1024 578 / 577, below it 500 4040 512
+     * 35.7 / 41.6; fp32 from 2 GFLOP: 1000 8003 512 277 / 214, 500 8003 256 92 / 95;
+     * the rows, in fp32 from 2 GFLOP: 500 8000 512 161 / 130, 1001 2000 512 104 / 104,
+     * 16-bit from 10: 1000 16000 512 79 / 81, 1000 8000 512 49.7 / 51.1):
      *  - dw's over M rows padded with zeros (D's, and a copy of x);
      *  - dx's over whole tiles of classes, and the rest of the vocabulary by a
      *    padded copy of its rows of w, whose part of dw comes by the workspace;

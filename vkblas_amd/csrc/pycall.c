@@ -1,6 +1,7 @@
 /*
  * pycall.c — the Python binding's calls without ctypes (module
- * vkblas_amd._call): vkblas_gemm_ex_async and the functions of vkblas_nn.h.
+ * vkblas_amd._call): vkblas_gemm_ex_async and the functions of vkblas_nn.h, and
+ * the check of those functions' numbers against their C types.
  *
  * A small call is bound by its launch on the host, and ctypes' conversion of
  * 25 arguments was the largest part of that: 3.1 us for vkblas_gemm_async and
