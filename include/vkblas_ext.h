@@ -67,7 +67,9 @@ typedef enum {
     VKBLAS_KERNEL_JOINED = 12,          /* GEMMs by their plans, then a kernel
                                            over their results                   */
     VKBLAS_KERNEL_FUSED = 13,           /* at the end of a GEMM kernel's tiles  */
-    VKBLAS_KERNEL_FEW = 14              /* one pass over the weight, few rows   */
+    VKBLAS_KERNEL_FEW = 14,             /* one pass over the weight, few rows   */
+    VKBLAS_KERNEL_EMBED = 15,           /* embedding and its gradient           */
+    VKBLAS_KERNEL_POLICY = 16           /* policy loss and its gradient         */
 } vkblas_kernel_t;
 
 typedef struct {

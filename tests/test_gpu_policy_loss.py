@@ -1,0 +1,249 @@
+"""vkblas_policy_loss_async and its gradient against the definition in float64: sizes around units and the small call,
+reductions, masks that leave sequences or everything empty, NaN and infinities where nothing counts, ratios at their
+bounds, no reference, advantages of a token and of a sequence, strides."""
+import math
+
+import pytest
+import torch
+
+import nn_ref as R
+import train_ref as D
+import vkblas_amd as vk
+
+pytestmark = pytest.mark.gpu
+LOW, HIGH, KL = D.f32(0.2), D.f32(0.28), D.f32(0.05)
+REDUCE = {"tokens": vk.REDUCE_TOKENS, "sequences": vk.REDUCE_SEQUENCES, "sum": vk.REDUCE_SUM}
+
+
+def stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+def inputs(B, T, seed=1, ref=True, per_token=True, masked=True, spread=0.2):
+    g = torch.Generator().manual_seed(seed)
+    old = (torch.rand(B, T, generator=g) + 1e-6).log()
+    logp = old + spread * torch.randn(B, T, generator=g)
+    r = old + 2 * spread * torch.randn(B, T, generator=g) if ref else None
+    adv = torch.randn(B, T if per_token else 1, generator=g)
+    mask = torch.ones(B, T, dtype=torch.uint8)
+    if masked:
+        mask = (torch.arange(T) < torch.randint(0, T + 1, (B, 1), generator=g)).to(torch.uint8) * 3
+        mask[torch.rand(B, T, generator=g) < 0.1] = 0
+        mask[0, 0] = 255
+        mask[1::7] = 0
+    return dict(logp=logp, old=old, ref=r, adv=adv, mask=mask, masked=masked)
+
+
+class Call:
+    """The inputs on the GPU: rows of T + pad floats, off elements past their alignment, NaN around them."""
+
+    def __init__(self, i, pad=0, off=0):
+        self.B, self.T = i["logp"].shape
+        buf = lambda v: None if v is None else R.Buf(*v.shape, "f32", pad, off, v)
+        self.bufs = [buf(i[k]) for k in ("logp", "old", "ref", "adv")]
+        self.mask = torch.full((self.B * (self.T + pad) + off,), 1, dtype=torch.uint8, device="cuda")
+        self.mask[off:].view(self.B, -1)[:, :self.T] = i["mask"].cuda()
+        args = []
+        for b in self.bufs[:3]:
+            args += [b.ptr if b else None, b.ld if b else 0]
+        a = self.bufs[3]
+        args += [a.ptr, a.ld, int(a.cols > 1 or self.T == 1)]
+        args += [self.mask.data_ptr() + off if i["masked"] else None, self.T + pad]
+        self.args, self.pad, self.off = args, pad, off
+
+    def loss(self, reduce="tokens", low=LOW, high=HIGH, kl=KL):
+        stats, norm = R.Buf(1, 4, "f32"), R.Buf(1, self.B, "f32")
+        vk.policy_loss_async(REDUCE[reduce], self.B, self.T, *self.args, low, high, kl, stats.ptr, norm.ptr,
+                             stream=stream())
+        assert vk.last_kernel() == vk.KERNEL_POLICY
+        stats.check_around()
+        norm.check_around()
+        return stats.get()[0], norm.get()[0]
+
+    def grad(self, norm, dloss, low=LOW, high=HIGH, kl=KL):
+        out, n = R.Buf(self.B, self.T, "f32", self.pad, self.off), R.Buf(1, self.B, "f32", values=norm[None])
+        dl = torch.tensor([dloss], dtype=torch.float32, device="cuda")
+        vk.policy_loss_backward_async(self.B, self.T, *self.args, low, high, kl, n.ptr, dl.data_ptr(), out.ptr, out.ld,
+                                      stream=stream())
+        out.check_around()
+        return out.get()
+
+
+def exact(i):
+    return [None if i[k] is None else i[k].double() for k in ("logp", "old", "ref", "adv")] + [i["mask"] != 0]
+
+
+def err(i):
+    """Relative error of a token's ratio and KL term: their arguments' rounding and a few operations."""
+    logp, old, ref, adv, mask = exact(i)
+    big = torch.where(mask, (logp - old).abs(), torch.zeros_like(logp)).max()
+    if ref is not None:
+        big = torch.maximum(big, torch.where(mask, (ref - logp).abs(), torch.zeros_like(logp)).max())
+    return R.STEP * (4 + float(big))
+
+
+def check_loss(got, i, reduce, low=LOW, high=HIGH, kl=KL):
+    stats, size, norm = D.policy(*exact(i), low, high, kl, reduce)
+    R.close(got[0], stats, err(i) * size + R.E * stats.abs(), "stats")
+    R.close(got[1], norm, 2 * R.E * norm, "norm")
+
+
+def check_grad(got, i, norm, dloss, low=LOW, high=HIGH, kl=KL):
+    g, size = D.policy_grad(*exact(i), low, high, kl, norm, dloss)
+    # the KL term's difference of two fp32 numbers is rounded once: e |d| <= size's own scale times e / slope of 1
+    logp, _, ref, _, mask = exact(i)
+    w = (norm * dloss).abs()[:, None]
+    diff = 0 if ref is None else torch.where(mask, w * abs(kl) * R.E * (ref - logp).abs() * torch.exp(ref - logp),
+                                             torch.zeros_like(logp))
+    R.close(got, g, err(i) * size + diff, "dlogp")
+    assert bool((got[i["mask"] == 0] == 0).all())
+
+
+# units of 256 tokens, the small call of 64 of them (one workgroup) and past it, many units of a sequence
+SIZES = [(1, 1), (1, 5), (3, 64), (8, 100), (2, 255), (2, 256), (2, 257), (64, 256), (65, 256), (63, 257), (1, 16384),
+         (1, 16385), (2, 40001), (300, 700), (5000, 3), (1, 2000001)]
+
+
+@pytest.mark.parametrize("B,T", SIZES)
+@pytest.mark.parametrize("reduce", REDUCE)
+def test_loss_and_gradient(B, T, reduce):
+    i = inputs(B, T, per_token=reduce != "sequences", ref=reduce != "sum")
+    c = Call(i)
+    got = c.loss(reduce)
+    check_loss(got, i, reduce)
+    check_grad(c.grad(got[1], 0.75), i, got[1], 0.75)
+
+
+@pytest.mark.parametrize("B,T", [(7, 130), (90, 301)])
+@pytest.mark.parametrize("pad,off", [(0, 0), (4, 0), (1, 0), (3, 1)])
+@pytest.mark.parametrize("masked", [True, False])
+def test_strides_alignment_and_no_mask(B, T, pad, off, masked):
+    i = inputs(B, T, masked=masked)
+    c = Call(i, pad, off)
+    got = c.loss("sequences")
+    check_loss(got, i, "sequences")
+    check_grad(c.grad(got[1], -2.0), i, got[1], -2.0)
+
+
+@pytest.mark.parametrize("B,T", [(6, 40), (100, 400)])
+@pytest.mark.parametrize("reduce", REDUCE)
+def test_what_does_not_count_may_hold_anything(B, T, reduce):
+    i = inputs(B, T)
+    out = i["mask"] == 0
+    clean = Call(i)
+    want = clean.loss(reduce)
+    grad = clean.grad(want[1], 1.0)
+    for v in (float("nan"), float("inf"), -float("inf"), torch.finfo(torch.float32).min):
+        for k in ("logp", "old", "ref", "adv"):
+            i[k][out] = v
+        c = Call(i)
+        assert all(torch.equal(a, b) for a, b in zip(c.loss(reduce), want))
+        assert torch.equal(c.grad(want[1], 1.0), grad)
+
+
+@pytest.mark.parametrize("B,T", [(1, 3), (5, 300), (200, 200)])
+@pytest.mark.parametrize("reduce", REDUCE)
+def test_nothing_counts(B, T, reduce):
+    i = inputs(B, T)
+    i["mask"][:] = 0
+    stats, norm = Call(i).loss(reduce)
+    assert bool((stats == 0).all()) and bool((norm == 0).all())
+    assert bool((Call(i).grad(norm, 1.0) == 0).all())
+
+
+def test_ratios_at_their_bounds():
+    """logp - old one unit to each side of log(1 + clip_high) and log(1 - clip_low), both signs of the advantage: the
+    side is the exact one."""
+    at = torch.tensor([math.log1p(HIGH), math.log1p(-LOW)], dtype=torch.float32)
+    d = torch.stack([at] + [torch.nextafter(at, at + s) for s in (1.0, -1.0)]).flatten()
+    # old of a far larger magnitude than the difference, so that an fp32 difference would round
+    old = torch.stack((torch.zeros(6), torch.full((6,), -4096.0)))
+    i = dict(logp=old + d, old=old, ref=None, mask=torch.ones(2, 6, dtype=torch.uint8), masked=True)
+    for sign in (1.0, -1.0):
+        i["adv"] = torch.full((2, 6), sign)
+        c = Call(i)
+        got = c.loss("sum")
+        check_loss(got, i, "sum")
+        assert float(got[0][2]) == float(D.policy(*exact(i), LOW, HIGH, KL, "sum")[0][2])
+        check_grad(c.grad(got[1], 1.0), i, got[1], 1.0)
+
+
+@pytest.mark.parametrize("low,high", [(0.0, 0.0), (1.0, 0.5), (3.0, 0.1), (float("inf"), float("inf")), (0.1, 1e30)])
+@pytest.mark.parametrize("kl", [0.0, 2.5, -1.0])
+def test_bounds_and_coefficients(low, high, kl):
+    low, high = D.f32(low), D.f32(high)
+    i = inputs(20, 50, spread=0.5)
+    c = Call(i)
+    got = c.loss("tokens", low, high, kl)
+    check_loss(got, i, "tokens", low, high, kl)
+    check_grad(c.grad(got[1], 1.0, low, high, kl), i, got[1], 1.0, low, high, kl)
+
+
+def test_far_apart_policies():
+    """Ratios that overflow are held by the bound for a positive advantage; kl_coef 0 leaves an infinite KL term out of
+    the loss."""
+    i = inputs(1, 4, masked=False)
+    i["old"][:], i["logp"][:] = -200.0, 0.0
+    i["ref"][:] = 200.0
+    i["adv"][:] = 1.0
+    c = Call(i)
+    stats, norm = c.loss("tokens", kl=0.0)
+    assert abs(float(stats[0]) + 1 + HIGH) < 1e-6 and math.isinf(stats[1]) and float(stats[2]) == 1.0
+    assert bool((c.grad(norm, 1.0, kl=0.0) == 0).all())
+    i["adv"][:] = -1.0
+    assert float(Call(i).loss("tokens", kl=0.0)[0][0]) == float("inf")
+    i["logp"][0, 2] = float("nan")
+    stats, norm = Call(i).loss("tokens")
+    assert math.isnan(stats[0])
+
+
+def test_small_kl_terms_keep_their_digits():
+    """exp(d) - d - 1 of d = 1e-4 is 5e-9: all of its bits, not those that a difference leaves."""
+    i = inputs(4, 64, masked=False)
+    i["old"] = i["logp"].clone()
+    i["ref"] = i["logp"] + 1e-4
+    c = Call(i)
+    got = c.loss("tokens")
+    ref = D.policy(*exact(i), LOW, HIGH, KL, "tokens")[0]
+    assert abs(float(got[0][1] / ref[1]) - 1) < 1e-5
+
+
+def test_gradient_against_differences():
+    """Central differences of the definition, h = 1e-5, away from the bounds."""
+    i = inputs(6, 30, spread=0.3)
+    logp, old, ref, adv, mask = exact(i)
+    ratio = torch.exp(logp - old)
+    near = ((ratio - 1 + LOW).abs() < 1e-3) | ((ratio - 1 - HIGH).abs() < 1e-3)
+    i["mask"][near] = 0
+    mask = i["mask"] != 0
+    c = Call(i)
+    norm = c.loss("sequences")[1]
+    got, h = c.grad(norm, 1.0), 1e-5
+    up, down = (D.policy_terms(logp + s * h, old, ref, adv, LOW, HIGH, KL)[0] for s in (1, -1))
+    diff = torch.where(mask, norm[:, None] * (up - down) / (2 * h), torch.zeros_like(up))
+    assert float((got - diff).abs().max()) <= 1e-6 * float(diff.abs().max())
+
+
+def test_gradient_in_place_of_logp():
+    i = inputs(10, 333)
+    c = Call(i)
+    norm = c.loss()[1]
+    want = c.grad(norm, 1.0)
+    dl = torch.ones(1, device="cuda")
+    n = norm.float().cuda()
+    vk.policy_loss_backward_async(10, 333, *c.args, LOW, HIGH, KL, n.data_ptr(), dl.data_ptr(), c.bufs[0].ptr,
+                                  c.bufs[0].ld, stream=stream())
+    assert torch.equal(c.bufs[0].get(), want)
+
+
+def test_equal_calls_give_equal_bits():
+    c = Call(inputs(300, 700))
+    first = c.loss()
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(c.loss(), first))
+
+
+def test_empty_batch():
+    args = 0, 5, None, 5, None, 5, None, 0, None, 5, 1, None, 0, 0.2, 0.2, 0.0
+    assert vk.policy_loss_async(0, *args, None, None) == vk.OK
+    assert vk.policy_loss_backward_async(*args, None, None, None, 5) == vk.OK

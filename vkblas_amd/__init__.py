@@ -10,10 +10,10 @@ and ``__graft_entry__``: it loads the built library with ctypes and mirrors the
 engine entry points (``vkblas_gemm_f32`` / ``vkblas_gemm_f16`` of the
 reference's ``src/vkblas.h:27-77``) with the same argument meaning and status
 codes.  There is no fallback: if the library is missing, loading raises.
-The asynchronous GEMMs and the operators of ``include/vkblas_nn.h`` (layer norm,
-gated projection, linear cross entropy, with their gradients; ``torch_nn`` wraps
-them for autograd) go through ``_call`` (csrc/pycall.c), which converts
-their arguments natively; arguments it does not know, and every call of an
+The asynchronous GEMMs and the operators of ``include/vkblas_nn.h`` and
+``include/vkblas_train.h`` (embedding, layer norm, gated projection, linear cross entropy
+and distillation, policy loss, with their gradients; ``torch_nn`` wraps them for autograd)
+go through ``_call`` (csrc/pycall.c), which converts their arguments natively; arguments it does not know, and every call of an
 interpreter it is not built for, go through ctypes.
 """
 from __future__ import annotations
@@ -41,6 +41,10 @@ DT_F32, DT_F16, DT_BF16 = 0, 1, 2
 SCALAR_HOST, SCALAR_DEV_F32, SCALAR_DEV_F16 = 0, 1, 2
 # vkblas_act_t (include/vkblas_nn.h)
 ACT_SILU, ACT_GELU, ACT_GELU_TANH, ACT_RELU = range(4)
+# vkblas_reduce_t (include/vkblas_train.h)
+REDUCE_TOKENS, REDUCE_SEQUENCES, REDUCE_SUM = range(3)
+# the most entries of a row in linear_distill_async (VKBLAS_DISTILL_TOP)
+DISTILL_TOP = 1024
 # vkblas_path_t
 PATH_NONE, PATH_TILE64, PATH_TILE128, PATH_TILE256, PATH_SPLITK, PATH_SKINNY, PATH_TAIL = range(7)
 PATH_NAMES = {0: "none", 1: "tile64", 2: "tile128", 3: "tile256", 4: "splitk", 5: "skinny", 6: "tail"}
@@ -75,7 +79,7 @@ _u32, _i64, _f, _vp, _int = ctypes.c_uint32, ctypes.c_int64, ctypes.c_float, cty
 _ENGINE_ARGS = [_int, _int, _u32, _u32, _u32, _f, _vp, _u32, _vp, _u32, _f, _vp, _u32, _u32, _i64, _i64, _i64]
 
 
-# include/vkblas_nn.h: the arguments of vkblas_<name>_async
+# include/vkblas_nn.h and vkblas_train.h: the arguments of vkblas_<name>_async
 _NN_ARGS = {
     "layer_norm": [_int, _int, _u32, _u32, _vp, _u32, _vp, _vp, _f, _vp, _u32, _vp, _vp, _vp],
     "layer_norm_backward": [_int, _int, _u32, _u32, _vp, _u32, _vp, _u32, _vp, _vp, _vp, _vp, _u32, _vp,
@@ -86,6 +90,16 @@ _NN_ARGS = {
     "linear_xent": [_int, _u32, _u32, _u32, _vp, _u32, _vp, _u32, _vp, _i64, _vp, _vp, _vp],
     "linear_xent_backward": [_int, _u32, _u32, _u32, _vp, _u32, _vp, _u32, _vp, _i64, _vp, _vp, _vp, _u32,
                                           _vp, _u32, _int, _f, _vp],
+    "embedding": [_int, _int, _u32, _u32, _u32, _vp, _i64, _vp, _u32, _f, _vp, _u32, _vp],
+    "embedding_backward": [_int, _u32, _u32, _u32, _vp, _i64, _vp, _u32, _f, _vp, _u32, _int, _f, _vp],
+    "linear_distill": [_int, _u32, _u32, _u32, _vp, _u32, _vp, _u32, _u32, _vp, _u32, _int, _vp, _u32, _f, _vp, _vp,
+                       _vp, _vp],
+    "linear_distill_backward": [_int, _u32, _u32, _u32, _vp, _u32, _vp, _u32, _u32, _vp, _u32, _int, _vp, _u32, _f, _vp,
+                                _vp, _vp, _vp, _u32, _vp, _u32, _int, _f, _vp],
+    "policy_loss": [_int, _u32, _u32, _vp, _u32, _vp, _u32, _vp, _u32, _vp, _u32, _u32, _vp, _u32, _f, _f, _f, _vp, _vp,
+                    _vp],
+    "policy_loss_backward": [_u32, _u32, _vp, _u32, _vp, _u32, _vp, _u32, _vp, _u32, _u32, _vp, _u32, _f, _f, _f, _vp,
+                             _vp, _vp, _u32, _vp],
 }
 
 
@@ -190,7 +204,7 @@ def last_path() -> int:
 # vkblas_kernel_t (include/vkblas_ext.h)
 KERNEL_NONE, KERNEL_GENERIC, KERNEL_GENERIC_CHECKED, KERNEL_PIPE256, KERNEL_PIPE128, KERNEL_PIPE128_4, \
     KERNEL_SKINNY, KERNEL_WAVEK, KERNEL_DIRECT, KERNEL_FLOW, KERNEL_NORM, KERNEL_NORM_LONG, \
-    KERNEL_JOINED, KERNEL_FUSED, KERNEL_FEW = range(15)
+    KERNEL_JOINED, KERNEL_FUSED, KERNEL_FEW, KERNEL_EMBED, KERNEL_POLICY = range(17)
 
 
 def workspace_release() -> None:
@@ -274,8 +288,8 @@ def gemm_batched_async(ab_type, c_type, op_a, op_b, M, N, K, alpha, A, lda, B, l
 
 
 def _nn(name, check, *args) -> int:
-    """A call of vkblas_nn.h; its status (raises if check).  A number that its C type does not hold is refused like
-    the sizes that the library refuses, not passed as what is left of it."""
+    """A call of vkblas_nn.h or vkblas_train.h; its status (raises if check).  A number that its C type
+    does not hold is refused like the sizes that the library refuses, not passed as what is left of it."""
     if not _nn_calls:
         load()
     native, addr, fn = _nn_calls[name]
@@ -333,6 +347,56 @@ def linear_xent_backward_async(dtype, M, V, K, x, ldx, w, ldw, target, ignore_in
     rows' loss gradients; each may be None."""
     return _nn("linear_xent_backward", check, dtype, M, V, K, x, ldx, w, ldw, target, ignore_index, lse,
                dloss, dx, lddx, dw, lddw, dw_dtype, beta, stream)
+
+
+def embedding_async(dtype, w_dtype, M, V, N, ids, pad_id, w, ldw, scale, y, ldy, stream=None, check=True) -> int:
+    """vkblas_embedding_async: y[m] = scale * w[ids[m]], zeros where ids[m] is
+    pad_id."""
+    return _nn("embedding", check, dtype, w_dtype, M, V, N, ids, pad_id, w, ldw, scale, y, ldy, stream)
+
+
+def embedding_backward_async(dtype, M, V, N, ids, pad_id, dy, lddy, scale, dw, lddw, dw_dtype, beta=0.0, stream=None,
+                             check=True) -> int:
+    """vkblas_embedding_backward_async: dw = beta dw + scale times the sums of
+    each id's rows of dy."""
+    return _nn("embedding_backward", check, dtype, M, V, N, ids, pad_id, dy, lddy, scale, dw, lddw, dw_dtype, beta,
+               stream)
+
+
+def linear_distill_async(dtype, M, V, K, x, ldx, w, ldw, n_top, top, ldtop, t_dtype, t, ldt, temperature, loss, lse,
+                         z_top, stream=None, check=True) -> int:
+    """vkblas_linear_distill_async: each row's distillation loss from the
+    teacher's top logits t at the classes top (M x n_top, negative: absent),
+    log-sum-exp of the tempered logits of x w^T, and z_top (M x n_top), those
+    logits at the classes."""
+    return _nn("linear_distill", check, dtype, M, V, K, x, ldx, w, ldw, n_top, top, ldtop, t_dtype, t, ldt, temperature,
+               loss, lse, z_top, stream)
+
+
+def linear_distill_backward_async(dtype, M, V, K, x, ldx, w, ldw, n_top, top, ldtop, t_dtype, t, ldt, temperature, lse,
+                                  z_top, dloss, dx, lddx, dw, lddw, dw_dtype, beta=0.0, stream=None,
+                                  check=True) -> int:
+    """vkblas_linear_distill_backward_async: dx and dw = beta dw + D^T x from the
+    rows' loss gradients; each may be None."""
+    return _nn("linear_distill_backward", check, dtype, M, V, K, x, ldx, w, ldw, n_top, top, ldtop, t_dtype, t, ldt,
+               temperature, lse, z_top, dloss, dx, lddx, dw, lddw, dw_dtype, beta, stream)
+
+
+def policy_loss_async(reduce, B, T, logp, ldp, old_logp, ldo, ref_logp, ldr, adv, ldadv, adv_step, mask, ldmask,
+                      clip_low, clip_high, kl_coef, stats, norm, stream=None, check=True) -> int:
+    """vkblas_policy_loss_async: the clipped policy loss with a KL term of B
+    sequences of T tokens; stats (4 floats): loss, KL term, bounds taken, ratio,
+    by weight; norm (B floats): a token's weight."""
+    return _nn("policy_loss", check, reduce, B, T, logp, ldp, old_logp, ldo, ref_logp, ldr, adv, ldadv, adv_step, mask,
+               ldmask, clip_low, clip_high, kl_coef, stats, norm, stream)
+
+
+def policy_loss_backward_async(B, T, logp, ldp, old_logp, ldo, ref_logp, ldr, adv, ldadv, adv_step, mask, ldmask,
+                               clip_low, clip_high, kl_coef, norm, dloss, dlogp, lddp, stream=None, check=True) -> int:
+    """vkblas_policy_loss_backward_async: dlogp from dloss (one float on the
+    device) and norm."""
+    return _nn("policy_loss_backward", check, B, T, logp, ldp, old_logp, ldo, ref_logp, ldr, adv, ldadv, adv_step, mask,
+               ldmask, clip_low, clip_high, kl_coef, norm, dloss, dlogp, lddp, stream)
 
 
 def gemm_f32(op_a, op_b, M, N, K, alpha, A, lda, B, ldb, beta, C, ldc, batch=1, sa=0, sb=0, sc=0) -> int:

@@ -1,8 +1,8 @@
 /*
  * engine_stub.c — the public C API of libvkblas_hipblas.so (include/vkblas.h,
- * include/vkblas_ext.h, include/vkblas_nn.h), forwarded to libvkblas_engine.so, the host
- * dispatcher and gfx950 kernels, which is loaded from this library's own
- * directory at the first call.
+ * include/vkblas_ext.h, include/vkblas_nn.h, include/vkblas_train.h), forwarded to
+ * libvkblas_engine.so, the host dispatcher and gfx950 kernels, which is loaded
+ * from this library's own directory at the first call.
  *
  * Why two libraries.  The reference is used as
  * `LD_PRELOAD=libvkblas_hipblas.so python script.py` (reference
@@ -30,7 +30,7 @@
 #include <stdio.h>
 #include <string.h>
 
-#include "vkblas_nn.h"
+#include "vkblas_train.h"
 
 #define ENGINE_NAME "libvkblas_engine.so"
 
@@ -169,3 +169,40 @@ VKB_ENGINE_FN(vkblas_status_t, VKBLAS_ERR_INIT, vkblas_linear_xent_backward_asyn
                void* dx, uint32_t lddx, void* dw, uint32_t lddw, vkblas_dtype_t dw_type, float beta, void* stream),
               (type, M, V, K, x, ldx, w, ldw, target, ignore_index, lse, dloss, dx, lddx, dw, lddw, dw_type, beta,
                stream))
+
+/* include/vkblas_train.h */
+VKB_ENGINE_FN(vkblas_status_t, VKBLAS_ERR_INIT, vkblas_embedding_async,
+              (vkblas_dtype_t type, vkblas_dtype_t w_type, uint32_t M, uint32_t V, uint32_t N, const int64_t* ids,
+               int64_t pad_id, const void* w, uint32_t ldw, float scale, void* y, uint32_t ldy, void* stream),
+              (type, w_type, M, V, N, ids, pad_id, w, ldw, scale, y, ldy, stream))
+VKB_ENGINE_FN(vkblas_status_t, VKBLAS_ERR_INIT, vkblas_embedding_backward_async,
+              (vkblas_dtype_t type, uint32_t M, uint32_t V, uint32_t N, const int64_t* ids, int64_t pad_id,
+               const void* dy, uint32_t lddy, float scale, void* dw, uint32_t lddw, vkblas_dtype_t dw_type, float beta,
+               void* stream),
+              (type, M, V, N, ids, pad_id, dy, lddy, scale, dw, lddw, dw_type, beta, stream))
+VKB_ENGINE_FN(vkblas_status_t, VKBLAS_ERR_INIT, vkblas_linear_distill_async,
+              (vkblas_dtype_t type, uint32_t M, uint32_t V, uint32_t K, const void* x, uint32_t ldx, const void* w,
+               uint32_t ldw, uint32_t n_top, const int64_t* top, uint32_t ldtop, vkblas_dtype_t t_type, const void* t,
+               uint32_t ldt, float temperature, float* loss, float* lse, float* z_top, void* stream),
+              (type, M, V, K, x, ldx, w, ldw, n_top, top, ldtop, t_type, t, ldt, temperature, loss, lse, z_top, stream))
+VKB_ENGINE_FN(vkblas_status_t, VKBLAS_ERR_INIT, vkblas_linear_distill_backward_async,
+              (vkblas_dtype_t type, uint32_t M, uint32_t V, uint32_t K, const void* x, uint32_t ldx, const void* w,
+               uint32_t ldw, uint32_t n_top, const int64_t* top, uint32_t ldtop, vkblas_dtype_t t_type, const void* t,
+               uint32_t ldt, float temperature, const float* lse, const float* z_top, const float* dloss, void* dx,
+               uint32_t lddx, void* dw, uint32_t lddw, vkblas_dtype_t dw_type, float beta, void* stream),
+              (type, M, V, K, x, ldx, w, ldw, n_top, top, ldtop, t_type, t, ldt, temperature, lse, z_top, dloss, dx, lddx,
+               dw, lddw, dw_type, beta, stream))
+VKB_ENGINE_FN(vkblas_status_t, VKBLAS_ERR_INIT, vkblas_policy_loss_async,
+              (vkblas_reduce_t reduce, uint32_t B, uint32_t T, const float* logp, uint32_t ldp, const float* old_logp,
+               uint32_t ldo, const float* ref_logp, uint32_t ldr, const float* adv, uint32_t ldadv, uint32_t adv_step,
+               const uint8_t* mask, uint32_t ldmask, float clip_low, float clip_high, float kl_coef, float* stats,
+               float* norm, void* stream),
+              (reduce, B, T, logp, ldp, old_logp, ldo, ref_logp, ldr, adv, ldadv, adv_step, mask, ldmask, clip_low,
+               clip_high, kl_coef, stats, norm, stream))
+VKB_ENGINE_FN(vkblas_status_t, VKBLAS_ERR_INIT, vkblas_policy_loss_backward_async,
+              (uint32_t B, uint32_t T, const float* logp, uint32_t ldp, const float* old_logp, uint32_t ldo,
+               const float* ref_logp, uint32_t ldr, const float* adv, uint32_t ldadv, uint32_t adv_step,
+               const uint8_t* mask, uint32_t ldmask, float clip_low, float clip_high, float kl_coef, const float* norm,
+               const float* dloss, float* dlogp, uint32_t lddp, void* stream),
+              (B, T, logp, ldp, old_logp, ldo, ref_logp, ldr, adv, ldadv, adv_step, mask, ldmask, clip_low, clip_high,
+               kl_coef, norm, dloss, dlogp, lddp, stream))

@@ -112,6 +112,7 @@ struct XentParams : KParams {
     // the targets' logits
     float2* parts;
     float* zt;
+    float c2;                // log2(e), over a distillation's temperature
     // gradient: rows and columns of D stored, zero past M and N
     uint32_t Ms, Ns;
     int64_t V, ignore;
@@ -172,12 +173,12 @@ struct XentStatsOp {
                     for (int r = 0; r < 4 * G::NQ; ++r) top = fmaxf(top, at(j, r));
 #pragma unroll
                 for (int d = 32; d >= G::FR; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-                const float off = (__builtin_isinf(top) ? 0.0f : top) * LOG2E;
+                const float off = (__builtin_isinf(top) ? 0.0f : top) * p.c2;
 #pragma unroll
                 for (int j = 0; j < G::NF; ++j)
 #pragma unroll
                     for (int r = 0; r < 4 * G::NQ; ++r)
-                        s += __builtin_amdgcn_exp2f(__builtin_fmaf(at(j, r), LOG2E, -off));
+                        s += __builtin_amdgcn_exp2f(__builtin_fmaf(at(j, r), p.c2, -off));
 #pragma unroll
                 for (int d = 32; d >= G::FR; d >>= 1) s += __shfl_xor(s, d);
                 const int64_t m = row0 + G::row(lane, i);
@@ -214,7 +215,7 @@ struct XentGradOp {
             for (int j = 0; j < G::NF; ++j)
 #pragma unroll
                 for (int r = 0; r < 4 * G::NQ; ++r) {
-                    const float x = k * __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][r], LOG2E, -l));
+                    const float x = k * __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][r], p.c2, -l));
                     acc[i][j][r] = skip ? 0.0f : x;
                 }
             const int64_t tc = t - p.v0 - col0;

@@ -1,16 +1,18 @@
 /*
- * nn.c — host side of the operators in vkblas_nn.h: argument checks, plans,
- * workspaces and the order of launches.  No reference counterpart (see
- * vkblas_nn.h).
+ * nn.c — host side of the operators in vkblas_nn.h and vkblas_train.h: argument
+ * checks, plans, workspaces and the order of launches.  No reference
+ * counterpart (see the headers).
  *
  * A call's workspace is its stream's (engine.c): the arrival counters and
  * partials of the call's own GEMMs first, then the operator's buffers.
  */
+#include <float.h>
+#include <math.h>
 #include <stdio.h>
 #include <string.h>
 #include <hip/hip_runtime_api.h>
 
-#include "vkblas_nn.h"
+#include "vkblas_train.h"
 #include "vkb_engine.h"
 #include "vkb_launch.h"
 #include "vkb_nn_launch.h"
@@ -135,10 +137,10 @@ static vkblas_status_t op_end(op_call* c, int kernel) {
 extern int vkb_launch_glu_f32(const vkb_op_args*, int, void*, int64_t, void*, int64_t, void*);
 extern int vkb_launch_glu_f16(const vkb_op_args*, int, void*, int64_t, void*, int64_t, void*);
 extern int vkb_launch_glu_bf16(const vkb_op_args*, int, void*, int64_t, void*, int64_t, void*);
-extern int vkb_launch_xent_stats_f32(const vkb_op_args*, const int64_t*, float*, float*, void*);
-extern int vkb_launch_xent_stats_f16(const vkb_op_args*, const int64_t*, float*, float*, void*);
-extern int vkb_launch_xent_stats_bf16(const vkb_op_args*, const int64_t*, float*, float*, void*);
-typedef int xent_grad_fn(const vkb_op_args*, uint32_t, uint32_t, uint32_t, uint32_t, const int64_t*, int64_t,
+extern int vkb_launch_xent_stats_f32(const vkb_op_args*, float, const int64_t*, float*, float*, void*);
+extern int vkb_launch_xent_stats_f16(const vkb_op_args*, float, const int64_t*, float*, float*, void*);
+extern int vkb_launch_xent_stats_bf16(const vkb_op_args*, float, const int64_t*, float*, float*, void*);
+typedef int xent_grad_fn(const vkb_op_args*, uint32_t, uint32_t, uint32_t, uint32_t, float, const int64_t*, int64_t,
                          const float*, const float*, vkb_scale, void*, int64_t, void*);
 extern xent_grad_fn vkb_launch_xent_grad_f32, vkb_launch_xent_grad_f16, vkb_launch_xent_grad_bf16;
 
@@ -147,17 +149,18 @@ int vkb_launch_glu(const vkb_op_args* a, int act, void* h, int64_t ldh, void* gu
                                                                              : vkb_launch_glu_f32)(
         a, act, h, ldh, gu, ldgu, stream);
 }
-int vkb_launch_xent_stats_op(const vkb_op_args* a, const int64_t* target, float* parts, float* zt, void* stream) {
+int vkb_launch_xent_stats_op(const vkb_op_args* a, float inv_t, const int64_t* target, float* parts, float* zt,
+                             void* stream) {
     return (a->type == VKB_T_F16 ? vkb_launch_xent_stats_f16 : a->type == VKB_T_BF16 ? vkb_launch_xent_stats_bf16
                                                                                     : vkb_launch_xent_stats_f32)(
-        a, target, parts, zt, stream);
+        a, inv_t, target, parts, zt, stream);
 }
-int vkb_launch_xent_grad_op(const vkb_op_args* a, uint32_t Ms, uint32_t Ns, uint32_t v0, uint32_t V,
+int vkb_launch_xent_grad_op(const vkb_op_args* a, uint32_t Ms, uint32_t Ns, uint32_t v0, uint32_t V, float inv_t,
                             const int64_t* target, int64_t ignore, const float* lse, const float* dloss,
                             vkb_scale scale, void* D, int64_t ldd, void* stream) {
     return (a->type == VKB_T_F16 ? vkb_launch_xent_grad_f16 : a->type == VKB_T_BF16 ? vkb_launch_xent_grad_bf16
                                                                                    : vkb_launch_xent_grad_f32)(
-        a, Ms, Ns, v0, V, target, ignore, lse, dloss, scale, D, ldd, stream);
+        a, Ms, Ns, v0, V, inv_t, target, ignore, lse, dloss, scale, D, ldd, stream);
 }
 uint32_t vkb_xent_slices(const vkb_op_args* a) {
     const uint64_t tile = vkb_tile_bn(a->tile);
@@ -635,6 +638,69 @@ static uint32_t piece_columns(uint32_t M, uint32_t V, uint64_t bytes, uint64_t e
     return (uint32_t)(n < V ? n : V);
 }
 
+/* lse of each row's logits times inv_t, and its loss (target NULL: none), on the
+ * call's workspace.  Returns the kernel for op_end(), VKBLAS_KERNEL_NONE where
+ * nothing could begin. */
+static int row_statistics(op_call* c, vkblas_dtype_t type, uint32_t M, uint32_t V, uint32_t K, float inv_t,
+                          const void* x, uint32_t ldx, const void* w, uint32_t ldw, const int64_t* target,
+                          int64_t ignore_index, float* loss, float* lse) {
+    void* stream = c->stream;
+    vkb_op_args a;
+    operand ox = as_is(x, ldx, 1, M, K), ow = as_is(w, ldw, 1, V, K);
+    if (fusable(type, M, V, K, &ox, &ow, 256, &a)) {
+        const uint32_t S = vkb_xent_slices(&a);
+        place(c, &ox, type);
+        place(c, &ow, type);
+        const size_t o_p = buf(c, (uint64_t)S * M * 2 * sizeof(float)), o_t = buf(c, (uint64_t)M * sizeof(float));
+        if (room(c) != VKBLAS_OK) return VKBLAS_KERNEL_NONE;
+        float *parts = at(c, o_p), *zt = at(c, o_t);
+        copies jobs = {.n = 0};
+        bring(c, &jobs, &ox, x, ldx);
+        bring(c, &jobs, &ow, w, ldw);
+        if (brought(c, &jobs, type, NULL)) {
+            bound(&a, &ox, &ow);
+            if (step(c, vkb_launch_xent_stats_op(&a, inv_t, target, parts, zt, stream), 0))
+                step(c, vkb_launch_xent_finish(M, V, S, inv_t, parts, zt, target, ignore_index, loss, lse, stream), 1);
+        }
+        return VKBLAS_KERNEL_FUSED;
+    }
+    const uint32_t n = piece_columns(M, V, JOIN_BYTES, sizeof(float)), ldz = (uint32_t)round_up(n, 4);
+    const uint32_t last = V % n;
+    const uint32_t per = (n + VKB_XENT_SLICE - 1) / VKB_XENT_SLICE;   /* slices of a piece; the last may have fewer */
+    const uint32_t S = V / n * per + (last + VKB_XENT_SLICE - 1) / VKB_XENT_SLICE;
+    const int rows = n == V && V <= VKB_XENT_ROW;                     /* one kernel for a row's statistics and loss */
+    const int few = n == V && few_forward(type, M, V, K, 0,
+                                          K % vec_of(type) || off_units(type, x, ldx) || off_units(type, w, ldw));
+    const uint32_t Kp = few ? K : joinable(type, M, K, &ox, &ow);
+    need_gemm(c, type, VKBLAS_DT_F32, VKBLAS_OP_N, VKBLAS_OP_T, M, n, Kp, ox.p, ox.ld, ow.p, ow.ld, ldz);
+    if (last) need_gemm(c, type, VKBLAS_DT_F32, VKBLAS_OP_N, VKBLAS_OP_T, M, last, Kp, ox.p, ox.ld, ow.p, ow.ld, ldz);
+    place(c, &ox, type);
+    place(c, &ow, type);
+    const size_t o_z = buf(c, (uint64_t)M * ldz * sizeof(float));
+    const size_t o_p = buf(c, (uint64_t)S * M * 2 * sizeof(float));
+    const size_t o_t = buf(c, (uint64_t)M * sizeof(float));
+    if (room(c) != VKBLAS_OK) return VKBLAS_KERNEL_NONE;
+    float *z = at(c, o_z), *parts = at(c, o_p), *zt = at(c, o_t);
+    copies jobs = {.n = 0};
+    bring(c, &jobs, &ox, x, ldx);
+    bring(c, &jobs, &ow, w, ldw);
+    int ok = brought(c, &jobs, type, NULL);
+    uint32_t slice = 0;
+    for (uint64_t v = 0; ok && v < V; v += n, slice += per) {
+        const uint32_t cols = (uint32_t)(V - v < n ? V - v : n);
+        const vkb_few_forward fw = {x, w, z, NULL, ldx, ldw, ldz, 0, M, V, K, 0};
+        ok = (few ? step(c, vkb_launch_few_forward(type, &fw, 0, stream), 0)
+                  : product(c, type, VKBLAS_DT_F32, VKBLAS_OP_N, VKBLAS_OP_T, M, cols, Kp, host_scalars(1.0f, 0.0f),
+                            ox.p, ox.ld, (const char*)ow.p + v * ow.ld * type_size(type), ow.ld, z, ldz, 0)) &&
+             (rows ? step(c, vkb_launch_xent_rows(M, V, inv_t, z, ldz, target, ignore_index, loss, lse, stream), 1)
+                   : step(c, vkb_launch_xent_stats(M, cols, (uint32_t)v, inv_t, z, ldz, target,
+                                                    parts + (uint64_t)slice * M * 2, zt, stream), 0));
+    }
+    if (ok && !rows)
+        step(c, vkb_launch_xent_finish(M, V, S, inv_t, parts, zt, target, ignore_index, loss, lse, stream), 1);
+    return VKBLAS_KERNEL_JOINED;
+}
+
 vkblas_status_t vkblas_linear_xent_async(vkblas_dtype_t type, uint32_t M, uint32_t V, uint32_t K, const void* x,
                                          uint32_t ldx, const void* w, uint32_t ldw, const int64_t* target,
                                          int64_t ignore_index, float* loss, float* lse, void* stream) {
@@ -646,96 +712,38 @@ vkblas_status_t vkblas_linear_xent_async(vkblas_dtype_t type, uint32_t M, uint32
     op_call c;
     op_begin(&c, "linear_xent", stream);
     if (vkb_engine_trace()) fprintf(stderr, "[vkblas] linear_xent type=%d M=%u V=%u K=%u\n", (int)type, M, V, K);
-    vkb_op_args a;
-    operand ox = as_is(x, ldx, 1, M, K), ow = as_is(w, ldw, 1, V, K);
-    if (fusable(type, M, V, K, &ox, &ow, 256, &a)) {
-        const uint32_t S = vkb_xent_slices(&a);
-        place(&c, &ox, type);
-        place(&c, &ow, type);
-        const size_t o_p = buf(&c, (uint64_t)S * M * 2 * sizeof(float)), o_t = buf(&c, (uint64_t)M * sizeof(float));
-        if (room(&c) != VKBLAS_OK) return c.st;
-        float *parts = at(&c, o_p), *zt = at(&c, o_t);
-        copies jobs = {.n = 0};
-        bring(&c, &jobs, &ox, x, ldx);
-        bring(&c, &jobs, &ow, w, ldw);
-        if (brought(&c, &jobs, type, NULL)) {
-            bound(&a, &ox, &ow);
-            if (step(&c, vkb_launch_xent_stats_op(&a, target, parts, zt, stream), 0))
-                step(&c, vkb_launch_xent_finish(M, V, S, parts, zt, target, ignore_index, loss, lse, stream), 1);
-        }
-        return op_end(&c, VKBLAS_KERNEL_FUSED);
-    }
-    const uint32_t n = piece_columns(M, V, JOIN_BYTES, sizeof(float)), ldz = (uint32_t)round_up(n, 4);
-    const uint32_t last = V % n;
-    const uint32_t per = (n + VKB_XENT_SLICE - 1) / VKB_XENT_SLICE;   /* slices of a piece; the last may have fewer */
-    const uint32_t S = V / n * per + (last + VKB_XENT_SLICE - 1) / VKB_XENT_SLICE;
-    const int rows = n == V && V <= VKB_XENT_ROW;                     /* one kernel for a row's statistics and loss */
-    const int few = n == V && few_forward(type, M, V, K, 0,
-                                          K % vec_of(type) || off_units(type, x, ldx) || off_units(type, w, ldw));
-    const uint32_t Kp = few ? K : joinable(type, M, K, &ox, &ow);
-    need_gemm(&c, type, VKBLAS_DT_F32, VKBLAS_OP_N, VKBLAS_OP_T, M, n, Kp, ox.p, ox.ld, ow.p, ow.ld, ldz);
-    if (last) need_gemm(&c, type, VKBLAS_DT_F32, VKBLAS_OP_N, VKBLAS_OP_T, M, last, Kp, ox.p, ox.ld, ow.p, ow.ld, ldz);
-    place(&c, &ox, type);
-    place(&c, &ow, type);
-    const size_t o_z = buf(&c, (uint64_t)M * ldz * sizeof(float));
-    const size_t o_p = buf(&c, (uint64_t)S * M * 2 * sizeof(float));
-    const size_t o_t = buf(&c, (uint64_t)M * sizeof(float));
-    if (room(&c) != VKBLAS_OK) return c.st;
-    float *z = at(&c, o_z), *parts = at(&c, o_p), *zt = at(&c, o_t);
-    copies jobs = {.n = 0};
-    bring(&c, &jobs, &ox, x, ldx);
-    bring(&c, &jobs, &ow, w, ldw);
-    int ok = brought(&c, &jobs, type, NULL);
-    uint32_t slice = 0;
-    for (uint64_t v = 0; ok && v < V; v += n, slice += per) {
-        const uint32_t cols = (uint32_t)(V - v < n ? V - v : n);
-        const vkb_few_forward fw = {x, w, z, NULL, ldx, ldw, ldz, 0, M, V, K, 0};
-        ok = (few ? step(&c, vkb_launch_few_forward(type, &fw, 0, stream), 0)
-                  : product(&c, type, VKBLAS_DT_F32, VKBLAS_OP_N, VKBLAS_OP_T, M, cols, Kp, host_scalars(1.0f, 0.0f),
-                            ox.p, ox.ld, (const char*)ow.p + v * ow.ld * type_size(type), ow.ld, z, ldz, 0)) &&
-             (rows ? step(&c, vkb_launch_xent_rows(M, V, z, ldz, target, ignore_index, loss, lse, stream), 1)
-                   : step(&c, vkb_launch_xent_stats(M, cols, (uint32_t)v, z, ldz, target,
-                                                    parts + (uint64_t)slice * M * 2, zt, stream), 0));
-    }
-    if (ok && !rows) step(&c, vkb_launch_xent_finish(M, V, S, parts, zt, target, ignore_index, loss, lse, stream), 1);
-    return op_end(&c, VKBLAS_KERNEL_JOINED);
+    const int kernel = row_statistics(&c, type, M, V, K, 1.0f, x, ldx, w, ldw, target, ignore_index, loss, lse);
+    return kernel == VKBLAS_KERNEL_NONE ? c.st : op_end(&c, kernel);
 }
 
-vkblas_status_t vkblas_linear_xent_backward_async(vkblas_dtype_t type, uint32_t M, uint32_t V, uint32_t K,
-                                                  const void* x, uint32_t ldx, const void* w, uint32_t ldw,
-                                                  const int64_t* target, int64_t ignore_index, const float* lse,
-                                                  const float* dloss, void* dx, uint32_t lddx, void* dw,
-                                                  uint32_t lddw, vkblas_dtype_t dw_type, float beta, void* stream) {
-    if (!known_type(type) || (dw && dw_type != type && dw_type != VKBLAS_DT_F32)) return VKBLAS_ERR_PARAM;
-    if (V == 0 || K == 0 || M > DIM_MAX || V > DIM_MAX || K > DIM_MAX || ldx < K || ldw < K || (dx && lddx < K) ||
-        (dw && lddw < K))
-        return VKBLAS_ERR_PARAM;
-    op_call c;
-    op_begin(&c, "linear_xent_backward", stream);
-    if (M == 0) return empty_gradient(&c, dw_type, V, K, dw, lddw, beta);
-    if (!x || !w || !target || !lse || !dloss) return VKBLAS_ERR_PARAM;
-    if (!dx && !dw) return VKBLAS_OK;
-    if (vkb_engine_trace())
-        fprintf(stderr, "[vkblas] linear_xent_backward type=%d M=%u V=%u K=%u\n", (int)type, M, V, K);
+/* dx and dw of a linear cross entropy, or (q) of a distillation, on the call's
+ * workspace. */
+static vkblas_status_t logits_backward(op_call* c, vkblas_dtype_t type, uint32_t M, uint32_t V, uint32_t K,
+                                       const void* x, uint32_t ldx, const void* w, uint32_t ldw, const int64_t* target,
+                                       int64_t ignore_index, vkb_distill* q, vkblas_dtype_t t_type, const float* z_top,
+                                       const float* lse, const float* dloss, void* dx, uint32_t lddx, void* dw,
+                                       uint32_t lddw, vkblas_dtype_t dw_type, float beta) {
+    void* stream = c->stream;
+    const float inv_t = q ? 1.0f / q->temp : 1.0f;
     const int off = K % vec_of(type) || off_units(type, x, ldx) || off_units(type, w, ldw);
-    if (few_backward_rows(type, M, V, K, off || V % 8)) {
+    if (!q && few_backward_rows(type, M, V, K, off || V % 8)) {
         const uint32_t ldz = (uint32_t)round_up(V, 4);
         vkb_few_backward p = {.x = x, .w = w, .dw = dw, .ldx = ldx, .ldw = ldw, .lddw = lddw, .M = M, .R = V, .K = K,
                               .beta = beta, .lse = lse, .dloss = dloss, .ldz = ldz, .ignore = ignore_index,
                               .target = target};
-        if (!off) need_gemm(&c, type, VKBLAS_DT_F32, VKBLAS_OP_N, VKBLAS_OP_T, M, V, K, x, ldx, w, ldw, ldz);
+        if (!off) need_gemm(c, type, VKBLAS_DT_F32, VKBLAS_OP_N, VKBLAS_OP_T, M, V, K, x, ldx, w, ldw, ldz);
         const uint32_t slices = vkb_few_slices(type, &p);
-        const size_t o_z = buf(&c, (uint64_t)M * ldz * sizeof(float));
-        const size_t o_part = dx ? buf(&c, (uint64_t)slices * M * K * sizeof(float)) : 0;
-        if (room(&c) != VKBLAS_OK) return c.st;
-        float* z = at(&c, o_z);
+        const size_t o_z = buf(c, (uint64_t)M * ldz * sizeof(float));
+        const size_t o_part = dx ? buf(c, (uint64_t)slices * M * K * sizeof(float)) : 0;
+        if (room(c) != VKBLAS_OK) return c->st;
+        float* z = at(c, o_z);
         p.z = z;
         const vkb_few_forward fw = {x, w, z, NULL, ldx, ldw, ldz, 0, M, V, K, 0};
-        const int ok = off ? step(&c, vkb_launch_few_forward(type, &fw, 0, stream), 0)
-                           : product(&c, type, VKBLAS_DT_F32, VKBLAS_OP_N, VKBLAS_OP_T, M, V, K,
+        const int ok = off ? step(c, vkb_launch_few_forward(type, &fw, 0, stream), 0)
+                           : product(c, type, VKBLAS_DT_F32, VKBLAS_OP_N, VKBLAS_OP_T, M, V, K,
                                      host_scalars(1.0f, 0.0f), x, ldx, w, ldw, z, ldz, 0);
-        if (!ok) return op_end(&c, VKBLAS_KERNEL_FEW);
-        return few_backward(&c, type, dw_type, &p, 0, o_part, slices, dx, lddx);
+        if (!ok) return op_end(c, VKBLAS_KERNEL_FEW);
+        return few_backward(c, type, dw_type, &p, 0, o_part, slices, dx, lddx);
     }
     /* D of a piece of the vocabulary at a time, in type: from the pipelined
      * kernel, or over the piece's logits in fp32 (fp32: in their place).
@@ -782,38 +790,51 @@ vkblas_status_t vkblas_linear_xent_backward_async(vkblas_dtype_t type, uint32_t 
         if (!cols) continue;
         const uint32_t main = whole ? (vpad ? (uint32_t)round_up(cols, 128) : cols / 128 * 128) : cols;
         if (!fused)
-            need_gemm(&c, type, VKBLAS_DT_F32, VKBLAS_OP_N, VKBLAS_OP_T, M, cols, K, x, ldx, w, ldw, ldd);
+            need_gemm(c, type, VKBLAS_DT_F32, VKBLAS_OP_N, VKBLAS_OP_T, M, cols, K, x, ldx, w, ldw, ldd);
         if (both) continue;
-        if (dx && main) need_gemm(&c, type, xt, VKBLAS_OP_N, VKBLAS_OP_N, M, Kp, main, NULL, ldd, ow.p, ow.ld, ldxo);
+        if (dx && main) need_gemm(c, type, xt, VKBLAS_OP_N, VKBLAS_OP_N, M, Kp, main, NULL, ldd, ow.p, ow.ld, ldxo);
         if (dw && main)
-            need_gemm(&c, type, pw ? wt : dw_type, VKBLAS_OP_T, VKBLAS_OP_N, main, Kp, Mp, NULL, ldd, ox.p, ox.ld,
+            need_gemm(c, type, pw ? wt : dw_type, VKBLAS_OP_T, VKBLAS_OP_N, main, Kp, Mp, NULL, ldd, ox.p, ox.ld,
                       pw ? Kp : lddw);
     }
     if (rest) {
-        if (dx) need_gemm(&c, type, xt, VKBLAS_OP_N, VKBLAS_OP_N, M, Kp, 128, NULL, ldd, NULL, Kp, ldxo);
-        if (dw) need_gemm(&c, type, wt, VKBLAS_OP_T, VKBLAS_OP_N, 128, Kp, Mp, NULL, ldd, ox.p, ox.ld, Kp);
+        if (dx) need_gemm(c, type, xt, VKBLAS_OP_N, VKBLAS_OP_N, M, Kp, 128, NULL, ldd, NULL, Kp, ldxo);
+        if (dw) need_gemm(c, type, wt, VKBLAS_OP_T, VKBLAS_OP_N, 128, Kp, Mp, NULL, ldd, ox.p, ox.ld, Kp);
     }
-    const size_t o_z = fused ? 0 : buf(&c, (uint64_t)M * ldd * sizeof(float));
-    const size_t o_d = f32 && !fused ? o_z : buf(&c, (uint64_t)Mp * ldd * es);
-    place(&c, &ox, type);
-    place(&c, &ow, type);
+    const size_t o_z = fused ? 0 : buf(c, (uint64_t)M * ldd * sizeof(float));
+    const size_t o_d = f32 && !fused ? o_z : buf(c, (uint64_t)Mp * ldd * es);
+    place(c, &ox, type);
+    place(c, &ow, type);
     operand tail = as_is(NULL, Kp, 1, rest, K);
     if (rest) {
         pad_to(&tail, 128, Kp);
-        place(&c, &tail, type);
+        place(c, &tail, type);
     }
-    const size_t o_x = acc ? buf(&c, (uint64_t)M * ldxo * sizeof(float)) : 0;
-    const size_t o_w = pw || rest ? buf(&c, (pw ? round_up(n, 128) : 128) * Kp * type_size(wt)) : 0;
-    const size_t o_s = buf(&c, 8 * sizeof(float));
-    if (room(&c) != VKBLAS_OK) return c.st;
-    float *z = at(&c, o_z), *scal = f32 ? NULL : (float*)at(&c, o_s);
-    void *d = at(&c, o_d), *xo = acc ? at(&c, o_x) : dx, *wo = at(&c, o_w);
+    const size_t o_x = acc ? buf(c, (uint64_t)M * ldxo * sizeof(float)) : 0;
+    const size_t o_w = pw || rest ? buf(c, (pw ? round_up(n, 128) : 128) * Kp * type_size(wt)) : 0;
+    const size_t o_s = buf(c, 8 * sizeof(float));
+    const size_t o_q = q ? buf(c, (uint64_t)M * q->n * sizeof(float)) : 0;
+    const size_t o_dl = q ? buf(c, (uint64_t)M * sizeof(float)) : 0;
+    const size_t o_t = q ? buf(c, (uint64_t)M * sizeof(int64_t)) : 0;
+    if (room(c) != VKBLAS_OK) return c->st;
+    float *z = at(c, o_z), *scal = f32 ? NULL : (float*)at(c, o_s);
+    void *d = at(c, o_d), *xo = acc ? at(c, o_x) : dx, *wo = at(c, o_w);
+    int ok = 1;
+    if (q) {
+        q->q_top = at(c, o_q);
+        q->dl = at(c, o_dl);
+        q->target = at(c, o_t);
+        ok = step(c, vkb_launch_distill_prepare(t_type, q, dloss, c->stream), 0);
+        dloss = q->dl;
+        target = q->target;
+        ignore_index = q->ignore;
+    }
     copies jobs = {.n = 0};
-    bring(&c, &jobs, &ox, x, ldx);
-    bring(&c, &jobs, &ow, w, ldw);
-    if (rest && dx) bring(&c, &jobs, &tail, (const char*)w + (uint64_t)(V - rest) * ldw * es, ldw);
+    bring(c, &jobs, &ox, x, ldx);
+    bring(c, &jobs, &ow, w, ldw);
+    if (rest && dx) bring(c, &jobs, &tail, (const char*)w + (uint64_t)(V - rest) * ldw * es, ldw);
     const vkb_scale scale = {scal, beta, !jobs.n && M <= VKB_SCALE_ROWS, M, V, dloss, target, ignore_index};
-    int ok = brought(&c, &jobs, type, scal && !scale.find ? &scale : NULL);
+    ok = ok && brought(c, &jobs, type, scal && !scale.find ? &scale : NULL);
     vkb_unpad_job out[2];        /* dw's rows still in the workspace, and dx */
     int outs = 0;
     int summed = 0;              /* dx holds a product already */
@@ -826,18 +847,20 @@ vkblas_status_t vkblas_linear_xent_backward_async(vkblas_dtype_t type, uint32_t 
             bound(&a, &ox, &ow);
             a.w = wv;
             a.N = cols;
-            ok = step(&c, vkb_launch_xent_grad_op(&a, Mp, (uint32_t)round_up(cols, whole ? 128 : 8), (uint32_t)v, V,
-                                                  target, ignore_index, lse, dloss, scale, d, ldd, stream), 0);
+            ok = step(c, vkb_launch_xent_grad_op(&a, Mp, (uint32_t)round_up(cols, whole ? 128 : 8), (uint32_t)v, V,
+                                                  inv_t, target, ignore_index, lse, dloss, scale, d, ldd, stream), 0);
         } else {
-            ok = product(&c, type, VKBLAS_DT_F32, VKBLAS_OP_N, VKBLAS_OP_T, M, cols, K, host_scalars(1.0f, 0.0f), x,
+            ok = product(c, type, VKBLAS_DT_F32, VKBLAS_OP_N, VKBLAS_OP_T, M, cols, K, host_scalars(1.0f, 0.0f), x,
                          ldx, wv, ldw, z, ldd, 0) &&
-                 step(&c, vkb_launch_xent_grad(type, M, cols, (uint32_t)v, V, z, ldd, target, ignore_index, lse, dloss,
-                                               scale, d, ldd, stream), 0);
+                 step(c, vkb_launch_xent_grad(type, M, cols, (uint32_t)v, V, inv_t, z, ldd, target, ignore_index, lse,
+                                               dloss, scale, d, ldd, stream), 0);
         }
+        if (ok && q)
+            ok = step(c, vkb_launch_distill_patch(type, q, (uint32_t)v, cols, lse, z_top, scal, d, ldd, stream), 0);
         if (ok && both) {
             const scalars sx = {1.0f, 0.0f, scal ? scal + 1 : NULL, scal ? scal + 4 : NULL};
             const scalars sw = {1.0f, beta, scal ? scal + 1 : NULL, scal ? scal + 2 : NULL};
-            pair(&c, type, dw_type, M, V, K, d, ldd, wv, ow.ld, dx, lddx, sx, ox.p, ox.ld, dw, lddw, sw);
+            pair(c, type, dw_type, M, V, K, d, ldd, wv, ow.ld, dx, lddx, sx, ox.p, ox.ld, dw, lddw, sw);
             break;
         }
         /* the whole tiles, then the tail */
@@ -852,10 +875,10 @@ vkblas_status_t vkblas_linear_xent_backward_async(vkblas_dtype_t type, uint32_t 
                                     scal ? scal + (by_ws ? 4 : 2) : NULL};
                 char* to = dwv + (t ? (uint64_t)main * lddw * type_size(dw_type) : 0);
                 if (by_ws && outs) {   /* the workspace's rows make room */
-                    ok = step(&c, vkb_launch_unpad(out, outs, stream), 1);
+                    ok = step(c, vkb_launch_unpad(out, outs, stream), 1);
                     outs = 0;
                 }
-                ok = ok && product(&c, type, by_ws ? wt : dw_type, VKBLAS_OP_T, VKBLAS_OP_N, by_ws ? sum : rows, Kp, Mp, sw,
+                ok = ok && product(c, type, by_ws ? wt : dw_type, VKBLAS_OP_T, VKBLAS_OP_N, by_ws ? sum : rows, Kp, Mp, sw,
                              dt, ldd, ox.p, ox.ld, by_ws ? wo : to, by_ws ? Kp : lddw, !by_ws);
                 if (by_ws)
                     out[outs++] = (vkb_unpad_job){wo, to, Kp, lddw, 1, rows, K, rows, (int)wt, (int)dw_type, beta};
@@ -863,7 +886,7 @@ vkblas_status_t vkblas_linear_xent_backward_async(vkblas_dtype_t type, uint32_t 
             if (ok && dx) {
                 const scalars sx = {1.0f, summed ? 1.0f : 0.0f, scal ? scal + 1 : NULL,
                                     scal ? scal + (summed ? 3 : 4) : NULL};
-                ok = product(&c, type, xt, VKBLAS_OP_N, VKBLAS_OP_N, M, Kp, sum, sx, dt, ldd, t ? tail.p : wv,
+                ok = product(c, type, xt, VKBLAS_OP_N, VKBLAS_OP_N, M, Kp, sum, sx, dt, ldd, t ? tail.p : wv,
                              t ? Kp : ow.ld, xo, ldxo, !acc);
                 summed = 1;
             }
@@ -871,6 +894,204 @@ vkblas_status_t vkblas_linear_xent_backward_async(vkblas_dtype_t type, uint32_t 
         v += cols;
     }
     if (acc) out[outs++] = (vkb_unpad_job){xo, dx, ldxo, lddx, 1, M, K, M, VKB_T_F32, (int)type, 0.0f};
-    if (ok && outs) step(&c, vkb_launch_unpad(out, outs, stream), 1);
-    return op_end(&c, fused ? VKBLAS_KERNEL_FUSED : VKBLAS_KERNEL_JOINED);
+    if (ok && outs) step(c, vkb_launch_unpad(out, outs, stream), 1);
+    return op_end(c, fused ? VKBLAS_KERNEL_FUSED : VKBLAS_KERNEL_JOINED);
+}
+
+vkblas_status_t vkblas_linear_xent_backward_async(vkblas_dtype_t type, uint32_t M, uint32_t V, uint32_t K,
+                                                  const void* x, uint32_t ldx, const void* w, uint32_t ldw,
+                                                  const int64_t* target, int64_t ignore_index, const float* lse,
+                                                  const float* dloss, void* dx, uint32_t lddx, void* dw,
+                                                  uint32_t lddw, vkblas_dtype_t dw_type, float beta, void* stream) {
+    if (!known_type(type) || (dw && dw_type != type && dw_type != VKBLAS_DT_F32)) return VKBLAS_ERR_PARAM;
+    if (V == 0 || K == 0 || M > DIM_MAX || V > DIM_MAX || K > DIM_MAX || ldx < K || ldw < K || (dx && lddx < K) ||
+        (dw && lddw < K))
+        return VKBLAS_ERR_PARAM;
+    op_call c;
+    op_begin(&c, "linear_xent_backward", stream);
+    if (M == 0) return empty_gradient(&c, dw_type, V, K, dw, lddw, beta);
+    if (!x || !w || !target || !lse || !dloss) return VKBLAS_ERR_PARAM;
+    if (!dx && !dw) return VKBLAS_OK;
+    if (vkb_engine_trace())
+        fprintf(stderr, "[vkblas] linear_xent_backward type=%d M=%u V=%u K=%u\n", (int)type, M, V, K);
+    return logits_backward(&c, type, M, V, K, x, ldx, w, ldw, target, ignore_index, NULL, type, NULL, lse, dloss, dx,
+                           lddx, dw, lddw, dw_type, beta);
+}
+
+/* ------------------------------------------------- distillation */
+
+/* A target that no class has */
+#define NO_TARGET INT64_MIN
+
+static int distill_args(vkblas_dtype_t type, uint32_t M, uint32_t V, uint32_t K, uint32_t ldx, uint32_t ldw,
+                        uint32_t n_top, uint32_t ldtop, vkblas_dtype_t t_type, uint32_t ldt, float temperature) {
+    if (!known_type(type) || (t_type != type && t_type != VKBLAS_DT_F32)) return 0;
+    if (V == 0 || K == 0 || M > DIM_MAX || V > DIM_MAX || K > DIM_MAX || ldx < K || ldw < K) return 0;
+    if (n_top == 0 || n_top > VKBLAS_DISTILL_TOP || ldtop < n_top || ldt < n_top) return 0;
+    return temperature > 0.0f && temperature <= FLT_MAX && 1.0f / temperature <= FLT_MAX;
+}
+
+vkblas_status_t vkblas_linear_distill_async(vkblas_dtype_t type, uint32_t M, uint32_t V, uint32_t K, const void* x,
+                                            uint32_t ldx, const void* w, uint32_t ldw, uint32_t n_top,
+                                            const int64_t* top, uint32_t ldtop, vkblas_dtype_t t_type, const void* t, uint32_t ldt,
+                                            float temperature, float* loss, float* lse, float* z_top, void* stream) {
+    if (!distill_args(type, M, V, K, ldx, ldw, n_top, ldtop, t_type, ldt, temperature)) return VKBLAS_ERR_PARAM;
+    if (M == 0) return VKBLAS_OK;
+    if (!x || !w || !top || !t || !loss || !lse || !z_top) return VKBLAS_ERR_PARAM;
+    op_call c;
+    op_begin(&c, "linear_distill", stream);
+    if (vkb_engine_trace())
+        fprintf(stderr, "[vkblas] linear_distill type=%d M=%u V=%u K=%u n_top=%u\n", (int)type, M, V, K, n_top);
+    const int kernel = row_statistics(&c, type, M, V, K, 1.0f / temperature, x, ldx, w, ldw, NULL, 0, NULL, lse);
+    if (kernel == VKBLAS_KERNEL_NONE) return c.st;
+    const vkb_distill q = {.M = M, .V = V, .n = n_top, .top = top, .ldtop = ldtop, .t = t, .ldt = ldt,
+                           .temp = temperature};
+    if (c.st == VKBLAS_OK)
+        step(&c, vkb_launch_distill_rows(type, t_type, &q, K, x, ldx, w, ldw, lse, loss, z_top, stream), 1);
+    return op_end(&c, kernel);
+}
+
+vkblas_status_t vkblas_linear_distill_backward_async(vkblas_dtype_t type, uint32_t M, uint32_t V, uint32_t K,
+                                                     const void* x, uint32_t ldx, const void* w, uint32_t ldw,
+                                                     uint32_t n_top, const int64_t* top, uint32_t ldtop,
+                                                     vkblas_dtype_t t_type, const void* t, uint32_t ldt,
+                                                     float temperature, const float* lse, const float* z_top,
+                                                     const float* dloss, void* dx, uint32_t lddx, void* dw,
+                                                     uint32_t lddw, vkblas_dtype_t dw_type, float beta, void* stream) {
+    if (!distill_args(type, M, V, K, ldx, ldw, n_top, ldtop, t_type, ldt, temperature)) return VKBLAS_ERR_PARAM;
+    if ((dw && dw_type != type && dw_type != VKBLAS_DT_F32) || (dx && lddx < K) || (dw && lddw < K))
+        return VKBLAS_ERR_PARAM;
+    op_call c;
+    op_begin(&c, "linear_distill_backward", stream);
+    if (M == 0) return empty_gradient(&c, dw_type, V, K, dw, lddw, beta);
+    if (!x || !w || !top || !t || !lse || !z_top || !dloss) return VKBLAS_ERR_PARAM;
+    if (!dx && !dw) return VKBLAS_OK;
+    if (vkb_engine_trace())
+        fprintf(stderr, "[vkblas] linear_distill_backward type=%d M=%u V=%u K=%u n_top=%u\n", (int)type, M, V, K,
+                n_top);
+    vkb_distill q = {.M = M, .V = V, .n = n_top, .top = top, .ldtop = ldtop, .t = t, .ldt = ldt, .temp = temperature,
+                     .ignore = NO_TARGET};
+    return logits_backward(&c, type, M, V, K, x, ldx, w, ldw, NULL, 0, &q, t_type, z_top, lse, dloss, dx, lddx, dw,
+                           lddw, dw_type, beta);
+}
+
+/* -------------------------------------------------------------- embedding */
+
+vkblas_status_t vkblas_embedding_async(vkblas_dtype_t type, vkblas_dtype_t w_type, uint32_t M, uint32_t V, uint32_t N,
+                                       const int64_t* ids, int64_t pad_id, const void* w, uint32_t ldw, float scale,
+                                       void* y, uint32_t ldy, void* stream) {
+    if (!known_type(type) || (w_type != type && w_type != VKBLAS_DT_F32)) return VKBLAS_ERR_PARAM;
+    if (V == 0 || N == 0 || M > DIM_MAX || V > DIM_MAX || N > DIM_MAX || ldw < N || ldy < N) return VKBLAS_ERR_PARAM;
+    if (M == 0) return VKBLAS_OK;
+    if (!ids || !w || !y) return VKBLAS_ERR_PARAM;
+    op_call c;
+    op_begin(&c, "embedding", stream);
+    if (vkb_engine_trace()) fprintf(stderr, "[vkblas] embedding type=%d M=%u V=%u N=%u\n", (int)type, M, V, N);
+    if (room(&c) != VKBLAS_OK) return c.st;
+    step(&c, vkb_launch_embedding(type, w_type, M, V, N, ids, pad_id, w, ldw, scale, y, ldy, stream), 1);
+    return op_end(&c, VKBLAS_KERNEL_EMBED);
+}
+
+vkblas_status_t vkblas_embedding_backward_async(vkblas_dtype_t type, uint32_t M, uint32_t V, uint32_t N,
+                                                const int64_t* ids, int64_t pad_id, const void* dy, uint32_t lddy,
+                                                float scale, void* dw, uint32_t lddw, vkblas_dtype_t dw_type,
+                                                float beta, void* stream) {
+    if (!known_type(type) || (dw_type != type && dw_type != VKBLAS_DT_F32)) return VKBLAS_ERR_PARAM;
+    if (V == 0 || N == 0 || M > DIM_MAX || V > DIM_MAX || N > DIM_MAX || lddy < N || lddw < N) return VKBLAS_ERR_PARAM;
+    if (!dw) return VKBLAS_ERR_PARAM;
+    op_call c;
+    op_begin(&c, "embedding_backward", stream);
+    if (M == 0) return empty_gradient(&c, dw_type, V, N, dw, lddw, beta);
+    if (!ids || !dy) return VKBLAS_ERR_PARAM;
+    if (vkb_engine_trace()) fprintf(stderr, "[vkblas] embedding_backward type=%d M=%u V=%u N=%u\n", (int)type, M, V, N);
+    /* chunks of 8 pairs, or as many as VKB_EMBED_CHUNKS have */
+    vkb_embedding_sums a = {.M = M, .V = V, .N = N, .dy = dy, .lddy = lddy, .dw = dw, .lddw = lddw, .scale = scale,
+                            .beta = beta};
+    a.chunk = (uint32_t)(((uint64_t)M + VKB_EMBED_CHUNKS - 1) / VKB_EMBED_CHUNKS);
+    if (a.chunk < 8) a.chunk = 8;
+    a.chunks = (uint32_t)(((uint64_t)M + a.chunk - 1) / a.chunk);
+    const int merges = M > VKB_EMBED_RUN;
+    const size_t o_k = buf(&c, (uint64_t)M * 4), o_o = buf(&c, (uint64_t)M * 4);
+    const size_t o_k2 = merges ? buf(&c, (uint64_t)M * 4) : 0, o_o2 = merges ? buf(&c, (uint64_t)M * 4) : 0;
+    const size_t o_p = a.chunks > 1 ? buf(&c, (uint64_t)a.chunks * 2 * N * sizeof(float)) : 0;
+    if (room(&c) != VKBLAS_OK) return c.st;
+    uint32_t *key = at(&c, o_k), *order = at(&c, o_o), *key2 = at(&c, o_k2), *order2 = at(&c, o_o2);
+    int ok = step(&c, vkb_launch_embedding_rank(M, V, ids, pad_id, key, order, dw_type, N,
+                                                beta == 0.0f ? dw : NULL, lddw, stream), beta == 0.0f);
+    for (uint64_t len = VKB_EMBED_RUN; ok && len < M; len *= VKB_EMBED_WAYS) {
+        ok = step(&c, vkb_launch_embedding_merge(M, len, key, order, key2, order2, stream), 0);
+        uint32_t *k = key, *o = order;
+        key = key2;
+        order = order2;
+        key2 = k;
+        order2 = o;
+    }
+    if (ok && beta != 0.0f && beta != 1.0f)
+        ok = step(&c, vkb_launch_embedding_scale(dw_type, M, V, N, key, dw, lddw, beta, stream), 1);
+    a.key = key;
+    a.order = order;
+    a.part = a.chunks > 1 ? (float*)at(&c, o_p) : NULL;
+    if (ok) step(&c, vkb_launch_embedding_sums(type, dw_type, &a, stream), 1);
+    return op_end(&c, VKBLAS_KERNEL_EMBED);
+}
+
+/* ------------------------------------------------------------ policy loss */
+
+static int policy_args(uint32_t B, uint32_t T, const float* logp, uint32_t ldp, const float* old_logp, uint32_t ldo,
+                       const float* ref_logp, uint32_t ldr, const float* adv, uint32_t ldadv, uint32_t adv_step,
+                       const uint8_t* mask, uint32_t ldmask, float clip_low, float clip_high, float kl_coef,
+                       vkb_policy* p) {
+    if (T == 0 || B > DIM_MAX || T > DIM_MAX || ldp < T || ldo < T || (ref_logp && ldr < T) || adv_step > 1 ||
+        ldadv < (adv_step ? T : 1) || (mask && ldmask < T))
+        return 0;
+    if (!(clip_low >= 0.0f) || !(clip_high >= 0.0f) || !(kl_coef >= -FLT_MAX && kl_coef <= FLT_MAX)) return 0;
+    /* the bounds as those of logp - old_logp; one at or below a ratio of 0 holds nothing back */
+    *p = (vkb_policy){.B = B, .T = T, .logp = logp, .old = old_logp, .ref = ref_logp, .adv = adv, .ldp = ldp,
+                      .ldo = ldo, .ldr = ldr, .ldadv = ldadv, .adv_step = adv_step, .mask = mask, .ldmask = ldmask,
+                      .low = clip_low < 1.0f ? log1p(-(double)clip_low) : -INFINITY, .high = log1p((double)clip_high),
+                      .r_low = (float)(1.0 - (double)clip_low), .r_high = (float)(1.0 + (double)clip_high),
+                      .kl = kl_coef};
+    if (B) vkb_policy_units(p);
+    return 1;
+}
+
+vkblas_status_t vkblas_policy_loss_async(vkblas_reduce_t reduce, uint32_t B, uint32_t T, const float* logp,
+                                         uint32_t ldp, const float* old_logp, uint32_t ldo, const float* ref_logp, uint32_t ldr,
+                                         const float* adv, uint32_t ldadv, uint32_t adv_step, const uint8_t* mask,
+                                         uint32_t ldmask, float clip_low, float clip_high, float kl_coef, float* stats,
+                                         float* norm, void* stream) {
+    vkb_policy p;
+    if (reduce < VKBLAS_REDUCE_TOKENS || reduce > VKBLAS_REDUCE_SUM ||
+        !policy_args(B, T, logp, ldp, old_logp, ldo, ref_logp, ldr, adv, ldadv, adv_step, mask, ldmask, clip_low,
+                     clip_high, kl_coef, &p))
+        return VKBLAS_ERR_PARAM;
+    if (B == 0) return VKBLAS_OK;
+    if (!logp || !old_logp || !adv || !stats || !norm) return VKBLAS_ERR_PARAM;
+    op_call c;
+    op_begin(&c, "policy_loss", stream);
+    if (vkb_engine_trace()) fprintf(stderr, "[vkblas] policy_loss reduce=%d B=%u T=%u\n", (int)reduce, B, T);
+    const size_t bytes = vkb_policy_part_bytes(&p), o_p = bytes ? buf(&c, bytes) : 0;
+    if (room(&c) != VKBLAS_OK) return c.st;
+    step(&c, vkb_launch_policy(&p, (int)reduce, bytes ? at(&c, o_p) : NULL, stats, norm, stream), 1);
+    return op_end(&c, VKBLAS_KERNEL_POLICY);
+}
+
+vkblas_status_t vkblas_policy_loss_backward_async(uint32_t B, uint32_t T, const float* logp, uint32_t ldp,
+                                                  const float* old_logp, uint32_t ldo, const float* ref_logp,
+                                                  uint32_t ldr, const float* adv, uint32_t ldadv, uint32_t adv_step,
+                                                  const uint8_t* mask, uint32_t ldmask, float clip_low, float clip_high,
+                                                  float kl_coef, const float* norm, const float* dloss, float* dlogp,
+                                                  uint32_t lddp, void* stream) {
+    vkb_policy p;
+    if (lddp < T || !policy_args(B, T, logp, ldp, old_logp, ldo, ref_logp, ldr, adv, ldadv, adv_step, mask, ldmask,
+                                 clip_low, clip_high, kl_coef, &p))
+        return VKBLAS_ERR_PARAM;
+    if (B == 0) return VKBLAS_OK;
+    if (!logp || !old_logp || !adv || !norm || !dloss || !dlogp) return VKBLAS_ERR_PARAM;
+    op_call c;
+    op_begin(&c, "policy_loss_backward", stream);
+    if (vkb_engine_trace()) fprintf(stderr, "[vkblas] policy_loss_backward B=%u T=%u\n", B, T);
+    if (room(&c) != VKBLAS_OK) return c.st;
+    step(&c, vkb_launch_policy_grad(&p, norm, dloss, dlogp, lddp, stream), 1);
+    return op_end(&c, VKBLAS_KERNEL_POLICY);
 }

@@ -6,7 +6,7 @@
 #include "gemm_mfma.hpp"
 #include "vkb_launch.h"
 #include "vkb_nn_launch.h"
-#include "vkblas_nn.h"
+#include "vkblas_train.h"
 
 namespace vkb {
 

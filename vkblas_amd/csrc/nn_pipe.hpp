@@ -64,17 +64,19 @@ static int launch_glu(const vkb_op_args* a, int act_code, void* h, int64_t ldh, 
 }
 
 template <typename T>
-static int launch_xent_stats(const vkb_op_args* a, const int64_t* target, float* parts, float* zt, hipStream_t st) {
+static int launch_xent_stats(const vkb_op_args* a, float inv_t, const int64_t* target, float* parts, float* zt,
+                             hipStream_t st) {
     XentParams p = op_params<T, XentParams>(a);
     p.target = target;
     p.parts = (float2*)parts;
     p.zt = zt;
+    p.c2 = inv_t * LOG2E;
     return launch_tiles<T, XentStatsOp<T>>(a, p, st);
 }
 
 template <typename T>
 static int launch_xent_grad(const vkb_op_args* a, uint32_t Ms, uint32_t Ns, uint32_t v0, uint32_t V,
-                            const int64_t* target, int64_t ignore, const float* lse, const float* dloss,
+                            float inv_t, const int64_t* target, int64_t ignore, const float* lse, const float* dloss,
                             vkb_scale scale, void* D, int64_t ldd, hipStream_t st) {
     XentParams p = op_params<T, XentParams>(a);
     p.target = target;
@@ -83,6 +85,7 @@ static int launch_xent_grad(const vkb_op_args* a, uint32_t Ms, uint32_t Ns, uint
     p.v0 = v0;
     p.V = V;
     p.ignore = ignore;
+    p.c2 = inv_t * LOG2E;
     p.lse = lse;
     p.dloss = dloss;
     p.scale = with_to<T>(scale);
@@ -98,14 +101,14 @@ static int launch_xent_grad(const vkb_op_args* a, uint32_t Ms, uint32_t Ns, uint
                                          int64_t ldgu, void* st) {                                                   \
         return vkb::launch_glu<T>(a, act, h, ldh, gu, ldgu, (hipStream_t)st);                                        \
     }                                                                                                                \
-    extern "C" int vkb_launch_xent_stats_##NAME(const vkb_op_args* a, const int64_t* target, float* parts,           \
-                                                float* zt, void* st) {                                               \
-        return vkb::launch_xent_stats<T>(a, target, parts, zt, (hipStream_t)st);                                     \
+    extern "C" int vkb_launch_xent_stats_##NAME(const vkb_op_args* a, float inv_t, const int64_t* target,            \
+                                                float* parts, float* zt, void* st) {                                 \
+        return vkb::launch_xent_stats<T>(a, inv_t, target, parts, zt, (hipStream_t)st);                              \
     }                                                                                                                \
     extern "C" int vkb_launch_xent_grad_##NAME(const vkb_op_args* a, uint32_t Ms, uint32_t Ns, uint32_t v0,          \
-                                               uint32_t V, const int64_t* target, int64_t ignore, const float* lse,  \
-                                               const float* dloss, vkb_scale scale, void* D, int64_t ldd,            \
-                                               void* st) {                                                           \
-        return vkb::launch_xent_grad<T>(a, Ms, Ns, v0, V, target, ignore, lse, dloss, scale, D, ldd,                 \
+                                               uint32_t V, float inv_t, const int64_t* target, int64_t ignore,       \
+                                               const float* lse, const float* dloss, vkb_scale scale, void* D,       \
+                                               int64_t ldd, void* st) {                                              \
+        return vkb::launch_xent_grad<T>(a, Ms, Ns, v0, V, inv_t, target, ignore, lse, dloss, scale, D, ldd,          \
                                         (hipStream_t)st);                                                            \
     }

@@ -1,7 +1,7 @@
 /*
  * pycall.c — the Python binding's calls without ctypes (module
- * vkblas_amd._call): vkblas_gemm_ex_async and the functions of vkblas_nn.h, and
- * the check of those functions' numbers against their C types.
+ * vkblas_amd._call): vkblas_gemm_ex_async and the functions of vkblas_nn.h
+ * and vkblas_train.h, and the check of those functions' numbers against their C types.
  *
  * A small call is bound by its launch on the host, and ctypes' conversion of
  * 25 arguments was the largest part of that: 3.1 us for vkblas_gemm_async and
@@ -16,7 +16,7 @@
  */
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
-#include "vkblas_nn.h"
+#include "vkblas_train.h"
 
 typedef vkblas_status_t (*gemm_ex_fn)(vkblas_dtype_t, vkblas_dtype_t, vkblas_op_t, vkblas_op_t, uint32_t, uint32_t,
                                       uint32_t, float, const void*, uint32_t, const void*, uint32_t, float, void*,
@@ -115,7 +115,7 @@ static int get_args(const char* name, const char* kind, PyObject* const* a, Py_s
     static PyObject* NAME(PyObject* self, PyObject* const* a, Py_ssize_t n) {                      \
         (void)self;                                                                                \
         unsigned long long v[sizeof(KIND)];                                                        \
-        float f[2];                                                                                \
+        float f[3];                                                                                \
         PyObject* result;                                                                          \
         if (!get_args(#NAME, KIND, a, n, v, f, &result)) return result;                            \
         int st;                                                                                    \
@@ -140,6 +140,23 @@ NN_CALL(linear_xent, "piiiipipipippp",
 NN_CALL(linear_xent_backward, "piiiipipipipppipiifp",
         (I(1), U(2), U(3), U(4), P(5), U(6), P(7), U(8), P(9), (int64_t)v[10], P(11), P(12), P(13), U(14), P(15),
          U(16), I(17), f[0], P(19)))
+
+NN_CALL(embedding, "piiiiipipifpip",
+        (I(1), I(2), U(3), U(4), U(5), P(6), (int64_t)v[7], P(8), U(9), f[0], P(11), U(12), P(13)))
+NN_CALL(embedding_backward, "piiiipipifpiifp",
+        (I(1), U(2), U(3), U(4), P(5), (int64_t)v[6], P(7), U(8), f[0], P(10), U(11), I(12), f[1], P(14)))
+NN_CALL(linear_distill, "piiiipipiipiipifpppp",
+        (I(1), U(2), U(3), U(4), P(5), U(6), P(7), U(8), U(9), P(10), U(11), I(12), P(13), U(14), f[0], P(16), P(17),
+         P(18), P(19)))
+NN_CALL(linear_distill_backward, "piiiipipiipiipifppppipiifp",
+        (I(1), U(2), U(3), U(4), P(5), U(6), P(7), U(8), U(9), P(10), U(11), I(12), P(13), U(14), f[0], P(16), P(17),
+         P(18), P(19), U(20), P(21), U(22), I(23), f[1], P(25)))
+NN_CALL(policy_loss, "piiipipipipiipifffppp",
+        (I(1), U(2), U(3), P(4), U(5), P(6), U(7), P(8), U(9), P(10), U(11), U(12), P(13), U(14), f[0], f[1], f[2], P(18),
+         P(19), P(20)))
+NN_CALL(policy_loss_backward, "piipipipipiipifffpppip",
+        (U(1), U(2), P(3), U(4), P(5), U(6), P(7), U(8), P(9), U(10), U(11), P(12), U(13), f[0], f[1], f[2], P(17), P(18),
+         P(19), U(20), P(21)))
 
 /* fits(kinds, arguments): whether the C types hold the whole numbers among
  * them; u: uint32_t, i: int, l: int64_t, anything else is not looked at */
@@ -170,6 +187,9 @@ static PyMethodDef methods[] = {
                          "vkblas_" #NAME "_async by address; None if an argument is not a plain int, float or None"}
                                 NN_METHOD(layer_norm), NN_METHOD(layer_norm_backward), NN_METHOD(glu),
                                 NN_METHOD(glu_backward), NN_METHOD(linear_xent), NN_METHOD(linear_xent_backward),
+                                NN_METHOD(embedding), NN_METHOD(embedding_backward), NN_METHOD(linear_distill),
+                                NN_METHOD(linear_distill_backward), NN_METHOD(policy_loss),
+                                NN_METHOD(policy_loss_backward),
                                 {"gemm_ex", (PyCFunction)(void (*)(void))gemm_ex, METH_FASTCALL,
                                  "vkblas_gemm_ex_async by address; None if an argument is not a plain int, float or None"},
                                 {NULL, NULL, 0, NULL}};

@@ -1,10 +1,11 @@
 /*
  * vkb_nn_launch.h — internal C ABI between the host side of the operators in
- * vkblas_nn.h (nn.c) and their gfx950 kernels.  As vkb_launch.h: plain
+ * vkblas_nn.h and vkblas_train.h (nn.c) and their gfx950 kernels.  As vkb_launch.h: plain
  * pointers and sizes, element types VKB_T_*, every launcher enqueues on the
  * stream and returns 0 or a hipError_t value.
  */
 #pragma once
+#include <stddef.h>
 #include <stdint.h>
 
 #ifdef __cplusplus
@@ -88,23 +89,97 @@ int vkb_glu_direct_fits(int type, uint32_t M, uint32_t N, uint32_t K, uint32_t l
 int vkb_launch_glu_direct(int type, int act, uint32_t M, uint32_t N, uint32_t K, const void* x, uint32_t ldx,
                           const void* w, uint32_t ldw, void* h, uint32_t ldh, void* gu, uint32_t ldgu, void* stream);
 
+/* Embedding (embedding.hip).  Its gradient: rank writes the M pairs (key, row of
+ * dy) sorted by key, then row, in each run of VKB_EMBED_RUN (key: the token's
+ * id, V where its row adds nothing), and zeroes dw (NULL: not); merge makes
+ * sorted runs of VKB_EMBED_WAYS * len out of ones of len; scale: dw = beta * dw
+ * on the rows of no token; sums: the rows of the tokens, the sorted pairs in
+ * `chunks` chunks of `chunk` (the last may be shorter), at most
+ * VKB_EMBED_CHUNKS, part chunks x 2 x N floats. */
+#define VKB_EMBED_RUN 4096u
+#define VKB_EMBED_WAYS 16u
+#define VKB_EMBED_CHUNKS 2048u
+int vkb_launch_embedding(int type, int w_type, uint32_t M, uint32_t V, uint32_t N, const int64_t* ids, int64_t pad,
+                         const void* w, int64_t ldw, float scale, void* y, int64_t ldy, void* stream);
+int vkb_launch_embedding_rank(uint32_t M, uint32_t V, const int64_t* ids, int64_t pad, uint32_t* key, uint32_t* order,
+                              int w_type, uint32_t N, void* dw, int64_t lddw, void* stream);
+int vkb_launch_embedding_merge(uint32_t M, uint64_t len, const uint32_t* key_in, const uint32_t* order_in,
+                               uint32_t* key, uint32_t* order, void* stream);
+int vkb_launch_embedding_scale(int w_type, uint32_t M, uint32_t V, uint32_t N, const uint32_t* key, void* dw,
+                               int64_t lddw, float beta, void* stream);
+typedef struct vkb_embedding_sums {
+    uint32_t M, V, N, chunk, chunks;
+    const uint32_t *key, *order;
+    const void* dy;
+    int64_t lddy;
+    void* dw;
+    int64_t lddw;
+    float scale, beta;
+    float* part;
+} vkb_embedding_sums;
+int vkb_launch_embedding_sums(int type, int w_type, const vkb_embedding_sums* a, void* stream);
+
+/* Policy loss (policy.hip) over `units` parts of a sequence each, `unit` tokens
+ * long.  loss: sums to part (NULL: the call is small, one workgroup does it
+ * all), vkb_policy_part_bytes; then finish; grad: dlogp. */
+typedef struct vkb_policy {
+    uint32_t B, T;
+    const float *logp, *old, *ref, *adv;
+    int64_t ldp, ldo, ldr, ldadv;
+    uint32_t adv_step;
+    const uint8_t* mask;
+    int64_t ldmask;
+    double low, high;                /* bounds of logp - old */
+    float r_low, r_high;             /* of its exponential */
+    float kl;
+    uint32_t unit, units;            /* units of a sequence */
+} vkb_policy;
+void vkb_policy_units(vkb_policy* p);
+size_t vkb_policy_part_bytes(const vkb_policy* p);   /* 0: none needed */
+int vkb_launch_policy(const vkb_policy* p, int reduce, void* part, float* stats, float* norm, void* stream);
+int vkb_launch_policy_grad(const vkb_policy* p, const float* norm, const float* dloss, float* dlogp, int64_t lddp,
+                           void* stream);
+
 /* Linear cross entropy (xent.hip).  stats: over z, columns v0 .. v0 + n - 1
- * of the logits, the pair (max, sum of exp(z - max)) of each row and each
+ * of the logits, the pair (max, sum of exp((z - max) inv_t)) of each row and each
  * VKB_XENT_SLICE columns, to parts[slice * M + m], and the target's logit to
- * zt[m].  finish: lse and loss of S such slices.  rows: both at once, for
+ * zt[m].  inv_t: 1, or 1 / temperature, with which lse is that of z inv_t and the
+ * loss is not asked for.  finish: lse and loss of S such slices.  rows: both at once, for
  * logits of at most VKB_XENT_ROW columns in all. */
 #define VKB_XENT_SLICE 4096u
-int vkb_launch_xent_stats(uint32_t M, uint32_t n, uint32_t v0, const float* z, int64_t ldz, const int64_t* target,
-                          float* parts, float* zt, void* stream);
+int vkb_launch_xent_stats(uint32_t M, uint32_t n, uint32_t v0, float inv_t, const float* z, int64_t ldz,
+                          const int64_t* target, float* parts, float* zt, void* stream);
 #define VKB_XENT_ROW 16384u
-int vkb_launch_xent_rows(uint32_t M, uint32_t V, const float* z, int64_t ldz, const int64_t* target, int64_t ignore,
-                         float* loss, float* lse, void* stream);
-int vkb_launch_xent_finish(uint32_t M, uint32_t V, uint32_t S, const float* parts, const float* zt,
+int vkb_launch_xent_rows(uint32_t M, uint32_t V, float inv_t, const float* z, int64_t ldz, const int64_t* target,
+                         int64_t ignore, float* loss, float* lse, void* stream);
+int vkb_launch_xent_finish(uint32_t M, uint32_t V, uint32_t S, float inv_t, const float* parts, const float* zt,
                            const int64_t* target, int64_t ignore, float* loss, float* lse, void* stream);
-/* D = scal[0] * dloss * (exp(z - lse) - [v == target]), without scal by 1. */
-int vkb_launch_xent_grad(int type, uint32_t M, uint32_t n, uint32_t v0, uint32_t V, const float* z, int64_t ldz,
-                         const int64_t* target, int64_t ignore, const float* lse, const float* dloss,
+/* D = scal[0] * dloss * (exp(z inv_t - lse) - [v == target]), without scal by 1. */
+int vkb_launch_xent_grad(int type, uint32_t M, uint32_t n, uint32_t v0, uint32_t V, float inv_t, const float* z,
+                         int64_t ldz, const int64_t* target, int64_t ignore, const float* lse, const float* dloss,
                          vkb_scale scale, void* D, int64_t ldd, void* stream);
+
+/* Distillation from a teacher's top logits (distill.hip).  rows: z_top and loss
+ * from lse.  prepare, for the backward pass: q_top (M x n), T dloss (dl) and
+ * targets for the kernels of D (ignore: a value no class has); patch: D's
+ * elements of columns v0 .. v0 + cols - 1 at the entries, with scal[0] as those
+ * kernels left it (NULL: 1). */
+typedef struct vkb_distill {
+    uint32_t M, V, n;
+    const int64_t* top;
+    int64_t ldtop;
+    const void* t;
+    int64_t ldt;
+    float temp;
+    int64_t ignore;
+    float *q_top, *dl;
+    int64_t* target;
+} vkb_distill;
+int vkb_launch_distill_rows(int type, int t_type, const vkb_distill* d, uint32_t K, const void* x, int64_t ldx,
+                            const void* w, int64_t ldw, const float* lse, float* loss, float* z_top, void* stream);
+int vkb_launch_distill_prepare(int t_type, const vkb_distill* d, const float* dloss, void* stream);
+int vkb_launch_distill_patch(int type, const vkb_distill* d, uint32_t v0, uint32_t cols, const float* lse,
+                             const float* z_top, const float* scal, void* D, int64_t ldd, void* stream);
 
 /* dx = D W and dw = beta dw + D^T x of a small gradient in one launch (pair.hip):
  * D M x R, W R x K, x M x K; dx of type, dw of w_type. */
@@ -172,10 +247,11 @@ int vkb_launch_glu(const vkb_op_args* a, int act, void* h, int64_t ldh, void* gu
 /* parts: a pair for each row and each half of a tile's columns (128 or 64),
  * vkb_xent_slices of them */
 uint32_t vkb_xent_slices(const vkb_op_args* a);
-int vkb_launch_xent_stats_op(const vkb_op_args* a, const int64_t* target, float* parts, float* zt, void* stream);
+int vkb_launch_xent_stats_op(const vkb_op_args* a, float inv_t, const int64_t* target, float* parts, float* zt,
+                             void* stream);
 /* D as vkb_launch_xent_grad, stored on Ms rows and Ns columns, zero past M and
  * N: at least those, at most them rounded up to 128, Ns a multiple of 8 */
-int vkb_launch_xent_grad_op(const vkb_op_args* a, uint32_t Ms, uint32_t Ns, uint32_t v0, uint32_t V,
+int vkb_launch_xent_grad_op(const vkb_op_args* a, uint32_t Ms, uint32_t Ns, uint32_t v0, uint32_t V, float inv_t,
                             const int64_t* target, int64_t ignore, const float* lse, const float* dloss,
                             vkb_scale scale, void* D, int64_t ldd, void* stream);
 

@@ -8,6 +8,10 @@
 // Infinities follow the formula: where top is not finite the exponentials
 // take 0 in its place, so an all -inf part has s = 0 and drops out of the
 // join, a +inf gives s = inf and lse = inf, and a NaN reaches s and lse.
+//
+// inv_t, 1 or the inverse of a distillation's temperature, multiplies the
+// logits: c = inv_t log2(e) takes it into the exponentials, and top stays that
+// of z.  With 1 the bits are those without it.
 #include "nn_common.hpp"
 #include "vkb_nn_launch.h"
 
@@ -39,9 +43,9 @@ __device__ __forceinline__ float block_sum(float v, float* sh) {
 
 // One workgroup per row and slice of VKB_XENT_SLICE columns, the slice in
 // registers between the two reductions; rows strided over y.
-__global__ __launch_bounds__(THREADS) void xent_stats_kernel(uint32_t M, uint32_t n, uint32_t v0, const float* z,
-                                                             int64_t ldz, const int64_t* target, float2* parts,
-                                                             float* zt) {
+__global__ __launch_bounds__(THREADS) void xent_stats_kernel(uint32_t M, uint32_t n, uint32_t v0, float c2,
+                                                             const float* z, int64_t ldz, const int64_t* target,
+                                                             float2* parts, float* zt) {
     constexpr int NV = VKB_XENT_SLICE / THREADS / 4;
     __shared__ float sh[WAVES];
     const int64_t c0 = (int64_t)blockIdx.x * VKB_XENT_SLICE + threadIdx.x * 4;
@@ -63,7 +67,7 @@ __global__ __launch_bounds__(THREADS) void xent_stats_kernel(uint32_t M, uint32_
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s += fast_exp(x[i][e] - off);
+            for (int e = 0; e < 4; ++e) s += __builtin_amdgcn_exp2f((x[i][e] - off) * c2);
         s = block_sum(s, sh);
         if (threadIdx.x == 0) {
             parts[(int64_t)blockIdx.x * M + m] = float2{top, s};
@@ -79,12 +83,14 @@ __global__ __launch_bounds__(THREADS) void xent_stats_kernel(uint32_t M, uint32_
 // joins slices j, j + 256 / FROWS, .., eight loads in flight; then the threads'
 // pairs join in LDS.
 constexpr int FROWS = 8, FSLICES = THREADS / FROWS;
-__global__ __launch_bounds__(THREADS) void xent_finish_kernel(uint32_t M, uint32_t V, uint32_t S, const float2* parts,
-                                                              const float* zt, const int64_t* target, int64_t ignore,
+__global__ __launch_bounds__(THREADS) void xent_finish_kernel(uint32_t M, uint32_t V, uint32_t S, float inv_t,
+                                                              const float2* parts, const float* zt,
+                                                              const int64_t* target, int64_t ignore,
                                                               float* loss, float* lse) {
     __shared__ float2 sh[FSLICES][FROWS + 1];
     const uint32_t r = threadIdx.x % FROWS, j = threadIdx.x / FROWS;
     const uint32_t m = blockIdx.x * FROWS + r;
+    const float c2 = inv_t * LOG2E;
     float top = -INFINITY, s = 0.0f;
     if (m < M)
         for (uint32_t i = j; i < S; i += 8 * FSLICES) {
@@ -98,9 +104,9 @@ __global__ __launch_bounds__(THREADS) void xent_finish_kernel(uint32_t M, uint32
 #pragma unroll
             for (int k = 0; k < 8; ++k) t = fmaxf(t, p[k].x);
             const float off = finite_or_0(t);
-            s *= fast_exp(top - off);
+            s *= __builtin_amdgcn_exp2f((top - off) * c2);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) s += p[k].y * fast_exp(p[k].x - off);
+            for (int k = 0; k < 8; ++k) s += p[k].y * __builtin_amdgcn_exp2f((p[k].x - off) * c2);
             top = t;
         }
     sh[j][r] = float2{top, s};
@@ -109,8 +115,8 @@ __global__ __launch_bounds__(THREADS) void xent_finish_kernel(uint32_t M, uint32
     for (uint32_t i = 1; i < FSLICES; ++i) top = fmaxf(top, sh[i][r].x);
     const float off = finite_or_0(top);
     s = 0.0f;
-    for (uint32_t i = 0; i < FSLICES; ++i) s += sh[i][r].y * fast_exp(sh[i][r].x - off);
-    const float l = off + logf(s);
+    for (uint32_t i = 0; i < FSLICES; ++i) s += sh[i][r].y * __builtin_amdgcn_exp2f((sh[i][r].x - off) * c2);
+    const float l = off * inv_t + logf(s);
     lse[m] = l;
     if (loss) {
         const int64_t t = target[m];
@@ -120,8 +126,9 @@ __global__ __launch_bounds__(THREADS) void xent_finish_kernel(uint32_t M, uint32
 
 // A row of at most VKB_XENT_ROW logits, in the registers of one workgroup.
 constexpr uint32_t ROW_THREADS = 1024;
-__global__ __launch_bounds__(ROW_THREADS) void xent_rows_kernel(uint32_t M, uint32_t V, const float* z, int64_t ldz,
-                                                                const int64_t* target, int64_t ignore, float* loss,
+__global__ __launch_bounds__(ROW_THREADS) void xent_rows_kernel(uint32_t M, uint32_t V, float inv_t,
+                                                                const float* z, int64_t ldz, const int64_t* target,
+                                                                int64_t ignore, float* loss,
                                                                 float* lse) {
     constexpr int NV = VKB_XENT_ROW / ROW_THREADS / 4;
     __shared__ float sh[2][ROW_THREADS / 64];
@@ -151,13 +158,13 @@ __global__ __launch_bounds__(ROW_THREADS) void xent_rows_kernel(uint32_t M, uint
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s += fast_exp(x[i][e] - off);
+            for (int e = 0; e < 4; ++e) s += __builtin_amdgcn_exp2f((x[i][e] - off) * (inv_t * LOG2E));
         s = wave_sum(s);
         if ((threadIdx.x & 63) == 0) sh[1][threadIdx.x >> 6] = s;
         __syncthreads();
         if (threadIdx.x == 0) {
             for (uint32_t i = 1; i < waves; ++i) s += sh[1][i];
-            const float l = off + logf(s);
+            const float l = off * inv_t + logf(s);
             lse[m] = l;
             if (loss) {
                 const int64_t t = target[m];
@@ -170,8 +177,8 @@ __global__ __launch_bounds__(ROW_THREADS) void xent_rows_kernel(uint32_t M, uint
 
 template <typename T>
 __global__ __launch_bounds__(WORK) void xent_grad_kernel(uint32_t M, uint32_t n, uint32_t v0, uint32_t V,
-                                                            const float* z, int64_t ldz, const int64_t* target,
-                                                            int64_t ignore, const float* lse, const float* dloss,
+                                                            float inv_t, const float* z, int64_t ldz,
+                                                            const int64_t* target, int64_t ignore, const float* lse, const float* dloss,
                                                             Scale scale, T* D, int64_t ldd) {
     constexpr int VEC = Elem<T>::VEC;
     const float sc = scale_of<T>(scale, dloss, target, M, V, ignore, blockIdx.x == 0 && threadIdx.x < 64, threadIdx.x & 63);
@@ -185,7 +192,7 @@ __global__ __launch_bounds__(WORK) void xent_grad_kernel(uint32_t M, uint32_t n,
         for (int q = 0; q < VEC; q += 4) unpack<float>(ld_chunk(z + (int64_t)m * ldz, c + q, n), x + q);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-            const float p = fast_exp(x[i] - l) - (c + i == t - v0 ? 1.0f : 0.0f);
+            const float p = fast_exp(x[i] * inv_t - l) - (c + i == t - v0 ? 1.0f : 0.0f);
             x[i] = t == ignore ? 0.0f : w * p;
         }
         st_chunk(D + (int64_t)m * ldd, c, n, pack<T>(x));
@@ -199,39 +206,40 @@ using namespace vkb;
 
 static uint32_t rows_y(uint32_t M) { return M < 65535u ? M : 65535u; }
 
-extern "C" int vkb_launch_xent_stats(uint32_t M, uint32_t n, uint32_t v0, const float* z, int64_t ldz,
-                                     const int64_t* target, float* parts, float* zt, void* stream) {
+extern "C" int vkb_launch_xent_stats(uint32_t M, uint32_t n, uint32_t v0, float inv_t, const float* z,
+                                     int64_t ldz, const int64_t* target, float* parts, float* zt, void* stream) {
     hipLaunchKernelGGL(xent_stats_kernel, dim3((n + VKB_XENT_SLICE - 1) / VKB_XENT_SLICE, rows_y(M)), dim3(THREADS), 0,
-                       (hipStream_t)stream, M, n, v0, z, ldz, target, (float2*)parts, zt);
+                       (hipStream_t)stream, M, n, v0, inv_t * LOG2E, z, ldz, target, (float2*)parts, zt);
     return (int)hipGetLastError();
 }
 
-extern "C" int vkb_launch_xent_finish(uint32_t M, uint32_t V, uint32_t S, const float* parts, const float* zt,
-                                      const int64_t* target, int64_t ignore, float* loss, float* lse, void* stream) {
+extern "C" int vkb_launch_xent_finish(uint32_t M, uint32_t V, uint32_t S, float inv_t, const float* parts,
+                                      const float* zt, const int64_t* target, int64_t ignore, float* loss, float* lse, void* stream) {
     const uint64_t groups = ((uint64_t)M + FROWS - 1) / FROWS;
     if (groups > 0xffffffffull / THREADS) return (int)hipErrorInvalidValue;
     hipLaunchKernelGGL(xent_finish_kernel, dim3((uint32_t)groups), dim3(THREADS), 0,
-                       (hipStream_t)stream, M, V, S, (const float2*)parts, zt, target, ignore, loss, lse);
+                       (hipStream_t)stream, M, V, S, inv_t, (const float2*)parts, zt, target, ignore, loss, lse);
     return (int)hipGetLastError();
 }
 
-extern "C" int vkb_launch_xent_rows(uint32_t M, uint32_t V, const float* z, int64_t ldz, const int64_t* target,
-                                    int64_t ignore, float* loss, float* lse, void* stream) {
+extern "C" int vkb_launch_xent_rows(uint32_t M, uint32_t V, float inv_t, const float* z, int64_t ldz,
+                                    const int64_t* target, int64_t ignore, float* loss, float* lse, void* stream) {
     if (V > VKB_XENT_ROW) return (int)hipErrorInvalidValue;
     // whole waves for 16 values a thread
     const uint32_t threads = (V + 1023) / 1024 * 64;
-    hipLaunchKernelGGL(xent_rows_kernel, dim3(M < 65536u ? M : 65536u), dim3(threads), 0, (hipStream_t)stream, M, V, z,
-                       ldz, target, ignore, loss, lse);
+    hipLaunchKernelGGL(xent_rows_kernel, dim3(M < 65536u ? M : 65536u), dim3(threads), 0, (hipStream_t)stream, M, V, inv_t,
+                       z, ldz, target, ignore, loss, lse);
     return (int)hipGetLastError();
 }
 
-extern "C" int vkb_launch_xent_grad(int type, uint32_t M, uint32_t n, uint32_t v0, uint32_t V, const float* z,
-                                    int64_t ldz, const int64_t* target, int64_t ignore, const float* lse,
+extern "C" int vkb_launch_xent_grad(int type, uint32_t M, uint32_t n, uint32_t v0, uint32_t V, float inv_t,
+                                    const float* z, int64_t ldz, const int64_t* target, int64_t ignore, const float* lse,
                                     const float* dloss, vkb_scale scale, void* D, int64_t ldd, void* stream) {
     const bool ok = with_type(type, [&](auto t) {
         using T = decltype(t);
         hipLaunchKernelGGL((xent_grad_kernel<T>), dim3(chunk_blocks(M, chunks_of<T>(n))), dim3(WORK), 0,
-                           (hipStream_t)stream, M, n, v0, V, z, ldz, target, ignore, lse, dloss, with_to<T>(scale), (T*)D, ldd);
+                           (hipStream_t)stream, M, n, v0, V, inv_t, z, ldz, target, ignore, lse, dloss, with_to<T>(scale),
+                           (T*)D, ldd);
     });
     return ok ? (int)hipGetLastError() : (int)hipErrorInvalidValue;
 }
