@@ -40,7 +40,7 @@ class Model(torch.nn.Module):
         self.head = torch.nn.Parameter((torch.randn(classes, width) * width ** -0.5).to(dtype))
 
     def forward(self, tokens, target):
-        x = self.embed[tokens]
+        x = vnn.embedding(tokens, self.embed)
         for b in self.blocks:
             x = b(x)
         return vnn.linear_cross_entropy(vnn.layer_norm(x, self.norm_w), self.head, target)
