@@ -15,8 +15,11 @@
 //    token that ends inside goes to dw, a part that began before the chunk or
 //    goes on after it to the workspace.
 //  - Join: a token of several chunks adds their parts in order.
-// Rows of dw without a token are zeroed beside the sort (beta = 0), left alone
-// (beta = 1), or scaled by a pass that searches each row's id.
+// Rows of dw without a token are zeroed or scaled beside the sums, by
+// workgroups that search the rows' ids (not for beta = 1).
+//
+// Few tokens (VKB_EMBED_DIRECT) take one launch without a workspace: each
+// workgroup looks all ids over for those of its own rows of dw.
 #include "nn_common.hpp"
 
 namespace vkb {
@@ -55,35 +58,40 @@ __device__ __forceinline__ uint32_t sort_key(int64_t id, int64_t pad, uint32_t V
 // run's keys each.  A pair before the token's counts where its key is at most
 // the token's, one after it where it is less.
 constexpr uint32_t RTOK = 16, RGROUPS = WORK / RTOK;
-template <typename W>
 __global__ __launch_bounds__(WORK) void rank_kernel(uint32_t M, uint32_t V, const int64_t* ids, int64_t pad,
-                                                    uint32_t* key, uint32_t* order, uint32_t rank_blocks, uint32_t N,
-                                                    W* dw, int64_t lddw) {
-    if (blockIdx.x >= rank_blocks) {      // dw = 0
-        constexpr int VEC = Elem<W>::VEC;
-        for_chunks(V, (N + VEC - 1) / VEC, rank_blocks, gridDim.x - rank_blocks, [&](uint64_t v, uint32_t k) {
-            st_chunk(dw + (int64_t)v * lddw, (int64_t)k * VEC, N, u32x4{0u, 0u, 0u, 0u});
-        });
-        return;
-    }
+                                                    uint32_t* key, uint32_t* order) {
     __shared__ __attribute__((aligned(16))) uint32_t keys[RUN];
     __shared__ uint32_t count[WORK];
     const uint32_t tok = threadIdx.x % RTOK, g = threadIdx.x / RTOK;
-    for (uint64_t first = (uint64_t)blockIdx.x * RTOK; first < M; first += (uint64_t)rank_blocks * RTOK) {
+    for (uint64_t first = (uint64_t)blockIdx.x * RTOK; first < M; first += (uint64_t)gridDim.x * RTOK) {
         const uint64_t run = first / RUN * RUN;
         const uint32_t n = (uint32_t)min((uint64_t)RUN, M - run), whole = (n + 3) / 4 * 4;
-        for (uint32_t i = threadIdx.x; i < whole; i += WORK) keys[i] = i < n ? sort_key(ids[run + i], pad, V) : ~0u;
+        int64_t id[RUN / WORK];               // all loads in flight
+#pragma unroll
+        for (uint32_t l = 0; l < RUN / WORK; ++l)
+            if (l * WORK < n) id[l] = ids[run + min(l * WORK + threadIdx.x, n - 1)];
+#pragma unroll
+        for (uint32_t l = 0; l < RUN / WORK; ++l) {
+            const uint32_t i = l * WORK + threadIdx.x;
+            if (i < whole) keys[i] = i < n ? sort_key(id[l], pad, V) : ~0u;
+        }
         __syncthreads();
         const uint32_t me = (uint32_t)(first - run) + tok;
         const uint32_t mine = me < n ? keys[me] : 0;
-        // groups take quads of keys in turn: neighbouring ones read neighbouring banks
+        // groups take quads of keys in turn: neighbouring ones read neighbouring banks.  The workgroup's tokens
+        // are 4 quads, so a quad of another place is before or after all of them.
+        const uint32_t here = (uint32_t)(first - run);
         uint32_t below = 0;
 #pragma unroll 4
         for (uint32_t i = 4 * g; i < whole; i += 4 * RGROUPS) {
             const u32x4 k = *(const u32x4*)(keys + i);
+            const uint32_t bound = mine + (i < here ? 1u : 0u);
 #pragma unroll
-            for (uint32_t e = 0; e < 4; ++e) below += k[e] < mine + (i + e < me ? 1u : 0u);
+            for (uint32_t e = 0; e < 4; ++e) below += k[e] < bound;
         }
+        // equal keys before the token among its neighbours
+        if (g == 0)
+            for (uint32_t i = here; i < me && i < n; ++i) below += keys[i] == mine;
         count[threadIdx.x] = below;
         __syncthreads();
         if (threadIdx.x < RTOK && me < n) {
@@ -96,8 +104,90 @@ __global__ __launch_bounds__(WORK) void rank_kernel(uint32_t M, uint32_t V, cons
     }
 }
 
-// Groups of WAYS sorted runs of `len` pairs into one.  The earlier run's pair
-// goes first among equal keys, so pairs stay in the order of m.
+// Groups of sorted runs into one.  The earlier run's pair goes first among equal
+// keys, so pairs stay in the order of m.
+//
+// Runs of RUN: a search is a chain of reads, so it runs in LDS, where a group's
+// keys fit (S = 1, WAYS runs), or the last of each S of them (S = 4, S WAYS
+// runs): then the S keys at the place found there are read and counted.
+// Searches count the keys below a bound, which for earlier runs is past the
+// pair's own key; SEARCHES of them run side by side.
+constexpr uint32_t SEARCHES = 8;
+template <uint32_t S>
+__global__ __launch_bounds__(WORK) void merge_runs_kernel(uint32_t M, const uint32_t* key_in, const uint32_t* order_in,
+                                                          uint32_t* key, uint32_t* order) {
+    constexpr uint32_t GROUP = RUN * WAYS * S, LEN = RUN / S;      // pairs of a group, keys of a run in LDS
+    __shared__ __attribute__((aligned(16))) uint32_t keys[LEN * WAYS * S];
+    const uint64_t first = (uint64_t)blockIdx.x * WORK, group = first / GROUP * GROUP;
+    const uint32_t n = (uint32_t)min((uint64_t)GROUP, M - group), runs = (n + RUN - 1) / RUN;
+    // whole runs, the last one filled up with keys above all others; LOADS in flight
+    constexpr uint32_t LOADS = RUN / 4 / WORK * 4;
+    for (uint32_t q0 = 0; q0 < runs * (RUN / 4); q0 += LOADS * WORK) {
+        u32x4 x[LOADS];
+#pragma unroll
+        for (uint32_t l = 0; l < LOADS; ++l) {
+            const uint32_t i = 4 * (q0 + l * WORK + threadIdx.x);
+            if (i + 4 <= n) x[l] = *(const u32x4*)(key_in + group + i);
+            else
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e) x[l][e] = i + e < n ? key_in[group + i + e] : ~0u;
+        }
+#pragma unroll
+        for (uint32_t l = 0; l < LOADS; ++l) {
+            const uint32_t q = q0 + l * WORK + threadIdx.x;
+            if (q >= runs * (RUN / 4)) continue;
+            if constexpr (S == 1) *(u32x4*)(keys + 4 * q) = x[l];
+            else keys[q] = x[l][3];
+        }
+    }
+    __syncthreads();
+    const uint32_t i = (uint32_t)(first - group) + threadIdx.x;
+    if (i >= n) return;
+    const uint32_t own = i / RUN, k = key_in[group + i], o = order_in[group + i];
+    uint32_t at = i % RUN;
+    for (uint32_t r0 = 0; r0 < runs; r0 += SEARCHES) {
+        uint32_t pos[SEARCHES];
+#pragma unroll
+        for (uint32_t r = 0; r < SEARCHES; ++r) pos[r] = 0;
+#pragma unroll
+        for (uint32_t step = LEN / 2; step; step /= 2)
+#pragma unroll
+            for (uint32_t r = 0; r < SEARCHES; ++r) {
+                const uint32_t* run = keys + min(r0 + r, runs - 1) * LEN;
+                pos[r] += run[pos[r] + step - 1] < k + (r0 + r < own ? 1u : 0u) ? step : 0u;
+            }
+#pragma unroll
+        for (uint32_t r = 0; r < SEARCHES; ++r) {
+            const uint32_t run = min(r0 + r, runs - 1), bound = k + (run < own ? 1u : 0u);
+            pos[r] += keys[run * LEN + pos[r]] < bound ? 1u : 0u;
+        }
+        if constexpr (S == 4) {
+            u32x4 x[SEARCHES];
+#pragma unroll
+            for (uint32_t r = 0; r < SEARCHES; ++r) {
+                const uint32_t j = 4 * (min(r0 + r, runs - 1) * LEN + min(pos[r], LEN - 1));
+                if (j + 4 <= n) x[r] = *(const u32x4*)(key_in + group + j);
+                else
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; ++e) x[r][e] = j + e < n ? key_in[group + j + e] : ~0u;
+            }
+#pragma unroll
+            for (uint32_t r = 0; r < SEARCHES; ++r) {
+                const uint32_t bound = k + (r0 + r < own ? 1u : 0u);
+                uint32_t c = 0;
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e) c += x[r][e] < bound ? 1u : 0u;
+                pos[r] = 4 * pos[r] + (pos[r] < LEN ? c : 0u);
+            }
+        }
+#pragma unroll
+        for (uint32_t r = 0; r < SEARCHES; ++r) at += r0 + r < runs && r0 + r != own ? pos[r] : 0u;
+    }
+    key[group + at] = k;
+    order[group + at] = o;
+}
+
+// Runs of `len`, WAYS at a time, searched in memory
 __global__ __launch_bounds__(WORK) void merge_kernel(uint32_t M, uint64_t len, uint32_t steps, const uint32_t* key_in,
                                                      const uint32_t* order_in, uint32_t* key, uint32_t* order) {
     const uint64_t i = (uint64_t)blockIdx.x * WORK + threadIdx.x;
@@ -131,29 +221,185 @@ __global__ __launch_bounds__(WORK) void merge_kernel(uint32_t M, uint64_t len, u
     order[group + at] = order_in[i];
 }
 
-// dw = beta * dw on the rows that no token has
-template <typename W>
-__global__ __launch_bounds__(WORK) void scale_others_kernel(uint32_t M, uint32_t V, uint32_t N, const uint32_t* key,
-                                                            W* dw, int64_t lddw, float beta) {
-    constexpr int VEC = Elem<W>::VEC;
-    for (uint64_t v = blockIdx.x; v < V; v += gridDim.x) {
-        uint32_t lo = 0, hi = M;
-        while (lo < hi) {
-            const uint32_t mid = lo + (hi - lo) / 2;
-            if (key[mid] < v) lo = mid + 1;
-            else hi = mid;
-        }
-        if (lo < M && key[lo] == v) continue;
-        W* row = dw + (int64_t)v * lddw;
-        for (int64_t c = (int64_t)threadIdx.x * VEC; c < N; c += (int64_t)WORK * VEC) {
-            float x[VEC];
-            unpack<W>(ld_chunk(row, c, N), x);
+// dw's columns c .. of a row: the sum of its rows of dy, scaled, and what was
+// there
+template <int VEC, typename W>
+__device__ __forceinline__ void put(W* row, int64_t c, int64_t N, float scale, float beta, const float* acc) {
+    constexpr int WV = Elem<W>::VEC;
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) x[i] *= beta;
-            st_chunk(row, c, N, pack<W>(x));
+    for (int q = 0; q < VEC; q += WV) {
+        if (c + q >= N) break;
+        float x[WV];
+        if (beta != 0.0f) {
+            unpack<W>(ld_chunk(row, c + q, N), x);
+#pragma unroll
+            for (int i = 0; i < WV; ++i) x[i] = beta * x[i] + scale * acc[q + i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < WV; ++i) x[i] = scale * acc[q + i];
+        }
+        st_chunk(row, c + q, N, pack<W>(x));
+    }
+}
+
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
+
+// ---- few tokens
+//
+// A workgroup: every ranges-th row of dw (frequent tokens often have
+// neighbouring ids), 64 x 16 bytes of dy's columns.  The ids of its rows are
+// listed in order of m.  A row with up to HEAVY is a wave's, one with more all
+// waves' on a part of the list each.  Rows without one are zeroed or scaled in
+// all of their columns, by the workgroups of the same rows in turn.
+constexpr uint32_t DIRECT = VKB_EMBED_DIRECT, DTHREADS = 512, DWAVES = DTHREADS / 64, DSTEPS = DIRECT / DTHREADS;
+constexpr uint32_t DROWS = 4096, HEAVY = 8, DBATCH = 8;   // DROWS: the most rows of a workgroup
+struct DirectParams {
+    uint32_t M, V, N, ranges;
+    const int64_t* ids;
+    int64_t pad;
+    const void* dy;
+    int64_t lddy;
+    void* dw;
+    int64_t lddw;
+    float scale, beta;
+};
+// acc += the rows of dy whose list entries a .. b - 1 are of row r
+template <typename T>
+__device__ __forceinline__ void add_listed(const DirectParams& p, const uint32_t* list, uint32_t a, uint32_t b, uint32_t r,
+                                           int64_t c, float* acc) {
+    constexpr int VEC = Elem<T>::VEC;
+    const uint32_t lane = threadIdx.x & 63;
+    for (uint32_t i = a; i < b; i += 64) {
+        const uint32_t e = i + lane < b ? list[i + lane] : ~0u;
+        uint64_t mask = __ballot(e / DIRECT == r);
+        while (mask) {
+            u32x4 x[DBATCH];
+            uint32_t n = 0;
+#pragma unroll
+            for (uint32_t k = 0; k < DBATCH; ++k) {
+                if (!mask) continue;
+                const int at = __builtin_ctzll(mask);
+                mask &= mask - 1;
+                const uint32_t m = (uint32_t)__builtin_amdgcn_readlane((int)e, at) % DIRECT;
+                x[k] = ld_chunk((const T*)p.dy + (int64_t)m * p.lddy, c, p.N);
+                ++n;
+            }
+#pragma unroll
+            for (uint32_t k = 0; k < DBATCH; ++k) {
+                if (k >= n) continue;
+                float f[VEC];
+                unpack<T>(x[k], f);
+#pragma unroll
+                for (int q = 0; q < VEC; ++q) acc[q] += f[q];
+            }
         }
     }
 }
+template <typename T, typename W>
+__global__ __launch_bounds__(DTHREADS) void direct_kernel(DirectParams p) {
+    constexpr int VEC = Elem<T>::VEC, WV = Elem<W>::VEC, COLS = 64 * VEC;
+    __shared__ uint32_t list[DIRECT];                    // the workgroup's row times DIRECT, and m
+    __shared__ uint32_t met[DROWS / 32], heavy[DROWS / 32], counts[DWAVES];
+    __shared__ float sums[DWAVES - 1][64][VEC + 1];
+    const uint32_t lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+    const uint32_t r0 = blockIdx.x, rows = (p.V - r0 + p.ranges - 1) / p.ranges;
+    const int64_t c = (int64_t)blockIdx.y * COLS + lane * VEC;
+    for (uint32_t i = threadIdx.x; i < (rows + 31) / 32; i += DTHREADS) met[i] = heavy[i] = 0;
+    // a wave's ids are consecutive: DSTEPS times 64 of them
+    const uint32_t first = wave * (DSTEPS * 64) + lane;
+    uint32_t at[DSTEPS];
+#pragma unroll
+    for (uint32_t s = 0; s < DSTEPS; ++s) {
+        const uint32_t m = first + s * 64;
+        const int64_t id = m < p.M ? p.ids[m] : -1;
+        const uint32_t v = id != p.pad && id >= 0 && id < p.V ? (uint32_t)id : p.V, r = v / p.ranges;
+        at[s] = v < p.V && v - r * p.ranges == r0 ? r : ~0u;
+    }
+    uint32_t n = 0;
+#pragma unroll
+    for (uint32_t s = 0; s < DSTEPS; ++s) n += (uint32_t)__popcll(__ballot(at[s] != ~0u));
+    if (lane == 0) counts[wave] = n;
+    __syncthreads();
+    uint32_t total = 0, base = 0;
+    for (uint32_t w = 0; w < DWAVES; ++w) {
+        if (w == wave) base = total;
+        total += counts[w];
+    }
+#pragma unroll
+    for (uint32_t s = 0; s < DSTEPS; ++s) {
+        const uint64_t mask = __ballot(at[s] != ~0u);
+        if (at[s] != ~0u) {
+            list[base + __popcll(mask & ((1ull << lane) - 1))] = at[s] * DIRECT + first + s * 64;
+            atomicOr(&met[at[s] / 32], 1u << at[s] % 32);
+        }
+        base += (uint32_t)__popcll(mask);
+    }
+    __syncthreads();
+    total = uniform(total);
+    W* dw = (W*)p.dw + (int64_t)r0 * p.lddw;
+    const int64_t step = (int64_t)p.ranges * p.lddw;
+    if (p.beta != 1.0f) {
+        // as many waves to a row as it has 64 chunks
+        const uint32_t per = min(DWAVES, (p.N + 64 * WV - 1) / (64 * WV)), at_once = DWAVES / per;
+        const uint32_t mine = wave / per < at_once ? wave / per + blockIdx.y * at_once : rows;
+        for (uint32_t r = mine; r < rows; r += gridDim.y * at_once) {
+            if (uniform(met[r / 32]) >> r % 32 & 1) continue;
+            W* row = dw + r * step;
+            for (int64_t k = (int64_t)(wave % per * 64 + lane) * WV; k < p.N; k += per * 64 * WV) {
+                u32x4 v = {0u, 0u, 0u, 0u};
+                if (p.beta != 0.0f) {
+                    float x[WV];
+                    unpack<W>(ld_chunk(row, k, p.N), x);
+#pragma unroll
+                    for (int e = 0; e < WV; ++e) x[e] *= p.beta;
+                    v = pack<W>(x);
+                }
+                st_chunk(row, k, p.N, v);
+            }
+        }
+    }
+    float acc[VEC];
+    auto clear = [&] {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) acc[i] = 0.0f;
+    };
+    bool any = false;
+    for (uint32_t r = wave; r < rows; r += DWAVES) {
+        if (!(uniform(met[r / 32]) >> r % 32 & 1)) continue;
+        uint32_t of = 0;
+        for (uint32_t i = 0; i < total; i += 64)
+            of += (uint32_t)__popcll(__ballot(i + lane < total && list[i + lane] / DIRECT == r));
+        if (of > HEAVY) {
+            if (lane == 0) atomicOr(&heavy[r / 32], 1u << r % 32);
+            any = true;
+            continue;
+        }
+        clear();
+        add_listed<T>(p, list, 0, total, r, c, acc);
+        put<VEC>(dw + r * step, c, p.N, p.scale, p.beta, acc);
+    }
+    if (!__syncthreads_or(any)) return;
+    const uint32_t each = (total + DWAVES - 1) / DWAVES, a = min(wave * each, total), b = min(a + each, total);
+    for (uint32_t r = 0; r < rows; ++r) {
+        if (!(uniform(heavy[r / 32]) >> r % 32 & 1)) continue;
+        clear();
+        add_listed<T>(p, list, a, b, r, c, acc);
+        if (wave) {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) sums[wave - 1][lane][i] = acc[i];
+        }
+        __syncthreads();
+        if (wave == 0) {
+            for (uint32_t w = 0; w < DWAVES - 1; ++w)
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) acc[i] += sums[w][lane][i];
+            put<VEC>(dw + r * step, c, p.N, p.scale, p.beta, acc);
+        }
+        __syncthreads();
+    }
+}
+
+// ---- sorted tokens
 
 struct SumParams {
     uint32_t M, V, N, chunk, chunks, blocks;    // blocks: of columns
@@ -166,52 +412,30 @@ struct SumParams {
     float* part;             // chunks x 2 x N: what began before a chunk, what goes on after it
 };
 
-// dw's columns c .. of a token: its sum, scaled, and what was there
-template <typename T, typename W>
-__device__ __forceinline__ void put(const SumParams& p, uint32_t v, int64_t c, const float* acc) {
-    constexpr int VEC = Elem<T>::VEC, WV = Elem<W>::VEC;
-    W* row = (W*)p.dw + (int64_t)v * p.lddw;
-#pragma unroll
-    for (int q = 0; q < VEC; q += WV) {
-        if (c + q >= p.N) break;
-        float x[WV];
-        if (p.beta != 0.0f) {
-            unpack<W>(ld_chunk(row, c + q, p.N), x);
-#pragma unroll
-            for (int i = 0; i < WV; ++i) x[i] = p.beta * x[i] + p.scale * acc[q + i];
-        } else {
-#pragma unroll
-            for (int i = 0; i < WV; ++i) x[i] = p.scale * acc[q + i];
-        }
-        st_chunk(row, c + q, p.N, pack<W>(x));
-    }
-}
-
-__device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
-
-// A wave: one chunk, 64 x 16 bytes of its rows' columns, SROWS rows in flight.
+// A wave: one chunk, 64 x 16 bytes of its rows' columns.  SROWS rows are in
+// flight while the SROWS before them are added up.
 constexpr uint32_t SROWS = 8;
 template <typename T, typename W>
-__global__ __launch_bounds__(WORK) void sum_kernel(SumParams p) {
+__device__ __forceinline__ void sum_unit(const SumParams& p, uint64_t unit) {
     constexpr int VEC = Elem<T>::VEC;
-    const uint64_t unit = (uint64_t)blockIdx.x * (WORK / 64) + uniform(threadIdx.x >> 6);
+    const uint32_t lane = threadIdx.x & 63;
     const uint32_t chunk = (uint32_t)(unit / p.blocks), block = (uint32_t)(unit % p.blocks);
     if (chunk >= p.chunks) return;
-    const int64_t c = ((int64_t)block * 64 + (threadIdx.x & 63)) * VEC;
+    const int64_t c = ((int64_t)block * 64 + lane) * VEC;
+    const bool whole = (int64_t)(block + 1) * 64 * VEC <= p.N;
     const uint32_t p0 = chunk * p.chunk, p1 = p0 + min(p.chunk, p.M - p0);
-    const uint32_t before = p0 ? uniform(p.key[p0 - 1]) : ~0u, after = p1 < p.M ? uniform(p.key[p1]) : ~0u;
     float acc[VEC];
-    uint32_t now = uniform(p.key[p0]);
-    bool began = now == before;
+    uint32_t now = ~0u;              // the token
+    bool began = false;              // ... before this chunk
     auto clear = [&] {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) acc[i] = 0.0f;
     };
-    // the token `now` ends here, or goes on in the next chunk
+    // the token ends here, or goes on in the next chunk
     auto done = [&](bool on) {
         if (c >= p.N) return;
         if (!began && !on) {
-            put<T, W>(p, now, c, acc);
+            put<VEC>((W*)p.dw + (int64_t)now * p.lddw, c, p.N, p.scale, p.beta, acc);
             return;
         }
         float* part = p.part + ((int64_t)chunk * 2 + (began ? 0 : 1)) * p.N;
@@ -220,21 +444,28 @@ __global__ __launch_bounds__(WORK) void sum_kernel(SumParams p) {
             if (c + q < p.N) st_chunk(part, c + q, p.N, pack<float>(acc + q));
     };
     clear();
-    // 64 pairs at a time in the lanes
-    for (uint32_t base = p0; base < p1 && now < p.V; base += 64) {
-        const uint32_t n = min(64u, p1 - base), mine = base + min(threadIdx.x & 63, n - 1);
-        const uint32_t keys = p.key[mine], rows = p.order[mine];
-        for (uint32_t i = 0; i < n; i += SROWS) {
-            u32x4 x[SROWS];
+    // VKB_EMBED_PAIRS pairs at a time in lanes 1 .. 62, the key before them and the one behind them beside
+    for (uint32_t base = p0; base < p1; base += VKB_EMBED_PAIRS) {
+        const uint32_t n = min(VKB_EMBED_PAIRS, p1 - base), at = min(base + lane, p.M) - (base + lane > 0 ? 1 : 0);
+        const uint32_t keys = p.key[at], rows = p.order[min(at, p1 - 1)];
+        auto key = [&](uint32_t i) { return (uint32_t)__builtin_amdgcn_readlane((int)keys, (int)(i + 1)); };
+        if (base == p0) {
+            now = key(0);
+            began = p0 && key(-1) == now;
+        }
+        auto load = [&](uint32_t i, u32x4* x) {
 #pragma unroll
             for (uint32_t r = 0; r < SROWS; ++r) {
-                const uint32_t m = (uint32_t)__builtin_amdgcn_readlane((int)rows, (int)min(i + r, n - 1));
-                x[r] = ld_chunk((const T*)p.dy + (int64_t)m * p.lddy, c, p.N);
+                const uint32_t m = (uint32_t)__builtin_amdgcn_readlane((int)rows, (int)min(i + r, n - 1) + 1);
+                const T* row = (const T*)p.dy + (int64_t)m * p.lddy;
+                x[r] = whole ? ld16_any(row + c) : ld_chunk(row, c, p.N);
             }
+        };
+        auto add = [&](uint32_t i, const u32x4* x) {
 #pragma unroll
             for (uint32_t r = 0; r < SROWS; ++r) {
                 if (i + r >= n || now >= p.V) continue;
-                const uint32_t k = (uint32_t)__builtin_amdgcn_readlane((int)keys, (int)(i + r));
+                const uint32_t k = key(i + r);
                 if (k != now) {
                     done(false);
                     clear();
@@ -247,9 +478,68 @@ __global__ __launch_bounds__(WORK) void sum_kernel(SumParams p) {
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) acc[e] += f[e];
             }
+        };
+        if (now >= p.V || key(0) >= p.V) {       // padding from here on
+            if (now < p.V) done(false);
+            return;
+        }
+        u32x4 x[SROWS], y[SROWS];
+        load(0, x);
+        for (uint32_t i = 0; i < n; i += 2 * SROWS) {
+            if (i + SROWS < n) load(i + SROWS, y);
+            add(i, x);
+            if (i + 2 * SROWS < n) load(i + 2 * SROWS, x);
+            if (i + SROWS < n) add(i + SROWS, y);
+        }
+        if (base + n == p1 && now < p.V) done(p1 < p.M && key(n) == now);
+    }
+}
+
+// FROWS rows of dw, those without a token zeroed or scaled: each wave searches
+// their ids among the sorted keys, a lane each, and takes its part of them.
+constexpr uint32_t FROWS = 64;
+template <typename W>
+__device__ __forceinline__ void fill_unit(const SumParams& p, uint64_t unit) {
+    constexpr int VEC = Elem<W>::VEC;
+    const uint32_t lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+    const uint64_t v0 = unit * FROWS;
+    const uint64_t v = v0 + lane;
+    uint32_t lo = 0, hi = v < p.V ? p.M : 0;
+    while (__any(lo < hi)) {
+        const uint32_t mid = lo + (hi - lo) / 2;
+        const bool less = lo < hi && p.key[mid] < v;
+        if (less) lo = mid + 1;
+        else if (lo < hi) hi = mid;
+    }
+    const bool none = v < p.V && !(lo < p.M && p.key[lo] == v);
+    const uint64_t mask = __ballot(none);
+    // as many waves to a row as it has 64 chunks
+    const uint32_t per = min(WORK / 64, (p.N + 64 * VEC - 1) / (64 * VEC)), at_once = WORK / 64 / per;
+    for (uint32_t r = wave / per; r < FROWS && wave / per < at_once; r += at_once) {
+        if (!(mask >> r & 1)) continue;
+        W* row = (W*)p.dw + (int64_t)(v0 + r) * p.lddw;
+        for (int64_t k = (int64_t)(wave % per * 64 + lane) * VEC; k < p.N; k += per * 64 * VEC) {
+            u32x4 x = {0u, 0u, 0u, 0u};
+            if (p.beta != 0.0f) {
+                float f[VEC];
+                unpack<W>(ld_chunk(row, k, p.N), f);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) f[i] *= p.beta;
+                x = pack<W>(f);
+            }
+            st_chunk(row, k, p.N, x);
         }
     }
-    if (now < p.V) done(now == after);
+}
+
+// The chunks and the rows without tokens in one launch, spread over one
+// another: both are bound by memory, the one by latency too.
+template <typename T, typename W>
+__global__ __launch_bounds__(WORK) void sum_kernel(SumParams p, uint32_t sums, uint32_t fills) {
+    const uint64_t b = blockIdx.x, all = (uint64_t)sums + fills;
+    const uint64_t s = b * sums / all, next = (b + 1) * sums / all;    // the s-th of the sums, where next is past s
+    if (next > s) sum_unit<T, W>(p, s * (WORK / 64) + uniform(threadIdx.x >> 6));
+    else fill_unit<W>(p, b - s);
 }
 
 // A token that begins in a chunk and goes on: that chunk's part and those of
@@ -307,7 +597,7 @@ __global__ __launch_bounds__(WORK) void join_kernel(SumParams p) {
     for (int w = 0; w < (int)WORK / 64 - 1; ++w)
 #pragma unroll
         for (int i = 0; i < VEC; ++i) acc[i] += sh[w][lane][i];
-    put<T, W>(p, k, c, acc);
+    put<VEC>((W*)p.dw + (int64_t)k * p.lddw, c, p.N, p.scale, p.beta, acc);
 }
 
 // f(T{}, W{}) for a type and one that is it or fp32
@@ -336,17 +626,48 @@ extern "C" int vkb_launch_embedding(int type, int w_type, uint32_t M, uint32_t V
     return ok ? (int)hipGetLastError() : (int)hipErrorInvalidValue;
 }
 
-extern "C" int vkb_launch_embedding_rank(uint32_t M, uint32_t V, const int64_t* ids, int64_t pad, uint32_t* key,
-                                         uint32_t* order, int w_type, uint32_t N, void* dw, int64_t lddw,
-                                         void* stream) {
-    const uint32_t tiles = (uint32_t)(((uint64_t)M + RTOK - 1) / RTOK), ranks = tiles < 65536 ? tiles : 65536;
-    const bool ok = with_type(w_type, [&](auto t) {
-        using W = decltype(t);
-        const uint32_t fill = dw ? chunk_blocks(V, chunks_of<W>(N)) : 0;
-        hipLaunchKernelGGL((rank_kernel<W>), dim3(ranks + fill), dim3(WORK), 0, (hipStream_t)stream, M, V, ids, pad,
-                           key, order, ranks, N, (W*)dw, lddw);
+extern "C" int vkb_launch_embedding_direct(int type, int w_type, uint32_t M, uint32_t V, uint32_t N, const int64_t* ids,
+                                           int64_t pad, const void* dy, int64_t lddy, float scale, void* dw,
+                                           int64_t lddw, float beta, void* stream) {
+    if (M > DIRECT) return (int)hipErrorInvalidValue;
+    const uint32_t cols = 64 * (type == VKB_T_F32 ? 4 : 8), blocks = (N + cols - 1) / cols;
+    // one wave of workgroups, or one for each 128 KB of a large dw, whose rows
+    // without tokens most of the time goes into (us for 1024 / 1536 / 4096 workgroups:
+    // bf16 1024 x 32000 x 1024 17.8 / 16.9 / 23.6, 2048 x 128000 x 4096 295 / 268 / 221)
+    const uint64_t bytes = (uint64_t)V * N * (w_type == VKB_T_F32 ? 4 : 2) >> 17;
+    const uint64_t want = bytes < 1024 ? 1024 : bytes < 8192 ? bytes : 8192;
+    uint64_t rows = ((uint64_t)V * blocks + want - 1) / want;
+    if (rows > DROWS) rows = DROWS;
+    const uint64_t ranges = (V + rows - 1) / rows;
+    if (ranges > 0xffffffffull / DTHREADS || blocks > 65535) return (int)hipErrorInvalidValue;
+    const DirectParams p{M, V, N, (uint32_t)ranges, ids, pad, dy, lddy, dw, lddw, scale, beta};
+    const bool ok = with_types(type, w_type, [&](auto t, auto o) {
+        using T = decltype(t);
+        using W = decltype(o);
+        hipLaunchKernelGGL((direct_kernel<T, W>), dim3((uint32_t)ranges, blocks), dim3(DTHREADS), 0,
+                           (hipStream_t)stream, p);
     });
     return ok ? (int)hipGetLastError() : (int)hipErrorInvalidValue;
+}
+
+extern "C" int vkb_launch_embedding_rank(uint32_t M, uint32_t V, const int64_t* ids, int64_t pad, uint32_t* key,
+                                         uint32_t* order, void* stream) {
+    const uint32_t tiles = (uint32_t)(((uint64_t)M + RTOK - 1) / RTOK);
+    hipLaunchKernelGGL(rank_kernel, dim3(tiles < 65536 ? tiles : 65536), dim3(WORK), 0, (hipStream_t)stream, M, V, ids,
+                       pad, key, order);
+    return (int)hipGetLastError();
+}
+
+extern "C" int vkb_launch_embedding_merge_runs(uint32_t M, const uint32_t* key_in, const uint32_t* order_in, uint32_t* key,
+                                               uint32_t* order, void* stream) {
+    const uint32_t blocks = (uint32_t)(((uint64_t)M + WORK - 1) / WORK);
+    if (M <= RUN * WAYS)
+        hipLaunchKernelGGL((merge_runs_kernel<1>), dim3(blocks), dim3(WORK), 0, (hipStream_t)stream, M, key_in, order_in,
+                           key, order);
+    else
+        hipLaunchKernelGGL((merge_runs_kernel<4>), dim3(blocks), dim3(WORK), 0, (hipStream_t)stream, M, key_in, order_in,
+                           key, order);
+    return (int)hipGetLastError();
 }
 
 extern "C" int vkb_launch_embedding_merge(uint32_t M, uint64_t len, const uint32_t* key_in, const uint32_t* order_in,
@@ -359,28 +680,19 @@ extern "C" int vkb_launch_embedding_merge(uint32_t M, uint64_t len, const uint32
     return (int)hipGetLastError();
 }
 
-extern "C" int vkb_launch_embedding_scale(int w_type, uint32_t M, uint32_t V, uint32_t N, const uint32_t* key, void* dw,
-                                          int64_t lddw, float beta, void* stream) {
-    const bool ok = with_type(w_type, [&](auto t) {
-        using W = decltype(t);
-        hipLaunchKernelGGL((scale_others_kernel<W>), dim3(V < 8192 ? V : 8192), dim3(WORK), 0, (hipStream_t)stream,
-                           M, V, N, key, (W*)dw, lddw, beta);
-    });
-    return ok ? (int)hipGetLastError() : (int)hipErrorInvalidValue;
-}
-
 extern "C" int vkb_launch_embedding_sums(int type, int w_type, const vkb_embedding_sums* a, void* stream) {
     const uint32_t cols = 64 * (type == VKB_T_F32 ? 4 : 8);
     SumParams p{a->M, a->V, a->N, a->chunk, a->chunks, (a->N + cols - 1) / cols, a->key, a->order, a->dy, a->lddy,
                 a->dw, a->lddw, a->scale, a->beta, a->part};
-    const uint64_t units = (uint64_t)p.chunks * p.blocks;
-    if (units > 0xffffffffull / WORK) return (int)hipErrorInvalidValue;
+    const uint64_t sums = ((uint64_t)p.chunks * p.blocks + WORK / 64 - 1) / (WORK / 64);
+    const uint64_t fills = p.beta == 1.0f ? 0 : ((uint64_t)p.V + FROWS - 1) / FROWS;
+    if (sums + fills > 0xffffffffull / WORK) return (int)hipErrorInvalidValue;
     int rc = (int)hipErrorInvalidValue;
     with_types(type, w_type, [&](auto t, auto o) {
         using T = decltype(t);
         using W = decltype(o);
-        hipLaunchKernelGGL((sum_kernel<T, W>), dim3((uint32_t)((units + 3) / 4)), dim3(WORK), 0, (hipStream_t)stream,
-                           p);
+        hipLaunchKernelGGL((sum_kernel<T, W>), dim3((uint32_t)(sums + fills)), dim3(WORK), 0, (hipStream_t)stream, p,
+                           (uint32_t)sums, (uint32_t)fills);
         rc = (int)hipGetLastError();
         if (rc != 0 || p.chunks == 1) return;
         hipLaunchKernelGGL((join_kernel<T, W>), dim3(p.blocks, p.chunks - 1), dim3(WORK), 0, (hipStream_t)stream, p);

@@ -1004,11 +1004,21 @@ vkblas_status_t vkblas_embedding_backward_async(vkblas_dtype_t type, uint32_t M,
     if (M == 0) return empty_gradient(&c, dw_type, V, N, dw, lddw, beta);
     if (!ids || !dy) return VKBLAS_ERR_PARAM;
     if (vkb_engine_trace()) fprintf(stderr, "[vkblas] embedding_backward type=%d M=%u V=%u N=%u\n", (int)type, M, V, N);
-    /* chunks of 8 pairs, or as many as VKB_EMBED_CHUNKS have */
+    if (M <= VKB_EMBED_DIRECT && (uint64_t)N <= 65535u * 256u) {
+        if (room(&c) != VKBLAS_OK) return c.st;
+        step(&c, vkb_launch_embedding_direct(type, dw_type, M, V, N, ids, pad_id, dy, lddy, scale, dw, lddw, beta, stream),
+             1);
+        return op_end(&c, VKBLAS_KERNEL_EMBED);
+    }
+    /* chunks of 8 pairs, or as many as leave 4096 waves: a token that ends in
+     * another chunk than it began in goes by the workspace */
     vkb_embedding_sums a = {.M = M, .V = V, .N = N, .dy = dy, .lddy = lddy, .dw = dw, .lddw = lddw, .scale = scale,
                             .beta = beta};
-    a.chunk = (uint32_t)(((uint64_t)M + VKB_EMBED_CHUNKS - 1) / VKB_EMBED_CHUNKS);
-    if (a.chunk < 8) a.chunk = 8;
+    const uint32_t cols = type == VKBLAS_DT_F32 ? 256 : 512;
+    uint64_t chunk = (uint64_t)M * ((N + cols - 1) / cols) / 4096;
+    if (chunk * VKB_EMBED_CHUNKS < M) chunk = ((uint64_t)M + VKB_EMBED_CHUNKS - 1) / VKB_EMBED_CHUNKS;
+    if (chunk > M) chunk = M;
+    a.chunk = chunk < 8 ? 8 : chunk <= VKB_EMBED_PAIRS ? (uint32_t)chunk : (uint32_t)round_up(chunk, VKB_EMBED_PAIRS);
     a.chunks = (uint32_t)(((uint64_t)M + a.chunk - 1) / a.chunk);
     const int merges = M > VKB_EMBED_RUN;
     const size_t o_k = buf(&c, (uint64_t)M * 4), o_o = buf(&c, (uint64_t)M * 4);
@@ -1016,18 +1026,18 @@ vkblas_status_t vkblas_embedding_backward_async(vkblas_dtype_t type, uint32_t M,
     const size_t o_p = a.chunks > 1 ? buf(&c, (uint64_t)a.chunks * 2 * N * sizeof(float)) : 0;
     if (room(&c) != VKBLAS_OK) return c.st;
     uint32_t *key = at(&c, o_k), *order = at(&c, o_o), *key2 = at(&c, o_k2), *order2 = at(&c, o_o2);
-    int ok = step(&c, vkb_launch_embedding_rank(M, V, ids, pad_id, key, order, dw_type, N,
-                                                beta == 0.0f ? dw : NULL, lddw, stream), beta == 0.0f);
-    for (uint64_t len = VKB_EMBED_RUN; ok && len < M; len *= VKB_EMBED_WAYS) {
-        ok = step(&c, vkb_launch_embedding_merge(M, len, key, order, key2, order2, stream), 0);
+    int ok = step(&c, vkb_launch_embedding_rank(M, V, ids, pad_id, key, order, stream), 0);
+    for (uint64_t len = VKB_EMBED_RUN; ok && len < M;
+         len = len == VKB_EMBED_RUN ? vkb_embedding_group(M) : len * VKB_EMBED_WAYS) {
+        ok = len == VKB_EMBED_RUN
+                 ? step(&c, vkb_launch_embedding_merge_runs(M, key, order, key2, order2, stream), 0)
+                 : step(&c, vkb_launch_embedding_merge(M, len, key, order, key2, order2, stream), 0);
         uint32_t *k = key, *o = order;
         key = key2;
         order = order2;
         key2 = k;
         order2 = o;
     }
-    if (ok && beta != 0.0f && beta != 1.0f)
-        ok = step(&c, vkb_launch_embedding_scale(dw_type, M, V, N, key, dw, lddw, beta, stream), 1);
     a.key = key;
     a.order = order;
     a.part = a.chunks > 1 ? (float*)at(&c, o_p) : NULL;
