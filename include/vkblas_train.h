@@ -137,7 +137,7 @@ typedef enum {
  * Needs a workspace for more than VKBLAS_POLICY_SMALL tokens (B * T, a sequence's
  * rounded up to 256).
  */
-#define VKBLAS_POLICY_SMALL 16384
+#define VKBLAS_POLICY_SMALL 4096
 vkblas_status_t vkblas_policy_loss_async(
     vkblas_reduce_t reduce, uint32_t B, uint32_t T,
     const float* logp, uint32_t ldp,

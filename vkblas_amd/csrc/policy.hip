@@ -47,15 +47,14 @@ __device__ __forceinline__ float kl_slope(float d) {
 }
 
 struct Token {
-    float r, adv, d;         // ratio, advantage, ref - logp
+    float r, d;              // ratio, ref - logp
     int side;                // 0: r A is taken, -1: the lower bound's, 1: the upper one's
 };
 // A NaN anywhere takes r A, which it reaches.
 __device__ __forceinline__ Token token(const vkb_policy& p, float logp, float old, float ref, float adv) {
     const double diff = (double)logp - (double)old;
     Token t;
-    t.r = fast_exp((float)diff);
-    t.adv = adv;
+    t.r = fast_exp(logp - old);
     t.d = ref - logp;
     t.side = adv > 0.0f && diff > p.high ? 1 : adv < 0.0f && diff < p.low ? -1 : 0;
     return t;
@@ -83,14 +82,19 @@ __device__ __forceinline__ uint32_t counted(const vkb_policy& p, int64_t b, int6
 struct Four {
     float logp[4], old[4], ref[4], adv[4];
 };
+// WHOLE: all four are of the sequence
+template <bool WHOLE>
 __device__ __forceinline__ void load4(const vkb_policy& p, int64_t b, int64_t t, Four& f) {
-    unpack<float>(ld_chunk(p.logp + b * p.ldp, t, p.T), f.logp);
-    unpack<float>(ld_chunk(p.old + b * p.ldo, t, p.T), f.old);
-    if (p.ref) unpack<float>(ld_chunk(p.ref + b * p.ldr, t, p.T), f.ref);
+    auto get = [&](const float* row, float* x) {
+        unpack<float>(WHOLE ? ld16_any(row + t) : ld_chunk(row, t, p.T), x);
+    };
+    get(p.logp + b * p.ldp, f.logp);
+    get(p.old + b * p.ldo, f.old);
+    if (p.ref) get(p.ref + b * p.ldr, f.ref);
     else
 #pragma unroll
         for (int e = 0; e < 4; ++e) f.ref[e] = f.logp[e];
-    if (p.adv_step) unpack<float>(ld_chunk(p.adv + b * p.ldadv, t, p.T), f.adv);
+    if (p.adv_step) get(p.adv + b * p.ldadv, f.adv);
     else
 #pragma unroll
         for (int e = 0; e < 4; ++e) f.adv[e] = p.adv[b * p.ldadv];
@@ -102,126 +106,175 @@ struct Sums {
     double v[NSUM];
 };
 __device__ __forceinline__ Sums zero_sums() { return Sums{{0.0, 0.0, 0.0, 0.0, 0.0}}; }
-// over groups of G lanes, in a fixed order
-template <typename S>
-__device__ __forceinline__ void lanes_sum(S& s, uint32_t G) {
-    for (uint32_t d = G / 2; d; d >>= 1)
-#pragma unroll
-        for (int i = 0; i < NSUM; ++i) s.v[i] += __shfl_xor(s.v[i], (int)d);
+
+// A wave's sum in a fixed order, in every lane: the steps of wave_reduce, on
+// both halves of a double
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_add(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xf, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, ROWS, 0xf, false);
+    return v + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double wave_sum(double v) {
+    v = dpp_add<0x111, 0xf>(v);
+    v = dpp_add<0x112, 0xf>(v);
+    v = dpp_add<0x114, 0xf>(v);
+    v = dpp_add<0x118, 0xf>(v);
+    v = dpp_add<0x142, 0xa>(v);
+    v = dpp_add<0x143, 0xc>(v);
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, 63);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), 63);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 
-// A wave's sums over the tokens t0 .. t1 - 1 of sequence b
-__device__ __forceinline__ Sums unit_sums(const vkb_policy& p, int64_t b, int64_t t0, int64_t t1, int lane) {
+// A wave's sums over the tokens of sequence b from t0 + 4 lane on, four every
+// `step`, below t1; the masks of AHEAD rounds are read before their arrays.
+// Tokens that do not count become ones whose terms are 0.  Four tokens are added
+// in fp32, as good as the terms themselves, and their sum in fp64.
+constexpr int AHEAD = 2;
+__device__ __forceinline__ Sums token_sums(const vkb_policy& p, int64_t b, int64_t t0, int64_t t1, int64_t step, int lane) {
     Sums s = zero_sums();
+    uint32_t tokens = 0, sides = 0;
     const bool by_kl = p.ref && p.kl != 0.0f;    // (0 * inf adds nothing)
-    for (int64_t t = t0 + 4 * lane; t < t1; t += 256) {
-        const uint32_t in = counted(p, b, t);
-        if (!in) continue;
-        Four f;
-        load4(p, b, t, f);
+    auto add = [&](uint32_t in, const Four& f) {
+        float loss = 0.0f, kls = 0.0f, rs = 0.0f;
+        tokens += __popc(in);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            if (!(in >> e & 1)) continue;
-            const Token k = token(p, f.logp[e], f.old[e], f.ref[e], f.adv[e]);
+            const bool is = in >> e & 1;
+            const float adv = is ? f.adv[e] : 0.0f;
+            const Token k = token(p, is ? f.logp[e] : 0.0f, is ? f.old[e] : 0.0f, is ? f.ref[e] : 0.0f, adv);
             const float kl = p.ref ? kl_term(k.d) : 0.0f;
             const float taken = k.side ? (k.side > 0 ? p.r_high : p.r_low) : k.r;
-            s.v[0] += (double)(by_kl ? p.kl * kl : 0.0f) - (double)taken * (double)k.adv;
-            s.v[1] += (double)kl;
-            s.v[2] += k.side ? 1.0 : 0.0;
-            s.v[3] += (double)k.r;
-            s.v[4] += 1.0;
+            loss += (by_kl ? p.kl * kl : 0.0f) - taken * adv;
+            kls += kl;
+            sides += k.side ? 1u : 0u;
+            rs += is ? k.r : 0.0f;
         }
-    }
-    lanes_sum(s, 64);
+        s.v[0] += (double)loss;
+        s.v[1] += (double)kls;
+        s.v[3] += (double)rs;
+    };
+    auto rounds = [&](auto whole, int64_t t) {
+        uint32_t in[AHEAD];
+        Four f[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) in[i] = t + step * i < t1 ? counted(p, b, t + step * i) : 0;
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+            if (in[i]) load4<decltype(whole)::value>(p, b, t + step * i, f[i]);
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+            if (in[i]) add(in[i], f[i]);
+    };
+    for (int64_t t = t0; t < t1; t += step * AHEAD)
+        if (t + step * (AHEAD - 1) + 256 <= t1) rounds(std::true_type{}, t + 4 * lane);
+        else rounds(std::false_type{}, t + 4 * lane);
+    s.v[2] = (double)sides;
+    s.v[4] = (double)tokens;
+#pragma unroll
+    for (int i = 0; i < NSUM; ++i) s.v[i] = wave_sum(s.v[i]);
     return s;
 }
 
-// The workgroup's 1024 threads over the units' sums: each sequence's by a group
-// of G threads, then all sequences' by the reduction's weights.
+// The workgroup over the units' sums (part: NSUM arrays of `count`): each
+// sequence's by a group of lanes, as many as B leaves of the threads, then all
+// sequences' by the reduction's weights.
 constexpr uint32_t FIN = 1024;
-template <typename GET>
-__device__ __forceinline__ void finish(uint32_t B, uint32_t units, int reduce, GET get, float* stats, float* norm,
-                                       double (*sh)[NSUM + 1]) {
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+struct Shared {
+    double waves[NSUM + 1][FIN / 64], tokens[FIN];       // tokens: of the first FIN sequences
+};
+__device__ __forceinline__ void finish(uint32_t B, uint32_t units, int reduce, const double* part, uint64_t count,
+                                       float* stats, float* norm, Shared& sh) {
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, threads = blockDim.x;
     uint32_t G = 1;
-    while (G < 64 && G < units) G *= 2;
+    while (G < 64 && G < units && 2 * G * B <= threads) G *= 2;
     const uint32_t at = threadIdx.x / G, in = threadIdx.x % G;
-    Sums total = zero_sums();
-    double some = 0.0;                        // sequences with tokens
-    auto sequence = [&](uint64_t b) {
-        Sums s = zero_sums();
-        if (b < B)
+    double total[NSUM + 1] = {0.0, 0.0, 0.0, 0.0, 0.0, 0.0};             // the last: sequences with tokens
+    for (uint64_t b = at; b < B; b += threads / G) {
+        double s[NSUM] = {0.0, 0.0, 0.0, 0.0, 0.0};
 #pragma unroll 4
-            for (uint32_t u = in; u < units; u += G) {
-                const Sums x = get(b * units + u);
+        for (uint32_t u = in; u < units; u += G)
 #pragma unroll
-                for (int i = 0; i < NSUM; ++i) s.v[i] += x.v[i];
-            }
-        lanes_sum(s, G);
-        return s;
-    };
-    for (uint64_t first = 0; first < B; first += FIN / G) {
-        const Sums s = sequence(first + at);
-        if (in || s.v[4] == 0.0) continue;
-        const double by = reduce == VKBLAS_REDUCE_SEQUENCES ? 1.0 / s.v[4] : 1.0;
+            for (int i = 0; i < NSUM; ++i) s[i] += part[i * count + b * units + u];
+        for (uint32_t d = G / 2; d; d >>= 1)
 #pragma unroll
-        for (int i = 0; i < NSUM; ++i) total.v[i] += s.v[i] * by;
-        some += 1.0;
+            for (int i = 0; i < NSUM; ++i) s[i] += __shfl_xor(s[i], (int)d);
+        if (in == 0 && b < FIN) sh.tokens[b] = s[4];
+        if (in || s[4] == 0.0) continue;
+        const double by = reduce == VKBLAS_REDUCE_SEQUENCES ? 1.0 / s[4] : 1.0;
+#pragma unroll
+        for (int i = 0; i < NSUM; ++i) total[i] += s[i] * by;
+        total[NSUM] += 1.0;
     }
-    lanes_sum(total, 64);
 #pragma unroll
-    for (int d = 32; d; d >>= 1) some += __shfl_xor(some, d);
-    if (lane == 0) {
-#pragma unroll
-        for (int i = 0; i < NSUM; ++i) sh[wave][i] = total.v[i];
-        sh[wave][NSUM] = some;
+    for (int i = 0; i <= NSUM; ++i) {
+        total[i] = wave_sum(total[i]);
+        if (lane == 0) sh.waves[i][wave] = total[i];
     }
     __syncthreads();
-    total = zero_sums();
-    some = 0.0;
-    for (uint32_t w = 0; w < FIN / 64; ++w) {
 #pragma unroll
-        for (int i = 0; i < NSUM; ++i) total.v[i] += sh[w][i];
-        some += sh[w][NSUM];
-    }
+    for (int i = 0; i <= NSUM; ++i) total[i] = wave_sum(lane < threads / 64 ? sh.waves[i][lane] : 0.0);
+    const double some = total[NSUM];
     const double weight = some == 0.0 ? 0.0 : reduce == VKBLAS_REDUCE_SUM ? 1.0
-                        : reduce == VKBLAS_REDUCE_TOKENS ? 1.0 / total.v[4] : 1.0 / some;
-    if (threadIdx.x < 4) stats[threadIdx.x] = (float)(total.v[threadIdx.x] * weight);
-    for (uint64_t first = 0; first < B; first += FIN / G) {
+                        : reduce == VKBLAS_REDUCE_TOKENS ? 1.0 / total[4] : 1.0 / some;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (threadIdx.x == (uint32_t)i) stats[i] = (float)(total[i] * weight);
+    for (uint64_t b = threadIdx.x; b < B; b += threads) {
         double n = 0.0;
-        if (first + at < B)
-            for (uint32_t u = in; u < units; u += G) n += get((first + at) * units + u).v[4];
-        for (uint32_t d = G / 2; d; d >>= 1) n += __shfl_xor(n, (int)d);
-        if (in == 0 && first + at < B)
-            norm[first + at] = (float)(n == 0.0 ? 0.0 : reduce == VKBLAS_REDUCE_SEQUENCES ? weight / n : weight);
+        if (b < FIN) n = sh.tokens[b];
+        else
+            for (uint32_t u = 0; u < units; ++u) n += part[4 * count + b * units + u];
+        norm[b] = (float)(n == 0.0 ? 0.0 : reduce == VKBLAS_REDUCE_SEQUENCES ? weight / n : weight);
     }
 }
 
-__global__ __launch_bounds__(WORK) void unit_kernel(vkb_policy p, Sums* part) {
-    const uint64_t unit = (uint64_t)blockIdx.x * (WORK / 64) + (threadIdx.x >> 6);
-    if (unit >= (uint64_t)p.B * p.units) return;
+// Units of a wave (sequences of up to 256 tokens) or of a workgroup's four
+template <bool SHORT>
+__global__ __launch_bounds__(WORK) void unit_kernel(vkb_policy p, double* part) {
+    constexpr uint32_t WAVES = WORK / 64;
+    __shared__ double sh[WAVES][NSUM];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint64_t unit = SHORT ? (uint64_t)blockIdx.x * WAVES + wave : blockIdx.x, count = (uint64_t)p.B * p.units;
+    if (unit >= count) return;
     const int64_t b = (int64_t)(unit / p.units), t0 = (int64_t)(unit % p.units) * p.unit;
-    const Sums s = unit_sums(p, b, t0, min(t0 + p.unit, (int64_t)p.T), threadIdx.x & 63);
-    if ((threadIdx.x & 63) == 0) part[unit] = s;
+    const int64_t t1 = min(t0 + p.unit, (int64_t)p.T);
+    Sums s = token_sums(p, b, SHORT ? t0 : t0 + 256 * wave, t1, SHORT ? 256 : 256 * WAVES, lane);
+    if (!SHORT) {
+#pragma unroll
+        for (int i = 0; i < NSUM; ++i)
+            if (lane == 0) sh[wave][i] = s.v[i];
+        __syncthreads();
+        if (wave) return;
+#pragma unroll
+        for (int i = 0; i < NSUM; ++i)
+            for (uint32_t w = 1; w < WAVES; ++w) s.v[i] += sh[w][i];
+    }
+#pragma unroll
+    for (int i = 0; i < NSUM; ++i)
+        if (lane == (uint32_t)i) part[i * count + unit] = s.v[i];
 }
-__global__ __launch_bounds__(FIN) void finish_kernel(vkb_policy p, int reduce, const Sums* part, float* stats,
+__global__ __launch_bounds__(FIN) void finish_kernel(vkb_policy p, int reduce, const double* part, float* stats,
                                                      float* norm) {
-    __shared__ double sh[FIN / 64][NSUM + 1];
-    finish(p.B, p.units, reduce, [&](uint64_t u) { return part[u]; }, stats, norm, sh);
+    __shared__ Shared sh;
+    finish(p.B, p.units, reduce, part, (uint64_t)p.B * p.units, stats, norm, sh);
 }
-// A small call: the units' sums in LDS
+// A small call: units of 256 tokens, their sums in LDS
 constexpr uint32_t SMALL = VKBLAS_POLICY_SMALL / 256;
 __global__ __launch_bounds__(FIN) void small_kernel(vkb_policy p, int reduce, float* stats, float* norm) {
-    __shared__ double sh[FIN / 64][NSUM + 1];
-    __shared__ Sums part[SMALL];
-    const uint32_t n = p.B * p.units;
-    for (uint32_t unit = threadIdx.x >> 6; unit < n; unit += FIN / 64) {
-        const int64_t t0 = (int64_t)(unit % p.units) * p.unit;
-        const Sums s = unit_sums(p, unit / p.units, t0, min(t0 + p.unit, (int64_t)p.T), threadIdx.x & 63);
-        if ((threadIdx.x & 63) == 0) part[unit] = s;
-    }
+    __shared__ Shared sh;
+    __shared__ double part[NSUM * SMALL];
+    const uint32_t units = (p.T + 255) / 256, n = p.B * units, unit = threadIdx.x >> 6;
+    const int64_t t0 = (int64_t)(unit % units) * 256;
+    const Sums s = token_sums(p, unit / units, t0, min(t0 + 256, (int64_t)p.T), 256, threadIdx.x & 63);
+#pragma unroll
+    for (int i = 0; i < NSUM; ++i)
+        if ((threadIdx.x & 63) == i) part[i * n + unit] = s.v[i];
     __syncthreads();
-    finish(p.B, p.units, reduce, [&](uint64_t u) { return part[u]; }, stats, norm, sh);
+    finish(p.B, units, reduce, part, n, stats, norm, sh);
 }
 
 __global__ __launch_bounds__(WORK) void grad_kernel(vkb_policy p, const float* norm, const float* dloss, float* dlogp,
@@ -234,12 +287,12 @@ __global__ __launch_bounds__(WORK) void grad_kernel(vkb_policy p, const float* n
         float g[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         if (in) {
             Four f;
-            load4(p, b, t, f);
+            load4<false>(p, b, t, f);
             const float by = dl * norm[b];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const Token x = token(p, f.logp[e], f.old[e], f.ref[e], f.adv[e]);
-                float s = x.side ? 0.0f : -x.adv * x.r;
+                float s = x.side ? 0.0f : -f.adv[e] * x.r;
                 if (by_kl) s += p.kl * kl_slope(x.d);
                 g[e] = in >> e & 1 ? by * s : 0.0f;
             }
@@ -253,31 +306,43 @@ __global__ __launch_bounds__(WORK) void grad_kernel(vkb_policy p, const float* n
 
 using namespace vkb;
 
-// Units of 256 tokens (a wave's four a lane) or as many as leave 16 waves a CU
+// A unit: a wave's 256 tokens, or 1024 times as many as leave 2048 workgroups
 extern "C" void vkb_policy_units(vkb_policy* p) {
-    uint64_t n = ((uint64_t)p->B * p->T + 4095) / 4096;
-    n = (n + 255) / 256 * 256;
-    if (n > p->T) n = p->T;
-    p->unit = (uint32_t)((n + 255) / 256 * 256);
-    p->units = (uint32_t)(((uint64_t)p->T + p->unit - 1) / p->unit);
+    if (p->T <= 256) {
+        p->unit = 256;
+        p->units = 1;
+        return;
+    }
+    const uint64_t n = ((uint64_t)p->B * p->T + 2047) / 2048;
+    const uint64_t unit = n < p->T ? (n + 1023) / 1024 * 1024 : ((uint64_t)p->T + 1023) / 1024 * 1024;
+    p->unit = (uint32_t)unit;
+    p->units = (uint32_t)(((uint64_t)p->T + unit - 1) / unit);
 }
-static bool small(const vkb_policy* p) { return (uint64_t)p->B * (((uint64_t)p->T + 255) / 256) <= SMALL; }
+// One wave each for up to 16 units of 256
+static uint64_t small_units(const vkb_policy* p) { return (uint64_t)p->B * (((uint64_t)p->T + 255) / 256); }
 extern "C" size_t vkb_policy_part_bytes(const vkb_policy* p) {
-    return small(p) ? 0 : (size_t)p->B * p->units * sizeof(Sums);
+    return small_units(p) <= SMALL ? 0 : (size_t)p->B * p->units * sizeof(Sums);   // as NSUM arrays
 }
 
 extern "C" int vkb_launch_policy(const vkb_policy* p, int reduce, void* part, float* stats, float* norm, void* stream) {
     if (!part) {
-        if (!small(p)) return (int)hipErrorInvalidValue;
-        hipLaunchKernelGGL(small_kernel, dim3(1), dim3(FIN), 0, (hipStream_t)stream, *p, reduce, stats, norm);
+        static_assert(SMALL <= FIN / 64, "a wave for each unit");
+        if (small_units(p) > SMALL) return (int)hipErrorInvalidValue;
+        hipLaunchKernelGGL(small_kernel, dim3(1), dim3(64 * (uint32_t)small_units(p)), 0, (hipStream_t)stream, *p, reduce,
+                           stats, norm);
         return (int)hipGetLastError();
     }
-    const uint64_t blocks = ((uint64_t)p->B * p->units + WORK / 64 - 1) / (WORK / 64);
+    const uint64_t count = (uint64_t)p->B * p->units, blocks = p->T <= 256 ? (count + WORK / 64 - 1) / (WORK / 64) : count;
     if (blocks > 0xffffffffull / WORK) return (int)hipErrorInvalidValue;
-    hipLaunchKernelGGL(unit_kernel, dim3((uint32_t)blocks), dim3(WORK), 0, (hipStream_t)stream, *p, (Sums*)part);
+    if (p->T <= 256)
+        hipLaunchKernelGGL((unit_kernel<true>), dim3((uint32_t)blocks), dim3(WORK), 0, (hipStream_t)stream, *p,
+                           (double*)part);
+    else
+        hipLaunchKernelGGL((unit_kernel<false>), dim3((uint32_t)blocks), dim3(WORK), 0, (hipStream_t)stream, *p,
+                           (double*)part);
     const int rc = (int)hipGetLastError();
     if (rc != 0) return rc;
-    hipLaunchKernelGGL(finish_kernel, dim3(1), dim3(FIN), 0, (hipStream_t)stream, *p, reduce, (const Sums*)part, stats,
+    hipLaunchKernelGGL(finish_kernel, dim3(1), dim3(FIN), 0, (hipStream_t)stream, *p, reduce, (const double*)part, stats,
                        norm);
     return (int)hipGetLastError();
 }

@@ -128,8 +128,8 @@ typedef struct vkb_embedding_sums {
 } vkb_embedding_sums;
 int vkb_launch_embedding_sums(int type, int w_type, const vkb_embedding_sums* a, void* stream);
 
-/* Policy loss (policy.hip) over `units` parts of a sequence each, `unit` tokens
- * long.  loss: sums to part (NULL: the call is small, one workgroup does it
+/* Policy loss (policy.hip) over `units` parts of each sequence, `unit` tokens
+ * long (vkb_policy_units).  loss: sums to part (NULL: the call is small, one workgroup does it
  * all), vkb_policy_part_bytes; then finish; grad: dlogp. */
 typedef struct vkb_policy {
     uint32_t B, T;
