@@ -17,22 +17,13 @@ namespace {
 
 constexpr uint32_t TOP = VKBLAS_DISTILL_TOP, WAVES = WORK / 64;
 
+constexpr int ABSENT = -1, BAD = -2, NONE = -3;
 struct Shared {
     float q[TOP];            // the teacher's logits over T, then its probabilities
-    int id[TOP];             // class, or ABSENT, or BAD
-    float part[WAVES];
+    __attribute__((aligned(16))) int id[TOP];      // class, or ABSENT, or BAD; NONE up to a whole quad
+    float high[WAVES], sum[WAVES];
+    uint32_t flags[WAVES];
 };
-constexpr int ABSENT = -1, BAD = -2;
-
-template <typename F>
-__device__ __forceinline__ float block_reduce(float v, float* sh, F join) {
-    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
-    __syncthreads();
-    float r = sh[0];
-    for (uint32_t i = 1; i < WAVES; ++i) r = join(r, sh[i]);
-    __syncthreads();
-    return r;
-}
 
 // A row's entries into LDS: classes, and t / T less the largest.  Returns the
 // log of their sum of exponentials.  counted: some entry is there and not of
@@ -40,41 +31,126 @@ __device__ __forceinline__ float block_reduce(float v, float* sh, F join) {
 template <typename TT>
 __device__ __forceinline__ float teacher(uint32_t n, uint32_t V, const int64_t* top, const TT* t, float inv_t,
                                          Shared& sh, bool& counted, bool& bad) {
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     float high = -INFINITY;
-    int any = 0, past = 0;
-    for (uint32_t j = threadIdx.x; j < n; j += WORK) {
-        const int64_t c = top[j];
+    bool any = false, past = false;
+    for (uint32_t j = threadIdx.x; j < (n + 3) / 4 * 4; j += WORK) {
+        const int64_t c = j < n ? top[j] : -1;
         const float v = c < 0 ? -INFINITY : (float)t[j] * inv_t;
-        sh.id[j] = c < 0 ? ABSENT : c < V ? (int)c : BAD;
-        sh.q[j] = v;
+        sh.id[j] = j >= n ? NONE : c < 0 ? ABSENT : c < V ? (int)c : BAD;
+        if (j < n) sh.q[j] = v;
         any |= !(v == -INFINITY);
         past |= c >= (int64_t)V;
         high = fmaxf(high, v);
     }
-    counted = __syncthreads_or(any) != 0;
-    bad = __syncthreads_or(past) != 0;
-    high = block_reduce(wave_max(high), sh.part, [](float a, float b) { return fmaxf(a, b); });
+    high = wave_max(high);
+    const uint32_t f = (__any(any) ? 1u : 0u) | (__any(past) ? 2u : 0u);
+    if (lane == 0) {
+        sh.high[wave] = high;
+        sh.flags[wave] = f;
+    }
+    __syncthreads();
+    uint32_t flags = 0;
+    for (uint32_t w = 0; w < WAVES; ++w) {
+        high = fmaxf(high, sh.high[w]);
+        flags |= sh.flags[w];
+    }
+    counted = flags & 1;
+    bad = flags & 2;
     if (high == -INFINITY) high = 0.0f;
     float s = 0.0f;
     for (uint32_t j = threadIdx.x; j < n; j += WORK) {
         sh.q[j] -= high;
         s += fast_exp(sh.q[j]);
     }
-    s = block_reduce(wave_sum(s), sh.part, [](float a, float b) { return a + b; });
+    s = wave_sum(s);
+    if (lane == 0) sh.sum[wave] = s;
+    __syncthreads();
+    s = 0.0f;
+    for (uint32_t w = 0; w < WAVES; ++w) s += sh.sum[w];
     return logf(s);
 }
 
-// One workgroup per row.  The waves take the entries DOTS at a time: one load of
-// x's chunk for DOTS of w's rows.
-constexpr uint32_t DOTS = 4;
+// A row's pair (top, s) as xent.hip's, of logits times inv_t = c2 / log2(e); the
+// threads' join: its log-sum-exp, in every thread
+struct Pair {
+    float top = -INFINITY, s = 0.0f;
+};
+__device__ __forceinline__ float finite_or_0(float x) { return __builtin_isinf(x) ? 0.0f : x; }
+__device__ __forceinline__ float block_lse(Pair p, float inv_t, float2* sh) {
+    const float c2 = inv_t * LOG2E;
+    float top = wave_max(p.top), off = finite_or_0(top);
+    float s = wave_sum(p.s * __builtin_amdgcn_exp2f((p.top - off) * c2));
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = float2{top, s};
+    __syncthreads();
+    for (uint32_t w = 0; w < WAVES; ++w) top = fmaxf(top, sh[w].x);
+    off = finite_or_0(top);
+    s = 0.0f;
+    for (uint32_t w = 0; w < WAVES; ++w) s += sh[w].y * __builtin_amdgcn_exp2f((sh[w].x - off) * c2);
+    return off * inv_t + logf(s);
+}
+// ... of S pairs of a row, `stride` apart
+__device__ __forceinline__ Pair join_parts(const float2* parts, uint64_t stride, uint32_t S, float c2) {
+    Pair p;
+    for (uint32_t i = threadIdx.x; i < S; i += 4 * WORK) {
+        float2 x[4];
+        float t = p.top;
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k)
+            x[k] = i + k * WORK < S ? parts[(i + k * WORK) * stride] : float2{-INFINITY, 0.0f};
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) t = fmaxf(t, x[k].x);
+        const float off = finite_or_0(t);
+        p.s *= __builtin_amdgcn_exp2f((p.top - off) * c2);
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) p.s += x[k].y * __builtin_amdgcn_exp2f((x[k].x - off) * c2);
+        p.top = t;
+    }
+    return p;
+}
+// ... of a row of V logits
+__device__ __forceinline__ Pair join_logits(const float* z, uint32_t V, float c2) {
+    Pair p;
+    for (int64_t c = 4 * threadIdx.x; c < V; c += 16 * WORK) {
+        float x[4][4], t = p.top;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int64_t at = c + 4 * k * WORK;
+            if (at + 4 <= V) unpack<float>(ld16_any(z + at), x[k]);
+            else
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[k][e] = at + e < V ? z[at + e] : -INFINITY;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) t = fmaxf(t, x[k][e]);
+        const float off = finite_or_0(t);
+        p.s *= __builtin_amdgcn_exp2f((p.top - off) * c2);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) p.s += __builtin_amdgcn_exp2f((x[k][e] - off) * c2);
+        p.top = t;
+    }
+    return p;
+}
+
+// One workgroup per row.  Its log-sum-exp comes from lse, from the parts that
+// tiles or slices left (then lse is written) or, with neither, from the logits.
+// The logits at the entries are read where the row is there, else computed, the
+// waves on DOTS entries at a time: one load of x's chunk for DOTS of w's rows.
+constexpr uint32_t DOTS = 8;
 template <typename T, typename TT>
 __global__ __launch_bounds__(WORK) void rows_kernel(uint32_t M, uint32_t V, uint32_t K, const T* x, int64_t ldx,
                                                     const T* w, int64_t ldw, uint32_t n, const int64_t* top,
                                                     int64_t ldtop, const TT* t, int64_t ldt, float temp, float inv_t,
-                                                    const float* lse, float* loss, float* z_top) {
+                                                    const float* logits, int64_t ldz, const float2* parts, uint32_t S,
+                                                    int have_lse, float* lse, float* loss, float* z_top) {
     constexpr int VEC = Elem<T>::VEC;
     __shared__ Shared sh;
-    __shared__ float z[TOP];
+    __shared__ float z[TOP], sums[WAVES];
+    __shared__ float2 pairs[WAVES];
     __shared__ uint32_t list[TOP], count;
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     for (uint64_t m = blockIdx.x; m < M; m += gridDim.x) {
@@ -92,7 +168,7 @@ __global__ __launch_bounds__(WORK) void rows_kernel(uint32_t M, uint32_t V, uint
             if (lane == 0) count = c;
         }
         __syncthreads();
-        const uint32_t there = count;
+        const uint32_t there = logits ? 0 : count;
         const T* xr = x + (int64_t)m * ldx;
         for (uint32_t g = wave * DOTS; g < there; g += WAVES * DOTS) {
             const T* row[DOTS];
@@ -102,7 +178,7 @@ __global__ __launch_bounds__(WORK) void rows_kernel(uint32_t M, uint32_t V, uint
                 row[e] = w + (int64_t)__builtin_amdgcn_readfirstlane(sh.id[list[min(g + e, there - 1)]]) * ldw;
                 acc[e] = 0.0f;
             }
-#pragma unroll 2
+#pragma unroll 1      // (two rounds of loads cost a wave per SIMD: 38 -> 51 us at 1000 rows of 200 entries, K = 1024)
             for (int64_t k = (int64_t)lane * VEC; k < K; k += 64 * VEC) {
                 float a[VEC];
                 unpack<T>(ld_chunk(xr, k, K), a);
@@ -120,18 +196,29 @@ __global__ __launch_bounds__(WORK) void rows_kernel(uint32_t M, uint32_t V, uint
                 if (lane == 0 && g + e < there) z[list[g + e]] = s;
             }
         }
+        float l;
+        if (have_lse) l = lse[m];
+        else
+            l = block_lse(S ? join_parts(parts + m, M, S, inv_t * LOG2E)
+                            : join_logits(logits + (int64_t)m * ldz, V, inv_t * LOG2E), inv_t, pairs);
+        if (!have_lse && threadIdx.x == 0) lse[m] = l;
         __syncthreads();
-        const float l = lse[m];
         float s = 0.0f;
         for (uint32_t j = threadIdx.x; j < n; j += WORK) {
             const int id = sh.id[j];
-            const float v = id == ABSENT ? 0.0f : id == BAD ? __builtin_nanf("") : z[j];
+            const float v = id == ABSENT ? 0.0f : id == BAD ? __builtin_nanf("")
+                          : logits ? logits[(int64_t)m * ldz + id] : z[j];
             z_top[(int64_t)m * n + j] = v;
             const float log_q = sh.q[j] - log_s, q = fast_exp(log_q);
             if (id != ABSENT && !(q == 0.0f)) s += q * (log_q - (v * inv_t - l));
         }
-        s = block_reduce(wave_sum(s), sh.part, [](float a, float b) { return a + b; });
-        if (threadIdx.x == 0) loss[m] = bad ? __builtin_nanf("") : counted ? temp * temp * s : 0.0f;
+        s = wave_sum(s);
+        if (lane == 0) sums[wave] = s;
+        __syncthreads();      // (the next row's entries are written past this)
+        if (threadIdx.x == 0) {
+            for (uint32_t i = 1; i < WAVES; ++i) s += sums[i];
+            loss[m] = bad ? __builtin_nanf("") : counted ? temp * temp * s : 0.0f;
+        }
     }
 }
 
@@ -149,26 +236,33 @@ __global__ __launch_bounds__(WORK) void prepare_kernel(uint32_t M, uint32_t V, u
     for (uint64_t m = blockIdx.x; m < M; m += gridDim.x) {
         bool counted, bad;
         const float log_s = teacher(n, V, top + (int64_t)m * ldtop, t + (int64_t)m * ldt, inv_t, sh, counted, bad);
-        uint32_t at = n;
-        __syncthreads();
+        int at = (int)n;
         for (uint32_t j = threadIdx.x; j < n; j += WORK) {
             sh.q[j] = sh.id[j] == ABSENT ? 0.0f : fast_exp(sh.q[j] - log_s);
-            if (sh.id[j] >= 0) at = min(at, j);
+            if (sh.id[j] >= 0) at = min(at, (int)j);
         }
-        for (int d = 32; d; d >>= 1) at = min(at, (uint32_t)__shfl_xor((int)at, d));
-        if ((threadIdx.x & 63) == 0) first[threadIdx.x >> 6] = (int)at;
+        for (int d = 32; d; d >>= 1) at = min(at, __shfl_xor(at, d));
+        if ((threadIdx.x & 63) == 0) first[threadIdx.x >> 6] = at;
         __syncthreads();
         for (uint32_t j = threadIdx.x; j < n; j += WORK) {
             const int id = sh.id[j];
-            float q = 0.0f;
-            if (id >= 0)
+            uint32_t same = 0;
+#pragma unroll 4
+            for (uint32_t i = 0; i < n; i += 4) {
+                const u32x4 c = *(const u32x4*)(sh.id + i);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) same += (int)c[e] == id ? 1u : 0u;
+            }
+            float q = sh.q[j];
+            if (same > 1 && id >= 0) {
+                q = 0.0f;
                 for (uint32_t i = 0; i < n; ++i) q += sh.id[i] == id ? sh.q[i] : 0.0f;
+            }
             q_top[(int64_t)m * n + j] = q;
         }
         if (threadIdx.x == 0) {
-            uint32_t f = n;
-            for (uint32_t i = 0; i < WAVES; ++i) f = min(f, (uint32_t)first[i]);
-            target[m] = bad ? (int64_t)V : counted && f < n ? (int64_t)sh.id[f] : ignore;
+            for (uint32_t i = 0; i < WAVES; ++i) at = min(at, first[i]);
+            target[m] = bad ? (int64_t)V : counted && at < (int)n ? (int64_t)sh.id[at] : ignore;
             dl[m] = temp * dloss[m];
         }
         __syncthreads();
@@ -201,15 +295,16 @@ using namespace vkb;
 static uint32_t row_blocks(uint32_t M) { return M < 65536 ? M : 65536; }
 
 extern "C" int vkb_launch_distill_rows(int type, int t_type, const vkb_distill* d, uint32_t K, const void* x,
-                                       int64_t ldx, const void* w, int64_t ldw, const float* lse, float* loss,
-                                       float* z_top, void* stream) {
+                                       int64_t ldx, const void* w, int64_t ldw, const vkb_distill_rows* r,
+                                       void* stream) {
     const bool ok = with_type(type, [&](auto e) {
         using T = decltype(e);
         auto launch = [&](auto f) {
             using TT = decltype(f);
             hipLaunchKernelGGL((rows_kernel<T, TT>), dim3(row_blocks(d->M)), dim3(WORK), 0, (hipStream_t)stream, d->M,
                                d->V, K, (const T*)x, ldx, (const T*)w, ldw, d->n, d->top, d->ldtop, (const TT*)d->t,
-                               d->ldt, d->temp, 1.0f / d->temp, lse, loss, z_top);
+                               d->ldt, d->temp, 1.0f / d->temp, r->z, r->ldz, (const float2*)r->parts, r->S, r->have_lse,
+                               r->lse, r->loss, r->z_top);
         };
         if (t_type == VKB_T_F32) launch(float{});
         else launch(e);

@@ -638,12 +638,34 @@ static uint32_t piece_columns(uint32_t M, uint32_t V, uint64_t bytes, uint64_t e
     return (uint32_t)(n < V ? n : V);
 }
 
-/* lse of each row's logits times inv_t, and its loss (target NULL: none), on the
- * call's workspace.  Returns the kernel for op_end(), VKBLAS_KERNEL_NONE where
- * nothing could begin. */
+/* A distillation's rows, from x and w and what row_statistics has of the logits. */
+typedef struct {
+    vkb_distill d;
+    vkblas_dtype_t t_type;
+    const void *x, *w;
+    uint32_t ldx, ldw;
+    vkb_distill_rows r;
+} teacher_rows;
+static int distill_rows(op_call* c, vkblas_dtype_t type, uint32_t K, teacher_rows* q, const float* z, uint32_t ldz,
+                        const float* parts, uint32_t S, int have_lse) {
+    q->r.z = z;
+    q->r.ldz = ldz;
+    q->r.parts = parts;
+    q->r.S = S;
+    q->r.have_lse = have_lse;
+    return step(c, vkb_launch_distill_rows(type, q->t_type, &q->d, K, q->x, q->ldx, q->w, q->ldw, &q->r, c->stream), 1);
+}
+/* A distillation's rows join their parts themselves up to this many, which saves
+ * the launch of the kernel that reads eight rows' at a time (us, with that kernel
+ * / without: f16 300 x 32003 x 1024 40.6 / 36.9). */
+#define JOIN_PARTS (1u << 18)
+
+/* lse of each row's logits times inv_t, and its loss (target NULL: none) or (q)
+ * that of a distillation, on the call's workspace.  Returns the kernel for
+ * op_end(), VKBLAS_KERNEL_NONE where nothing could begin. */
 static int row_statistics(op_call* c, vkblas_dtype_t type, uint32_t M, uint32_t V, uint32_t K, float inv_t,
                           const void* x, uint32_t ldx, const void* w, uint32_t ldw, const int64_t* target,
-                          int64_t ignore_index, float* loss, float* lse) {
+                          int64_t ignore_index, float* loss, float* lse, teacher_rows* q) {
     void* stream = c->stream;
     vkb_op_args a;
     operand ox = as_is(x, ldx, 1, M, K), ow = as_is(w, ldw, 1, V, K);
@@ -659,8 +681,11 @@ static int row_statistics(op_call* c, vkblas_dtype_t type, uint32_t M, uint32_t 
         bring(c, &jobs, &ow, w, ldw);
         if (brought(c, &jobs, type, NULL)) {
             bound(&a, &ox, &ow);
-            if (step(c, vkb_launch_xent_stats_op(&a, inv_t, target, parts, zt, stream), 0))
-                step(c, vkb_launch_xent_finish(M, V, S, inv_t, parts, zt, target, ignore_index, loss, lse, stream), 1);
+            const int join = q && (uint64_t)M * S <= JOIN_PARTS;
+            if (step(c, vkb_launch_xent_stats_op(&a, inv_t, target, parts, zt, stream), 0) &&
+                (join || step(c, vkb_launch_xent_finish(M, V, S, inv_t, parts, zt, target, ignore_index, loss, lse,
+                                                        stream), 1)) && q)
+                distill_rows(c, type, K, q, NULL, 0, parts, S, !join);
         }
         return VKBLAS_KERNEL_FUSED;
     }
@@ -692,12 +717,15 @@ static int row_statistics(op_call* c, vkblas_dtype_t type, uint32_t M, uint32_t 
         ok = (few ? step(c, vkb_launch_few_forward(type, &fw, 0, stream), 0)
                   : product(c, type, VKBLAS_DT_F32, VKBLAS_OP_N, VKBLAS_OP_T, M, cols, Kp, host_scalars(1.0f, 0.0f),
                             ox.p, ox.ld, (const char*)ow.p + v * ow.ld * type_size(type), ow.ld, z, ldz, 0)) &&
-             (rows ? step(c, vkb_launch_xent_rows(M, V, inv_t, z, ldz, target, ignore_index, loss, lse, stream), 1)
+             (rows && q ? distill_rows(c, type, K, q, z, ldz, NULL, 0, 0)
+              : rows ? step(c, vkb_launch_xent_rows(M, V, inv_t, z, ldz, target, ignore_index, loss, lse, stream), 1)
                    : step(c, vkb_launch_xent_stats(M, cols, (uint32_t)v, inv_t, z, ldz, target,
                                                     parts + (uint64_t)slice * M * 2, zt, stream), 0));
     }
-    if (ok && !rows)
-        step(c, vkb_launch_xent_finish(M, V, S, inv_t, parts, zt, target, ignore_index, loss, lse, stream), 1);
+    const int join = q && (uint64_t)M * S <= JOIN_PARTS;
+    if (ok && !rows && !join)
+        ok = step(c, vkb_launch_xent_finish(M, V, S, inv_t, parts, zt, target, ignore_index, loss, lse, stream), 1);
+    if (ok && !rows && q) distill_rows(c, type, K, q, n == V ? z : NULL, ldz, parts, S, !join);
     return VKBLAS_KERNEL_JOINED;
 }
 
@@ -712,7 +740,7 @@ vkblas_status_t vkblas_linear_xent_async(vkblas_dtype_t type, uint32_t M, uint32
     op_call c;
     op_begin(&c, "linear_xent", stream);
     if (vkb_engine_trace()) fprintf(stderr, "[vkblas] linear_xent type=%d M=%u V=%u K=%u\n", (int)type, M, V, K);
-    const int kernel = row_statistics(&c, type, M, V, K, 1.0f, x, ldx, w, ldw, target, ignore_index, loss, lse);
+    const int kernel = row_statistics(&c, type, M, V, K, 1.0f, x, ldx, w, ldw, target, ignore_index, loss, lse, NULL);
     return kernel == VKBLAS_KERNEL_NONE ? c.st : op_end(&c, kernel);
 }
 
@@ -942,13 +970,12 @@ vkblas_status_t vkblas_linear_distill_async(vkblas_dtype_t type, uint32_t M, uin
     op_begin(&c, "linear_distill", stream);
     if (vkb_engine_trace())
         fprintf(stderr, "[vkblas] linear_distill type=%d M=%u V=%u K=%u n_top=%u\n", (int)type, M, V, K, n_top);
-    const int kernel = row_statistics(&c, type, M, V, K, 1.0f / temperature, x, ldx, w, ldw, NULL, 0, NULL, lse);
-    if (kernel == VKBLAS_KERNEL_NONE) return c.st;
-    const vkb_distill q = {.M = M, .V = V, .n = n_top, .top = top, .ldtop = ldtop, .t = t, .ldt = ldt,
-                           .temp = temperature};
-    if (c.st == VKBLAS_OK)
-        step(&c, vkb_launch_distill_rows(type, t_type, &q, K, x, ldx, w, ldw, lse, loss, z_top, stream), 1);
-    return op_end(&c, kernel);
+    teacher_rows q = {.d = {.M = M, .V = V, .n = n_top, .top = top, .ldtop = ldtop, .t = t, .ldt = ldt,
+                            .temp = temperature},
+                      .t_type = t_type, .x = x, .w = w, .ldx = ldx, .ldw = ldw,
+                      .r = {.lse = lse, .loss = loss, .z_top = z_top}};
+    const int kernel = row_statistics(&c, type, M, V, K, 1.0f / temperature, x, ldx, w, ldw, NULL, 0, NULL, lse, &q);
+    return kernel == VKBLAS_KERNEL_NONE ? c.st : op_end(&c, kernel);
 }
 
 vkblas_status_t vkblas_linear_distill_backward_async(vkblas_dtype_t type, uint32_t M, uint32_t V, uint32_t K,

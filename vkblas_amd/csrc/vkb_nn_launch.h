@@ -168,8 +168,9 @@ int vkb_launch_xent_grad(int type, uint32_t M, uint32_t n, uint32_t v0, uint32_t
                          int64_t ldz, const int64_t* target, int64_t ignore, const float* lse, const float* dloss,
                          vkb_scale scale, void* D, int64_t ldd, void* stream);
 
-/* Distillation from a teacher's top logits (distill.hip).  rows: z_top and loss
- * from lse.  prepare, for the backward pass: q_top (M x n), T dloss (dl) and
+/* Distillation from a teacher's top logits (distill.hip).  rows: lse, z_top and
+ * loss, from the logits z where they are there (NULL: not), lse as it is
+ * (have_lse) or from S parts as xent stats leaves them (0: from z).  prepare, for the backward pass: q_top (M x n), T dloss (dl) and
  * targets for the kernels of D (ignore: a value no class has); patch: D's
  * elements of columns v0 .. v0 + cols - 1 at the entries, with scal[0] as those
  * kernels left it (NULL: 1). */
@@ -184,8 +185,16 @@ typedef struct vkb_distill {
     float *q_top, *dl;
     int64_t* target;
 } vkb_distill;
+typedef struct vkb_distill_rows {
+    const float* z;
+    int64_t ldz;
+    const float* parts;
+    uint32_t S;
+    int have_lse;
+    float *lse, *loss, *z_top;
+} vkb_distill_rows;
 int vkb_launch_distill_rows(int type, int t_type, const vkb_distill* d, uint32_t K, const void* x, int64_t ldx,
-                            const void* w, int64_t ldw, const float* lse, float* loss, float* z_top, void* stream);
+                            const void* w, int64_t ldw, const vkb_distill_rows* r, void* stream);
 int vkb_launch_distill_prepare(int t_type, const vkb_distill* d, const float* dloss, void* stream);
 int vkb_launch_distill_patch(int type, const vkb_distill* d, uint32_t v0, uint32_t cols, const float* lse,
                              const float* z_top, const float* scal, void* D, int64_t ldd, void* stream);
