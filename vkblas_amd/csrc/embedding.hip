@@ -221,25 +221,95 @@ __global__ __launch_bounds__(WORK) void merge_kernel(uint32_t M, uint64_t len, u
     order[group + at] = order_in[i];
 }
 
-// dw's columns c .. of a row: the sum of its rows of dy, scaled, and what was
-// there
-template <int VEC, typename W>
-__device__ __forceinline__ void put(W* row, int64_t c, int64_t N, float scale, float beta, const float* acc) {
-    constexpr int WV = Elem<W>::VEC;
-#pragma unroll
-    for (int q = 0; q < VEC; q += WV) {
-        if (c + q >= N) break;
-        float x[WV];
-        if (beta != 0.0f) {
-            unpack<W>(ld_chunk(row, c + q, N), x);
-#pragma unroll
-            for (int i = 0; i < WV; ++i) x[i] = beta * x[i] + scale * acc[q + i];
-        } else {
-#pragma unroll
-            for (int i = 0; i < WV; ++i) x[i] = scale * acc[q + i];
-        }
-        st_chunk(row, c + q, N, pack<W>(x));
+// A wave's 64 x 16 bytes of a row's columns, without branches around the loads:
+// VECTOR, 16 bytes a lane, where N is of whole 16-byte units or the wave's
+// columns all exist (lanes past the row's end read its last ones and write
+// nothing); else single columns, 64 apart, the last one read in the place of
+// those past it.
+template <typename T, bool VECTOR>
+struct Cols {
+    static constexpr int VEC = Elem<T>::VEC;
+    static constexpr uint32_t ROWS = 8;          // in flight
+    struct Row {
+        u32x4 v;
+    };
+    int64_t c, N;
+    bool in;
+    __device__ __forceinline__ Cols(int64_t block, uint32_t lane, int64_t n) : N(n) {
+        const int64_t at = (block * 64 + lane) * VEC;
+        in = at < N;
+        c = min(at, N - VEC);
     }
+    __device__ __forceinline__ Row load(const T* row) const { return Row{ld16_any(row + c)}; }
+    static __device__ __forceinline__ void add(const Row& r, float* acc) {
+        float f[VEC];
+        unpack<T>(r.v, f);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) acc[i] += f[i];
+    }
+    template <typename E>
+    __device__ __forceinline__ void get(const E* row, float* x) const {
+#pragma unroll
+        for (int q = 0; q < VEC; q += Elem<E>::VEC) unpack<E>(ld16_any(row + c + q), x + q);
+    }
+    template <typename E>
+    __device__ __forceinline__ void put(E* row, const float* x) const {
+        if (!in) return;
+#pragma unroll
+        for (int q = 0; q < VEC; q += Elem<E>::VEC) *(u32x4_any*)(row + c + q) = pack<E>(x + q);
+    }
+};
+template <typename T>
+struct Cols<T, false> {
+    static constexpr int VEC = Elem<T>::VEC;
+    static constexpr uint32_t ROWS = 4;          // a register for each of VEC values
+    struct Row {
+        T v[VEC];
+    };
+    int64_t c, N;
+    __device__ __forceinline__ Cols(int64_t block, uint32_t lane, int64_t n) : c(block * 64 * VEC + lane), N(n) {}
+    __device__ __forceinline__ int64_t at(int i) const { return min(c + 64 * i, N - 1); }
+    __device__ __forceinline__ Row load(const T* row) const {
+        Row r;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) r.v[i] = row[at(i)];
+        return r;
+    }
+    static __device__ __forceinline__ void add(const Row& r, float* acc) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) acc[i] += (float)r.v[i];
+    }
+    template <typename E>
+    __device__ __forceinline__ void get(const E* row, float* x) const {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) x[i] = (float)row[at(i)];
+    }
+    template <typename E>
+    __device__ __forceinline__ void put(E* row, const float* x) const {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+            if (c + 64 * i < N) row[c + 64 * i] = (E)x[i];
+    }
+};
+// f(true_type) where the wave's columns can go by vectors
+template <int VEC, typename F>
+__device__ __forceinline__ void with_cols(int64_t block, uint32_t N, F f) {
+    if (N % VEC == 0 || (block + 1) * 64 * VEC <= N) f(std::true_type{});
+    else f(std::false_type{});
+}
+// A row of dw: its sum, scaled, and what was there
+template <typename COLS, typename W>
+__device__ __forceinline__ void put_sum(const COLS& cols, W* row, float scale, float beta, const float* acc) {
+    float x[COLS::VEC];
+    if (beta != 0.0f) {
+        cols.get(row, x);
+#pragma unroll
+        for (int i = 0; i < COLS::VEC; ++i) x[i] = beta * x[i] + scale * acc[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < COLS::VEC; ++i) x[i] = scale * acc[i];
+    }
+    cols.put(row, x);
 }
 
 __device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
@@ -252,7 +322,7 @@ __device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__bui
 // waves' on a part of the list each.  Rows without one are zeroed or scaled in
 // all of their columns, by the workgroups of the same rows in turn.
 constexpr uint32_t DIRECT = VKB_EMBED_DIRECT, DTHREADS = 512, DWAVES = DTHREADS / 64, DSTEPS = DIRECT / DTHREADS;
-constexpr uint32_t DROWS = 4096, HEAVY = 8, DBATCH = 8;   // DROWS: the most rows of a workgroup
+constexpr uint32_t DROWS = 4096, HEAVY = 8;   // DROWS: the most rows of a workgroup
 struct DirectParams {
     uint32_t M, V, N, ranges;
     const int64_t* ids;
@@ -264,46 +334,38 @@ struct DirectParams {
     float scale, beta;
 };
 // acc += the rows of dy whose list entries a .. b - 1 are of row r
-template <typename T>
-__device__ __forceinline__ void add_listed(const DirectParams& p, const uint32_t* list, uint32_t a, uint32_t b, uint32_t r,
-                                           int64_t c, float* acc) {
-    constexpr int VEC = Elem<T>::VEC;
+template <typename T, typename COLS>
+__device__ __forceinline__ void add_listed(const DirectParams& p, const COLS& cols, const uint32_t* list, uint32_t a,
+                                           uint32_t b, uint32_t r, float* acc) {
     const uint32_t lane = threadIdx.x & 63;
     for (uint32_t i = a; i < b; i += 64) {
         const uint32_t e = i + lane < b ? list[i + lane] : ~0u;
         uint64_t mask = __ballot(e / DIRECT == r);
         while (mask) {
-            u32x4 x[DBATCH];
-            uint32_t n = 0;
+            typename COLS::Row x[COLS::ROWS];
+            const uint32_t n = (uint32_t)__popcll(mask);
 #pragma unroll
-            for (uint32_t k = 0; k < DBATCH; ++k) {
-                if (!mask) continue;
+            for (uint32_t k = 0; k < COLS::ROWS; ++k) {
+                if (k >= n) continue;
                 const int at = __builtin_ctzll(mask);
                 mask &= mask - 1;
                 const uint32_t m = (uint32_t)__builtin_amdgcn_readlane((int)e, at) % DIRECT;
-                x[k] = ld_chunk((const T*)p.dy + (int64_t)m * p.lddy, c, p.N);
-                ++n;
+                x[k] = cols.load((const T*)p.dy + (int64_t)m * p.lddy);
             }
 #pragma unroll
-            for (uint32_t k = 0; k < DBATCH; ++k) {
-                if (k >= n) continue;
-                float f[VEC];
-                unpack<T>(x[k], f);
-#pragma unroll
-                for (int q = 0; q < VEC; ++q) acc[q] += f[q];
-            }
+            for (uint32_t k = 0; k < COLS::ROWS; ++k)
+                if (k < n) COLS::add(x[k], acc);
         }
     }
 }
 template <typename T, typename W>
 __global__ __launch_bounds__(DTHREADS) void direct_kernel(DirectParams p) {
-    constexpr int VEC = Elem<T>::VEC, WV = Elem<W>::VEC, COLS = 64 * VEC;
+    constexpr int VEC = Elem<T>::VEC, WV = Elem<W>::VEC;
     __shared__ uint32_t list[DIRECT];                    // the workgroup's row times DIRECT, and m
     __shared__ uint32_t met[DROWS / 32], heavy[DROWS / 32], counts[DWAVES];
     __shared__ float sums[DWAVES - 1][64][VEC + 1];
     const uint32_t lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     const uint32_t r0 = blockIdx.x, rows = (p.V - r0 + p.ranges - 1) / p.ranges;
-    const int64_t c = (int64_t)blockIdx.y * COLS + lane * VEC;
     for (uint32_t i = threadIdx.x; i < (rows + 31) / 32; i += DTHREADS) met[i] = heavy[i] = 0;
     // a wave's ids are consecutive: DSTEPS times 64 of them
     const uint32_t first = wave * (DSTEPS * 64) + lane;
@@ -358,45 +420,47 @@ __global__ __launch_bounds__(DTHREADS) void direct_kernel(DirectParams p) {
             }
         }
     }
-    float acc[VEC];
-    auto clear = [&] {
+    with_cols<VEC>(blockIdx.y, p.N, [&](auto vector) {
+        const Cols<T, decltype(vector)::value> cols(blockIdx.y, lane, p.N);
+        float acc[VEC];
+        auto sum = [&](uint32_t r, uint32_t a, uint32_t b) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) acc[i] = 0.0f;
-    };
-    bool any = false;
-    for (uint32_t r = wave; r < rows; r += DWAVES) {
-        if (!(uniform(met[r / 32]) >> r % 32 & 1)) continue;
-        uint32_t of = 0;
-        for (uint32_t i = 0; i < total; i += 64)
-            of += (uint32_t)__popcll(__ballot(i + lane < total && list[i + lane] / DIRECT == r));
-        if (of > HEAVY) {
-            if (lane == 0) atomicOr(&heavy[r / 32], 1u << r % 32);
-            any = true;
-            continue;
+            for (int i = 0; i < VEC; ++i) acc[i] = 0.0f;
+            add_listed<T>(p, cols, list, a, b, r, acc);
+        };
+        bool any = false;
+        for (uint32_t r = wave; r < rows; r += DWAVES) {
+            if (!(uniform(met[r / 32]) >> r % 32 & 1)) continue;
+            uint32_t of = 0;
+            for (uint32_t i = 0; i < total; i += 64)
+                of += (uint32_t)__popcll(__ballot(i + lane < total && list[i + lane] / DIRECT == r));
+            if (of > HEAVY) {
+                if (lane == 0) atomicOr(&heavy[r / 32], 1u << r % 32);
+                any = true;
+                continue;
+            }
+            sum(r, 0, total);
+            put_sum(cols, dw + r * step, p.scale, p.beta, acc);
         }
-        clear();
-        add_listed<T>(p, list, 0, total, r, c, acc);
-        put<VEC>(dw + r * step, c, p.N, p.scale, p.beta, acc);
-    }
-    if (!__syncthreads_or(any)) return;
-    const uint32_t each = (total + DWAVES - 1) / DWAVES, a = min(wave * each, total), b = min(a + each, total);
-    for (uint32_t r = 0; r < rows; ++r) {
-        if (!(uniform(heavy[r / 32]) >> r % 32 & 1)) continue;
-        clear();
-        add_listed<T>(p, list, a, b, r, c, acc);
-        if (wave) {
+        if (!__syncthreads_or(any)) return;
+        const uint32_t each = (total + DWAVES - 1) / DWAVES, a = min(wave * each, total), b = min(a + each, total);
+        for (uint32_t r = 0; r < rows; ++r) {
+            if (!(uniform(heavy[r / 32]) >> r % 32 & 1)) continue;
+            sum(r, a, b);
+            if (wave) {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) sums[wave - 1][lane][i] = acc[i];
-        }
-        __syncthreads();
-        if (wave == 0) {
-            for (uint32_t w = 0; w < DWAVES - 1; ++w)
+                for (int i = 0; i < VEC; ++i) sums[wave - 1][lane][i] = acc[i];
+            }
+            __syncthreads();
+            if (wave == 0) {
+                for (uint32_t w = 0; w < DWAVES - 1; ++w)
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) acc[i] += sums[w][lane][i];
-            put<VEC>(dw + r * step, c, p.N, p.scale, p.beta, acc);
+                    for (int i = 0; i < VEC; ++i) acc[i] += sums[w][lane][i];
+                put_sum(cols, dw + r * step, p.scale, p.beta, acc);
+            }
+            __syncthreads();
         }
-        __syncthreads();
-    }
+    });
 }
 
 // ---- sorted tokens
@@ -412,17 +476,11 @@ struct SumParams {
     float* part;             // chunks x 2 x N: what began before a chunk, what goes on after it
 };
 
-// A wave: one chunk, 64 x 16 bytes of its rows' columns.  SROWS rows are in
-// flight while the SROWS before them are added up.
-constexpr uint32_t SROWS = 8;
-template <typename T, typename W>
-__device__ __forceinline__ void sum_unit(const SumParams& p, uint64_t unit) {
+// A wave: one chunk, 64 x 16 bytes of its rows' columns.
+template <typename T, typename W, typename COLS>
+__device__ __forceinline__ void sum_chunk(const SumParams& p, const COLS& cols, uint32_t chunk) {
     constexpr int VEC = Elem<T>::VEC;
     const uint32_t lane = threadIdx.x & 63;
-    const uint32_t chunk = (uint32_t)(unit / p.blocks), block = (uint32_t)(unit % p.blocks);
-    if (chunk >= p.chunks) return;
-    const int64_t c = ((int64_t)block * 64 + lane) * VEC;
-    const bool whole = (int64_t)(block + 1) * 64 * VEC <= p.N;
     const uint32_t p0 = chunk * p.chunk, p1 = p0 + min(p.chunk, p.M - p0);
     float acc[VEC];
     uint32_t now = ~0u;              // the token
@@ -431,18 +489,7 @@ __device__ __forceinline__ void sum_unit(const SumParams& p, uint64_t unit) {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) acc[i] = 0.0f;
     };
-    // the token ends here, or goes on in the next chunk
-    auto done = [&](bool on) {
-        if (c >= p.N) return;
-        if (!began && !on) {
-            put<VEC>((W*)p.dw + (int64_t)now * p.lddw, c, p.N, p.scale, p.beta, acc);
-            return;
-        }
-        float* part = p.part + ((int64_t)chunk * 2 + (began ? 0 : 1)) * p.N;
-#pragma unroll
-        for (int q = 0; q < VEC; q += 4)
-            if (c + q < p.N) st_chunk(part, c + q, p.N, pack<float>(acc + q));
-    };
+    float* part = p.part + (int64_t)chunk * 2 * p.N;
     clear();
     // VKB_EMBED_PAIRS pairs at a time in lanes 1 .. 62, the key before them and the one behind them beside
     for (uint32_t base = p0; base < p1; base += VKB_EMBED_PAIRS) {
@@ -453,46 +500,46 @@ __device__ __forceinline__ void sum_unit(const SumParams& p, uint64_t unit) {
             now = key(0);
             began = p0 && key(-1) == now;
         }
-        auto load = [&](uint32_t i, u32x4* x) {
-#pragma unroll
-            for (uint32_t r = 0; r < SROWS; ++r) {
-                const uint32_t m = (uint32_t)__builtin_amdgcn_readlane((int)rows, (int)min(i + r, n - 1) + 1);
-                const T* row = (const T*)p.dy + (int64_t)m * p.lddy;
-                x[r] = whole ? ld16_any(row + c) : ld_chunk(row, c, p.N);
-            }
+        // the token ends before another one or the padding
+        auto done = [&] {
+            if (began) cols.put(part, acc);
+            else put_sum(cols, (W*)p.dw + (int64_t)now * p.lddw, p.scale, p.beta, acc);
+            clear();
+            began = false;
         };
-        auto add = [&](uint32_t i, const u32x4* x) {
+        for (uint32_t i = 0; i < n; i += COLS::ROWS) {
+            if (now >= p.V) return;
+            typename COLS::Row x[COLS::ROWS];
 #pragma unroll
-            for (uint32_t r = 0; r < SROWS; ++r) {
-                if (i + r >= n || now >= p.V) continue;
+            for (uint32_t r = 0; r < COLS::ROWS; ++r) {
+                const uint32_t m = (uint32_t)__builtin_amdgcn_readlane((int)rows, (int)min(i + r, n - 1) + 1);
+                x[r] = cols.load((const T*)p.dy + (int64_t)m * p.lddy);
+            }
+#pragma unroll
+            for (uint32_t r = 0; r < COLS::ROWS; ++r) {
+                if (i + r >= n) continue;
                 const uint32_t k = key(i + r);
                 if (k != now) {
-                    done(false);
-                    clear();
+                    if (now < p.V) done();
                     now = k;
-                    began = false;
-                    if (now >= p.V) continue;
                 }
-                float f[VEC];
-                unpack<T>(x[r], f);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) acc[e] += f[e];
+                if (k < p.V) COLS::add(x[r], acc);
             }
-        };
-        if (now >= p.V || key(0) >= p.V) {       // padding from here on
-            if (now < p.V) done(false);
-            return;
         }
-        u32x4 x[SROWS], y[SROWS];
-        load(0, x);
-        for (uint32_t i = 0; i < n; i += 2 * SROWS) {
-            if (i + SROWS < n) load(i + SROWS, y);
-            add(i, x);
-            if (i + 2 * SROWS < n) load(i + 2 * SROWS, x);
-            if (i + SROWS < n) add(i + SROWS, y);
-        }
-        if (base + n == p1 && now < p.V) done(p1 < p.M && key(n) == now);
+        if (base + n < p1 || now >= p.V) continue;
+        // the last token: it ends here, or goes on
+        if (p1 < p.M && key(n) == now) cols.put(began ? part : part + p.N, acc);
+        else done();
     }
+}
+template <typename T, typename W>
+__device__ __forceinline__ void sum_unit(const SumParams& p, uint64_t unit) {
+    const uint32_t chunk = (uint32_t)(unit / p.blocks), block = (uint32_t)(unit % p.blocks);
+    if (chunk >= p.chunks) return;
+    with_cols<Elem<T>::VEC>(block, p.N, [&](auto vector) {
+        const Cols<T, decltype(vector)::value> cols(block, threadIdx.x & 63, p.N);
+        sum_chunk<T, W>(p, cols, chunk);
+    });
 }
 
 // FROWS rows of dw, those without a token zeroed or scaled: each wave searches
@@ -562,42 +609,36 @@ __global__ __launch_bounds__(WORK) void join_kernel(SumParams p) {
     }
     const uint32_t parts = lo - chunk + 1, each = (parts + 3) / 4;
     const uint32_t a = min(wave * each, parts), b = min(a + each, parts);
-    const int64_t c = ((int64_t)block * 64 + lane) * VEC;
-    float acc[VEC];
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) acc[i] = 0.0f;
     // part i: the tail of the first chunk, then the heads of the others
     auto row = [&](uint32_t i) { return p.part + ((int64_t)(chunk + i) * 2 + (i ? 0 : 1)) * p.N; };
-    if (c < p.N)
+    with_cols<VEC>(block, p.N, [&](auto vector) {
+        const Cols<T, decltype(vector)::value> cols(block, lane, p.N);
+        float acc[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) acc[i] = 0.0f;
         for (uint32_t i = a; i < b; i += 4) {
-            u32x4 x[4][VEC / 4];
+            float x[4][VEC];
+#pragma unroll
+            for (uint32_t r = 0; r < 4; ++r) cols.get(row(min(i + r, b - 1)), x[r]);
 #pragma unroll
             for (uint32_t r = 0; r < 4; ++r)
+                if (i + r < b) {
 #pragma unroll
-                for (int q = 0; q < VEC; q += 4) x[r][q / 4] = ld_chunk(row(min(i + r, b - 1)), c + q, p.N);
-#pragma unroll
-            for (uint32_t r = 0; r < 4; ++r) {
-                if (i + r >= b) continue;
-#pragma unroll
-                for (int q = 0; q < VEC; q += 4) {
-                    float f[4];
-                    unpack<float>(x[r][q / 4], f);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[q + e] += f[e];
+                    for (int e = 0; e < VEC; ++e) acc[e] += x[r][e];
                 }
-            }
         }
-    if (wave) {
+        if (wave) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) sh[wave - 1][lane][i] = acc[i];
-    }
-    __syncthreads();
-    if (wave || c >= p.N) return;
+            for (int i = 0; i < VEC; ++i) sh[wave - 1][lane][i] = acc[i];
+        }
+        __syncthreads();
+        if (wave) return;
 #pragma unroll
-    for (int w = 0; w < (int)WORK / 64 - 1; ++w)
+        for (int w = 0; w < (int)WORK / 64 - 1; ++w)
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) acc[i] += sh[w][lane][i];
-    put<VEC>((W*)p.dw + (int64_t)k * p.lddw, c, p.N, p.scale, p.beta, acc);
+            for (int i = 0; i < VEC; ++i) acc[i] += sh[w][lane][i];
+        put_sum(cols, (W*)p.dw + (int64_t)k * p.lddw, p.scale, p.beta, acc);
+    });
 }
 
 // f(T{}, W{}) for a type and one that is it or fp32
