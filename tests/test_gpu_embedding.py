@@ -91,9 +91,11 @@ def check_gradient(got, dy, ids, V, wt, scale, beta=0.0, dw0=None, pad_id=PAD):
     return dw
 
 
-# chunks of the sorted pairs (8 up to 16384 rows), runs of 4096, merges of up to 16 of them, a second level of merges
-GRAD_SIZES = SIZES + [(8, 3, 70), (9, 3, 70), (4095, 3, 8), (8192, 5, 24), (12289, 100000, 8), (16385, 40, 264),
-                      (65536, 3000, 16), (65537, 257, 9), (150001, 1000, 5)]
+# one launch (up to 2048 and 4096 rows), chunks of the sorted pairs, runs of 2048, merges of up to 16 and 64 of them, a
+# second level of merges (past 131072)
+GRAD_SIZES = SIZES + [(8, 3, 70), (9, 3, 70), (2047, 5, 24), (2048, 700, 72), (2049, 9, 8), (4095, 3, 8), (4097, 3, 8),
+                      (6145, 1, 20), (8192, 5, 24), (12289, 100000, 8), (16385, 40, 264), (32768, 200, 16),
+                      (32769, 3, 16), (65536, 3000, 16), (65537, 257, 9), (131073, 50, 8), (150001, 1000, 5)]
 
 
 @pytest.mark.parametrize("M,V,N", GRAD_SIZES)

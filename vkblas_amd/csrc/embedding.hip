@@ -321,7 +321,10 @@ __device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__bui
 // listed in order of m.  A row with up to HEAVY is a wave's, one with more all
 // waves' on a part of the list each.  Rows without one are zeroed or scaled in
 // all of their columns, by the workgroups of the same rows in turn.
-constexpr uint32_t DIRECT = VKB_EMBED_DIRECT, DTHREADS = 512, DWAVES = DTHREADS / 64, DSTEPS = DIRECT / DTHREADS;
+// Against the sort and its three launches (us, sorted / so, bf16): 2048 x 32000 x
+// 1024 29.5 / 18.5, 4096 x 32000 x 1024 30 / 23, 4096 x 500 x 512 21 / 12, and with
+// three tokens in ten the same 35 / 42; all of 4096 the same 41 / 81.
+constexpr uint32_t DIRECT = VKB_EMBED_DIRECT, DTHREADS = 512, DWAVES = DTHREADS / 64;
 constexpr uint32_t DROWS = 4096, HEAVY = 8;   // DROWS: the most rows of a workgroup
 struct DirectParams {
     uint32_t M, V, N, ranges;
@@ -358,10 +361,10 @@ __device__ __forceinline__ void add_listed(const DirectParams& p, const COLS& co
         }
     }
 }
-template <typename T, typename W>
+template <typename T, typename W, uint32_t DSTEPS>
 __global__ __launch_bounds__(DTHREADS) void direct_kernel(DirectParams p) {
     constexpr int VEC = Elem<T>::VEC, WV = Elem<W>::VEC;
-    __shared__ uint32_t list[DIRECT];                    // the workgroup's row times DIRECT, and m
+    __shared__ uint32_t list[DSTEPS * DTHREADS];         // the workgroup's row times DIRECT, and m
     __shared__ uint32_t met[DROWS / 32], heavy[DROWS / 32], counts[DWAVES];
     __shared__ float sums[DWAVES - 1][64][VEC + 1];
     const uint32_t lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
@@ -590,11 +593,14 @@ __global__ __launch_bounds__(WORK) void sum_kernel(SumParams p, uint32_t sums, u
 }
 
 // A token that begins in a chunk and goes on: that chunk's part and those of
-// the chunks it fills, the waves on a quarter each, in order.
+// the chunks it fills, the waves on a quarter each, in order, JROWS in flight.
+// (Eight waves: level, a token's 80 parts 3 us faster, 4000 workgroups with two
+// parts or none each 4 us slower.)
+constexpr uint32_t JTHREADS = 256, JWAVES = JTHREADS / 64, JROWS = 8;
 template <typename T, typename W>
-__global__ __launch_bounds__(WORK) void join_kernel(SumParams p) {
+__global__ __launch_bounds__(JTHREADS) void join_kernel(SumParams p) {
     constexpr int VEC = Elem<T>::VEC;
-    __shared__ float sh[WORK / 64 - 1][64][VEC + 1];
+    __shared__ float sh[JWAVES - 1][64][VEC + 1];
     const uint32_t chunk = blockIdx.y, block = blockIdx.x;
     const uint32_t lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     const uint32_t p0 = chunk * p.chunk, p1 = p0 + p.chunk;      // the last chunk is not here
@@ -607,7 +613,7 @@ __global__ __launch_bounds__(WORK) void join_kernel(SumParams p) {
         if (p.key[mid * p.chunk] == k) lo = mid;
         else hi = mid - 1;
     }
-    const uint32_t parts = lo - chunk + 1, each = (parts + 3) / 4;
+    const uint32_t parts = lo - chunk + 1, each = (parts + JWAVES - 1) / JWAVES;
     const uint32_t a = min(wave * each, parts), b = min(a + each, parts);
     // part i: the tail of the first chunk, then the heads of the others
     auto row = [&](uint32_t i) { return p.part + ((int64_t)(chunk + i) * 2 + (i ? 0 : 1)) * p.N; };
@@ -616,12 +622,13 @@ __global__ __launch_bounds__(WORK) void join_kernel(SumParams p) {
         float acc[VEC];
 #pragma unroll
         for (int i = 0; i < VEC; ++i) acc[i] = 0.0f;
-        for (uint32_t i = a; i < b; i += 4) {
-            float x[4][VEC];
+        for (uint32_t i = a; i < b; i += JROWS) {
+            float x[JROWS][VEC];
 #pragma unroll
-            for (uint32_t r = 0; r < 4; ++r) cols.get(row(min(i + r, b - 1)), x[r]);
+            for (uint32_t r = 0; r < JROWS; ++r)
+                if (i + r < b) cols.get(row(i + r), x[r]);
 #pragma unroll
-            for (uint32_t r = 0; r < 4; ++r)
+            for (uint32_t r = 0; r < JROWS; ++r)
                 if (i + r < b) {
 #pragma unroll
                     for (int e = 0; e < VEC; ++e) acc[e] += x[r][e];
@@ -634,7 +641,7 @@ __global__ __launch_bounds__(WORK) void join_kernel(SumParams p) {
         __syncthreads();
         if (wave) return;
 #pragma unroll
-        for (int w = 0; w < (int)WORK / 64 - 1; ++w)
+        for (int w = 0; w < (int)JWAVES - 1; ++w)
 #pragma unroll
             for (int i = 0; i < VEC; ++i) acc[i] += sh[w][lane][i];
         put_sum(cols, (W*)p.dw + (int64_t)k * p.lddw, p.scale, p.beta, acc);
@@ -685,8 +692,13 @@ extern "C" int vkb_launch_embedding_direct(int type, int w_type, uint32_t M, uin
     const bool ok = with_types(type, w_type, [&](auto t, auto o) {
         using T = decltype(t);
         using W = decltype(o);
-        hipLaunchKernelGGL((direct_kernel<T, W>), dim3((uint32_t)ranges, blocks), dim3(DTHREADS), 0,
-                           (hipStream_t)stream, p);
+        // half the steps for half the tokens: fp32 1003 x 997 x 515 9.1 -> 7.7 us
+        if (M <= DIRECT / 2)
+            hipLaunchKernelGGL((direct_kernel<T, W, DIRECT / 2 / DTHREADS>), dim3((uint32_t)ranges, blocks), dim3(DTHREADS),
+                               0, (hipStream_t)stream, p);
+        else
+            hipLaunchKernelGGL((direct_kernel<T, W, DIRECT / DTHREADS>), dim3((uint32_t)ranges, blocks), dim3(DTHREADS), 0,
+                               (hipStream_t)stream, p);
     });
     return ok ? (int)hipGetLastError() : (int)hipErrorInvalidValue;
 }
@@ -736,7 +748,7 @@ extern "C" int vkb_launch_embedding_sums(int type, int w_type, const vkb_embeddi
                            (uint32_t)sums, (uint32_t)fills);
         rc = (int)hipGetLastError();
         if (rc != 0 || p.chunks == 1) return;
-        hipLaunchKernelGGL((join_kernel<T, W>), dim3(p.blocks, p.chunks - 1), dim3(WORK), 0, (hipStream_t)stream, p);
+        hipLaunchKernelGGL((join_kernel<T, W>), dim3(p.blocks, p.chunks - 1), dim3(JTHREADS), 0, (hipStream_t)stream, p);
         rc = (int)hipGetLastError();
     });
     return rc;
