@@ -46,8 +46,10 @@ vkblas_status_t vkblas_embedding_async(
  * gradient of a w that is the output projection's too (tied weights) adds to
  * what vkblas_linear_xent_backward_async left there.
  * The rows of a token are summed in fp32 in an order that depends on ids, M, N
- * and the types alone: equal calls give equal bits.  Needs a workspace.
+ * and the types alone: equal calls give equal bits.  Needs a workspace for more
+ * than VKBLAS_EMBEDDING_SMALL tokens (or N above 2^24 - 256).
  */
+#define VKBLAS_EMBEDDING_SMALL 4096
 vkblas_status_t vkblas_embedding_backward_async(
     vkblas_dtype_t type,
     uint32_t M, uint32_t V, uint32_t N,

@@ -170,6 +170,20 @@ def test_empty_batch():
     dw.check_around()
 
 
+def test_a_vocabulary_of_many_rows():
+    """More rows than the fill has workgroups of 64."""
+    M, V = 5000, 70_000_001
+    ids = torch.randint(0, V, (M,), device="cuda")
+    ids[0], ids[1], ids[2] = V - 1, 0, V - 1
+    dy = torch.randn(M, 1, device="cuda")
+    for beta in (0.0, 0.5):
+        dw = torch.full((V, 1), 2.0, device="cuda")
+        vk.embedding_backward_async(vk.DT_F32, M, V, 1, ids.data_ptr(), PAD, dy.data_ptr(), 1, 1.0, dw.data_ptr(), 1,
+                                    vk.DT_F32, beta, stream=stream())
+        want = torch.full((V, 1), 2.0 * beta, device="cuda", dtype=torch.float64).index_add(0, ids, dy.double())
+        assert float((dw - want).abs().max()) <= 1e-5
+
+
 def test_offsets_past_32_bits():
     """A vocabulary of 2.2e9 elements: the last rows are read and written where they are."""
     V, N = 540000, 4096

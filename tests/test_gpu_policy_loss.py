@@ -114,6 +114,20 @@ def test_loss_and_gradient(B, T, reduce):
     check_grad(c.grad(got[1], 0.75), i, got[1], 0.75)
 
 
+@pytest.mark.parametrize("B,T", [(5_000_000, 1), (1_100_000, 257)])
+def test_more_sequences_than_workgroups(B, T):
+    """Against the definition on the GPU, equal rows: sequences of equal tokens."""
+    base = torch.linspace(-0.3, 0.3, 7, device="cuda").repeat(B // 7 + 1)[:B, None].expand(B, T).contiguous()
+    zero, adv = torch.zeros(B, T, device="cuda"), torch.ones(B, 1, device="cuda")
+    stats, norm = torch.empty(4, device="cuda"), torch.empty(B, device="cuda")
+    vk.policy_loss_async(vk.REDUCE_SEQUENCES, B, T, base.data_ptr(), T, zero.data_ptr(), T, None, 0, adv.data_ptr(), 1,
+                         0, None, 0, LOW, HIGH, 0.0, stats.data_ptr(), norm.data_ptr(), stream=stream())
+    r = base[:, 0].double().exp()
+    want = torch.stack([-r.clamp(max=1 + HIGH).mean(), 0 * r[0], (r > 1 + HIGH).double().mean(), r.mean()])
+    assert float((stats.double() - want).abs().max()) <= 1e-6
+    assert float((norm.double() * B * T - 1).abs().max()) <= 1e-6
+
+
 @pytest.mark.parametrize("B,T", [(7, 130), (90, 301)])
 @pytest.mark.parametrize("pad,off", [(0, 0), (4, 0), (1, 0), (3, 1)])
 @pytest.mark.parametrize("masked", [True, False])

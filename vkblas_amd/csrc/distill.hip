@@ -222,8 +222,8 @@ __global__ __launch_bounds__(WORK) void rows_kernel(uint32_t M, uint32_t V, uint
     }
 }
 
-// The backward pass's rows: q of each entry's class (both entries' where a class
-// occurs twice), T dloss, and a target for D's kernels: `ignore` where the row
+// The backward pass's rows: q of each entry's class (both entries' at the first
+// where a class occurs twice, -1 at the other: one of them patches D), T dloss, and a target for D's kernels: `ignore` where the row
 // is not counted, V where it is bad, else the first entry's class, whose
 // element the patch writes over.
 template <typename TT>
@@ -256,7 +256,12 @@ __global__ __launch_bounds__(WORK) void prepare_kernel(uint32_t M, uint32_t V, u
             float q = sh.q[j];
             if (same > 1 && id >= 0) {
                 q = 0.0f;
-                for (uint32_t i = 0; i < n; ++i) q += sh.id[i] == id ? sh.q[i] : 0.0f;
+                bool again = false;
+                for (uint32_t i = 0; i < n; ++i) {
+                    q += sh.id[i] == id ? sh.q[i] : 0.0f;
+                    again |= i < j && sh.id[i] == id;
+                }
+                if (again) q = -1.0f;
             }
             q_top[(int64_t)m * n + j] = q;
         }
@@ -281,9 +286,10 @@ __global__ __launch_bounds__(WORK) void patch_kernel(uint32_t M, uint32_t V, uin
     for (uint64_t i = (uint64_t)blockIdx.x * WORK + threadIdx.x; i < total; i += (uint64_t)gridDim.x * WORK) {
         const uint64_t m = i / n;
         const int64_t id = top[(int64_t)m * ldtop + (int64_t)(i - m * n)], c = id - v0;
-        if (id < 0 || c < 0 || c >= cols || target[m] == ignore || target[m] >= V) continue;
+        const float q = q_top[i];
+        if (id < 0 || c < 0 || c >= cols || q < 0.0f || target[m] == ignore || target[m] >= V) continue;
         const float p = fast_exp(z_top[i] * inv_t - lse[m]);
-        D[(int64_t)m * ldd + c] = (T)(dl[m] * sc * (p - q_top[i]));
+        D[(int64_t)m * ldd + c] = (T)(dl[m] * sc * (p - q));
     }
 }
 

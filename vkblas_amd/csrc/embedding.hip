@@ -324,7 +324,7 @@ __device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__bui
 // Against the sort and its three launches (us, sorted / so, bf16): 2048 x 32000 x
 // 1024 29.5 / 18.5, 4096 x 32000 x 1024 30 / 23, 4096 x 500 x 512 21 / 12, and with
 // three tokens in ten the same 35 / 42; all of 4096 the same 41 / 81.
-constexpr uint32_t DIRECT = VKB_EMBED_DIRECT, DTHREADS = 512, DWAVES = DTHREADS / 64;
+constexpr uint32_t DIRECT = VKBLAS_EMBEDDING_SMALL, DTHREADS = 512, DWAVES = DTHREADS / 64;
 constexpr uint32_t DROWS = 4096, HEAVY = 8;   // DROWS: the most rows of a workgroup
 struct DirectParams {
     uint32_t M, V, N, ranges;
@@ -549,10 +549,9 @@ __device__ __forceinline__ void sum_unit(const SumParams& p, uint64_t unit) {
 // their ids among the sorted keys, a lane each, and takes its part of them.
 constexpr uint32_t FROWS = 64;
 template <typename W>
-__device__ __forceinline__ void fill_unit(const SumParams& p, uint64_t unit) {
+__device__ __forceinline__ void fill_unit(const SumParams& p, uint64_t v0) {
     constexpr int VEC = Elem<W>::VEC;
     const uint32_t lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-    const uint64_t v0 = unit * FROWS;
     const uint64_t v = v0 + lane;
     uint32_t lo = 0, hi = v < p.V ? p.M : 0;
     while (__any(lo < hi)) {
@@ -589,7 +588,8 @@ __global__ __launch_bounds__(WORK) void sum_kernel(SumParams p, uint32_t sums, u
     const uint64_t b = blockIdx.x, all = (uint64_t)sums + fills;
     const uint64_t s = b * sums / all, next = (b + 1) * sums / all;    // the s-th of the sums, where next is past s
     if (next > s) sum_unit<T, W>(p, s * (WORK / 64) + uniform(threadIdx.x >> 6));
-    else fill_unit<W>(p, b - s);
+    else
+        for (uint64_t v0 = (b - s) * FROWS; v0 < p.V; v0 += (uint64_t)fills * FROWS) fill_unit<W>(p, v0);
 }
 
 // A token that begins in a chunk and goes on: that chunk's part and those of
@@ -738,7 +738,8 @@ extern "C" int vkb_launch_embedding_sums(int type, int w_type, const vkb_embeddi
     SumParams p{a->M, a->V, a->N, a->chunk, a->chunks, (a->N + cols - 1) / cols, a->key, a->order, a->dy, a->lddy,
                 a->dw, a->lddw, a->scale, a->beta, a->part};
     const uint64_t sums = ((uint64_t)p.chunks * p.blocks + WORK / 64 - 1) / (WORK / 64);
-    const uint64_t fills = p.beta == 1.0f ? 0 : ((uint64_t)p.V + FROWS - 1) / FROWS;
+    uint64_t fills = p.beta == 1.0f ? 0 : ((uint64_t)p.V + FROWS - 1) / FROWS;
+    if (fills > 1u << 20) fills = 1u << 20;
     if (sums + fills > 0xffffffffull / WORK) return (int)hipErrorInvalidValue;
     int rc = (int)hipErrorInvalidValue;
     with_types(type, w_type, [&](auto t, auto o) {

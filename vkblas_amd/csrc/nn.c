@@ -1031,7 +1031,7 @@ vkblas_status_t vkblas_embedding_backward_async(vkblas_dtype_t type, uint32_t M,
     if (M == 0) return empty_gradient(&c, dw_type, V, N, dw, lddw, beta);
     if (!ids || !dy) return VKBLAS_ERR_PARAM;
     if (vkb_engine_trace()) fprintf(stderr, "[vkblas] embedding_backward type=%d M=%u V=%u N=%u\n", (int)type, M, V, N);
-    if (M <= VKB_EMBED_DIRECT && (uint64_t)N <= 65535u * 256u) {
+    if (M <= VKBLAS_EMBEDDING_SMALL && N <= 65535u * 256u) {
         if (room(&c) != VKBLAS_OK) return c.st;
         step(&c, vkb_launch_embedding_direct(type, dw_type, M, V, N, ids, pad_id, dy, lddy, scale, dw, lddw, beta, stream),
              1);

@@ -238,24 +238,26 @@ __global__ __launch_bounds__(WORK) void unit_kernel(vkb_policy p, double* part) 
     constexpr uint32_t WAVES = WORK / 64;
     __shared__ double sh[WAVES][NSUM];
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint64_t unit = SHORT ? (uint64_t)blockIdx.x * WAVES + wave : blockIdx.x, count = (uint64_t)p.B * p.units;
-    if (unit >= count) return;
-    const int64_t b = (int64_t)(unit / p.units), t0 = (int64_t)(unit % p.units) * p.unit;
-    const int64_t t1 = min(t0 + p.unit, (int64_t)p.T);
-    Sums s = token_sums(p, b, SHORT ? t0 : t0 + 256 * wave, t1, SHORT ? 256 : 256 * WAVES, lane);
-    if (!SHORT) {
+    const uint64_t count = (uint64_t)p.B * p.units, step = (uint64_t)gridDim.x * (SHORT ? WAVES : 1);
+    for (uint64_t unit = SHORT ? (uint64_t)blockIdx.x * WAVES + wave : blockIdx.x; unit < count; unit += step) {
+        const int64_t b = (int64_t)(unit / p.units), t0 = (int64_t)(unit % p.units) * p.unit;
+        const int64_t t1 = min(t0 + p.unit, (int64_t)p.T);
+        Sums s = token_sums(p, b, SHORT ? t0 : t0 + 256 * wave, t1, SHORT ? 256 : 256 * WAVES, lane);
+        if (!SHORT) {
+            __syncthreads();                 // the unit before is read
+#pragma unroll
+            for (int i = 0; i < NSUM; ++i)
+                if (lane == 0) sh[wave][i] = s.v[i];
+            __syncthreads();
+            if (wave) continue;
+#pragma unroll
+            for (int i = 0; i < NSUM; ++i)
+                for (uint32_t w = 1; w < WAVES; ++w) s.v[i] += sh[w][i];
+        }
 #pragma unroll
         for (int i = 0; i < NSUM; ++i)
-            if (lane == 0) sh[wave][i] = s.v[i];
-        __syncthreads();
-        if (wave) return;
-#pragma unroll
-        for (int i = 0; i < NSUM; ++i)
-            for (uint32_t w = 1; w < WAVES; ++w) s.v[i] += sh[w][i];
+            if (lane == (uint32_t)i) part[i * count + unit] = s.v[i];
     }
-#pragma unroll
-    for (int i = 0; i < NSUM; ++i)
-        if (lane == (uint32_t)i) part[i * count + unit] = s.v[i];
 }
 __global__ __launch_bounds__(FIN) void finish_kernel(vkb_policy p, int reduce, const double* part, float* stats,
                                                      float* norm) {
@@ -333,13 +335,11 @@ extern "C" int vkb_launch_policy(const vkb_policy* p, int reduce, void* part, fl
         return (int)hipGetLastError();
     }
     const uint64_t count = (uint64_t)p->B * p->units, blocks = p->T <= 256 ? (count + WORK / 64 - 1) / (WORK / 64) : count;
-    if (blocks > 0xffffffffull / WORK) return (int)hipErrorInvalidValue;
+    const dim3 grid((uint32_t)(blocks < 1u << 20 ? blocks : 1u << 20));
     if (p->T <= 256)
-        hipLaunchKernelGGL((unit_kernel<true>), dim3((uint32_t)blocks), dim3(WORK), 0, (hipStream_t)stream, *p,
-                           (double*)part);
+        hipLaunchKernelGGL((unit_kernel<true>), grid, dim3(WORK), 0, (hipStream_t)stream, *p, (double*)part);
     else
-        hipLaunchKernelGGL((unit_kernel<false>), dim3((uint32_t)blocks), dim3(WORK), 0, (hipStream_t)stream, *p,
-                           (double*)part);
+        hipLaunchKernelGGL((unit_kernel<false>), grid, dim3(WORK), 0, (hipStream_t)stream, *p, (double*)part);
     const int rc = (int)hipGetLastError();
     if (rc != 0) return rc;
     hipLaunchKernelGGL(finish_kernel, dim3(1), dim3(FIN), 0, (hipStream_t)stream, *p, reduce, (const double*)part, stats,
