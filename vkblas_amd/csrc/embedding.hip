@@ -15,8 +15,8 @@
 //    token that ends inside goes to dw, a part that began before the chunk or
 //    goes on after it to the workspace.
 //  - Join: a token of several chunks adds their parts in order.
-// Rows of dw without a token are zeroed or scaled beside the sums, by
-// workgroups that search the rows' ids (not for beta = 1).
+// dw is zeroed beside the first step of the sort (beta = 0), or its rows without
+// a token are scaled by a pass that searches their ids (not for beta = 1).
 //
 // Few tokens (VKB_EMBED_DIRECT) take one launch without a workspace: each
 // workgroup looks all ids over for those of its own rows of dw.
@@ -58,12 +58,26 @@ __device__ __forceinline__ uint32_t sort_key(int64_t id, int64_t pad, uint32_t V
 // run's keys each.  A pair before the token's counts where its key is at most
 // the token's, one after it where it is less.
 constexpr uint32_t RTOK = 16, RGROUPS = WORK / RTOK;
+//
+// The workgroups from ranks on zero dw, 16 bytes a thread: stores are fastest
+// from many short workgroups (1 GiB of zeros: 4 KB each 6.8 TB/s, 8 KB 6.1, 512 KB 5.7,
+// 8192 workgroups in strides 4.6; rows with tokens left out, which takes a look at
+// a map of them, 4.6 beside the sums).
+template <typename W>
 __global__ __launch_bounds__(WORK) void rank_kernel(uint32_t M, uint32_t V, const int64_t* ids, int64_t pad,
-                                                    uint32_t* key, uint32_t* order) {
+                                                    uint32_t* key, uint32_t* order, uint32_t ranks, uint32_t N, W* dw,
+                                                    int64_t lddw) {
+    if (blockIdx.x >= ranks) {
+        constexpr int VEC = Elem<W>::VEC;
+        for_chunks(V, (N + VEC - 1) / VEC, ranks, gridDim.x - ranks, [&](uint64_t v, uint32_t k) {
+            st_chunk(dw + (int64_t)v * lddw, (int64_t)k * VEC, N, u32x4{0u, 0u, 0u, 0u});
+        });
+        return;
+    }
     __shared__ __attribute__((aligned(16))) uint32_t keys[RUN];
     __shared__ uint32_t count[WORK];
     const uint32_t tok = threadIdx.x % RTOK, g = threadIdx.x / RTOK;
-    for (uint64_t first = (uint64_t)blockIdx.x * RTOK; first < M; first += (uint64_t)gridDim.x * RTOK) {
+    for (uint64_t first = (uint64_t)blockIdx.x * RTOK; first < M; first += (uint64_t)ranks * RTOK) {
         const uint64_t run = first / RUN * RUN;
         const uint32_t n = (uint32_t)min((uint64_t)RUN, M - run), whole = (n + 3) / 4 * 4;
         int64_t id[RUN / WORK];               // all loads in flight
@@ -536,7 +550,8 @@ __device__ __forceinline__ void sum_chunk(const SumParams& p, const COLS& cols, 
     }
 }
 template <typename T, typename W>
-__device__ __forceinline__ void sum_unit(const SumParams& p, uint64_t unit) {
+__global__ __launch_bounds__(WORK) void sum_kernel(SumParams p) {
+    const uint64_t unit = (uint64_t)blockIdx.x * (WORK / 64) + uniform(threadIdx.x >> 6);
     const uint32_t chunk = (uint32_t)(unit / p.blocks), block = (uint32_t)(unit % p.blocks);
     if (chunk >= p.chunks) return;
     with_cols<Elem<T>::VEC>(block, p.N, [&](auto vector) {
@@ -545,51 +560,38 @@ __device__ __forceinline__ void sum_unit(const SumParams& p, uint64_t unit) {
     });
 }
 
-// FROWS rows of dw, those without a token zeroed or scaled: each wave searches
-// their ids among the sorted keys, a lane each, and takes its part of them.
+// dw = beta * dw on the rows without a token: each wave searches the ids of
+// FROWS rows among the sorted keys, a lane each, and takes its part of them.
 constexpr uint32_t FROWS = 64;
 template <typename W>
-__device__ __forceinline__ void fill_unit(const SumParams& p, uint64_t v0) {
+__global__ __launch_bounds__(WORK) void others_kernel(uint32_t M, uint32_t V, uint32_t N, const uint32_t* key, W* dw,
+                                                      int64_t lddw, float beta) {
     constexpr int VEC = Elem<W>::VEC;
     const uint32_t lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-    const uint64_t v = v0 + lane;
-    uint32_t lo = 0, hi = v < p.V ? p.M : 0;
-    while (__any(lo < hi)) {
-        const uint32_t mid = lo + (hi - lo) / 2;
-        const bool less = lo < hi && p.key[mid] < v;
-        if (less) lo = mid + 1;
-        else if (lo < hi) hi = mid;
-    }
-    const bool none = v < p.V && !(lo < p.M && p.key[lo] == v);
-    const uint64_t mask = __ballot(none);
     // as many waves to a row as it has 64 chunks
-    const uint32_t per = min(WORK / 64, (p.N + 64 * VEC - 1) / (64 * VEC)), at_once = WORK / 64 / per;
-    for (uint32_t r = wave / per; r < FROWS && wave / per < at_once; r += at_once) {
-        if (!(mask >> r & 1)) continue;
-        W* row = (W*)p.dw + (int64_t)(v0 + r) * p.lddw;
-        for (int64_t k = (int64_t)(wave % per * 64 + lane) * VEC; k < p.N; k += per * 64 * VEC) {
-            u32x4 x = {0u, 0u, 0u, 0u};
-            if (p.beta != 0.0f) {
+    const uint32_t per = min(WORK / 64, (N + 64 * VEC - 1) / (64 * VEC)), at_once = WORK / 64 / per;
+    for (uint64_t v0 = (uint64_t)blockIdx.x * FROWS; v0 < V; v0 += (uint64_t)gridDim.x * FROWS) {
+        const uint64_t v = v0 + lane;
+        uint32_t lo = 0, hi = v < V ? M : 0;
+        while (__any(lo < hi)) {
+            const uint32_t mid = lo + (hi - lo) / 2;
+            const bool less = lo < hi && key[mid] < v;
+            if (less) lo = mid + 1;
+            else if (lo < hi) hi = mid;
+        }
+        const uint64_t mask = __ballot(v < V && !(lo < M && key[lo] == v));
+        for (uint32_t r = wave / per; r < FROWS && wave / per < at_once; r += at_once) {
+            if (!(mask >> r & 1)) continue;
+            W* row = dw + (int64_t)(v0 + r) * lddw;
+            for (int64_t k = (int64_t)(wave % per * 64 + lane) * VEC; k < N; k += per * 64 * VEC) {
                 float f[VEC];
-                unpack<W>(ld_chunk(row, k, p.N), f);
+                unpack<W>(ld_chunk(row, k, N), f);
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) f[i] *= p.beta;
-                x = pack<W>(f);
+                for (int i = 0; i < VEC; ++i) f[i] *= beta;
+                st_chunk(row, k, N, pack<W>(f));
             }
-            st_chunk(row, k, p.N, x);
         }
     }
-}
-
-// The chunks and the rows without tokens in one launch, spread over one
-// another: both are bound by memory, the one by latency too.
-template <typename T, typename W>
-__global__ __launch_bounds__(WORK) void sum_kernel(SumParams p, uint32_t sums, uint32_t fills) {
-    const uint64_t b = blockIdx.x, all = (uint64_t)sums + fills;
-    const uint64_t s = b * sums / all, next = (b + 1) * sums / all;    // the s-th of the sums, where next is past s
-    if (next > s) sum_unit<T, W>(p, s * (WORK / 64) + uniform(threadIdx.x >> 6));
-    else
-        for (uint64_t v0 = (b - s) * FROWS; v0 < p.V; v0 += (uint64_t)fills * FROWS) fill_unit<W>(p, v0);
 }
 
 // A token that begins in a chunk and goes on: that chunk's part and those of
@@ -662,13 +664,19 @@ bool with_types(int type, int other, F f) {
 
 using namespace vkb;
 
+// One chunk a thread, up to 2^22 workgroups
+static uint32_t blocks_of(uint64_t chunks) {
+    const uint64_t b = (chunks + WORK - 1) / WORK;
+    return (uint32_t)(b < 1u << 22 ? b : 1u << 22);
+}
+
 extern "C" int vkb_launch_embedding(int type, int w_type, uint32_t M, uint32_t V, uint32_t N, const int64_t* ids,
                                     int64_t pad, const void* w, int64_t ldw, float scale, void* y, int64_t ldy,
                                     void* stream) {
     const bool ok = with_types(type, w_type, [&](auto t, auto o) {
         using T = decltype(t);
         using W = decltype(o);
-        hipLaunchKernelGGL((lookup_kernel<T, W>), dim3(chunk_blocks(M, chunks_of<T>(N))), dim3(WORK), 0,
+        hipLaunchKernelGGL((lookup_kernel<T, W>), dim3(blocks_of((uint64_t)M * chunks_of<T>(N))), dim3(WORK), 0,
                            (hipStream_t)stream, M, V, N, ids, pad, (const W*)w, ldw, scale, (T*)y, ldy);
     });
     return ok ? (int)hipGetLastError() : (int)hipErrorInvalidValue;
@@ -704,11 +712,16 @@ extern "C" int vkb_launch_embedding_direct(int type, int w_type, uint32_t M, uin
 }
 
 extern "C" int vkb_launch_embedding_rank(uint32_t M, uint32_t V, const int64_t* ids, int64_t pad, uint32_t* key,
-                                         uint32_t* order, void* stream) {
-    const uint32_t tiles = (uint32_t)(((uint64_t)M + RTOK - 1) / RTOK);
-    hipLaunchKernelGGL(rank_kernel, dim3(tiles < 65536 ? tiles : 65536), dim3(WORK), 0, (hipStream_t)stream, M, V, ids,
-                       pad, key, order);
-    return (int)hipGetLastError();
+                                         uint32_t* order, int w_type, uint32_t N, void* dw, int64_t lddw,
+                                         void* stream) {
+    const uint32_t tiles = (uint32_t)(((uint64_t)M + RTOK - 1) / RTOK), ranks = tiles < 65536 ? tiles : 65536;
+    const bool ok = with_type(w_type, [&](auto t) {
+        using W = decltype(t);
+        const uint32_t fill = dw ? blocks_of((uint64_t)V * chunks_of<W>(N)) : 0;
+        hipLaunchKernelGGL((rank_kernel<W>), dim3(ranks + fill), dim3(WORK), 0, (hipStream_t)stream, M, V, ids, pad, key,
+                           order, ranks, N, (W*)dw, lddw);
+    });
+    return ok ? (int)hipGetLastError() : (int)hipErrorInvalidValue;
 }
 
 extern "C" int vkb_launch_embedding_merge_runs(uint32_t M, const uint32_t* key_in, const uint32_t* order_in, uint32_t* key,
@@ -733,20 +746,28 @@ extern "C" int vkb_launch_embedding_merge(uint32_t M, uint64_t len, const uint32
     return (int)hipGetLastError();
 }
 
+extern "C" int vkb_launch_embedding_others(int w_type, uint32_t M, uint32_t V, uint32_t N, const uint32_t* key, void* dw,
+                                           int64_t lddw, float beta, void* stream) {
+    const bool ok = with_type(w_type, [&](auto t) {
+        using W = decltype(t);
+        const uint32_t b = (uint32_t)(((uint64_t)V + FROWS - 1) / FROWS);
+        hipLaunchKernelGGL((others_kernel<W>), dim3(b < 1u << 20 ? b : 1u << 20), dim3(WORK), 0, (hipStream_t)stream, M,
+                           V, N, key, (W*)dw, lddw, beta);
+    });
+    return ok ? (int)hipGetLastError() : (int)hipErrorInvalidValue;
+}
+
 extern "C" int vkb_launch_embedding_sums(int type, int w_type, const vkb_embedding_sums* a, void* stream) {
     const uint32_t cols = 64 * (type == VKB_T_F32 ? 4 : 8);
     SumParams p{a->M, a->V, a->N, a->chunk, a->chunks, (a->N + cols - 1) / cols, a->key, a->order, a->dy, a->lddy,
                 a->dw, a->lddw, a->scale, a->beta, a->part};
     const uint64_t sums = ((uint64_t)p.chunks * p.blocks + WORK / 64 - 1) / (WORK / 64);
-    uint64_t fills = p.beta == 1.0f ? 0 : ((uint64_t)p.V + FROWS - 1) / FROWS;
-    if (fills > 1u << 20) fills = 1u << 20;
-    if (sums + fills > 0xffffffffull / WORK) return (int)hipErrorInvalidValue;
+    if (sums > 0xffffffffull / WORK) return (int)hipErrorInvalidValue;
     int rc = (int)hipErrorInvalidValue;
     with_types(type, w_type, [&](auto t, auto o) {
         using T = decltype(t);
         using W = decltype(o);
-        hipLaunchKernelGGL((sum_kernel<T, W>), dim3((uint32_t)(sums + fills)), dim3(WORK), 0, (hipStream_t)stream, p,
-                           (uint32_t)sums, (uint32_t)fills);
+        hipLaunchKernelGGL((sum_kernel<T, W>), dim3((uint32_t)sums), dim3(WORK), 0, (hipStream_t)stream, p);
         rc = (int)hipGetLastError();
         if (rc != 0 || p.chunks == 1) return;
         hipLaunchKernelGGL((join_kernel<T, W>), dim3(p.blocks, p.chunks - 1), dim3(JTHREADS), 0, (hipStream_t)stream, p);

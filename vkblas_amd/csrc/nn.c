@@ -1053,7 +1053,8 @@ vkblas_status_t vkblas_embedding_backward_async(vkblas_dtype_t type, uint32_t M,
     const size_t o_p = a.chunks > 1 ? buf(&c, (uint64_t)a.chunks * 2 * N * sizeof(float)) : 0;
     if (room(&c) != VKBLAS_OK) return c.st;
     uint32_t *key = at(&c, o_k), *order = at(&c, o_o), *key2 = at(&c, o_k2), *order2 = at(&c, o_o2);
-    int ok = step(&c, vkb_launch_embedding_rank(M, V, ids, pad_id, key, order, stream), 0);
+    int ok = step(&c, vkb_launch_embedding_rank(M, V, ids, pad_id, key, order, dw_type, N,
+                                                beta == 0.0f ? dw : NULL, lddw, stream), beta == 0.0f);
     for (uint64_t len = VKB_EMBED_RUN; ok && len < M;
          len = len == VKB_EMBED_RUN ? vkb_embedding_group(M) : len * VKB_EMBED_WAYS) {
         ok = len == VKB_EMBED_RUN
@@ -1065,6 +1066,8 @@ vkblas_status_t vkblas_embedding_backward_async(vkblas_dtype_t type, uint32_t M,
         key2 = k;
         order2 = o;
     }
+    if (ok && beta != 0.0f && beta != 1.0f)
+        ok = step(&c, vkb_launch_embedding_others(dw_type, M, V, N, key, dw, lddw, beta, stream), 1);
     a.key = key;
     a.order = order;
     a.part = a.chunks > 1 ? (float*)at(&c, o_p) : NULL;

@@ -91,9 +91,10 @@ int vkb_launch_glu_direct(int type, int act, uint32_t M, uint32_t N, uint32_t K,
 
 /* Embedding (embedding.hip).  Its gradient: rank writes the M pairs (key, row of
  * dy) sorted by key, then row, in each run of VKB_EMBED_RUN (key: the token's
- * id, V where its row adds nothing); merge_runs makes sorted runs of
- * vkb_embedding_group pairs out of those, merge ones of VKB_EMBED_WAYS * len out
- * of ones of len; sums: all of dw from the sorted pairs in `chunks` chunks of
+ * id, V where its row adds nothing), and zeroes dw (NULL: not); merge_runs makes
+ * sorted runs of vkb_embedding_group pairs out of those, merge ones of
+ * VKB_EMBED_WAYS * len out of ones of len; others: dw = beta * dw on the rows of
+ * no token; sums: the rows of the tokens, the sorted pairs in `chunks` chunks of
  * `chunk` (the last may be shorter), at most VKB_EMBED_CHUNKS, part chunks x 2 x
  * N floats.
  * direct: all of it in one launch, for up to VKBLAS_EMBEDDING_SMALL rows. */
@@ -110,11 +111,13 @@ static inline uint64_t vkb_embedding_group(uint32_t M) {
 int vkb_launch_embedding(int type, int w_type, uint32_t M, uint32_t V, uint32_t N, const int64_t* ids, int64_t pad,
                          const void* w, int64_t ldw, float scale, void* y, int64_t ldy, void* stream);
 int vkb_launch_embedding_rank(uint32_t M, uint32_t V, const int64_t* ids, int64_t pad, uint32_t* key, uint32_t* order,
-                              void* stream);
+                              int w_type, uint32_t N, void* dw, int64_t lddw, void* stream);
 int vkb_launch_embedding_merge_runs(uint32_t M, const uint32_t* key_in, const uint32_t* order_in, uint32_t* key,
                                     uint32_t* order, void* stream);
 int vkb_launch_embedding_merge(uint32_t M, uint64_t len, const uint32_t* key_in, const uint32_t* order_in,
                                uint32_t* key, uint32_t* order, void* stream);
+int vkb_launch_embedding_others(int w_type, uint32_t M, uint32_t V, uint32_t N, const uint32_t* key, void* dw,
+                                int64_t lddw, float beta, void* stream);
 typedef struct vkb_embedding_sums {
     uint32_t M, V, N, chunk, chunks;
     const uint32_t *key, *order;
