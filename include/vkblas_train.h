@@ -47,9 +47,11 @@ vkblas_status_t vkblas_embedding_async(
  * what vkblas_linear_xent_backward_async left there.
  * The rows of a token are summed in fp32 in an order that depends on ids, M, N
  * and the types alone: equal calls give equal bits.  Needs a workspace for more
- * than VKBLAS_EMBEDDING_SMALL tokens (or N above 2^24 - 256).
+ * than VKBLAS_EMBEDDING_SMALL tokens or a gradient of more than
+ * VKBLAS_EMBEDDING_SMALL_BYTES (V * N of dw_type), or N above 2^24 - 256.
  */
 #define VKBLAS_EMBEDDING_SMALL 4096
+#define VKBLAS_EMBEDDING_SMALL_BYTES ((uint64_t)64 << 20)
 vkblas_status_t vkblas_embedding_backward_async(
     vkblas_dtype_t type,
     uint32_t M, uint32_t V, uint32_t N,

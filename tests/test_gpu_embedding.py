@@ -105,6 +105,17 @@ def test_gradient(M, V, N, dt, wt):
     check_gradient(gradient(dy, ids, V, dt, wt, 1.5), dy, ids, V, wt, 1.5)
 
 
+@pytest.mark.parametrize("M,V,N", [(1, 40000, 1000), (3, 33000, 1025), (300, 70001, 520), (4096, 16400, 2050)])
+@pytest.mark.parametrize("beta", [0.0, 1.0, 0.5])
+def test_gradient_of_few_tokens_and_a_large_one(M, V, N, beta):
+    """More bytes than the one launch takes: the sort of one run.  On the GPU."""
+    dy, ids = R.values(M, N, "bf16", 1).cuda(), tokens(M, V, 2).cuda()
+    dw0 = torch.linspace(-1, 1, V, dtype=torch.float32).double()[:, None].expand(V, N).contiguous().cuda()
+    got = gradient(dy, ids, V, "bf16", "f32", 1.5, beta, dw0)
+    dw, err = D.embedding_grad(dy, ids, V, 1.5, PAD, beta, dw0)
+    R.close(got.cuda(), dw, R.rounded(dw, "f32", err), "dw")
+
+
 @pytest.mark.parametrize("M,V,N", [(7, 5, 130), (100, 64, 257), (5000, 900, 72), (70000, 30, 24)])
 @pytest.mark.parametrize("kind", ["one", "uniform", "usual"])
 @pytest.mark.parametrize("dt,wt", [("f32", "f32"), ("bf16", "bf16"), ("f16", "f32")])

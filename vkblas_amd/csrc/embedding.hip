@@ -18,8 +18,8 @@
 // dw is zeroed beside the first step of the sort (beta = 0), or its rows without
 // a token are scaled by a pass that searches their ids (not for beta = 1).
 //
-// Few tokens (VKB_EMBED_DIRECT) take one launch without a workspace: each
-// workgroup looks all ids over for those of its own rows of dw.
+// Few tokens and a small dw take one launch without a workspace: each workgroup
+// looks all ids over for those of its own rows of dw.
 #include "nn_common.hpp"
 
 namespace vkb {
@@ -687,12 +687,9 @@ extern "C" int vkb_launch_embedding_direct(int type, int w_type, uint32_t M, uin
                                            int64_t lddw, float beta, void* stream) {
     if (M > DIRECT) return (int)hipErrorInvalidValue;
     const uint32_t cols = 64 * (type == VKB_T_F32 ? 4 : 8), blocks = (N + cols - 1) / cols;
-    // one wave of workgroups, or one for each 128 KB of a large dw, whose rows
-    // without tokens most of the time goes into (us for 1024 / 1536 / 4096 workgroups:
-    // bf16 1024 x 32000 x 1024 17.8 / 16.9 / 23.6, 2048 x 128000 x 4096 295 / 268 / 221)
-    const uint64_t bytes = (uint64_t)V * N * (w_type == VKB_T_F32 ? 4 : 2) >> 17;
-    const uint64_t want = bytes < 1024 ? 1024 : bytes < 8192 ? bytes : 8192;
-    uint64_t rows = ((uint64_t)V * blocks + want - 1) / want;
+    // one wave of workgroups (us for 256 / 1024 / 4096: fp32 1003 x 997 x 515 9.9 / 9.0 /
+    // 12.2, bf16 1024 x 32000 x 1024 35 / 17.8 / 23.6)
+    uint64_t rows = ((uint64_t)V * blocks + 1023) / 1024;
     if (rows > DROWS) rows = DROWS;
     const uint64_t ranges = (V + rows - 1) / rows;
     if (ranges > 0xffffffffull / DTHREADS || blocks > 65535) return (int)hipErrorInvalidValue;

@@ -1031,7 +1031,12 @@ vkblas_status_t vkblas_embedding_backward_async(vkblas_dtype_t type, uint32_t M,
     if (M == 0) return empty_gradient(&c, dw_type, V, N, dw, lddw, beta);
     if (!ids || !dy) return VKBLAS_ERR_PARAM;
     if (vkb_engine_trace()) fprintf(stderr, "[vkblas] embedding_backward type=%d M=%u V=%u N=%u\n", (int)type, M, V, N);
-    if (M <= VKBLAS_EMBEDDING_SMALL && N <= 65535u * 256u) {
+    /* one launch, but for a large dw: its workgroups then have many rows each, and the
+     * zeros a bad pattern of stores (us, one launch / sorted, bf16: 1024 x 32000 x 1024,
+     * 66 MB, 17.6 / 28; 1000 x 64000 x 1024 38 / 30; 1 x 128000 x 4096 186 / 156;
+     * 4000 x 128000 x 4096 218 / 183) */
+    if (M <= VKBLAS_EMBEDDING_SMALL && N <= 65535u * 256u &&
+        (uint64_t)V * N * type_size(dw_type) <= VKBLAS_EMBEDDING_SMALL_BYTES) {
         if (room(&c) != VKBLAS_OK) return c.st;
         step(&c, vkb_launch_embedding_direct(type, dw_type, M, V, N, ids, pad_id, dy, lddy, scale, dw, lddw, beta, stream),
              1);

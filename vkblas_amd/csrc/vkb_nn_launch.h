@@ -97,7 +97,8 @@ int vkb_launch_glu_direct(int type, int act, uint32_t M, uint32_t N, uint32_t K,
  * no token; sums: the rows of the tokens, the sorted pairs in `chunks` chunks of
  * `chunk` (the last may be shorter), at most VKB_EMBED_CHUNKS, part chunks x 2 x
  * N floats.
- * direct: all of it in one launch, for up to VKBLAS_EMBEDDING_SMALL rows. */
+ * direct: all of it in one launch, for up to VKBLAS_EMBEDDING_SMALL rows and a dw
+ * of up to VKBLAS_EMBEDDING_SMALL_BYTES. */
 int vkb_launch_embedding_direct(int type, int w_type, uint32_t M, uint32_t V, uint32_t N, const int64_t* ids,
                                 int64_t pad, const void* dy, int64_t lddy, float scale, void* dw, int64_t lddw,
                                 float beta, void* stream);
