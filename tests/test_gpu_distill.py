@@ -210,6 +210,25 @@ def test_extreme_logits():
     assert bool((zt[:, 1] == -float("inf")).all())
 
 
+@pytest.mark.parametrize("tt,dt", [("f32", "f32"), ("f32", "f16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("temp", [0.25, 1.0])
+def test_teachers_lowest_values_over_a_small_temperature(tt, dt, temp):
+    """Logits that leave the type's range once they are over the temperature count by their differences, as others of
+    the same differences do, in both passes."""
+    M, V, K, n = 9, 300, 64, 6
+    x, w, top, t, lse, dloss = grad_inputs(M, V, K, n, dt, temp, tt)
+    top, top[5, 2] = torch.arange(7, 7 + n).repeat(M, 1), -1
+    high = torch.finfo(R.TORCH[tt]).max
+    results = []
+    for level in (0.0, -high, high):
+        t = torch.full((M, n), level, dtype=torch.float64)
+        t[1::2, 3] = -torch.inf if level <= 0.0 else -high
+        results.append((*forward(x, w, top, t, temp, dt, tt),
+                        *backward(x, w, top, t, lse, dloss, temp, dt, tt)))
+        assert all(bool(torch.isfinite(r).all()) for r in results[-1])
+        assert all(torch.equal(a, b) for a, b in zip(results[-1], results[0]))
+
+
 @pytest.mark.parametrize("loss_scale", [1e-12, 1.0, 1e20])
 def test_fp16_gradients_of_any_size(loss_scale):
     args = grad_inputs(60, 400, 64, 20, "f16", 4.0, loss_scale=loss_scale)

@@ -19,13 +19,14 @@ constexpr uint32_t TOP = VKBLAS_DISTILL_TOP, WAVES = WORK / 64;
 
 constexpr int ABSENT = -1, BAD = -2, NONE = -3;
 struct Shared {
-    float q[TOP];            // the teacher's logits over T, then its probabilities
+    float q[TOP];            // the teacher's logits, then over T, then its probabilities
     __attribute__((aligned(16))) int id[TOP];      // class, or ABSENT, or BAD; NONE up to a whole quad
     float high[WAVES], sum[WAVES];
     uint32_t flags[WAVES];
 };
 
-// A row's entries into LDS: classes, and t / T less the largest.  Returns the
+// A row's entries into LDS: classes, and t / T less the largest (the difference
+// first: t of the type's lowest value over a T below 1 is no -inf).  Returns the
 // log of their sum of exponentials.  counted: some entry is there and not of
 // probability 0 (a NaN is not); bad: some class is past V.
 template <typename TT>
@@ -36,7 +37,7 @@ __device__ __forceinline__ float teacher(uint32_t n, uint32_t V, const int64_t* 
     bool any = false, past = false;
     for (uint32_t j = threadIdx.x; j < (n + 3) / 4 * 4; j += WORK) {
         const int64_t c = j < n ? top[j] : -1;
-        const float v = c < 0 ? -INFINITY : (float)t[j] * inv_t;
+        const float v = c < 0 ? -INFINITY : (float)t[j];
         sh.id[j] = j >= n ? NONE : c < 0 ? ABSENT : c < V ? (int)c : BAD;
         if (j < n) sh.q[j] = v;
         any |= !(v == -INFINITY);
@@ -60,7 +61,7 @@ __device__ __forceinline__ float teacher(uint32_t n, uint32_t V, const int64_t* 
     if (high == -INFINITY) high = 0.0f;
     float s = 0.0f;
     for (uint32_t j = threadIdx.x; j < n; j += WORK) {
-        sh.q[j] -= high;
+        sh.q[j] = (sh.q[j] - high) * inv_t;
         s += fast_exp(sh.q[j]);
     }
     s = wave_sum(s);
