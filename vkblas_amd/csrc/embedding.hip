@@ -27,6 +27,9 @@ namespace {
 
 constexpr uint32_t RUN = VKB_EMBED_RUN, WAYS = VKB_EMBED_WAYS;
 
+// Bound by its reads and writes: fp32 to bf16 16384 x 4096, 403 MB, 44 us (9.2 TB/s: a
+// frequent token's row comes out of the caches).  One chunk a thread, many short
+// workgroups: 8192 in strides 47 us.
 template <typename T, typename W>
 __global__ __launch_bounds__(WORK) void lookup_kernel(uint32_t M, uint32_t V, uint32_t N, const int64_t* ids,
                                                       int64_t pad, const W* w, int64_t ldw, float scale, T* y,
@@ -57,12 +60,13 @@ __device__ __forceinline__ uint32_t sort_key(int64_t id, int64_t pad, uint32_t V
 // RTOK tokens of a run per workgroup, 16 groups of threads on a part of the
 // run's keys each.  A pair before the token's counts where its key is at most
 // the token's, one after it where it is less.
-constexpr uint32_t RTOK = 16, RGROUPS = WORK / RTOK;
 //
 // The workgroups from ranks on zero dw, 16 bytes a thread: stores are fastest
 // from many short workgroups (1 GiB of zeros: 4 KB each 6.8 TB/s, 8 KB 6.1, 512 KB 5.7,
 // 8192 workgroups in strides 4.6; rows with tokens left out, which takes a look at
-// a map of them, 4.6 beside the sums).
+// a map of them, 4.6 beside the sums).  16384 tokens' ranks take 8 us by themselves, and
+// beside 1 GB of zeros, 150 us, nothing.
+constexpr uint32_t RTOK = 16, RGROUPS = WORK / RTOK;
 template <typename W>
 __global__ __launch_bounds__(WORK) void rank_kernel(uint32_t M, uint32_t V, const int64_t* ids, int64_t pad,
                                                     uint32_t* key, uint32_t* order, uint32_t ranks, uint32_t N, W* dw,
@@ -335,9 +339,11 @@ __device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__bui
 // listed in order of m.  A row with up to HEAVY is a wave's, one with more all
 // waves' on a part of the list each.  Rows without one are zeroed or scaled in
 // all of their columns, by the workgroups of the same rows in turn.
-// Against the sort and its three launches (us, sorted / so, bf16): 2048 x 32000 x
-// 1024 29.5 / 18.5, 4096 x 32000 x 1024 30 / 23, 4096 x 500 x 512 21 / 12, and with
-// three tokens in ten the same 35 / 42; all of 4096 the same 41 / 81.
+// Against the sort and its launches (us, sorted / so): bf16 64 x 1000 x 512 11.1 / 6.6,
+// 1024 x 32000 x 1024 18.5 / 17.7, 4096 x 32000 x 1024 25.1 / 22.7, 4096 x 500 x 512
+// 19.5 / 12.8, fp32 1003 x 997 x 515 12.3 / 7.4, 4096 x 16000 x 1024 25.7 / 26.4; where
+// few tokens fill the batch the sort is ahead, three in ten of 4096 the same 35 / 42,
+// all of them 41 / 81.
 constexpr uint32_t DIRECT = VKBLAS_EMBEDDING_SMALL, DTHREADS = 512, DWAVES = DTHREADS / 64;
 constexpr uint32_t DROWS = 4096, HEAVY = 8;   // DROWS: the most rows of a workgroup
 struct DirectParams {
@@ -493,7 +499,10 @@ struct SumParams {
     float* part;             // chunks x 2 x N: what began before a chunk, what goes on after it
 };
 
-// A wave: one chunk, 64 x 16 bytes of its rows' columns.
+// A wave: one chunk, 64 x 16 bytes of its rows' columns, ROWS of dy's rows in
+// flight.  bf16 16384 x 4096 into a vocabulary of 128000: 63 us for 134 MB of dy and
+// 70 MB of sums and parts, which leave after the zeros' 1 GB has gone through the
+// caches.
 template <typename T, typename W, typename COLS>
 __device__ __forceinline__ void sum_chunk(const SumParams& p, const COLS& cols, uint32_t chunk) {
     constexpr int VEC = Elem<T>::VEC;
@@ -699,11 +708,11 @@ extern "C" int vkb_launch_embedding_direct(int type, int w_type, uint32_t M, uin
         using W = decltype(o);
         // half the steps for half the tokens: fp32 1003 x 997 x 515 9.1 -> 7.7 us
         if (M <= DIRECT / 2)
-            hipLaunchKernelGGL((direct_kernel<T, W, DIRECT / 2 / DTHREADS>), dim3((uint32_t)ranges, blocks), dim3(DTHREADS),
-                               0, (hipStream_t)stream, p);
+            hipLaunchKernelGGL((direct_kernel<T, W, DIRECT / 2 / DTHREADS>), dim3((uint32_t)ranges, blocks),
+                               dim3(DTHREADS), 0, (hipStream_t)stream, p);
         else
-            hipLaunchKernelGGL((direct_kernel<T, W, DIRECT / DTHREADS>), dim3((uint32_t)ranges, blocks), dim3(DTHREADS), 0,
-                               (hipStream_t)stream, p);
+            hipLaunchKernelGGL((direct_kernel<T, W, DIRECT / DTHREADS>), dim3((uint32_t)ranges, blocks),
+                               dim3(DTHREADS), 0, (hipStream_t)stream, p);
     });
     return ok ? (int)hipGetLastError() : (int)hipErrorInvalidValue;
 }
@@ -715,21 +724,21 @@ extern "C" int vkb_launch_embedding_rank(uint32_t M, uint32_t V, const int64_t* 
     const bool ok = with_type(w_type, [&](auto t) {
         using W = decltype(t);
         const uint32_t fill = dw ? blocks_of((uint64_t)V * chunks_of<W>(N)) : 0;
-        hipLaunchKernelGGL((rank_kernel<W>), dim3(ranks + fill), dim3(WORK), 0, (hipStream_t)stream, M, V, ids, pad, key,
-                           order, ranks, N, (W*)dw, lddw);
+        hipLaunchKernelGGL((rank_kernel<W>), dim3(ranks + fill), dim3(WORK), 0, (hipStream_t)stream, M, V, ids, pad,
+                           key, order, ranks, N, (W*)dw, lddw);
     });
     return ok ? (int)hipGetLastError() : (int)hipErrorInvalidValue;
 }
 
-extern "C" int vkb_launch_embedding_merge_runs(uint32_t M, const uint32_t* key_in, const uint32_t* order_in, uint32_t* key,
-                                               uint32_t* order, void* stream) {
+extern "C" int vkb_launch_embedding_merge_runs(uint32_t M, const uint32_t* key_in, const uint32_t* order_in,
+                                               uint32_t* key, uint32_t* order, void* stream) {
     const uint32_t blocks = (uint32_t)(((uint64_t)M + WORK - 1) / WORK);
     if (M <= RUN * WAYS)
-        hipLaunchKernelGGL((merge_runs_kernel<1>), dim3(blocks), dim3(WORK), 0, (hipStream_t)stream, M, key_in, order_in,
-                           key, order);
+        hipLaunchKernelGGL((merge_runs_kernel<1>), dim3(blocks), dim3(WORK), 0, (hipStream_t)stream, M, key_in,
+                           order_in, key, order);
     else
-        hipLaunchKernelGGL((merge_runs_kernel<4>), dim3(blocks), dim3(WORK), 0, (hipStream_t)stream, M, key_in, order_in,
-                           key, order);
+        hipLaunchKernelGGL((merge_runs_kernel<4>), dim3(blocks), dim3(WORK), 0, (hipStream_t)stream, M, key_in,
+                           order_in, key, order);
     return (int)hipGetLastError();
 }
 
@@ -767,7 +776,8 @@ extern "C" int vkb_launch_embedding_sums(int type, int w_type, const vkb_embeddi
         hipLaunchKernelGGL((sum_kernel<T, W>), dim3((uint32_t)sums), dim3(WORK), 0, (hipStream_t)stream, p);
         rc = (int)hipGetLastError();
         if (rc != 0 || p.chunks == 1) return;
-        hipLaunchKernelGGL((join_kernel<T, W>), dim3(p.blocks, p.chunks - 1), dim3(JTHREADS), 0, (hipStream_t)stream, p);
+        hipLaunchKernelGGL((join_kernel<T, W>), dim3(p.blocks, p.chunks - 1), dim3(JTHREADS), 0, (hipStream_t)stream,
+                           p);
         rc = (int)hipGetLastError();
     });
     return rc;

@@ -657,7 +657,9 @@ static int distill_rows(op_call* c, vkblas_dtype_t type, uint32_t K, teacher_row
 }
 /* A distillation's rows join their parts themselves up to this many, which saves
  * the launch of the kernel that reads eight rows' at a time (us, with that kernel
- * / without: f16 300 x 32003 x 1024 40.6 / 36.9). */
+ * / without: f16 300 x 2003 x 256 14.7 / 12.7, 300 x 32003 x 1024 40.0 / 38.4, bf16 2048
+ * x 32000 x 1024 129.3 / 128.9; more parts 1000 x 128000 x 1024 241 / 246, 8192 x 128000
+ * x 64 569 / 593). */
 #define JOIN_PARTS (1u << 18)
 
 /* lse of each row's logits times inv_t, and its loss (target NULL: none) or (q)
@@ -961,8 +963,8 @@ static int distill_args(vkblas_dtype_t type, uint32_t M, uint32_t V, uint32_t K,
 
 vkblas_status_t vkblas_linear_distill_async(vkblas_dtype_t type, uint32_t M, uint32_t V, uint32_t K, const void* x,
                                             uint32_t ldx, const void* w, uint32_t ldw, uint32_t n_top,
-                                            const int64_t* top, uint32_t ldtop, vkblas_dtype_t t_type, const void* t, uint32_t ldt,
-                                            float temperature, float* loss, float* lse, float* z_top, void* stream) {
+                                            const int64_t* top, uint32_t ldtop, vkblas_dtype_t t_type,
+                                            const void* t, uint32_t ldt, float temperature, float* loss, float* lse, float* z_top, void* stream) {
     if (!distill_args(type, M, V, K, ldx, ldw, n_top, ldtop, t_type, ldt, temperature)) return VKBLAS_ERR_PARAM;
     if (M == 0) return VKBLAS_OK;
     if (!x || !w || !top || !t || !loss || !lse || !z_top) return VKBLAS_ERR_PARAM;
@@ -1033,8 +1035,8 @@ vkblas_status_t vkblas_embedding_backward_async(vkblas_dtype_t type, uint32_t M,
     if (vkb_engine_trace()) fprintf(stderr, "[vkblas] embedding_backward type=%d M=%u V=%u N=%u\n", (int)type, M, V, N);
     /* one launch, but for a large dw: its workgroups then have many rows each, and the
      * zeros a bad pattern of stores (us, one launch / sorted, bf16: 1024 x 32000 x 1024,
-     * 66 MB, 17.6 / 28; 1000 x 64000 x 1024 38 / 30; 1 x 128000 x 4096 186 / 156;
-     * 4000 x 128000 x 4096 218 / 183) */
+     * 66 MB, 17.7 / 18.5; 1000 x 64000 x 1024 38 / 30; 1 x 128000 x 4096 221 / 156;
+     * 4000 x 128000 x 4096 315 / 182) */
     if (M <= VKBLAS_EMBEDDING_SMALL && N <= 65535u * 256u &&
         (uint64_t)V * N * type_size(dw_type) <= VKBLAS_EMBEDDING_SMALL_BYTES) {
         if (room(&c) != VKBLAS_OK) return c.st;
@@ -1042,8 +1044,9 @@ vkblas_status_t vkblas_embedding_backward_async(vkblas_dtype_t type, uint32_t M,
              1);
         return op_end(&c, VKBLAS_KERNEL_EMBED);
     }
-    /* chunks of 8 pairs, or as many as leave 4096 waves: a token that ends in
-     * another chunk than it began in goes by the workspace */
+    /* chunks of 8 pairs, or as many as leave 4096 waves (us, 4096 / 8192: 16384 x 128000
+     * x 4096 226 / 230, 41249 x 446 x 6978 176 / 168): a token that ends in another
+     * chunk than it began in goes by the workspace */
     vkb_embedding_sums a = {.M = M, .V = V, .N = N, .dy = dy, .lddy = lddy, .dw = dw, .lddw = lddw, .scale = scale,
                             .beta = beta};
     const uint32_t cols = type == VKBLAS_DT_F32 ? 256 : 512;
@@ -1101,8 +1104,8 @@ static int policy_args(uint32_t B, uint32_t T, const float* logp, uint32_t ldp, 
 }
 
 vkblas_status_t vkblas_policy_loss_async(vkblas_reduce_t reduce, uint32_t B, uint32_t T, const float* logp,
-                                         uint32_t ldp, const float* old_logp, uint32_t ldo, const float* ref_logp, uint32_t ldr,
-                                         const float* adv, uint32_t ldadv, uint32_t adv_step, const uint8_t* mask,
+                                         uint32_t ldp, const float* old_logp, uint32_t ldo,
+                                         const float* ref_logp, uint32_t ldr, const float* adv, uint32_t ldadv, uint32_t adv_step, const uint8_t* mask,
                                          uint32_t ldmask, float clip_low, float clip_high, float kl_coef, float* stats,
                                          float* norm, void* stream) {
     vkb_policy p;

@@ -1,12 +1,18 @@
 // policy.hip — clipped policy loss with a KL term on token log probabilities.
 //
 // A token's loss is a few operations on four or five floats, so the loss over a
-// batch is a pass over its arrays and a sum.  A wave takes a unit, a part of a
-// sequence, four tokens a lane at a time, and skips the arrays where no token
-// of a lane's four counts: the padding behind a sequence costs its mask alone.
-// A token's terms are fp32; sums are fp64, and so is logp - old, on which the
-// side of a bound depends: r > 1 + clip_high exactly where logp - old >
-// log(1 + clip_high).
+// batch is a pass over its arrays and a sum, bound by the reads: 13 to 17 bytes
+// a token.  A workgroup takes a unit, a sequence or a part of one (a wave where
+// sequences have up to 256 tokens), four tokens a lane at a time, and skips the
+// arrays where no token of a lane's four counts: the padding behind a sequence
+// costs its mask alone.  A token's terms are fp32; sums are fp64, and so is logp -
+// old, on which the side of a bound depends: r > 1 + clip_high exactly where
+// logp - old > log(1 + clip_high).
+//
+// 1024 sequences of 8192 tokens, half of them padding: 20.8 us (3.6 TB/s of the
+// bytes that it reads) and 5.8 for the finish, one workgroup over 2048 units; the
+// gradient, which writes the padding's zeros too, 20 us (5.4 TB/s).  A call of up to 16 units of 256 tokens is one workgroup,
+// 7.2 us with its launch.
 #include "nn_common.hpp"
 
 namespace vkb {
@@ -129,12 +135,28 @@ __device__ __forceinline__ double wave_sum(double v) {
     return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 
-// A wave's sums over the tokens of sequence b from t0 + 4 lane on, four every
+// A count's, likewise
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_add(uint32_t v) {
+    return v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ uint32_t wave_sum(uint32_t v) {
+    v = dpp_add<0x111, 0xf>(v);
+    v = dpp_add<0x112, 0xf>(v);
+    v = dpp_add<0x114, 0xf>(v);
+    v = dpp_add<0x118, 0xf>(v);
+    v = dpp_add<0x142, 0xa>(v);
+    v = dpp_add<0x143, 0xc>(v);
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+
+// A lane's sums over the tokens of sequence b from t0 + 4 lane on, four every
 // `step`, below t1; the masks of AHEAD rounds are read before their arrays.
 // Tokens that do not count become ones whose terms are 0.  Four tokens are added
 // in fp32, as good as the terms themselves, and their sum in fp64.
 constexpr int AHEAD = 2;
-__device__ __forceinline__ Sums token_sums(const vkb_policy& p, int64_t b, int64_t t0, int64_t t1, int64_t step, int lane) {
+__device__ __forceinline__ Sums lane_sums(const vkb_policy& p, int64_t b, int64_t t0, int64_t t1, int64_t step,
+                                          int lane) {
     Sums s = zero_sums();
     uint32_t tokens = 0, sides = 0;
     const bool by_kl = p.ref && p.kl != 0.0f;    // (0 * inf adds nothing)
@@ -174,25 +196,64 @@ __device__ __forceinline__ Sums token_sums(const vkb_policy& p, int64_t b, int64
         else rounds(std::false_type{}, t + 4 * lane);
     s.v[2] = (double)sides;
     s.v[4] = (double)tokens;
+    return s;
+}
+// ... a wave's
+__device__ __forceinline__ Sums token_sums(const vkb_policy& p, int64_t b, int64_t t0, int64_t t1, int64_t step,
+                                           int lane) {
+    Sums s = lane_sums(p, b, t0, t1, step, lane);
 #pragma unroll
     for (int i = 0; i < NSUM; ++i) s.v[i] = wave_sum(s.v[i]);
     return s;
 }
 
-// The workgroup over the units' sums (part: NSUM arrays of `count`): each
-// sequence's by a group of lanes, as many as B leaves of the threads, then all
-// sequences' by the reduction's weights.
+// What sequences sum to, by the reduction's weights, and those that have tokens
+struct Total {
+    double v[NSUM + 1];
+};
+__device__ __forceinline__ void add_sequence(Total& t, const double* s, int reduce) {
+    if (s[4] == 0.0) return;
+    const double by = reduce == VKBLAS_REDUCE_SEQUENCES ? 1.0 / s[4] : 1.0;
+#pragma unroll
+    for (int i = 0; i < NSUM; ++i) t.v[i] += s[i] * by;
+    t.v[NSUM] += 1.0;
+}
+// The threads' totals joined: stats (write), and the batch's weight
 constexpr uint32_t FIN = 1024;
+__device__ __forceinline__ double settle(Total t, int reduce, bool write, float* stats, double (*sh)[FIN / 64]) {
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int i = 0; i <= NSUM; ++i) {
+        t.v[i] = wave_sum(t.v[i]);
+        if (lane == 0) sh[i][wave] = t.v[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i <= NSUM; ++i) t.v[i] = wave_sum(lane < blockDim.x / 64 ? sh[i][lane] : 0.0);
+    const double some = t.v[NSUM];
+    const double weight = some == 0.0 ? 0.0 : reduce == VKBLAS_REDUCE_SUM ? 1.0
+                        : reduce == VKBLAS_REDUCE_TOKENS ? 1.0 / t.v[4] : 1.0 / some;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (write && threadIdx.x == (uint32_t)i) stats[i] = (float)(t.v[i] * weight);
+    return weight;
+}
+__device__ __forceinline__ float norm_of(double tokens, double weight, int reduce) {
+    return (float)(tokens == 0.0 ? 0.0 : reduce == VKBLAS_REDUCE_SEQUENCES ? weight / tokens : weight);
+}
+
+// The workgroup over the units' sums (part: NSUM arrays of `count`): each
+// sequence's by a group of lanes, as many as B leaves of the threads.
 struct Shared {
     double waves[NSUM + 1][FIN / 64], tokens[FIN];       // tokens: of the first FIN sequences
 };
 __device__ __forceinline__ void finish(uint32_t B, uint32_t units, int reduce, const double* part, uint64_t count,
                                        float* stats, float* norm, Shared& sh) {
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, threads = blockDim.x;
+    const uint32_t threads = blockDim.x;
     uint32_t G = 1;
     while (G < 64 && G < units && 2 * G * B <= threads) G *= 2;
     const uint32_t at = threadIdx.x / G, in = threadIdx.x % G;
-    double total[NSUM + 1] = {0.0, 0.0, 0.0, 0.0, 0.0, 0.0};             // the last: sequences with tokens
+    Total total = {};
     for (uint64_t b = at; b < B; b += threads / G) {
         double s[NSUM] = {0.0, 0.0, 0.0, 0.0, 0.0};
 #pragma unroll 4
@@ -203,57 +264,36 @@ __device__ __forceinline__ void finish(uint32_t B, uint32_t units, int reduce, c
 #pragma unroll
             for (int i = 0; i < NSUM; ++i) s[i] += __shfl_xor(s[i], (int)d);
         if (in == 0 && b < FIN) sh.tokens[b] = s[4];
-        if (in || s[4] == 0.0) continue;
-        const double by = reduce == VKBLAS_REDUCE_SEQUENCES ? 1.0 / s[4] : 1.0;
-#pragma unroll
-        for (int i = 0; i < NSUM; ++i) total[i] += s[i] * by;
-        total[NSUM] += 1.0;
+        if (in == 0) add_sequence(total, s, reduce);
     }
-#pragma unroll
-    for (int i = 0; i <= NSUM; ++i) {
-        total[i] = wave_sum(total[i]);
-        if (lane == 0) sh.waves[i][wave] = total[i];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i <= NSUM; ++i) total[i] = wave_sum(lane < threads / 64 ? sh.waves[i][lane] : 0.0);
-    const double some = total[NSUM];
-    const double weight = some == 0.0 ? 0.0 : reduce == VKBLAS_REDUCE_SUM ? 1.0
-                        : reduce == VKBLAS_REDUCE_TOKENS ? 1.0 / total[4] : 1.0 / some;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (threadIdx.x == (uint32_t)i) stats[i] = (float)(total[i] * weight);
+    const double weight = settle(total, reduce, true, stats, sh.waves);
     for (uint64_t b = threadIdx.x; b < B; b += threads) {
         double n = 0.0;
         if (b < FIN) n = sh.tokens[b];
         else
             for (uint32_t u = 0; u < units; ++u) n += part[4 * count + b * units + u];
-        norm[b] = (float)(n == 0.0 ? 0.0 : reduce == VKBLAS_REDUCE_SEQUENCES ? weight / n : weight);
+        norm[b] = norm_of(n, weight, reduce);
     }
 }
 
-// Units of a wave (sequences of up to 256 tokens) or of a workgroup's four
-template <bool SHORT>
+// Sequences of several units, one a workgroup
+constexpr uint32_t WAVES = WORK / 64;
 __global__ __launch_bounds__(WORK) void unit_kernel(vkb_policy p, double* part) {
-    constexpr uint32_t WAVES = WORK / 64;
     __shared__ double sh[WAVES][NSUM];
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint64_t count = (uint64_t)p.B * p.units, step = (uint64_t)gridDim.x * (SHORT ? WAVES : 1);
-    for (uint64_t unit = SHORT ? (uint64_t)blockIdx.x * WAVES + wave : blockIdx.x; unit < count; unit += step) {
+    const uint64_t count = (uint64_t)p.B * p.units;
+    for (uint64_t unit = blockIdx.x; unit < count; unit += gridDim.x) {
         const int64_t b = (int64_t)(unit / p.units), t0 = (int64_t)(unit % p.units) * p.unit;
-        const int64_t t1 = min(t0 + p.unit, (int64_t)p.T);
-        Sums s = token_sums(p, b, SHORT ? t0 : t0 + 256 * wave, t1, SHORT ? 256 : 256 * WAVES, lane);
-        if (!SHORT) {
-            __syncthreads();                 // the unit before is read
+        Sums s = token_sums(p, b, t0 + 256 * wave, min(t0 + p.unit, (int64_t)p.T), 256 * WAVES, lane);
+        __syncthreads();                     // the unit before is read
 #pragma unroll
-            for (int i = 0; i < NSUM; ++i)
-                if (lane == 0) sh[wave][i] = s.v[i];
-            __syncthreads();
-            if (wave) continue;
+        for (int i = 0; i < NSUM; ++i)
+            if (lane == 0) sh[wave][i] = s.v[i];
+        __syncthreads();
+        if (wave) continue;
 #pragma unroll
-            for (int i = 0; i < NSUM; ++i)
-                for (uint32_t w = 1; w < WAVES; ++w) s.v[i] += sh[w][i];
-        }
+        for (int i = 0; i < NSUM; ++i)
+            for (uint32_t w = 1; w < WAVES; ++w) s.v[i] += sh[w][i];
 #pragma unroll
         for (int i = 0; i < NSUM; ++i)
             if (lane == (uint32_t)i) part[i * count + unit] = s.v[i];
@@ -263,6 +303,69 @@ __global__ __launch_bounds__(FIN) void finish_kernel(vkb_policy p, int reduce, c
                                                      float* norm) {
     __shared__ Shared sh;
     finish(p.B, p.units, reduce, part, (uint64_t)p.B * p.units, stats, norm, sh);
+}
+
+// Sequences of one unit: a wave's (SHORT, up to 256 tokens) or a workgroup's
+// own.  Their tokens are counted, and each lane adds its sums by the
+// reduction's weight: lanes and waves are joined once for all of a workgroup's
+// sequences, and the finish reads as many totals as there are workgroups
+// (part: NSUM + 1 arrays of those, then each sequence's tokens).  Against each
+// sequence's five sums to memory and one workgroup over them (us): 65536 x 128
+// 115 -> 52, 16384 x 1024 71 -> 61, 8192 x 256 22 -> 16.  What is left at many short
+// sequences is arithmetic, a wave's whatever its lanes hold.
+template <bool SHORT>
+__global__ __launch_bounds__(WORK) void whole_kernel(vkb_policy p, int reduce, double* part) {
+    __shared__ double totals[WAVES][NSUM + 1];
+    __shared__ uint32_t counts[2][WAVES];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    double* tokens = part + (NSUM + 1) * (uint64_t)gridDim.x;
+    Total total = {};
+    uint32_t turn = 0;
+    for (uint64_t b = SHORT ? (uint64_t)blockIdx.x * WAVES + wave : blockIdx.x; b < p.B;
+         b += (uint64_t)gridDim.x * (SHORT ? WAVES : 1)) {
+        const Sums s = lane_sums(p, (int64_t)b, SHORT ? 0 : 256 * wave, p.T, SHORT ? 256 : 256 * WAVES, lane);
+        uint32_t n = wave_sum((uint32_t)s.v[4]);
+        if (!SHORT) {
+            if (lane == 0) counts[turn][wave] = n;
+            __syncthreads();             // (one a sequence: the next one's counts go to the other half)
+            n = 0;
+            for (uint32_t w = 0; w < WAVES; ++w) n += counts[turn][w];
+            turn ^= 1;
+        }
+        const bool first = lane == 0 && (SHORT || wave == 0);
+        if (first) tokens[b] = (double)n;
+        if (n == 0) continue;
+        const double by = reduce == VKBLAS_REDUCE_SEQUENCES ? 1.0 / (double)n : 1.0;
+#pragma unroll
+        for (int i = 0; i < NSUM; ++i) total.v[i] += s.v[i] * by;
+        total.v[NSUM] += first ? 1.0 : 0.0;
+    }
+#pragma unroll
+    for (int i = 0; i <= NSUM; ++i) {
+        total.v[i] = wave_sum(total.v[i]);
+        if (lane == 0) totals[wave][i] = total.v[i];
+    }
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int i = 0; i <= NSUM; ++i) {
+        for (uint32_t w = 1; w < WAVES; ++w) total.v[i] += totals[w][i];
+        if (lane == (uint32_t)i) part[i * (uint64_t)gridDim.x + blockIdx.x] = total.v[i];
+    }
+}
+// Every workgroup adds the `count` totals, and writes its part of norm
+__global__ __launch_bounds__(FIN) void whole_finish_kernel(uint32_t B, int reduce, const double* part, uint32_t count,
+                                                           float* stats, float* norm) {
+    __shared__ double sh[NSUM + 1][FIN / 64];
+    Total total = {};
+#pragma unroll 2
+    for (uint32_t j = threadIdx.x; j < count; j += FIN)
+#pragma unroll
+        for (int i = 0; i <= NSUM; ++i) total.v[i] += part[(uint64_t)i * count + j];
+    const double weight = settle(total, reduce, blockIdx.x == 0, stats, sh);
+    const double* tokens = part + (NSUM + 1) * (uint64_t)count;
+    for (uint64_t b = (uint64_t)blockIdx.x * FIN + threadIdx.x; b < B; b += (uint64_t)gridDim.x * FIN)
+        norm[b] = norm_of(tokens[b], weight, reduce);
 }
 // A small call: units of 256 tokens, their sums in LDS
 constexpr uint32_t SMALL = VKBLAS_POLICY_SMALL / 256;
@@ -279,6 +382,8 @@ __global__ __launch_bounds__(FIN) void small_kernel(vkb_policy p, int reduce, fl
     finish(p.B, units, reduce, part, n, stats, norm, sh);
 }
 
+// Four tokens a thread; dlogp is written whole, so the floor counts 4 bytes a
+// token more
 __global__ __launch_bounds__(WORK) void grad_kernel(vkb_policy p, const float* norm, const float* dloss, float* dlogp,
                                                     int64_t lddp) {
     const float dl = dloss[0];
@@ -322,28 +427,48 @@ extern "C" void vkb_policy_units(vkb_policy* p) {
 }
 // One wave each for up to 16 units of 256
 static uint64_t small_units(const vkb_policy* p) { return (uint64_t)p->B * (((uint64_t)p->T + 255) / 256); }
+// Workgroups of sequences of one unit (us for 512 / 1024 / 2048 / 4096 of them:
+// 65536 x 128 81 / 52 / 52 / 53, 4096 x 4096 73 / 49 / 48 / 47)
+constexpr uint32_t WHOLE_BLOCKS = 2048;
+static uint32_t whole_blocks(const vkb_policy* p) {
+    const uint32_t n = p->T <= 256 ? (p->B + WAVES - 1) / WAVES : p->B;
+    return n < WHOLE_BLOCKS ? n : WHOLE_BLOCKS;
+}
 extern "C" size_t vkb_policy_part_bytes(const vkb_policy* p) {
-    return small_units(p) <= SMALL ? 0 : (size_t)p->B * p->units * sizeof(Sums);   // as NSUM arrays
+    if (small_units(p) <= SMALL) return 0;
+    if (p->units == 1) return ((size_t)whole_blocks(p) * (NSUM + 1) + p->B) * sizeof(double);
+    return (size_t)p->B * p->units * sizeof(Sums);   // as NSUM arrays
 }
 
 extern "C" int vkb_launch_policy(const vkb_policy* p, int reduce, void* part, float* stats, float* norm, void* stream) {
     if (!part) {
         static_assert(SMALL <= FIN / 64, "a wave for each unit");
         if (small_units(p) > SMALL) return (int)hipErrorInvalidValue;
-        hipLaunchKernelGGL(small_kernel, dim3(1), dim3(64 * (uint32_t)small_units(p)), 0, (hipStream_t)stream, *p, reduce,
-                           stats, norm);
+        hipLaunchKernelGGL(small_kernel, dim3(1), dim3(64 * (uint32_t)small_units(p)), 0, (hipStream_t)stream, *p,
+                           reduce, stats, norm);
         return (int)hipGetLastError();
     }
-    const uint64_t count = (uint64_t)p->B * p->units, blocks = p->T <= 256 ? (count + WORK / 64 - 1) / (WORK / 64) : count;
-    const dim3 grid((uint32_t)(blocks < 1u << 20 ? blocks : 1u << 20));
-    if (p->T <= 256)
-        hipLaunchKernelGGL((unit_kernel<true>), grid, dim3(WORK), 0, (hipStream_t)stream, *p, (double*)part);
+    const bool whole = p->units == 1;
+    const uint32_t blocks = whole_blocks(p);
+    const uint64_t count = (uint64_t)p->B * p->units;
+    if (whole && p->T <= 256)
+        hipLaunchKernelGGL((whole_kernel<true>), dim3(blocks), dim3(WORK), 0, (hipStream_t)stream, *p, reduce,
+                           (double*)part);
+    else if (whole)
+        hipLaunchKernelGGL((whole_kernel<false>), dim3(blocks), dim3(WORK), 0, (hipStream_t)stream, *p, reduce,
+                           (double*)part);
     else
-        hipLaunchKernelGGL((unit_kernel<false>), grid, dim3(WORK), 0, (hipStream_t)stream, *p, (double*)part);
+        hipLaunchKernelGGL(unit_kernel, dim3((uint32_t)(count < 1u << 20 ? count : 1u << 20)), dim3(WORK), 0,
+                           (hipStream_t)stream, *p, (double*)part);
     const int rc = (int)hipGetLastError();
     if (rc != 0) return rc;
-    hipLaunchKernelGGL(finish_kernel, dim3(1), dim3(FIN), 0, (hipStream_t)stream, *p, reduce, (const double*)part, stats,
-                       norm);
+    const uint32_t n = (uint32_t)(((uint64_t)p->B + FIN - 1) / FIN);
+    if (whole)
+        hipLaunchKernelGGL(whole_finish_kernel, dim3(n < 64 ? n : 64), dim3(FIN), 0, (hipStream_t)stream, p->B, reduce,
+                           (const double*)part, blocks, stats, norm);
+    else
+        hipLaunchKernelGGL(finish_kernel, dim3(1), dim3(FIN), 0, (hipStream_t)stream, *p, reduce, (const double*)part,
+                           stats, norm);
     return (int)hipGetLastError();
 }
 

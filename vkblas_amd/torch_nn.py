@@ -253,8 +253,8 @@ class _LinearDistillation(torch.autograd.Function):
         with torch.cuda.device(m.device):
             vk.linear_distill_backward_async(_TYPES[m.dtype], m.shape[0], w.shape[0], m.shape[1], _ptr(m), _ld(m),
                                              _ptr(w), _ld(w), c.shape[1], _ptr(c), _ld(c), _TYPES[t.dtype], _ptr(t),
-                                             _ld(t), ctx.temperature, _ptr(lse), _ptr(z_top), _ptr(d), _ptr(dx), m.shape[1],
-                                             _ptr(dw), m.shape[1], _TYPES[w.dtype], 0.0, stream=_stream(m))
+                                             _ld(t), ctx.temperature, _ptr(lse), _ptr(z_top), _ptr(d), _ptr(dx),
+                                             m.shape[1], _ptr(dw), m.shape[1], _TYPES[w.dtype], 0.0, stream=_stream(m))
         return dx.view(ctx.x_shape) if dx is not None else None, dw, None, None, None
 
 
