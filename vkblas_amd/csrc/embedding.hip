@@ -27,8 +27,9 @@ namespace {
 
 constexpr uint32_t RUN = VKB_EMBED_RUN, WAYS = VKB_EMBED_WAYS;
 
-// Bound by its reads and writes: fp32 to bf16 16384 x 4096, 403 MB, 44 us (9.2 TB/s: a
-// frequent token's row comes out of the caches).  One chunk a thread, many short
+// Bound by its reads and writes: fp32 to bf16 16384 x 4096, 403 MB, 45 us (164 MB of
+// the 268 that it reads come from HBM, a frequent token's row out of the caches: 6.6
+// TB/s).  One chunk a thread, many short
 // workgroups: 8192 in strides 47 us.
 template <typename T, typename W>
 __global__ __launch_bounds__(WORK) void lookup_kernel(uint32_t M, uint32_t V, uint32_t N, const int64_t* ids,
