@@ -102,7 +102,7 @@ def check_grad(got, i, norm, dloss, low=LOW, high=HIGH, kl=KL):
 # units of 256 tokens, the small call of 64 of them (one workgroup) and past it, many units of a sequence
 SIZES = [(1, 1), (1, 5), (3, 64), (8, 100), (2, 255), (2, 256), (2, 257), (64, 256), (65, 256), (63, 257), (1, 16384),
          (1, 16385), (16, 256), (17, 256), (15, 257), (2, 40001), (300, 700), (5000, 3), (1, 2000001),
-         (9000, 5), (2500, 300), (70001, 2), (2049, 257)]
+         (9000, 5), (2500, 300), (70001, 2), (2049, 257), (2047, 257), (2048, 1025)]
 
 
 @pytest.mark.parametrize("B,T", SIZES)

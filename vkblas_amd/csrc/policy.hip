@@ -3,7 +3,7 @@
 // A token's loss is a few operations on four or five floats, so the loss over a
 // batch is a pass over its arrays and a sum, bound by the reads: 13 to 17 bytes
 // a token.  A workgroup takes a unit, a sequence or a part of one (a wave where
-// sequences have up to 256 tokens), four tokens a lane at a time, and skips the
+// there are many short sequences), four tokens a lane at a time, and skips the
 // arrays where no token of a lane's four counts: the padding behind a sequence
 // costs its mask alone.  A token's terms are fp32; sums are fp64, and so is logp -
 // old, on which the side of a bound depends: r > 1 + clip_high exactly where
@@ -305,15 +305,15 @@ __global__ __launch_bounds__(FIN) void finish_kernel(vkb_policy p, int reduce, c
     finish(p.B, p.units, reduce, part, (uint64_t)p.B * p.units, stats, norm, sh);
 }
 
-// Sequences of one unit: a wave's (SHORT, up to 256 tokens) or a workgroup's
+// Sequences of one unit: a wave's (WAVE) or a workgroup's
 // own.  Their tokens are counted, and each lane adds its sums by the
 // reduction's weight: lanes and waves are joined once for all of a workgroup's
 // sequences, and the finish reads as many totals as there are workgroups
 // (part: NSUM + 1 arrays of those, then each sequence's tokens).  Against each
 // sequence's five sums to memory and one workgroup over them (us): 65536 x 128
-// 115 -> 52, 16384 x 1024 71 -> 61, 8192 x 256 22 -> 16.  What is left at many short
+// 115 -> 52, 16384 x 1024 71 -> 49, 8192 x 256 22 -> 16.  What is left at many short
 // sequences is arithmetic, a wave's whatever its lanes hold.
-template <bool SHORT>
+template <bool WAVE>
 __global__ __launch_bounds__(WORK) void whole_kernel(vkb_policy p, int reduce, double* part) {
     __shared__ double totals[WAVES][NSUM + 1];
     __shared__ uint32_t counts[2][WAVES];
@@ -321,18 +321,18 @@ __global__ __launch_bounds__(WORK) void whole_kernel(vkb_policy p, int reduce, d
     double* tokens = part + (NSUM + 1) * (uint64_t)gridDim.x;
     Total total = {};
     uint32_t turn = 0;
-    for (uint64_t b = SHORT ? (uint64_t)blockIdx.x * WAVES + wave : blockIdx.x; b < p.B;
-         b += (uint64_t)gridDim.x * (SHORT ? WAVES : 1)) {
-        const Sums s = lane_sums(p, (int64_t)b, SHORT ? 0 : 256 * wave, p.T, SHORT ? 256 : 256 * WAVES, lane);
+    for (uint64_t b = WAVE ? (uint64_t)blockIdx.x * WAVES + wave : blockIdx.x; b < p.B;
+         b += (uint64_t)gridDim.x * (WAVE ? WAVES : 1)) {
+        const Sums s = lane_sums(p, (int64_t)b, WAVE ? 0 : 256 * wave, p.T, WAVE ? 256 : 256 * WAVES, lane);
         uint32_t n = wave_sum((uint32_t)s.v[4]);
-        if (!SHORT) {
+        if (!WAVE) {
             if (lane == 0) counts[turn][wave] = n;
             __syncthreads();             // (one a sequence: the next one's counts go to the other half)
             n = 0;
             for (uint32_t w = 0; w < WAVES; ++w) n += counts[turn][w];
             turn ^= 1;
         }
-        const bool first = lane == 0 && (SHORT || wave == 0);
+        const bool first = lane == 0 && (WAVE || wave == 0);
         if (first) tokens[b] = (double)n;
         if (n == 0) continue;
         const double by = reduce == VKBLAS_REDUCE_SEQUENCES ? 1.0 / (double)n : 1.0;
@@ -413,7 +413,8 @@ __global__ __launch_bounds__(WORK) void grad_kernel(vkb_policy p, const float* n
 
 using namespace vkb;
 
-// A unit: a wave's 256 tokens, or 1024 times as many as leave 2048 workgroups
+// A unit: sequences of up to 256 tokens, or 1024 tokens times as many as leave 2048
+// workgroups
 extern "C" void vkb_policy_units(vkb_policy* p) {
     if (p->T <= 256) {
         p->unit = 256;
@@ -427,11 +428,16 @@ extern "C" void vkb_policy_units(vkb_policy* p) {
 }
 // One wave each for up to 16 units of 256
 static uint64_t small_units(const vkb_policy* p) { return (uint64_t)p->B * (((uint64_t)p->T + 255) / 256); }
+// Whether sequences of one unit are a wave's: up to 256 tokens leave a workgroup's
+// others nothing, and up to 1024 are so where there are waves enough (us, a
+// workgroup / a wave each: 1024 x 1000 12.0 / 14.3, 2048 x 512 15.2 / 11.7, 2048 x 1024
+// 16.4 / 15.3, 16384 x 300 48 / 25, 16384 x 1024 61 / 49; 4096 x 4096 47 / 49).
+static bool by_wave(const vkb_policy* p) { return p->T <= 256 || (p->T <= 1024 && p->B >= 2048); }
 // Workgroups of sequences of one unit (us for 512 / 1024 / 2048 / 4096 of them:
 // 65536 x 128 81 / 52 / 52 / 53, 4096 x 4096 73 / 49 / 48 / 47)
 constexpr uint32_t WHOLE_BLOCKS = 2048;
 static uint32_t whole_blocks(const vkb_policy* p) {
-    const uint32_t n = p->T <= 256 ? (p->B + WAVES - 1) / WAVES : p->B;
+    const uint32_t n = by_wave(p) ? (p->B + WAVES - 1) / WAVES : p->B;
     return n < WHOLE_BLOCKS ? n : WHOLE_BLOCKS;
 }
 extern "C" size_t vkb_policy_part_bytes(const vkb_policy* p) {
@@ -451,7 +457,7 @@ extern "C" int vkb_launch_policy(const vkb_policy* p, int reduce, void* part, fl
     const bool whole = p->units == 1;
     const uint32_t blocks = whole_blocks(p);
     const uint64_t count = (uint64_t)p->B * p->units;
-    if (whole && p->T <= 256)
+    if (whole && by_wave(p))
         hipLaunchKernelGGL((whole_kernel<true>), dim3(blocks), dim3(WORK), 0, (hipStream_t)stream, *p, reduce,
                            (double*)part);
     else if (whole)
