@@ -91,11 +91,12 @@ def check_gradient(got, dy, ids, V, wt, scale, beta=0.0, dw0=None, pad_id=PAD):
     return dw
 
 
-# one launch (up to 2048 and 4096 rows), chunks of the sorted pairs, runs of 2048, merges of up to 16 and 64 of them, a
-# second level of merges (past 131072)
+# one launch (up to 2048 and 4096 rows), chunks of the sorted pairs, runs of 1024, merges of up to 16 and 64 of them, a
+# second level of merges (past 65536)
 GRAD_SIZES = SIZES + [(8, 3, 70), (9, 3, 70), (2047, 5, 24), (2048, 700, 72), (2049, 9, 8), (4095, 3, 8), (4097, 3, 8),
                       (6145, 1, 20), (8192, 5, 24), (12289, 100000, 8), (16385, 40, 264), (32768, 200, 16),
-                      (32769, 3, 16), (65536, 3000, 16), (65537, 257, 9), (131073, 50, 8), (150001, 1000, 5)]
+                      (32769, 3, 16), (65536, 3000, 16), (65537, 257, 9), (131073, 50, 8), (150001, 1000, 5),
+                      (16384, 90, 8)]
 
 
 @pytest.mark.parametrize("M,V,N", GRAD_SIZES)
@@ -105,7 +106,8 @@ def test_gradient(M, V, N, dt, wt):
     check_gradient(gradient(dy, ids, V, dt, wt, 1.5), dy, ids, V, wt, 1.5)
 
 
-@pytest.mark.parametrize("M,V,N", [(1, 40000, 1000), (3, 33000, 1025), (300, 70001, 520), (4096, 16400, 2050)])
+@pytest.mark.parametrize("M,V,N", [(1, 40000, 1000), (3, 33000, 1025), (300, 70001, 520), (1024, 34000, 1000),
+                                   (1025, 34000, 1000), (4096, 16400, 2050)])
 @pytest.mark.parametrize("beta", [0.0, 1.0, 0.5])
 def test_gradient_of_few_tokens_and_a_large_one(M, V, N, beta):
     """More bytes than the one launch takes: the sort of one run.  On the GPU."""

@@ -65,8 +65,9 @@ __device__ __forceinline__ uint32_t sort_key(int64_t id, int64_t pad, uint32_t V
 // The workgroups from ranks on zero dw, 16 bytes a thread: stores are fastest
 // from many short workgroups (1 GiB of zeros: 4 KB each 6.8 TB/s, 8 KB 6.1, 512 KB 5.7,
 // 8192 workgroups in strides 4.6; rows with tokens left out, which takes a look at
-// a map of them, 4.6 beside the sums).  16384 tokens' ranks take 8 us by themselves, and
-// beside 1 GB of zeros, 150 us, nothing.
+// a map of them, 4.6 beside the sums).  Beside 1 GB of them, 150 us, the ranks cost
+// nothing.  Runs of 1024 / 2048: 16384 tokens and 65 MB of zeros 11.8 / 14.5 us, and
+// their merge 4.1 / 4.0; 65536 and 33 MB 14.7 / 20.2, and 13.4 / 9.7.
 constexpr uint32_t RTOK = 16, RGROUPS = WORK / RTOK;
 template <typename W>
 __global__ __launch_bounds__(WORK) void rank_kernel(uint32_t M, uint32_t V, const int64_t* ids, int64_t pad,
@@ -130,22 +131,28 @@ __global__ __launch_bounds__(WORK) void rank_kernel(uint32_t M, uint32_t V, cons
 // keys fit (S = 1, WAYS runs), or the last of each S of them (S = 4, S WAYS
 // runs): then the S keys at the place found there are read and counted.
 // Searches count the keys below a bound, which for earlier runs is past the
-// pair's own key; SEARCHES of them run side by side.
-constexpr uint32_t SEARCHES = 8;
+// pair's own key; SEARCHES of them run side by side, and MGROUPS waves share the
+// runs of 64 pairs (with one wave for all of them, runs of 2048, 16384 pairs took 6.0 us,
+// not 4.0, and 65536 pairs 18, not 9.7: the LDS leaves a CU few workgroups, so few waves
+// to hide the searches' chains).
+constexpr uint32_t MGROUPS = 4, MTHREADS = MGROUPS * WORK;
 template <uint32_t S>
-__global__ __launch_bounds__(WORK) void merge_runs_kernel(uint32_t M, const uint32_t* key_in, const uint32_t* order_in,
-                                                          uint32_t* key, uint32_t* order) {
+__global__ __launch_bounds__(MTHREADS) void merge_runs_kernel(uint32_t M, const uint32_t* key_in,
+                                                              const uint32_t* order_in, uint32_t* key,
+                                                              uint32_t* order) {
     constexpr uint32_t GROUP = RUN * WAYS * S, LEN = RUN / S;      // pairs of a group, keys of a run in LDS
+    constexpr uint32_t SEARCHES = S == 1 ? 4 : 8;
+    __shared__ uint32_t places[MGROUPS - 1][WORK];
     __shared__ __attribute__((aligned(16))) uint32_t keys[LEN * WAYS * S];
     const uint64_t first = (uint64_t)blockIdx.x * WORK, group = first / GROUP * GROUP;
     const uint32_t n = (uint32_t)min((uint64_t)GROUP, M - group), runs = (n + RUN - 1) / RUN;
     // whole runs, the last one filled up with keys above all others; LOADS in flight
-    constexpr uint32_t LOADS = RUN / 4 / WORK * 4;
-    for (uint32_t q0 = 0; q0 < runs * (RUN / 4); q0 += LOADS * WORK) {
+    constexpr uint32_t LOADS = 4;
+    for (uint32_t q0 = 0; q0 < runs * (RUN / 4); q0 += LOADS * MTHREADS) {
         u32x4 x[LOADS];
 #pragma unroll
         for (uint32_t l = 0; l < LOADS; ++l) {
-            const uint32_t i = 4 * (q0 + l * WORK + threadIdx.x);
+            const uint32_t i = 4 * (q0 + l * MTHREADS + threadIdx.x);
             if (i + 4 <= n) x[l] = *(const u32x4*)(key_in + group + i);
             else
 #pragma unroll
@@ -153,18 +160,18 @@ __global__ __launch_bounds__(WORK) void merge_runs_kernel(uint32_t M, const uint
         }
 #pragma unroll
         for (uint32_t l = 0; l < LOADS; ++l) {
-            const uint32_t q = q0 + l * WORK + threadIdx.x;
+            const uint32_t q = q0 + l * MTHREADS + threadIdx.x;
             if (q >= runs * (RUN / 4)) continue;
             if constexpr (S == 1) *(u32x4*)(keys + 4 * q) = x[l];
             else keys[q] = x[l][3];
         }
     }
     __syncthreads();
-    const uint32_t i = (uint32_t)(first - group) + threadIdx.x;
-    if (i >= n) return;
+    const uint32_t share = threadIdx.x / WORK, pair = threadIdx.x % WORK;
+    const uint32_t i = min((uint32_t)(first - group) + pair, n - 1);
     const uint32_t own = i / RUN, k = key_in[group + i], o = order_in[group + i];
-    uint32_t at = i % RUN;
-    for (uint32_t r0 = 0; r0 < runs; r0 += SEARCHES) {
+    uint32_t at = 0;
+    for (uint32_t r0 = share * SEARCHES; r0 < runs; r0 += MGROUPS * SEARCHES) {
         uint32_t pos[SEARCHES];
 #pragma unroll
         for (uint32_t r = 0; r < SEARCHES; ++r) pos[r] = 0;
@@ -202,6 +209,12 @@ __global__ __launch_bounds__(WORK) void merge_runs_kernel(uint32_t M, const uint
 #pragma unroll
         for (uint32_t r = 0; r < SEARCHES; ++r) at += r0 + r < runs && r0 + r != own ? pos[r] : 0u;
     }
+    if (share) places[share - 1][pair] = at;
+    __syncthreads();
+    if (share || (uint32_t)(first - group) + pair >= n) return;
+    at += i % RUN;
+#pragma unroll
+    for (uint32_t s = 0; s < MGROUPS - 1; ++s) at += places[s][pair];
     key[group + at] = k;
     order[group + at] = o;
 }
@@ -341,8 +354,8 @@ __device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__bui
 // waves' on a part of the list each.  Rows without one are zeroed or scaled in
 // all of their columns, by the workgroups of the same rows in turn.
 // Against the sort and its launches (us, sorted / so): bf16 64 x 1000 x 512 11.1 / 6.6,
-// 1024 x 32000 x 1024 18.5 / 17.7, 4096 x 32000 x 1024 25.1 / 22.7, 4096 x 500 x 512
-// 19.5 / 12.8, fp32 1003 x 997 x 515 12.3 / 7.4, 4096 x 16000 x 1024 25.7 / 26.4; where
+// 1024 x 32000 x 1024 18.1 / 17.7, 4096 x 32000 x 1024 24.1 / 22.8, 4096 x 500 x 512
+// 16.7 / 12.7, fp32 1003 x 997 x 515 12.0 / 7.4, 4096 x 16000 x 1024 25.1 / 26.4; where
 // few tokens fill the batch the sort is ahead, three in ten of 4096 the same 35 / 42,
 // all of them 41 / 81.
 constexpr uint32_t DIRECT = VKBLAS_EMBEDDING_SMALL, DTHREADS = 512, DWAVES = DTHREADS / 64;
@@ -608,7 +621,7 @@ __global__ __launch_bounds__(WORK) void others_kernel(uint32_t M, uint32_t V, ui
 // the chunks it fills, the waves on a quarter each, in order, JROWS in flight.
 // (Eight waves: level, a token's 80 parts 3 us faster, 4000 workgroups with two
 // parts or none each 4 us slower.)
-constexpr uint32_t JTHREADS = 256, JWAVES = JTHREADS / 64, JROWS = 8;
+constexpr uint32_t JTHREADS = 256, JWAVES = JTHREADS / 64, JROWS = 8, AHEAD = 4;
 template <typename T, typename W>
 __global__ __launch_bounds__(JTHREADS) void join_kernel(SumParams p) {
     constexpr int VEC = Elem<T>::VEC;
@@ -618,12 +631,20 @@ __global__ __launch_bounds__(JTHREADS) void join_kernel(SumParams p) {
     const uint32_t p0 = chunk * p.chunk, p1 = p0 + p.chunk;      // the last chunk is not here
     const uint32_t k = p.key[p1 - 1];
     if (k >= p.V || p.key[p1] != k || (p0 && p.key[p0] == k && p.key[p0 - 1] == k)) return;
-    // the last chunk whose first key is k: keys are sorted
-    uint32_t lo = chunk + 1, hi = p.chunks - 1;
-    while (lo < hi) {
-        const uint32_t mid = (lo + hi + 1) / 2;
-        if (p.key[mid * p.chunk] == k) lo = mid;
-        else hi = mid - 1;
+    // the last chunk whose first key is k, AHEAD chunks a lane at a time (by a binary search, a chain of
+    // reads, 0.9 us more)
+    uint32_t lo = chunk;
+    for (uint32_t n = 64 * AHEAD; n == 64 * AHEAD; lo += n) {
+        uint32_t first[AHEAD];
+        n = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < AHEAD; ++i) {
+            const uint32_t c = lo + 1 + i * 64 + lane;
+            first[i] = p.key[min(c, p.chunks - 1) * p.chunk];
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < AHEAD; ++i)
+            n += (uint32_t)__popcll(__ballot(lo + 1 + i * 64 + lane < p.chunks && first[i] == k));
     }
     const uint32_t parts = lo - chunk + 1, each = (parts + JWAVES - 1) / JWAVES;
     const uint32_t a = min(wave * each, parts), b = min(a + each, parts);
@@ -735,10 +756,10 @@ extern "C" int vkb_launch_embedding_merge_runs(uint32_t M, const uint32_t* key_i
                                                uint32_t* key, uint32_t* order, void* stream) {
     const uint32_t blocks = (uint32_t)(((uint64_t)M + WORK - 1) / WORK);
     if (M <= RUN * WAYS)
-        hipLaunchKernelGGL((merge_runs_kernel<1>), dim3(blocks), dim3(WORK), 0, (hipStream_t)stream, M, key_in,
+        hipLaunchKernelGGL((merge_runs_kernel<1>), dim3(blocks), dim3(MTHREADS), 0, (hipStream_t)stream, M, key_in,
                            order_in, key, order);
     else
-        hipLaunchKernelGGL((merge_runs_kernel<4>), dim3(blocks), dim3(WORK), 0, (hipStream_t)stream, M, key_in,
+        hipLaunchKernelGGL((merge_runs_kernel<4>), dim3(blocks), dim3(MTHREADS), 0, (hipStream_t)stream, M, key_in,
                            order_in, key, order);
     return (int)hipGetLastError();
 }

@@ -1035,7 +1035,7 @@ vkblas_status_t vkblas_embedding_backward_async(vkblas_dtype_t type, uint32_t M,
     if (vkb_engine_trace()) fprintf(stderr, "[vkblas] embedding_backward type=%d M=%u V=%u N=%u\n", (int)type, M, V, N);
     /* one launch, but for a large dw: its workgroups then have many rows each, and the
      * zeros a bad pattern of stores (us, one launch / sorted, bf16: 1024 x 32000 x 1024,
-     * 66 MB, 17.7 / 18.5; 1000 x 64000 x 1024 38 / 30; 1 x 128000 x 4096 221 / 156;
+     * 66 MB, 17.7 / 18.1; 1000 x 64000 x 1024 38 / 30; 1 x 128000 x 4096 221 / 156;
      * 4000 x 128000 x 4096 315 / 182) */
     if (M <= VKBLAS_EMBEDDING_SMALL && N <= 65535u * 256u &&
         (uint64_t)V * N * type_size(dw_type) <= VKBLAS_EMBEDDING_SMALL_BYTES) {

@@ -11,8 +11,8 @@
 //
 // 1024 sequences of 8192 tokens, half of them padding: 20.8 us (3.6 TB/s of the
 // bytes that it reads) and 5.8 for the finish, one workgroup over 2048 units; the
-// gradient, which writes the padding's zeros too, 20 us (5.4 TB/s).  A call of up to 16 units of 256 tokens is one workgroup,
-// 7.2 us with its launch.
+// gradient, which writes the padding's zeros too, 20 us (5.4 TB/s).  A call of up to
+// 16 units of 256 tokens is one workgroup, 7.2 us with its launch.
 #include "nn_common.hpp"
 
 namespace vkb {

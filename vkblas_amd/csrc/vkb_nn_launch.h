@@ -102,7 +102,7 @@ int vkb_launch_glu_direct(int type, int act, uint32_t M, uint32_t N, uint32_t K,
 int vkb_launch_embedding_direct(int type, int w_type, uint32_t M, uint32_t V, uint32_t N, const int64_t* ids,
                                 int64_t pad, const void* dy, int64_t lddy, float scale, void* dw, int64_t lddw,
                                 float beta, void* stream);
-#define VKB_EMBED_RUN 2048u
+#define VKB_EMBED_RUN 1024u
 #define VKB_EMBED_WAYS 16u
 static inline uint64_t vkb_embedding_group(uint32_t M) {
     return (uint64_t)VKB_EMBED_RUN * VKB_EMBED_WAYS * (M <= VKB_EMBED_RUN * VKB_EMBED_WAYS ? 1 : 4);
