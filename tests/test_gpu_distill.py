@@ -148,6 +148,20 @@ def test_large(M, V, K, n, dt):
     check_backward(backward(*args, 2.0, dt), *args, 2.0, dt)
 
 
+# enough entries that the tiles of the logits leave those at the entries: tiles of 128 (in four LDS stages and two) and
+# of 256, an odd K, more slices than 1023, more rows than workgroups
+@pytest.mark.parametrize("M,V,K,n,dt", [(1100, 1000, 1024, 480, "bf16"), (1100, 1000, 1027, 480, "f16"),
+                                        (1100, 6001, 1024, 480, "bf16"), (600, 20000, 2048, 448, "f16"),
+                                        (515, 140001, 1024, 1024, "bf16"), (70001, 600, 520, 16, "bf16"),
+                                        (1050, 129, 1024, 500, "f16")])
+@pytest.mark.parametrize("pad", [0, 5])
+def test_many_entries(M, V, K, n, dt, pad):
+    x, w, top, t = inputs(M, V, K, n, dt, device="cuda")
+    top[7, 3], top[8, n - 1], top[9] = V, 2 ** 40, 5        # two bad rows, and one of one class
+    t[9] = t[9].nan_to_num(0.5, 0.5, 0.5)
+    check_forward(forward(x, w, top, t, 1.5, dt, pad=pad), x, w, top, t, 1.5)
+
+
 @pytest.mark.parametrize("K", [16, 128])
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
 def test_pieces(dt, K):

@@ -137,21 +137,73 @@ __device__ __forceinline__ Pair join_logits(const float* z, uint32_t V, float c2
     return p;
 }
 
+// Where the tiles of the logits leave those at the entries: each row's entries by
+// slices of `width` classes, in counting order (which entry of a slice goes first
+// is no matter: each has a place of its own in z_top).  M stride + M n small numbers
+// to write; bound by a row's chain of five passes over LDS.
+template <uint32_t SLICES>
+__global__ __launch_bounds__(WORK) void table_kernel(uint32_t M, uint32_t V, uint32_t n, const int64_t* top,
+                                                     int64_t ldtop, uint32_t width, uint32_t stride, uint32_t* list,
+                                                     uint16_t* offs) {
+    constexpr uint32_t EACH = SLICES / WORK;
+    __shared__ uint32_t count[SLICES], waves[WAVES];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (uint64_t m = blockIdx.x; m < M; m += gridDim.x) {
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < SLICES; i += WORK) count[i] = 0;
+        __syncthreads();
+        for (uint32_t j = threadIdx.x; j < n; j += WORK) {
+            const int64_t c = top[(int64_t)m * ldtop + j];
+            if (c >= 0 && c < V) atomicAdd(&count[(uint32_t)c / width], 1u);
+        }
+        __syncthreads();
+        // the places before each slice: a thread's EACH, the lanes' before it, the waves' before those
+        uint32_t own[EACH], sum = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < EACH; ++i) {
+            own[i] = sum;
+            sum += count[threadIdx.x * EACH + i];
+        }
+        uint32_t before = sum;
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint32_t x = (uint32_t)__shfl_up((int)before, d);
+            before += lane >= (uint32_t)d ? x : 0;
+        }
+        if (lane == 63) waves[wave] = before;
+        before -= sum;
+        __syncthreads();
+        for (uint32_t w = 0; w < wave; ++w) before += waves[w];
+#pragma unroll
+        for (uint32_t i = 0; i < EACH; ++i) {
+            const uint32_t s = threadIdx.x * EACH + i;
+            count[s] = before + own[i];
+        }
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < stride; i += WORK) offs[m * stride + i] = (uint16_t)count[i];
+        __syncthreads();
+        for (uint32_t j = threadIdx.x; j < n; j += WORK) {
+            const int64_t c = top[(int64_t)m * ldtop + j];
+            if (c < 0 || c >= V) continue;
+            const uint32_t s = (uint32_t)c / width;
+            list[m * n + atomicAdd(&count[s], 1u)] = j * width + ((uint32_t)c - s * width);
+        }
+    }
+}
+
 // One workgroup per row.  Its log-sum-exp comes from lse, from the parts that
 // tiles or slices left (then lse is written) or, with neither, from the logits.
-// The logits at the entries are read where the row is there, else computed, the
+// The logits at the entries are there (given), read where the row is, or computed, the
 // waves on DOTS entries at a time: one load of x's chunk for DOTS of w's rows.
 // Those rows of w are the kernel's bytes: 4096 rows of 64 entries, K = 4096 and 128000
-// classes in bf16, 165 us for 2.1 GB, half of it from HBM (6.4 TB/s), beside 3.1 ms
-// for the logits.  (Tiles that keep the entries' logits themselves would need a
-// table of each tile's entries.)
+// classes in bf16, 165 us for 2.1 GB, half of it from HBM (6.4 TB/s).
 constexpr uint32_t DOTS = 8;
 template <typename T, typename TT>
 __global__ __launch_bounds__(WORK) void rows_kernel(uint32_t M, uint32_t V, uint32_t K, const T* x, int64_t ldx,
                                                     const T* w, int64_t ldw, uint32_t n, const int64_t* top,
                                                     int64_t ldtop, const TT* t, int64_t ldt, float temp, float inv_t,
                                                     const float* logits, int64_t ldz, const float2* parts, uint32_t S,
-                                                    int have_lse, float* lse, float* loss, float* z_top) {
+                                                    int have_lse, int given, float* lse, float* loss,
+                                                    float* z_top) {
     constexpr int VEC = Elem<T>::VEC;
     __shared__ Shared sh;
     __shared__ float z[TOP], sums[WAVES];
@@ -173,7 +225,7 @@ __global__ __launch_bounds__(WORK) void rows_kernel(uint32_t M, uint32_t V, uint
             if (lane == 0) count = c;
         }
         __syncthreads();
-        const uint32_t there = logits ? 0 : count;
+        const uint32_t there = logits || given ? 0 : count;
         const T* xr = x + (int64_t)m * ldx;
         for (uint32_t g = wave * DOTS; g < there; g += WAVES * DOTS) {
             const T* row[DOTS];
@@ -212,7 +264,7 @@ __global__ __launch_bounds__(WORK) void rows_kernel(uint32_t M, uint32_t V, uint
         for (uint32_t j = threadIdx.x; j < n; j += WORK) {
             const int id = sh.id[j];
             const float v = id == ABSENT ? 0.0f : id == BAD ? __builtin_nanf("")
-                          : logits ? logits[(int64_t)m * ldz + id] : z[j];
+                          : given ? z_top[(int64_t)m * n + j] : logits ? logits[(int64_t)m * ldz + id] : z[j];
             z_top[(int64_t)m * n + j] = v;
             const float log_q = sh.q[j] - log_s, q = fast_exp(log_q);
             if (id != ABSENT && !(q == 0.0f)) s += q * (log_q - (v * inv_t - l));
@@ -317,13 +369,25 @@ extern "C" int vkb_launch_distill_rows(int type, int t_type, const vkb_distill* 
             using TT = decltype(f);
             hipLaunchKernelGGL((rows_kernel<T, TT>), dim3(row_blocks(d->M)), dim3(WORK), 0, (hipStream_t)stream, d->M,
                                d->V, K, (const T*)x, ldx, (const T*)w, ldw, d->n, d->top, d->ldtop, (const TT*)d->t,
-                               d->ldt, d->temp, 1.0f / d->temp, r->z, r->ldz, (const float2*)r->parts, r->S, r->have_lse,
-                               r->lse, r->loss, r->z_top);
+                               d->ldt, d->temp, 1.0f / d->temp, r->z, r->ldz, (const float2*)r->parts, r->S,
+                               r->have_lse, r->given, r->lse, r->loss, r->z_top);
         };
         if (t_type == VKB_T_F32) launch(float{});
         else launch(e);
     });
     return ok ? (int)hipGetLastError() : (int)hipErrorInvalidValue;
+}
+
+extern "C" int vkb_launch_distill_table(const vkb_distill* d, const vkb_distill_table* t, void* stream) {
+    if (t->stride > VKB_DISTILL_SLICES + 1) return (int)hipErrorInvalidValue;
+    if (t->stride <= 1024)
+        hipLaunchKernelGGL(table_kernel<1024>, dim3(row_blocks(d->M)), dim3(WORK), 0, (hipStream_t)stream, d->M, d->V,
+                           d->n, d->top, d->ldtop, t->width, t->stride, t->list, t->offs);
+    else
+        hipLaunchKernelGGL((table_kernel<VKB_DISTILL_SLICES + WORK>), dim3(row_blocks(d->M)), dim3(WORK), 0,
+                           (hipStream_t)stream, d->M, d->V, d->n, d->top, d->ldtop, t->width, t->stride, t->list,
+                           t->offs);
+    return (int)hipGetLastError();
 }
 
 extern "C" int vkb_launch_distill_prepare(int t_type, const vkb_distill* d, const float* dloss, void* stream) {

@@ -191,6 +191,73 @@ struct XentStatsOp {
     }
 };
 
+// A distillation's statistics: those, and the logits at each row's entries, from
+// a table of them by slice (a wave's WT columns): offs[m][slice] .. offs[m][slice
+// + 1] - 1 are the row's in list[m], an entry and a column of the slice each.  A
+// fragment's rows that have any go through LDS, from where the lanes that share a
+// row take one entry each; the first ones of all fragments are loaded at once.
+// (Before the statistics: held across them, the accumulators spill.)  16-bit
+// operands: in fp32 the products of single entries cost a tenth beside the logits.
+struct DistillParams : XentParams {
+    const uint32_t* list;
+    const uint16_t* offs;
+    uint32_t n, stride;      // entries of a row, and offsets
+    float* z_top;
+};
+template <typename T>
+struct DistillStatsOp {
+    using Params = DistillParams;
+    static constexpr bool PLAIN = false, GATED = false;
+    template <int WT, int SH, int LDS, typename ACC>
+    static __device__ __forceinline__ void run(const Params& p, ACC& acc, char* lds, int m0, int n0, int wave,
+                                               int lane) {
+        using G = Frag<WT, SH>;
+        constexpr int SHARE = 64 / G::FR, STR = WT + 4;
+        static_assert(4 * G::FR * STR * (int)sizeof(float) <= LDS, "rows exceed LDS");
+        const int64_t row0 = m0 + (wave >> 1) * WT, slice = n0 / WT + (wave & 1);
+        const uint32_t sub = (uint32_t)lane / G::FR;
+        uint32_t span[G::NF], first[G::NF];          // span: the lane's first entry, and the end
+#pragma unroll
+        for (int i = 0; i < G::NF; ++i) {
+            const int64_t m = row0 + G::row(lane, i);
+            span[i] = 0;
+            if (m < p.M) {
+                const uint16_t* o = p.offs + m * p.stride + slice;
+                span[i] = o[0] + sub | (uint32_t)o[1] << 16;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < G::NF; ++i)
+            if ((span[i] & 0xffff) < span[i] >> 16)
+                first[i] = p.list[(row0 + G::row(lane, i)) * p.n + (span[i] & 0xffff)];
+        float* row = (float*)lds + (wave * G::FR + G::row(lane, 0)) * STR;
+#pragma unroll
+        for (int i = 0; i < G::NF; ++i) {
+            __builtin_amdgcn_sched_barrier(0);
+            uint32_t k = span[i] & 0xffff;
+            const uint32_t end = span[i] >> 16;
+            if (!__any(k < end)) continue;
+#pragma unroll
+            for (int j = 0; j < G::NF; ++j)
+#pragma unroll
+                for (int q = 0; q < G::NQ; ++q)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) row[G::col(lane, j, q) + e] = acc[i][j][4 * q + e];
+            // (the compiler does not reorder a wave's accesses across lanes past the waits)
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            const int64_t at = (row0 + G::row(lane, i)) * p.n;
+            for (uint32_t entry = first[i]; k < end; k += SHARE) {
+                const uint32_t here = entry;
+                if (k + SHARE < end) entry = p.list[at + k + SHARE];
+                p.z_top[at + here / WT] = row[here % WT];
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0);       // one row's copies of the accumulators at a time
+        }
+        XentStatsOp<T>::template run<WT, SH, LDS>(p, acc, lds, m0, n0, wave, lane);
+    }
+};
+
 // D = scal * dloss * (exp(z - lse) - [v == target]), rounded to T (as an operand of
 // two products).  4096 x 65536 x 4096 bf16 1.67 ms, 1.32 PFLOP/s.
 template <typename T>

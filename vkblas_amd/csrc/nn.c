@@ -140,6 +140,8 @@ extern int vkb_launch_glu_bf16(const vkb_op_args*, int, void*, int64_t, void*, i
 extern int vkb_launch_xent_stats_f32(const vkb_op_args*, float, const int64_t*, float*, float*, void*);
 extern int vkb_launch_xent_stats_f16(const vkb_op_args*, float, const int64_t*, float*, float*, void*);
 extern int vkb_launch_xent_stats_bf16(const vkb_op_args*, float, const int64_t*, float*, float*, void*);
+typedef int distill_stats_fn(const vkb_op_args*, float, float*, const vkb_distill_table*, float*, void*);
+extern distill_stats_fn vkb_launch_distill_stats_f32, vkb_launch_distill_stats_f16, vkb_launch_distill_stats_bf16;
 typedef int xent_grad_fn(const vkb_op_args*, uint32_t, uint32_t, uint32_t, uint32_t, float, const int64_t*, int64_t,
                          const float*, const float*, vkb_scale, void*, int64_t, void*);
 extern xent_grad_fn vkb_launch_xent_grad_f32, vkb_launch_xent_grad_f16, vkb_launch_xent_grad_bf16;
@@ -154,6 +156,12 @@ int vkb_launch_xent_stats_op(const vkb_op_args* a, float inv_t, const int64_t* t
     return (a->type == VKB_T_F16 ? vkb_launch_xent_stats_f16 : a->type == VKB_T_BF16 ? vkb_launch_xent_stats_bf16
                                                                                     : vkb_launch_xent_stats_f32)(
         a, inv_t, target, parts, zt, stream);
+}
+int vkb_launch_distill_stats_op(const vkb_op_args* a, float inv_t, float* parts, const vkb_distill_table* t,
+                                float* z_top, void* stream) {
+    return (a->type == VKB_T_F16 ? vkb_launch_distill_stats_f16 : a->type == VKB_T_BF16 ? vkb_launch_distill_stats_bf16
+                                                                                       : vkb_launch_distill_stats_f32)(
+        a, inv_t, parts, t, z_top, stream);
 }
 int vkb_launch_xent_grad_op(const vkb_op_args* a, uint32_t Ms, uint32_t Ns, uint32_t v0, uint32_t V, float inv_t,
                             const int64_t* target, int64_t ignore, const float* lse, const float* dloss,
@@ -661,6 +669,17 @@ static int distill_rows(op_call* c, vkblas_dtype_t type, uint32_t K, teacher_row
  * x 32000 x 1024 129.3 / 128.9; more parts 1000 x 128000 x 1024 241 / 246, 8192 x 128000
  * x 64 569 / 593). */
 #define JOIN_PARTS (1u << 18)
+/* Whether the tiles leave the logits at a distillation's entries, or single
+ * products with rows of w make them: those read n K elements a row, a look at the
+ * table costs each tile its time whatever it finds, and the table a launch (us, by
+ * products / by tiles, bf16: 4096 x 32000 x 4096, 8 entries 792 / 785, 64 886 / 797,
+ * 256 1335 / 810, 1024 3836 / 911; 4096 x 128000 x 4096, 16 entries 3048 / 3102, 64 3135 /
+ * 3102, 256 3625 / 3135; 4096 x 32000 x 1024, 64 264 / 271, 256 360 / 285; 2048 x 8000 x
+ * 1024, 64 55 / 58, 256 104 / 88; 300 x 32003 x 1024, 20 39 / 47, 256 61 / 79). */
+static int by_tiles(vkblas_dtype_t type, uint32_t M, uint32_t V, uint32_t K, uint32_t n, uint32_t S) {
+    return type != VKBLAS_DT_F32 && S <= VKB_DISTILL_SLICES && (uint64_t)n * K >= 2ull * V &&
+           (double)M * n * K >= 1 << 29;
+}
 
 /* lse of each row's logits times inv_t, and its loss (target NULL: none) or (q)
  * that of a distillation, on the call's workspace.  Returns the kernel for
@@ -675,7 +694,11 @@ static int row_statistics(op_call* c, vkblas_dtype_t type, uint32_t M, uint32_t 
         const uint32_t S = vkb_xent_slices(&a);
         place(c, &ox, type);
         place(c, &ow, type);
+        const int table = q && by_tiles(type, M, V, K, q->d.n, S);
+        vkb_distill_table t = {.n = q ? q->d.n : 0, .width = vkb_tile_bn(a.tile) / 2, .stride = S + 1};
         const size_t o_p = buf(c, (uint64_t)S * M * 2 * sizeof(float)), o_t = buf(c, (uint64_t)M * sizeof(float));
+        const size_t o_l = table ? buf(c, (uint64_t)M * t.n * sizeof(uint32_t)) : 0;
+        const size_t o_o = table ? buf(c, (uint64_t)M * t.stride * sizeof(uint16_t)) : 0;
         if (room(c) != VKBLAS_OK) return VKBLAS_KERNEL_NONE;
         float *parts = at(c, o_p), *zt = at(c, o_t);
         copies jobs = {.n = 0};
@@ -684,7 +707,17 @@ static int row_statistics(op_call* c, vkblas_dtype_t type, uint32_t M, uint32_t 
         if (brought(c, &jobs, type, NULL)) {
             bound(&a, &ox, &ow);
             const int join = q && (uint64_t)M * S <= JOIN_PARTS;
-            if (step(c, vkb_launch_xent_stats_op(&a, inv_t, target, parts, zt, stream), 0) &&
+            int ok;
+            if (table) {
+                t.list = at(c, o_l);
+                t.offs = at(c, o_o);
+                q->r.given = 1;
+                ok = step(c, vkb_launch_distill_table(&q->d, &t, stream), 0) &&
+                     step(c, vkb_launch_distill_stats_op(&a, inv_t, parts, &t, q->r.z_top, stream), 1);
+            } else {
+                ok = step(c, vkb_launch_xent_stats_op(&a, inv_t, target, parts, zt, stream), 0);
+            }
+            if (ok &&
                 (join || step(c, vkb_launch_xent_finish(M, V, S, inv_t, parts, zt, target, ignore_index, loss, lse,
                                                         stream), 1)) && q)
                 distill_rows(c, type, K, q, NULL, 0, parts, S, !join);

@@ -75,6 +75,23 @@ static int launch_xent_stats(const vkb_op_args* a, float inv_t, const int64_t* t
 }
 
 template <typename T>
+static int launch_distill_stats(const vkb_op_args* a, float inv_t, float* parts, const vkb_distill_table* t,
+                                float* z_top, hipStream_t st) {
+    if constexpr (sizeof(T) != 2) return (int)hipErrorInvalidValue;
+    else {
+    DistillParams p = op_params<T, DistillParams>(a);
+    p.parts = (float2*)parts;
+    p.c2 = inv_t * LOG2E;
+    p.list = t->list;
+    p.offs = t->offs;
+    p.n = t->n;
+    p.stride = t->stride;
+    p.z_top = z_top;
+    return launch_tiles<T, DistillStatsOp<T>>(a, p, st);
+    }
+}
+
+template <typename T>
 static int launch_xent_grad(const vkb_op_args* a, uint32_t Ms, uint32_t Ns, uint32_t v0, uint32_t V,
                             float inv_t, const int64_t* target, int64_t ignore, const float* lse, const float* dloss,
                             vkb_scale scale, void* D, int64_t ldd, hipStream_t st) {
@@ -104,6 +121,10 @@ static int launch_xent_grad(const vkb_op_args* a, uint32_t Ms, uint32_t Ns, uint
     extern "C" int vkb_launch_xent_stats_##NAME(const vkb_op_args* a, float inv_t, const int64_t* target,            \
                                                 float* parts, float* zt, void* st) {                                 \
         return vkb::launch_xent_stats<T>(a, inv_t, target, parts, zt, (hipStream_t)st);                              \
+    }                                                                                                                \
+    extern "C" int vkb_launch_distill_stats_##NAME(const vkb_op_args* a, float inv_t, float* parts,                  \
+                                                   const vkb_distill_table* t, float* z_top, void* st) {             \
+        return vkb::launch_distill_stats<T>(a, inv_t, parts, t, z_top, (hipStream_t)st);                             \
     }                                                                                                                \
     extern "C" int vkb_launch_xent_grad_##NAME(const vkb_op_args* a, uint32_t Ms, uint32_t Ns, uint32_t v0,          \
                                                uint32_t V, float inv_t, const int64_t* target, int64_t ignore,       \

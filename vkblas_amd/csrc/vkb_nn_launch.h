@@ -173,8 +173,9 @@ int vkb_launch_xent_grad(int type, uint32_t M, uint32_t n, uint32_t v0, uint32_t
 
 /* Distillation from a teacher's top logits (distill.hip).  rows: lse, z_top and
  * loss, from the logits z where they are there (NULL: not), lse as it is
- * (have_lse) or from S parts as xent stats leaves them (0: from z).  prepare, for the backward pass: q_top (M x n), T dloss (dl) and
- * targets for the kernels of D (ignore: a value no class has); patch: D's
+ * (have_lse) or from S parts as xent stats leaves them (0: from z).  prepare, for
+ * the backward pass: q_top (M x n), T dloss (dl) and targets for the kernels of D
+ * (ignore: a value no class has); patch: D's
  * elements of columns v0 .. v0 + cols - 1 at the entries, with scal[0] as those
  * kernels left it (NULL: 1). */
 typedef struct vkb_distill {
@@ -193,9 +194,19 @@ typedef struct vkb_distill_rows {
     int64_t ldz;
     const float* parts;
     uint32_t S;
-    int have_lse;
+    int have_lse, given;             /* given: z_top has the logits of the entries with a class */
     float *lse, *loss, *z_top;
 } vkb_distill_rows;
+/* table: each row's entries by slices of `width` classes (a wave's columns of a
+ * tile), for vkb_launch_distill_stats_op, which leaves lse's parts, and the logits
+ * at the entries that have a class in z_top (rows then has them given) */
+typedef struct vkb_distill_table {
+    uint32_t* list;                  /* M x n */
+    uint16_t* offs;                  /* M x stride: the slices', and one more */
+    uint32_t n, width, stride;
+} vkb_distill_table;
+#define VKB_DISTILL_SLICES 4096
+int vkb_launch_distill_table(const vkb_distill* d, const vkb_distill_table* t, void* stream);
 int vkb_launch_distill_rows(int type, int t_type, const vkb_distill* d, uint32_t K, const void* x, int64_t ldx,
                             const void* w, int64_t ldw, const vkb_distill_rows* r, void* stream);
 int vkb_launch_distill_prepare(int t_type, const vkb_distill* d, const float* dloss, void* stream);
@@ -270,6 +281,8 @@ int vkb_launch_glu(const vkb_op_args* a, int act, void* h, int64_t ldh, void* gu
 uint32_t vkb_xent_slices(const vkb_op_args* a);
 int vkb_launch_xent_stats_op(const vkb_op_args* a, float inv_t, const int64_t* target, float* parts, float* zt,
                              void* stream);
+int vkb_launch_distill_stats_op(const vkb_op_args* a, float inv_t, float* parts, const vkb_distill_table* t,
+                                float* z_top, void* stream);
 /* D as vkb_launch_xent_grad, stored on Ms rows and Ns columns, zero past M and
  * N: at least those, at most them rounded up to 128, Ns a multiple of 8 */
 int vkb_launch_xent_grad_op(const vkb_op_args* a, uint32_t Ms, uint32_t Ns, uint32_t v0, uint32_t V, float inv_t,
