@@ -17,10 +17,10 @@ namespace {
 
 constexpr uint32_t TOP = VKBLAS_DISTILL_TOP, WAVES = WORK / 64;
 
-constexpr int ABSENT = -1, BAD = -2, NONE = -3;
+constexpr int ABSENT = -1, BAD = -2;
 struct Shared {
     float q[TOP];            // the teacher's logits, then over T, then its probabilities
-    __attribute__((aligned(16))) int id[TOP];      // class, or ABSENT, or BAD; NONE up to a whole quad
+    int id[TOP];             // class, or ABSENT, or BAD
     float high[WAVES], sum[WAVES];
     uint32_t flags[WAVES];
 };
@@ -35,11 +35,11 @@ __device__ __forceinline__ float teacher(uint32_t n, uint32_t V, const int64_t* 
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     float high = -INFINITY;
     bool any = false, past = false;
-    for (uint32_t j = threadIdx.x; j < (n + 3) / 4 * 4; j += WORK) {
-        const int64_t c = j < n ? top[j] : -1;
+    for (uint32_t j = threadIdx.x; j < n; j += WORK) {
+        const int64_t c = top[j];
         const float v = c < 0 ? -INFINITY : (float)t[j];
-        sh.id[j] = j >= n ? NONE : c < 0 ? ABSENT : c < V ? (int)c : BAD;
-        if (j < n) sh.q[j] = v;
+        sh.id[j] = c < 0 ? ABSENT : c < V ? (int)c : BAD;
+        sh.q[j] = v;
         any |= !(v == -INFINITY);
         past |= c >= (int64_t)V;
         high = fmaxf(high, v);
@@ -282,16 +282,27 @@ __global__ __launch_bounds__(WORK) void rows_kernel(uint32_t M, uint32_t V, uint
 // The backward pass's rows: q of each entry's class (where a class occurs twice
 // both entries' at the first, -1 at the other: one of them patches D), T dloss,
 // and a target for D's kernels: `ignore` where the row is not counted, V where it
-// is bad, else the first entry's class, whose element the patch writes over.  10 us
-// at 4096 rows of 64.
-template <typename TT>
+// is bad, else the first entry's class, whose element the patch writes over.
+// Classes that occur twice are found by a hash of the row's in LDS (us at 4096 rows, by
+// comparing each pair of entries / so: 64 entries 10.2 / 9.7, 256 24 / 12, 1024 245 / 41;
+// 64 entries with the 24 KB that 1024 need 16).
+template <typename TT, uint32_t CAP>
 __global__ __launch_bounds__(WORK) void prepare_kernel(uint32_t M, uint32_t V, uint32_t n, const int64_t* top,
                                                        int64_t ldtop, const TT* t, int64_t ldt, float temp, float inv_t,
                                                        const float* dloss, int64_t ignore, float* q_top,
                                                        int64_t* target, float* dl) {
     __shared__ Shared sh;
-    __shared__ int first[WAVES];
+    __shared__ int first[WAVES], key[2 * CAP];           // key: a place's class, or ABSENT
+    __shared__ uint32_t leader[2 * CAP], times[2 * CAP];
+    uint32_t bits = 6;
+    while (1u << bits < 2 * n) ++bits;
+    const uint32_t places = 1u << bits;
     for (uint64_t m = blockIdx.x; m < M; m += gridDim.x) {
+        for (uint32_t i = threadIdx.x; i < places; i += WORK) {
+            key[i] = ABSENT;
+            leader[i] = n;
+            times[i] = 0;
+        }
         bool counted, bad;
         const float log_s = teacher(n, V, top + (int64_t)m * ldtop, t + (int64_t)m * ldt, inv_t, sh, counted, bad);
         int at = (int)n;
@@ -301,25 +312,32 @@ __global__ __launch_bounds__(WORK) void prepare_kernel(uint32_t M, uint32_t V, u
         }
         for (int d = 32; d; d >>= 1) at = min(at, __shfl_xor(at, d));
         if ((threadIdx.x & 63) == 0) first[threadIdx.x >> 6] = at;
-        __syncthreads();
-        for (uint32_t j = threadIdx.x; j < n; j += WORK) {
-            const int id = sh.id[j];
-            uint32_t same = 0;
-#pragma unroll 4
-            for (uint32_t i = 0; i < n; i += 4) {
-                const u32x4 c = *(const u32x4*)(sh.id + i);
+        uint32_t place[CAP / WORK];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) same += (int)c[e] == id ? 1u : 0u;
+        for (uint32_t l = 0; l < CAP / WORK; ++l) {
+            const uint32_t j = l * WORK + threadIdx.x;
+            const int id = j < n ? sh.id[j] : ABSENT;
+            place[l] = places;
+            if (id < 0) continue;
+            uint32_t h = (uint32_t)id * 2654435761u >> (32 - bits);
+            for (;; h = (h + 1) & (places - 1)) {        // (at most half of the places are taken)
+                const int there = atomicCAS(&key[h], ABSENT, id);
+                if (there == ABSENT || there == id) break;
             }
+            atomicMin(&leader[h], j);
+            atomicAdd(&times[h], 1u);
+            place[l] = h;
+        }
+        __syncthreads();
+#pragma unroll
+        for (uint32_t l = 0; l < CAP / WORK; ++l) {
+            const uint32_t j = l * WORK + threadIdx.x, h = place[l];
+            if (j >= n) continue;
             float q = sh.q[j];
-            if (same > 1 && id >= 0) {
-                q = 0.0f;
-                bool again = false;
-                for (uint32_t i = 0; i < n; ++i) {
-                    q += sh.id[i] == id ? sh.q[i] : 0.0f;
-                    again |= i < j && sh.id[i] == id;
-                }
-                if (again) q = -1.0f;
+            if (h < places && times[h] > 1) {
+                if (leader[h] != j) q = -1.0f;
+                else
+                    for (uint32_t i = j + 1; i < n; ++i) q += sh.id[i] == sh.id[j] ? sh.q[i] : 0.0f;
             }
             q_top[(int64_t)m * n + j] = q;
         }
@@ -391,11 +409,16 @@ extern "C" int vkb_launch_distill_table(const vkb_distill* d, const vkb_distill_
 }
 
 extern "C" int vkb_launch_distill_prepare(int t_type, const vkb_distill* d, const float* dloss, void* stream) {
+    if (d->n > TOP) return (int)hipErrorInvalidValue;
     const bool ok = with_type(t_type, [&](auto f) {
         using TT = decltype(f);
-        hipLaunchKernelGGL((prepare_kernel<TT>), dim3(row_blocks(d->M)), dim3(WORK), 0, (hipStream_t)stream, d->M, d->V,
-                           d->n, d->top, d->ldtop, (const TT*)d->t, d->ldt, d->temp, 1.0f / d->temp, dloss, d->ignore,
-                           d->q_top, d->target, d->dl);
+        auto launch = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3(row_blocks(d->M)), dim3(WORK), 0, (hipStream_t)stream, d->M, d->V, d->n,
+                               d->top, d->ldtop, (const TT*)d->t, d->ldt, d->temp, 1.0f / d->temp, dloss, d->ignore,
+                               d->q_top, d->target, d->dl);
+        };
+        if (d->n <= WORK) launch(prepare_kernel<TT, WORK>);
+        else launch(prepare_kernel<TT, TOP>);
     });
     return ok ? (int)hipGetLastError() : (int)hipErrorInvalidValue;
 }
