@@ -60,7 +60,9 @@ class Step:
 
 STEPS = [("embedding", 5000, 300, 264, "bf16"), ("distill", 300, 5003, 256, "bf16"), ("policy", 300, 700, 1, "f32"),
          ("distill_grad", 300, 5003, 256, "f16"), ("embedding", 40000, 2000, 65, "f32"),
-         ("distill_grad", 40, 900, 72, "f32"), ("distill", 9, 20000, 64, "f32"), ("policy", 20, 9000, 1, "f32"), ("distill_grad", 1200, 2003, 200, "bf16")]
+         ("distill_grad", 40, 900, 72, "f32"), ("distill", 9, 20000, 64, "f32"), ("policy", 20, 9000, 1, "f32"),
+         ("distill_grad", 1200, 2003, 200, "bf16"), ("distill", 11000, 300, 4096, "bf16"), ("policy", 9000, 300, 1, "f32"),
+         ("policy", 300, 90, 1, "f32")]
 
 
 def alone():

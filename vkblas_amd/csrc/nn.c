@@ -997,7 +997,8 @@ static int distill_args(vkblas_dtype_t type, uint32_t M, uint32_t V, uint32_t K,
 vkblas_status_t vkblas_linear_distill_async(vkblas_dtype_t type, uint32_t M, uint32_t V, uint32_t K, const void* x,
                                             uint32_t ldx, const void* w, uint32_t ldw, uint32_t n_top,
                                             const int64_t* top, uint32_t ldtop, vkblas_dtype_t t_type,
-                                            const void* t, uint32_t ldt, float temperature, float* loss, float* lse, float* z_top, void* stream) {
+                                            const void* t, uint32_t ldt, float temperature, float* loss, float* lse,
+                                            float* z_top, void* stream) {
     if (!distill_args(type, M, V, K, ldx, ldw, n_top, ldtop, t_type, ldt, temperature)) return VKBLAS_ERR_PARAM;
     if (M == 0) return VKBLAS_OK;
     if (!x || !w || !top || !t || !loss || !lse || !z_top) return VKBLAS_ERR_PARAM;
@@ -1138,7 +1139,8 @@ static int policy_args(uint32_t B, uint32_t T, const float* logp, uint32_t ldp, 
 
 vkblas_status_t vkblas_policy_loss_async(vkblas_reduce_t reduce, uint32_t B, uint32_t T, const float* logp,
                                          uint32_t ldp, const float* old_logp, uint32_t ldo,
-                                         const float* ref_logp, uint32_t ldr, const float* adv, uint32_t ldadv, uint32_t adv_step, const uint8_t* mask,
+                                         const float* ref_logp, uint32_t ldr, const float* adv, uint32_t ldadv,
+                                         uint32_t adv_step, const uint8_t* mask,
                                          uint32_t ldmask, float clip_low, float clip_high, float kl_coef, float* stats,
                                          float* norm, void* stream) {
     vkb_policy p;
