@@ -106,6 +106,13 @@ def test_gradient(M, V, N, dt, wt):
     check_gradient(gradient(dy, ids, V, dt, wt, 1.5), dy, ids, V, wt, 1.5)
 
 
+@pytest.mark.parametrize("kind", ["usual", "uniform"])
+def test_gradient_of_more_tokens_than_a_launch_merges_at_once(kind):
+    M, V, N = 4_300_001, 5000, 4
+    dy, ids = R.values(M, N, "bf16", 1), tokens(M, V, 2, kind)
+    check_gradient(gradient(dy, ids, V, "bf16", "f32", 0.5), dy, ids, V, "f32", 0.5)
+
+
 @pytest.mark.parametrize("M,V,N", [(1, 40000, 1000), (3, 33000, 1025), (300, 70001, 520), (1024, 34000, 1000),
                                    (1025, 34000, 1000), (4096, 16400, 2050)])
 @pytest.mark.parametrize("beta", [0.0, 1.0, 0.5])

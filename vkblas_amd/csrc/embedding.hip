@@ -144,79 +144,83 @@ __global__ __launch_bounds__(MTHREADS) void merge_runs_kernel(uint32_t M, const 
     constexpr uint32_t SEARCHES = S == 1 ? 4 : 8;
     __shared__ uint32_t places[MGROUPS - 1][WORK];
     __shared__ __attribute__((aligned(16))) uint32_t keys[LEN * WAYS * S];
-    const uint64_t first = (uint64_t)blockIdx.x * WORK, group = first / GROUP * GROUP;
-    const uint32_t n = (uint32_t)min((uint64_t)GROUP, M - group), runs = (n + RUN - 1) / RUN;
-    // whole runs, the last one filled up with keys above all others; LOADS in flight
-    constexpr uint32_t LOADS = 4;
-    for (uint32_t q0 = 0; q0 < runs * (RUN / 4); q0 += LOADS * MTHREADS) {
-        u32x4 x[LOADS];
+    for (uint64_t first = (uint64_t)blockIdx.x * WORK; first < M; first += (uint64_t)gridDim.x * WORK) {
+        const uint64_t group = first / GROUP * GROUP;
+        const uint32_t n = (uint32_t)min((uint64_t)GROUP, M - group), runs = (n + RUN - 1) / RUN;
+        // whole runs, the last one filled up with keys above all others; LOADS in flight
+        constexpr uint32_t LOADS = 4;
+        for (uint32_t q0 = 0; q0 < runs * (RUN / 4); q0 += LOADS * MTHREADS) {
+            u32x4 x[LOADS];
 #pragma unroll
-        for (uint32_t l = 0; l < LOADS; ++l) {
-            const uint32_t i = 4 * (q0 + l * MTHREADS + threadIdx.x);
-            if (i + 4 <= n) x[l] = *(const u32x4*)(key_in + group + i);
-            else
-#pragma unroll
-                for (uint32_t e = 0; e < 4; ++e) x[l][e] = i + e < n ? key_in[group + i + e] : ~0u;
-        }
-#pragma unroll
-        for (uint32_t l = 0; l < LOADS; ++l) {
-            const uint32_t q = q0 + l * MTHREADS + threadIdx.x;
-            if (q >= runs * (RUN / 4)) continue;
-            if constexpr (S == 1) *(u32x4*)(keys + 4 * q) = x[l];
-            else keys[q] = x[l][3];
-        }
-    }
-    __syncthreads();
-    const uint32_t share = threadIdx.x / WORK, pair = threadIdx.x % WORK;
-    const uint32_t i = min((uint32_t)(first - group) + pair, n - 1);
-    const uint32_t own = i / RUN, k = key_in[group + i], o = order_in[group + i];
-    uint32_t at = 0;
-    for (uint32_t r0 = share * SEARCHES; r0 < runs; r0 += MGROUPS * SEARCHES) {
-        uint32_t pos[SEARCHES];
-#pragma unroll
-        for (uint32_t r = 0; r < SEARCHES; ++r) pos[r] = 0;
-#pragma unroll
-        for (uint32_t step = LEN / 2; step; step /= 2)
-#pragma unroll
-            for (uint32_t r = 0; r < SEARCHES; ++r) {
-                const uint32_t* run = keys + min(r0 + r, runs - 1) * LEN;
-                pos[r] += run[pos[r] + step - 1] < k + (r0 + r < own ? 1u : 0u) ? step : 0u;
-            }
-#pragma unroll
-        for (uint32_t r = 0; r < SEARCHES; ++r) {
-            const uint32_t run = min(r0 + r, runs - 1), bound = k + (run < own ? 1u : 0u);
-            pos[r] += keys[run * LEN + pos[r]] < bound ? 1u : 0u;
-        }
-        if constexpr (S == 4) {
-            u32x4 x[SEARCHES];
-#pragma unroll
-            for (uint32_t r = 0; r < SEARCHES; ++r) {
-                const uint32_t j = 4 * (min(r0 + r, runs - 1) * LEN + min(pos[r], LEN - 1));
-                if (j + 4 <= n) x[r] = *(const u32x4*)(key_in + group + j);
+            for (uint32_t l = 0; l < LOADS; ++l) {
+                const uint32_t i = 4 * (q0 + l * MTHREADS + threadIdx.x);
+                if (i + 4 <= n) x[l] = *(const u32x4*)(key_in + group + i);
                 else
 #pragma unroll
-                    for (uint32_t e = 0; e < 4; ++e) x[r][e] = j + e < n ? key_in[group + j + e] : ~0u;
+                    for (uint32_t e = 0; e < 4; ++e) x[l][e] = i + e < n ? key_in[group + i + e] : ~0u;
             }
 #pragma unroll
-            for (uint32_t r = 0; r < SEARCHES; ++r) {
-                const uint32_t bound = k + (r0 + r < own ? 1u : 0u);
-                uint32_t c = 0;
-#pragma unroll
-                for (uint32_t e = 0; e < 4; ++e) c += x[r][e] < bound ? 1u : 0u;
-                pos[r] = 4 * pos[r] + (pos[r] < LEN ? c : 0u);
+            for (uint32_t l = 0; l < LOADS; ++l) {
+                const uint32_t q = q0 + l * MTHREADS + threadIdx.x;
+                if (q >= runs * (RUN / 4)) continue;
+                if constexpr (S == 1) *(u32x4*)(keys + 4 * q) = x[l];
+                else keys[q] = x[l][3];
             }
         }
+        __syncthreads();
+        const uint32_t share = threadIdx.x / WORK, pair = threadIdx.x % WORK;
+        const uint32_t i = min((uint32_t)(first - group) + pair, n - 1);
+        const uint32_t own = i / RUN, k = key_in[group + i], o = order_in[group + i];
+        uint32_t at = 0;
+        for (uint32_t r0 = share * SEARCHES; r0 < runs; r0 += MGROUPS * SEARCHES) {
+            uint32_t pos[SEARCHES];
 #pragma unroll
-        for (uint32_t r = 0; r < SEARCHES; ++r) at += r0 + r < runs && r0 + r != own ? pos[r] : 0u;
+            for (uint32_t r = 0; r < SEARCHES; ++r) pos[r] = 0;
+#pragma unroll
+            for (uint32_t step = LEN / 2; step; step /= 2)
+#pragma unroll
+                for (uint32_t r = 0; r < SEARCHES; ++r) {
+                    const uint32_t* run = keys + min(r0 + r, runs - 1) * LEN;
+                    pos[r] += run[pos[r] + step - 1] < k + (r0 + r < own ? 1u : 0u) ? step : 0u;
+                }
+#pragma unroll
+            for (uint32_t r = 0; r < SEARCHES; ++r) {
+                const uint32_t run = min(r0 + r, runs - 1), bound = k + (run < own ? 1u : 0u);
+                pos[r] += keys[run * LEN + pos[r]] < bound ? 1u : 0u;
+            }
+            if constexpr (S == 4) {
+                u32x4 x[SEARCHES];
+#pragma unroll
+                for (uint32_t r = 0; r < SEARCHES; ++r) {
+                    const uint32_t j = 4 * (min(r0 + r, runs - 1) * LEN + min(pos[r], LEN - 1));
+                    if (j + 4 <= n) x[r] = *(const u32x4*)(key_in + group + j);
+                    else
+#pragma unroll
+                        for (uint32_t e = 0; e < 4; ++e) x[r][e] = j + e < n ? key_in[group + j + e] : ~0u;
+                }
+#pragma unroll
+                for (uint32_t r = 0; r < SEARCHES; ++r) {
+                    const uint32_t bound = k + (r0 + r < own ? 1u : 0u);
+                    uint32_t c = 0;
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; ++e) c += x[r][e] < bound ? 1u : 0u;
+                    pos[r] = 4 * pos[r] + (pos[r] < LEN ? c : 0u);
+                }
+            }
+#pragma unroll
+            for (uint32_t r = 0; r < SEARCHES; ++r) at += r0 + r < runs && r0 + r != own ? pos[r] : 0u;
+        }
+        if (share) places[share - 1][pair] = at;
+        __syncthreads();
+        if (share == 0 && (uint32_t)(first - group) + pair < n) {
+            at += i % RUN;
+#pragma unroll
+            for (uint32_t s = 0; s < MGROUPS - 1; ++s) at += places[s][pair];
+            key[group + at] = k;
+            order[group + at] = o;
+        }
+        __syncthreads();                 // the next pairs' keys and places
     }
-    if (share) places[share - 1][pair] = at;
-    __syncthreads();
-    if (share || (uint32_t)(first - group) + pair >= n) return;
-    at += i % RUN;
-#pragma unroll
-    for (uint32_t s = 0; s < MGROUPS - 1; ++s) at += places[s][pair];
-    key[group + at] = k;
-    order[group + at] = o;
 }
 
 // Runs of `len`, WAYS at a time, searched in memory
@@ -754,7 +758,7 @@ extern "C" int vkb_launch_embedding_rank(uint32_t M, uint32_t V, const int64_t* 
 
 extern "C" int vkb_launch_embedding_merge_runs(uint32_t M, const uint32_t* key_in, const uint32_t* order_in,
                                                uint32_t* key, uint32_t* order, void* stream) {
-    const uint32_t blocks = (uint32_t)(((uint64_t)M + WORK - 1) / WORK);
+    const uint32_t all = (uint32_t)(((uint64_t)M + WORK - 1) / WORK), blocks = all < 16384 ? all : 16384;
     if (M <= RUN * WAYS)
         hipLaunchKernelGGL((merge_runs_kernel<1>), dim3(blocks), dim3(MTHREADS), 0, (hipStream_t)stream, M, key_in,
                            order_in, key, order);
