@@ -137,7 +137,9 @@ typedef enum {
  *   0 for a sequence without any; kept for the backward pass
  *   stats: 4 floats, sums over the tokens that count, by weight: of L (the
  *   loss), of exp(d) - d - 1, of the tokens whose bound was taken (c A < r A), of r
- * Which side of a bound r lies on is decided in fp64, and so are the sums.
+ * Which side of a bound r lies on is decided in fp64, and so are the sums.  r and
+ * exp(d) are fp32, infinite past its range; an advantage of 0 takes no part in L
+ * whatever r is, unless logp - old_logp is not finite.
  * Needs a workspace for more than VKBLAS_POLICY_SMALL tokens (B * T, a sequence's
  * rounded up to 256).
  */

@@ -262,3 +262,55 @@ def test_empty_batch():
     args = 0, 5, None, 5, None, 5, None, 0, None, 5, 1, None, 0, 0.2, 0.2, 0.0
     assert vk.policy_loss_async(0, *args, None, None) == vk.OK
     assert vk.policy_loss_backward_async(*args, None, None, None, 5) == vk.OK
+
+
+# ---- ratios past fp32
+
+def overflowing(B, T, per_token):
+    """Tokens (or whole sequences) without an advantage whose ratio is past fp32's range, and the same with a ratio of
+    1: they add the same to everything but the mean ratio."""
+    i = inputs(B, T, per_token=per_token)
+    i["mask"][-1] = 1
+    none = torch.zeros(B, T, dtype=torch.bool)
+    none[:, ::3] = True
+    if not per_token:
+        none[:] = False
+        none[::2] = True
+        none[-1] = True
+    i["adv"][none if per_token else none[:, :1]] = 0.0
+    i["adv"][0, 0] = -0.0 if none[0, 0] else i["adv"][0, 0]
+    i["ref"][none], i["logp"][none] = 0.125, 0.0
+    i["old"][none] = 0.0
+    plain = dict(i, old=i["old"].clone())
+    i["old"][none] = -200.0
+    return i, plain
+
+
+# the small call, units, a sequence a wave, a sequence a workgroup
+OVERFLOW = [(1, 7), (20, 9000), (3000, 70), (300, 700)]
+
+
+@pytest.mark.parametrize("B,T", OVERFLOW)
+@pytest.mark.parametrize("reduce", REDUCE)
+@pytest.mark.parametrize("per_token", [True, False])
+def test_no_advantage_times_a_ratio_past_fp32_is_nothing(B, T, reduce, per_token):
+    i, plain = overflowing(B, T, per_token)
+    want, got = Call(plain).loss(reduce), Call(i).loss(reduce)
+    check_loss(want, plain, reduce)
+    assert torch.equal(got[0][:3], want[0][:3]) and math.isinf(got[0][3]) and torch.equal(got[1], want[1])
+    grad = Call(plain).grad(want[1], 0.5)
+    check_grad(grad, plain, want[1], 0.5)
+    assert torch.equal(Call(i).grad(want[1], 0.5), grad)
+
+
+@pytest.mark.parametrize("key,v", [("logp", math.nan), ("old", math.nan), ("adv", math.nan), ("old", -math.inf)])
+def test_no_advantage_hides_no_nan(key, v):
+    """A NaN reaches the loss through an advantage of 0 too, and so does 0 times an infinite difference."""
+    i = inputs(2, 30, masked=False)
+    i["adv"][1, 4] = 0.0
+    i[key][1, 4] = v
+    c = Call(i)
+    stats, norm = c.loss("tokens", kl=0.0)
+    assert math.isnan(stats[0])
+    g = c.grad(norm, 1.0, kl=0.0)
+    assert bool(torch.isnan(g[1, 4])) and int(torch.isnan(g).sum()) == 1

@@ -54,14 +54,18 @@ __device__ __forceinline__ float kl_slope(float d) {
 
 struct Token {
     float r, d;              // ratio, ref - logp
+    float by;                // what A is multiplied by where r A is taken
     int side;                // 0: r A is taken, -1: the lower bound's, 1: the upper one's
 };
-// A NaN anywhere takes r A, which it reaches.
+// A NaN anywhere takes r A, which it reaches.  r of finite numbers may be past fp32's
+// range, and an advantage of 0 times it is 0 all the same: logp - old, which is finite
+// where they are, stands in for it.
 __device__ __forceinline__ Token token(const vkb_policy& p, float logp, float old, float ref, float adv) {
     const double diff = (double)logp - (double)old;
     Token t;
     t.r = fast_exp(logp - old);
     t.d = ref - logp;
+    t.by = adv == 0.0f ? logp - old : t.r;
     t.side = adv > 0.0f && diff > p.high ? 1 : adv < 0.0f && diff < p.low ? -1 : 0;
     return t;
 }
@@ -169,7 +173,7 @@ __device__ __forceinline__ Sums lane_sums(const vkb_policy& p, int64_t b, int64_
             const float adv = is ? f.adv[e] : 0.0f;
             const Token k = token(p, is ? f.logp[e] : 0.0f, is ? f.old[e] : 0.0f, is ? f.ref[e] : 0.0f, adv);
             const float kl = p.ref ? kl_term(k.d) : 0.0f;
-            const float taken = k.side ? (k.side > 0 ? p.r_high : p.r_low) : k.r;
+            const float taken = k.side ? (k.side > 0 ? p.r_high : p.r_low) : k.by;
             loss += (by_kl ? p.kl * kl : 0.0f) - taken * adv;
             kls += kl;
             sides += k.side ? 1u : 0u;
@@ -399,7 +403,7 @@ __global__ __launch_bounds__(WORK) void grad_kernel(vkb_policy p, const float* n
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const Token x = token(p, f.logp[e], f.old[e], f.ref[e], f.adv[e]);
-                float s = x.side ? 0.0f : -f.adv[e] * x.r;
+                float s = x.side ? 0.0f : -f.adv[e] * x.by;
                 if (by_kl) s += p.kl * kl_slope(x.d);
                 g[e] = in >> e & 1 ? by * s : 0.0f;
             }
