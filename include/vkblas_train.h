@@ -159,6 +159,7 @@ vkblas_status_t vkblas_policy_loss_async(
  * Its gradient, dlogp[b][t] = dloss[0] * norm[b] * dL/dlogp (dloss one float in
  * device memory, of stats[0]); 0 where the token does not count:
  *   dL/dlogp = -A r [r A <= c A] + kl_coef * (1 - exp(d))
+ * A dloss of 0 gives zeros where the inputs are finite, whatever r and exp(d) are.
  * dlogp (B x T) may be logp, with its leading dimension.  Needs no workspace.
  */
 vkblas_status_t vkblas_policy_loss_backward_async(

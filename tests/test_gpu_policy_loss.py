@@ -314,3 +314,20 @@ def test_no_advantage_hides_no_nan(key, v):
     assert math.isnan(stats[0])
     g = c.grad(norm, 1.0, kl=0.0)
     assert bool(torch.isnan(g[1, 4])) and int(torch.isnan(g).sum()) == 1
+
+
+@pytest.mark.parametrize("shape", [(1, 7), (20, 9000)])
+def test_a_loss_gradient_of_0_leaves_none(shape):
+    """Whatever a token's ratio and KL term grow to; a NaN or an infinity among the inputs stays a NaN."""
+    i = inputs(*shape, masked=False)
+    i["logp"][:] = 0.0
+    i["old"][0, ::2], i["ref"][0, 1::2] = -200.0, 200.0
+    i["adv"][:] = -1.0
+    norm = torch.ones(shape[0], dtype=torch.float64)
+    assert bool(torch.isinf(Call(i).grad(norm, 1.0)[0]).all())
+    assert bool((Call(i).grad(norm, 0.0) == 0).all())
+    for key, v in (("logp", math.nan), ("old", -math.inf), ("ref", math.inf), ("adv", -math.inf)):
+        j = {**i, key: i[key].clone()}
+        j[key][0, 3] = v
+        g = Call(j).grad(norm, 0.0)
+        assert bool(torch.isnan(g[0, 3])) and int(torch.isnan(g).sum()) == 1 and bool((g.nan_to_num(0) == 0).all())

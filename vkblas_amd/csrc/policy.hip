@@ -405,6 +405,9 @@ __global__ __launch_bounds__(WORK) void grad_kernel(vkb_policy p, const float* n
                 const Token x = token(p, f.logp[e], f.old[e], f.ref[e], f.adv[e]);
                 float s = x.side ? 0.0f : -f.adv[e] * x.by;
                 if (by_kl) s += p.kl * kl_slope(x.d);
+                // 0 times a slope past fp32's range is 0: its arguments, finite where the inputs are, stand in
+                if (by == 0.0f && !__builtin_isfinite(s))
+                    s = (x.side ? 0.0f : f.adv[e] + (f.logp[e] - f.old[e])) + (by_kl ? x.d : 0.0f);
                 g[e] = in >> e & 1 ? by * s : 0.0f;
             }
         }
