@@ -67,7 +67,9 @@ vkblas_status_t vkblas_embedding_backward_async(
  * all V classes:
  *   lse[m] = log sum_v exp(z[m][v] / T)
  *   loss[m] = T^2 * sum_j q_j (log q_j - log p[top[m][j]])
- *   x: M x K; w: V x K, of one type; T > 0
+ *   x: M x K; w: V x K, of one type
+ *   T > 0, T^2 and log2(e) / T within fp32's range; the loss's error is T^2 times
+ *   that of log-sum-exps in fp32
  *   top: M x n_top classes (leading dimension ldtop); t: the teacher's logits
  *   there, M x n_top of t_type, F32 or type; n_top up to VKBLAS_DISTILL_TOP
  *   top[m][j] < 0: the entry is absent, whatever t holds there; a t of -inf

@@ -283,3 +283,21 @@ def test_empty_batch():
         vk.linear_distill_backward_async(*args, None, None, None, None, 30, dw.ptr, dw.ld, 0, beta, stream=stream())
         assert bool((dw.get() == want).all())
     dw.check_around()
+
+
+@pytest.mark.parametrize("M,V,K", [(5, 300, 64), (300, 2000, 128)])
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("temp", [4.3e-39, 1.84e19])
+def test_temperatures_at_the_ends_of_fp32(M, V, K, dt, temp):
+    """Equal logits: log V whatever divides them, and a loss that is T^2 log(V / n) with n of the entries at the
+    teacher's highest logit, or all: 0 or infinite in fp32.  No NaN in the gradients."""
+    x, w = torch.zeros(M, K, dtype=torch.float64), R.values(V, K, dt, 2)
+    top, t = torch.arange(6).repeat(M, 1), torch.zeros(M, 6, dtype=torch.float64)
+    t[1::2, 2] = -1.0
+    loss, lse, zt = forward(x, w, top, t, temp, dt)
+    want = torch.full((M,), float(torch.tensor(float(V), dtype=torch.float64).log()), dtype=torch.float64)
+    R.close(lse, want, 600 * R.E + R.STEP * (want + 1), "lse")
+    assert torch.equal(loss.float(), D.distill(x, w, top, t, temp)[0][0].float()) and bool((zt == 0).all())
+    assert float(loss[0]) == (0.0 if temp < 1 else float("inf"))
+    dx, dw = backward(x, w, top, t, want, torch.ones(M, dtype=torch.float64), temp, dt, wt="f32")
+    assert bool(torch.isfinite(dx).all()) and bool((dw == 0).all())

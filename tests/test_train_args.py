@@ -88,3 +88,16 @@ def test_header_symbols_are_exported():
     assert names == {f"vkblas_{n}_async" for n in CALLS}
     assert all(hasattr(vk.load(), n) for n in names)
     assert int(re.search(r"#define VKBLAS_DISTILL_TOP (\d+)", text).group(1)) == vk.DISTILL_TOP
+
+
+@pytest.mark.parametrize("op", ["linear_distill", "linear_distill_backward"])
+def test_temperatures_that_leave_fp32(op):
+    """log2(e) / T and T^2 have to be numbers: refused past that, taken up to it."""
+    fn, good = CALLS[op]
+    for t in (1e-45, 2.95e-39, 4.2e-39, 1.85e19, 1e30, 3e38):
+        assert fn(**{**good, "temperature": t}, check=False) == vk.ERR_PARAM, t
+        assert fn(**{**good, "temperature": t, "M": 0, "dw": None} if "dw" in good else
+                  {**good, "temperature": t, "M": 0}, check=False) == vk.ERR_PARAM, t
+    for t in (4.3e-39, 1e-20, 1e10, 1.84e19):
+        assert fn(**{**good, "temperature": t, "M": 0, "dw": None} if "dw" in good else
+                  {**good, "temperature": t, "M": 0}) == vk.OK, t

@@ -985,13 +985,15 @@ vkblas_status_t vkblas_linear_xent_backward_async(vkblas_dtype_t type, uint32_t 
 
 /* A target that no class has */
 #define NO_TARGET INT64_MIN
+#define LOG2E 1.4426950408889634f
 
 static int distill_args(vkblas_dtype_t type, uint32_t M, uint32_t V, uint32_t K, uint32_t ldx, uint32_t ldw,
                         uint32_t n_top, uint32_t ldtop, vkblas_dtype_t t_type, uint32_t ldt, float temperature) {
     if (!known_type(type) || (t_type != type && t_type != VKBLAS_DT_F32)) return 0;
     if (V == 0 || K == 0 || M > DIM_MAX || V > DIM_MAX || K > DIM_MAX || ldx < K || ldw < K) return 0;
     if (n_top == 0 || n_top > VKBLAS_DISTILL_TOP || ldtop < n_top || ldt < n_top) return 0;
-    return temperature > 0.0f && temperature <= FLT_MAX && 1.0f / temperature <= FLT_MAX;
+    /* what the kernels multiply by: T^2 the loss, log2(e) / T the logits */
+    return temperature > 0.0f && temperature * temperature <= FLT_MAX && 1.0f / temperature * LOG2E <= FLT_MAX;
 }
 
 vkblas_status_t vkblas_linear_distill_async(vkblas_dtype_t type, uint32_t M, uint32_t V, uint32_t K, const void* x,
