@@ -331,3 +331,15 @@ def test_a_loss_gradient_of_0_leaves_none(shape):
         j[key][0, 3] = v
         g = Call(j).grad(norm, 0.0)
         assert bool(torch.isnan(g[0, 3])) and int(torch.isnan(g).sum()) == 1 and bool((g.nan_to_num(0) == 0).all())
+
+
+@pytest.mark.parametrize("B,T", [(20, 9000), (300, 9000), (1024, 8192), (1100, 8192), (2047, 3001)])
+@pytest.mark.parametrize("reduce", REDUCE)
+def test_units_of_many_sequences(B, T, reduce):
+    """Several units each of a few to more sequences than the finish keeps the tokens of, some without any."""
+    i = inputs(B, T, per_token=reduce != "sum")
+    assert bool((i["mask"] == 0).all(1).any())
+    c = Call(i)
+    got = c.loss(reduce)
+    check_loss(got, i, reduce)
+    check_grad(c.grad(got[1], 0.75), i, got[1], 0.75)
