@@ -343,3 +343,38 @@ def test_units_of_many_sequences(B, T, reduce):
     got = c.loss(reduce)
     check_loss(got, i, reduce)
     check_grad(c.grad(got[1], 0.75), i, got[1], 0.75)
+
+
+def misjudged(bound, upper, n=64):
+    """fp32 pairs whose exact difference lies on one side of the bound and whose fp32 difference on the other, and
+    which of them are past it."""
+    g = torch.Generator().manual_seed(3)
+    # multiples of 2^-30, finer than the difference's own step
+    small = -torch.randint(2 ** 21, 2 ** 24, (20000,), generator=g).float() * 2.0 ** -30
+    near = (small.double() - abs(bound)).float()
+    other = torch.cat((near, torch.nextafter(near, near + 1), torch.nextafter(near, near - 1)))
+    small = small.repeat(3)
+    logp, old = (small, other) if upper else (other, small)
+    exact_diff = logp.double() - old.double()
+    past = exact_diff > bound if upper else exact_diff < bound
+    wrong = past != ((logp - old).double() > bound if upper else (logp - old).double() < bound)
+    # (far from the bound against what float64's own exp and log are off by)
+    pick = torch.nonzero(wrong & ((exact_diff - bound).abs() > 1e-11))[:n, 0]
+    return logp[pick], old[pick], past[pick]
+
+
+# bounds whose logarithm lies below and above the middle of a step of fp32: the fp32 difference falls short of it, or
+# goes past it
+@pytest.mark.parametrize("clip,upper,past", [(0.3, True, True), (0.2, True, False), (0.1, False, True),
+                                             (0.3, False, False)])
+def test_sides_that_an_fp32_difference_takes_wrongly(clip, upper, past):
+    clip = D.f32(clip)
+    logp, old, held = misjudged(math.log1p(clip if upper else -clip), upper)
+    assert len(logp) >= 20 and bool((held == past).all())
+    i = dict(logp=logp[None], old=old[None], ref=None, adv=torch.full((1, len(logp)), 1.0 if upper else -1.0),
+             mask=torch.ones(1, len(logp), dtype=torch.uint8), masked=True)
+    assert torch.equal(D.policy_terms(*exact(i)[:4], clip, clip, KL)[2][0], held)
+    c = Call(i)
+    stats, norm = c.loss("sum", clip, clip)
+    assert float(stats[2]) == float(held.sum())
+    assert torch.equal(c.grad(norm, 1.0, clip, clip)[0] == 0, held)
