@@ -301,3 +301,16 @@ def test_temperatures_at_the_ends_of_fp32(M, V, K, dt, temp):
     assert float(loss[0]) == (0.0 if temp < 1 else float("inf"))
     dx, dw = backward(x, w, top, t, want, torch.ones(M, dtype=torch.float64), temp, dt, wt="f32")
     assert bool(torch.isfinite(dx).all()) and bool((dw == 0).all())
+
+
+@pytest.mark.parametrize("n", [3, 256, 257, 1024])
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_rows_of_one_class_and_of_two(n, dt):
+    """Every entry of a row the same class, and two classes in turn: one of their entries has all of the probability."""
+    M, V, K = 40, 700, 64
+    x, w, top, t, lse, dloss = grad_inputs(M, V, K, n, dt, 1.5)
+    t = t.nan_to_num(0.25, 0.25, 0.25)
+    top[::2], top[1::2] = 5, 699
+    top[1::2, ::2] = 0
+    check_forward(forward(x, w, top, t, 1.5, dt), x, w, top, t, 1.5)
+    check_backward(backward(x, w, top, t, lse, dloss, 1.5, dt), x, w, top, t, lse, dloss, 1.5, dt)

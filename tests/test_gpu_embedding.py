@@ -220,3 +220,18 @@ def test_offsets_past_32_bits():
                        stream=stream())
     torch.cuda.synchronize()
     assert torch.equal(y, w[ids])
+
+
+@pytest.mark.parametrize("dt,V", [("f32", 2 ** 24), ("bf16", 2 ** 25), ("bf16", 2 ** 25 - 4097)])
+@pytest.mark.parametrize("beta", [0.0, 1.0, 0.5])
+def test_the_one_launch_of_the_most_rows(dt, V, beta):
+    """One column of a gradient of 64 MiB: as many rows as a workgroup lists.  On the GPU."""
+    M = 4096
+    g = torch.Generator().manual_seed(4)
+    ids = torch.randint(0, V, (M,), generator=g)
+    ids[:40], ids[40], ids[41], ids[42] = V - 1, 0, PAD, V
+    dy = R.values(M, 1, dt, 1).cuda()
+    dw0 = torch.linspace(-1, 1, V, dtype=torch.float32, device="cuda").to(R.TORCH[dt]).double()[:, None]
+    got = gradient(dy, ids, V, dt, dt, 0.5, beta, dw0)
+    dw, err = D.embedding_grad(dy, ids.cuda(), V, 0.5, PAD, beta, dw0)
+    R.close(got.cuda(), dw, R.rounded(dw, dt, err), "dw")
