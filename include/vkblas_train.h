@@ -45,7 +45,7 @@ vkblas_status_t vkblas_embedding_async(
  * F32.  beta = 1 reads and writes the rows of the tokens that occur alone: the
  * gradient of a w that is the output projection's too (tied weights) adds to
  * what vkblas_linear_xent_backward_async left there.
- * The rows of a token are summed in fp32 in an order that depends on ids, M, N
+ * The rows of a token are summed in fp32 in an order that depends on ids, M, V, N
  * and the types alone: equal calls give equal bits.  Needs a workspace for more
  * than VKBLAS_EMBEDDING_SMALL tokens or a gradient of more than
  * VKBLAS_EMBEDDING_SMALL_BYTES (V * N of dw_type), or N above 2^24 - 256.
@@ -97,7 +97,7 @@ vkblas_status_t vkblas_linear_distill_async(
  *   D[m][v] = T * dloss[m] * (p[v] - sum of q_j over the j with top[m][j] == v)
  *   dx = D w,  dw = beta * dw + D^T x
  * D is scaled and rounded as vkblas_linear_xent_backward_async's.  dloss of a row
- * that is not counted may hold anything.
+ * that is not counted may hold anything (its x adds 0 times itself to dw).
  *   dx: M x K or NULL; dw: V x K of dw_type or NULL
  * Needs a workspace.
  */
@@ -139,9 +139,10 @@ typedef enum {
  *   0 for a sequence without any; kept for the backward pass
  *   stats: 4 floats, sums over the tokens that count, by weight: of L (the
  *   loss), of exp(d) - d - 1, of the tokens whose bound was taken (c A < r A), of r
- * Which side of a bound r lies on is decided in fp64, and so are the sums.  r and
- * exp(d) are fp32, infinite past its range; an advantage of 0 takes no part in L
- * whatever r is, unless logp - old_logp is not finite.
+ * Which side of a bound r lies on is decided in fp64.  A token's terms are fp32,
+ * and so are the sums of four tokens that a lane takes at once; those are added
+ * up in fp64.  r and exp(d) past fp32's range are infinite; an advantage of 0
+ * takes no part in L whatever r is, unless logp - old_logp is not finite.
  * Needs a workspace for more than VKBLAS_POLICY_SMALL tokens (B * T, a sequence's
  * rounded up to 256).
  */

@@ -675,7 +675,8 @@ static int distill_rows(op_call* c, vkblas_dtype_t type, uint32_t K, teacher_row
  * products / by tiles, bf16: 4096 x 32000 x 4096, 8 entries 792 / 785, 64 886 / 797,
  * 256 1335 / 810, 1024 3836 / 911; 4096 x 128000 x 4096, 16 entries 3048 / 3102, 64 3135 /
  * 3102, 256 3625 / 3135; 4096 x 32000 x 1024, 64 264 / 271, 256 360 / 285; 2048 x 8000 x
- * 1024, 64 55 / 58, 256 104 / 88; 300 x 32003 x 1024, 20 39 / 47, 256 61 / 79). */
+ * 1024, 64 55 / 58, 256 104 / 88; 300 x 32003 x 1024, 20 39 / 47, 256 61 / 79).  The rule's
+ * border lies where both sides are within 3 %, on either side of it. */
 static int by_tiles(vkblas_dtype_t type, uint32_t M, uint32_t V, uint32_t K, uint32_t n, uint32_t S) {
     return type != VKBLAS_DT_F32 && S <= VKB_DISTILL_SLICES && (uint64_t)n * K >= 2ull * V &&
            (double)M * n * K >= 1 << 29;

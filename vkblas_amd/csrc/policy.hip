@@ -1,13 +1,13 @@
 // policy.hip — clipped policy loss with a KL term on token log probabilities.
 //
 // A token's loss is a few operations on four or five floats, so the loss over a
-// batch is a pass over its arrays and a sum, bound by the reads: 13 to 17 bytes
-// a token.  A workgroup takes a unit, a sequence or a part of one (a wave where
+// batch is a pass over its arrays and a sum, bound by the reads: 8 bytes a token,
+// 1 with a mask, 4 each with a reference and with its own advantage.  A workgroup takes a unit, a sequence or a part of one (a wave where
 // there are many short sequences), four tokens a lane at a time, and skips the
 // arrays where no token of a lane's four counts: the padding behind a sequence
-// costs its mask alone.  A token's terms are fp32; sums are fp64, and so is logp -
-// old, on which the side of a bound depends: r > 1 + clip_high exactly where
-// logp - old > log(1 + clip_high).
+// costs its mask alone.  A token's terms and the sum of a lane's four are fp32, the
+// sums of those fp64, and so is logp - old, on which the side of a bound depends: r >
+// 1 + clip_high exactly where logp - old > log(1 + clip_high).
 //
 // 1024 sequences of 8192 tokens, half of them padding: 20.8 us (3.6 TB/s of the
 // bytes that it reads) and 5.8 for the finish, one workgroup over 2048 units; the
@@ -19,7 +19,7 @@ namespace vkb {
 namespace {
 
 // exp(d) - d - 1 without the cancellation of a small d: d^2 sum d^k / (k + 2)!
-// within |d| <= 1 (the 11th term is below 2^-28 of the first)
+// within |d| <= 1 (the terms left out are below 2^-30 of the sum)
 __device__ __forceinline__ float kl_term(float d) {
     if (fabsf(d) > 1.0f) return fast_exp(d) - d - 1.0f;
     float s = 1.0f / 479001600.0f;
@@ -35,7 +35,7 @@ __device__ __forceinline__ float kl_term(float d) {
     s = __builtin_fmaf(s, d, 0.5f);
     return s * d * d;
 }
-// 1 - exp(d), likewise
+// 1 - exp(d), likewise (below 2^-28)
 __device__ __forceinline__ float kl_slope(float d) {
     if (fabsf(d) > 1.0f) return 1.0f - fast_exp(d);
     float s = 1.0f / 39916800.0f;
@@ -315,7 +315,7 @@ __global__ __launch_bounds__(FIN) void finish_kernel(vkb_policy p, int reduce, c
 // sequences, and the finish reads as many totals as there are workgroups
 // (part: NSUM + 1 arrays of those, then each sequence's tokens).  Against each
 // sequence's five sums to memory and one workgroup over them (us): 65536 x 128
-// 115 -> 52, 16384 x 1024 71 -> 49, 8192 x 256 22 -> 16.  What is left at many short
+// 115 -> 53, 16384 x 1024 71 -> 49, 8192 x 256 22 -> 16.  What is left at many short
 // sequences is arithmetic, a wave's whatever its lanes hold.
 template <bool WAVE>
 __global__ __launch_bounds__(WORK) void whole_kernel(vkb_policy p, int reduce, double* part) {
